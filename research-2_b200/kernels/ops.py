@@ -147,7 +147,7 @@ def build_all(head_dims=()) -> None:
     """Compile every kernel library that does not depend on a model, and the attention kernels
     for the given head sizes (a model compiles its own head size at first use otherwise)."""
     for source in ("rowwise", "recurrent", "state_scan", "decay_chunks", "streams", "routing", "gemm_simt", "gemm_tc", "few_rows", "step_io", "attention_simt", "attention_prefill_tc", "latent_attention",
-                   "sampling", "wait_selftest"):
+                   "sampling", "adjust_logits", "top_logits", "distill", "wait_selftest"):
         _lib(source)
     kernel_library("sfu_probe")  # (profiling/sfu_probe.py: a measurement, no part of a step)
     for head_dim in head_dims:
@@ -1905,3 +1905,169 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
                                        _p(key0), _p(key1), _p(sample_pos), _p(out), _stream())
     _check(status, "sample")
     return out
+
+
+# ---- rows of logits: what stands before the draw, what is written down of them, what a student learns from ----
+
+TOP_MOST = 256   # the most logits of a row that top_logits returns and distill_loss takes
+
+
+def _logit_rows(logits: torch.Tensor, what: str) -> tuple[int, int, int, int]:
+    """(type's code, rows, vocabulary, row stride) of a tensor of logits."""
+    _need(logits, "logits", dim=2)
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise KernelError(f"{what}: logits must be float32 or bfloat16, got {logits.dtype}")
+    if logits.shape[1] < 1:
+        raise KernelError(f"{what}: logits of no tokens")
+    return dtype_code(logits.dtype), logits.shape[0], logits.shape[1], _rows(logits, "logits")
+
+
+def _per_row(t: torch.Tensor | None, name: str, dtype, rows: int, logits: torch.Tensor) -> None:
+    if t is None:
+        return
+    _need(t, name, dtype, 1)
+    if t.device != logits.device:
+        raise KernelError(f"{name} must be on the logits' device")
+    if t.shape[0] < rows or not t.is_contiguous():
+        raise KernelError(f"{name} must be contiguous with a number for each of {rows} rows, got shape {tuple(t.shape)} stride {t.stride()}")
+
+
+def _like_logits(logits: torch.Tensor, out: torch.Tensor | None, what: str) -> torch.Tensor:
+    """The output beside rows of logits: `out`, checked, or new rows that are as far apart as the logits' (so that a row starts at the
+    same alignment in both and is written in 16-byte pieces) where that wastes little."""
+    rows, vocab = logits.shape
+    if out is None:
+        ld = _rows(logits, "logits")
+        ld = ld if vocab <= ld <= vocab + max(64, vocab // 16) else vocab
+        return torch.empty_strided((rows, vocab), (ld, 1), dtype=logits.dtype, device=logits.device)
+    _need(out, "out", logits.dtype, 2)
+    if out.shape != logits.shape or out.device != logits.device:
+        raise KernelError(f"{what}: out must have the logits' shape and device, got {tuple(out.shape)} on {out.device}")
+    ld = _rows(out, "out")
+    if rows > 1 and ld < vocab:
+        raise KernelError(f"{what}: rows of out overlap")
+    same = out.data_ptr() == logits.data_ptr() and (rows <= 1 or ld == _rows(logits, "logits"))
+    if not same and rows:
+        def span(t):
+            return t.data_ptr(), t.data_ptr() + ((rows - 1) * _rows(t, "rows") + vocab) * t.element_size()
+        (a, b), (c, d) = span(out), span(logits)
+        if a < d and c < b:
+            raise KernelError(f"{what}: out overlaps the logits without being the same rows")
+    return out
+
+
+def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, slots: torch.Tensor | None = None,
+                  lengths: torch.Tensor | None = None, prompt_lengths: torch.Tensor | None = None, repetition: torch.Tensor | None = None,
+                  presence: torch.Tensor | None = None, frequency: torch.Tensor | None = None, bias_start: torch.Tensor | None = None,
+                  bias_ids: torch.Tensor | None = None, bias_values: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                  mask_rows: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Penalties, biases and masks on rows of logits [R, V] (float32 or bfloat16) -> rows of the same type: new ones, or `out` (which may be
+    the logits themselves).
+
+    `history` int32 [S, L] holds tokens: row r's are history[slots[r], :lengths[r]] (`slots` None: history[r]), the first prompt_lengths[r]
+    of them its prompt's (`prompt_lengths` None: none); tokens outside the vocabulary count for nothing. For a token of the prompt or the
+    answer x becomes x / repetition[r] where it is positive and x * repetition[r] elsewhere; one that stands c > 0 times in the answer then
+    loses frequency[r] * c + presence[r] (a parameter left out changes nothing).
+    `bias_start` int32 [R + 1]: entries bias_start[r] to bias_start[r + 1] of `bias_ids` (int32) and `bias_values` (float32) are row r's
+    and are added to their tokens, in order where a token is named more than once; tokens outside the vocabulary are left out.
+    `mask` int32 [M, >= V / 32]: where bit t % 32 of word t / 32 of row mask_rows[r] is 0 the logit becomes -inf (`mask_rows` None: row r;
+    a number outside [0, M): no mask). A mask that leaves nothing leaves a row of -inf, which `sample` answers with token 0."""
+    code, rows, vocab, ld = _logit_rows(logits, "adjust_logits")
+    history_rows = cap = history_ld = n_masks = mask_ld = n_biases = 0
+    if history is not None:
+        _need(history, "history", torch.int32, 2)
+        history_ld, (history_rows, cap) = _rows(history, "history"), history.shape
+        if lengths is None:
+            raise KernelError("adjust_logits: a history needs lengths")
+        if slots is None and history_rows < rows:
+            raise KernelError(f"adjust_logits: {rows} rows, a history of {history_rows} and no slots")
+    elif any(t is not None for t in (repetition, presence, frequency)):
+        raise KernelError("adjust_logits: penalties need a history")
+    for name, t, dtype in (("slots", slots, torch.int32), ("lengths", lengths, torch.int32), ("prompt_lengths", prompt_lengths, torch.int32),
+                           ("repetition", repetition, torch.float32), ("presence", presence, torch.float32),
+                           ("frequency", frequency, torch.float32), ("mask_rows", mask_rows, torch.int32)):
+        _per_row(t, name, dtype, rows, logits)
+    if bias_start is not None:
+        _per_row(bias_start, "bias_start", torch.int32, rows + 1, logits)
+        if bias_ids is None or bias_values is None:
+            raise KernelError("adjust_logits: biases need bias_ids and bias_values")
+        n_biases = bias_ids.shape[0] if bias_ids.dim() == 1 else -1
+        _per_row(bias_ids, "bias_ids", torch.int32, n_biases, logits)
+        _per_row(bias_values, "bias_values", torch.float32, n_biases, logits)
+    if mask is not None:
+        _need(mask, "mask", torch.int32, 2)
+        n_masks, mask_ld = mask.shape[0], _rows(mask, "mask")
+        if mask.shape[1] * 32 < vocab:
+            raise KernelError(f"adjust_logits: masks of {mask.shape[1]} words are shorter than {vocab} tokens")
+        if mask_rows is None and n_masks < rows:
+            raise KernelError(f"adjust_logits: {rows} rows, {n_masks} masks and no mask_rows")
+    for name, t in (("history", history), ("mask", mask)):
+        if t is not None and t.device != logits.device:
+            raise KernelError(f"{name} must be on the logits' device")
+    out = _like_logits(logits, out, "adjust_logits")
+    if rows == 0:
+        return out
+    status = _lib("adjust_logits").r2_adjust_logits(
+        code, _p(logits), C.c_longlong(ld), _p(out), C.c_longlong(_rows(out, "out")), rows, vocab, _p(history if history_rows else None),
+        C.c_longlong(history_ld), history_rows, cap, _p(slots), _p(lengths), _p(prompt_lengths), _p(repetition), _p(presence), _p(frequency),
+        _p(bias_start if n_biases else None), _p(bias_ids), _p(bias_values), n_biases, _p(mask if n_masks else None), C.c_longlong(mask_ld),
+        n_masks, _p(mask_rows), _stream())
+    _check(status, "adjust_logits")
+    return out
+
+
+def _temperature(temperature: float, what: str) -> float:
+    if not 1e-6 <= float(temperature) < float("inf"):
+        raise KernelError(f"{what}: the temperature must be finite and at least 1e-6, got {temperature}")
+    return float(temperature)
+
+
+def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0):
+    """The k largest logits of every row of [R, V] (float32 or bfloat16; k up to 256 and V): (values float32 [R, k] from the largest down,
+    their tokens int32 [R, k], log_sum float32 [R]), equal values from the lowest token up and NaN below all others; log_sum is the
+    logarithm of the row's sum of exp(x / temperature), so values / temperature - log_sum are log-probabilities."""
+    code, rows, vocab, ld = _logit_rows(logits, "top_logits")
+    if not 1 <= k <= min(vocab, TOP_MOST):
+        raise KernelError(f"top_logits: k must be in [1, {min(vocab, TOP_MOST)}], got {k}")
+    temperature = _temperature(temperature, "top_logits")
+    values = torch.empty(rows, k, dtype=torch.float32, device=logits.device)
+    ids = torch.empty(rows, k, dtype=torch.int32, device=logits.device)
+    log_sum = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    if rows:
+        _check(_lib("top_logits").r2_top_logits(code, _p(logits), C.c_longlong(ld), rows, vocab, k, C.c_float(temperature), _p(values), _p(ids),
+                                                _p(log_sum), _stream()), "top_logits")
+    return values, ids, log_sum
+
+
+def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, *, log_sum: torch.Tensor | None = None,
+                 temperature: float = 1.0, weight: torch.Tensor | None = None, gradient: bool = True, out: torch.Tensor | None = None):
+    """A student's loss against a teacher's top logits, row by row: (loss float32 [R], gradient [R, V] with respect to the logits in their
+    type, or None without `gradient`); `out` takes the gradient (it may be the logits themselves).
+
+    `logits` [R, V] are the student's (float32 or bfloat16), `ids` int32 [R, K] and `teacher` float32 [R, K] the teacher's top logits (K up to
+    256; a token stands once in a row; an id outside the vocabulary, -1 say, is no entry). With q = softmax(logits / temperature),
+    loss = weight * temperature^2 * KL(p || q). `log_sum` float32 [R] (top_logits' at the same temperature): p_k = exp(teacher / temperature -
+    log_sum), and what is left of p stands against what is left of q as one more outcome (where the student leaves nothing, that outcome is
+    left out). Without it p = softmax(teacher / temperature) over the listed tokens alone. `weight` float32 [R]: a row of weight 0 is not
+    read; its loss and gradient are 0. A row without entries and without `log_sum` has the loss 0, one whose logits are all -inf, or hold
+    +inf or NaN, a loss of NaN."""
+    code, rows, vocab, ld = _logit_rows(logits, "distill_loss")
+    _need(ids, "ids", torch.int32, 2)
+    _need(teacher, "teacher", torch.float32, 2)
+    k = ids.shape[1]
+    if ids.shape[0] != rows or teacher.shape != ids.shape or not 1 <= k <= TOP_MOST:
+        raise KernelError(f"distill_loss: ids and teacher must be [{rows}, 1 to {TOP_MOST}], got {tuple(ids.shape)} and {tuple(teacher.shape)}")
+    if not ids.is_contiguous() or not teacher.is_contiguous() or ids.device != logits.device or teacher.device != logits.device:
+        raise KernelError("distill_loss: ids and teacher must be contiguous and on the logits' device")
+    _per_row(log_sum, "log_sum", torch.float32, rows, logits)
+    _per_row(weight, "weight", torch.float32, rows, logits)
+    temperature = _temperature(temperature, "distill_loss")
+    if out is not None and not gradient:
+        raise KernelError("distill_loss: out is where the gradient goes, and none is asked for")
+    loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    grad = _like_logits(logits, out, "distill_loss") if gradient else None
+    if rows:
+        _check(_lib("distill").r2_distill(code, _p(logits), C.c_longlong(ld), rows, vocab, _p(ids), _p(teacher), k, _p(log_sum), _p(weight),
+                                          C.c_float(temperature), _p(loss), _p(grad), C.c_longlong(_rows(grad, "out") if gradient else 0),
+                                          _stream()), "distill_loss")
+    return loss, grad
