@@ -71,3 +71,65 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
   const uint32_t b = __float_as_uint(v + 0.f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+
+// A piece of the row for a reader that may also be its writer in the same launch (no read-only path), not kept in L1. Elements beyond the row
+// are -inf.
+template <typename T>
+__device__ __forceinline__ uint4 load_once(const RowPieces<T>& row, int g) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(reinterpret_cast<const uint4*>(row.base) + g));
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void blank_outside(uint4& raw, const RowPieces<T>& row, int g) {
+  if (row.whole(g)) return;
+  const int first = row.first(g);
+  uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < RowPieces<T>::PER; ++i) {
+    if (first + i >= 0 && first + i < row.vocab) continue;
+    if (sizeof(T) == 4) w[i & 3] = 0xff800000u;
+    else w[(i >> 1) & 3] = (i & 1) ? (w[(i >> 1) & 3] & 0x0000ffffu) | 0xff800000u : (w[(i >> 1) & 3] & 0xffff0000u) | 0x0000ff80u;
+  }
+  raw = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {  // 2^x within 2^-22; 0 below the normal range
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The CTAs of a cluster along x share a row.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t cluster_address(const void* own, uint32_t rank) {  // of `own` in the shared memory of CTA `rank`
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(uint32_t(__cvta_generic_to_shared(own))), "r"(rank));
+  return there;
+}
+__device__ __forceinline__ void cluster_store(uint32_t address, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(address), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+
+template <typename... KArgs, typename... Args>
+static inline void r2_launch_clusters(void (*kernel)(KArgs...), int cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                      Args&&... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = (g_r2_pdl && !t_r2_plain_order) ? 2 : 1;
+  cudaLaunchKernelEx(&config, kernel, static_cast<Args&&>(args)...);  // a failure shows in launch_status()
+}
