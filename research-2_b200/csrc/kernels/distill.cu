@@ -11,25 +11,29 @@
 // teacher and a student that nearly agree lose no digits to cancellation, and for the same reason the mass outside the list is summed from its own
 // tokens, not taken from 1. A row whose weight is 0 is not read: its loss and gradient are 0 whatever stands there.
 //
-// A row is read once and its gradient written once: the CTAs of a cluster hold a row's 16-byte pieces in registers between the two. A
-// thread sums exponentials against its own maximum, warps and CTAs join these with their maxima, and one cluster barrier stands between
-// the sums and the gradient; float32 rows keep the exponentials in the logits' place, so that each is computed once. Rows beyond what
-// eight CTAs hold are read a second time.
+// A row is read once and its gradient written once. The CTAs of a cluster hold a row's 16-byte pieces in shared memory between the two; a
+// thread sums exponentials against its own maximum, and every warp sends what it has to all CTAs of the cluster, whose barriers count the
+// bytes. Clusters walk over the rows: while one is worked on, the next one's pieces are on their way. The listed tokens are taken out of a
+// row (their places become -inf) before it is summed, so that what is left is summed without looking at the list. Losses alone, and rows that
+// no cluster holds, take a second kernel that streams.
 #include "logit_rows.cuh"
+#include "sm100_ptx.cuh"
 
 namespace {
 
 constexpr int MOST_K = 256;
 constexpr int MOST_RANKS = 8;
-constexpr int PIECES = 8;   // of a thread, in registers
+constexpr int MOST_WARPS = 8;      // of a block, that work on pieces
+#define R2_ERR_TIMEOUT_SHARES 8
 
 struct DistillArgs {
   const void* logits; long long ld;
-  int vocab, k, ranks;
+  int rows, vocab, k, ranks, per;   // per: pieces of a row that a CTA has, whatever the row's alignment (the last one has what is left)
   const int32_t* ids; const float* teacher; const float* log_sum; const float* weight;
   float tau;
   float* loss;
   void* grad; long long grad_ld;
+  int* error;
 };
 
 __device__ __forceinline__ float no_less(float reference) { return reference == -INFINITY ? 0.f : reference; }
@@ -42,15 +46,367 @@ __device__ __forceinline__ float3 warp_join(float3 v) {
   return make_float3(common, warp_sum(v.y * f), warp_sum(v.z * f));
 }
 
-// ONE: a CTA's share of a row fits its registers. TAIL: there is a log_sum.
-template <typename T, int THREADS, bool ONE, bool TAIL>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
-distill_kernel(const DistillArgs a) {
-  constexpr int PER = RowPieces<T>::PER, CHUNK = THREADS * PIECES, WORDS = CHUNK * PER / 32;
-  constexpr bool KEEP = ONE && sizeof(T) == 4;   // exponentials stand in the logits' place
-  __shared__ uint32_t listed[WORDS];
-  __shared__ float parts[THREADS / 32][4];
-  __shared__ __align__(16) float4 shares[MOST_RANKS];
+
+// What a row's list says, from shared memory, by every warp for itself: the logarithm that the teacher's exponentials are taken against, and
+// their sum's mass.
+__device__ __forceinline__ float2 teacher_mass(const float* teacher, int k, int lane, bool tail, float log_sum) {
+  float against = log_sum, mass = 0.f;
+  if (!tail) {
+    float most = -INFINITY, sum = 0.f;
+    for (int j = lane; j < k; j += 32) most = fmaxf(most, teacher[j]);
+    most = no_less(warp_max(most));
+    for (int j = lane; j < k; j += 32) sum += expf(teacher[j] - most);
+    against = most + logf(warp_sum(sum));
+    if (against == -INFINITY) against = 0.f;   // no entries
+  }
+  for (int j = lane; j < k; j += 32) mass += expf(teacher[j] - against);
+  return make_float2(against, warp_sum(mass));
+}
+
+// The student's side of a row, joined over its warps.
+struct Student {
+  float common, total, inv_total, rest, rest_p, outside, whole;
+
+  Student() = default;
+  // From (reference, sum over listed, sum over others) of every warp, by any warp for itself.
+  __device__ __forceinline__ Student(const float4* shares, int n, int lane, bool tail, float mass) {
+    float3 v = make_float3(-INFINITY, 0.f, 0.f);
+    for (int i = lane; i < n; i += 32) {
+      const float4 s = shares[i];
+      const float m = fmaxf(v.x, s.x), f = rebase(v.x, m), g = rebase(s.x, m);
+      v = make_float3(m, v.y * f + s.y * g, v.z * f + s.z * g);
+    }
+    v = warp_join(v);
+    common = v.x;
+    total = v.y + v.z;
+    inv_total = __frcp_rn(total);
+    outside = whole = mass;
+    rest = v.z * inv_total;
+    rest_p = 0.f;
+    if (tail) {
+      rest_p = rest > 0.f ? fmaxf(1.f - mass, 0.f) : 0.f;
+      if (rest_p > 0.f) {
+        outside = __fdividef(mass - v.y * inv_total, rest);
+        whole = 1.f;
+      }
+    }
+  }
+
+  // The row's divergence, by one warp.
+  __device__ __forceinline__ float divergence(const int32_t* ids, const float* teacher, const float* xk, int k, int lane, bool tail, float c,
+                                              float against, float mass) const {
+    const float log2_total = log2f(total);
+    float kl = 0.f;
+    for (int j = lane; j < k; j += 32) {
+      if (ids[j] < 0) continue;
+      const float lq = (fmaf(xk[j], c, -common) - log2_total) * 0.693147181f, lp = teacher[j] - against, p = expf(lp), d = lp - lq;
+      if (tail) kl += p > 0.f ? p * (d + expm1f(-d)) : expf(lq);
+      else if (p > 0.f) kl += p * d;
+    }
+    kl = warp_sum(kl);
+    if (tail) {
+      const float d = logf(rest_p) - logf(rest);
+      kl += rest_p > 0.f ? rest_p * (d + expm1f(-d)) : rest > 0.f ? rest : mass - 1.f;
+    }
+    return kl;
+  }
+};
+
+// Entry j's gradient, over what stands there. A list that names a token more than once (`twice`): its first entry writes for all.
+template <typename T>
+__device__ __forceinline__ void write_listed(T* grad, const int32_t* ids, const float* teacher, const float* logits, int k, int j, bool twice,
+                                             float c, float against, float scale, const Student& q) {
+  float p = expf(teacher[j] - against), x = logits[j];
+  if (twice) {
+    p = 0.f;
+    for (int o = 0; o < k; ++o) {
+      if (ids[o] != ids[j]) continue;
+      if (o < j) return;
+      p += expf(teacher[o] - against);
+      x = fmaxf(x, logits[o]);   // (one entry took the logit out of the row, the others found -inf)
+    }
+  }
+  grad[ids[j]] = from_float<T>(scale * (exp2_approx(fmaf(x, c, -q.common)) * q.inv_total * q.whole - p));
+}
+
+// Sets the bits of the listed tokens among `bits` tokens from `zero` on; whether one was set already.
+__device__ __forceinline__ bool mark_listed(uint32_t* listed, const int32_t* ids, int k, int zero, int bits, int tid, int threads) {
+  bool again = false;
+  for (int j = tid; j < k; j += threads) {
+    const int at = ids[j] - zero;
+    if (ids[j] < 0 || at < 0 || at >= bits) continue;
+    const uint32_t bit = 1u << (at & 31);
+    again |= (atomicOr(&listed[at >> 5], bit) & bit) != 0u;
+  }
+  return again;
+}
+
+// One piece's exponentials (in v) into the sums over listed tokens and over the others.
+template <bool TAIL, int PER>
+__device__ __forceinline__ void add_piece(const float (&v)[PER], uint32_t bits, float& in_list, float& others) {
+  if (!TAIL || bits == 0u) {
+    float all = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) all += v[e];
+    others += all;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    if ((bits >> e) & 1u) in_list += v[e];
+    else others += v[e];
+  }
+}
+
+// Takes an element of the staged row out of it: what stood there; -inf stays.
+__device__ __forceinline__ float take_out(float* at) { return __uint_as_float(atomicExch(reinterpret_cast<unsigned int*>(at), 0xff800000u)); }
+__device__ __forceinline__ float take_out(bf16* at) {
+  unsigned short* bits = reinterpret_cast<unsigned short*>(at);
+  unsigned short old = *bits, seen;
+  while ((seen = atomicCAS(bits, old, static_cast<unsigned short>(0xff80))) != old) old = seen;
+  return __uint_as_float(static_cast<uint32_t>(old) << 16);
+}
+
+// 16 bytes into another CTA's shared memory, counted by that CTA's barrier; both places by their address there.
+__device__ __forceinline__ void send(uint32_t to, uint32_t barrier, float4 v) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "f"(v.x), "f"(v.y),
+               "f"(v.z), "f"(v.w), "r"(barrier)
+               : "memory");
+}
+__device__ __forceinline__ bool arrived(uint32_t barrier, uint32_t parity) {   // false: gave up
+  for (uint32_t spin = 0; spin < r2ptx::SPIN_LIMIT; ++spin) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(barrier), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (spin > 1024) __nanosleep(64);
+  }
+  return false;
+}
+
+// A block is eight warps (fewer for short rows) that work on pieces and one more that works on lists: it brings the next row's list, takes
+// its mass, and finishes the loss of the row before, all beside the others, which meet it once a row.
+template <typename T>
+__global__ void __launch_bounds__(32 * (MOST_WARPS + 1), 2)
+distill_held_kernel(const DistillArgs a) {
+  constexpr int PER = RowPieces<T>::PER, AHEAD = 16 / PER;   // pieces that a thread takes at a time
+  extern __shared__ __align__(16) uint4 staged[];            // [2][per]: this row's and the next row's pieces
+  __shared__ __align__(16) float4 shares[2][MOST_RANKS * MOST_WARPS];
+  __shared__ __align__(8) uint64_t shared_in[2];             // barriers: every warp of the cluster has sent
+  __shared__ int32_t ids[2][MOST_K];
+  __shared__ float teacher[2][MOST_K], xk[2][MOST_K], taken[MOST_K];
+  __shared__ float2 of_teacher[2];   // what the teacher's exponentials are taken against, and their sum
+  __shared__ Student students[2];
+  __shared__ int twice[2];
+  pdl_launch_dependents();
+  const int threads = int(blockDim.x) - 32, warps = threads >> 5;   // that work on pieces
+  const int ranks = a.ranks, step = int(gridDim.x) / ranks, rank = int(blockIdx.x) % ranks, tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+  const int g0 = rank * a.per, k = a.k;
+  const bool tail = a.log_sum != nullptr;
+  const float c = 1.44269504f / a.tau;
+  int row = int(blockIdx.x) / ranks, b = 0;
+  auto weight = [&](int r) { return r >= a.rows ? 0.f : a.weight != nullptr ? a.weight[r] : 1.f; };
+  if (tid < 2) {
+    r2ptx::mbar_init(r2ptx::smem_u32(&shared_in[tid]), 1u);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  cluster_arrive();
+  pdl_wait();
+  float w = weight(row), w_next = weight(row + step);
+
+  if (warp == warps) {
+    const float inv = 1.f / a.tau;
+    auto bring_list = [&](int r, int b) {
+      const float log_sum = tail ? a.log_sum[r] : 0.f;
+#pragma unroll 4
+      for (int j = lane; j < k; j += 32) {
+        const int id = a.ids[(long long)r * k + j];
+        const float t = a.teacher[(long long)r * k + j];
+        const bool held = id >= 0 && id < a.vocab;
+        ids[b][j] = held ? id : -1;
+        teacher[b][j] = held ? t * inv : -INFINITY;
+      }
+      __syncwarp();
+      if (rank == 0) {
+#pragma unroll 4
+        for (int j = lane; j < k; j += 32) xk[b][j] = ids[b][j] >= 0 ? to_float(static_cast<const T*>(a.logits)[(long long)r * a.ld + ids[b][j]]) : 0.f;
+      }
+      const float2 m = teacher_mass(teacher[b], k, lane, tail, log_sum);
+      if (lane == 0) {
+        of_teacher[b] = m;
+        twice[b] = 0;
+      }
+      __syncwarp();
+    };
+    float w_before = 0.f;
+    if (w != 0.f) bring_list(row, 0);
+    cluster_wait();
+    for (int before = -1;; row += step, b ^= 1) {
+      __syncthreads();
+      if (before >= 0 && rank == 0) {   // the loss of the row before
+        float loss = 0.f;
+        if (w_before != 0.f) {
+          const float2 t = of_teacher[b ^ 1];
+          loss = w_before * a.tau * a.tau * students[b ^ 1].divergence(ids[b ^ 1], teacher[b ^ 1], xk[b ^ 1], k, lane, tail, c, t.x, t.y);
+        }
+        if (lane == 0) a.loss[before] = loss;
+      }
+      if (row >= a.rows) return;
+      const float w_after = weight(row + 2 * step);
+      if (w_next != 0.f) bring_list(row + step, b ^ 1);
+      before = row;
+      w_before = w;
+      w = w_next;
+      w_next = w_after;
+    }
+  }
+
+  auto fetch = [&](int r, int b) {
+    const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)r * a.ld, a.vocab);
+    const int n = min(a.per, x.count - g0);
+    const uint4* from = reinterpret_cast<const uint4*>(x.base) + g0;
+    const uint32_t to = r2ptx::smem_u32(staged + b * a.per);
+#pragma unroll 4
+    for (int at = tid; at < n; at += threads) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + at * 16), "l"(from + at) : "memory");
+  };
+  auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); };
+  if (w != 0.f) fetch(row, 0);
+  cluster_wait();
+  uint32_t turn = 0;   // rows that the cluster has joined its sums for
+  for (; row < a.rows; row += step, b ^= 1) {
+    const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)row * a.ld, a.vocab);
+    const int n = max(0, min(a.per, x.count - g0)), last = x.count - 1 - g0, zero = x.first(g0);
+    T* grad = static_cast<T*>(a.grad) + (long long)row * a.grad_ld;
+    uint4* out = reinterpret_cast<uint4*>(grad - x.phase) + g0;
+    const bool vectors = (reinterpret_cast<uintptr_t>(out) & 15) == 0;   // the gradient's row starts at the logits' alignment
+    const float w_after = weight(row + 2 * step);
+    // pieces from `low` up to `high` lie in the row as a whole; the ends of the row may not
+    const int low = g0 == 0 && x.phase > 0 ? 1 : 0, high = last >= 0 && last < n && !x.whole(g0 + last) ? min(n, last) : n;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();   // the row and its list are there; the row before has done with its own
+    if (w_next != 0.f) fetch(row + step, b ^ 1);
+    uint4* pieces = staged + b * a.per;
+    T* tokens = reinterpret_cast<T*>(pieces);
+    // this lane's token at the row's ends (the first warp's: in a first piece, in a last piece)
+    int end = -1;
+    if (warp == 0 && lane < 2 * PER) {
+      const int at = lane < PER ? lane : last * PER + lane - PER;
+      if (lane < PER ? low == 1 && (last > 0 || high == n) : high < n) end = at;
+    }
+    if (w == 0.f) {
+      const float zeros[PER] = {};
+#pragma unroll 1
+      for (int at = low + tid; at < high; at += threads) store_piece<T, PER>(grad, x.first(g0 + at), a.vocab, zeros, vectors);
+      if (end >= 0 && zero + end >= 0 && zero + end < a.vocab) grad[zero + end] = from_float<T>(0.f);
+    } else {
+      if (end >= 0 && (zero + end < 0 || zero + end >= a.vocab)) {
+        tokens[end] = from_float<T>(-INFINITY);
+        end = -1;
+      }
+      const uint32_t barrier = r2ptx::smem_u32(&shared_in[turn & 1]);
+      if (tid == 0) r2ptx::mbar_expect_tx(barrier, uint32_t(ranks * warps) * 16u);
+      float reference = -INFINITY, in_list = 0.f, others = 0.f;
+#pragma unroll 1
+      for (int j = tid; j < k; j += threads) {
+        const int at = ids[b][j] - zero;
+        if (ids[b][j] < 0 || at < 0 || at >= n * PER) continue;
+        const float v = take_out(tokens + at);
+        if (v == -INFINITY) twice[b] = 1;
+        taken[j] = v;   // (read again behind a barrier)
+        const float m = fmaxf(reference, v * c);
+        in_list = in_list * rebase(reference, m) + exp2_approx(fmaf(v, c, -no_less(m)));
+        reference = m;
+      }
+      meet();
+#pragma unroll 1
+      for (int at0 = tid; at0 < n; at0 += AHEAD * threads) {
+        float v[AHEAD][PER], most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const uint32_t nothing = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+          uint4 raw = make_uint4(nothing, nothing, nothing, nothing);
+          if (at0 + i * threads < n) raw = pieces[at0 + i * threads];
+          unpack(raw, v[i], static_cast<const T*>(nullptr));
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+          for (int e = 0; e < PER; ++e) most = fmaxf(most, v[i][e]);
+        if (most * c > reference) {
+          const float f = rebase(reference, most * c);
+          in_list *= f;
+          others *= f;
+          reference = most * c;
+        }
+        const float shift = no_less(reference);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          float all = 0.f;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) all += exp2_approx(fmaf(v[i][e], c, -shift));
+          others += all;
+        }
+      }
+      const float3 sums = warp_join(make_float3(reference, in_list, others));
+      if (lane < ranks)
+        send(cluster_address(&shares[turn & 1][rank * warps + warp], lane), cluster_address(&shared_in[turn & 1], lane),
+             make_float4(sums.x, sums.y, sums.z, 0.f));
+      if (!arrived(barrier, (turn >> 1) & 1) && lane == 0) atomicMax(a.error, R2_ERR_TIMEOUT_SHARES);
+      const float2 t = of_teacher[b];
+      const Student q(shares[turn & 1], ranks * warps, lane, tail, t.y);
+      ++turn;
+      if (tid == 0) students[b] = q;
+      const float scale = w * a.tau, by = scale * q.outside * q.inv_total;
+      if (!vectors) {
+#pragma unroll 1
+        for (int at = low + tid; at < high; at += threads) {
+          float v[PER];
+          unpack(pieces[at], v, static_cast<const T*>(nullptr));
+#pragma unroll
+          for (int e = 0; e < PER; ++e) grad[x.first(g0 + at) + e] = from_float<T>(exp2_approx(fmaf(v[e], c, -q.common)) * by);
+        }
+      }
+#pragma unroll 1
+      for (int at0 = vectors ? low + tid : high; at0 < high; at0 += AHEAD * threads) {
+        uint4 raw[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+          if (at0 + i * threads < high) raw[i] = pieces[at0 + i * threads];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          float v[PER];
+          unpack(raw[i], v, static_cast<const T*>(nullptr));
+#pragma unroll
+          for (int e = 0; e < PER; ++e) v[e] = exp2_approx(fmaf(v[e], c, -q.common)) * by;
+          if (at0 + i * threads < high) out[at0 + i * threads] = pack(v, static_cast<const T*>(nullptr));
+        }
+      }
+      if (end >= 0) grad[zero + end] = from_float<T>(exp2_approx(fmaf(to_float(tokens[end]), c, -q.common)) * by);
+      meet();   // the listed tokens' gradients lie over what stands there
+#pragma unroll 1
+      for (int j = tid; j < k; j += threads) {
+        const int at = ids[b][j] - zero;
+        if (ids[b][j] >= 0 && at >= 0 && at < n * PER) write_listed(grad, ids[b], teacher[b], taken, k, j, twice[b] != 0, c, t.x, scale, q);
+      }
+    }
+    w = w_next;
+    w_next = w_after;
+  }
+  __syncthreads();
+}
+
+// Losses alone (one pass over the row), and gradients of rows that no cluster holds (two).
+template <typename T, bool TAIL>
+__global__ void __launch_bounds__(512, 2)
+distill_streamed_kernel(const DistillArgs a) {
+  constexpr int THREADS = 512, PER = RowPieces<T>::PER, DEPTH = 4;
+  extern __shared__ __align__(16) uint32_t bits_s[];   // a bit for each token of this CTA's share
+  __shared__ __align__(16) float4 shares[MOST_RANKS * (THREADS / 32)];
   __shared__ int32_t ids[MOST_K];
   __shared__ float teacher[MOST_K], xk[MOST_K];
   __shared__ int twice;
@@ -61,7 +417,7 @@ distill_kernel(const DistillArgs a) {
   const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)row * a.ld, a.vocab);
   T* grad = a.grad != nullptr ? static_cast<T*>(a.grad) + (long long)row * a.grad_ld : nullptr;
   const bool vectors = ((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(x.base + x.phase)) & 15) == 0;
-  const int per = (x.count + ranks - 1) / ranks, g0 = rank * per, n = max(0, min(per, x.count - g0));
+  const int g0 = rank * a.per, n = max(0, min(a.per, x.count - g0));
   const float w = a.weight != nullptr ? a.weight[row] : 1.f;
   if (w == 0.f) {  // (every CTA of the cluster)
     if (grad != nullptr) {
@@ -71,17 +427,7 @@ distill_kernel(const DistillArgs a) {
     if (rank == 0 && tid == 0) a.loss[row] = 0.f;
     return;
   }
-  if (ranks > 1) cluster_arrive();   // this CTA runs: the others may write into its shared memory once all have arrived
-
-  uint4 raw[PIECES];
-  auto load = [&](int c0) {
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int at = c0 + tid + i * THREADS;
-      if (at < n) raw[i] = load_once(x, g0 + at);
-    }
-  };
-  load(0);
+  if (ranks > 1) cluster_arrive();
   const float inv = 1.f / a.tau, c = 1.44269504f / a.tau;
   for (int j = tid; j < k; j += THREADS) {
     const int id = a.ids[(long long)row * k + j];
@@ -90,201 +436,159 @@ distill_kernel(const DistillArgs a) {
     teacher[j] = held ? a.teacher[(long long)row * k + j] * inv : -INFINITY;
     xk[j] = held ? to_float(x.base[x.phase + id]) : 0.f;
   }
-
-  float3 sums = make_float3(-INFINITY, 0.f, 0.f);   // this thread's reference (an exponent of two), over listed tokens, over the others
-  for (int c0 = 0; ONE ? c0 == 0 : c0 < n; c0 += CHUNK) {
-    if (!ONE && c0 > 0) {
-      __syncthreads();
-      load(c0);
-    }
-    if (TAIL || c0 == 0) {
-      const int zero = x.first(g0 + c0);   // the token of the first bit
-      for (int i = tid; i < WORDS; i += THREADS) listed[i] = 0u;
-      __syncthreads();
-      for (int j = tid; j < k; j += THREADS) {
-        const int at = ids[j] - zero;
-        if (ids[j] >= 0 && at >= 0 && at < CHUNK * PER) {
-          const uint32_t bit = 1u << (at & 31);
-          if (atomicOr(&listed[at >> 5], bit) & bit) twice = 1;
-        }
-      }
-      __syncthreads();
-    }
+  if (TAIL || grad != nullptr)
+    for (int i = tid; i < (n * PER + 31) / 32; i += THREADS) bits_s[i] = 0u;
+  __syncthreads();
+  if (TAIL || grad != nullptr)
+    if (mark_listed(bits_s, ids, k, x.first(g0), n * PER, tid, THREADS)) twice = 1;
+  __syncthreads();
+  float reference = -INFINITY, in_list = 0.f, others = 0.f;
+  for (int c0 = tid; c0 < n; c0 += DEPTH * THREADS) {
+    uint4 raw[DEPTH];
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i)
+      if (c0 + i * THREADS < n) raw[i] = load_once(x, g0 + c0 + i * THREADS);
     float most = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int at = c0 + tid + i * THREADS;
-      if (at >= n) continue;
-      blank_outside(raw[i], x, g0 + at);
+    for (int i = 0; i < DEPTH; ++i) {
+      if (c0 + i * THREADS >= n) continue;
+      blank_outside(raw[i], x, g0 + c0 + i * THREADS);
       float v[PER];
       unpack(raw[i], v, static_cast<const T*>(nullptr));
 #pragma unroll
       for (int e = 0; e < PER; ++e) most = fmaxf(most, v[e]);
     }
-    const float reference = fmaxf(sums.x, most * c), shift = no_less(reference);
-    if (!ONE) {
-      const float f = rebase(sums.x, shift);
-      sums.y *= f;
-      sums.z *= f;
+    if (most * c > reference) {
+      const float f = rebase(reference, most * c);
+      in_list *= f;
+      others *= f;
+      reference = most * c;
     }
-    sums.x = reference;
+    const float shift = no_less(reference);
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int at = tid + i * THREADS;
-      if (c0 + at >= n) continue;
-      float v[PER];
-      unpack(raw[i], v, static_cast<const T*>(nullptr));
-#pragma unroll
-      for (int e = 0; e < PER; ++e) v[e] = exp2_approx(fmaf(v[e], c, -shift));
-      float all = 0.f;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) all += v[e];
-      uint32_t bits = 0u;
-      if (TAIL) bits = (listed[at * PER / 32] >> (at * PER % 32)) & ((1u << PER) - 1u);
-      if (bits == 0u) {
-        sums.z += all;
-      } else {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-          if ((bits >> e) & 1u) sums.y += v[e];
-          else sums.z += v[e];
-        }
-      }
-      if (KEEP) raw[i] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-    }
-  }
-
-  // the teacher's side, in every warp for itself: no barrier
-  float t_sum = 0.f, mass = 0.f;
-  if (TAIL) {
-    t_sum = a.log_sum[row];
-  } else {
-    float t_max = -INFINITY;
-    for (int j = lane; j < k; j += 32) t_max = fmaxf(t_max, teacher[j]);
-    t_max = no_less(warp_max(t_max));
-    for (int j = lane; j < k; j += 32) t_sum += teacher[j] == -INFINITY ? 0.f : expf(teacher[j] - t_max);
-    t_sum = t_max + logf(warp_sum(t_sum));
-  }
-  auto log_p = [&](int j) { return teacher[j] == -INFINITY ? -INFINITY : teacher[j] - t_sum; };
-  for (int j = lane; j < k; j += 32) mass += expf(log_p(j));
-  mass = warp_sum(mass);
-
-  const float own_reference = sums.x;
-  sums = warp_join(sums);
-  if (lane == 0) {
-    parts[tid >> 5][0] = sums.x;
-    parts[tid >> 5][1] = sums.y;
-    parts[tid >> 5][2] = sums.z;
-  }
-  __syncthreads();
-  if (tid < 32) {
-    const bool some = tid < THREADS / 32;
-    const float3 v = warp_join(make_float3(some ? parts[tid % (THREADS / 32)][0] : -INFINITY, some ? parts[tid % (THREADS / 32)][1] : 0.f,
-                                           some ? parts[tid % (THREADS / 32)][2] : 0.f));
-    if (ranks > 1) {
-      cluster_wait();
-      if (tid < ranks) cluster_store(cluster_address(&shares[rank], tid), make_float4(v.x, v.y, v.z, 0.f));
-    } else if (tid == 0) {
-      shares[0] = make_float4(v.x, v.y, v.z, 0.f);
-    }
-  } else if (ranks > 1) {
-    cluster_wait();
-  }
-  if (ranks > 1) {
-    cluster_arrive();
-    cluster_wait();
-  } else {
-    __syncthreads();
-  }
-  float common = -INFINITY, in_list = 0.f, rest = 0.f;
-  for (int r = 0; r < ranks; ++r) common = fmaxf(common, shares[r].x);
-  for (int r = 0; r < ranks; ++r) {
-    const float f = rebase(shares[r].x, common);
-    in_list += shares[r].y * f;
-    rest += shares[r].z * f;
-  }
-  const float total = in_list + rest;   // (without TAIL everything stands in `rest`)
-  float outside = mass, whole = mass, rest_p = 0.f;
-  rest /= total;
-  if (TAIL) {
-    rest_p = rest > 0.f ? fmaxf(1.f - mass, 0.f) : 0.f;
-    if (rest_p > 0.f) {
-      outside = (mass - in_list / total) / rest;
-      whole = 1.f;
-    }
-  }
-  const float log2_total = log2f(total), log2_e = 0.693147181f;
-  if (rank == 0 && tid < 32) {
-    float kl = 0.f;
-    for (int j = lane; j < k; j += 32) {
-      if (ids[j] < 0) continue;
-      const float lq = (fmaf(xk[j], c, -common) - log2_total) * log2_e, lp = log_p(j), p = expf(lp), d = lp - lq;
-      if (TAIL) kl += p > 0.f ? p * (d + expm1f(-d)) : expf(lq);
-      else if (p > 0.f) kl += p * d;
-    }
-    kl = warp_sum(kl);
-    if (TAIL) {
-      const float d = logf(rest_p) - logf(rest);
-      kl += rest_p > 0.f ? rest_p * (d + expm1f(-d)) : rest > 0.f ? rest : mass - 1.f;
-    }
-    if (lane == 0) a.loss[row] = w * a.tau * a.tau * kl;
-  }
-  if (grad == nullptr) return;
-
-  const float scale = w * a.tau, by = scale * outside / total, f = rebase(own_reference, common) * by;
-  for (int c0 = 0; ONE ? c0 == 0 : c0 < n; c0 += CHUNK) {
-    if (!ONE) load(c0);
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int at = c0 + tid + i * THREADS;
+    for (int i = 0; i < DEPTH; ++i) {
+      const int at = c0 + i * THREADS;
       if (at >= n) continue;
       float v[PER];
       unpack(raw[i], v, static_cast<const T*>(nullptr));
 #pragma unroll
-      for (int e = 0; e < PER; ++e) v[e] = KEEP ? v[e] * f : exp2_approx(fmaf(v[e], c, -common)) * by;
-      store_piece<T, PER>(grad, x.first(g0 + at), a.vocab, v, vectors);
+      for (int e = 0; e < PER; ++e) v[e] = exp2_approx(fmaf(v[e], c, -shift));
+      uint32_t bits = 0u;
+      if (TAIL) bits = (bits_s[at * PER / 32] >> (at * PER % 32)) & ((1u << PER) - 1u);
+      add_piece<TAIL>(v, bits, in_list, others);
     }
   }
-  __syncthreads();   // what follows lies over it
-  const int from = x.first(g0), to = from + n * PER;
-  for (int j = tid; j < k; j += THREADS) {
-    const int id = ids[j];
-    if (id < 0 || id < from || id >= to) continue;
-    float p = expf(log_p(j));
-    if (twice) {  // a list that names a token more than once: its first entry writes for all
-      bool earlier = false;
-      p = 0.f;
-      for (int o = 0; o < k; ++o) {
-        if (ids[o] != id) continue;
-        earlier |= o < j;
-        p += expf(log_p(o));
-      }
-      if (earlier) continue;
+  const float3 sums = warp_join(make_float3(reference, in_list, others));
+  if (ranks > 1) {
+    cluster_wait();
+    if (lane < ranks) cluster_store(cluster_address(&shares[rank * (THREADS / 32) + (tid >> 5)], lane), make_float4(sums.x, sums.y, sums.z, 0.f));
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    if (lane == 0) shares[tid >> 5] = make_float4(sums.x, sums.y, sums.z, 0.f);
+    __syncthreads();
+  }
+  if (grad == nullptr && (rank > 0 || tid >= 32)) return;
+  const float2 t = teacher_mass(teacher, k, lane, TAIL, TAIL ? a.log_sum[row] : 0.f);
+  const Student q(shares, ranks * (THREADS / 32), lane, TAIL, t.y);
+  if (rank == 0 && tid < 32) {
+    const float kl = q.divergence(ids, teacher, xk, k, lane, TAIL, c, t.x, t.y);
+    if (lane == 0) a.loss[row] = w * a.tau * a.tau * kl;
+  }
+  if (grad == nullptr) return;
+  const float scale = w * a.tau, by = scale * q.outside * q.inv_total;
+  for (int c0 = tid; c0 < n; c0 += DEPTH * THREADS) {
+    uint4 raw[DEPTH];
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i)
+      if (c0 + i * THREADS < n) raw[i] = load_once(x, g0 + c0 + i * THREADS);
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      if (c0 + i * THREADS >= n) continue;
+      float v[PER];
+      unpack(raw[i], v, static_cast<const T*>(nullptr));
+#pragma unroll
+      for (int e = 0; e < PER; ++e) v[e] = exp2_approx(fmaf(v[e], c, -q.common)) * by;
+      store_piece<T, PER>(grad, x.first(g0 + c0 + i * THREADS), a.vocab, v, vectors);
     }
-    grad[id] = from_float<T>(scale * (exp2_approx(fmaf(xk[j], c, -common)) / total * whole - p));
+  }
+  __syncthreads();
+  for (int j = tid; j < k; j += THREADS) {
+    const int at = ids[j] - x.first(g0);
+    if (ids[j] >= 0 && at >= 0 && at < n * PER) write_listed(grad, ids, teacher, xk, k, j, twice != 0, c, t.x, scale, q);
   }
 }
 
-template <typename T, int THREADS, bool ONE>
-void launch_tail(const DistillArgs& a, int rows, cudaStream_t stream) {
-  const dim3 grid(unsigned(rows) * unsigned(a.ranks));
-  if (a.log_sum != nullptr) r2_launch_clusters(distill_kernel<T, THREADS, ONE, true>, a.ranks, grid, dim3(THREADS), size_t(0), stream, a);
-  else r2_launch_clusters(distill_kernel<T, THREADS, ONE, false>, a.ranks, grid, dim3(THREADS), size_t(0), stream, a);
-}
+constexpr int MOST_STREAMED_BITS = 1 << 20;   // tokens of a CTA's share (128 KB of bits)
+
+constexpr int HELD_TWO = 3300, HELD_ONE = 6800;   // pieces of a CTA's share where two CTAs, or one, fit an SM (two rows' shares in shared memory)
 
 template <typename T>
-int launch(DistillArgs a, int rows, cudaStream_t stream) {
-  const int pieces = (a.vocab + 2 * RowPieces<T>::PER - 2) / RowPieces<T>::PER;   // of a row at any alignment, at most
-  if (pieces <= 128 * PIECES) {
-    a.ranks = 1;
-    launch_tail<T, 128, true>(a, rows, stream);
-    return launch_status();
+int launch_held(const DistillArgs& a, cudaStream_t stream) {
+  const int warps = max(1, min(MOST_WARPS, a.per / 64));
+  const size_t smem = size_t(a.per) * 32;
+  static std::atomic<bool> allowed[64];
+  const int status = allow_smem(distill_held_kernel<T>, size_t(HELD_ONE) * 32, allowed);
+  if (status != R2_OK) return status;
+  // how many clusters run at a time, asked once for each device and shape (a table that forgets)
+  struct Resident {
+    std::atomic<unsigned long long> shape_and_clusters;
+  };
+  static Resident resident[64];
+  int device = 0, clusters = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return int(e);
+  const unsigned long long shape = (static_cast<unsigned long long>(device) << 56) | (static_cast<unsigned long long>(a.ranks) << 48) |
+                                   (static_cast<unsigned long long>(a.per) << 24);
+  Resident& place = resident[(a.per * 8 + a.ranks + device) % 64];
+  const unsigned long long known = place.shape_and_clusters.load(std::memory_order_relaxed);
+  if ((known >> 24) == (shape >> 24) && known != 0) {
+    clusters = int(known & 0xffffff);
+  } else {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(a.ranks) * 4096u);
+    config.blockDim = dim3(unsigned(32 * (warps + 1)));
+    config.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(a.ranks);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&clusters, distill_held_kernel<T>, &config);
+    if (e != cudaSuccess) return int(e);
+    if (clusters < 1) return R2_UNSUPPORTED;
+    place.shape_and_clusters.store(shape | static_cast<unsigned long long>(clusters), std::memory_order_relaxed);
   }
-  a.ranks = min(MOST_RANKS, (pieces + 512 * PIECES - 1) / (512 * PIECES));
-  if ((long long)rows * a.ranks > 0x7fffffffLL) return R2_BAD_SHAPE;
-  if ((pieces + a.ranks - 1) / a.ranks <= 512 * PIECES) launch_tail<T, 512, true>(a, rows, stream);
-  else launch_tail<T, 512, false>(a, rows, stream);
+  r2_launch_clusters(distill_held_kernel<T>, a.ranks, dim3(unsigned(min(a.rows, clusters) * a.ranks)), dim3(unsigned(32 * (warps + 1))), smem, stream, a);
   return launch_status();
+}
+
+template <typename T, bool TAIL>
+int launch_streamed(DistillArgs a, int pieces, cudaStream_t stream) {
+  // a row to a CTA where there are CTAs enough for the SMs, else cut over several
+  a.ranks = 1;
+  while (a.ranks < MOST_RANKS && ((long long)a.rows * a.ranks < 296 || (pieces / a.ranks + 1) * RowPieces<T>::PER > MOST_STREAMED_BITS)
+         && pieces / a.ranks > 1024) a.ranks *= 2;
+  const int per = a.per = (pieces + a.ranks - 1) / a.ranks;
+  if (per * RowPieces<T>::PER > MOST_STREAMED_BITS) return R2_UNSUPPORTED;
+  if ((long long)a.rows * a.ranks > 0x7fffffffLL) return R2_BAD_SHAPE;
+  static std::atomic<bool> allowed[64];
+  const int status = allow_smem(distill_streamed_kernel<T, TAIL>, MOST_STREAMED_BITS / 8, allowed);
+  if (status != R2_OK) return status;
+  r2_launch_clusters(distill_streamed_kernel<T, TAIL>, a.ranks, dim3(unsigned(a.rows) * unsigned(a.ranks)), dim3(512),
+                     size_t(per * RowPieces<T>::PER + 31) / 32 * 4, stream, a);
+  return launch_status();
+}
+
+template <typename T, bool TAIL>
+int launch(DistillArgs a, cudaStream_t stream) {
+  const int pieces = (a.vocab + 2 * RowPieces<T>::PER - 2) / RowPieces<T>::PER;   // of a row at any alignment, at most
+  if (a.grad == nullptr || pieces > MOST_RANKS * HELD_ONE) return launch_streamed<T, TAIL>(a, pieces, stream);
+  a.ranks = min(MOST_RANKS, (pieces + HELD_TWO - 1) / HELD_TWO);
+  a.per = (pieces + a.ranks - 1) / a.ranks;
+  return launch_held<T>(a, stream);
 }
 
 }  // namespace
@@ -293,11 +597,12 @@ int launch(DistillArgs a, int rows, cudaStream_t stream) {
 // [rows] or null -> loss [rows] float; grad [rows, vocab] of dtype with row stride grad_ld, null, or the logits themselves.
 extern "C" int r2_distill(int dtype, const void* logits, long long ld, int rows, int vocab, const int32_t* ids, const float* teacher, int k,
                           const float* log_sum, const float* weight, float temperature, float* loss, void* grad, long long grad_ld,
-                          cudaStream_t stream) {
+                          int* error, cudaStream_t stream) {
   if (dtype != R2_F32 && dtype != R2_BF16) return R2_BAD_DTYPE;
   if (rows < 0 || vocab < 1 || vocab > (1 << 30) || ld < vocab || (grad != nullptr && grad_ld < vocab) || k < 1) return R2_BAD_SHAPE;
   if (k > MOST_K || !(temperature > 0.f)) return R2_UNSUPPORTED;
   if (rows == 0) return R2_OK;
-  const DistillArgs a = {logits, ld, vocab, k, 1, ids, teacher, log_sum, weight, temperature, loss, grad, grad_ld};
-  return dtype == R2_F32 ? launch<float>(a, rows, stream) : launch<bf16>(a, rows, stream);
+  const DistillArgs a = {logits, ld, rows, vocab, k, 1, 0, ids, teacher, log_sum, weight, temperature, loss, grad, grad_ld, error};
+  if (log_sum != nullptr) return dtype == R2_F32 ? launch<float, true>(a, stream) : launch<bf16, true>(a, stream);
+  return dtype == R2_F32 ? launch<float, false>(a, stream) : launch<bf16, false>(a, stream);
 }

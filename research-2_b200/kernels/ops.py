@@ -38,6 +38,7 @@ class KernelTimeout(KernelError):
         5: "a key/value tile of prefill attention did not arrive (tensor copy)",
         6: "a stage of the tensor-core prefill attention did not complete",
         7: "a step of the resident decode kernel did not reach its grid barrier",
+        8: "the sums of a row that CTAs share (distillation) did not arrive",
         99: "a wait that a test let run out",
     }
 
@@ -1939,7 +1940,10 @@ def _like_logits(logits: torch.Tensor, out: torch.Tensor | None, what: str) -> t
     if out is None:
         ld = _rows(logits, "logits")
         ld = ld if vocab <= ld <= vocab + max(64, vocab // 16) else vocab
-        return torch.empty_strided((rows, vocab), (ld, 1), dtype=logits.dtype, device=logits.device)
+        skip = logits.data_ptr() % 16 // logits.element_size()
+        if skip == 0:
+            return torch.empty_strided((rows, vocab), (ld, 1), dtype=logits.dtype, device=logits.device)
+        return torch.empty(max(0, rows - 1) * ld + vocab + skip, dtype=logits.dtype, device=logits.device).as_strided((rows, vocab), (ld, 1), skip)
     _need(out, "out", logits.dtype, 2)
     if out.shape != logits.shape or out.device != logits.device:
         raise KernelError(f"{what}: out must have the logits' shape and device, got {tuple(out.shape)} on {out.device}")
@@ -2069,5 +2073,5 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
     if rows:
         _check(_lib("distill").r2_distill(code, _p(logits), C.c_longlong(ld), rows, vocab, _p(ids), _p(teacher), k, _p(log_sum), _p(weight),
                                           C.c_float(temperature), _p(loss), _p(grad), C.c_longlong(_rows(grad, "out") if gradient else 0),
-                                          _stream()), "distill_loss")
+                                          _p(_workspace(logits.device).error), _stream()), "distill_loss")
     return loss, grad
