@@ -189,15 +189,73 @@ __device__ __forceinline__ bool arrived(uint32_t barrier, uint32_t parity) {   /
   return false;
 }
 
-// A block is eight warps (fewer for short rows) that work on pieces and one more that works on lists: it brings the next row's list, takes
-// its mass, and finishes the loss of the row before, all beside the others, which meet it once a row.
+// Sums of exponentials against a reference that the thread chooses as it goes.
+template <typename T>
+struct Sums {
+  float reference = -INFINITY, in_list = 0.f, others = 0.f;   // an exponent of two; what is summed is 2^(x c - reference)
+
+  __device__ __forceinline__ void raise(float to) {
+    if (!(to > reference)) return;
+    const float f = rebase(reference, to);
+    in_list *= f;
+    others *= f;
+    reference = to;
+  }
+  // N pieces. The reference is raised where a sum leaves the middle of the range; a maximum of every piece is not looked for.
+  template <int N>
+  __device__ __forceinline__ void add(const uint4 (&raw)[N], float c) {
+    constexpr int PAIRS = RowPieces<T>::PER / 2;
+    const uint64_t cc = two_of(c, c);
+    float sum;
+    auto exponentials = [&]() {
+      const float shift = -no_less(reference);
+      const uint64_t ss = two_of(shift, shift);
+      uint64_t acc[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        uint64_t p[PAIRS];
+        unpack_pairs(raw[i], p, static_cast<const T*>(nullptr));
+        acc[i] = exp2_two(fma_two(p[0], cc, ss));
+#pragma unroll
+        for (int j = 1; j < PAIRS; ++j) acc[i] = add_two(acc[i], exp2_two(fma_two(p[j], cc, ss)));
+      }
+#pragma unroll
+      for (int i = 1; i < N; ++i) acc[0] = add_two(acc[0], acc[i]);
+      const float2 v = halves(acc[0]);
+      sum = v.x + v.y;
+    };
+    exponentials();
+    if (reference == -INFINITY || !(sum > 1e-18f && sum < 1e18f)) {
+      const float before = reference;
+      raise(most(raw) * c);
+      if (reference != before) exponentials();
+    }
+    others += sum;
+  }
+  template <int N>
+  static __device__ __forceinline__ float most(const uint4 (&raw)[N]) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float v[RowPieces<T>::PER];
+      unpack(raw[i], v, static_cast<const T*>(nullptr));
+#pragma unroll
+      for (int e = 0; e < RowPieces<T>::PER; ++e) m = fmaxf(m, v[e]);
+    }
+    return m;
+  }
+};
+
+// A block is eight warps (fewer for short rows) that work on pieces and one more that brings: it has the next row's share copied, brings
+// its list and takes its mass, and finishes the loss of the row before, all beside the others, which meet it once a row. Rows that weigh
+// nothing are not brought; `slot` counts the others, two at a time.
 template <typename T>
 __global__ void __launch_bounds__(32 * (MOST_WARPS + 1), 2)
 distill_held_kernel(const DistillArgs a) {
   constexpr int PER = RowPieces<T>::PER, AHEAD = 16 / PER;   // pieces that a thread takes at a time
-  extern __shared__ __align__(16) uint4 staged[];            // [2][per]: this row's and the next row's pieces
+  extern __shared__ __align__(16) uint4 staged[];            // [2][per]
   __shared__ __align__(16) float4 shares[2][MOST_RANKS * MOST_WARPS];
-  __shared__ __align__(8) uint64_t shared_in[2];             // barriers: every warp of the cluster has sent
+  __shared__ __align__(8) uint64_t landed[2], shared_in[2];  // barriers: a row's share is there; every warp of the cluster has sent its sums
   __shared__ int32_t ids[2][MOST_K];
   __shared__ float teacher[2][MOST_K], xk[2][MOST_K], taken[MOST_K];
   __shared__ float2 of_teacher[2];   // what the teacher's exponentials are taken against, and their sum
@@ -209,19 +267,33 @@ distill_held_kernel(const DistillArgs a) {
   const int g0 = rank * a.per, k = a.k;
   const bool tail = a.log_sum != nullptr;
   const float c = 1.44269504f / a.tau;
-  int row = int(blockIdx.x) / ranks, b = 0;
+  int row = int(blockIdx.x) / ranks;
+  uint32_t slot = 0;   // rows brought so far, less this one: its places are slot % 2, its barriers' phase slot / 2
   auto weight = [&](int r) { return r >= a.rows ? 0.f : a.weight != nullptr ? a.weight[r] : 1.f; };
-  if (tid < 2) {
-    r2ptx::mbar_init(r2ptx::smem_u32(&shared_in[tid]), 1u);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  cluster_arrive();
-  pdl_wait();
-  float w = weight(row), w_next = weight(row + step);
 
   if (warp == warps) {
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        r2ptx::mbar_init(r2ptx::smem_u32(&landed[i]), 1u);
+        r2ptx::mbar_init(r2ptx::smem_u32(&shared_in[i]), 1u);
+      }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    cluster_arrive();
+    pdl_wait();
     const float inv = 1.f / a.tau;
-    auto bring_list = [&](int r, int b) {
+    auto bring = [&](int r, int b) {
+      if (lane == 0) {
+        const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)r * a.ld, a.vocab);
+        const uint32_t bytes = uint32_t(min(a.per, x.count - g0)) * 16u, barrier = r2ptx::smem_u32(&landed[b]);
+        r2ptx::mbar_expect_tx(barrier, bytes);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                         r2ptx::smem_u32(staged + b * a.per)),
+                     "l"(reinterpret_cast<const uint4*>(x.base) + g0), "r"(bytes), "r"(barrier)
+                     : "memory");
+      }
       const float log_sum = tail ? a.log_sum[r] : 0.f;
 #pragma unroll 4
       for (int j = lane; j < k; j += 32) {
@@ -243,22 +315,24 @@ distill_held_kernel(const DistillArgs a) {
       }
       __syncwarp();
     };
-    float w_before = 0.f;
-    if (w != 0.f) bring_list(row, 0);
+    float w = weight(row), w_next = weight(row + step), w_before = 0.f;
+    if (w != 0.f) bring(row, 0);
     cluster_wait();
-    for (int before = -1;; row += step, b ^= 1) {
+    for (int before = -1;; row += step) {
       __syncthreads();
       if (before >= 0 && rank == 0) {   // the loss of the row before
         float loss = 0.f;
         if (w_before != 0.f) {
-          const float2 t = of_teacher[b ^ 1];
-          loss = w_before * a.tau * a.tau * students[b ^ 1].divergence(ids[b ^ 1], teacher[b ^ 1], xk[b ^ 1], k, lane, tail, c, t.x, t.y);
+          const int b = (slot - 1) & 1;
+          const float2 t = of_teacher[b];
+          loss = w_before * a.tau * a.tau * students[b].divergence(ids[b], teacher[b], xk[b], k, lane, tail, c, t.x, t.y);
         }
         if (lane == 0) a.loss[before] = loss;
       }
       if (row >= a.rows) return;
       const float w_after = weight(row + 2 * step);
-      if (w_next != 0.f) bring_list(row + step, b ^ 1);
+      if (w != 0.f) ++slot;
+      if (w_next != 0.f) bring(row + step, slot & 1);
       before = row;
       w_before = w;
       w = w_next;
@@ -266,19 +340,12 @@ distill_held_kernel(const DistillArgs a) {
     }
   }
 
-  auto fetch = [&](int r, int b) {
-    const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)r * a.ld, a.vocab);
-    const int n = min(a.per, x.count - g0);
-    const uint4* from = reinterpret_cast<const uint4*>(x.base) + g0;
-    const uint32_t to = r2ptx::smem_u32(staged + b * a.per);
-#pragma unroll 4
-    for (int at = tid; at < n; at += threads) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + at * 16), "l"(from + at) : "memory");
-  };
+  cluster_arrive();
+  pdl_wait();
   auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); };
-  if (w != 0.f) fetch(row, 0);
+  float w = weight(row), w_next = weight(row + step);
   cluster_wait();
-  uint32_t turn = 0;   // rows that the cluster has joined its sums for
-  for (; row < a.rows; row += step, b ^= 1) {
+  for (; row < a.rows; row += step) {
     const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)row * a.ld, a.vocab);
     const int n = max(0, min(a.per, x.count - g0)), last = x.count - 1 - g0, zero = x.first(g0);
     T* grad = static_cast<T*>(a.grad) + (long long)row * a.grad_ld;
@@ -287,11 +354,10 @@ distill_held_kernel(const DistillArgs a) {
     const float w_after = weight(row + 2 * step);
     // pieces from `low` up to `high` lie in the row as a whole; the ends of the row may not
     const int low = g0 == 0 && x.phase > 0 ? 1 : 0, high = last >= 0 && last < n && !x.whole(g0 + last) ? min(n, last) : n;
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();   // the row and its list are there; the row before has done with its own
-    if (w_next != 0.f) fetch(row + step, b ^ 1);
+    const int b = slot & 1;
     uint4* pieces = staged + b * a.per;
     T* tokens = reinterpret_cast<T*>(pieces);
+    __syncthreads();   // the row's list is there; the row before has done with its own
     // this lane's token at the row's ends (the first warp's: in a first piece, in a last piece)
     int end = -1;
     if (warp == 0 && lane < 2 * PER) {
@@ -304,13 +370,15 @@ distill_held_kernel(const DistillArgs a) {
       for (int at = low + tid; at < high; at += threads) store_piece<T, PER>(grad, x.first(g0 + at), a.vocab, zeros, vectors);
       if (end >= 0 && zero + end >= 0 && zero + end < a.vocab) grad[zero + end] = from_float<T>(0.f);
     } else {
+      const uint32_t barrier = r2ptx::smem_u32(&shared_in[b]), phase = (slot >> 1) & 1;
+      ++slot;
+      if (!r2ptx::mbar_wait(r2ptx::smem_u32(&landed[b]), phase) && lane == 0) atomicMax(a.error, R2_ERR_TIMEOUT_SHARES);
       if (end >= 0 && (zero + end < 0 || zero + end >= a.vocab)) {
         tokens[end] = from_float<T>(-INFINITY);
         end = -1;
       }
-      const uint32_t barrier = r2ptx::smem_u32(&shared_in[turn & 1]);
       if (tid == 0) r2ptx::mbar_expect_tx(barrier, uint32_t(ranks * warps) * 16u);
-      float reference = -INFINITY, in_list = 0.f, others = 0.f;
+      Sums<T> sums;
 #pragma unroll 1
       for (int j = tid; j < k; j += threads) {
         const int at = ids[b][j] - zero;
@@ -318,73 +386,58 @@ distill_held_kernel(const DistillArgs a) {
         const float v = take_out(tokens + at);
         if (v == -INFINITY) twice[b] = 1;
         taken[j] = v;   // (read again behind a barrier)
-        const float m = fmaxf(reference, v * c);
-        in_list = in_list * rebase(reference, m) + exp2_approx(fmaf(v, c, -no_less(m)));
-        reference = m;
+        sums.raise(v * c);
+        sums.in_list += exp2_approx(fmaf(v, c, -no_less(sums.reference)));
       }
       meet();
-#pragma unroll 1
-      for (int at0 = tid; at0 < n; at0 += AHEAD * threads) {
-        float v[AHEAD][PER], most = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          const uint32_t nothing = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
-          uint4 raw = make_uint4(nothing, nothing, nothing, nothing);
-          if (at0 + i * threads < n) raw = pieces[at0 + i * threads];
-          unpack(raw, v[i], static_cast<const T*>(nullptr));
-        }
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-          for (int e = 0; e < PER; ++e) most = fmaxf(most, v[i][e]);
-        if (most * c > reference) {
-          const float f = rebase(reference, most * c);
-          in_list *= f;
-          others *= f;
-          reference = most * c;
-        }
-        const float shift = no_less(reference);
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          float all = 0.f;
-#pragma unroll
-          for (int e = 0; e < PER; ++e) all += exp2_approx(fmaf(v[i][e], c, -shift));
-          others += all;
-        }
-      }
-      const float3 sums = warp_join(make_float3(reference, in_list, others));
-      if (lane < ranks)
-        send(cluster_address(&shares[turn & 1][rank * warps + warp], lane), cluster_address(&shared_in[turn & 1], lane),
-             make_float4(sums.x, sums.y, sums.z, 0.f));
-      if (!arrived(barrier, (turn >> 1) & 1) && lane == 0) atomicMax(a.error, R2_ERR_TIMEOUT_SHARES);
-      const float2 t = of_teacher[b];
-      const Student q(shares[turn & 1], ranks * warps, lane, tail, t.y);
-      ++turn;
-      if (tid == 0) students[b] = q;
-      const float scale = w * a.tau, by = scale * q.outside * q.inv_total;
-      if (!vectors) {
-#pragma unroll 1
-        for (int at = low + tid; at < high; at += threads) {
-          float v[PER];
-          unpack(pieces[at], v, static_cast<const T*>(nullptr));
-#pragma unroll
-          for (int e = 0; e < PER; ++e) grad[x.first(g0 + at) + e] = from_float<T>(exp2_approx(fmaf(v[e], c, -q.common)) * by);
-        }
+      int at = tid;
+      if (at < n) {
+        const uint4 first[1] = {pieces[at]};
+        sums.raise(Sums<T>::most(first) * c);
       }
 #pragma unroll 1
-      for (int at0 = vectors ? low + tid : high; at0 < high; at0 += AHEAD * threads) {
+      for (; at + (AHEAD - 1) * threads < n; at += AHEAD * threads) {
         uint4 raw[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-          if (at0 + i * threads < high) raw[i] = pieces[at0 + i * threads];
+        for (int i = 0; i < AHEAD; ++i) raw[i] = pieces[at + i * threads];
+        sums.add(raw, c);
+      }
+#pragma unroll 1
+      for (; at < n; at += threads) {
+        const uint4 raw[1] = {pieces[at]};
+        sums.add(raw, c);
+      }
+      const float3 joined = warp_join(make_float3(sums.reference, sums.in_list, sums.others));
+      if (lane < ranks)
+        send(cluster_address(&shares[b][rank * warps + warp], lane), cluster_address(&shared_in[b], lane), make_float4(joined.x, joined.y, joined.z, 0.f));
+      if (!arrived(barrier, phase) && lane == 0) atomicMax(a.error, R2_ERR_TIMEOUT_SHARES);
+      const float2 t = of_teacher[b];
+      const Student q(shares[b], ranks * warps, lane, tail, t.y);
+      if (tid == 0) students[b] = q;
+      const float scale = w * a.tau, by = scale * q.outside * q.inv_total;
+      if (vectors) {
+        const uint64_t cc = two_of(c, c), ss = two_of(-q.common, -q.common), bb = two_of(by, by);
+        auto gradient = [&](const uint4& raw) {
+          uint64_t p[PER / 2];
+          unpack_pairs(raw, p, static_cast<const T*>(nullptr));
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          float v[PER];
-          unpack(raw[i], v, static_cast<const T*>(nullptr));
+          for (int i = 0; i < PER / 2; ++i) p[i] = mul_two(exp2_two(fma_two(p[i], cc, ss)), bb);
+          return pack_pairs(p, static_cast<const T*>(nullptr));
+        };
+        at = low + tid;
+#pragma unroll 1
+        for (; at + (AHEAD - 1) * threads < high; at += AHEAD * threads) {
+          uint4 raw[AHEAD];
 #pragma unroll
-          for (int e = 0; e < PER; ++e) v[e] = exp2_approx(fmaf(v[e], c, -q.common)) * by;
-          if (at0 + i * threads < high) out[at0 + i * threads] = pack(v, static_cast<const T*>(nullptr));
+          for (int i = 0; i < AHEAD; ++i) raw[i] = pieces[at + i * threads];
+#pragma unroll
+          for (int i = 0; i < AHEAD; ++i) out[at + i * threads] = gradient(raw[i]);
         }
+#pragma unroll 1
+        for (; at < high; at += threads) out[at] = gradient(pieces[at]);
+      } else {
+#pragma unroll 1
+        for (at = low * PER + tid; at < high * PER; at += threads) grad[zero + at] = from_float<T>(exp2_approx(fmaf(to_float(tokens[at]), c, -q.common)) * by);
       }
       if (end >= 0) grad[zero + end] = from_float<T>(exp2_approx(fmaf(to_float(tokens[end]), c, -q.common)) * by);
       meet();   // the listed tokens' gradients lie over what stands there
@@ -393,6 +446,7 @@ distill_held_kernel(const DistillArgs a) {
         const int at = ids[b][j] - zero;
         if (ids[b][j] >= 0 && at >= 0 && at < n * PER) write_listed(grad, ids[b], teacher[b], taken, k, j, twice[b] != 0, c, t.x, scale, q);
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (the next copy into these places comes by another path)
     }
     w = w_next;
     w_next = w_after;

@@ -133,3 +133,58 @@ static inline void r2_launch_clusters(void (*kernel)(KArgs...), int cluster, dim
   config.numAttrs = (g_r2_pdl && !t_r2_plain_order) ? 2 : 1;
   cudaLaunchKernelEx(&config, kernel, static_cast<Args&&>(args)...);  // a failure shows in launch_status()
 }
+
+// Two floats side by side: one instruction for both, each rounded as the single one rounds.
+__device__ __forceinline__ uint64_t two_of(float lo, float hi) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ float2 halves(uint64_t p) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_two(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t exp2_two(uint64_t p) {
+  const float2 v = halves(p);
+  return two_of(exp2_approx(v.x), exp2_approx(v.y));
+}
+// A piece as pairs.
+__device__ __forceinline__ void unpack_pairs(const uint4& raw, uint64_t (&p)[2], const float*) {
+  p[0] = two_of(__uint_as_float(raw.x), __uint_as_float(raw.y));
+  p[1] = two_of(__uint_as_float(raw.z), __uint_as_float(raw.w));
+}
+__device__ __forceinline__ void unpack_pairs(const uint4& raw, uint64_t (&p)[4], const bf16*) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = two_of(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ uint4 pack_pairs(const uint64_t (&p)[2], const float*) {
+  const float2 a = halves(p[0]), b = halves(p[1]);
+  return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+}
+__device__ __forceinline__ uint4 pack_pairs(const uint64_t (&p)[4], const bf16*) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = halves(p[i]);
+    const __nv_bfloat162 two = __floats2bfloat162_rn(v.x, v.y);
+    w[i] = *reinterpret_cast<const uint32_t*>(&two);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
