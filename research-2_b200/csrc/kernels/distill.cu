@@ -23,7 +23,7 @@ namespace {
 
 constexpr int MOST_K = 256;
 constexpr int MOST_RANKS = 8;
-constexpr int MOST_WARPS = 8;      // of a block, that work on pieces
+constexpr int MOST_WARPS = 12;     // of a block, that work on pieces
 #define R2_ERR_TIMEOUT_SHARES 8
 
 struct DistillArgs {
@@ -35,10 +35,6 @@ struct DistillArgs {
   void* grad; long long grad_ld;
   int* error;
 };
-
-__device__ __forceinline__ float no_less(float reference) { return reference == -INFINITY ? 0.f : reference; }
-// what sums against `reference` are in sums against `common`, the largest of several references
-__device__ __forceinline__ float rebase(float reference, float common) { return reference == -INFINITY ? 0.f : exp2_approx(reference - common); }
 
 // One (reference, sum over listed, sum over others) per lane into one per warp.
 __device__ __forceinline__ float3 warp_join(float3 v) {
@@ -141,21 +137,17 @@ __device__ __forceinline__ bool mark_listed(uint32_t* listed, const int32_t* ids
   return again;
 }
 
-// One piece's exponentials (in v) into the sums over listed tokens and over the others.
-template <bool TAIL, int PER>
-__device__ __forceinline__ void add_piece(const float (&v)[PER], uint32_t bits, float& in_list, float& others) {
-  if (!TAIL || bits == 0u) {
-    float all = 0.f;
+// Elements of a piece to -inf.
+template <typename T>
+__device__ __forceinline__ void blank_bits(uint4& raw, uint32_t bits) {
+  uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int e = 0; e < PER; ++e) all += v[e];
-    others += all;
-    return;
+  for (int i = 0; i < RowPieces<T>::PER; ++i) {
+    if (!((bits >> i) & 1u)) continue;
+    if (sizeof(T) == 4) w[i & 3] = 0xff800000u;
+    else w[(i >> 1) & 3] = (i & 1) ? (w[(i >> 1) & 3] & 0x0000ffffu) | 0xff800000u : (w[(i >> 1) & 3] & 0xffff0000u) | 0x0000ff80u;
   }
-#pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    if ((bits >> e) & 1u) in_list += v[e];
-    else others += v[e];
-  }
+  raw = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Takes an element of the staged row out of it: what stood there; -inf stays.
@@ -246,16 +238,16 @@ struct Sums {
   }
 };
 
-// A block is eight warps (fewer for short rows) that work on pieces and one more that brings: it has the next row's share copied, brings
+// A block is twelve warps (fewer for short rows) that work on pieces and one more that brings: it has the next row's share copied, brings
 // its list and takes its mass, and finishes the loss of the row before, all beside the others, which meet it once a row. Rows that weigh
 // nothing are not brought; `slot` counts the others, two at a time.
 template <typename T>
 __global__ void __launch_bounds__(32 * (MOST_WARPS + 1), 2)
 distill_held_kernel(const DistillArgs a) {
   constexpr int PER = RowPieces<T>::PER, AHEAD = 16 / PER;   // pieces that a thread takes at a time
-  extern __shared__ __align__(16) uint4 staged[];            // [2][per]
+  extern __shared__ __align__(16) uint4 pieces[];            // of this CTA's share
   __shared__ __align__(16) float4 shares[2][MOST_RANKS * MOST_WARPS];
-  __shared__ __align__(8) uint64_t landed[2], shared_in[2];  // barriers: a row's share is there; every warp of the cluster has sent its sums
+  __shared__ __align__(8) uint64_t landed, shared_in[2];     // barriers: a row's share is there; every warp of the cluster has sent its sums
   __shared__ int32_t ids[2][MOST_K];
   __shared__ float teacher[2][MOST_K], xk[2][MOST_K], taken[MOST_K];
   __shared__ float2 of_teacher[2];   // what the teacher's exponentials are taken against, and their sum
@@ -273,10 +265,8 @@ distill_held_kernel(const DistillArgs a) {
 
   if (warp == warps) {
     if (lane == 0) {
-      for (int i = 0; i < 2; ++i) {
-        r2ptx::mbar_init(r2ptx::smem_u32(&landed[i]), 1u);
-        r2ptx::mbar_init(r2ptx::smem_u32(&shared_in[i]), 1u);
-      }
+      r2ptx::mbar_init(r2ptx::smem_u32(&landed), 1u);
+      for (int i = 0; i < 2; ++i) r2ptx::mbar_init(r2ptx::smem_u32(&shared_in[i]), 1u);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
@@ -284,16 +274,6 @@ distill_held_kernel(const DistillArgs a) {
     pdl_wait();
     const float inv = 1.f / a.tau;
     auto bring = [&](int r, int b) {
-      if (lane == 0) {
-        const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)r * a.ld, a.vocab);
-        const uint32_t bytes = uint32_t(min(a.per, x.count - g0)) * 16u, barrier = r2ptx::smem_u32(&landed[b]);
-        r2ptx::mbar_expect_tx(barrier, bytes);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                         r2ptx::smem_u32(staged + b * a.per)),
-                     "l"(reinterpret_cast<const uint4*>(x.base) + g0), "r"(bytes), "r"(barrier)
-                     : "memory");
-      }
       const float log_sum = tail ? a.log_sum[r] : 0.f;
 #pragma unroll 4
       for (int j = lane; j < k; j += 32) {
@@ -343,8 +323,17 @@ distill_held_kernel(const DistillArgs a) {
   cluster_arrive();
   pdl_wait();
   auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); };
+  auto copy = [&](int r) {   // one thread's: a row's share into its place
+    const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)r * a.ld, a.vocab);
+    const uint32_t bytes = uint32_t(min(a.per, x.count - g0)) * 16u, barrier = r2ptx::smem_u32(&landed);
+    r2ptx::mbar_expect_tx(barrier, bytes);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(r2ptx::smem_u32(pieces)),
+                 "l"(reinterpret_cast<const uint4*>(x.base) + g0), "r"(bytes), "r"(barrier)
+                 : "memory");
+  };
   float w = weight(row), w_next = weight(row + step);
   cluster_wait();
+  if (tid == 0 && w != 0.f) copy(row);
   for (; row < a.rows; row += step) {
     const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)row * a.ld, a.vocab);
     const int n = max(0, min(a.per, x.count - g0)), last = x.count - 1 - g0, zero = x.first(g0);
@@ -355,7 +344,6 @@ distill_held_kernel(const DistillArgs a) {
     // pieces from `low` up to `high` lie in the row as a whole; the ends of the row may not
     const int low = g0 == 0 && x.phase > 0 ? 1 : 0, high = last >= 0 && last < n && !x.whole(g0 + last) ? min(n, last) : n;
     const int b = slot & 1;
-    uint4* pieces = staged + b * a.per;
     T* tokens = reinterpret_cast<T*>(pieces);
     __syncthreads();   // the row's list is there; the row before has done with its own
     // this lane's token at the row's ends (the first warp's: in a first piece, in a last piece)
@@ -366,13 +354,14 @@ distill_held_kernel(const DistillArgs a) {
     }
     if (w == 0.f) {
       const float zeros[PER] = {};
+      if (tid == 0 && w_next != 0.f) copy(row + step);
 #pragma unroll 1
       for (int at = low + tid; at < high; at += threads) store_piece<T, PER>(grad, x.first(g0 + at), a.vocab, zeros, vectors);
       if (end >= 0 && zero + end >= 0 && zero + end < a.vocab) grad[zero + end] = from_float<T>(0.f);
     } else {
       const uint32_t barrier = r2ptx::smem_u32(&shared_in[b]), phase = (slot >> 1) & 1;
       ++slot;
-      if (!r2ptx::mbar_wait(r2ptx::smem_u32(&landed[b]), phase) && lane == 0) atomicMax(a.error, R2_ERR_TIMEOUT_SHARES);
+      if (!r2ptx::mbar_wait(r2ptx::smem_u32(&landed), (slot - 1) & 1) && lane == 0) atomicMax(a.error, R2_ERR_TIMEOUT_SHARES);
       if (end >= 0 && (zero + end < 0 || zero + end >= a.vocab)) {
         tokens[end] = from_float<T>(-INFINITY);
         end = -1;
@@ -440,13 +429,14 @@ distill_held_kernel(const DistillArgs a) {
         for (at = low * PER + tid; at < high * PER; at += threads) grad[zero + at] = from_float<T>(exp2_approx(fmaf(to_float(tokens[at]), c, -q.common)) * by);
       }
       if (end >= 0) grad[zero + end] = from_float<T>(exp2_approx(fmaf(to_float(tokens[end]), c, -q.common)) * by);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (the next copy comes by another path than what was written here)
       meet();   // the listed tokens' gradients lie over what stands there
+      if (tid == 0 && w_next != 0.f) copy(row + step);
 #pragma unroll 1
       for (int j = tid; j < k; j += threads) {
         const int at = ids[b][j] - zero;
         if (ids[b][j] >= 0 && at >= 0 && at < n * PER) write_listed(grad, ids[b], teacher[b], taken, k, j, twice[b] != 0, c, t.x, scale, q);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (the next copy into these places comes by another path)
     }
     w = w_next;
     w_next = w_after;
@@ -456,9 +446,9 @@ distill_held_kernel(const DistillArgs a) {
 
 // Losses alone (one pass over the row), and gradients of rows that no cluster holds (two).
 template <typename T, bool TAIL>
-__global__ void __launch_bounds__(512, 2)
+__global__ void __launch_bounds__(256, 4)
 distill_streamed_kernel(const DistillArgs a) {
-  constexpr int THREADS = 512, PER = RowPieces<T>::PER, DEPTH = 4;
+  constexpr int THREADS = 256, PER = RowPieces<T>::PER, DEPTH = 4;
   extern __shared__ __align__(16) uint32_t bits_s[];   // a bit for each token of this CTA's share
   __shared__ __align__(16) float4 shares[MOST_RANKS * (THREADS / 32)];
   __shared__ int32_t ids[MOST_K];
@@ -496,42 +486,61 @@ distill_streamed_kernel(const DistillArgs a) {
   if (TAIL || grad != nullptr)
     if (mark_listed(bits_s, ids, k, x.first(g0), n * PER, tid, THREADS)) twice = 1;
   __syncthreads();
-  float reference = -INFINITY, in_list = 0.f, others = 0.f;
-  for (int c0 = tid; c0 < n; c0 += DEPTH * THREADS) {
-    uint4 raw[DEPTH];
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i)
-      if (c0 + i * THREADS < n) raw[i] = load_once(x, g0 + c0 + i * THREADS);
-    float most = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) {
-      if (c0 + i * THREADS >= n) continue;
-      blank_outside(raw[i], x, g0 + c0 + i * THREADS);
-      float v[PER];
-      unpack(raw[i], v, static_cast<const T*>(nullptr));
-#pragma unroll
-      for (int e = 0; e < PER; ++e) most = fmaxf(most, v[e]);
-    }
-    if (most * c > reference) {
-      const float f = rebase(reference, most * c);
-      in_list *= f;
-      others *= f;
-      reference = most * c;
-    }
-    const float shift = no_less(reference);
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) {
-      const int at = c0 + i * THREADS;
-      if (at >= n) continue;
-      float v[PER];
-      unpack(raw[i], v, static_cast<const T*>(nullptr));
-#pragma unroll
-      for (int e = 0; e < PER; ++e) v[e] = exp2_approx(fmaf(v[e], c, -shift));
-      uint32_t bits = 0u;
-      if (TAIL) bits = (bits_s[at * PER / 32] >> (at * PER % 32)) & ((1u << PER) - 1u);
-      add_piece<TAIL>(v, bits, in_list, others);
+  Sums<T> own;
+  if (TAIL) {
+    for (int j = tid; j < k; j += THREADS) {
+      const int at = ids[j] - x.first(g0);
+      if (ids[j] < 0 || at < 0 || at >= n * PER) continue;
+      // (of a token that the list names more than once, one entry counts)
+      bool first = true;
+      if (twice)
+        for (int o = 0; o < j; ++o) first &= ids[o] != ids[j];
+      if (!first) continue;
+      own.raise(xk[j] * c);
+      own.in_list += exp2_approx(fmaf(xk[j], c, -no_less(own.reference)));
     }
   }
+  // listed tokens and places that are not the row's are -inf in what is summed
+  auto clear = [&](uint4& raw, int at) {
+    if (TAIL) {
+      const uint32_t bits = (bits_s[at * PER / 32] >> (at * PER % 32)) & ((1u << PER) - 1u);
+      if (bits != 0u) blank_bits<T>(raw, bits);
+    }
+    if (g0 + at == 0 || g0 + at == x.count - 1) blank_outside(raw, x, g0 + at);
+  };
+  uint4 raw[DEPTH];
+  auto load = [&](int at) {
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) raw[i] = load_once(x, g0 + at + i * THREADS);
+  };
+  int at = tid;
+  if (at + (DEPTH - 1) * THREADS < n) {
+    load(at);
+    uint4 first[DEPTH];
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      first[i] = raw[i];
+      clear(first[i], at + i * THREADS);
+    }
+    own.raise(Sums<T>::most(first) * c);
+  }
+#pragma unroll 1
+  for (; at + (DEPTH - 1) * THREADS < n; at += DEPTH * THREADS) {
+    uint4 now[DEPTH];
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) now[i] = raw[i];
+    if (at + (2 * DEPTH - 1) * THREADS < n) load(at + DEPTH * THREADS);
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) clear(now[i], at + i * THREADS);
+    own.add(now, c);
+  }
+#pragma unroll 1
+  for (; at < n; at += THREADS) {
+    uint4 one[1] = {load_once(x, g0 + at)};
+    clear(one[0], at);
+    own.add(one, c);
+  }
+  const float reference = own.reference, in_list = own.in_list, others = own.others;
   const float3 sums = warp_join(make_float3(reference, in_list, others));
   if (ranks > 1) {
     cluster_wait();
@@ -575,14 +584,14 @@ distill_streamed_kernel(const DistillArgs a) {
 
 constexpr int MOST_STREAMED_BITS = 1 << 20;   // tokens of a CTA's share (128 KB of bits)
 
-constexpr int HELD_TWO = 3300, HELD_ONE = 6800;   // pieces of a CTA's share where two CTAs, or one, fit an SM (two rows' shares in shared memory)
+constexpr int HELD_TWO = 6600, HELD_ONE = 13600;   // pieces of a CTA's share where two CTAs, or one, fit an SM
 
 template <typename T>
 int launch_held(const DistillArgs& a, cudaStream_t stream) {
   const int warps = max(1, min(MOST_WARPS, a.per / 64));
-  const size_t smem = size_t(a.per) * 32;
+  const size_t smem = size_t(a.per) * 16;
   static std::atomic<bool> allowed[64];
-  const int status = allow_smem(distill_held_kernel<T>, size_t(HELD_ONE) * 32, allowed);
+  const int status = allow_smem(distill_held_kernel<T>, size_t(HELD_ONE) * 16, allowed);
   if (status != R2_OK) return status;
   // how many clusters run at a time, asked once for each device and shape (a table that forgets)
   struct Resident {
@@ -623,7 +632,7 @@ template <typename T, bool TAIL>
 int launch_streamed(DistillArgs a, int pieces, cudaStream_t stream) {
   // a row to a CTA where there are CTAs enough for the SMs, else cut over several
   a.ranks = 1;
-  while (a.ranks < MOST_RANKS && ((long long)a.rows * a.ranks < 296 || (pieces / a.ranks + 1) * RowPieces<T>::PER > MOST_STREAMED_BITS)
+  while (a.ranks < MOST_RANKS && ((long long)a.rows * a.ranks < 592 || (pieces / a.ranks + 1) * RowPieces<T>::PER > MOST_STREAMED_BITS)
          && pieces / a.ranks > 1024) a.ranks *= 2;
   const int per = a.per = (pieces + a.ranks - 1) / a.ranks;
   if (per * RowPieces<T>::PER > MOST_STREAMED_BITS) return R2_UNSUPPORTED;
@@ -631,7 +640,7 @@ int launch_streamed(DistillArgs a, int pieces, cudaStream_t stream) {
   static std::atomic<bool> allowed[64];
   const int status = allow_smem(distill_streamed_kernel<T, TAIL>, MOST_STREAMED_BITS / 8, allowed);
   if (status != R2_OK) return status;
-  r2_launch_clusters(distill_streamed_kernel<T, TAIL>, a.ranks, dim3(unsigned(a.rows) * unsigned(a.ranks)), dim3(512),
+  r2_launch_clusters(distill_streamed_kernel<T, TAIL>, a.ranks, dim3(unsigned(a.rows) * unsigned(a.ranks)), dim3(256),
                      size_t(per * RowPieces<T>::PER + 31) / 32 * 4, stream, a);
   return launch_status();
 }

@@ -102,6 +102,11 @@ __device__ __forceinline__ float exp2_approx(float x) {  // 2^x within 2^-22; 0 
   return y;
 }
 
+// Sums of exponentials are kept against a reference, an exponent of two; -inf where nothing has been summed.
+__device__ __forceinline__ float no_less(float reference) { return reference == -INFINITY ? 0.f : reference; }
+// what sums against `reference` are in sums against `common`, the largest of several references
+__device__ __forceinline__ float rebase(float reference, float common) { return reference == -INFINITY ? 0.f : exp2_approx(reference - common); }
+
 // The CTAs of a cluster along x share a row.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }

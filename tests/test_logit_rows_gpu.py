@@ -513,3 +513,25 @@ def test_distill_many_rows_some_of_no_weight(vocab, dtype):
     want = weight.double()[:, None] * (q - target - torch.where(listed, 0.0, rest_p * q / rest))
     off = (gradient.double() - want).abs()
     assert torch.all(off <= 1e-5 * (q + p.amax(1, keepdim=True) * listed) + 4e-6 * q / rest + (2.0**-8 * want.abs() if dtype == BF16 else 0))
+
+
+@pytest.mark.parametrize("around", [math.inf, -math.inf, math.nan, 1e30, -1e30])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [37, 3003, 9001, 50257, 131079])
+def test_logit_rows_do_not_depend_on_what_lies_around_them(around, dtype, vocab):
+    values = random_logits(3, vocab, vocab).to(dtype)
+    buf = torch.full((3, vocab + 37), around, dtype=dtype, device=DEV)
+    x = buf[:, 5: 5 + vocab]
+    x.copy_(values)
+    alone = values.to(DEV)
+    a, b = ops().top_logits(x, 20, temperature=2.0), ops().top_logits(alone, 20, temperature=2.0)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.allclose(a[2], b[2], rtol=0, atol=1e-5)
+    for log_sum in (None, b[2] + 0.25):
+        for gradient in (True, False):
+            loss, g = ops().distill_loss(x, b[1], b[0] * 0.5, log_sum=log_sum, temperature=2.0, gradient=gradient)
+            want, w = ops().distill_loss(alone, b[1], b[0] * 0.5, log_sum=log_sum, temperature=2.0, gradient=gradient)
+            assert torch.allclose(loss, want, rtol=1e-4, atol=1e-5)
+            if gradient:
+                assert torch.allclose(g.float(), w.float(), rtol=1e-4 if dtype == F32 else 2.0**-7, atol=1e-7)
+    arguments = dict(history=i32([[1, 2, 3]] * 3), lengths=i32([3, 2, 1]), presence=f32([1.0] * 3))
+    assert torch.equal(ops().adjust_logits(x, **arguments), ops().adjust_logits(alone, **arguments))
