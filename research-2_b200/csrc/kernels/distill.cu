@@ -137,19 +137,6 @@ __device__ __forceinline__ bool mark_listed(uint32_t* listed, const int32_t* ids
   return again;
 }
 
-// Elements of a piece to -inf.
-template <typename T>
-__device__ __forceinline__ void blank_bits(uint4& raw, uint32_t bits) {
-  uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-  for (int i = 0; i < RowPieces<T>::PER; ++i) {
-    if (!((bits >> i) & 1u)) continue;
-    if (sizeof(T) == 4) w[i & 3] = 0xff800000u;
-    else w[(i >> 1) & 3] = (i & 1) ? (w[(i >> 1) & 3] & 0x0000ffffu) | 0xff800000u : (w[(i >> 1) & 3] & 0xffff0000u) | 0x0000ff80u;
-  }
-  raw = make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // Takes an element of the staged row out of it: what stood there; -inf stays.
 __device__ __forceinline__ float take_out(float* at) { return __uint_as_float(atomicExch(reinterpret_cast<unsigned int*>(at), 0xff800000u)); }
 __device__ __forceinline__ float take_out(bf16* at) {
@@ -504,7 +491,7 @@ distill_streamed_kernel(const DistillArgs a) {
   auto clear = [&](uint4& raw, int at) {
     if (TAIL) {
       const uint32_t bits = (bits_s[at * PER / 32] >> (at * PER % 32)) & ((1u << PER) - 1u);
-      if (bits != 0u) blank_bits<T>(raw, bits);
+      if (bits != 0u) keep_bits<T>(raw, ~bits);
     }
     if (g0 + at == 0 || g0 + at == x.count - 1) blank_outside(raw, x, g0 + at);
   };

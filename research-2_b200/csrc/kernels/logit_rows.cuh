@@ -82,18 +82,52 @@ __device__ __forceinline__ uint4 load_once(const RowPieces<T>& row, int g) {
                : "l"(reinterpret_cast<const uint4*>(row.base) + g));
   return v;
 }
+// Elements of a piece to -inf where their bits are 0. A bit becomes a byte's highest (the product puts bit i at 8 i + 7 and nothing else
+// there), and a byte's highest bit becomes whole bytes (prmt's sign mode).
+__device__ __forceinline__ uint32_t spread(uint32_t four_bits) { return (four_bits * 0x10204080u) & 0x80808080u; }
+__device__ __forceinline__ uint32_t signs(uint32_t bytes, uint32_t selector) {
+  uint32_t d;
+  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(d) : "r"(bytes), "r"(selector));
+  return d;
+}
+template <typename T>
+__device__ __forceinline__ void keep_bits(uint4& raw, uint32_t bits) {
+  uint32_t m[4];
+  const uint32_t low = spread(bits & 15u);
+  if (sizeof(T) == 4) {
+    m[0] = signs(low, 0x8888u);
+    m[1] = signs(low, 0x9999u);
+    m[2] = signs(low, 0xaaaau);
+    m[3] = signs(low, 0xbbbbu);
+  } else {
+    const uint32_t high = spread((bits >> 4) & 15u);
+    m[0] = signs(low, 0x9988u);
+    m[1] = signs(low, 0xbbaau);
+    m[2] = signs(high, 0x9988u);
+    m[3] = signs(high, 0xbbaau);
+  }
+  constexpr uint32_t NOTHING = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+  raw = make_uint4((raw.x & m[0]) | (NOTHING & ~m[0]), (raw.y & m[1]) | (NOTHING & ~m[1]), (raw.z & m[2]) | (NOTHING & ~m[2]),
+                   (raw.w & m[3]) | (NOTHING & ~m[3]));
+}
 template <typename T>
 __device__ __forceinline__ void blank_outside(uint4& raw, const RowPieces<T>& row, int g) {
   if (row.whole(g)) return;
   const int first = row.first(g);
-  uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t bits = first < 0 ? (1u << -first) - 1u : 0u;
+  if (first + RowPieces<T>::PER > row.vocab) bits |= ~0u << (row.vocab - first);
+  keep_bits<T>(raw, ~bits);
+}
+// A piece's elements that belong to the row, one by one.
+template <typename T>
+__device__ __noinline__ void store_elements(T* row, int first, int vocab, uint4 raw) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
   for (int i = 0; i < RowPieces<T>::PER; ++i) {
-    if (first + i >= 0 && first + i < row.vocab) continue;
-    if (sizeof(T) == 4) w[i & 3] = 0xff800000u;
-    else w[(i >> 1) & 3] = (i & 1) ? (w[(i >> 1) & 3] & 0x0000ffffu) | 0xff800000u : (w[(i >> 1) & 3] & 0xffff0000u) | 0x0000ff80u;
+    if (first + i < 0 || first + i >= vocab) continue;
+    if (sizeof(T) == 4) reinterpret_cast<uint32_t*>(row)[first + i] = w[i & 3];
+    else reinterpret_cast<uint16_t*>(row)[first + i] = uint16_t(w[(i >> 1) & 3] >> (i % 2 * 16));
   }
-  raw = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {  // 2^x within 2^-22; 0 below the normal range

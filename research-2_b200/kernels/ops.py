@@ -1913,51 +1913,89 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
 TOP_MOST = 256   # the most logits of a row that top_logits returns and distill_loss takes
 
 
-def _logit_rows(logits: torch.Tensor, what: str) -> tuple[int, int, int, int]:
-    """(type's code, rows, vocabulary, row stride) of a tensor of logits."""
-    _need(logits, "logits", dim=2)
-    if logits.dtype not in (torch.float32, torch.bfloat16):
-        raise KernelError(f"{what}: logits must be float32 or bfloat16, got {logits.dtype}")
-    if logits.shape[1] < 1:
+_LOGIT_SIGNATURES = {
+    "adjust_logits": [C.c_int, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int] +
+                     [C.c_void_p] * 9 + [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p, C.c_void_p],
+    "top_logits": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
+    "distill": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
+                C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p],
+}
+_logit_entries: dict = {}
+
+
+def _logit_entry(name: str):
+    """The C entry of one of these operators with its argument types set: addresses and numbers go in as plain integers. (A step calls
+    them between two kernels of a few microseconds; an object per argument took as long as the kernels.)"""
+    entry = _logit_entries.get(name)
+    lib = _libs.get(name)
+    if entry is None or entry[0] is not lib:
+        lib = _lib(name)
+        fn = getattr(lib, "r2_" + name)
+        fn.argtypes = _LOGIT_SIGNATURES[name]
+        entry = _logit_entries[name] = (lib, fn)
+    return entry[1]
+
+
+def _current_stream(device: int) -> int:
+    """The stream that a launch on tensors of `device` goes to; the device has to be the current one, as for every kernel here."""
+    if device != torch._C._cuda_getDevice():
+        raise KernelError(f"the tensors are on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _logit_rows(logits: torch.Tensor, what: str) -> tuple[int, int, int, int, int]:
+    """(type's code, rows, vocabulary, row stride, device) of a tensor of logits."""
+    if logits.dim() != 2:
+        raise KernelError(f"{what}: logits must have 2 dimensions, got shape {tuple(logits.shape)}")
+    dtype, device = logits.dtype, logits.get_device()
+    if device < 0:
+        raise KernelError(f"{what}: logits must be a CUDA tensor (there is no CPU path)")
+    if dtype is not torch.float32 and dtype is not torch.bfloat16:
+        raise KernelError(f"{what}: logits must be float32 or bfloat16, got {dtype}")
+    rows, vocab = logits.shape
+    if vocab < 1:
         raise KernelError(f"{what}: logits of no tokens")
-    return dtype_code(logits.dtype), logits.shape[0], logits.shape[1], _rows(logits, "logits")
+    ld, inner = logits.stride()
+    if vocab > 1 and inner != 1:
+        raise KernelError(f"{what}: logits must have contiguous rows, got shape {tuple(logits.shape)} stride {logits.stride()}")
+    if rows <= 1:
+        ld = max(ld, vocab)
+    return (F32 if dtype is torch.float32 else BF16), rows, vocab, ld, device
 
 
-def _per_row(t: torch.Tensor | None, name: str, dtype, rows: int, logits: torch.Tensor) -> None:
+def _per_row(t: torch.Tensor | None, name: str, dtype, rows: int, device: int) -> int:
+    """The address of a number per row, checked; 0 for none."""
     if t is None:
-        return
-    _need(t, name, dtype, 1)
-    if t.device != logits.device:
-        raise KernelError(f"{name} must be on the logits' device")
-    if t.shape[0] < rows or not t.is_contiguous():
-        raise KernelError(f"{name} must be contiguous with a number for each of {rows} rows, got shape {tuple(t.shape)} stride {t.stride()}")
+        return 0
+    if t.dtype is not dtype or t.get_device() != device or t.dim() != 1 or t.shape[0] < rows or (rows > 1 and t.stride(0) != 1):
+        raise KernelError(f"{name} must be {dtype} on the logits' device, contiguous, with a number for each of {rows} rows; got {t.dtype} on "
+                          f"{t.device}, shape {tuple(t.shape)} stride {t.stride()}")
+    return t.data_ptr()
 
 
-def _like_logits(logits: torch.Tensor, out: torch.Tensor | None, what: str) -> torch.Tensor:
-    """The output beside rows of logits: `out`, checked, or new rows that are as far apart as the logits' (so that a row starts at the
-    same alignment in both and is written in 16-byte pieces) where that wastes little."""
+def _like_logits(logits: torch.Tensor, ld: int, out: torch.Tensor | None, what: str) -> tuple[torch.Tensor, int]:
+    """The output beside rows of logits and its row stride: `out`, checked, or new rows that are as far apart as the logits' and start at
+    the same place of 16 bytes (so that a row is written in the pieces in which it is read) where that wastes little."""
     rows, vocab = logits.shape
     if out is None:
-        ld = _rows(logits, "logits")
-        ld = ld if vocab <= ld <= vocab + max(64, vocab // 16) else vocab
+        if ld > vocab + max(64, vocab // 16):
+            ld = vocab
         skip = logits.data_ptr() % 16 // logits.element_size()
         if skip == 0:
-            return torch.empty_strided((rows, vocab), (ld, 1), dtype=logits.dtype, device=logits.device)
-        return torch.empty(max(0, rows - 1) * ld + vocab + skip, dtype=logits.dtype, device=logits.device).as_strided((rows, vocab), (ld, 1), skip)
+            return torch.empty_strided((rows, vocab), (ld, 1), dtype=logits.dtype, device=logits.device), ld
+        return torch.empty(max(0, rows - 1) * ld + vocab + skip, dtype=logits.dtype, device=logits.device).as_strided((rows, vocab), (ld, 1), skip), ld
     _need(out, "out", logits.dtype, 2)
     if out.shape != logits.shape or out.device != logits.device:
         raise KernelError(f"{what}: out must have the logits' shape and device, got {tuple(out.shape)} on {out.device}")
-    ld = _rows(out, "out")
-    if rows > 1 and ld < vocab:
+    to = _rows(out, "out")
+    if rows > 1 and to < vocab:
         raise KernelError(f"{what}: rows of out overlap")
-    same = out.data_ptr() == logits.data_ptr() and (rows <= 1 or ld == _rows(logits, "logits"))
-    if not same and rows:
-        def span(t):
-            return t.data_ptr(), t.data_ptr() + ((rows - 1) * _rows(t, "rows") + vocab) * t.element_size()
-        (a, b), (c, d) = span(out), span(logits)
-        if a < d and c < b:
+    if rows and not (out.data_ptr() == logits.data_ptr() and (rows == 1 or to == ld)):
+        size = logits.element_size()
+        a, c = out.data_ptr(), logits.data_ptr()
+        if a < c + ((rows - 1) * ld + vocab) * size and c < a + ((rows - 1) * to + vocab) * size:
             raise KernelError(f"{what}: out overlaps the logits without being the same rows")
-    return out
+    return out, to
 
 
 def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, slots: torch.Tensor | None = None,
@@ -1976,46 +2014,47 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     and are added to their tokens, in order where a token is named more than once; tokens outside the vocabulary are left out.
     `mask` int32 [M, >= V / 32]: where bit t % 32 of word t / 32 of row mask_rows[r] is 0 the logit becomes -inf (`mask_rows` None: row r;
     a number outside [0, M): no mask). A mask that leaves nothing leaves a row of -inf, which `sample` answers with token 0."""
-    code, rows, vocab, ld = _logit_rows(logits, "adjust_logits")
-    history_rows = cap = history_ld = n_masks = mask_ld = n_biases = 0
+    code, rows, vocab, ld, device = _logit_rows(logits, "adjust_logits")
+    history_rows = cap = history_ld = history_at = n_masks = mask_ld = mask_at = n_biases = bias_at = 0
     if history is not None:
-        _need(history, "history", torch.int32, 2)
+        if history.dtype is not torch.int32 or history.dim() != 2 or history.get_device() != device:
+            raise KernelError(f"history must be int32 [requests, tokens] on the logits' device, got {history.dtype} {tuple(history.shape)} on {history.device}")
         history_ld, (history_rows, cap) = _rows(history, "history"), history.shape
         if lengths is None:
             raise KernelError("adjust_logits: a history needs lengths")
         if slots is None and history_rows < rows:
             raise KernelError(f"adjust_logits: {rows} rows, a history of {history_rows} and no slots")
-    elif any(t is not None for t in (repetition, presence, frequency)):
+        if history_rows > 0:
+            history_at = history.data_ptr()
+    elif repetition is not None or presence is not None or frequency is not None:
         raise KernelError("adjust_logits: penalties need a history")
-    for name, t, dtype in (("slots", slots, torch.int32), ("lengths", lengths, torch.int32), ("prompt_lengths", prompt_lengths, torch.int32),
-                           ("repetition", repetition, torch.float32), ("presence", presence, torch.float32),
-                           ("frequency", frequency, torch.float32), ("mask_rows", mask_rows, torch.int32)):
-        _per_row(t, name, dtype, rows, logits)
     if bias_start is not None:
-        _per_row(bias_start, "bias_start", torch.int32, rows + 1, logits)
         if bias_ids is None or bias_values is None:
             raise KernelError("adjust_logits: biases need bias_ids and bias_values")
         n_biases = bias_ids.shape[0] if bias_ids.dim() == 1 else -1
-        _per_row(bias_ids, "bias_ids", torch.int32, n_biases, logits)
-        _per_row(bias_values, "bias_values", torch.float32, n_biases, logits)
+        bias_at = _per_row(bias_start, "bias_start", torch.int32, rows + 1, device)
+    ids_at = _per_row(bias_ids, "bias_ids", torch.int32, n_biases, device)
+    values_at = _per_row(bias_values, "bias_values", torch.float32, n_biases, device)
     if mask is not None:
-        _need(mask, "mask", torch.int32, 2)
+        if mask.dtype is not torch.int32 or mask.dim() != 2 or mask.get_device() != device:
+            raise KernelError(f"mask must be int32 [masks, words] on the logits' device, got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
         n_masks, mask_ld = mask.shape[0], _rows(mask, "mask")
         if mask.shape[1] * 32 < vocab:
             raise KernelError(f"adjust_logits: masks of {mask.shape[1]} words are shorter than {vocab} tokens")
         if mask_rows is None and n_masks < rows:
             raise KernelError(f"adjust_logits: {rows} rows, {n_masks} masks and no mask_rows")
-    for name, t in (("history", history), ("mask", mask)):
-        if t is not None and t.device != logits.device:
-            raise KernelError(f"{name} must be on the logits' device")
-    out = _like_logits(logits, out, "adjust_logits")
+        if n_masks > 0:
+            mask_at = mask.data_ptr()
+    numbers = [_per_row(slots, "slots", torch.int32, rows, device), _per_row(lengths, "lengths", torch.int32, rows, device),
+               _per_row(prompt_lengths, "prompt_lengths", torch.int32, rows, device), _per_row(repetition, "repetition", torch.float32, rows, device),
+               _per_row(presence, "presence", torch.float32, rows, device), _per_row(frequency, "frequency", torch.float32, rows, device)]
+    which_at = _per_row(mask_rows, "mask_rows", torch.int32, rows, device)
+    out, out_ld = _like_logits(logits, ld, out, "adjust_logits")
     if rows == 0:
         return out
-    status = _lib("adjust_logits").r2_adjust_logits(
-        code, _p(logits), C.c_longlong(ld), _p(out), C.c_longlong(_rows(out, "out")), rows, vocab, _p(history if history_rows else None),
-        C.c_longlong(history_ld), history_rows, cap, _p(slots), _p(lengths), _p(prompt_lengths), _p(repetition), _p(presence), _p(frequency),
-        _p(bias_start if n_biases else None), _p(bias_ids), _p(bias_values), n_biases, _p(mask if n_masks else None), C.c_longlong(mask_ld),
-        n_masks, _p(mask_rows), _stream())
+    status = _logit_entry("adjust_logits")(code, logits.data_ptr(), ld, out.data_ptr(), out_ld, rows, vocab, history_at, history_ld, history_rows,
+                                           cap, *numbers, bias_at if n_biases else 0, ids_at, values_at, n_biases, mask_at, mask_ld, n_masks, which_at,
+                                           _current_stream(device))
     _check(status, "adjust_logits")
     return out
 
@@ -2030,16 +2069,17 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0):
     """The k largest logits of every row of [R, V] (float32 or bfloat16; k up to 256 and V): (values float32 [R, k] from the largest down,
     their tokens int32 [R, k], log_sum float32 [R]), equal values from the lowest token up and NaN below all others; log_sum is the
     logarithm of the row's sum of exp(x / temperature), so values / temperature - log_sum are log-probabilities."""
-    code, rows, vocab, ld = _logit_rows(logits, "top_logits")
+    code, rows, vocab, ld, device = _logit_rows(logits, "top_logits")
     if not 1 <= k <= min(vocab, TOP_MOST):
         raise KernelError(f"top_logits: k must be in [1, {min(vocab, TOP_MOST)}], got {k}")
     temperature = _temperature(temperature, "top_logits")
-    values = torch.empty(rows, k, dtype=torch.float32, device=logits.device)
-    ids = torch.empty(rows, k, dtype=torch.int32, device=logits.device)
-    log_sum = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    where = logits.device
+    values = torch.empty((rows, k), dtype=torch.float32, device=where)
+    ids = torch.empty((rows, k), dtype=torch.int32, device=where)
+    log_sum = torch.empty(rows, dtype=torch.float32, device=where)
     if rows:
-        _check(_lib("top_logits").r2_top_logits(code, _p(logits), C.c_longlong(ld), rows, vocab, k, C.c_float(temperature), _p(values), _p(ids),
-                                                _p(log_sum), _stream()), "top_logits")
+        _check(_logit_entry("top_logits")(code, logits.data_ptr(), ld, rows, vocab, k, temperature, values.data_ptr(), ids.data_ptr(),
+                                          log_sum.data_ptr(), _current_stream(device)), "top_logits")
     return values, ids, log_sum
 
 
@@ -2055,23 +2095,24 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
     left out). Without it p = softmax(teacher / temperature) over the listed tokens alone. `weight` float32 [R]: a row of weight 0 is not
     read; its loss and gradient are 0. A row without entries and without `log_sum` has the loss 0, one whose logits are all -inf, or hold
     +inf or NaN, a loss of NaN."""
-    code, rows, vocab, ld = _logit_rows(logits, "distill_loss")
-    _need(ids, "ids", torch.int32, 2)
-    _need(teacher, "teacher", torch.float32, 2)
+    code, rows, vocab, ld, device = _logit_rows(logits, "distill_loss")
+    if ids.dtype is not torch.int32 or teacher.dtype is not torch.float32 or ids.dim() != 2:
+        raise KernelError(f"distill_loss: ids must be int32 [rows, K] and teacher float32, got {ids.dtype} {tuple(ids.shape)} and {teacher.dtype}")
     k = ids.shape[1]
     if ids.shape[0] != rows or teacher.shape != ids.shape or not 1 <= k <= TOP_MOST:
         raise KernelError(f"distill_loss: ids and teacher must be [{rows}, 1 to {TOP_MOST}], got {tuple(ids.shape)} and {tuple(teacher.shape)}")
-    if not ids.is_contiguous() or not teacher.is_contiguous() or ids.device != logits.device or teacher.device != logits.device:
+    if not ids.is_contiguous() or not teacher.is_contiguous() or ids.get_device() != device or teacher.get_device() != device:
         raise KernelError("distill_loss: ids and teacher must be contiguous and on the logits' device")
-    _per_row(log_sum, "log_sum", torch.float32, rows, logits)
-    _per_row(weight, "weight", torch.float32, rows, logits)
+    log_sum_at = _per_row(log_sum, "log_sum", torch.float32, rows, device)
+    weight_at = _per_row(weight, "weight", torch.float32, rows, device)
     temperature = _temperature(temperature, "distill_loss")
     if out is not None and not gradient:
         raise KernelError("distill_loss: out is where the gradient goes, and none is asked for")
-    loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    grad = _like_logits(logits, out, "distill_loss") if gradient else None
+    where = logits.device
+    loss = torch.empty(rows, dtype=torch.float32, device=where)
+    grad, grad_ld = _like_logits(logits, ld, out, "distill_loss") if gradient else (None, 0)
     if rows:
-        _check(_lib("distill").r2_distill(code, _p(logits), C.c_longlong(ld), rows, vocab, _p(ids), _p(teacher), k, _p(log_sum), _p(weight),
-                                          C.c_float(temperature), _p(loss), _p(grad), C.c_longlong(_rows(grad, "out") if gradient else 0),
-                                          _p(_workspace(logits.device).error), _stream()), "distill_loss")
+        _check(_logit_entry("distill")(code, logits.data_ptr(), ld, rows, vocab, ids.data_ptr(), teacher.data_ptr(), k, log_sum_at, weight_at,
+                                       temperature, loss.data_ptr(), grad.data_ptr() if gradient else 0, grad_ld, _workspace(where).error.data_ptr(),
+                                       _current_stream(device)), "distill_loss")
     return loss, grad
