@@ -1,4 +1,4 @@
-"""Command line: generate tokens, write a random model folder, replay a trace.
+"""Command line: generate tokens, write a random model folder, replay a trace, write a teacher's top logits.
 
 Option names follow the reference's `kelpie serve` where it has them (`--model`, `--device`,
 `--max-requests`, `--num-slabs`, `--capture/--no-capture`: kelpie-http/kelpie_http/sdk/serve.py:
@@ -8,6 +8,7 @@ offline generation command; this one takes and prints token ids ("the core sees 
 only", kelpie/docs/core-api.md:18).
 
     python -m research_2_b200 generate --model DIR --prompt-tokens 5,17,3 --max-new-tokens 16
+    python -m research_2_b200 teach --model DIR --tokens 5,17,3 --top 64 --out lesson.npz
     python -m research_2_b200 random --config config.json --seed 0 --out DIR
     python -m research_2_b200 replay --model DIR --dtype float32 --out DIR --max-tokens 256 < steps.jsonl
 """
@@ -57,13 +58,46 @@ def cmd_generate(args) -> int:
         print("generate: give --prompt-tokens (repeatable) or --prompt-len", file=sys.stderr)
         return 2
     outs = generate(
-        args.model, prompts, args.max_new_tokens, temperature=args.temperature, top_k=args.top_k, seed=args.seed,
+        args.model, prompts, args.max_new_tokens, controls=_controls(args), temperature=args.temperature, top_k=args.top_k, seed=args.seed,
         stop_token_ids=_ints(args.stop_token_ids), device=args.device, dtype=args.dtype, capture=args.capture,
         max_requests=args.max_requests, num_slabs=args.num_slabs, block_size=args.block_size, max_seq_len=args.max_seq_len,
         max_batch_tokens=args.max_batch_tokens, max_batch_reqs=args.max_batch_reqs, chunk_size=args.chunk_size, reserve_ratio=args.reserve_ratio,
         order=args.order)
     for prompt, out in zip(prompts, outs):
         print(json.dumps({"prompt": prompt, "tokens": out}))
+    return 0
+
+
+def _controls(args):
+    from .sampling.controls import AllowedTokens, Controls
+
+    bias = {}
+    for pair in filter(None, args.logit_bias.replace(" ", "").split(",")):
+        token, _, value = pair.partition(":")
+        bias[int(token)] = float(value)
+    grammar = None
+    if args.allow_tokens:
+        from .config.registry import load_config
+
+        _, cfg = load_config(args.model)
+        grammar = AllowedTokens(_ints(args.allow_tokens), cfg.vocab_size)
+    return Controls(args.repetition_penalty, args.presence_penalty, args.frequency_penalty, bias or None, grammar)
+
+
+def cmd_teach(args) -> int:
+    import numpy as np
+
+    from .engine.teach import teach
+
+    sequences = [_ints(t) for t in args.tokens]
+    if not sequences:
+        print("teach: give --tokens (repeatable)", file=sys.stderr)
+        return 2
+    lessons = teach(args.model, sequences, args.top, args.temperature, dtype=args.dtype, device=args.device)
+    arrays = {f"{name}_{i}": getattr(lesson, name) for i, lesson in enumerate(lessons) for name in ("tokens", "ids", "teacher", "log_sum")}
+    with open(args.out, "wb") as f:
+        np.savez(f, temperature=np.float32(args.temperature), **arrays)
+    print(args.out)
     return 0
 
 
@@ -101,6 +135,11 @@ def main(argv=None) -> int:
     g.add_argument("--top-k", type=int, default=0)
     g.add_argument("--seed", type=int, default=0)
     g.add_argument("--stop-token-ids", default="", metavar="7,9")
+    g.add_argument("--repetition-penalty", type=float, default=1.0, help="divides the positive logits of tokens already there, multiplies the others")
+    g.add_argument("--presence-penalty", type=float, default=0.0, help="taken from the logits of tokens that stand in the answer")
+    g.add_argument("--frequency-penalty", type=float, default=0.0, help="taken from them as often as they stand there")
+    g.add_argument("--logit-bias", default="", metavar="7:1.5,9:-inf", help="added to the logits of single tokens")
+    g.add_argument("--allow-tokens", default="", metavar="1,2,3", help="only these tokens may be drawn")
     g.set_defaults(fn=cmd_generate)
     r = sub.add_parser("random", help="write a model folder with random weights from a config.json and a seed")
     r.add_argument("--config", required=True)
@@ -109,6 +148,15 @@ def main(argv=None) -> int:
     r.add_argument("--std", type=float, default=0.02)
     r.add_argument("--store-dtype", default="bfloat16", choices=("bfloat16", "float32"))
     r.set_defaults(fn=cmd_random)
+    e = sub.add_parser("teach", help="write a model's largest next-token logits along given tokens (.npz), for a student to learn from")
+    e.add_argument("--model", required=True, help="a folder with config.json and model.safetensors")
+    e.add_argument("--tokens", action="append", default=[], metavar="1,2,3", help="one sequence; repeat for more")
+    e.add_argument("--top", type=int, default=64, help="logits of a row (up to 256)")
+    e.add_argument("--temperature", type=float, default=1.0, help="at which the student's loss will be taken")
+    e.add_argument("--out", required=True)
+    e.add_argument("--dtype", default="bfloat16", choices=("bfloat16", "float32"))
+    e.add_argument("--device", default="cuda:0")
+    e.set_defaults(fn=cmd_teach)
     t = sub.add_parser("replay", help="feed given tokens step by step and write logits (bin/trace_run)")
     t.add_argument("--model", required=True)
     t.add_argument("--dtype", required=True, choices=("bfloat16", "float32"))

@@ -24,6 +24,20 @@ finish_step_kernel(const int32_t* __restrict__ tokens, int n, int32_t* host_toke
   if (threadIdx.x == 0) *turn += 1u;
 }
 
+// The step's rows into the table of what requests hold: history[slot of the row's entry][position] = token. Rows of no entry and places
+// outside the table are left out.
+__global__ void __launch_bounds__(128)
+keep_tokens_kernel(int32_t* history, long long ld, int slots, int places, const int32_t* __restrict__ input_ids, const int32_t* __restrict__ positions,
+                   const int32_t* __restrict__ row_entry, const int32_t* __restrict__ state_slot, int n_rows, int n_entries) {
+  pdl_wait();
+  const int t = blockIdx.x * 128 + threadIdx.x;
+  if (t >= n_rows) return;
+  const int entry = row_entry[t], at = positions[t];
+  if (entry < 0 || entry >= n_entries || at < 0 || at >= places) return;
+  const int slot = state_slot[entry];
+  if (slot >= 0 && slot < slots) history[slot * ld + at] = input_ids[t];
+}
+
 // The device's address of pinned host memory, or null where the device cannot reach it.
 extern "C" void* r2_host_address(void* host) {
   void* p = nullptr;
@@ -47,5 +61,14 @@ extern "C" int r2_finish_step(const int32_t* tokens, int n, int32_t* host_tokens
                               cudaStream_t stream) {
   if (n < 0 || n_error < 0 || n_error > 128) return R2_BAD_SHAPE;
   r2_launch(finish_step_kernel, dim3(1), dim3(128), size_t(0), stream, tokens, n, host_tokens, error, n_error, host_error, turn);
+  return launch_status();
+}
+
+extern "C" int r2_keep_tokens(int32_t* history, long long ld, int slots, int places, const int32_t* input_ids, const int32_t* positions,
+                              const int32_t* row_entry, const int32_t* state_slot, int n_rows, int n_entries, cudaStream_t stream) {
+  if (n_rows <= 0) return R2_OK;
+  if (slots < 1 || places < 1 || ld < places || n_entries < 0) return R2_BAD_SHAPE;
+  r2_launch(keep_tokens_kernel, dim3(unsigned(n_rows + 127) / 128), dim3(128), size_t(0), stream, history, ld, slots, places, input_ids, positions,
+            row_entry, state_slot, n_rows, n_entries);
   return launch_status();
 }

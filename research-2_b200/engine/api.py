@@ -22,20 +22,29 @@ def run(model, *, device: str = "cuda:0", dtype: str = "bfloat16", **options) ->
 
 def generate(  # noqa: PLR0913
     model, prompts, max_new_tokens: int, temperature: float = 0.0, top_k: int = 0, seed: int = 0,
-    stop_token_ids=(), *, device: str = "cuda:0", dtype: str = "bfloat16", **options,
+    stop_token_ids=(), *, controls=None, device: str = "cuda:0", dtype: str = "bfloat16", **options,
 ) -> list[list[int]]:
     """Token ids in, token ids out: every prompt's continuation, in the order of `prompts`.
-    Request i draws with key (seed, i), so its tokens do not depend on the batch it runs in."""
+    Request i draws with key (seed, i), so its tokens do not depend on the batch it runs in.
+    `controls`: one `Controls` for all prompts, or one (or None) for each."""
     options.setdefault("max_requests", max(1, min(len(prompts), 256)))
     with run(model, device=device, dtype=dtype, seed=seed, **options) as engine:
-        return generate_with(engine, prompts, max_new_tokens, temperature, top_k, seed, stop_token_ids)
+        return generate_with(engine, prompts, max_new_tokens, temperature, top_k, seed, stop_token_ids, controls=controls)
 
 
-def generate_with(engine: Engine, prompts, max_new_tokens, temperature=0.0, top_k=0, seed=0, stop_token_ids=(), wait=False):
-    """Continuations of all prompts through one engine, as many at a time as it has request slots. With
+def generate_with(engine: Engine, prompts, max_new_tokens, temperature=0.0, top_k=0, seed=0, stop_token_ids=(), wait=False, controls=None, ended=None):
+    """Continuations of all prompts through one engine, as many at a time as it has request slots. `ended(i, rid)`, where given, is called
+    when prompt i's request has ended (its log-probabilities can be asked for then). With
     `wait=False` (the default) a step is only launched before the requests are polled, so the host's share
     of a step runs while the GPU works; the tokens are the same."""
     from .scheduler import Full
+
+    if isinstance(controls, (list, tuple)) and len(controls) != len(prompts):
+        raise ValueError(f"{len(prompts)} prompts and controls for {len(controls)}")
+
+    def asked(i: int) -> dict:
+        own = controls[i] if isinstance(controls, (list, tuple)) else controls
+        return {} if own is None else {"controls": own}
 
     out: list[list[int]] = [[] for _ in prompts]
     live: dict[int, int] = {}
@@ -44,7 +53,7 @@ def generate_with(engine: Engine, prompts, max_new_tokens, temperature=0.0, top_
         while nxt < len(prompts):
             try:
                 rid = engine.submit(prompts[nxt], max_new_tokens, temperature, stop_token_ids, top_k,
-                                    seed=(seed & 0xFFFFFFFF) | (nxt << 32))
+                                    seed=(seed & 0xFFFFFFFF) | (nxt << 32), **asked(nxt))
             except Full:
                 break
             live[rid] = nxt
@@ -54,5 +63,7 @@ def generate_with(engine: Engine, prompts, max_new_tokens, temperature=0.0, top_
             p = engine.poll(rid)
             out[live[rid]] += p.new_tokens
             if p.finished:
+                if ended is not None:
+                    ended(live[rid], rid)
                 del live[rid]
     return out

@@ -27,6 +27,7 @@ class Engine:
         self._plan: Plan | None = None
         self.events: list[StepEvent] = []
         self.keep_events = False
+        self._controls = None   # of requests that ask something of their logits, once there has been one
         self._launched = None   # (graph, number of entries) of a step that runs and is not committed yet
 
     @classmethod
@@ -50,31 +51,57 @@ class Engine:
     # ---- requests --------------------------------------------------------------------------
     def submit(  # noqa: PLR0913
         self, prompt, max_new_tokens: int, temperature: float = 0.0, stop_token_ids=(), top_k: int = 0,
-        seed: int | None = None,
+        seed: int | None = None, controls=None,
     ) -> int:
         """Queue a request; it is admitted at the next step. `seed` keys this request's random
-        draws (default: the engine's seed and the request's ordinal)."""
+        draws (default: the engine's seed and the request's ordinal). `controls`
+        (`sampling.controls.Controls`) asks for penalties, biases, a grammar or log-probabilities;
+        steps with such requests are completed before they return."""
+        vocab_size = self.scheduler.config.vocab_size
+        if controls is not None:
+            controls = controls.checked(vocab_size)
         if seed is None:
             seed = (self.seed & 0xFFFFFFFF) | ((self._ordinal & 0xFFFFFFFF) << 32)
         rid = self.scheduler.submit(prompt, max_new_tokens, temperature, top_k, seed, stop_token_ids)
         self._ordinal += 1
         self._pending[rid] = []
+        if self._controls is not None:
+            self._controls.forget(rid)   # (an id that is given again)
+        if controls:
+            if self._controls is None:
+                from .controls import StepControls
+
+                config = self.scheduler.config
+                self._controls = StepControls(self.step_fn, config.max_requests, config.max_seq_len, vocab_size)
+            self._controls.add(rid, controls, len(prompt))
         return rid
+
+    def logprobs(self, rid: int):
+        """`sampling.controls.TokenLogprobs` of every token of a request that asked for them (`Controls.top_logprobs`), also after its
+        end, until its id is given to another request."""
+        if self._controls is None:
+            raise KeyError(f"no request {rid} with controls")
+        return self._controls.logprobs(rid)
 
     def cancel(self, rid: int) -> None:
         self.finish()
         self.scheduler.cancel(rid)
         self._pending.pop(rid, None)
+        if self._controls is not None:
+            self._controls.forget(rid)
 
     def poll(self, rid: int) -> Poll:
-        return self.scheduler.poll(rid)
+        p = self.scheduler.poll(rid)
+        if p.finished and self._controls is not None:
+            self._controls.forget(rid, keep=True)
+        return p
 
     def wait(self, rid: int, timeout_s: float | None = None) -> Poll:
         """Step until the request has finished; returns all tokens not polled before."""
         deadline = None if timeout_s is None else time.monotonic() + timeout_s
         tokens: list[int] = []
         while True:
-            p = self.scheduler.poll(rid)
+            p = self.poll(rid)
             tokens += p.new_tokens
             if p.finished:
                 self._pending.pop(rid, None)
@@ -115,16 +142,30 @@ class Engine:
         that runs as a CUDA graph is only launched: `finish()`, or the next `step`, `plan`, `wait`,
         `cancel` or `close`, waits for its tokens and commits them (`poll` before that returns
         what earlier steps produced); the return value is then None."""
+        if self._controls is not None and self._controls.requests:
+            self.finish(want_event=self.keep_events)
+            self._controls.check(lambda rid: not self.scheduler.request_info(rid)["state"].startswith("finished"))
         plan = self.plan()
         if plan is None:
             return None
         batch = self.build_batch(plan)
+        if self._controls is not None and self._controls.requests and self._controls.concerns(plan):
+            return self._controlled_step(batch, plan)
         graph = self.step_fn.launch_graph(batch)
         if graph is not None:
             self._launched = (graph, plan.n_entries)
             return self.finish() if wait else None
         tokens = self.step_fn.step_and_sample(batch)
         self.commit(self.step_fn.tokens_to_host(batch, tokens) if hasattr(tokens, "data_ptr") else np.asarray(tokens, dtype=np.int32))
+        event = self.scheduler.event()
+        if self.keep_events:
+            self.events.append(event)
+        return event
+
+    def _controlled_step(self, batch, plan) -> StepEvent:
+        tokens = self._controls.step(batch, plan)
+        self.commit(tokens)
+        self._controls.committed(plan, tokens)   # (the plan's arrays hold until the next one)
         event = self.scheduler.event()
         if self.keep_events:
             self.events.append(event)

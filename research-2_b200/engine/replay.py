@@ -62,6 +62,14 @@ class Replay:
 
     def step(self, record: dict) -> np.ndarray | None:
         """Run one step; returns the wanted logits [n, vocab] (None when nothing is wanted)."""
+        return self._step(record, lambda logits: logits.to(torch.float32).cpu().numpy())
+
+    def step_top(self, record: dict, k: int, temperature: float = 1.0) -> tuple[np.ndarray, np.ndarray, np.ndarray] | None:
+        """Run one step; returns of the wanted rows the k largest logits, their tokens and the logarithm of the row's sum of
+        exponentials at the temperature (`ops.top_logits`), instead of all logits: what a student learns from."""
+        return self._step(record, lambda logits: tuple(t.cpu().numpy() for t in ops.top_logits(logits, k, temperature=temperature)))
+
+    def _step(self, record: dict, take):
         entries = record.get("entries", [])
         reqs, starts, token_lists, wants = [], [], [], []
         self.pages_of_last_step = {}
@@ -94,7 +102,7 @@ class Replay:
             for entry, tokens in zip(entries, token_lists):
                 self.fed[str(entry["id"])] += len(tokens)
             if n_want:
-                result = logits.to(torch.float32).cpu().numpy()
+                result = take(logits)
             else:
                 torch.cuda.synchronize(self.step_fn.device)
             ops.raise_on_device_error(self.step_fn.device)  # a kernel that gave up a bounded wait: the step is void
@@ -120,6 +128,9 @@ def main(argv=None) -> int:
     ap.add_argument("--max-live", type=int, default=4, help="the most requests that are live at a time")
     ap.add_argument("--round-to", type=int, default=64, help="each request's token count is rounded up to a multiple of this")
     ap.add_argument("--capture", action="store_true", help="run steps as CUDA graphs where generation would")
+    ap.add_argument("--top", type=int, default=0, help="write each wanted row's largest logits instead of all: <step>.top.f32 and <step>.ids.i32 "
+                    "[wanted, TOP], <step>.logsum.f32 [wanted]")
+    ap.add_argument("--temperature", type=float, default=1.0, help="of the logarithm of the sum of exponentials beside --top")
     args = ap.parse_args(argv)
     out = Path(args.out)
     out.mkdir(parents=True, exist_ok=True)
@@ -130,8 +141,14 @@ def main(argv=None) -> int:
         if not line:
             continue
         record = json.loads(line)
-        logits = replay.step(record)
-        if logits is not None:
-            logits.astype("<f4").tofile(out / f"{record['step']}.f32")
+        if args.top:
+            top = replay.step_top(record, args.top, args.temperature)
+            if top is not None:
+                for values, name, kind in zip(top, ("top.f32", "ids.i32", "logsum.f32"), ("<f4", "<i4", "<f4")):
+                    values.astype(kind).tofile(out / f"{record['step']}.{name}")
+        else:
+            logits = replay.step(record)
+            if logits is not None:
+                logits.astype("<f4").tofile(out / f"{record['step']}.f32")
         print(f"done {record['step']}", flush=True)
     return 0

@@ -307,8 +307,8 @@ class StepFunction:
         self.h2d_bytes += batch.buf.nbytes
         return StepContext(batch, dev)
 
-    def _launch_by_launch(self, batch: StepBatch, sampled: bool) -> torch.Tensor:
-        """The pass of a batch that is no graph: logits, or with `sampled` the tokens."""
+    def _launch_by_launch(self, batch: StepBatch, sampled: bool) -> tuple[torch.Tensor, StepContext]:
+        """The pass of a batch that is no graph: logits, or with `sampled` the tokens, and the context that it read."""
         # in a caller's own graph nothing can wait for what lies outside it: the caller orders its replays
         ordered = not torch.cuda.is_current_stream_capturing()
         if ordered:
@@ -322,7 +322,7 @@ class StepFunction:
             if self._pass_done is None:
                 self._pass_done = torch.cuda.Event()
             self.order.end(self._pass_done)
-        return out
+        return out, ctx
 
     def validate(self, batch: StepBatch) -> None:
         """Host-side bounds checks of a batch that the caller filled. A batch that the scheduler
@@ -352,6 +352,12 @@ class StepFunction:
         """Logits [n_logit_rows, vocab] float32 on the device."""
         if batch.n_tokens == 0:
             return torch.empty(0, self.model.vocab_size, dtype=torch.float32, device=self.device)
+        return self.logits_and_context(batch)[0]
+
+    @torch.no_grad()
+    def logits_and_context(self, batch: StepBatch) -> tuple[torch.Tensor, StepContext]:
+        """Logits [n_logit_rows, vocab] float32 of a batch that has rows, and the context that the pass read (a graph's is as large as its
+        capacities; both hold until the next pass)."""
         self.validate(batch)
         with torch.cuda.device(self.device):
             graph = self._graph_of(batch)
@@ -360,7 +366,7 @@ class StepFunction:
                     batch.pad()
                 graph.replay(batch)
                 self.h2d_bytes += batch.buf.nbytes
-                return graph.logits[: batch.n_logit_rows]
+                return graph.logits[: batch.n_logit_rows], graph.ctx
             return self._launch_by_launch(batch, sampled=False)
 
     def launch_graph(self, batch: StepBatch) -> StepGraph | None:
@@ -393,7 +399,7 @@ class StepFunction:
                 graph.replay(batch)
                 self.h2d_bytes += batch.buf.nbytes
                 return graph.tokens[: batch.n_logit_rows]
-            return self._launch_by_launch(batch, sampled=True)
+            return self._launch_by_launch(batch, sampled=True)[0]
 
 
 def logit_rows_of_last(batch: StepBatch) -> np.ndarray:

@@ -1908,6 +1908,19 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     return out
 
 
+def keep_tokens(history: torch.Tensor, input_ids: torch.Tensor, positions: torch.Tensor, row_entry: torch.Tensor, state_slot: torch.Tensor) -> None:
+    """A step's rows into the table of the tokens that requests hold, int32 [requests, places]: history[state_slot[row_entry[t]],
+    positions[t]] = input_ids[t]; rows of no entry (-1) and places outside the table are left out."""
+    _need(history, "history", torch.int32, 2)
+    rows = input_ids.shape[0]
+    for name, t in (("input_ids", input_ids), ("positions", positions), ("row_entry", row_entry), ("state_slot", state_slot)):
+        _need(t, name, torch.int32, 1)
+        if not t.is_contiguous() or (t.shape[0] < rows and name != "state_slot"):
+            raise KernelError(f"keep_tokens: {name} must be contiguous, with a number for each of {rows} rows")
+    _check(_lib("step_io").r2_keep_tokens(_p(history), C.c_longlong(_rows(history, "history")), history.shape[0], history.shape[1], _p(input_ids),
+                                          _p(positions), _p(row_entry), _p(state_slot), rows, state_slot.shape[0], _stream()), "keep_tokens")
+
+
 # ---- rows of logits: what stands before the draw, what is written down of them, what a student learns from ----
 
 TOP_MOST = 256   # the most logits of a row that top_logits returns and distill_loss takes
@@ -1919,7 +1932,9 @@ _LOGIT_SIGNATURES = {
     "top_logits": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
     "distill": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
                 C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p],
+    "scale_rows": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p],
 }
+_LOGIT_LIBRARIES = {"scale_rows": "distill"}   # where the library has another name than the entry
 _logit_entries: dict = {}
 
 
@@ -1927,9 +1942,9 @@ def _logit_entry(name: str):
     """The C entry of one of these operators with its argument types set: addresses and numbers go in as plain integers. (A step calls
     them between two kernels of a few microseconds; an object per argument took as long as the kernels.)"""
     entry = _logit_entries.get(name)
-    lib = _libs.get(name)
+    lib = _libs.get(_LOGIT_LIBRARIES.get(name, name))
     if entry is None or entry[0] is not lib:
-        lib = _lib(name)
+        lib = _lib(_LOGIT_LIBRARIES.get(name, name))
         fn = getattr(lib, "r2_" + name)
         fn.argtypes = _LOGIT_SIGNATURES[name]
         entry = _logit_entries[name] = (lib, fn)
@@ -1967,10 +1982,21 @@ def _per_row(t: torch.Tensor | None, name: str, dtype, rows: int, device: int) -
     """The address of a number per row, checked; 0 for none."""
     if t is None:
         return 0
-    if t.dtype is not dtype or t.get_device() != device or t.dim() != 1 or t.shape[0] < rows or (rows > 1 and t.stride(0) != 1):
+    if t.dtype is not dtype or t.get_device() != device or t.dim() != 1 or t.numel() < rows or not t.is_contiguous():
         raise KernelError(f"{name} must be {dtype} on the logits' device, contiguous, with a number for each of {rows} rows; got {t.dtype} on "
                           f"{t.device}, shape {tuple(t.shape)} stride {t.stride()}")
     return t.data_ptr()
+
+
+def _table(t: torch.Tensor, name: str, device: int) -> tuple[int, int, int, int]:
+    """(address, 0 without rows; rows, columns, row stride) of a table of int32 whose rows are contiguous."""
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.get_device() != device:
+        raise KernelError(f"{name} must be a table of int32 on the logits' device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    rows, columns = t.shape
+    ld, inner = t.stride()
+    if columns > 1 and inner != 1:
+        raise KernelError(f"{name} must have contiguous rows, got shape {tuple(t.shape)} stride {t.stride()}")
+    return (t.data_ptr() if rows else 0), rows, columns, ld
 
 
 def _like_logits(logits: torch.Tensor, ld: int, out: torch.Tensor | None, what: str) -> tuple[torch.Tensor, int]:
@@ -2017,15 +2043,11 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     code, rows, vocab, ld, device = _logit_rows(logits, "adjust_logits")
     history_rows = cap = history_ld = history_at = n_masks = mask_ld = mask_at = n_biases = bias_at = 0
     if history is not None:
-        if history.dtype is not torch.int32 or history.dim() != 2 or history.get_device() != device:
-            raise KernelError(f"history must be int32 [requests, tokens] on the logits' device, got {history.dtype} {tuple(history.shape)} on {history.device}")
-        history_ld, (history_rows, cap) = _rows(history, "history"), history.shape
+        history_at, history_rows, cap, history_ld = _table(history, "history", device)
         if lengths is None:
             raise KernelError("adjust_logits: a history needs lengths")
         if slots is None and history_rows < rows:
             raise KernelError(f"adjust_logits: {rows} rows, a history of {history_rows} and no slots")
-        if history_rows > 0:
-            history_at = history.data_ptr()
     elif repetition is not None or presence is not None or frequency is not None:
         raise KernelError("adjust_logits: penalties need a history")
     if bias_start is not None:
@@ -2036,15 +2058,11 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     ids_at = _per_row(bias_ids, "bias_ids", torch.int32, n_biases, device)
     values_at = _per_row(bias_values, "bias_values", torch.float32, n_biases, device)
     if mask is not None:
-        if mask.dtype is not torch.int32 or mask.dim() != 2 or mask.get_device() != device:
-            raise KernelError(f"mask must be int32 [masks, words] on the logits' device, got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
-        n_masks, mask_ld = mask.shape[0], _rows(mask, "mask")
-        if mask.shape[1] * 32 < vocab:
-            raise KernelError(f"adjust_logits: masks of {mask.shape[1]} words are shorter than {vocab} tokens")
+        mask_at, n_masks, words, mask_ld = _table(mask, "mask", device)
+        if words * 32 < vocab:
+            raise KernelError(f"adjust_logits: masks of {words} words are shorter than {vocab} tokens")
         if mask_rows is None and n_masks < rows:
             raise KernelError(f"adjust_logits: {rows} rows, {n_masks} masks and no mask_rows")
-        if n_masks > 0:
-            mask_at = mask.data_ptr()
     numbers = [_per_row(slots, "slots", torch.int32, rows, device), _per_row(lengths, "lengths", torch.int32, rows, device),
                _per_row(prompt_lengths, "prompt_lengths", torch.int32, rows, device), _per_row(repetition, "repetition", torch.float32, rows, device),
                _per_row(presence, "presence", torch.float32, rows, device), _per_row(frequency, "frequency", torch.float32, rows, device)]
@@ -2073,10 +2091,10 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0):
     if not 1 <= k <= min(vocab, TOP_MOST):
         raise KernelError(f"top_logits: k must be in [1, {min(vocab, TOP_MOST)}], got {k}")
     temperature = _temperature(temperature, "top_logits")
-    where = logits.device
-    values = torch.empty((rows, k), dtype=torch.float32, device=where)
-    ids = torch.empty((rows, k), dtype=torch.int32, device=where)
-    log_sum = torch.empty(rows, dtype=torch.float32, device=where)
+    where = logits.device   # (empty_strided costs two thirds of what empty does)
+    values = torch.empty_strided((rows, k), (k, 1), dtype=torch.float32, device=where)
+    ids = torch.empty_strided((rows, k), (k, 1), dtype=torch.int32, device=where)
+    log_sum = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=where)
     if rows:
         _check(_logit_entry("top_logits")(code, logits.data_ptr(), ld, rows, vocab, k, temperature, values.data_ptr(), ids.data_ptr(),
                                           log_sum.data_ptr(), _current_stream(device)), "top_logits")
@@ -2109,10 +2127,21 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
     if out is not None and not gradient:
         raise KernelError("distill_loss: out is where the gradient goes, and none is asked for")
     where = logits.device
-    loss = torch.empty(rows, dtype=torch.float32, device=where)
+    loss = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=where)
     grad, grad_ld = _like_logits(logits, ld, out, "distill_loss") if gradient else (None, 0)
     if rows:
         _check(_logit_entry("distill")(code, logits.data_ptr(), ld, rows, vocab, ids.data_ptr(), teacher.data_ptr(), k, log_sum_at, weight_at,
                                        temperature, loss.data_ptr(), grad.data_ptr() if gradient else 0, grad_ld, _workspace(where).error.data_ptr(),
                                        _current_stream(device)), "distill_loss")
     return loss, grad
+
+
+def scale_rows(x: torch.Tensor, factors: torch.Tensor) -> torch.Tensor:
+    """Rows x [R, V] (float32 or bfloat16) times a float32 factor each, in place; `factors` has one for every row, or one for all. A row whose
+    factor is 1 is not touched, so that a gradient which is wanted as it stands costs a look at its factors."""
+    code, rows, vocab, ld, device = _logit_rows(x, "scale_rows")
+    one = factors.numel() == 1
+    at = _per_row(factors.reshape(1) if one else factors, "factors", torch.float32, 1 if one else rows, device)
+    if rows:
+        _check(_logit_entry("scale_rows")(code, x.data_ptr(), ld, rows, vocab, at, 0 if one else 1, _current_stream(device)), "scale_rows")
+    return x
