@@ -74,14 +74,14 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
 
 // A piece of the row for a reader that may also be its writer in the same launch (no read-only path), not kept in L1. Elements beyond the row
 // are -inf.
-template <typename T>
-__device__ __forceinline__ uint4 load_once(const RowPieces<T>& row, int g) {
+__device__ __forceinline__ uint4 load_16(const uint4* from) {
   uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(reinterpret_cast<const uint4*>(row.base) + g));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(from));
   return v;
 }
+template <typename T>
+__device__ __forceinline__ uint4 load_once(const RowPieces<T>& row, int g) { return load_16(reinterpret_cast<const uint4*>(row.base) + g); }
+
 // Elements of a piece to -inf where their bits are 0. A bit becomes a byte's highest (the product puts bit i at 8 i + 7 and nothing else
 // there), and a byte's highest bit becomes whole bytes (prmt's sign mode).
 __device__ __forceinline__ uint32_t spread(uint32_t four_bits) { return (four_bits * 0x10204080u) & 0x80808080u; }
