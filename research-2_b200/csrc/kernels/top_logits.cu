@@ -2,25 +2,29 @@
 // the row's sum of exponentials at a temperature.
 //
 // A row is read once. While it passes, a thread sums exponentials against its own maximum and keeps the maximum of every group of four
-// 16-byte pieces. The k-th largest of the 384 reading threads' maxima (or a little less) is a value that at least k elements reach, and what
-// reaches it stands in the groups whose maximum does: little more than k groups of 16 or 32 elements, which are read again and give little
-// more than k candidates. Their order is found by counting for each how many stand above it. Values are compared as unsigned keys in the
+// 16-byte pieces. The k-th largest of the maxima of 384 pairs of threads (or a little less) is a value that at least k elements reach, and
+// what reaches it stands in the groups whose maximum does: little more than k groups of 16 or 32 elements, which are read again and give
+// little more than k candidates. Their order is found by counting for each how many stand above it. Values are compared as unsigned keys in the
 // floats' order, with the token as the lower half.
 //
 // Rows whose candidates do not fit (thousands of equal values at the edge of the list, or fewer than k numbers that are not NaN) are gone
 // over again: the exact k-th value by counts in bins of the keys' range, bin by bin narrower, everything above it, and equal values in the
 // order of their tokens until the list is full.
 //
-// Twelve warps of a CTA read, row after row, and four choose: the candidates of one row are looked for while the next one passes. Few rows
-// are cut over the CTAs of a cluster, whose candidates meet in the first one's shared memory.
+// An SM has one CTA: 24 warps read, row after row, and two teams of four choose, in turn: the candidates of two rows are looked for while the
+// next one passes. Few rows are cut over the CTAs of a cluster, whose candidates meet in the first one's shared memory.
 #include "logit_rows.cuh"
 
 namespace {
 
-constexpr int READERS = 384, CHOOSERS = 128, READING_WARPS = READERS / 32, CHOOSING_WARPS = CHOOSERS / 32;
+constexpr int READERS = 768, PAIRS_OF_READERS = READERS / 2, READING_WARPS = READERS / 32;
+constexpr int CHOOSERS = 128, CHOOSING_WARPS = CHOOSERS / 32, TEAMS = 2;   // of a team
+// Rows that are between reading and choosing. A place is always the same team's: with a place that changed teams, one that is ahead of the
+// other would take the readers' word for the other's row as its own.
+constexpr int PLACES = 2 * TEAMS;
 constexpr int MOST_K = 256, MOST_RANKS = 8;
 constexpr int DEPTH = 4;      // pieces of a group
-constexpr int SLOTS = 9;      // groups of a thread (of several rounds each in long rows)
+constexpr int SLOTS = 6;      // groups of a thread (of several rounds each in long rows)
 constexpr int CAP = 2304;     // candidates
 constexpr int BINS = 512;
 constexpr int LEVELS = 4;     // 9 bits of a 32-bit key at each
@@ -33,12 +37,14 @@ struct TopArgs {
   float* values; int32_t* ids; float* log_sum;
 };
 
-struct Shared {
-  // of two rows in turn, from those who read to those who choose
-  uint32_t groups[2][SLOTS][READERS];     // the groups' maxima, as keys
-  uint32_t most[2][READERS];              // the threads' maxima
-  float2 sums[2][READING_WARPS];          // the warps' references and sums
-  // the choosers' own
+// From those who read to those who choose.
+struct __align__(16) Place {
+  uint32_t groups[SLOTS][READERS];        // the groups' maxima, as keys
+  uint32_t most[PAIRS_OF_READERS];        // the maxima of pairs of threads
+  float2 sums[READING_WARPS];             // the warps' references and sums
+};
+// A team's own.
+struct __align__(16) Shared {
   unsigned long long found[MOST_SORTED];  // candidates: key, then the token's complement
   uint32_t bins[BINS];
   uint32_t chosen[BINS];                  // groups that are read again: slot * READERS + thread
@@ -46,25 +52,53 @@ struct Shared {
   uint32_t low, high, above, n_found, n_chosen;
   float2 rank_sums[MOST_RANKS];           // of the cluster's CTAs
   uint32_t n_of[MOST_RANKS];
+  int team;
+};
+struct TopShared {
+  Place places[PLACES];
+  Shared teams[TEAMS];
 };
 
-__device__ __forceinline__ void choosers_meet() { asm volatile("bar.sync 1, %0;" ::"n"(CHOOSERS) : "memory"); }
-// Between those who read and those who choose, for each of the two rows' places: they are full, they may be filled again.
-__device__ __forceinline__ void wait_full(int b) {
-  if (b) asm volatile("bar.sync 3, %0;" ::"n"(READERS + CHOOSERS) : "memory");
-  else asm volatile("bar.sync 2, %0;" ::"n"(READERS + CHOOSERS) : "memory");
+template <int ID, int COUNT> __device__ __forceinline__ void bar_sync() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(COUNT) : "memory"); }
+template <int ID, int COUNT> __device__ __forceinline__ void bar_arrive() { asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(COUNT) : "memory"); }
+__device__ __forceinline__ void choosers_meet(int team) {
+  if (team) bar_sync<2, CHOOSERS>();
+  else bar_sync<1, CHOOSERS>();
 }
-__device__ __forceinline__ void say_full(int b) {
-  if (b) asm volatile("bar.arrive 3, %0;" ::"n"(READERS + CHOOSERS) : "memory");
-  else asm volatile("bar.arrive 2, %0;" ::"n"(READERS + CHOOSERS) : "memory");
+// Between the readers and the team whose turn it is, for each place: it is full, it may be filled again.
+constexpr int BOTH = READERS + CHOOSERS;
+static_assert(PLACES == 4, "a case for each place");
+__device__ __forceinline__ void wait_full(int p) {
+  switch (p) {
+    case 0: return bar_sync<3, BOTH>();
+    case 1: return bar_sync<4, BOTH>();
+    case 2: return bar_sync<5, BOTH>();
+    default: return bar_sync<6, BOTH>();
+  }
 }
-__device__ __forceinline__ void wait_empty(int b) {
-  if (b) asm volatile("bar.sync 5, %0;" ::"n"(READERS + CHOOSERS) : "memory");
-  else asm volatile("bar.sync 4, %0;" ::"n"(READERS + CHOOSERS) : "memory");
+__device__ __forceinline__ void say_full(int p) {
+  switch (p) {
+    case 0: return bar_arrive<3, BOTH>();
+    case 1: return bar_arrive<4, BOTH>();
+    case 2: return bar_arrive<5, BOTH>();
+    default: return bar_arrive<6, BOTH>();
+  }
 }
-__device__ __forceinline__ void say_empty(int b) {
-  if (b) asm volatile("bar.arrive 5, %0;" ::"n"(READERS + CHOOSERS) : "memory");
-  else asm volatile("bar.arrive 4, %0;" ::"n"(READERS + CHOOSERS) : "memory");
+__device__ __forceinline__ void wait_empty(int p) {
+  switch (p) {
+    case 0: return bar_sync<7, BOTH>();
+    case 1: return bar_sync<8, BOTH>();
+    case 2: return bar_sync<9, BOTH>();
+    default: return bar_sync<10, BOTH>();
+  }
+}
+__device__ __forceinline__ void say_empty(int p) {
+  switch (p) {
+    case 0: return bar_arrive<7, BOTH>();
+    case 1: return bar_arrive<8, BOTH>();
+    case 2: return bar_arrive<9, BOTH>();
+    default: return bar_arrive<10, BOTH>();
+  }
 }
 
 __device__ __forceinline__ float value_of(uint32_t key) {
@@ -78,7 +112,7 @@ __device__ __forceinline__ unsigned long long composite(uint32_t key, int token)
 // One level: the bins of the keys in [low, high] are counted; from the top, the bin at which the count (with `above`, keys over `high`)
 // reaches k becomes the range. True once the bins are single keys.
 __device__ __forceinline__ bool narrow(Shared& s, int k, int shift, int tid) {
-  choosers_meet();
+  choosers_meet(s.team);
   if (tid < 32) {
     const int lane = tid;
     uint32_t c[BINS / 32], sum = 0u;   // lane l has the bins from BINS - 1 - 16 l down
@@ -110,7 +144,7 @@ __device__ __forceinline__ bool narrow(Shared& s, int k, int shift, int tid) {
       }
     }
   }
-  choosers_meet();
+  choosers_meet(s.team);
   return shift == 0;
 }
 __device__ __forceinline__ int shift_of(uint32_t low, uint32_t high) {   // (high - low) >> shift < BINS
@@ -166,28 +200,28 @@ __device__ __noinline__ void go_over(Shared& s, const Row<T>& row, int k, uint32
       }
     }
   };
-  choosers_meet();
+  choosers_meet(s.team);
   if (tid == 0) {
     s.low = reached;
     s.high = 0xffffffffu;
     s.above = 0u;
     s.n_found = 0u;
   }
-  choosers_meet();
+  choosers_meet(s.team);
   // whether fewer than k lie above `reached`: then it is the k-th value
   uint32_t more = 0u;
   over([&](uint32_t key, int) { more += key > reached ? 1u : 0u; });
   more = __reduce_add_sync(0xffffffffu, more);
   if (lane == 0) atomicAdd(&s.n_found, more);
-  choosers_meet();
+  choosers_meet(s.team);
   const bool is_kth = s.n_found < uint32_t(k);
-  choosers_meet();
+  choosers_meet(s.team);
   if (is_kth) {
     if (tid == 0) s.high = s.low;
   } else {
     for (int level = 0; level < LEVELS; ++level) {
       for (int b = tid; b < BINS; b += CHOOSERS) s.bins[b] = 0u;
-      choosers_meet();
+      choosers_meet(s.team);
       const uint32_t low = s.low, high = s.high;
       const int shift = shift_of(low, high);
       over([&](uint32_t key, int) {
@@ -197,12 +231,12 @@ __device__ __noinline__ void go_over(Shared& s, const Row<T>& row, int k, uint32
     }
   }
   if (tid == 0) s.n_found = 0u;
-  choosers_meet();
+  choosers_meet(s.team);
   const uint32_t kth = s.low;
   over([&](uint32_t key, int token) {
     if (key > kth) s.found[atomicAdd(&s.n_found, 1u)] = composite(key, token);   // (fewer than k)
   });
-  choosers_meet();
+  choosers_meet(s.team);
   // equal values in the tokens' order
   int wanted = k - int(s.n_found), have = int(s.n_found);
   for (int base = 0; base < row.n && wanted > 0; base += CHOOSERS) {
@@ -222,9 +256,9 @@ __device__ __noinline__ void go_over(Shared& s, const Row<T>& row, int k, uint32
       const uint32_t other = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += other;
     }
-    choosers_meet();
+    choosers_meet(s.team);
     if (lane == 31) s.warp_numbers[warp] = upto;
-    choosers_meet();
+    choosers_meet(s.team);
     uint32_t before = upto - mine, all = 0u;
     for (int i = 0; i < CHOOSING_WARPS; ++i) {
       before += i < warp ? s.warp_numbers[i] : 0u;
@@ -239,14 +273,14 @@ __device__ __noinline__ void go_over(Shared& s, const Row<T>& row, int k, uint32
     wanted -= taken;
     have += taken;
   }
-  choosers_meet();
+  choosers_meet(s.team);
   if (tid == 0) s.n_found = uint32_t(have);
-  choosers_meet();
+  choosers_meet(s.team);
 }
 
 // What a CTA's readers do with a share of a row: its groups' and threads' maxima, its warps' sums.
 template <typename T>
-__device__ __forceinline__ void read_share(Shared& s, const Row<T>& row, int b, int rounds, int shift, float c, int tid) {
+__device__ __forceinline__ void read_share(Place& place, const Row<T>& row, int rounds, int shift, float c, int tid) {
   constexpr int PAIRS = RowPieces<T>::PER / 2;
   const int together = 1 << shift;
   const uint64_t cc = two_of(c, c);
@@ -281,7 +315,7 @@ __device__ __forceinline__ void read_share(Shared& s, const Row<T>& row, int b, 
     sum += both.x + both.y;
     slot_max = max(slot_max, logit_key(most));
     if (--until == 0) {
-      s.groups[b][slot][tid] = slot_max;
+      place.groups[slot][tid] = slot_max;
       thread_max = max(thread_max, slot_max);
       slot_max = 0u;
       ++slot;
@@ -313,21 +347,22 @@ __device__ __forceinline__ void read_share(Shared& s, const Row<T>& row, int b, 
     take(one);
   }
   if (until != together) {
-    s.groups[b][slot][tid] = slot_max;
+    place.groups[slot][tid] = slot_max;
     thread_max = max(thread_max, slot_max);
   }
-  s.most[b][tid] = thread_max;
+  thread_max = max(thread_max, __shfl_xor_sync(0xffffffffu, thread_max, 1));
+  if ((tid & 1) == 0) place.most[tid >> 1] = thread_max;
   const float common = warp_max(reference);
   sum = warp_sum(sum * rebase(reference, common));
-  if ((tid & 31) == 0) s.sums[b][tid >> 5] = make_float2(common, sum);
+  if ((tid & 31) == 0) place.sums[tid >> 5] = make_float2(common, sum);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(READERS + CHOOSERS, 2)
+__global__ void __launch_bounds__(READERS + TEAMS * CHOOSERS, 1)
 top_kernel(const TopArgs a) {
   constexpr int PER = RowPieces<T>::PER;
   extern __shared__ __align__(16) uint8_t top_smem[];
-  Shared& s = *reinterpret_cast<Shared*>(top_smem);
+  TopShared& shared = *reinterpret_cast<TopShared*>(top_smem);
   pdl_launch_dependents();
   const int ranks = a.ranks, step = int(gridDim.x) / ranks, rank = int(blockIdx.x) % ranks, first_row = int(blockIdx.x) / ranks;
   const float c = 1.44269504f / a.tau;
@@ -343,11 +378,11 @@ top_kernel(const TopArgs a) {
 
   if (threadIdx.x < READERS) {
     const int tid = int(threadIdx.x);
-    for (int r = first_row, turn = 0; r < a.rows; r += step, ++turn) {
+    for (int r = first_row, turn = 0, p = 0; r < a.rows; r += step, ++turn, p = p + 1 == PLACES ? 0 : p + 1) {
       const Row<T> row = share_of(r);
-      if (turn >= 2) wait_empty(turn & 1);
-      read_share(s, row, turn & 1, (row.n + READERS * DEPTH - 1) / (READERS * DEPTH), shift, c, tid);
-      say_full(turn & 1);
+      if (turn >= PLACES) wait_empty(p);
+      read_share(shared.places[p], row, (row.n + READERS * DEPTH - 1) / (READERS * DEPTH), shift, c, tid);
+      say_full(p);
     }
     if (ranks > 1) {  // (one row to a cluster: the choosers' two barriers)
       cluster_arrive();
@@ -358,26 +393,36 @@ top_kernel(const TopArgs a) {
     return;
   }
 
-  const int tid = int(threadIdx.x) - READERS, lane = tid & 31;
-  for (int r = first_row, turn = 0; r < a.rows; r += step, ++turn) {
+  const int team = (int(threadIdx.x) - READERS) / CHOOSERS, tid = (int(threadIdx.x) - READERS) % CHOOSERS, lane = tid & 31;
+  Shared& s = shared.teams[team];
+  if (tid == 0) s.team = team;
+  if (team > 0 && ranks > 1) {  // (one row to a cluster, the first team's)
+    cluster_arrive();
+    cluster_wait();
+    cluster_arrive();
+    cluster_wait();
+    return;
+  }
+  for (int r = first_row + team * step, turn = team; r < a.rows; r += TEAMS * step, turn += TEAMS) {
     const Row<T> row = share_of(r);
-    const int b = turn & 1, rounds = (row.n + READERS * DEPTH - 1) / (READERS * DEPTH), slots = (rounds + (1 << shift) - 1) >> shift;
+    const int p = turn % PLACES, rounds = (row.n + READERS * DEPTH - 1) / (READERS * DEPTH), slots = (rounds + (1 << shift) - 1) >> shift;
+    Place& place = shared.places[p];
     const int first_token = max(0, row.x.first(row.g0)), end_token = min(a.vocab, row.x.first(row.g0) + row.n * PER);
     const int k = min(a.k, end_token - first_token);   // of this share
-    choosers_meet();   // (the row before has been written out)
+    choosers_meet(team);   // (the row before has been written out)
     if (tid == 0) s.n_found = s.n_chosen = s.above = 0u;
-    wait_full(b);
-    float2 part = lane < READING_WARPS ? s.sums[b][lane] : make_float2(-INFINITY, 0.f);
+    wait_full(p);
+    float2 part = lane < READING_WARPS ? place.sums[lane] : make_float2(-INFINITY, 0.f);
     float common = warp_max(part.x), total = warp_sum(part.y * rebase(part.x, common));
     uint32_t reached = 0u;
     bool fits = true;
     if (row.n >= READERS) {   // a group for every reader
-      // what k readers' maxima or a few more reach, by halving, in every warp for itself
-      constexpr int OWN = READERS / 32;
+      // what k pairs' maxima or a few more reach, by halving, in every warp for itself
+      constexpr int OWN = PAIRS_OF_READERS / 32;
       uint32_t most[OWN], low = 0xffffffffu, high = 0u;
 #pragma unroll
       for (int i = 0; i < OWN; ++i) {
-        most[i] = s.most[b][lane + i * 32];
+        most[i] = place.most[lane + i * 32];
         low = min(low, most[i]);
         high = max(high, most[i]);
       }
@@ -397,17 +442,26 @@ top_kernel(const TopArgs a) {
       reached = low;
       // the groups that reach it
 #pragma unroll
-      for (int i = 0; i < READERS / CHOOSERS; ++i) {
-        const int reader = tid + i * CHOOSERS;
-        if (s.most[b][reader] < reached) continue;
-        for (int g = 0; g < slots; ++g) {
-          if (s.groups[b][g][reader] < reached) continue;
-          const uint32_t place = atomicAdd(&s.n_chosen, 1u);
-          if (place < uint32_t(BINS)) s.chosen[place] = uint32_t(g * READERS + reader);
+      for (int i = 0; i < PAIRS_OF_READERS / CHOOSERS; ++i) {
+        const int pair = tid + i * CHOOSERS;
+        if (place.most[pair] < reached) continue;
+        uint2 both[SLOTS];
+#pragma unroll
+        for (int g = 0; g < SLOTS; ++g) both[g] = g < slots ? *reinterpret_cast<const uint2*>(&place.groups[g][2 * pair]) : make_uint2(0u, 0u);
+#pragma unroll
+        for (int g = 0; g < SLOTS; ++g) {
+          if (g < slots && both[g].x >= reached) {
+            const uint32_t at = atomicAdd(&s.n_chosen, 1u);
+            if (at < uint32_t(BINS)) s.chosen[at] = uint32_t(g * READERS + 2 * pair);
+          }
+          if (g < slots && both[g].y >= reached) {
+            const uint32_t at = atomicAdd(&s.n_chosen, 1u);
+            if (at < uint32_t(BINS)) s.chosen[at] = uint32_t(g * READERS + 2 * pair + 1);
+          }
         }
       }
-      choosers_meet();
-      if (r + 2 * step < a.rows) say_empty(b);
+      choosers_meet(s.team);
+      if (r + PLACES * step < a.rows) say_empty(p);
       fits = s.n_chosen <= uint32_t(BINS);
       if (fits) {
         // their pieces again, a piece a thread, several on their way
@@ -419,11 +473,11 @@ top_kernel(const TopArgs a) {
           int at[WAY];
 #pragma unroll
           for (int i = 0; i < WAY; ++i) {
-            const int p = p0 + i * CHOOSERS;
+            const int piece = p0 + i * CHOOSERS;
             at[i] = row.n;
-            if (p < pieces) {
-              const uint32_t group = s.chosen[p >> (shift + 2)];
-              at[i] = ((int(group / READERS) << (shift + 2)) + (p & ((DEPTH << shift) - 1))) * READERS + int(group % READERS);
+            if (piece < pieces) {
+              const uint32_t group = s.chosen[piece >> (shift + 2)];
+              at[i] = ((int(group / READERS) << (shift + 2)) + (piece & ((DEPTH << shift) - 1))) * READERS + int(group % READERS);
             }
             if (at[i] < row.n) raw[i] = row.load(at[i]);
           }
@@ -445,8 +499,8 @@ top_kernel(const TopArgs a) {
         }
       }
     } else {   // a short share: everything is a candidate, or too many for the list
-      choosers_meet();
-      if (r + 2 * step < a.rows) say_empty(b);
+      choosers_meet(s.team);
+      if (r + PLACES * step < a.rows) say_empty(p);
       if (tid == 0) s.n_found = uint32_t(end_token - first_token);
       if (end_token - first_token <= CAP) {
         for (int at = tid; at < row.n; at += CHOOSERS) {
@@ -460,9 +514,9 @@ top_kernel(const TopArgs a) {
         }
       }
     }
-    choosers_meet();
+    choosers_meet(s.team);
     if (!fits || s.n_found > uint32_t(CAP)) go_over(s, row, k, reached, tid);
-    else if (s.n_found < uint32_t(k)) go_over(s, row, k, 0u, tid);
+    if (s.n_found < uint32_t(k)) go_over(s, row, k, 0u, tid);   // (fewer than k numbers that are not NaN)
 
     // the cluster's candidates into its first CTA
     int n = int(s.n_found);
@@ -494,13 +548,13 @@ top_kernel(const TopArgs a) {
         unsigned long long keep[EACH];
 #pragma unroll
         for (int i = 0; i < EACH; ++i) keep[i] = tid + i * CHOOSERS < count ? s.found[from + tid + i * CHOOSERS] : 0ull;
-        choosers_meet();
+        choosers_meet(s.team);
 #pragma unroll
         for (int i = 0; i < EACH; ++i)
           if (tid + i * CHOOSERS < count) s.found[all + tid + i * CHOOSERS] = keep[i];
         all += count;
       }
-      choosers_meet();
+      choosers_meet(s.team);
       n = all;
     }
     if (tid == 0) a.log_sum[r] = (no_less(common) + log2f(total)) * 0.693147181f;
@@ -509,14 +563,19 @@ top_kernel(const TopArgs a) {
     int32_t* ids = a.ids + (long long)r * a.k;
     if (n <= 4 * CHOOSERS) {
       // a candidate's place: how many stand above it
+      if ((n & 1) && tid == 0) s.found[n] = 0ull;
+      choosers_meet(s.team);
       for (int i = tid; i < n; i += CHOOSERS) {
         const unsigned long long mine = s.found[i];
-        int place = 0;
-#pragma unroll 8
-        for (int j = 0; j < n; ++j) place += s.found[j] > mine ? 1 : 0;
-        if (place < a.k) {
-          values[place] = value_of(uint32_t(mine >> 32));
-          ids[place] = int32_t(0xffffffffu - uint32_t(mine & 0xffffffffull));
+        int above = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; j += 2) {
+          const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(s.found + j);   // (behind the last one stands a 0)
+          above += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
+        }
+        if (above < a.k) {
+          values[above] = value_of(uint32_t(mine >> 32));
+          ids[above] = int32_t(0xffffffffu - uint32_t(mine & 0xffffffffull));
         }
       }
       continue;
@@ -525,7 +584,7 @@ top_kernel(const TopArgs a) {
     int size = 4 * CHOOSERS;
     while (size < n) size *= 2;
     for (int i = n + tid; i < size; i += CHOOSERS) s.found[i] = 0ull;
-    choosers_meet();
+    choosers_meet(s.team);
     for (int run = 2; run <= size; run *= 2) {
       for (int apart = run / 2; apart > 0; apart /= 2) {
         for (int i = tid; i < size / 2; i += CHOOSERS) {
@@ -536,7 +595,7 @@ top_kernel(const TopArgs a) {
             s.found[hi] = x;
           }
         }
-        choosers_meet();
+        choosers_meet(s.team);
       }
     }
     for (int i = tid; i < a.k; i += CHOOSERS) {
@@ -550,14 +609,14 @@ template <typename T>
 int launch(TopArgs a, int rows, cudaStream_t stream) {
   const int pieces = (a.vocab + 2 * RowPieces<T>::PER - 2) / RowPieces<T>::PER;   // of a row at any alignment, at most
   a.ranks = 1;
-  while (a.ranks < MOST_RANKS && (long long)rows * a.ranks * 2 <= 296 && pieces / (2 * a.ranks) >= 1024) a.ranks *= 2;
+  while (a.ranks < MOST_RANKS && (long long)rows * a.ranks * 2 <= 148 && pieces / (2 * a.ranks) >= 1024) a.ranks *= 2;
   a.per = (pieces + a.ranks - 1) / a.ranks;
   if ((long long)rows * a.ranks > 0x7fffffffLL) return R2_BAD_SHAPE;
   static std::atomic<bool> allowed[64];
-  const int status = allow_smem(top_kernel<T>, sizeof(Shared), allowed);
+  const int status = allow_smem(top_kernel<T>, sizeof(TopShared), allowed);
   if (status != R2_OK) return status;
-  const int walking = a.ranks > 1 ? rows : min(rows, 2 * 148);   // as many as run at a time
-  r2_launch_clusters(top_kernel<T>, a.ranks, dim3(unsigned(walking) * unsigned(a.ranks)), dim3(READERS + CHOOSERS), sizeof(Shared), stream, a);
+  const int walking = a.ranks > 1 ? rows : min(rows, 148);   // as many as run at a time
+  r2_launch_clusters(top_kernel<T>, a.ranks, dim3(unsigned(walking) * unsigned(a.ranks)), dim3(READERS + TEAMS * CHOOSERS), sizeof(TopShared), stream, a);
   return launch_status();
 }
 

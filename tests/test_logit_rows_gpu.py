@@ -223,6 +223,21 @@ def test_top_logits_of_equal_values(vocab):
     check_top(rows_at(x, BF16, 3), 200)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_top_logits_of_many_rows_some_of_equal_values(dtype):
+    """Several rows a CTA, those that are gone over (equal values, few numbers) next to others, in every order."""
+    rows, vocab, k = 900, 9001, 40
+    x = random_logits(rows, vocab, 6).to(dtype).to(DEV)
+    kind = torch.randint(0, 5, (rows,), generator=torch.Generator().manual_seed(2)).to(DEV)
+    kind[100:130], kind[450:600] = 0, 1
+    x[kind == 0] = 1.5
+    x[kind == 1, 20:] = -math.inf
+    x[kind == 2] = (torch.arange(vocab, device=DEV) % 7).to(dtype)
+    values, ids, _ = ops().top_logits(x, k)
+    order = torch.argsort(x.float(), dim=1, descending=True, stable=True)[:, :k]
+    assert torch.equal(ids.long(), order) and torch.equal(values, torch.gather(x.float(), 1, order))
+
+
 @pytest.mark.parametrize("order", ["rising", "falling"])
 def test_top_logits_of_rows_in_order(order):
     x = torch.linspace(-20, 20, 50257)[None].repeat(2, 1)
