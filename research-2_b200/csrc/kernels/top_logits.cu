@@ -278,21 +278,62 @@ __device__ __noinline__ void go_over(Shared& s, const Row<T>& row, int k, uint32
   choosers_meet(s.team);
 }
 
-// What a CTA's readers do with a share of a row: its groups' and threads' maxima, its warps' sums.
-template <typename T>
-__device__ __forceinline__ void read_share(Place& place, const Row<T>& row, int rounds, int shift, float c, int tid) {
-  constexpr int PAIRS = RowPieces<T>::PER / 2;
+// What a CTA's readers do: shares of rows, round after round, the pieces of the two rounds behind the one in hand on their way, over the rows'
+// ends too. Of every share its groups' and pairs' maxima and its warps' sums.
+template <typename T, typename ShareOf>
+__device__ __forceinline__ void read_shares(TopShared& shared, const ShareOf& share_of, int first_row, int rows, int step, int shift, float c, int tid) {
+  constexpr int PAIRS = RowPieces<T>::PER / 2, ROUND = READERS * DEPTH;
   const int together = 1 << shift;
   const uint64_t cc = two_of(c, c);
-  float reference = -INFINITY, sum = 0.f;
-  uint32_t thread_max = 0u, slot_max = 0u;
-  int slot = 0, until = together;   // the slot that is being filled, the rounds that it still takes
-  const uint4* from = reinterpret_cast<const uint4*>(row.x.base) + row.g0 + tid;
-  auto load = [&](uint4 (&raw)[DEPTH], int round) {
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) raw[i] = load_16(from + round * (READERS * DEPTH) + i * READERS);
+  // the round that is asked for next
+  int next_row = first_row, next_round = 0, next_n = 0;
+  const uint4* from = nullptr;
+  auto open = [&]() {
+    if (next_row >= rows) return;
+    const Row<T> row = share_of(next_row);
+    next_n = row.n;
+    from = reinterpret_cast<const uint4*>(row.x.base) + row.g0 + tid;
   };
-  auto take = [&](const uint4 (&raw)[DEPTH]) {
+  open();
+  auto ask = [&](uint4 (&raw)[DEPTH]) {
+    if (next_row >= rows) return;
+    if ((next_round + 1) * ROUND <= next_n) {
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) raw[i] = load_16(from + i * READERS);
+    } else {
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) {
+        const uint32_t nothing = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+        raw[i] = make_uint4(nothing, nothing, nothing, nothing);
+        if (next_round * ROUND + i * READERS + tid < next_n) raw[i] = load_16(from + i * READERS);
+      }
+    }
+    from += ROUND;
+    if (++next_round * ROUND >= next_n) {
+      next_row += step;
+      next_round = 0;
+      open();
+    }
+  };
+  // the round in hand
+  int r = first_row, round = 0, rounds = 0, turn = 0, slot = 0, until = together;   // until: rounds that the slot still takes
+  float reference = -INFINITY, sum = 0.f;
+  uint32_t pair_max = 0u, slot_max = 0u;
+  auto take = [&](uint4 (&raw)[DEPTH]) {
+    Place& place = shared.places[turn % PLACES];
+    if (round == 0) {
+      rounds = (share_of(r).n + ROUND - 1) / ROUND;
+      if (turn >= PLACES) wait_empty(turn % PLACES);
+    }
+    const bool last = round + 1 == rounds;
+    if (round == 0 || last) {   // the ends of the row
+      const Row<T> row = share_of(r);
+      if (row.g0 == 0 && round == 0 && tid == 0) blank_outside(raw[0], row.x, 0);
+      const int end = row.x.count - 1 - row.g0 - round * ROUND;
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i)
+        if (end == i * READERS + tid && end + round * ROUND < row.n) blank_outside(raw[i], row.x, row.x.count - 1);
+    }
     const float most = largest<T, DEPTH>(raw), up = fminf(most * c, 3e38f);   // (an infinity sums to infinity against any number)
     if (up > reference) {
       sum *= rebase(reference, up);
@@ -314,47 +355,39 @@ __device__ __forceinline__ void read_share(Place& place, const Row<T>& row, int 
     const float2 both = halves(acc[0]);
     sum += both.x + both.y;
     slot_max = max(slot_max, logit_key(most));
-    if (--until == 0) {
+    if (--until == 0 || last) {
       place.groups[slot][tid] = slot_max;
-      thread_max = max(thread_max, slot_max);
+      pair_max = max(pair_max, slot_max);
       slot_max = 0u;
       ++slot;
       until = together;
     }
+    ++round;
+    if (!last) return;
+    pair_max = max(pair_max, __shfl_xor_sync(0xffffffffu, pair_max, 1));
+    if ((tid & 1) == 0) place.most[tid >> 1] = pair_max;
+    const float common = warp_max(reference);
+    sum = warp_sum(sum * rebase(reference, common));
+    if ((tid & 31) == 0) place.sums[tid >> 5] = make_float2(common, sum);
+    say_full(turn % PLACES);
+    reference = -INFINITY;
+    sum = 0.f;
+    pair_max = 0u;
+    round = slot = 0;
+    r += step;
+    ++turn;
   };
-  // two groups' pieces are on their way in turn; the last round may end early, and has the row's last piece
-  const int full = rounds - 1;
   uint4 one[DEPTH], two[DEPTH];
-  if (full > 0) load(one, 0);
-  if (full > 1) load(two, 1);
-  if (row.g0 == 0 && tid == 0 && full > 0) blank_outside(one[0], row.x, 0);
-  int round = 0;
+  ask(one);
+  ask(two);
 #pragma unroll 1
-  for (; round + 2 <= full; round += 2) {
+  while (r < rows) {
     take(one);
-    if (round + 2 < full) load(one, round + 2);
+    ask(one);
+    if (r >= rows) break;
     take(two);
-    if (round + 3 < full) load(two, round + 3);
+    ask(two);
   }
-  if (round < full) take(one);
-  if (rounds > 0) {
-    const int at = full * READERS * DEPTH + tid;
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) {
-      const uint32_t nothing = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
-      one[i] = at + i * READERS < row.n ? row.load(at + i * READERS) : make_uint4(nothing, nothing, nothing, nothing);
-    }
-    take(one);
-  }
-  if (until != together) {
-    place.groups[slot][tid] = slot_max;
-    thread_max = max(thread_max, slot_max);
-  }
-  thread_max = max(thread_max, __shfl_xor_sync(0xffffffffu, thread_max, 1));
-  if ((tid & 1) == 0) place.most[tid >> 1] = thread_max;
-  const float common = warp_max(reference);
-  sum = warp_sum(sum * rebase(reference, common));
-  if ((tid & 31) == 0) place.sums[tid >> 5] = make_float2(common, sum);
 }
 
 template <typename T>
@@ -378,12 +411,7 @@ top_kernel(const TopArgs a) {
 
   if (threadIdx.x < READERS) {
     const int tid = int(threadIdx.x);
-    for (int r = first_row, turn = 0, p = 0; r < a.rows; r += step, ++turn, p = p + 1 == PLACES ? 0 : p + 1) {
-      const Row<T> row = share_of(r);
-      if (turn >= PLACES) wait_empty(p);
-      read_share(shared.places[p], row, (row.n + READERS * DEPTH - 1) / (READERS * DEPTH), shift, c, tid);
-      say_full(p);
-    }
+    read_shares<T>(shared, share_of, first_row, a.rows, step, shift, c, tid);
     if (ranks > 1) {  // (one row to a cluster: the choosers' two barriers)
       cluster_arrive();
       cluster_wait();
@@ -467,6 +495,7 @@ top_kernel(const TopArgs a) {
         // their pieces again, a piece a thread, several on their way
         const int pieces = int(s.n_chosen) << (shift + 2);
         constexpr int WAY = 4;
+        const float reached_value = value_of(reached);
 #pragma unroll 1
         for (int p0 = tid; p0 < pieces; p0 += WAY * CHOOSERS) {
           uint4 raw[WAY];
@@ -488,12 +517,11 @@ top_kernel(const TopArgs a) {
             unpack(raw[i], v, static_cast<const T*>(nullptr));
 #pragma unroll
             for (int e = 0; e < PER; ++e) {
-              const uint32_t key = logit_key(v[e]);
+              if (!(v[e] >= reached_value)) continue;
               const int token = row.x.first(row.g0 + at[i]) + e;
-              if (key >= reached && row.inside(token)) {
-                const uint32_t place = atomicAdd(&s.n_found, 1u);
-                if (place < uint32_t(CAP)) s.found[place] = composite(key, token);
-              }
+              if (!row.inside(token)) continue;
+              const uint32_t place = atomicAdd(&s.n_found, 1u);
+              if (place < uint32_t(CAP)) s.found[place] = composite(logit_key(v[e]), token);
             }
           }
         }
@@ -567,12 +595,14 @@ top_kernel(const TopArgs a) {
       choosers_meet(s.team);
       for (int i = tid; i < n; i += CHOOSERS) {
         const unsigned long long mine = s.found[i];
-        int above = 0;
+        int above = 0, also = 0;
 #pragma unroll 4
         for (int j = 0; j < n; j += 2) {
           const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(s.found + j);   // (behind the last one stands a 0)
-          above += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
+          above += two.x > mine ? 1 : 0;
+          also += two.y > mine ? 1 : 0;
         }
+        above += also;
         if (above < a.k) {
           values[above] = value_of(uint32_t(mine >> 32));
           ids[above] = int32_t(0xffffffffu - uint32_t(mine & 0xffffffffull));
