@@ -131,6 +131,20 @@ def test_adjust_logits(rows, vocab, cap, n_biases, dtype):
         assert inside.data_ptr() == case.x.data_ptr() and torch.equal(inside, got)
 
 
+@pytest.mark.parametrize("vocab,cap", [(3000, 16384), (40001, 40000)])
+def test_adjust_logits_long_histories(vocab, cap):
+    """Histories longer than the counts that 16 bits hold, one token standing in almost all of one."""
+    case = Adjust(2, vocab, cap, 5, 11, F32, 1, 2)
+    case.history[case.slots[0], 100:] = 17
+    case.lengths[0], case.prompts[0] = cap, 30
+    got = ops().adjust_logits(case.x, **case.arguments())
+    want = case.want()
+    fine = np.isfinite(want)
+    off = np.abs(got.double().cpu().numpy()[fine] - want[fine])
+    # the penalty of a token that stands c times: c * frequency in float32
+    assert np.array_equal(np.isfinite(got.cpu().numpy()), fine) and np.all(off <= 8 * EPS * (60 + np.abs(want[fine])))
+
+
 def test_adjust_logits_writes_nothing_but_its_rows():
     case = Adjust(3, 1031, 50, 9, 5, BF16, offset=3, pad=6)
     out = rows_at(torch.zeros(3, 1031), BF16, 1, 4)
@@ -328,6 +342,24 @@ def test_distill_loss(rows, vocab, k, dtype, tail):
         assert torch.equal(case.run(out=apart)[1], gradient)
         loss_in, inside = case.run(out=case.x)
         assert inside.data_ptr() == case.x.data_ptr() and torch.equal(inside, gradient) and torch.equal(loss_in, loss)
+
+
+@pytest.mark.parametrize("vocab,dtype", [(440011, F32), (880007, BF16)])
+def test_distill_loss_of_rows_that_no_cluster_holds(vocab, dtype):
+    case = Distill(2, vocab, 9, 1, dtype, True, 2.0, 1, 0)
+    loss, gradient = case.run()
+    case.check(loss, gradient)
+    inside = case.run(out=case.x)
+    assert torch.equal(inside[0], loss) and torch.equal(inside[1], gradient)
+
+
+def test_distill_lists_that_name_a_token_twice():
+    """The gradient counts every entry; nothing else is promised of such a list."""
+    case = Distill(2, 3001, 6, 2, F32, False, 1.0)
+    case.ids[:, 3] = case.ids[:, 0]
+    loss, gradient = case.run()
+    want = case.want()[1]
+    assert torch.isfinite(loss).all() and np.all(np.abs(gradient.double().cpu().numpy() - want) <= 1e-5)
 
 
 @pytest.mark.parametrize("rows", [1, 20, 150, 400])
