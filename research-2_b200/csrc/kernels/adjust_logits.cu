@@ -17,7 +17,7 @@
 
 namespace {
 
-constexpr int DEPTH = 4;   // pieces of a thread on their way
+constexpr int DEPTH = 4, CHUNK = 4;   // pieces, and entries of the history, of a thread on their way
 // A place: the token stands in the prompt, it has a bias, how often it stands in the answer. 16 bits where no history is longer than their
 // counts, else 32.
 template <typename W> struct Place {
@@ -69,9 +69,12 @@ adjust_kernel(const AdjustArgs a) {
   const uint32_t* mask = mask_row >= 0 && mask_row < a.n_masks ? a.mask + (long long)mask_row * a.mask_ld : nullptr;
   const int length = slot >= 0 && slot < a.history_rows ? max(0, min(length_asked, a.history_cap)) : 0;
   const int32_t* tokens = a.history + (long long)slot * a.history_ld;
-  int ahead[4];
+  int ahead[CHUNK];   // entries of the history
+  auto load_tokens = [&](int i0) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ahead[i] = tid + i * THREADS < length ? __ldg(tokens + tid + i * THREADS) : -1;
+    for (int i = 0; i < CHUNK; ++i) ahead[i] = i0 + i * THREADS < length ? __ldg(tokens + i0 + i * THREADS) : -1;
+  };
+  load_tokens(tid);
   int bias_token = -1;
   float bias_value = 0.f;
   if (bias_begin + tid < bias_end) {
@@ -105,25 +108,33 @@ adjust_kernel(const AdjustArgs a) {
   if (mask != nullptr) load_first();
 
   // what the request holds of this segment (places before and behind the row may be counted in, and are never written out)
-  auto count = [&](int token, int i) {
-    const uint32_t at = uint32_t(token - zero), shift = at % EACH * 16;
-    bool first = false;
-    if (at < uint32_t(size) && i < length) {
-      const uint32_t before = i < prompt ? atomicOr(&places[at / EACH], PROMPT << shift) : atomicAdd(&places[at / EACH], 1u << shift);
-      first = ((before >> shift) & ANY) == 0u;
-    }
-    const uint32_t firsts = __ballot_sync(0xffffffffu, first);
-    if (firsts == 0u) return;
-    int base = 0;
-    if (lane == 0) base = atomicAdd(&n_touched, __popc(firsts));
-    base = __shfl_sync(0xffffffffu, base, 0);
-    if (first) touched[base + __popc(firsts & ((1u << lane) - 1u))] = uint16_t(at);
-  };
+#pragma unroll 1
+  for (int i0 = tid; i0 - tid < length; i0 += CHUNK * THREADS) {
+    if (i0 != tid) load_tokens(i0);
+    uint32_t firsts[CHUNK];   // of the warp's lanes, those whose entry is its token's first
+    int all = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i * THREADS < length) count(ahead[i], tid + i * THREADS);
-#pragma unroll 4
-  for (int i = tid + 4 * THREADS; i - tid < length; i += THREADS) count(i < length ? __ldg(tokens + i) : -1, i);
+    for (int c = 0; c < CHUNK; ++c) {
+      const int i = i0 + c * THREADS;
+      const uint32_t at = uint32_t(ahead[c] - zero), shift = at % EACH * 16;
+      bool first = false;
+      if (at < uint32_t(size) && i < length) {
+        const uint32_t before = i < prompt ? atomicOr(&places[at / EACH], PROMPT << shift) : atomicAdd(&places[at / EACH], 1u << shift);
+        first = ((before >> shift) & ANY) == 0u;
+      }
+      firsts[c] = __ballot_sync(0xffffffffu, first);
+      all += __popc(firsts[c]);
+    }
+    if (all == 0) continue;
+    int base = 0;
+    if (lane == 0) base = atomicAdd(&n_touched, all);
+    base = __shfl_sync(0xffffffffu, base, 0);
+#pragma unroll
+    for (int c = 0; c < CHUNK; ++c) {
+      if ((firsts[c] >> lane) & 1u) touched[base + __popc(firsts[c] & ((1u << lane) - 1u))] = uint16_t(ahead[c] - zero);
+      base += __popc(firsts[c]);
+    }
+  }
   __syncthreads();
   auto mark = [&](int token) {
     const uint32_t at = uint32_t(token - zero), shift = at % EACH * 16;
