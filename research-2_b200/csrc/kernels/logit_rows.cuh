@@ -79,6 +79,10 @@ __device__ __forceinline__ uint4 load_16(const uint4* from) {
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(from));
   return v;
 }
+__device__ __forceinline__ void load_16_if(uint4& v, const uint4* from, bool asked) {   // (else what was there stays)
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n @p ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
+               : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w) : "l"(from), "r"(uint32_t(asked)));
+}
 template <typename T>
 __device__ __forceinline__ uint4 load_once(const RowPieces<T>& row, int g) { return load_16(reinterpret_cast<const uint4*>(row.base) + g); }
 

@@ -2,34 +2,33 @@
 // the row's sum of exponentials at a temperature.
 //
 // A row is read once. While it passes, a thread sums exponentials against its own maximum and keeps the maximum of every group of four
-// 16-byte pieces. The k-th largest of the maxima of 384 pairs of threads (or a little less) is a value that at least k elements reach, and
+// 16-byte pieces. The k-th largest of the maxima of 320 pairs of threads (or a little less) is a value that at least k elements reach, and
 // what reaches it stands in the groups whose maximum does: little more than k groups of 16 or 32 elements, which are read again and give
-// little more than k candidates. Their order is found by counting for each how many stand above it. Values are compared as unsigned keys in the
+// little more than k candidates. Warps sort 32 of them at a time, and a candidate's place is how many stand above it in all of these runs. Values are compared as unsigned keys in the
 // floats' order, with the token as the lower half.
 //
 // Rows whose candidates do not fit (thousands of equal values at the edge of the list, or fewer than k numbers that are not NaN) are gone
 // over again: the exact k-th value by counts in bins of the keys' range, bin by bin narrower, everything above it, and equal values in the
 // order of their tokens until the list is full.
 //
-// An SM has one CTA: 24 warps read, row after row, and two teams of four choose, in turn: the candidates of two rows are looked for while the
-// next one passes. Few rows are cut over the CTAs of a cluster, whose candidates meet in the first one's shared memory.
+// An SM has one CTA: 20 warps read, row after row, and two teams of four choose, in turn: the candidates of two rows are looked for while the
+// next one passes. Behind a CTA's last row nothing passes any more, and its readers choose it themselves. Few rows are cut over the CTAs of
+// a cluster, whose candidates meet in the first one's shared memory.
 #include "logit_rows.cuh"
 
 namespace {
 
-constexpr int READERS = 768, PAIRS_OF_READERS = READERS / 2, READING_WARPS = READERS / 32;
-constexpr int CHOOSERS = 128, CHOOSING_WARPS = CHOOSERS / 32, TEAMS = 2;   // of a team
+constexpr int READERS = 640, PAIRS_OF_READERS = READERS / 2, READING_WARPS = READERS / 32;
+constexpr int CHOOSERS = 128, TEAMS = 2;   // of a team
 // Rows that are between reading and choosing. A place is always the same team's: with a place that changed teams, one that is ahead of the
 // other would take the readers' word for the other's row as its own.
 constexpr int PLACES = 2 * TEAMS;
 constexpr int MOST_K = 256, MOST_RANKS = 8;
 constexpr int DEPTH = 4;      // pieces of a group
-constexpr int SLOTS = 6;      // groups of a thread (of several rounds each in long rows)
-constexpr int CAP = 2304;     // candidates
-constexpr int BINS = 512;
+constexpr int SLOTS = 8;      // groups of a thread (of several rounds each in long rows)
+constexpr int CAP = 1536;     // candidates
+constexpr int MOST_CHOSEN = 1024, BINS = 512;
 constexpr int LEVELS = 4;     // 9 bits of a 32-bit key at each
-constexpr int MOST_SORTED = 4096;
-
 struct TopArgs {
   const void* logits; long long ld;
   int rows, vocab, k, ranks, per;
@@ -39,30 +38,40 @@ struct TopArgs {
 
 // From those who read to those who choose.
 struct __align__(16) Place {
-  uint32_t groups[SLOTS][READERS];        // the groups' maxima, as keys
-  uint32_t most[PAIRS_OF_READERS];        // the maxima of pairs of threads
+  uint16_t groups[SLOTS][READERS];        // the groups' maxima: the upper halves of their keys
+  uint32_t most[PAIRS_OF_READERS];        // the maxima of pairs of threads, as keys
   float2 sums[READING_WARPS];             // the warps' references and sums
 };
 // A team's own.
 struct __align__(16) Shared {
-  unsigned long long found[MOST_SORTED];  // candidates: key, then the token's complement
-  uint32_t bins[BINS];
-  uint32_t chosen[BINS];                  // groups that are read again: slot * READERS + thread
-  uint32_t warp_numbers[CHOOSING_WARPS];
+  unsigned long long found[CAP];          // candidates: key, then the token's complement
+  union {
+    uint16_t chosen[MOST_CHOSEN];         // groups that are read again: slot * READERS + thread
+    uint32_t bins[BINS];
+  };
+  uint32_t warp_numbers[READING_WARPS];
   uint32_t low, high, above, n_found, n_chosen;
   float2 rank_sums[MOST_RANKS];           // of the cluster's CTAs
   uint32_t n_of[MOST_RANKS];
   int team;
 };
+// (Shared memory is missing to L1, which holds what loads have on their way: with 220 KB of it instead of 91 a pass took a quarter longer.)
 struct TopShared {
   Place places[PLACES];
-  Shared teams[TEAMS];
+  Shared teams[TEAMS + 1];   // the last one: the readers'
 };
+// Clusters have one row, the readers': what they send each other stands in the other places, what the first CTA puts together in the teams'.
+static_assert((MOST_RANKS - 1) * MOST_K * sizeof(unsigned long long) <= (PLACES - 1) * sizeof(Place), "");
+static_assert(MOST_RANKS * MOST_K * sizeof(unsigned long long) <= TEAMS * sizeof(Shared), "");
+static_assert(SLOTS * READERS <= 65536 && PAIRS_OF_READERS >= MOST_K && PAIRS_OF_READERS < 1024, "");
 
 template <int ID, int COUNT> __device__ __forceinline__ void bar_sync() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(COUNT) : "memory"); }
 template <int ID, int COUNT> __device__ __forceinline__ void bar_arrive() { asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(COUNT) : "memory"); }
+// those who choose a row: a team, or the readers
+template <int THREADS>
 __device__ __forceinline__ void choosers_meet(int team) {
-  if (team) bar_sync<2, CHOOSERS>();
+  if (THREADS == READERS) bar_sync<11, READERS>();
+  else if (team) bar_sync<2, CHOOSERS>();
   else bar_sync<1, CHOOSERS>();
 }
 // Between the readers and the team whose turn it is, for each place: it is full, it may be filled again.
@@ -109,10 +118,29 @@ __device__ __forceinline__ unsigned long long composite(uint32_t key, int token)
   return (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - uint32_t(token));
 }
 
+// The least value of the type that reaches a key.
+template <typename T> __device__ __forceinline__ T value_from(uint32_t key);
+template <> __device__ __forceinline__ float value_from<float>(uint32_t key) { return value_of(key); }
+template <> __device__ __forceinline__ bf16 value_from<bf16>(uint32_t key) { return __float2bfloat16_ru(value_of(key)); }
+// A piece's elements that are not less than `least`, as bits.
+__device__ __forceinline__ uint32_t reaching(const uint4& raw, float least) {
+  return (__uint_as_float(raw.x) >= least ? 1u : 0u) | (__uint_as_float(raw.y) >= least ? 2u : 0u) | (__uint_as_float(raw.z) >= least ? 4u : 0u) |
+         (__uint_as_float(raw.w) >= least ? 8u : 0u);
+}
+__device__ __forceinline__ uint32_t reaching(const uint4& raw, bf16 least) {
+  const __nv_bfloat162 both = __bfloat162bfloat162(least);
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t bits = 0u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) bits |= __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[j]), both) & (0x00020001u << (2 * j));
+  return (bits | bits >> 16) & 0xffu;
+}
+
 // One level: the bins of the keys in [low, high] are counted; from the top, the bin at which the count (with `above`, keys over `high`)
 // reaches k becomes the range. True once the bins are single keys.
+template <int THREADS>
 __device__ __forceinline__ bool narrow(Shared& s, int k, int shift, int tid) {
-  choosers_meet(s.team);
+  choosers_meet<THREADS>(s.team);
   if (tid < 32) {
     const int lane = tid;
     uint32_t c[BINS / 32], sum = 0u;   // lane l has the bins from BINS - 1 - 16 l down
@@ -144,7 +172,7 @@ __device__ __forceinline__ bool narrow(Shared& s, int k, int shift, int tid) {
       }
     }
   }
-  choosers_meet(s.team);
+  choosers_meet<THREADS>(s.team);
   return shift == 0;
 }
 __device__ __forceinline__ int shift_of(uint32_t low, uint32_t high) {   // (high - low) >> shift < BINS
@@ -185,12 +213,12 @@ __device__ __forceinline__ float largest(const uint4 (&raw)[N]) {
 }
 
 // The row again, from its exact k-th value: at least k of the share's elements reach `reached`, or it is 0.
-template <typename T>
+template <typename T, int THREADS>
 __device__ __noinline__ void go_over(Shared& s, const Row<T>& row, int k, uint32_t reached, int tid) {
   constexpr int PER = RowPieces<T>::PER;
   const int lane = tid & 31, warp = tid >> 5;
   auto over = [&](auto&& f) {   // every element of the share: (key, token)
-    for (int at = tid; at < row.n; at += CHOOSERS) {
+    for (int at = tid; at < row.n; at += THREADS) {
       float v[PER];
       unpack(row.load(at), v, static_cast<const T*>(nullptr));
 #pragma unroll
@@ -200,46 +228,46 @@ __device__ __noinline__ void go_over(Shared& s, const Row<T>& row, int k, uint32
       }
     }
   };
-  choosers_meet(s.team);
+  choosers_meet<THREADS>(s.team);
   if (tid == 0) {
     s.low = reached;
     s.high = 0xffffffffu;
     s.above = 0u;
     s.n_found = 0u;
   }
-  choosers_meet(s.team);
+  choosers_meet<THREADS>(s.team);
   // whether fewer than k lie above `reached`: then it is the k-th value
   uint32_t more = 0u;
   over([&](uint32_t key, int) { more += key > reached ? 1u : 0u; });
   more = __reduce_add_sync(0xffffffffu, more);
   if (lane == 0) atomicAdd(&s.n_found, more);
-  choosers_meet(s.team);
+  choosers_meet<THREADS>(s.team);
   const bool is_kth = s.n_found < uint32_t(k);
-  choosers_meet(s.team);
+  choosers_meet<THREADS>(s.team);
   if (is_kth) {
     if (tid == 0) s.high = s.low;
   } else {
     for (int level = 0; level < LEVELS; ++level) {
-      for (int b = tid; b < BINS; b += CHOOSERS) s.bins[b] = 0u;
-      choosers_meet(s.team);
+      for (int b = tid; b < BINS; b += THREADS) s.bins[b] = 0u;
+      choosers_meet<THREADS>(s.team);
       const uint32_t low = s.low, high = s.high;
       const int shift = shift_of(low, high);
       over([&](uint32_t key, int) {
         if (key >= low && key <= high) atomicAdd(&s.bins[(key - low) >> shift], 1u);
       });
-      if (narrow(s, k, shift, tid)) break;
+      if (narrow<THREADS>(s, k, shift, tid)) break;
     }
   }
   if (tid == 0) s.n_found = 0u;
-  choosers_meet(s.team);
+  choosers_meet<THREADS>(s.team);
   const uint32_t kth = s.low;
   over([&](uint32_t key, int token) {
     if (key > kth) s.found[atomicAdd(&s.n_found, 1u)] = composite(key, token);   // (fewer than k)
   });
-  choosers_meet(s.team);
+  choosers_meet<THREADS>(s.team);
   // equal values in the tokens' order
   int wanted = k - int(s.n_found), have = int(s.n_found);
-  for (int base = 0; base < row.n && wanted > 0; base += CHOOSERS) {
+  for (int base = 0; base < row.n && wanted > 0; base += THREADS) {
     const int at = base + tid;
     uint32_t equal = 0u;
     if (at < row.n) {
@@ -256,11 +284,11 @@ __device__ __noinline__ void go_over(Shared& s, const Row<T>& row, int k, uint32
       const uint32_t other = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += other;
     }
-    choosers_meet(s.team);
+    choosers_meet<THREADS>(s.team);
     if (lane == 31) s.warp_numbers[warp] = upto;
-    choosers_meet(s.team);
+    choosers_meet<THREADS>(s.team);
     uint32_t before = upto - mine, all = 0u;
-    for (int i = 0; i < CHOOSING_WARPS; ++i) {
+    for (int i = 0; i < THREADS / 32; ++i) {
       before += i < warp ? s.warp_numbers[i] : 0u;
       all += s.warp_numbers[i];
     }
@@ -273,66 +301,64 @@ __device__ __noinline__ void go_over(Shared& s, const Row<T>& row, int k, uint32
     wanted -= taken;
     have += taken;
   }
-  choosers_meet(s.team);
+  choosers_meet<THREADS>(s.team);
   if (tid == 0) s.n_found = uint32_t(have);
-  choosers_meet(s.team);
+  choosers_meet<THREADS>(s.team);
 }
 
 // What a CTA's readers do: shares of rows, round after round, the pieces of the two rounds behind the one in hand on their way, over the rows'
-// ends too. Of every share its groups' and pairs' maxima and its warps' sums.
+// ends too. Of every share its groups' and pairs' maxima and its warps' sums. -> the turn of the last one.
 template <typename T, typename ShareOf>
-__device__ __forceinline__ void read_shares(TopShared& shared, const ShareOf& share_of, int first_row, int rows, int step, int shift, float c, int tid) {
+__device__ __forceinline__ int read_shares(TopShared& shared, const ShareOf& share_of, int first_row, int rows, int step, int shift, float c, int tid) {
   constexpr int PAIRS = RowPieces<T>::PER / 2, ROUND = READERS * DEPTH;
   const int together = 1 << shift;
   const uint64_t cc = two_of(c, c);
-  // the round that is asked for next
-  int next_row = first_row, next_round = 0, next_n = 0;
+  // the round that is asked for next, and the pieces from its first one on
+  int next_row = first_row, next_left = 0;
   const uint4* from = nullptr;
   auto open = [&]() {
     if (next_row >= rows) return;
     const Row<T> row = share_of(next_row);
-    next_n = row.n;
+    next_left = row.n;
     from = reinterpret_cast<const uint4*>(row.x.base) + row.g0 + tid;
   };
   open();
   auto ask = [&](uint4 (&raw)[DEPTH]) {
     if (next_row >= rows) return;
-    if ((next_round + 1) * ROUND <= next_n) {
+    if (next_left > ROUND) {
 #pragma unroll
       for (int i = 0; i < DEPTH; ++i) raw[i] = load_16(from + i * READERS);
+      from += ROUND;
+      next_left -= ROUND;
     } else {
 #pragma unroll
-      for (int i = 0; i < DEPTH; ++i) {
-        const uint32_t nothing = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
-        raw[i] = make_uint4(nothing, nothing, nothing, nothing);
-        if (next_round * ROUND + i * READERS + tid < next_n) raw[i] = load_16(from + i * READERS);
-      }
-    }
-    from += ROUND;
-    if (++next_round * ROUND >= next_n) {
+      for (int i = 0; i < DEPTH; ++i) load_16_if(raw[i], from + i * READERS, i * READERS + tid < next_left);
       next_row += step;
-      next_round = 0;
       open();
     }
   };
   // the round in hand
-  int r = first_row, round = 0, rounds = 0, turn = 0, slot = 0, until = together;   // until: rounds that the slot still takes
+  int r = first_row, left = 0, turn = 0, slot = 0, until = together;   // left: pieces from its first one on; until: rounds that the slot still takes
   float reference = -INFINITY, sum = 0.f;
   uint32_t pair_max = 0u, slot_max = 0u;
   auto take = [&](uint4 (&raw)[DEPTH]) {
     Place& place = shared.places[turn % PLACES];
-    if (round == 0) {
-      rounds = (share_of(r).n + ROUND - 1) / ROUND;
+    if (left == 0) {
+      const Row<T> row = share_of(r);
+      left = row.n;
+      if (row.g0 == 0 && tid == 0) blank_outside(raw[0], row.x, 0);
       if (turn >= PLACES) wait_empty(turn % PLACES);
     }
-    const bool last = round + 1 == rounds;
-    if (round == 0 || last) {   // the ends of the row
+    const bool last = left <= ROUND;
+    const int end = left - 1 - tid;   // the share's last piece is this thread's i-th where i * READERS == end
+    if (last) {
       const Row<T> row = share_of(r);
-      if (row.g0 == 0 && round == 0 && tid == 0) blank_outside(raw[0], row.x, 0);
-      const int end = row.x.count - 1 - row.g0 - round * ROUND;
+      const uint32_t nothing = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
-      for (int i = 0; i < DEPTH; ++i)
-        if (end == i * READERS + tid && end + round * ROUND < row.n) blank_outside(raw[i], row.x, row.x.count - 1);
+      for (int i = 0; i < DEPTH; ++i) {
+        if (i * READERS > end) raw[i] = make_uint4(nothing, nothing, nothing, nothing);
+        else if (i * READERS == end && row.g0 + row.n == row.x.count) blank_outside(raw[i], row.x, row.x.count - 1);
+      }
     }
     const float most = largest<T, DEPTH>(raw), up = fminf(most * c, 3e38f);   // (an infinity sums to infinity against any number)
     if (up > reference) {
@@ -341,43 +367,51 @@ __device__ __forceinline__ void read_shares(TopShared& shared, const ShareOf& sh
     }
     const float minus = -no_less(reference);
     const uint64_t ss = two_of(minus, minus);
-    uint64_t acc[DEPTH];
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) {
+    auto sum_of = [&](const uint4& piece) {
       uint64_t p[PAIRS];
-      unpack_pairs(raw[i], p, static_cast<const T*>(nullptr));
-      acc[i] = exp2_two(fma_two(p[0], cc, ss));
+      unpack_pairs(piece, p, static_cast<const T*>(nullptr));
+      uint64_t acc = exp2_two(fma_two(p[0], cc, ss));
 #pragma unroll
-      for (int j = 1; j < PAIRS; ++j) acc[i] = add_two(acc[i], exp2_two(fma_two(p[j], cc, ss)));
+      for (int j = 1; j < PAIRS; ++j) acc = add_two(acc, exp2_two(fma_two(p[j], cc, ss)));
+      return acc;
+    };
+    uint64_t acc = 0ull;
+    if (!last) {
+      uint64_t of[DEPTH];
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) of[i] = sum_of(raw[i]);
+      acc = add_two(add_two(of[0], of[1]), add_two(of[2], of[3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i)
+        if (i * READERS <= end) acc = add_two(acc, sum_of(raw[i]));
     }
-#pragma unroll
-    for (int i = 1; i < DEPTH; ++i) acc[0] = add_two(acc[0], acc[i]);
-    const float2 both = halves(acc[0]);
+    const float2 both = halves(acc);
     sum += both.x + both.y;
     slot_max = max(slot_max, logit_key(most));
     if (--until == 0 || last) {
-      place.groups[slot][tid] = slot_max;
+      place.groups[slot][tid] = uint16_t(slot_max >> 16);
       pair_max = max(pair_max, slot_max);
       slot_max = 0u;
       ++slot;
       until = together;
     }
-    ++round;
+    left -= ROUND;
     if (!last) return;
     pair_max = max(pair_max, __shfl_xor_sync(0xffffffffu, pair_max, 1));
     if ((tid & 1) == 0) place.most[tid >> 1] = pair_max;
     const float common = warp_max(reference);
     sum = warp_sum(sum * rebase(reference, common));
     if ((tid & 31) == 0) place.sums[tid >> 5] = make_float2(common, sum);
-    say_full(turn % PLACES);
+    r += step;
+    if (r < rows) say_full(turn % PLACES);   // (the last one is the readers' own)
     reference = -INFINITY;
     sum = 0.f;
     pair_max = 0u;
-    round = slot = 0;
-    r += step;
+    left = slot = 0;
     ++turn;
   };
-  uint4 one[DEPTH], two[DEPTH];
+  uint4 one[DEPTH] = {}, two[DEPTH] = {};
   ask(one);
   ask(two);
 #pragma unroll 1
@@ -388,17 +422,254 @@ __device__ __forceinline__ void read_shares(TopShared& shared, const ShareOf& sh
     take(two);
     ask(two);
   }
+  return turn - 1;
+}
+
+// A warp's values from the largest down.
+__device__ __forceinline__ unsigned long long sorted(unsigned long long v, int lane) {
+#pragma unroll
+  for (int run = 2; run <= 32; run *= 2) {
+#pragma unroll
+    for (int apart = run / 2; apart > 0; apart /= 2) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, v, apart);
+      const bool larger = ((lane & run) == 0) == ((lane & apart) == 0);   // this lane keeps the larger one
+      if (larger == (other > v)) v = other;
+    }
+  }
+  return v;
+}
+// How many of a run of 32 stand above `mine`.
+__device__ __forceinline__ int above_in(const unsigned long long* run, unsigned long long mine) {
+  int at = 0;
+#pragma unroll
+  for (int step = 16; step > 0; step /= 2) at += run[at + step - 1] > mine ? step : 0;
+  return at + (run[at] > mine ? 1 : 0);
+}
+// Places on a list for every thread's `mine` entries, one atomic a warp. -> the first one's.
+__device__ __forceinline__ uint32_t places_for(uint32_t mine, uint32_t* count, int lane) {
+  uint32_t upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t other = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += other;
+  }
+  uint32_t base = 0u;
+  if (lane == 31) base = atomicAdd(count, upto);
+  return __shfl_sync(0xffffffffu, base, 31) + upto - mine;
+}
+
+// A row's k, from its share's maxima and sums; `released` once the place is no longer read. (A cluster's shares are chosen by readers.)
+template <typename T, int THREADS, typename Released>
+__device__ __forceinline__ void choose(const TopArgs& a, TopShared& shared, Shared& s, const Place& place, const Row<T>& row, int r, int shift, int rank,
+                                       int tid, const Released& released) {
+  constexpr int PER = RowPieces<T>::PER;
+  const int lane = tid & 31, warp = tid >> 5, slots = ((row.n + READERS * DEPTH - 1) / (READERS * DEPTH) + (1 << shift) - 1) >> shift;
+  const int first_token = max(0, row.x.first(row.g0)), end_token = min(a.vocab, row.x.first(row.g0) + row.n * PER);
+  const int k = min(a.k, end_token - first_token);   // of this share
+  float common = 0.f, total = 0.f;   // (the second warp's)
+  auto write_sum = [&]() {
+    if (lane == 0) a.log_sum[r] = (no_less(common) + log2f(total)) * 0.693147181f;
+  };
+  if (warp == 1) {
+    const float2 part = lane < READING_WARPS ? place.sums[lane] : make_float2(-INFINITY, 0.f);
+    common = warp_max(part.x);
+    total = warp_sum(part.y * rebase(part.x, common));
+    if (a.ranks == 1) write_sum();
+  }
+  // what k pairs' maxima or a few more reach, three values tried at a time (their counts in ten bits each)
+  if (warp == 0) {
+    constexpr int OWN = PAIRS_OF_READERS / 32;
+    uint32_t most[OWN], low = 0xffffffffu, high = 0u;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      most[i] = place.most[lane + i * 32];
+      low = min(low, most[i]);
+      high = max(high, most[i]);
+    }
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    const int enough = k + max(8, k / 8);
+    while (low < high) {
+      const uint32_t half = (high - low) / 2, one = low + half / 2 + 1, two = low + half + 1, three = two + half / 2;   // all in (low, high]
+      uint32_t reach = 0u;
+#pragma unroll
+      for (int i = 0; i < OWN; ++i)
+        reach += (most[i] >= one ? 1u : 0u) + (most[i] >= two ? 1u << 10 : 0u) + (most[i] >= three ? 1u << 20 : 0u);
+      reach = __reduce_add_sync(0xffffffffu, reach);
+      const int of_one = int(reach & 1023u), of_two = int((reach >> 10) & 1023u), of_three = int(reach >> 20);
+      int of_low = 0;
+      if (of_three >= k) {
+        low = three;
+        of_low = of_three;
+      } else if (of_two >= k) {
+        low = two;
+        high = three - 1;
+        of_low = of_two;
+      } else if (of_one >= k) {
+        low = one;
+        high = two - 1;
+        of_low = of_one;
+      } else {
+        high = one - 1;
+      }
+      if (of_low >= k && of_low <= enough) break;
+    }
+    if (lane == 0) s.low = low;
+  }
+  choosers_meet<THREADS>(s.team);
+  const uint32_t reached = s.low;
+  // the groups that reach it
+  constexpr int EACH = (PAIRS_OF_READERS + THREADS - 1) / THREADS;
+  uint32_t hits[EACH], mine = 0u;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int pair = tid + i * THREADS;
+    hits[i] = 0u;
+    if (pair < PAIRS_OF_READERS && place.most[pair] >= reached) {
+#pragma unroll
+      for (int g = 0; g < SLOTS; ++g) {
+        if (g >= slots) continue;
+        const uint32_t both = *reinterpret_cast<const uint32_t*>(&place.groups[g][2 * pair]);
+        hits[i] |= ((both & 0xffffu) >= (reached >> 16) ? 1u << (2 * g) : 0u) | ((both >> 16) >= (reached >> 16) ? 2u << (2 * g) : 0u);
+      }
+    }
+    mine += uint32_t(__popc(hits[i]));
+  }
+  if (__any_sync(0xffffffffu, mine != 0u)) {
+    uint32_t at = places_for(mine, &s.n_chosen, lane);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      for (uint32_t left = hits[i]; left != 0u; left &= left - 1u, ++at) {
+        const int bit = __ffs(int(left)) - 1;
+        if (at < uint32_t(MOST_CHOSEN)) s.chosen[at] = uint16_t((bit >> 1) * READERS + 2 * (tid + i * THREADS) + (bit & 1));
+      }
+    }
+  }
+  choosers_meet<THREADS>(s.team);
+  released();
+  const bool fits = s.n_chosen <= uint32_t(MOST_CHOSEN);
+  if (fits) {
+    // their pieces again, a piece a thread, several on their way
+    const int pieces = int(s.n_chosen) << (shift + 2);
+    constexpr int WAY = 2;
+    const T least = value_from<T>(reached);
+#pragma unroll 1
+    for (int p0 = 0; p0 < pieces; p0 += WAY * THREADS) {
+      uint4 raw[WAY];
+      int at[WAY];
+      uint32_t found = 0u;   // elements that reach it
+#pragma unroll
+      for (int i = 0; i < WAY; ++i) {
+        const int piece = p0 + tid + i * THREADS;
+        at[i] = row.n;
+        if (piece < pieces) {
+          const uint32_t group = s.chosen[piece >> (shift + 2)];
+          at[i] = ((int(group / READERS) << (shift + 2)) + (piece & ((DEPTH << shift) - 1))) * READERS + int(group % READERS);
+        }
+        if (at[i] < row.n) raw[i] = load_once(row.x, row.g0 + at[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < WAY; ++i) {
+        if (at[i] >= row.n) continue;
+        const int first = row.x.first(row.g0 + at[i]);
+        uint32_t bits = reaching(raw[i], least);
+        if (first < 0) bits &= ~0u << -first;
+        if (first + PER > a.vocab) bits &= (1u << (a.vocab - first)) - 1u;
+        found |= bits << (i * PER);
+      }
+      if (!__any_sync(0xffffffffu, found != 0u)) continue;
+      uint32_t to = places_for(uint32_t(__popc(found)), &s.n_found, lane);
+#pragma unroll 1
+      for (; found != 0u; found &= found - 1u, ++to) {   // (few of a thread: their words are picked out of its registers)
+        const int bit = __ffs(int(found)) - 1, i = bit / PER, e = bit % PER, w = e * 4 / PER;
+        uint4 piece = raw[0];
+        int from = at[0];
+#pragma unroll
+        for (int o = 1; o < WAY; ++o) {
+          if (o == i) {
+            piece = raw[o];
+            from = at[o];
+          }
+        }
+        const uint32_t word = (w & 2) ? ((w & 1) ? piece.w : piece.z) : ((w & 1) ? piece.y : piece.x);
+        const float v = __uint_as_float(PER == 4 ? word : (e & 1) ? word & 0xffff0000u : word << 16);
+        if (to < uint32_t(CAP)) s.found[to] = composite(logit_key(v), row.x.first(row.g0 + from) + e);
+      }
+    }
+  }
+  choosers_meet<THREADS>(s.team);
+  if (!fits || s.n_found > uint32_t(CAP)) go_over<T, THREADS>(s, row, k, reached, tid);
+  if (s.n_found < uint32_t(k)) go_over<T, THREADS>(s, row, k, 0u, tid);   // (fewer than k numbers that are not NaN)
+
+  // runs of 32 from the largest down, filled up with 0
+  unsigned long long* list = s.found;
+  int n = (int(s.n_found) + 31) / 32 * 32;
+  for (int i = tid; i < n; i += THREADS) list[i] = sorted(i < int(s.n_found) ? list[i] : 0ull, lane);
+  choosers_meet<THREADS>(s.team);
+  // what stands at place `above` of them all: f(above, candidate)
+  auto in_order = [&](auto&& f) {
+    for (int i = tid; i < n; i += THREADS) {
+      const unsigned long long mine = list[i];
+      int above = 0;
+#pragma unroll 4
+      for (int run = 0; run < n; run += 32) above += above_in(list + run, mine);
+      if (mine != 0ull && above < a.k) f(above, mine);
+    }
+  };
+  if (THREADS == READERS && a.ranks > 1) {
+    unsigned long long* sent = reinterpret_cast<unsigned long long*>(&shared.places[1]);   // by the other CTAs, MOST_K places each
+    cluster_wait();   // (the first CTA runs)
+    const uint32_t to = cluster_address(sent, 0) + uint32_t(max(0, rank - 1) * MOST_K) * 8u;
+    auto send = [&](int at, unsigned long long v) {
+      if (rank > 0) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + uint32_t(at) * 8u), "l"(v) : "memory");
+      else reinterpret_cast<unsigned long long*>(&shared.teams[0])[at] = v;
+    };
+    if (n <= MOST_K) {
+      for (int i = tid; i < n; i += THREADS) send(i, list[i]);
+    } else {   // the first k of them, in order
+      in_order(send);
+      n = (k + 31) / 32 * 32;
+      if (tid < n - k) send(k + tid, 0ull);
+    }
+    if (tid == 32) {
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_address(s.n_of, 0) + uint32_t(rank) * 4u), "r"(uint32_t(n)) : "memory");
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_address(s.rank_sums, 0) + uint32_t(rank) * 8u), "f"(common), "f"(total) : "memory");
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (rank > 0) return;
+    if (warp == 1) {
+      const float2 part = lane < a.ranks ? s.rank_sums[lane] : make_float2(-INFINITY, 0.f);
+      common = warp_max(part.x);
+      total = warp_sum(part.y * rebase(part.x, common));
+      write_sum();
+    }
+    list = reinterpret_cast<unsigned long long*>(&shared.teams[0]);
+    static_assert(READERS >= MOST_K, "one of a CTA's candidates a thread");
+#pragma unroll 1
+    for (int q = 1; q < a.ranks; ++q) {
+      const int count = int(s.n_of[q]);
+      if (tid < count) list[n + tid] = sent[(q - 1) * MOST_K + tid];
+      n += count;
+    }
+    choosers_meet<THREADS>(s.team);
+  }
+  float* values = a.values + (long long)r * a.k;
+  int32_t* ids = a.ids + (long long)r * a.k;
+  in_order([&](int at, unsigned long long entry) {
+    values[at] = value_of(uint32_t(entry >> 32));
+    ids[at] = int32_t(0xffffffffu - uint32_t(entry & 0xffffffffull));
+  });
 }
 
 template <typename T>
 __global__ void __launch_bounds__(READERS + TEAMS * CHOOSERS, 1)
 top_kernel(const TopArgs a) {
-  constexpr int PER = RowPieces<T>::PER;
   extern __shared__ __align__(16) uint8_t top_smem[];
   TopShared& shared = *reinterpret_cast<TopShared*>(top_smem);
   pdl_launch_dependents();
+  if (a.ranks > 1) cluster_arrive();   // (waited for before anything is sent)
   const int ranks = a.ranks, step = int(gridDim.x) / ranks, rank = int(blockIdx.x) % ranks, first_row = int(blockIdx.x) / ranks;
-  const float c = 1.44269504f / a.tau;
   auto share_of = [&](int r) {
     Row<T> row = {RowPieces<T>(static_cast<const T*>(a.logits) + (long long)r * a.ld, a.vocab), rank * a.per, 0};
     row.n = max(0, min(a.per, row.x.count - row.g0));
@@ -407,231 +678,38 @@ top_kernel(const TopArgs a) {
   const int most_rounds = (a.per + READERS * DEPTH - 1) / (READERS * DEPTH);
   int shift = 0;   // a group is 2^shift rounds
   while ((SLOTS << shift) < most_rounds) ++shift;
-  pdl_wait();
 
   if (threadIdx.x < READERS) {
     const int tid = int(threadIdx.x);
-    read_shares<T>(shared, share_of, first_row, a.rows, step, shift, c, tid);
-    if (ranks > 1) {  // (one row to a cluster: the choosers' two barriers)
-      cluster_arrive();
-      cluster_wait();
-      cluster_arrive();
-      cluster_wait();
+    Shared& s = shared.teams[TEAMS];
+    if (tid == 0) {
+      s.team = TEAMS;
+      s.n_found = s.n_chosen = s.above = 0u;
     }
+    pdl_wait();
+    const int turn = read_shares<T>(shared, share_of, first_row, a.rows, step, shift, 1.44269504f / a.tau, tid), r = first_row + turn * step;
+    choosers_meet<READERS>(TEAMS);
+    choose<T, READERS>(a, shared, s, shared.places[turn % PLACES], share_of(r), r, shift, rank, tid, [] {});
     return;
   }
 
-  const int team = (int(threadIdx.x) - READERS) / CHOOSERS, tid = (int(threadIdx.x) - READERS) % CHOOSERS, lane = tid & 31;
+  const int team = (int(threadIdx.x) - READERS) / CHOOSERS, tid = (int(threadIdx.x) - READERS) % CHOOSERS;
   Shared& s = shared.teams[team];
-  if (tid == 0) s.team = team;
-  if (team > 0 && ranks > 1) {  // (one row to a cluster, the first team's)
-    cluster_arrive();
-    cluster_wait();
-    cluster_arrive();
-    cluster_wait();
-    return;
-  }
-  for (int r = first_row + team * step, turn = team; r < a.rows; r += TEAMS * step, turn += TEAMS) {
-    const Row<T> row = share_of(r);
-    const int p = turn % PLACES, rounds = (row.n + READERS * DEPTH - 1) / (READERS * DEPTH), slots = (rounds + (1 << shift) - 1) >> shift;
-    Place& place = shared.places[p];
-    const int first_token = max(0, row.x.first(row.g0)), end_token = min(a.vocab, row.x.first(row.g0) + row.n * PER);
-    const int k = min(a.k, end_token - first_token);   // of this share
-    choosers_meet(team);   // (the row before has been written out)
+  if (tid == 0 && ranks == 1) s.team = team;
+  pdl_wait();
+  for (int r = first_row + team * step, turn = team; r + step < a.rows; r += TEAMS * step, turn += TEAMS) {
+    const int p = turn % PLACES;
+    choosers_meet<CHOOSERS>(team);   // (the row before has been written out)
     if (tid == 0) s.n_found = s.n_chosen = s.above = 0u;
     wait_full(p);
-    float2 part = lane < READING_WARPS ? place.sums[lane] : make_float2(-INFINITY, 0.f);
-    float common = warp_max(part.x), total = warp_sum(part.y * rebase(part.x, common));
-    uint32_t reached = 0u;
-    bool fits = true;
-    if (row.n >= READERS) {   // a group for every reader
-      // what k pairs' maxima or a few more reach, by halving, in every warp for itself
-      constexpr int OWN = PAIRS_OF_READERS / 32;
-      uint32_t most[OWN], low = 0xffffffffu, high = 0u;
-#pragma unroll
-      for (int i = 0; i < OWN; ++i) {
-        most[i] = place.most[lane + i * 32];
-        low = min(low, most[i]);
-        high = max(high, most[i]);
-      }
-      low = __reduce_min_sync(0xffffffffu, low);
-      high = __reduce_max_sync(0xffffffffu, high);
-      const int enough = k + max(8, k / 8);
-      while (low < high) {
-        const uint32_t middle = low + (high - low) / 2 + 1;
-        int reach = 0;
-#pragma unroll
-        for (int i = 0; i < OWN; ++i) reach += most[i] >= middle ? 1 : 0;
-        reach = __reduce_add_sync(0xffffffffu, reach);
-        if (reach >= k) low = middle;
-        else high = middle - 1;
-        if (reach >= k && reach <= enough) break;
-      }
-      reached = low;
-      // the groups that reach it
-#pragma unroll
-      for (int i = 0; i < PAIRS_OF_READERS / CHOOSERS; ++i) {
-        const int pair = tid + i * CHOOSERS;
-        if (place.most[pair] < reached) continue;
-        uint2 both[SLOTS];
-#pragma unroll
-        for (int g = 0; g < SLOTS; ++g) both[g] = g < slots ? *reinterpret_cast<const uint2*>(&place.groups[g][2 * pair]) : make_uint2(0u, 0u);
-#pragma unroll
-        for (int g = 0; g < SLOTS; ++g) {
-          if (g < slots && both[g].x >= reached) {
-            const uint32_t at = atomicAdd(&s.n_chosen, 1u);
-            if (at < uint32_t(BINS)) s.chosen[at] = uint32_t(g * READERS + 2 * pair);
-          }
-          if (g < slots && both[g].y >= reached) {
-            const uint32_t at = atomicAdd(&s.n_chosen, 1u);
-            if (at < uint32_t(BINS)) s.chosen[at] = uint32_t(g * READERS + 2 * pair + 1);
-          }
-        }
-      }
-      choosers_meet(s.team);
+    choose<T, CHOOSERS>(a, shared, s, shared.places[p], share_of(r), r, shift, rank, tid, [&] {
       if (r + PLACES * step < a.rows) say_empty(p);
-      fits = s.n_chosen <= uint32_t(BINS);
-      if (fits) {
-        // their pieces again, a piece a thread, several on their way
-        const int pieces = int(s.n_chosen) << (shift + 2);
-        constexpr int WAY = 4;
-        const float reached_value = value_of(reached);
-#pragma unroll 1
-        for (int p0 = tid; p0 < pieces; p0 += WAY * CHOOSERS) {
-          uint4 raw[WAY];
-          int at[WAY];
-#pragma unroll
-          for (int i = 0; i < WAY; ++i) {
-            const int piece = p0 + i * CHOOSERS;
-            at[i] = row.n;
-            if (piece < pieces) {
-              const uint32_t group = s.chosen[piece >> (shift + 2)];
-              at[i] = ((int(group / READERS) << (shift + 2)) + (piece & ((DEPTH << shift) - 1))) * READERS + int(group % READERS);
-            }
-            if (at[i] < row.n) raw[i] = row.load(at[i]);
-          }
-#pragma unroll
-          for (int i = 0; i < WAY; ++i) {
-            if (at[i] >= row.n) continue;
-            float v[PER];
-            unpack(raw[i], v, static_cast<const T*>(nullptr));
-#pragma unroll
-            for (int e = 0; e < PER; ++e) {
-              if (!(v[e] >= reached_value)) continue;
-              const int token = row.x.first(row.g0 + at[i]) + e;
-              if (!row.inside(token)) continue;
-              const uint32_t place = atomicAdd(&s.n_found, 1u);
-              if (place < uint32_t(CAP)) s.found[place] = composite(logit_key(v[e]), token);
-            }
-          }
-        }
-      }
-    } else {   // a short share: everything is a candidate, or too many for the list
-      choosers_meet(s.team);
-      if (r + PLACES * step < a.rows) say_empty(p);
-      if (tid == 0) s.n_found = uint32_t(end_token - first_token);
-      if (end_token - first_token <= CAP) {
-        for (int at = tid; at < row.n; at += CHOOSERS) {
-          float v[PER];
-          unpack(row.load(at), v, static_cast<const T*>(nullptr));
-#pragma unroll
-          for (int e = 0; e < PER; ++e) {
-            const int token = row.x.first(row.g0 + at) + e;
-            if (row.inside(token)) s.found[token - first_token] = composite(logit_key(v[e]), token);
-          }
-        }
-      }
-    }
-    choosers_meet(s.team);
-    if (!fits || s.n_found > uint32_t(CAP)) go_over(s, row, k, reached, tid);
-    if (s.n_found < uint32_t(k)) go_over(s, row, k, 0u, tid);   // (fewer than k numbers that are not NaN)
-
-    // the cluster's candidates into its first CTA
-    int n = int(s.n_found);
-    if (ranks > 1) {
-      if (n > MOST_SORTED / MOST_RANKS) {   // (more than the first CTA has places for from each: the exact k)
-        go_over(s, row, k, reached, tid);
-        n = k;
-      }
-      cluster_arrive();   // the first CTA has what it found itself in the first of its places, the others are free
-      cluster_wait();
-      const uint32_t found = cluster_address(s.found, 0), counts = cluster_address(s.n_of, 0), sums = cluster_address(s.rank_sums, 0);
-      if (rank > 0)
-        for (int i = tid; i < n; i += CHOOSERS)
-          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(found + uint32_t(rank * (MOST_SORTED / MOST_RANKS) + i) * 8u), "l"(s.found[i]) : "memory");
-      if (tid == 0) {
-        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(counts + uint32_t(rank) * 4u), "r"(uint32_t(n)) : "memory");
-        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(sums + uint32_t(rank) * 8u), "f"(common), "f"(total) : "memory");
-      }
-      cluster_arrive();
-      cluster_wait();
-      if (rank > 0) return;
-      part = lane < ranks ? s.rank_sums[lane] : make_float2(-INFINITY, 0.f);
-      common = warp_max(part.x);
-      total = warp_sum(part.y * rebase(part.x, common));
-      int all = n;   // close the gaps
-      for (int q = 1; q < ranks; ++q) {
-        const int count = int(s.n_of[q]), from = q * (MOST_SORTED / MOST_RANKS);
-        constexpr int EACH = MOST_SORTED / MOST_RANKS / CHOOSERS;
-        unsigned long long keep[EACH];
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) keep[i] = tid + i * CHOOSERS < count ? s.found[from + tid + i * CHOOSERS] : 0ull;
-        choosers_meet(s.team);
-#pragma unroll
-        for (int i = 0; i < EACH; ++i)
-          if (tid + i * CHOOSERS < count) s.found[all + tid + i * CHOOSERS] = keep[i];
-        all += count;
-      }
-      choosers_meet(s.team);
-      n = all;
-    }
-    if (tid == 0) a.log_sum[r] = (no_less(common) + log2f(total)) * 0.693147181f;
-
-    float* values = a.values + (long long)r * a.k;
-    int32_t* ids = a.ids + (long long)r * a.k;
-    if (n <= 4 * CHOOSERS) {
-      // a candidate's place: how many stand above it
-      if ((n & 1) && tid == 0) s.found[n] = 0ull;
-      choosers_meet(s.team);
-      for (int i = tid; i < n; i += CHOOSERS) {
-        const unsigned long long mine = s.found[i];
-        int above = 0, also = 0;
-#pragma unroll 4
-        for (int j = 0; j < n; j += 2) {
-          const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(s.found + j);   // (behind the last one stands a 0)
-          above += two.x > mine ? 1 : 0;
-          also += two.y > mine ? 1 : 0;
-        }
-        above += also;
-        if (above < a.k) {
-          values[above] = value_of(uint32_t(mine >> 32));
-          ids[above] = int32_t(0xffffffffu - uint32_t(mine & 0xffffffffull));
-        }
-      }
-      continue;
-    }
-    // many candidates: sorted in place (bitonic, from the largest down)
-    int size = 4 * CHOOSERS;
-    while (size < n) size *= 2;
-    for (int i = n + tid; i < size; i += CHOOSERS) s.found[i] = 0ull;
-    choosers_meet(s.team);
-    for (int run = 2; run <= size; run *= 2) {
-      for (int apart = run / 2; apart > 0; apart /= 2) {
-        for (int i = tid; i < size / 2; i += CHOOSERS) {
-          const int lo = 2 * i - (i & (apart - 1)), hi = lo + apart;
-          const unsigned long long x = s.found[lo], y = s.found[hi];
-          if ((x < y) == ((lo & run) == 0)) {
-            s.found[lo] = y;
-            s.found[hi] = x;
-          }
-        }
-        choosers_meet(s.team);
-      }
-    }
-    for (int i = tid; i < a.k; i += CHOOSERS) {
-      values[i] = value_of(uint32_t(s.found[i] >> 32));
-      ids[i] = int32_t(0xffffffffu - uint32_t(s.found[i] & 0xffffffffull));
-    }
+    });
+  }
+  if (ranks > 1) {  // (one row to a cluster: its readers' barriers)
+    cluster_wait();
+    cluster_arrive();
+    cluster_wait();
   }
 }
 

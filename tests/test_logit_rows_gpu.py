@@ -252,6 +252,19 @@ def test_top_logits_of_many_rows_some_of_equal_values(dtype):
     assert torch.equal(ids.long(), order) and torch.equal(values, torch.gather(x.float(), 1, order))
 
 
+@pytest.mark.parametrize("rows", [2, 37, 400])
+@pytest.mark.parametrize("vocab,k", [(1300, 256), (2049, 129), (2561, 256), (5120, 200), (10241, 256), (40001, 256), (90003, 256)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_top_logits_of_many_candidates(rows, vocab, k, dtype):
+    """Long lists, whose candidates fill many runs, from one row over several CTAs to several rows a CTA; every third row has few values."""
+    x = random_logits(rows, vocab, vocab + rows)
+    x[::3] = torch.round(x[::3] * 4)
+    x = rows_at(x, dtype, 1, 2)
+    values, ids, _ = ops().top_logits(x, k)
+    order = torch.argsort(x.float(), dim=1, descending=True, stable=True)[:, :k]
+    assert torch.equal(ids.long(), order) and torch.equal(values, torch.gather(x.float(), 1, order))
+
+
 @pytest.mark.parametrize("order", ["rising", "falling"])
 def test_top_logits_of_rows_in_order(order):
     x = torch.linspace(-20, 20, 50257)[None].repeat(2, 1)
