@@ -15,16 +15,20 @@
 // next one passes. Behind a CTA's last row nothing passes any more, and its readers choose it themselves. Few rows are cut over the CTAs of
 // a cluster, whose candidates meet in the first one's shared memory.
 #include "logit_rows.cuh"
+#include "sm100_ptx.cuh"
+
+#define R2_ERR_TIMEOUT_ROUND 9
 
 namespace {
 
-constexpr int READERS = 640, PAIRS_OF_READERS = READERS / 2, READING_WARPS = READERS / 32;
-constexpr int CHOOSERS = 128, TEAMS = 2;   // of a team
+constexpr int READERS = 512, READING_WARPS = READERS / 32;
+constexpr int CHOOSERS = 160, TEAMS = 2;   // of a team
 // Rows that are between reading and choosing. A place is always the same team's: with a place that changed teams, one that is ahead of the
 // other would take the readers' word for the other's row as its own.
 constexpr int PLACES = 2 * TEAMS;
 constexpr int MOST_K = 256, MOST_RANKS = 8;
 constexpr int DEPTH = 4;      // pieces of a group
+constexpr int STAGES = 3;     // rounds on their way
 constexpr int SLOTS = 8;      // groups of a thread (of several rounds each in long rows)
 constexpr int CAP = 1536;     // candidates
 constexpr int MOST_CHOSEN = 1024, BINS = 512;
@@ -34,12 +38,13 @@ struct TopArgs {
   int rows, vocab, k, ranks, per;
   float tau;
   float* values; int32_t* ids; float* log_sum;
+  int* error;
 };
 
 // From those who read to those who choose.
 struct __align__(16) Place {
-  uint16_t groups[SLOTS][READERS];        // the groups' maxima: the upper halves of their keys
-  uint32_t most[PAIRS_OF_READERS];        // the maxima of pairs of threads, as keys
+  uint16_t groups[SLOTS][READERS];        // the groups' maxima, rounded down to bfloat16
+  uint16_t most[READERS];                 // the threads'
   float2 sums[READING_WARPS];             // the warps' references and sums
 };
 // A team's own.
@@ -55,15 +60,16 @@ struct __align__(16) Shared {
   uint32_t n_of[MOST_RANKS];
   int team;
 };
-// (Shared memory is missing to L1, which holds what loads have on their way: with 220 KB of it instead of 91 a pass took a quarter longer.)
 struct TopShared {
+  uint4 rounds[STAGES][READERS * DEPTH];   // a share's pieces, copied
   Place places[PLACES];
   Shared teams[TEAMS + 1];   // the last one: the readers'
+  uint64_t full[STAGES], empty[STAGES];
 };
 // Clusters have one row, the readers': what they send each other stands in the other places, what the first CTA puts together in the teams'.
 static_assert((MOST_RANKS - 1) * MOST_K * sizeof(unsigned long long) <= (PLACES - 1) * sizeof(Place), "");
 static_assert(MOST_RANKS * MOST_K * sizeof(unsigned long long) <= TEAMS * sizeof(Shared), "");
-static_assert(SLOTS * READERS <= 65536 && PAIRS_OF_READERS >= MOST_K && PAIRS_OF_READERS < 1024, "");
+static_assert(SLOTS * READERS <= 65536 && READERS >= MOST_K && READERS < 1024 && 2 * SLOTS <= 16, "");
 
 template <int ID, int COUNT> __device__ __forceinline__ void bar_sync() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(COUNT) : "memory"); }
 template <int ID, int COUNT> __device__ __forceinline__ void bar_arrive() { asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(COUNT) : "memory"); }
@@ -118,21 +124,25 @@ __device__ __forceinline__ unsigned long long composite(uint32_t key, int token)
   return (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - uint32_t(token));
 }
 
-// The least value of the type that reaches a key.
-template <typename T> __device__ __forceinline__ T value_from(uint32_t key);
-template <> __device__ __forceinline__ float value_from<float>(uint32_t key) { return value_of(key); }
-template <> __device__ __forceinline__ bf16 value_from<bf16>(uint32_t key) { return __float2bfloat16_ru(value_of(key)); }
+__device__ __forceinline__ uint32_t floor_bits(float v) { return uint32_t(__bfloat16_as_ushort(__float2bfloat16_rd(v))); }
+// bfloat16 bits as 16-bit keys in the numbers' order, and back
+__device__ __forceinline__ uint32_t short_key(uint32_t bits) { return (bits & 0x8000u) ? ~bits & 0xffffu : bits | 0x8000u; }
+__device__ __forceinline__ __nv_bfloat162 both_of(uint32_t key) {
+  const uint32_t bits = (key & 0x8000u) ? key & 0x7fffu : ~key & 0xffffu;
+  return __bfloat162bfloat162(__ushort_as_bfloat16(static_cast<unsigned short>(bits)));
+}
+__device__ __forceinline__ __nv_bfloat162 as_two(uint32_t word) { return *reinterpret_cast<const __nv_bfloat162*>(&word); }
 // A piece's elements that are not less than `least`, as bits.
-__device__ __forceinline__ uint32_t reaching(const uint4& raw, float least) {
+__device__ __forceinline__ uint32_t reaching(const uint4& raw, __nv_bfloat162 both, const float*) {
+  const float least = __low2float(both);
   return (__uint_as_float(raw.x) >= least ? 1u : 0u) | (__uint_as_float(raw.y) >= least ? 2u : 0u) | (__uint_as_float(raw.z) >= least ? 4u : 0u) |
          (__uint_as_float(raw.w) >= least ? 8u : 0u);
 }
-__device__ __forceinline__ uint32_t reaching(const uint4& raw, bf16 least) {
-  const __nv_bfloat162 both = __bfloat162bfloat162(least);
+__device__ __forceinline__ uint32_t reaching(const uint4& raw, __nv_bfloat162 both, const bf16*) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
   uint32_t bits = 0u;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) bits |= __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[j]), both) & (0x00020001u << (2 * j));
+  for (int j = 0; j < 4; ++j) bits |= __hge2_mask(as_two(w[j]), both) & (0x00020001u << (2 * j));
   return (bits | bits >> 16) & 0xffu;
 }
 
@@ -306,59 +316,89 @@ __device__ __noinline__ void go_over(Shared& s, const Row<T>& row, int k, uint32
   choosers_meet<THREADS>(s.team);
 }
 
-// What a CTA's readers do: shares of rows, round after round, the pieces of the two rounds behind the one in hand on their way, over the rows'
-// ends too. Of every share its groups' and pairs' maxima and its warps' sums. -> the turn of the last one.
+// What a CTA's bringing thread does: shares of rows, round after round, over the rows' ends too, into the stages that have been read.
 template <typename T, typename ShareOf>
-__device__ __forceinline__ int read_shares(TopShared& shared, const ShareOf& share_of, int first_row, int rows, int step, int shift, float c, int tid) {
+__device__ __forceinline__ void bring_shares(TopShared& shared, const ShareOf& share_of, int first_row, int rows, int step, int* error) {
+  constexpr int ROUND = READERS * DEPTH;
+  int n = 0;
+  for (int r = first_row; r < rows; r += step) {
+    const Row<T> row = share_of(r);
+    const uint4* from = reinterpret_cast<const uint4*>(row.x.base) + row.g0;
+    for (int left = row.n; left > 0; left -= ROUND, from += ROUND, ++n) {
+      const int stage = n % STAGES;
+      if (n >= STAGES && !r2ptx::mbar_wait(r2ptx::smem_u32(&shared.empty[stage]), uint32_t(n / STAGES - 1) & 1u)) {
+        atomicMax(error, R2_ERR_TIMEOUT_ROUND);
+        return;
+      }
+      const uint32_t bytes = uint32_t(min(left, ROUND)) * 16u, barrier = r2ptx::smem_u32(&shared.full[stage]);
+      r2ptx::mbar_expect_tx(barrier, bytes);
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       r2ptx::smem_u32(shared.rounds[stage])), "l"(from), "r"(bytes), "r"(barrier)
+                   : "memory");
+    }
+  }
+}
+
+// (Out of the loop's way. The place's next copy comes by another path than what is written here.)
+template <typename T>
+__device__ __noinline__ void blank_in(uint4& place, const RowPieces<T>& x, int g) {
+  uint4 piece = place;
+  blank_outside(piece, x, g);
+  place = piece;
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// What its readers do. Of every share its groups' and pairs' maxima and its warps' sums. -> the turn of the last one.
+template <typename T, typename ShareOf>
+__device__ __forceinline__ int read_shares(TopShared& shared, const ShareOf& share_of, int first_row, int rows, int step, int shift, float c, int tid,
+                                           int* error) {
   constexpr int PAIRS = RowPieces<T>::PER / 2, ROUND = READERS * DEPTH;
   const int together = 1 << shift;
   const uint64_t cc = two_of(c, c);
-  // the round that is asked for next, and the pieces from its first one on
-  int next_row = first_row, next_left = 0;
-  const uint4* from = nullptr;
-  auto open = [&]() {
-    if (next_row >= rows) return;
-    const Row<T> row = share_of(next_row);
-    next_left = row.n;
-    from = reinterpret_cast<const uint4*>(row.x.base) + row.g0 + tid;
-  };
-  open();
-  auto ask = [&](uint4 (&raw)[DEPTH]) {
-    if (next_row >= rows) return;
-    if (next_left > ROUND) {
-#pragma unroll
-      for (int i = 0; i < DEPTH; ++i) raw[i] = load_16(from + i * READERS);
-      from += ROUND;
-      next_left -= ROUND;
-    } else {
-#pragma unroll
-      for (int i = 0; i < DEPTH; ++i) load_16_if(raw[i], from + i * READERS, i * READERS + tid < next_left);
-      next_row += step;
-      open();
-    }
-  };
+  uint32_t stage = 0u, phase = 0u;
+  bool lost = false;
   // the round in hand
   int r = first_row, left = 0, turn = 0, slot = 0, until = together;   // left: pieces from its first one on; until: rounds that the slot still takes
   float reference = -INFINITY, sum = 0.f;
-  uint32_t pair_max = 0u, slot_max = 0u;
-  auto take = [&](uint4 (&raw)[DEPTH]) {
+  float row_max = -INFINITY, slot_max = -INFINITY;
+#pragma unroll 1
+  while (r < rows) {
     Place& place = shared.places[turn % PLACES];
+    bool begins = false;
     if (left == 0) {
       const Row<T> row = share_of(r);
       left = row.n;
-      if (row.g0 == 0 && tid == 0) blank_outside(raw[0], row.x, 0);
+      begins = row.g0 == 0;
       if (turn >= PLACES) wait_empty(turn % PLACES);
     }
     const bool last = left <= ROUND;
     const int end = left - 1 - tid;   // the share's last piece is this thread's i-th where i * READERS == end
-    if (last) {
+    if (!lost && !r2ptx::mbar_wait(r2ptx::smem_u32(&shared.full[stage]), phase)) {
+      lost = true;
+      atomicMax(error, R2_ERR_TIMEOUT_ROUND);
+    }
+    if (begins && tid == 0) blank_in(shared.rounds[stage][0], share_of(r).x, 0);   // the ends of the row
+    if (last && end >= 0 && end % READERS == 0) {
       const Row<T> row = share_of(r);
+      if (row.g0 + row.n == row.x.count) blank_in(shared.rounds[stage][left - 1], row.x, row.x.count - 1);
+    }
+    uint4 raw[DEPTH];
+    if (!last) {
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) raw[i] = shared.rounds[stage][i * READERS + tid];
+    } else {
       const uint32_t nothing = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
       for (int i = 0; i < DEPTH; ++i) {
-        if (i * READERS > end) raw[i] = make_uint4(nothing, nothing, nothing, nothing);
-        else if (i * READERS == end && row.g0 + row.n == row.x.count) blank_outside(raw[i], row.x, row.x.count - 1);
+        raw[i] = make_uint4(nothing, nothing, nothing, nothing);
+        if (i * READERS <= end) raw[i] = shared.rounds[stage][i * READERS + tid];
       }
+    }
+    __syncwarp();
+    if ((tid & 31) == 0) r2ptx::mbar_arrive(r2ptx::smem_u32(&shared.empty[stage]));
+    if (++stage == STAGES) {
+      stage = 0u;
+      phase ^= 1u;
     }
     const float most = largest<T, DEPTH>(raw), up = fminf(most * c, 3e38f);   // (an infinity sums to infinity against any number)
     if (up > reference) {
@@ -388,18 +428,17 @@ __device__ __forceinline__ int read_shares(TopShared& shared, const ShareOf& sha
     }
     const float2 both = halves(acc);
     sum += both.x + both.y;
-    slot_max = max(slot_max, logit_key(most));
+    slot_max = fmaxf(slot_max, most);
     if (--until == 0 || last) {
-      place.groups[slot][tid] = uint16_t(slot_max >> 16);
-      pair_max = max(pair_max, slot_max);
-      slot_max = 0u;
+      place.groups[slot][tid] = uint16_t(floor_bits(slot_max));
+      row_max = fmaxf(row_max, slot_max);
+      slot_max = -INFINITY;
       ++slot;
       until = together;
     }
     left -= ROUND;
-    if (!last) return;
-    pair_max = max(pair_max, __shfl_xor_sync(0xffffffffu, pair_max, 1));
-    if ((tid & 1) == 0) place.most[tid >> 1] = pair_max;
+    if (!last) continue;
+    place.most[tid] = uint16_t(floor_bits(row_max));
     const float common = warp_max(reference);
     sum = warp_sum(sum * rebase(reference, common));
     if ((tid & 31) == 0) place.sums[tid >> 5] = make_float2(common, sum);
@@ -407,20 +446,9 @@ __device__ __forceinline__ int read_shares(TopShared& shared, const ShareOf& sha
     if (r < rows) say_full(turn % PLACES);   // (the last one is the readers' own)
     reference = -INFINITY;
     sum = 0.f;
-    pair_max = 0u;
+    row_max = -INFINITY;
     left = slot = 0;
     ++turn;
-  };
-  uint4 one[DEPTH] = {}, two[DEPTH] = {};
-  ask(one);
-  ask(two);
-#pragma unroll 1
-  while (r < rows) {
-    take(one);
-    ask(one);
-    if (r >= rows) break;
-    take(two);
-    ask(two);
   }
   return turn - 1;
 }
@@ -476,25 +504,32 @@ __device__ __forceinline__ void choose(const TopArgs& a, TopShared& shared, Shar
     total = warp_sum(part.y * rebase(part.x, common));
     if (a.ranks == 1) write_sum();
   }
-  // what k pairs' maxima or a few more reach, three values tried at a time (their counts in ten bits each)
+  // what k threads' maxima or a few more reach, three values tried at a time (their counts in ten bits each)
+  const uint32_t* most = reinterpret_cast<const uint32_t*>(place.most);
   if (warp == 0) {
-    constexpr int OWN = PAIRS_OF_READERS / 32;
-    uint32_t most[OWN], low = 0xffffffffu, high = 0u;
+    constexpr int OWN = READERS / 64;   // pairs
+    __nv_bfloat162 own[OWN], least, largest;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
-      most[i] = place.most[lane + i * 32];
-      low = min(low, most[i]);
-      high = max(high, most[i]);
+      own[i] = as_two(most[lane + i * 32]);
+      least = i == 0 ? own[i] : __hmin2(least, own[i]);
+      largest = i == 0 ? own[i] : __hmax2(largest, own[i]);
     }
-    low = __reduce_min_sync(0xffffffffu, low);
-    high = __reduce_max_sync(0xffffffffu, high);
+    least = __halves2bfloat162(__hmin(__low2bfloat16(least), __high2bfloat16(least)), __hmax(__low2bfloat16(largest), __high2bfloat16(largest)));
+    uint32_t low = __reduce_min_sync(0xffffffffu, short_key(__bfloat16_as_ushort(__low2bfloat16(least))));
+    uint32_t high = __reduce_max_sync(0xffffffffu, short_key(__bfloat16_as_ushort(__high2bfloat16(least))));
     const int enough = k + max(8, k / 8);
     while (low < high) {
       const uint32_t half = (high - low) / 2, one = low + half / 2 + 1, two = low + half + 1, three = two + half / 2;   // all in (low, high]
+      const __nv_bfloat162 of_key[3] = {both_of(one), both_of(two), both_of(three)};
       uint32_t reach = 0u;
 #pragma unroll
-      for (int i = 0; i < OWN; ++i)
-        reach += (most[i] >= one ? 1u : 0u) + (most[i] >= two ? 1u << 10 : 0u) + (most[i] >= three ? 1u << 20 : 0u);
+      for (int t = 0; t < 3; ++t) {
+        __nv_bfloat162 count = __hge2(own[0], of_key[t]);
+#pragma unroll
+        for (int i = 1; i < OWN; ++i) count = __hadd2(count, __hge2(own[i], of_key[t]));
+        reach += uint32_t(__low2float(count) + __high2float(count)) << (10 * t);
+      }
       reach = __reduce_add_sync(0xffffffffu, reach);
       const int of_one = int(reach & 1023u), of_two = int((reach >> 10) & 1023u), of_three = int(reach >> 20);
       int of_low = 0;
@@ -517,21 +552,20 @@ __device__ __forceinline__ void choose(const TopArgs& a, TopShared& shared, Shar
     if (lane == 0) s.low = low;
   }
   choosers_meet<THREADS>(s.team);
-  const uint32_t reached = s.low;
+  const __nv_bfloat162 least = both_of(s.low);
+  const uint32_t reached = logit_key(__low2float(least));
   // the groups that reach it
-  constexpr int EACH = (PAIRS_OF_READERS + THREADS - 1) / THREADS;
+  constexpr int EACH = (READERS / 2 + THREADS - 1) / THREADS;
   uint32_t hits[EACH], mine = 0u;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int pair = tid + i * THREADS;
     hits[i] = 0u;
-    if (pair < PAIRS_OF_READERS && place.most[pair] >= reached) {
+    if (pair < READERS / 2 && __hge2_mask(as_two(most[pair]), least) != 0u) {
 #pragma unroll
-      for (int g = 0; g < SLOTS; ++g) {
-        if (g >= slots) continue;
-        const uint32_t both = *reinterpret_cast<const uint32_t*>(&place.groups[g][2 * pair]);
-        hits[i] |= ((both & 0xffffu) >= (reached >> 16) ? 1u << (2 * g) : 0u) | ((both >> 16) >= (reached >> 16) ? 2u << (2 * g) : 0u);
-      }
+      for (int g = 0; g < SLOTS; ++g)
+        if (g < slots) hits[i] |= __hge2_mask(as_two(reinterpret_cast<const uint32_t*>(place.groups[g])[pair]), least) & (0x00020001u << (2 * g));
+      hits[i] = (hits[i] | hits[i] >> 16) & 0xffffu;
     }
     mine += uint32_t(__popc(hits[i]));
   }
@@ -552,7 +586,6 @@ __device__ __forceinline__ void choose(const TopArgs& a, TopShared& shared, Shar
     // their pieces again, a piece a thread, several on their way
     const int pieces = int(s.n_chosen) << (shift + 2);
     constexpr int WAY = 2;
-    const T least = value_from<T>(reached);
 #pragma unroll 1
     for (int p0 = 0; p0 < pieces; p0 += WAY * THREADS) {
       uint4 raw[WAY];
@@ -572,7 +605,7 @@ __device__ __forceinline__ void choose(const TopArgs& a, TopShared& shared, Shar
       for (int i = 0; i < WAY; ++i) {
         if (at[i] >= row.n) continue;
         const int first = row.x.first(row.g0 + at[i]);
-        uint32_t bits = reaching(raw[i], least);
+        uint32_t bits = reaching(raw[i], least, static_cast<const T*>(nullptr));
         if (first < 0) bits &= ~0u << -first;
         if (first + PER > a.vocab) bits &= (1u << (a.vocab - first)) - 1u;
         found |= bits << (i * PER);
@@ -663,7 +696,7 @@ __device__ __forceinline__ void choose(const TopArgs& a, TopShared& shared, Shar
 }
 
 template <typename T>
-__global__ void __launch_bounds__(READERS + TEAMS * CHOOSERS, 1)
+__global__ void __launch_bounds__(READERS + TEAMS * CHOOSERS + 32, 1)
 top_kernel(const TopArgs a) {
   extern __shared__ __align__(16) uint8_t top_smem[];
   TopShared& shared = *reinterpret_cast<TopShared*>(top_smem);
@@ -679,21 +712,35 @@ top_kernel(const TopArgs a) {
   int shift = 0;   // a group is 2^shift rounds
   while ((SLOTS << shift) < most_rounds) ++shift;
 
-  if (threadIdx.x < READERS) {
-    const int tid = int(threadIdx.x);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      r2ptx::mbar_init(r2ptx::smem_u32(&shared.full[i]), 1u);
+      r2ptx::mbar_init(r2ptx::smem_u32(&shared.empty[i]), uint32_t(READING_WARPS));
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+
+  if (threadIdx.x >= TEAMS * CHOOSERS + 32) {
+    const int tid = int(threadIdx.x) - TEAMS * CHOOSERS - 32;
     Shared& s = shared.teams[TEAMS];
     if (tid == 0) {
       s.team = TEAMS;
       s.n_found = s.n_chosen = s.above = 0u;
     }
     pdl_wait();
-    const int turn = read_shares<T>(shared, share_of, first_row, a.rows, step, shift, 1.44269504f / a.tau, tid), r = first_row + turn * step;
+    const int turn = read_shares<T>(shared, share_of, first_row, a.rows, step, shift, 1.44269504f / a.tau, tid, a.error), r = first_row + turn * step;
     choosers_meet<READERS>(TEAMS);
     choose<T, READERS>(a, shared, s, shared.places[turn % PLACES], share_of(r), r, shift, rank, tid, [] {});
     return;
   }
 
-  const int team = (int(threadIdx.x) - READERS) / CHOOSERS, tid = (int(threadIdx.x) - READERS) % CHOOSERS;
+  const int team = int(threadIdx.x) / CHOOSERS, tid = int(threadIdx.x) % CHOOSERS;   // TEAMS: who brings
+  if (team == TEAMS) {
+    pdl_wait();
+    if (tid == 0) bring_shares<T>(shared, share_of, first_row, a.rows, step, a.error);
+    __syncwarp();
+  } else {
   Shared& s = shared.teams[team];
   if (tid == 0 && ranks == 1) s.team = team;
   pdl_wait();
@@ -705,6 +752,7 @@ top_kernel(const TopArgs a) {
     choose<T, CHOOSERS>(a, shared, s, shared.places[p], share_of(r), r, shift, rank, tid, [&] {
       if (r + PLACES * step < a.rows) say_empty(p);
     });
+  }
   }
   if (ranks > 1) {  // (one row to a cluster: its readers' barriers)
     cluster_wait();
@@ -724,7 +772,7 @@ int launch(TopArgs a, int rows, cudaStream_t stream) {
   const int status = allow_smem(top_kernel<T>, sizeof(TopShared), allowed);
   if (status != R2_OK) return status;
   const int walking = a.ranks > 1 ? rows : min(rows, 148);   // as many as run at a time
-  r2_launch_clusters(top_kernel<T>, a.ranks, dim3(unsigned(walking) * unsigned(a.ranks)), dim3(READERS + TEAMS * CHOOSERS), sizeof(TopShared), stream, a);
+  r2_launch_clusters(top_kernel<T>, a.ranks, dim3(unsigned(walking) * unsigned(a.ranks)), dim3(READERS + TEAMS * CHOOSERS + 32), sizeof(TopShared), stream, a);
   return launch_status();
 }
 
@@ -732,11 +780,11 @@ int launch(TopArgs a, int rows, cudaStream_t stream) {
 
 // logits [rows, vocab] of dtype with row stride ld -> values [rows, k] float, ids [rows, k], log_sum [rows].
 extern "C" int r2_top_logits(int dtype, const void* logits, long long ld, int rows, int vocab, int k, float temperature, float* values,
-                             int32_t* ids, float* log_sum, cudaStream_t stream) {
+                             int32_t* ids, float* log_sum, int* error, cudaStream_t stream) {
   if (dtype != R2_F32 && dtype != R2_BF16) return R2_BAD_DTYPE;
   if (rows < 0 || vocab < 1 || vocab > (1 << 30) || ld < vocab || k < 1 || k > vocab) return R2_BAD_SHAPE;
   if (k > MOST_K || !(temperature > 0.f)) return R2_UNSUPPORTED;
   if (rows == 0) return R2_OK;
-  const TopArgs a = {logits, ld, rows, vocab, k, 1, 0, temperature, values, ids, log_sum};
+  const TopArgs a = {logits, ld, rows, vocab, k, 1, 0, temperature, values, ids, log_sum, error};
   return dtype == R2_F32 ? launch<float>(a, rows, stream) : launch<bf16>(a, rows, stream);
 }

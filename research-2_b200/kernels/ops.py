@@ -39,6 +39,7 @@ class KernelTimeout(KernelError):
         6: "a stage of the tensor-core prefill attention did not complete",
         7: "a step of the resident decode kernel did not reach its grid barrier",
         8: "the sums of a row that CTAs share (distillation) did not arrive",
+        9: "a round of a row's logits did not arrive or was not read (top logits, bulk copy)",
         99: "a wait that a test let run out",
     }
 
@@ -1929,7 +1930,7 @@ TOP_MOST = 256   # the most logits of a row that top_logits returns and distill_
 _LOGIT_SIGNATURES = {
     "adjust_logits": [C.c_int, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int] +
                      [C.c_void_p] * 9 + [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p, C.c_void_p],
-    "top_logits": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
+    "top_logits": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float] + [C.c_void_p] * 5,
     "distill": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
                 C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p],
     "scale_rows": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p],
@@ -2097,7 +2098,7 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0):
     log_sum = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=where)
     if rows:
         _check(_logit_entry("top_logits")(code, logits.data_ptr(), ld, rows, vocab, k, temperature, values.data_ptr(), ids.data_ptr(),
-                                          log_sum.data_ptr(), _current_stream(device)), "top_logits")
+                                          log_sum.data_ptr(), _workspace(where).error.data_ptr(), _current_stream(device)), "top_logits")
     return values, ids, log_sum
 
 
