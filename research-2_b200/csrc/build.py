@@ -1,11 +1,15 @@
-"""Compiles the native code on first use and loads it with ctypes.
+"""Compiles the native code on first use and loads it.
 
-Two kinds of library come out of this folder:
+Three kinds of library come out of this folder:
 
   * the host library (cache manager, scheduler): `host/*.cc` with g++, no CUDA needed;
   * kernel libraries: `kernels/*.cu` with nvcc for sm_100a, one library per source file and
     set of `-D` definitions, so that a model compiles only the variants that it needs
-    (for example attention for its own head size).
+    (for example attention for its own head size);
+  * the faces module (`faces/*.cc` with g++, a module of Python's): operators called with tensors, for
+    the few whose calls cost more than their kernels.
+
+The first two are loaded with ctypes.
 
 Built files go to `csrc/_build/` inside the package when that folder can be written, else to
 a per-user folder under the system's temporary directory. A library is rebuilt when its
@@ -17,10 +21,13 @@ from __future__ import annotations
 
 import ctypes
 import hashlib
+import importlib.machinery
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 import threading
 import time
@@ -32,7 +39,7 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-r
 GXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra"]
 
 _lock = threading.Lock()
-_loaded: dict[str, ctypes.CDLL] = {}
+_loaded: dict[str, object] = {}
 
 
 class BuildError(RuntimeError):
@@ -99,8 +106,19 @@ def _headers(folder: Path) -> list[Path]:
     return sorted(list(folder.glob("*.h")) + list(folder.glob("*.cuh")))
 
 
+def _load_library(key: str, path: Path) -> ctypes.CDLL:
+    return ctypes.CDLL(str(path))
+
+
+def _load_module(key: str, path: Path):
+    loader = importlib.machinery.ExtensionFileLoader(key, str(path))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(key, loader))
+    loader.exec_module(module)
+    return module
+
+
 def _build_and_load(key: str, sources: list[Path], deps: list[Path], cmd_prefix: list[str], flags: list[str],
-                    link_flags: list[str], compiler: str, include: list[str] = ()) -> ctypes.CDLL:
+                    link_flags: list[str], compiler: str, include: list[str] = (), load=_load_library):
     """`include`: the folder of the headers in `deps`, whose contents (not whose path) decide whether a library is current."""
     with _lock:
         if key in _loaded:
@@ -119,8 +137,8 @@ def _build_and_load(key: str, sources: list[Path], deps: list[Path], cmd_prefix:
                     except OSError:
                         pass
         try:
-            lib = ctypes.CDLL(str(out))
-        except OSError as err:
+            lib = load(key, out)
+        except (OSError, ImportError) as err:
             raise BuildError(f"loading {out} failed: {err}") from None
         _loaded[key] = lib
         return lib
@@ -136,6 +154,22 @@ def host_library() -> ctypes.CDLL:
         # for the CPU tests: run python with LD_PRELOAD set to g++'s libasan.so and libubsan.so
         flags = ["-O1", "-g", "-fno-omit-frame-pointer", "-fsanitize=address,undefined"] + [f for f in flags if f != "-O2"]
     return _build_and_load("r2host", sources, _headers(folder), [gxx], flags, [], gxx)
+
+
+def faces_module():
+    """Operators called with tensors (they need torch's and Python's headers, and know its classes: a library per version)."""
+    import torch
+
+    folder = CSRC / "faces"
+    home = Path(torch.__file__).resolve().parent
+    cuda = Path(find_nvcc()).resolve().parent.parent
+    gxx = shutil.which("g++") or "g++"
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", f'-DR2_TORCH="{torch.__version__}"', f"-DR2_PYTHON={sys.hexversion}"]
+    include = [f for path in (home / "include", home / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+                              Path(sysconfig.get_paths()["include"])) for f in ("-isystem", str(path))]
+    link = ["-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]   # (loaded already, by torch itself)
+    return _build_and_load("r2faces", sorted(folder.glob("*.cc")), _headers(folder), [gxx], flags, link, gxx, include=include + [f"-L{home / 'lib'}"],
+                           load=_load_module)
 
 
 def kernel_library(source: str, defines: dict[str, int | str] | None = None) -> ctypes.CDLL:

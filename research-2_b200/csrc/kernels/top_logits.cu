@@ -2,18 +2,27 @@
 // the row's sum of exponentials at a temperature.
 //
 // A row is read once. While it passes, a thread sums exponentials against its own maximum and keeps the maximum of every group of four
-// 16-byte pieces. The k-th largest of the maxima of 320 pairs of threads (or a little less) is a value that at least k elements reach, and
-// what reaches it stands in the groups whose maximum does: little more than k groups of 16 or 32 elements, which are read again and give
-// little more than k candidates. Warps sort 32 of them at a time, and a candidate's place is how many stand above it in all of these runs. Values are compared as unsigned keys in the
-// floats' order, with the token as the lower half.
+// 16-byte pieces, rounded down to bfloat16. What k of the 512 threads' maxima (or a few more) reach is a value that at least k elements reach,
+// and what reaches it stands in the groups whose maximum does: little more than k groups of 16 or 32 elements, which are read again and give
+// little more than k candidates. Warps sort 32 of them at a time, and a candidate's place is how many stand above it in all of these runs.
+// Candidates are compared as unsigned keys in the floats' order, with the token as the lower half.
 //
 // Rows whose candidates do not fit (thousands of equal values at the edge of the list, or fewer than k numbers that are not NaN) are gone
 // over again: the exact k-th value by counts in bins of the keys' range, bin by bin narrower, everything above it, and equal values in the
 // order of their tokens until the list is full.
 //
-// An SM has one CTA: 20 warps read, row after row, and two teams of four choose, in turn: the candidates of two rows are looked for while the
-// next one passes. Behind a CTA's last row nothing passes any more, and its readers choose it themselves. Few rows are cut over the CTAs of
-// a cluster, whose candidates meet in the first one's shared memory.
+// An SM has one CTA. One thread brings: it has rounds of 32 KB copied into three stages, over the rows' ends too, so that memory never waits
+// for a row's end. 16 warps read them, and two teams of five choose, in turn: the candidates of two rows are looked for while the next one
+// passes. Behind a CTA's last row nothing passes any more, and its readers choose it themselves. Few rows are cut over the CTAs of a cluster,
+// whose candidates meet in the first one's shared memory: while twice as many CTAs still have an SM each and 1,024 pieces a share.
+//
+// What bounds it. Bytes: the readers alone take 2,048 float32 rows of 50,257 at 6.6 TB/s, as fast as a copy. With the teams beside them (k 64)
+// a pass is 75.6 us (5.46 TB/s): choosing a row is a chain of some 16,000 cycles for a team, as long as two rows take to pass, and the last
+// row's 8,000 have nothing beside them. 1,000 bfloat16 rows of 128,001 (k 128): 63.0 us (4.08 TB/s), of which the readers take 50, for twice the
+// exponentials a byte. A single row of 50,257 (k 5): 6.7 us, 2.6 of them until it is read, the rest the chain: a value by halving, groups, pieces, runs,
+// the cluster's hand-over.
+// Measured and not taken: readers' loads into their registers (85.2 and 67.1 us: what is on its way is bound by registers and by what shared
+// memory leaves of L1), two stages (83.0, 63.7), three teams of three warps (75.6, 64.3) or four (81.2, 62.3), 20 reading warps (79.0, 63.5).
 #include "logit_rows.cuh"
 #include "sm100_ptx.cuh"
 
@@ -736,15 +745,14 @@ top_kernel(const TopArgs a) {
   }
 
   const int team = int(threadIdx.x) / CHOOSERS, tid = int(threadIdx.x) % CHOOSERS;   // TEAMS: who brings
+  if (team < TEAMS && tid == 0 && ranks == 1) shared.teams[team].team = team;
+  pdl_wait();
   if (team == TEAMS) {
-    pdl_wait();
     if (tid == 0) bring_shares<T>(shared, share_of, first_row, a.rows, step, a.error);
     __syncwarp();
-  } else {
-  Shared& s = shared.teams[team];
-  if (tid == 0 && ranks == 1) s.team = team;
-  pdl_wait();
-  for (int r = first_row + team * step, turn = team; r + step < a.rows; r += TEAMS * step, turn += TEAMS) {
+  }
+  for (int r = team < TEAMS ? first_row + team * step : a.rows, turn = team; r + step < a.rows; r += TEAMS * step, turn += TEAMS) {
+    Shared& s = shared.teams[team];
     const int p = turn % PLACES;
     choosers_meet<CHOOSERS>(team);   // (the row before has been written out)
     if (tid == 0) s.n_found = s.n_chosen = s.above = 0u;
@@ -752,7 +760,6 @@ top_kernel(const TopArgs a) {
     choose<T, CHOOSERS>(a, shared, s, shared.places[p], share_of(r), r, shift, rank, tid, [&] {
       if (r + PLACES * step < a.rows) say_empty(p);
     });
-  }
   }
   if (ranks > 1) {  // (one row to a cluster: its readers' barriers)
     cluster_wait();

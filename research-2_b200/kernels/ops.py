@@ -13,7 +13,7 @@ import os
 
 import torch
 
-from ..csrc.build import kernel_library
+from ..csrc.build import faces_module, kernel_library
 
 F32, BF16 = 0, 1
 ACT_NONE, ACT_GELU_TANH, ACT_GELU_ERF = 0, 1, 2
@@ -151,6 +151,7 @@ def build_all(head_dims=()) -> None:
     for source in ("rowwise", "recurrent", "state_scan", "decay_chunks", "streams", "routing", "gemm_simt", "gemm_tc", "few_rows", "step_io", "attention_simt", "attention_prefill_tc", "latent_attention",
                    "sampling", "adjust_logits", "top_logits", "distill", "wait_selftest"):
         _lib(source)
+    faces_module()
     kernel_library("sfu_probe")  # (profiling/sfu_probe.py: a measurement, no part of a step)
     for head_dim in head_dims:
         _lib_for_head_dim("attention_decode", head_dim)
@@ -1952,6 +1953,29 @@ def _logit_entry(name: str):
     return entry[1]
 
 
+_logit_faces: dict = {}
+_error_addresses: dict = {}
+
+
+def _logit_face(name: str):
+    """The operator called with tensors (`csrc/faces`): (status, tensors ...) for a plain call, None for one that the checks here have to look at."""
+    face = _logit_faces.get(name)
+    if face is None or face[0] is not _libs.get(name):
+        entry, module = _logit_entry(name), faces_module()
+        module.bind(name, C.cast(entry, C.c_void_p).value)
+        face = _logit_faces[name] = (_libs[name], getattr(module, name))
+    return face[1]
+
+
+def _error_address(t: torch.Tensor) -> int:
+    """Of the word in which kernels record a wait that ran out, on a tensor's device."""
+    device = t.get_device()
+    address = _error_addresses.get(device)
+    if address is None:
+        address = _error_addresses[device] = _workspace(t.device).error.data_ptr()
+    return address
+
+
 def _current_stream(device: int) -> int:
     """The stream that a launch on tensors of `device` goes to; the device has to be the current one, as for every kernel here."""
     if device != torch._C._cuda_getDevice():
@@ -2041,6 +2065,12 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     and are added to their tokens, in order where a token is named more than once; tokens outside the vocabulary are left out.
     `mask` int32 [M, >= V / 32]: where bit t % 32 of word t / 32 of row mask_rows[r] is 0 the logit becomes -inf (`mask_rows` None: row r;
     a number outside [0, M): no mask). A mask that leaves nothing leaves a row of -inf, which `sample` answers with token 0."""
+    if logits.is_cuda:
+        done = _logit_face("adjust_logits")(logits, history, slots, lengths, prompt_lengths, repetition, presence, frequency, bias_start, bias_ids,
+                                            bias_values, mask, mask_rows, out)
+        if done is not None:
+            _check(done[0], "adjust_logits")
+            return done[1]
     code, rows, vocab, ld, device = _logit_rows(logits, "adjust_logits")
     history_rows = cap = history_ld = history_at = n_masks = mask_ld = mask_at = n_biases = bias_at = 0
     if history is not None:
@@ -2088,6 +2118,11 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0):
     """The k largest logits of every row of [R, V] (float32 or bfloat16; k up to 256 and V): (values float32 [R, k] from the largest down,
     their tokens int32 [R, k], log_sum float32 [R]), equal values from the lowest token up and NaN below all others; log_sum is the
     logarithm of the row's sum of exp(x / temperature), so values / temperature - log_sum are log-probabilities."""
+    if logits.is_cuda:
+        done = _logit_face("top_logits")(logits, k, temperature, _error_address(logits))
+        if done is not None:
+            _check(done[0], "top_logits")
+            return done[1:]
     code, rows, vocab, ld, device = _logit_rows(logits, "top_logits")
     if not 1 <= k <= min(vocab, TOP_MOST):
         raise KernelError(f"top_logits: k must be in [1, {min(vocab, TOP_MOST)}], got {k}")
@@ -2114,6 +2149,11 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
     left out). Without it p = softmax(teacher / temperature) over the listed tokens alone. `weight` float32 [R]: a row of weight 0 is not
     read; its loss and gradient are 0. A row without entries and without `log_sum` has the loss 0, one whose logits are all -inf, or hold
     +inf or NaN, a loss of NaN."""
+    if logits.is_cuda:
+        done = _logit_face("distill")(logits, ids, teacher, log_sum, temperature, weight, gradient, out, _error_address(logits))
+        if done is not None:
+            _check(done[0], "distill_loss")
+            return done[1:]
     code, rows, vocab, ld, device = _logit_rows(logits, "distill_loss")
     if ids.dtype is not torch.int32 or teacher.dtype is not torch.float32 or ids.dim() != 2:
         raise KernelError(f"distill_loss: ids must be int32 [rows, K] and teacher float32, got {ids.dtype} {tuple(ids.shape)} and {teacher.dtype}")

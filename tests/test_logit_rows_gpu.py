@@ -595,3 +595,68 @@ def test_logit_rows_do_not_depend_on_what_lies_around_them(around, dtype, vocab)
                 assert torch.allclose(g.float(), w.float(), rtol=1e-4 if dtype == F32 else 2.0**-7, atol=1e-7)
     arguments = dict(history=i32([[1, 2, 3]] * 3), lengths=i32([3, 2, 1]), presence=f32([1.0] * 3))
     assert torch.equal(ops().adjust_logits(x, **arguments), ops().adjust_logits(alone, **arguments))
+
+
+# ---- calls in one step, and through the checks --------------------------------------------------
+
+class Other(torch.Tensor):
+    pass
+
+
+def adjusting(rows: int) -> dict:
+    return dict(history=i32([[3, 5, 5, 8]] * 4), slots=i32([3, 0, 1][:rows]), lengths=i32([4, 2, 0][:rows]), prompt_lengths=i32([1, 0, 0][:rows]),
+                repetition=f32([1.3, 1.0, 2.0][:rows]), presence=f32([0.5, 0.25, 0.0][:rows]), frequency=f32([0.1, 0.0, 1.0][:rows]),
+                bias_start=i32([0, 2, 2, 3][: rows + 1]), bias_ids=i32([9, 3, 11]), bias_values=f32([1.0, -2.0, -math.inf]),
+                mask=i32([[-2] * 40]), mask_rows=i32([0, -1, 0][:rows]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("offset,pad", [(0, 0), (1, 3), (0, 4000)])
+def test_a_call_in_one_step_is_the_call_through_the_checks(dtype, offset, pad):
+    """A subclass's call takes the way through the checks, the same tensor's takes one step."""
+    o, x = ops(), rows_at(random_logits(3, 1280, 31), dtype, offset, pad)
+    other = x.as_subclass(Other)
+    face = o._logit_face("top_logits")
+    assert face(x, 5, 1.0, o._error_address(x)) is not None and face(other, 5, 1.0, o._error_address(x)) is None
+    for a, b in zip(o.top_logits(x, 7, temperature=2), o.top_logits(other, 7, temperature=2)):
+        assert torch.equal(a, b) and a.dtype == b.dtype and a.stride() == b.stride()
+    values, ids, log_sum = o.top_logits(x, 7)
+    for log in (None, log_sum):
+        for a, b in zip(o.distill_loss(x, ids, values, log_sum=log, weight=f32([1.0, 0.0, 0.5])),
+                        o.distill_loss(other, ids, values, log_sum=log, weight=f32([1.0, 0.0, 0.5]))):
+            assert torch.equal(a, b) and a.stride() == b.stride() and a.data_ptr() % 16 == b.data_ptr() % 16
+    assert o.distill_loss(x, ids, values, gradient=False)[1] is None
+    a, b = o.adjust_logits(x, **adjusting(3)), o.adjust_logits(other, **adjusting(3))
+    assert torch.equal(a, b) and a.stride() == b.stride() and a.data_ptr() % 16 == b.data_ptr() % 16
+    whole = x.clone()
+    assert o.adjust_logits(whole, **adjusting(3), out=whole) is whole and torch.equal(whole, a)
+    one = adjusting(1)
+    assert torch.equal(o.adjust_logits(x[:1], **one), a[:1])
+
+
+def test_what_one_step_does_not_take():
+    o, x = ops(), random_logits(3, 1280, 5).to(DEV)
+    values, ids, log_sum = o.top_logits(x, 7)
+    at = o._error_address(x)
+    top, adjust, distill = (o._logit_face(name) for name in ("top_logits", "adjust_logits", "distill"))
+    for refused in ((x.double(), 5, 1.0, at), (x.cpu(), 5, 1.0, at), (x[0], 5, 1.0, at), (x.t(), 5, 1.0, at), (x[:0], 5, 1.0, at), (x, 0, 1.0, at),
+                    (x, 257, 1.0, at), (x, 5.0, 1.0, at), (x, 1 << 70, 1.0, at), (x, 5, 0.0, at), (x, 5, math.nan, at), (x, 5, math.inf, at),
+                    (x, 5, "1", at), (x, 5, 1.0), ("x", 5, 1.0, at)):
+        assert top(*refused) is None
+    good = [x, ids, values, log_sum, 1.0, None, True, None, at]
+    assert distill(*good) is not None
+    for i, wrong in ((1, ids.long()), (1, ids[:2]), (1, None), (2, values.bfloat16()), (2, values[:, :3]), (3, log_sum[:2]), (3, log_sum.double()),
+                     (4, -1.0), (5, log_sum[:1]), (6, 1), (7, x.bfloat16()), (7, x[:, 1:]), (7, ids)):
+        assert distill(*good[:i], wrong, *good[i + 1:]) is None, (i, wrong)
+    shared = torch.zeros(4 * 1280, device=DEV)
+    a, b = shared[: 3 * 1280].view(3, 1280), shared[1280:].view(3, 1280)
+    assert distill(a, ids, values, log_sum, 1.0, None, True, b, at) is None
+    order = ("history", "slots", "lengths", "prompt_lengths", "repetition", "presence", "frequency", "bias_start", "bias_ids", "bias_values", "mask",
+             "mask_rows", "out")
+    given = {**dict.fromkeys(order), **adjusting(3)}
+    assert adjust(x, *given.values()) is not None
+    for name, wrong in (("history", None), ("history", given["history"][0]), ("history", given["history"].long()), ("lengths", None),
+                        ("lengths", given["lengths"][:2]), ("slots", given["slots"].float()), ("repetition", given["repetition"].double()),
+                        ("bias_start", given["bias_start"][:3]), ("bias_start", None), ("bias_ids", None), ("bias_values", given["bias_values"][:2]),
+                        ("mask", given["mask"][:, :39]), ("mask_rows", None), ("out", x[:, :1279]), ("out", x.cpu())):
+        assert adjust(x, *{**given, name: wrong}.values()) is None, name
