@@ -16,6 +16,10 @@
 // bytes. Clusters walk over the rows: while one is worked on, the next one's pieces are on their way. The listed tokens are taken out of a
 // row (their places become -inf) before it is summed, so that what is left is summed without looking at the list. Losses alone, and rows that
 // no cluster holds, take a second kernel that streams.
+//
+// What bounds it. 1,024 float32 rows of 50,257 (64 listed): 75 us for 399 MB, 5.3 TB/s, 0.81 of a copy; nothing runs beside the first share's arrival
+// and the last one's gradient, 8 us. 4,096 bfloat16 rows (32 listed): 153 us, 5.1 TB/s: the special-function units are busy 58 % of the time,
+// with two exponentials a number. Losses of 2,047 float32 rows of 128,001: 163 us, 6.0 TB/s, 0.92 of a copy. 16 rows of 1,031: 4.9 us, a row's chain.
 #include "logit_rows.cuh"
 #include "sm100_ptx.cuh"
 
@@ -571,7 +575,10 @@ distill_streamed_kernel(const DistillArgs a) {
 
 constexpr int MOST_STREAMED_BITS = 1 << 20;   // tokens of a CTA's share (128 KB of bits)
 
-constexpr int HELD_TWO = 6600, HELD_ONE = 13600;   // pieces of a CTA's share where two CTAs, or one, fit an SM
+// Pieces of a CTA's share where two CTAs, or one, fit an SM. A row takes as few CTAs as hold it with two to an SM, so that one's sum runs beside
+// the other's copies (1,024 rows of 50,257: two CTAs of 100 KB a row 75 us, one of 200 KB with an SM to itself 77, shares for three or
+// four CTAs an SM 100 to 117); eight CTAs of a whole SM each hold the longest rows.
+constexpr int HELD_TWO = 6600, HELD_ONE = 13600;
 
 template <typename T>
 int launch_held(const DistillArgs& a, cudaStream_t stream) {
