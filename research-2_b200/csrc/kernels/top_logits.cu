@@ -14,7 +14,8 @@
 // An SM has one CTA. One thread brings: it has rounds of 32 KB copied into three stages, over the rows' ends too, so that memory never waits
 // for a row's end. 16 warps read them, and two teams of five choose, in turn: the candidates of two rows are looked for while the next one
 // passes. Behind a CTA's last row nothing passes any more, and its readers choose it themselves. Few rows are cut over the CTAs of a cluster,
-// whose candidates meet in the first one's shared memory: while twice as many CTAs still have an SM each and 1,024 pieces a share.
+// whose candidates meet in the first one's shared memory: while twice as many CTAs still have an SM each and 1,024 pieces a share. Short rows
+// have a kernel of their own, whose threads hold them: seven rows an SM, or 28 of a warp each.
 //
 // What bounds it. Bytes: the readers alone take 2,048 float32 rows of 50,257 at 6.6 TB/s, as fast as a copy. With the teams beside them (k 64)
 // a pass is 75.6 us (5.46 TB/s): choosing a row is a chain of some 16,000 cycles for a team, as long as two rows take to pass, and the last
@@ -41,6 +42,7 @@ constexpr int STAGES = 3;     // rounds on their way
 constexpr int SLOTS = 8;      // groups of a thread (of several rounds each in long rows)
 constexpr int CAP = 1536;     // candidates
 constexpr int MOST_CHOSEN = 1024, BINS = 512;
+constexpr int SHORT_THREADS = 128, SHORT_PIECES = 8;   // of a short row: its threads where a warp does not do, and what each holds
 constexpr int LEVELS = 4;     // 9 bits of a 32-bit key at each
 struct TopArgs {
   const void* logits; long long ld;
@@ -56,9 +58,10 @@ struct __align__(16) Place {
   uint16_t most[READERS];                 // the threads'
   float2 sums[READING_WARPS];             // the warps' references and sums
 };
-// A team's own.
-struct __align__(16) Shared {
-  unsigned long long found[CAP];          // candidates: key, then the token's complement
+// Of those who choose a row.
+template <int N>
+struct __align__(16) Lists {
+  unsigned long long found[N];            // candidates: key, then the token's complement
   union {
     uint16_t chosen[MOST_CHOSEN];         // groups that are read again: slot * READERS + thread
     uint32_t bins[BINS];
@@ -69,6 +72,7 @@ struct __align__(16) Shared {
   uint32_t n_of[MOST_RANKS];
   int team;
 };
+using Shared = Lists<CAP>;
 struct TopShared {
   uint4 rounds[STAGES][READERS * DEPTH];   // a share's pieces, copied
   Place places[PLACES];
@@ -78,14 +82,17 @@ struct TopShared {
 // Clusters have one row, the readers': what they send each other stands in the other places, what the first CTA puts together in the teams'.
 static_assert((MOST_RANKS - 1) * MOST_K * sizeof(unsigned long long) <= (PLACES - 1) * sizeof(Place), "");
 static_assert(MOST_RANKS * MOST_K * sizeof(unsigned long long) <= TEAMS * sizeof(Shared), "");
+static_assert(CHOOSERS != SHORT_THREADS && READERS != SHORT_THREADS, "each has its own barrier");
 static_assert(SLOTS * READERS <= 65536 && READERS >= MOST_K && READERS < 1024 && 2 * SLOTS <= 16, "");
 
 template <int ID, int COUNT> __device__ __forceinline__ void bar_sync() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(COUNT) : "memory"); }
 template <int ID, int COUNT> __device__ __forceinline__ void bar_arrive() { asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(COUNT) : "memory"); }
-// those who choose a row: a team, or the readers
+// those who choose a row: a team, the readers, or all of a short row's
 template <int THREADS>
 __device__ __forceinline__ void choosers_meet(int team) {
-  if (THREADS == READERS) bar_sync<11, READERS>();
+  if (THREADS == 32) __syncwarp();
+  else if (THREADS == SHORT_THREADS) __syncthreads();
+  else if (THREADS == READERS) bar_sync<11, READERS>();
   else if (team) bar_sync<2, CHOOSERS>();
   else bar_sync<1, CHOOSERS>();
 }
@@ -157,8 +164,8 @@ __device__ __forceinline__ uint32_t reaching(const uint4& raw, __nv_bfloat162 bo
 
 // One level: the bins of the keys in [low, high] are counted; from the top, the bin at which the count (with `above`, keys over `high`)
 // reaches k becomes the range. True once the bins are single keys.
-template <int THREADS>
-__device__ __forceinline__ bool narrow(Shared& s, int k, int shift, int tid) {
+template <int THREADS, typename L>
+__device__ __forceinline__ bool narrow(L& s, int k, int shift, int tid) {
   choosers_meet<THREADS>(s.team);
   if (tid < 32) {
     const int lane = tid;
@@ -232,8 +239,8 @@ __device__ __forceinline__ float largest(const uint4 (&raw)[N]) {
 }
 
 // The row again, from its exact k-th value: at least k of the share's elements reach `reached`, or it is 0.
-template <typename T, int THREADS>
-__device__ __noinline__ void go_over(Shared& s, const Row<T>& row, int k, uint32_t reached, int tid) {
+template <typename T, int THREADS, typename L>
+__device__ __noinline__ void go_over(L& s, const Row<T>& row, int k, uint32_t reached, int tid) {
   constexpr int PER = RowPieces<T>::PER;
   const int lane = tid & 31, warp = tid >> 5;
   auto over = [&](auto&& f) {   // every element of the share: (key, token)
@@ -482,6 +489,26 @@ __device__ __forceinline__ int above_in(const unsigned long long* run, unsigned 
   for (int step = 16; step > 0; step /= 2) at += run[at + step - 1] > mine ? step : 0;
   return at + (run[at] > mine ? 1 : 0);
 }
+// What stands at place `above` of a list's runs: f(above, candidate), for the first k.
+template <int THREADS, typename F>
+__device__ __forceinline__ void in_order(const unsigned long long* list, int n, int k, int tid, F&& f) {
+  for (int i = tid; i < n; i += THREADS) {
+    const unsigned long long mine = list[i];
+    int above = 0;
+#pragma unroll 4
+    for (int run = 0; run < n; run += 32) above += above_in(list + run, mine);
+    if (mine != 0ull && above < k) f(above, mine);
+  }
+}
+template <int THREADS>
+__device__ __forceinline__ void write_list(const TopArgs& a, int r, const unsigned long long* list, int n, int tid) {
+  float* values = a.values + (long long)r * a.k;
+  int32_t* ids = a.ids + (long long)r * a.k;
+  in_order<THREADS>(list, n, a.k, tid, [&](int at, unsigned long long entry) {
+    values[at] = value_of(uint32_t(entry >> 32));
+    ids[at] = int32_t(0xffffffffu - uint32_t(entry & 0xffffffffull));
+  });
+}
 // Places on a list for every thread's `mine` entries, one atomic a warp. -> the first one's.
 __device__ __forceinline__ uint32_t places_for(uint32_t mine, uint32_t* count, int lane) {
   uint32_t upto = mine;
@@ -648,16 +675,6 @@ __device__ __forceinline__ void choose(const TopArgs& a, TopShared& shared, Shar
   int n = (int(s.n_found) + 31) / 32 * 32;
   for (int i = tid; i < n; i += THREADS) list[i] = sorted(i < int(s.n_found) ? list[i] : 0ull, lane);
   choosers_meet<THREADS>(s.team);
-  // what stands at place `above` of them all: f(above, candidate)
-  auto in_order = [&](auto&& f) {
-    for (int i = tid; i < n; i += THREADS) {
-      const unsigned long long mine = list[i];
-      int above = 0;
-#pragma unroll 4
-      for (int run = 0; run < n; run += 32) above += above_in(list + run, mine);
-      if (mine != 0ull && above < a.k) f(above, mine);
-    }
-  };
   if (THREADS == READERS && a.ranks > 1) {
     unsigned long long* sent = reinterpret_cast<unsigned long long*>(&shared.places[1]);   // by the other CTAs, MOST_K places each
     cluster_wait();   // (the first CTA runs)
@@ -669,7 +686,7 @@ __device__ __forceinline__ void choose(const TopArgs& a, TopShared& shared, Shar
     if (n <= MOST_K) {
       for (int i = tid; i < n; i += THREADS) send(i, list[i]);
     } else {   // the first k of them, in order
-      in_order(send);
+      in_order<THREADS>(list, n, a.k, tid, send);
       n = (k + 31) / 32 * 32;
       if (tid < n - k) send(k + tid, 0ull);
     }
@@ -696,12 +713,7 @@ __device__ __forceinline__ void choose(const TopArgs& a, TopShared& shared, Shar
     }
     choosers_meet<THREADS>(s.team);
   }
-  float* values = a.values + (long long)r * a.k;
-  int32_t* ids = a.ids + (long long)r * a.k;
-  in_order([&](int at, unsigned long long entry) {
-    values[at] = value_of(uint32_t(entry >> 32));
-    ids[at] = int32_t(0xffffffffu - uint32_t(entry & 0xffffffffull));
-  });
+  write_list<THREADS>(a, r, list, n, tid);
 }
 
 template <typename T>
@@ -769,8 +781,156 @@ top_kernel(const TopArgs a) {
 }
 
 template <typename T>
+__device__ __noinline__ uint4 blanked(uint4 raw, RowPieces<T> x, int g) {   // (out of the way)
+  blank_outside(raw, x, g);
+  return raw;
+}
+
+// A short row, which its threads hold: a warp, or four. Nothing is read again, and an SM has as many rows in hand as registers allow.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 32 ? 28 : 7)
+top_short_kernel(const TopArgs a) {
+  constexpr int PER = RowPieces<T>::PER, PAIRS = PER / 2, WARPS = THREADS / 32, HOLDS = SHORT_PIECES;
+  constexpr int MOST = THREADS == 32 ? 512 : 1024;
+  __shared__ Lists<MOST> s;
+  __shared__ float2 sums[WARPS];
+  pdl_launch_dependents();
+  const int tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5, r = int(blockIdx.x);
+  if (tid == 0) {
+    s.team = 0;
+    s.n_found = s.above = 0u;
+  }
+  choosers_meet<THREADS>(0);
+  pdl_wait();
+  Row<T> row = {RowPieces<T>(static_cast<const T*>(a.logits) + (long long)r * a.ld, a.vocab), 0, 0};
+  row.n = row.x.count;
+  const int n = row.n, k = a.k;
+  const uint32_t nothing = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+  uint4 raw[HOLDS];
+#pragma unroll
+  for (int i = 0; i < HOLDS; ++i) {
+    raw[i] = make_uint4(nothing, nothing, nothing, nothing);
+    load_16_if(raw[i], reinterpret_cast<const uint4*>(row.x.base) + i * THREADS + tid, i * THREADS + tid < n);
+  }
+#pragma unroll
+  for (int i = 0; i < HOLDS; ++i)
+    if (i * THREADS + tid == n - 1 || (i == 0 && tid == 0)) raw[i] = blanked(raw[i], row.x, i * THREADS + tid);
+
+  // sums, and the maxima of the pieces
+  const float c = 1.44269504f / a.tau;
+  float most[HOLDS], row_most = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < HOLDS; ++i) {
+    const uint4 one[1] = {raw[i]};
+    most[i] = largest<T, 1>(one);
+    row_most = fmaxf(row_most, most[i]);
+  }
+  const float reference = warp_max(fminf(row_most * c, 3e38f)), minus = -no_less(reference);
+  const uint64_t cc = two_of(c, c), ss = two_of(minus, minus);
+  uint64_t acc = 0ull;
+#pragma unroll
+  for (int i = 0; i < HOLDS; ++i) {
+    if (i * THREADS + warp * 32 >= n) continue;
+    uint64_t p[PAIRS];
+    unpack_pairs(raw[i], p, static_cast<const T*>(nullptr));
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) acc = add_two(acc, exp2_two(fma_two(p[j], cc, ss)));
+  }
+  const float2 both = halves(acc);
+  float common = reference, total = warp_sum(both.x + both.y);
+  if (WARPS > 1) {
+    if (lane == 0) sums[warp] = make_float2(common, total);
+    __syncthreads();
+    const float2 part = lane < WARPS ? sums[lane] : make_float2(-INFINITY, 0.f);
+    common = warp_max(part.x);
+    total = warp_sum(part.y * rebase(part.x, common));
+  }
+  if (tid == 0) a.log_sum[r] = (no_less(common) + log2f(total)) * 0.693147181f;
+
+  // what k pieces' maxima reach, or k numbers where there are not twice as many pieces: two values tried at a time (counts in 16 bits each)
+  const bool fine = n < 2 * k;
+  uint32_t low = 0x7fu, high = 0xff80u;   // -inf, inf
+  const int enough = k + max(8, k / 8);
+  for (int turn = 0; low < high; turn ^= 1) {
+    const uint32_t third = (high - low) / 3, one = low + third + 1, two = high - third;   // in (low, high], one <= two
+    const __nv_bfloat162 of_one = both_of(one), of_two = both_of(two);
+    const float least_one = __low2float(of_one), least_two = __low2float(of_two);
+    uint32_t reach = 0u;
+    if (fine) {
+#pragma unroll
+      for (int i = 0; i < HOLDS; ++i) {
+        if (i * THREADS + warp * 32 >= n) continue;
+        reach += uint32_t(__popc(reaching(raw[i], of_one, static_cast<const T*>(nullptr)))) +
+                 (uint32_t(__popc(reaching(raw[i], of_two, static_cast<const T*>(nullptr)))) << 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < HOLDS; ++i) reach += (most[i] >= least_one ? 1u : 0u) + (most[i] >= least_two ? 1u << 16 : 0u);
+    }
+    reach = __reduce_add_sync(0xffffffffu, reach);
+    if (WARPS > 1) {
+      if (lane == 0) s.bins[turn * WARPS + warp] = reach;
+      __syncthreads();
+      reach = 0u;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) reach += s.bins[turn * WARPS + w];
+    }
+    const int reach_one = int(reach & 0xffffu), reach_two = int(reach >> 16);
+    int of_low = 0;
+    if (reach_two >= k) {
+      low = two;
+      of_low = reach_two;
+    } else if (reach_one >= k) {
+      low = one;
+      high = two - 1;
+      of_low = reach_one;
+    } else {
+      high = one - 1;
+    }
+    if (of_low >= k && of_low <= enough) break;
+  }
+  const __nv_bfloat162 least = both_of(low);
+  uint32_t bits[HOLDS], mine = 0u;
+#pragma unroll
+  for (int i = 0; i < HOLDS; ++i) {
+    const int at = i * THREADS + tid, first = row.x.first(at);
+    bits[i] = at < n ? reaching(raw[i], least, static_cast<const T*>(nullptr)) : 0u;
+    if (first < 0) bits[i] &= ~0u << -first;
+    if (first < a.vocab && first + PER > a.vocab) bits[i] &= (1u << (a.vocab - first)) - 1u;
+    mine += uint32_t(__popc(bits[i]));
+  }
+  uint32_t to = places_for(mine, &s.n_found, lane);
+#pragma unroll
+  for (int i = 0; i < HOLDS; ++i) {
+#pragma unroll 1
+    for (uint32_t left = bits[i]; left != 0u; left &= left - 1u, ++to) {
+      const int e = __ffs(int(left)) - 1, w = e * 4 / PER;
+      const uint32_t word = (w & 2) ? ((w & 1) ? raw[i].w : raw[i].z) : ((w & 1) ? raw[i].y : raw[i].x);
+      const float v = __uint_as_float(PER == 4 ? word : (e & 1) ? word & 0xffff0000u : word << 16);
+      if (to < uint32_t(MOST)) s.found[to] = composite(logit_key(v), row.x.first(i * THREADS + tid) + e);
+    }
+  }
+  choosers_meet<THREADS>(0);
+  const uint32_t reached = logit_key(__low2float(least));
+  if (s.n_found > uint32_t(MOST)) go_over<T, THREADS>(s, row, k, reached, tid);
+  if (s.n_found < uint32_t(k)) go_over<T, THREADS>(s, row, k, 0u, tid);   // (fewer than k numbers that are not NaN)
+  const int filled = (int(s.n_found) + 31) / 32 * 32;
+  for (int i = tid; i < filled; i += THREADS) s.found[i] = sorted(i < int(s.n_found) ? s.found[i] : 0ull, lane);
+  choosers_meet<THREADS>(0);
+  write_list<THREADS>(a, r, s.found, filled, tid);
+}
+
+template <typename T>
 int launch(TopArgs a, int rows, cudaStream_t stream) {
   const int pieces = (a.vocab + 2 * RowPieces<T>::PER - 2) / RowPieces<T>::PER;   // of a row at any alignment, at most
+  // Rows that 128 threads hold in their registers (4,096 rows of 4,000 float32 numbers, k 64: 36 us, the other kernel 69; 16 rows 6.0, 6.1). One
+  // warp where that does, there is a row for every scheduler and k is not large (4,096 rows of 300, k 10: 8.4 us, 128 threads 19.5; but 300 rows
+  // of 1,000, k 100: 9.9, 7.9; 2,000 of them, k 256: 36.5, 31.6).
+  if (pieces <= SHORT_PIECES * SHORT_THREADS) {
+    if (pieces <= SHORT_PIECES * 32 && rows >= 4 * 148 && a.k <= 128) r2_launch(top_short_kernel<T, 32>, dim3(unsigned(rows)), dim3(32), size_t(0), stream, a);
+    else r2_launch(top_short_kernel<T, SHORT_THREADS>, dim3(unsigned(rows)), dim3(SHORT_THREADS), size_t(0), stream, a);
+    return launch_status();
+  }
   a.ranks = 1;
   while (a.ranks < MOST_RANKS && (long long)rows * a.ranks * 2 <= 148 && pieces / (2 * a.ranks) >= 1024) a.ranks *= 2;
   a.per = (pieces + a.ranks - 1) / a.ranks;

@@ -265,6 +265,28 @@ def test_top_logits_of_many_candidates(rows, vocab, k, dtype):
     assert torch.equal(ids.long(), order) and torch.equal(values, torch.gather(x.float(), 1, order))
 
 
+@pytest.mark.parametrize("rows", [3, 700])
+@pytest.mark.parametrize("vocab,k", [(1, 1), (9, 9), (129, 128), (257, 5), (511, 200), (1020, 64), (1029, 128), (2044, 256), (2053, 100), (4080, 33), (4105, 64), (8190, 20)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_top_logits_of_short_rows(rows, vocab, k, dtype):
+    """A warp's rows, 128 threads' rows and the first that they do not hold; some of few values, of few numbers, of none."""
+    x = random_logits(rows, vocab, vocab + 3 * rows)
+    x[::4] = torch.round(x[::4])
+    x[1::16, vocab // 3:] = -math.inf
+    x[2::16] = 0.5
+    x = rows_at(x, dtype, 3, 1)
+    values, ids, log_sum = ops().top_logits(x, k, temperature=1.5)
+    order = torch.argsort(x.float(), dim=1, descending=True, stable=True)[:, :k]
+    assert torch.equal(ids.long(), order) and torch.equal(values, torch.gather(x.float(), 1, order))
+    want = torch.logsumexp(x.double() / 1.5, dim=1)
+    assert torch.all((log_sum == want) | ((log_sum.double() - want).abs() <= 1e-5 + 4 * EPS * want.abs()))   # (-inf equals -inf)
+    if rows > 3:
+        holed = x.clone()
+        holed[::5] = math.nan
+        holed[1::5, :: 2] = math.nan
+        check_top(holed[:12], k)
+
+
 @pytest.mark.parametrize("order", ["rising", "falling"])
 def test_top_logits_of_rows_in_order(order):
     x = torch.linspace(-20, 20, 50257)[None].repeat(2, 1)
