@@ -19,7 +19,7 @@
 //
 // What bounds it. 1,024 float32 rows of 50,257 (64 listed): 75 us for 399 MB, 5.3 TB/s, 0.81 of a copy; nothing runs beside the first share's arrival
 // and the last one's gradient, 8 us. 4,096 bfloat16 rows (32 listed): 153 us, 5.1 TB/s: the special-function units are busy 58 % of the time,
-// with two exponentials a number. Losses of 2,047 float32 rows of 128,001: 163 us, 6.0 TB/s, 0.92 of a copy. 16 rows of 1,031: 4.9 us, a row's chain.
+// with two exponentials a number. Losses of 2,047 float32 rows of 128,001: 156 us, 6.3 TB/s, 0.96 of a copy. 16 rows of 1,031: 4.9 us, a row's chain.
 #include "logit_rows.cuh"
 #include "sm100_ptx.cuh"
 
@@ -436,10 +436,10 @@ distill_held_kernel(const DistillArgs a) {
 }
 
 // Losses alone (one pass over the row), and gradients of rows that no cluster holds (two).
-template <typename T, bool TAIL>
-__global__ void __launch_bounds__(256, 4)
+template <typename T, bool TAIL, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 distill_streamed_kernel(const DistillArgs a) {
-  constexpr int THREADS = 256, PER = RowPieces<T>::PER, DEPTH = 4;
+  constexpr int PER = RowPieces<T>::PER, DEPTH = 4;
   extern __shared__ __align__(16) uint32_t bits_s[];   // a bit for each token of this CTA's share
   __shared__ __align__(16) float4 shares[MOST_RANKS * (THREADS / 32)];
   __shared__ int32_t ids[MOST_K];
@@ -582,7 +582,10 @@ constexpr int HELD_TWO = 6600, HELD_ONE = 13600;
 
 template <typename T>
 int launch_held(const DistillArgs& a, cudaStream_t stream) {
-  const int warps = max(1, min(MOST_WARPS, a.per / 64));
+  // Short rows get few warps, so that more of them are in hand: two pieces a thread at least, and beyond three warps sixteen (4,096 rows of 4,000
+  // float32 numbers: twelve warps 62 us, three 30; 2,000 of 12,000: twelve 61, five 52; 100 of 4,000: twelve 6.0, three 6.2, one 8.0). By the row alone: its
+  // sums are then added in the same order in every call.
+  const int warps = max(1, min(min(MOST_WARPS, a.per / 64), max(3, a.per / 512)));
   const size_t smem = size_t(a.per) * 16;
   static std::atomic<bool> allowed[64];
   const int status = allow_smem(distill_held_kernel<T>, size_t(HELD_ONE) * 16, allowed);
@@ -596,7 +599,7 @@ int launch_held(const DistillArgs& a, cudaStream_t stream) {
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return int(e);
   const unsigned long long shape = (static_cast<unsigned long long>(device) << 56) | (static_cast<unsigned long long>(a.ranks) << 48) |
-                                   (static_cast<unsigned long long>(a.per) << 24);
+                                   (static_cast<unsigned long long>(a.per * 16 + warps) << 24);
   Resident& place = resident[(a.per * 8 + a.ranks + device) % 64];
   const unsigned long long known = place.shape_and_clusters.load(std::memory_order_relaxed);
   if ((known >> 24) == (shape >> 24) && known != 0) {
@@ -622,21 +625,28 @@ int launch_held(const DistillArgs& a, cudaStream_t stream) {
   return launch_status();
 }
 
+template <typename T, bool TAIL, int THREADS>
+int launch_streamed(const DistillArgs& a, cudaStream_t stream) {
+  static std::atomic<bool> allowed[64];
+  const int status = allow_smem(distill_streamed_kernel<T, TAIL, THREADS>, MOST_STREAMED_BITS / 8, allowed);
+  if (status != R2_OK) return status;
+  r2_launch_clusters(distill_streamed_kernel<T, TAIL, THREADS>, a.ranks, dim3(unsigned(a.rows) * unsigned(a.ranks)), dim3(THREADS),
+                     size_t(a.per * RowPieces<T>::PER + 31) / 32 * 4, stream, a);
+  return launch_status();
+}
 template <typename T, bool TAIL>
 int launch_streamed(DistillArgs a, int pieces, cudaStream_t stream) {
   // a row to a CTA where there are CTAs enough for the SMs, else cut over several
   a.ranks = 1;
   while (a.ranks < MOST_RANKS && ((long long)a.rows * a.ranks < 592 || (pieces / a.ranks + 1) * RowPieces<T>::PER > MOST_STREAMED_BITS)
          && pieces / a.ranks > 1024) a.ranks *= 2;
-  const int per = a.per = (pieces + a.ranks - 1) / a.ranks;
-  if (per * RowPieces<T>::PER > MOST_STREAMED_BITS) return R2_UNSUPPORTED;
+  a.per = (pieces + a.ranks - 1) / a.ranks;
+  if (a.per * RowPieces<T>::PER > MOST_STREAMED_BITS) return R2_UNSUPPORTED;
   if ((long long)a.rows * a.ranks > 0x7fffffffLL) return R2_BAD_SHAPE;
-  static std::atomic<bool> allowed[64];
-  const int status = allow_smem(distill_streamed_kernel<T, TAIL>, MOST_STREAMED_BITS / 8, allowed);
-  if (status != R2_OK) return status;
-  r2_launch_clusters(distill_streamed_kernel<T, TAIL>, a.ranks, dim3(unsigned(a.rows) * unsigned(a.ranks)), dim3(256),
-                     size_t(per * RowPieces<T>::PER + 31) / 32 * 4, stream, a);
-  return launch_status();
+  // Half the threads where the rows are more than four CTAs an SM (2,047 rows of 128,001, 100 listed: 163 us with 256 threads, 156 with 128;
+  // 4,096 of 4,000: 45, 29; but 592 of 50,257: 19.9, 24.5).
+  if ((long long)a.rows * a.ranks > 592) return launch_streamed<T, TAIL, 128>(a, stream);
+  return launch_streamed<T, TAIL, 256>(a, stream);
 }
 
 template <typename T, bool TAIL>

@@ -597,6 +597,26 @@ def test_distill_many_rows_some_of_no_weight(vocab, dtype):
     assert torch.all(off <= 1e-5 * (q + p.amax(1, keepdim=True) * listed) + 4e-6 * q / rest + (2.0**-8 * want.abs() if dtype == BF16 else 0))
 
 
+@pytest.mark.parametrize("rows,vocab,k", [(700, 257, 3), (900, 1000, 20), (700, 4001, 64), (650, 12007, 9), (1300, 33, 5)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_distill_of_many_short_rows_is_that_of_few(rows, vocab, k, dtype):
+    """More rows than there are places take other numbers of threads; a row's loss and gradient are those of a call on a few rows."""
+    gen = torch.Generator().manual_seed(rows)
+    x = rows_at(random_logits(rows, vocab, rows), dtype, 1, 2)
+    values, ids, log_sum = ops().top_logits(rows_at(torch.randn(rows, vocab, generator=gen) * 3, F32), k)
+    weight = torch.rand(rows, generator=gen).to(DEV)
+    weight[::7] = 0.0
+    for log in (log_sum, None):
+        loss, gradient = ops().distill_loss(x, ids, values, log_sum=log, weight=weight, temperature=1.5)
+        alone, _ = ops().distill_loss(x, ids, values, log_sum=log, weight=weight, temperature=1.5, gradient=False)
+        assert torch.allclose(alone, loss, rtol=1e-4, atol=1e-5)
+        for at in (0, 128, rows - 60):
+            part = slice(at, at + 60)
+            one, its = ops().distill_loss(x[part], ids[part], values[part], log_sum=None if log is None else log[part], weight=weight[part], temperature=1.5)
+            assert torch.allclose(one, loss[part], rtol=1e-4, atol=1e-5)
+            assert torch.allclose(its.float(), gradient[part].float(), rtol=1e-4 if dtype == F32 else 2.0**-7, atol=1e-7)
+
+
 @pytest.mark.parametrize("around", [math.inf, -math.inf, math.nan, 1e30, -1e30])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("vocab", [37, 3003, 9001, 50257, 131079])
