@@ -236,7 +236,9 @@ template <typename T, typename W>
 int launch_segments(AdjustArgs a, cudaStream_t stream) {
   constexpr int PER = RowPieces<T>::PER;
   const int pieces = (a.vocab + 2 * PER - 2) / PER;   // of a row at any alignment, at most
-  const int most = 64 * 1024 / int(sizeof(W)) / PER;  // of a segment: 64 KB of places
+  // Tokens of a segment, at most: 64 KB of places for long histories, 32 KB, and so more CTAs an SM, for short ones or none (300 rows of 50,257 bfloat16: up
+  // to 6,000 tokens 35 us, with 32 KB 40; up to 1,000 tokens 23.0, 21.7; none 17.8, 17.0, with 16 KB 19.5).
+  const int most = (a.history != nullptr && a.history_cap > 2048 ? 64 : 32) * 1024 / int(sizeof(W)) / PER;
   // as many segments as it takes to have three CTAs to an SM (none below 2,048 tokens), more where the places need it: every segment counts the
   // whole history. (256 bfloat16 rows of 128,001: four segments with 64 KB of places 52.9 us, eight with 32 KB 57.6; 64 float32 rows of
   // 50,257: seven segments 8.6, three 9.6, fourteen 11.0; one row: 24 segments 2.9, three 4.3, 49 2.8; eight rows: 24 segments 4.5, three 6.1, 49 4.6.)
