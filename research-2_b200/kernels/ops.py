@@ -2055,7 +2055,7 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
                   bias_ids: torch.Tensor | None = None, bias_values: torch.Tensor | None = None, mask: torch.Tensor | None = None,
                   mask_rows: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Penalties, biases and masks on rows of logits [R, V] (float32 or bfloat16) -> rows of the same type: new ones, or `out` (which may be
-    the logits themselves).
+    the logits themselves). Where nothing is asked of the logits and there is no `out`, they are what is returned.
 
     `history` int32 [S, L] holds tokens: row r's are history[slots[r], :lengths[r]] (`slots` None: history[r]), the first prompt_lengths[r]
     of them its prompt's (`prompt_lengths` None: none); tokens outside the vocabulary count for nothing. For a token of the prompt or the
@@ -2065,6 +2065,12 @@ def adjust_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, 
     and are added to their tokens, in order where a token is named more than once; tokens outside the vocabulary are left out.
     `mask` int32 [M, >= V / 32]: where bit t % 32 of word t / 32 of row mask_rows[r] is 0 the logit becomes -inf (`mask_rows` None: row r;
     a number outside [0, M): no mask). A mask that leaves nothing leaves a row of -inf, which `sample` answers with token 0."""
+    if (history is None and mask is None and bias_start is None and out is None and slots is None and lengths is None and prompt_lengths is None
+            and repetition is None and presence is None and frequency is None and bias_ids is None and bias_values is None and mask_rows is None):
+        _, _, vocab, ld, _ = _logit_rows(logits, "adjust_logits")
+        if ld < vocab:
+            raise KernelError("adjust_logits: rows of logits overlap")
+        return logits
     if logits.is_cuda:
         done = _logit_face("adjust_logits")(logits, history, slots, lengths, prompt_lengths, repetition, presence, frequency, bias_start, bias_ids,
                                             bias_values, mask, mask_rows, out)

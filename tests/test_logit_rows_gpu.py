@@ -676,6 +676,15 @@ def test_a_call_in_one_step_is_the_call_through_the_checks(dtype, offset, pad):
     assert torch.equal(o.adjust_logits(x[:1], **one), a[:1])
 
 
+def test_logits_of_which_nothing_is_asked():
+    x = random_logits(3, 40, 9).to(DEV)
+    assert ops().adjust_logits(x) is x
+    new = ops().adjust_logits(x, mask=i32([[-1, -1]] * 3))
+    assert new is not x and new.data_ptr() != x.data_ptr() and torch.equal(new, x)
+    to = torch.empty_like(x)
+    assert ops().adjust_logits(x, out=to) is to and torch.equal(to, x)
+
+
 def test_what_one_step_does_not_take():
     o, x = ops(), random_logits(3, 1280, 5).to(DEV)
     values, ids, log_sum = o.top_logits(x, 7)
