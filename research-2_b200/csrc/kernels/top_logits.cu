@@ -364,7 +364,7 @@ __device__ __noinline__ void blank_in(uint4& place, const RowPieces<T>& x, int g
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// What its readers do. Of every share its groups' and pairs' maxima and its warps' sums. -> the turn of the last one.
+// What its readers do. Of every share its groups' and threads' maxima and its warps' sums. -> the turn of the last one.
 template <typename T, typename ShareOf>
 __device__ __forceinline__ int read_shares(TopShared& shared, const ShareOf& share_of, int first_row, int rows, int step, int shift, float c, int tid,
                                            int* error) {
@@ -465,6 +465,10 @@ __device__ __forceinline__ int read_shares(TopShared& shared, const ShareOf& sha
     row_max = -INFINITY;
     left = slot = 0;
     ++turn;
+  }
+  if (lost) {  // (copies still under way get as long again: one of a barrier's two phases is always over)
+    for (int i = 0; i < STAGES; ++i)
+      for (uint32_t of = 0u; of < 2u; ++of) r2ptx::mbar_wait(r2ptx::smem_u32(&shared.full[i]), of);
   }
   return turn - 1;
 }
