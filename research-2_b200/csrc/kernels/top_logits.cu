@@ -18,8 +18,8 @@
 // have a kernel of their own, whose threads hold them: seven rows an SM, or 28 of a warp each.
 //
 // What bounds it. Bytes: the readers alone take 2,048 float32 rows of 50,257 at 6.6 TB/s, as fast as a copy. With the teams beside them (k 64)
-// a pass is 75.6 us (5.46 TB/s): choosing a row is a chain of some 16,000 cycles for a team, as long as two rows take to pass, and the last
-// row's 8,000 have nothing beside them. 1,000 bfloat16 rows of 128,001 (k 128): 63.0 us (4.08 TB/s), of which the readers take 50, for twice the
+// a pass is 75.7 us (5.45 TB/s): choosing a row is a chain of some 16,000 cycles for a team, as long as two rows take to pass, and the last
+// row's 8,000 have nothing beside them. 1,000 bfloat16 rows of 128,001 (k 128): 63.8 us (4.03 TB/s), of which the readers take 50, for twice the
 // exponentials a byte. A single row of 50,257 (k 5): 6.7 us, 2.6 of them until it is read, the rest the chain: a value by halving, groups, pieces, runs,
 // the cluster's hand-over.
 // Measured and not taken: readers' loads into their registers (85.2 and 67.1 us: what is on its way is bound by registers and by what shared
