@@ -28,7 +28,11 @@ namespace {
 constexpr int MOST_K = 256;
 constexpr int MOST_RANKS = 8;
 constexpr int MOST_WARPS = 12;     // of a block, that work on pieces
+constexpr uint32_t LANDING = 4096; // polls, some 16 ms, for 16 bytes that another CTA has sent already
 #define R2_ERR_TIMEOUT_SHARES 8
+#ifndef R2_SHARE_POLLS
+#define R2_SHARE_POLLS r2ptx::SPIN_LIMIT   // of a wait for a row's share or for the cluster's sums (a test lets them run out)
+#endif
 
 struct DistillArgs {
   const void* logits; long long ld;
@@ -156,8 +160,8 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t barrier, float4 v) {
                "f"(v.z), "f"(v.w), "r"(barrier)
                : "memory");
 }
-__device__ __forceinline__ bool arrived(uint32_t barrier, uint32_t parity) {   // false: gave up
-  for (uint32_t spin = 0; spin < r2ptx::SPIN_LIMIT; ++spin) {
+__device__ __forceinline__ bool arrived(uint32_t barrier, uint32_t parity, uint32_t polls = R2_SHARE_POLLS) {   // false: gave up
+  for (uint32_t spin = 0; spin < polls; ++spin) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -232,6 +236,11 @@ struct Sums {
 // A block is twelve warps (fewer for short rows) that work on pieces and one more that brings: it has the next row's share copied, brings
 // its list and takes its mass, and finishes the loss of the row before, all beside the others, which meet it once a row. Rows that weigh
 // nothing are not brought; `slot` counts the others, two at a time.
+//
+// A wait that ran out ends the CTA's walk: at the row's next barrier its threads learn of it, the rows from that one on become NaN (the loss in
+// the first CTA, each CTA's share of the gradient), and nothing more is copied or sent. The cluster's other CTAs then miss its sums and end
+// likewise. A CTA that gave up stays until the others have sent what they send, what they sent has had its time (LANDING), and its own copy has landed
+// or had as long again as a wait takes.
 template <typename T>
 __global__ void __launch_bounds__(32 * (MOST_WARPS + 1), 2)
 distill_held_kernel(const DistillArgs a) {
@@ -253,6 +262,17 @@ distill_held_kernel(const DistillArgs a) {
   int row = int(blockIdx.x) / ranks;
   uint32_t slot = 0;   // rows brought so far, less this one: its places are slot % 2, its barriers' phase slot / 2
   auto weight = [&](int r) { return r >= a.rows ? 0.f : a.weight != nullptr ? a.weight[r] : 1.f; };
+  uint32_t copies = 0;   // of one thread, begun
+  // The end of a CTA that gave up (all of its threads). The cluster's barrier counts CTAs that have ended as arrived. Which sums still come is not
+  // known: both phases of both barriers are waited for, one of which is over.
+  auto settle = [&]() {
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (tid != 0) return;
+    if (copies > 0) arrived(r2ptx::smem_u32(&landed), (copies - 1) & 1, r2ptx::SPIN_LIMIT);
+    for (uint32_t of = 0u; of < 4u; ++of) arrived(r2ptx::smem_u32(&shared_in[of >> 1]), of & 1, LANDING);
+  };
 
   if (warp == warps) {
     if (lane == 0) {
@@ -290,15 +310,21 @@ distill_held_kernel(const DistillArgs a) {
     if (w != 0.f) bring(row, 0);
     cluster_wait();
     for (int before = -1;; row += step) {
-      __syncthreads();
+      const bool gave_up = __syncthreads_or(0) != 0;
       if (before >= 0 && rank == 0) {   // the loss of the row before
-        float loss = 0.f;
-        if (w_before != 0.f) {
+        float loss = w_before != 0.f ? NAN : 0.f;
+        if (w_before != 0.f && !gave_up) {
           const int b = (slot - 1) & 1;
           const float2 t = of_teacher[b];
           loss = w_before * a.tau * a.tau * students[b].divergence(ids[b], teacher[b], xk[b], k, lane, tail, c, t.x, t.y);
         }
         if (lane == 0) a.loss[before] = loss;
+      }
+      if (gave_up) {
+        if (rank == 0 && lane == 0)
+          for (; row < a.rows; row += step) a.loss[row] = weight(row) != 0.f ? NAN : 0.f;
+        settle();
+        return;
       }
       if (row >= a.rows) return;
       const float w_after = weight(row + 2 * step);
@@ -317,6 +343,7 @@ distill_held_kernel(const DistillArgs a) {
   auto copy = [&](int r) {   // one thread's: a row's share into its place
     const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)r * a.ld, a.vocab);
     const uint32_t bytes = uint32_t(min(a.per, x.count - g0)) * 16u, barrier = r2ptx::smem_u32(&landed);
+    ++copies;
     r2ptx::mbar_expect_tx(barrier, bytes);
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(r2ptx::smem_u32(pieces)),
                  "l"(reinterpret_cast<const uint4*>(x.base) + g0), "r"(bytes), "r"(barrier)
@@ -325,6 +352,7 @@ distill_held_kernel(const DistillArgs a) {
   float w = weight(row), w_next = weight(row + step);
   cluster_wait();
   if (tid == 0 && w != 0.f) copy(row);
+  bool lost = false, gave_up = false;   // a wait of this thread ran out; of any of the CTA's
   for (; row < a.rows; row += step) {
     const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)row * a.ld, a.vocab);
     const int n = max(0, min(a.per, x.count - g0)), last = x.count - 1 - g0, zero = x.first(g0);
@@ -336,7 +364,8 @@ distill_held_kernel(const DistillArgs a) {
     const int low = g0 == 0 && x.phase > 0 ? 1 : 0, high = last >= 0 && last < n && !x.whole(g0 + last) ? min(n, last) : n;
     const int b = slot & 1;
     T* tokens = reinterpret_cast<T*>(pieces);
-    __syncthreads();   // the row's list is there; the row before has done with its own
+    gave_up = __syncthreads_or(lost) != 0;   // the row's list is there; the row before has done with its own
+    if (gave_up) break;
     // this lane's token at the row's ends (the first warp's: in a first piece, in a last piece)
     int end = -1;
     if (warp == 0 && lane < 2 * PER) {
@@ -352,7 +381,7 @@ distill_held_kernel(const DistillArgs a) {
     } else {
       const uint32_t barrier = r2ptx::smem_u32(&shared_in[b]), phase = (slot >> 1) & 1;
       ++slot;
-      if (!r2ptx::mbar_wait(r2ptx::smem_u32(&landed), (slot - 1) & 1) && lane == 0) atomicMax(a.error, R2_ERR_TIMEOUT_SHARES);
+      lost = !arrived(r2ptx::smem_u32(&landed), (slot - 1) & 1);
       if (end >= 0 && (zero + end < 0 || zero + end >= a.vocab)) {
         tokens[end] = from_float<T>(-INFINITY);
         end = -1;
@@ -387,10 +416,11 @@ distill_held_kernel(const DistillArgs a) {
         const uint4 raw[1] = {pieces[at]};
         sums.add(raw, c);
       }
+      if (lost) sums.others = NAN;   // (no sums of a share that is not there)
       const float3 joined = warp_join(make_float3(sums.reference, sums.in_list, sums.others));
       if (lane < ranks)
         send(cluster_address(&shares[b][rank * warps + warp], lane), cluster_address(&shared_in[b], lane), make_float4(joined.x, joined.y, joined.z, 0.f));
-      if (!arrived(barrier, phase) && lane == 0) atomicMax(a.error, R2_ERR_TIMEOUT_SHARES);
+      lost |= !arrived(barrier, phase);
       const float2 t = of_teacher[b];
       const Student q(shares[b], ranks * warps, lane, tail, t.y);
       if (tid == 0) students[b] = q;
@@ -422,7 +452,7 @@ distill_held_kernel(const DistillArgs a) {
       if (end >= 0) grad[zero + end] = from_float<T>(exp2_approx(fmaf(to_float(tokens[end]), c, -q.common)) * by);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (the next copy comes by another path than what was written here)
       meet();   // the listed tokens' gradients lie over what stands there
-      if (tid == 0 && w_next != 0.f) copy(row + step);
+      if (tid == 0 && w_next != 0.f && !lost) copy(row + step);
 #pragma unroll 1
       for (int j = tid; j < k; j += threads) {
         const int at = ids[b][j] - zero;
@@ -432,7 +462,17 @@ distill_held_kernel(const DistillArgs a) {
     w = w_next;
     w_next = w_after;
   }
-  __syncthreads();
+  if (!gave_up) gave_up = __syncthreads_or(lost) != 0;
+  if (!gave_up) return;
+  if (tid == 0) atomicMax(a.error, R2_ERR_TIMEOUT_SHARES);
+  for (int r = row - step; r < a.rows; r += step) {
+    const RowPieces<T> x(static_cast<const T*>(a.logits) + (long long)r * a.ld, a.vocab);
+    T* grad = static_cast<T*>(a.grad) + (long long)r * a.grad_ld;
+    const int end = min(a.vocab, x.first(g0 + a.per));
+    const T value = from_float<T>(weight(r) != 0.f ? NAN : 0.f);
+    for (int token = max(0, x.first(g0)) + tid; token < end; token += threads) grad[token] = value;
+  }
+  settle();
 }
 
 // Losses alone (one pass over the row), and gradients of rows that no cluster holds (two).

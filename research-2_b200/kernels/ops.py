@@ -153,6 +153,7 @@ def build_all(head_dims=()) -> None:
         _lib(source)
     faces_module()
     kernel_library("sfu_probe")  # (profiling/sfu_probe.py: a measurement, no part of a step)
+    kernel_library("distill", {"R2_SHARE_POLLS": 0})  # (waits that run out at once, for a test)
     for head_dim in head_dims:
         _lib_for_head_dim("attention_decode", head_dim)
         if head_dim <= 128:

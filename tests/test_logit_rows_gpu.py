@@ -711,3 +711,37 @@ def test_what_one_step_does_not_take():
                         ("bias_start", given["bias_start"][:3]), ("bias_start", None), ("bias_ids", None), ("bias_values", given["bias_values"][:2]),
                         ("mask", given["mask"][:, :39]), ("mask_rows", None), ("out", x[:, :1279]), ("out", x.cpu())):
         assert adjust(x, *{**given, name: wrong}.values()) is None, name
+
+
+# ---- waits that run out --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,vocab", [(1, 1031), (3, 50257), (700, 30011)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_distill_waits_that_run_out_leave_nan_and_a_code(rows, vocab, dtype):
+    """Every wait for a row's share or for the cluster's sums gives up at once, with copies and sums under way: rows that weigh something are
+    NaN, the others 0, the code says so, nothing is written beside the rows, and the next call is right."""
+    from research_2_b200.csrc.build import kernel_library
+
+    o = ops()
+    case = Distill(rows, vocab, 9, rows, dtype, True, 1.5, 1, 2)
+    case.weight[::3] = 0.0
+    if rows == 1:
+        case.weight[0] = 1.0
+    want = case.run()
+    entry = kernel_library("distill", {"R2_SHARE_POLLS": 0}).r2_distill
+    entry.argtypes = o._LOGIT_SIGNATURES["distill"]
+    ids, values, log_sum, weight = (t.to(DEV) for t in (case.ids, case.values, case.log_sum, case.weight))
+    loss = torch.full((rows,), -1.0, device=DEV)
+    buf = torch.full((rows, vocab + 3), -1.0, dtype=dtype, device=DEV)
+    grad = buf[:, 1: 1 + vocab]
+    assert entry(0 if dtype == F32 else 1, case.x.data_ptr(), case.x.stride(0), rows, vocab, ids.data_ptr(), values.data_ptr(), 9, log_sum.data_ptr(),
+                 weight.data_ptr(), 1.5, loss.data_ptr(), grad.data_ptr(), grad.stride(0), o._error_address(case.x), o._current_stream(0)) == 0
+    with pytest.raises(o.KernelTimeout):
+        o.raise_on_device_error(DEV)
+    weighs = weight != 0
+    assert torch.isnan(loss[weighs]).all() and torch.all(loss[~weighs] == 0)
+    assert torch.isnan(grad[weighs]).all() and torch.all(grad[~weighs] == 0)
+    assert torch.all(buf[:, 0] == -1) and torch.all(buf[:, 1 + vocab:] == -1)
+    again = case.run()
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+    assert o.device_errors(DEV) == 0
