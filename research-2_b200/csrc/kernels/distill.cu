@@ -9,10 +9,13 @@
 //
 // With "another token" both sides are whole distributions and the loss is summed as p log(p / q) - p + q, terms that are never negative: a
 // teacher and a student that nearly agree lose no digits to cancellation, and for the same reason the mass outside the list is summed from its own
-// tokens, not taken from 1. A row whose weight is 0 is not read: its loss and gradient are 0 whatever stands there.
+// tokens, not taken from 1. It is summed against a reference of its own: against the row's largest logit it would be nothing in 32 bits where the
+// list stands 87 temperatures above all others, and the outcome whose loss is largest would be lost. So its logarithm is at hand however little it
+// is, and the others' gradients, shares of what is pulled outside the list, are taken against that reference as well. "Another token" is left out
+// only where the student leaves it nothing at all. A row whose weight is 0 is not read: its loss and gradient are 0 whatever stands there.
 //
 // A row is read once and its gradient written once. The CTAs of a cluster hold a row's 16-byte pieces in shared memory between the two; a
-// thread sums exponentials against its own maximum, and every warp sends what it has to all CTAs of the cluster, whose barriers count the
+// thread sums exponentials against its own maxima, and every warp sends what it has to all CTAs of the cluster, whose barriers count the
 // bytes. Clusters walk over the rows: while one is worked on, the next one's pieces are on their way. The listed tokens are taken out of a
 // row (their places become -inf) before it is summed, so that what is left is summed without looking at the list. Losses alone, and rows that
 // no cluster holds, take a second kernel that streams.
@@ -44,12 +47,11 @@ struct DistillArgs {
   int* error;
 };
 
-// One (reference, sum over listed, sum over others) per lane into one per warp.
-__device__ __forceinline__ float3 warp_join(float3 v) {
-  const float common = warp_max(v.x), f = rebase(v.x, common);
-  return make_float3(common, warp_sum(v.y * f), warp_sum(v.z * f));
+// (reference, sum) over the listed tokens and over the others: one of every lane into one of the warp.
+__device__ __forceinline__ float4 warp_join(float4 v) {
+  const float listed = warp_max(v.x), others = warp_max(v.z);
+  return make_float4(listed, warp_sum(v.y * rebase(v.x, listed)), others, warp_sum(v.w * rebase(v.z, others)));
 }
-
 
 // What a row's list says, from shared memory, by every warp for itself: the logarithm that the teacher's exponentials are taken against, and
 // their sum's mass.
@@ -69,29 +71,37 @@ __device__ __forceinline__ float2 teacher_mass(const float* teacher, int k, int 
 
 // The student's side of a row, joined over its warps.
 struct Student {
-  float common, total, inv_total, rest, rest_p, outside, whole;
+  float common, total, inv_total, whole;   // whole: the mass that its tokens' gradients share
+  float rest, log_rest, rest_p;            // the mass outside the list, its logarithm (-inf: none at all), the teacher's where the student has some
+  float from, by;                          // an unlisted token's gradient: by 2^(x c - from)
 
   Student() = default;
-  // From (reference, sum over listed, sum over others) of every warp, by any warp for itself.
+  // From (reference, sum) over the listed and over the others of every warp, by any warp for itself.
   __device__ __forceinline__ Student(const float4* shares, int n, int lane, bool tail, float mass) {
-    float3 v = make_float3(-INFINITY, 0.f, 0.f);
+    float4 v = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
     for (int i = lane; i < n; i += 32) {
       const float4 s = shares[i];
-      const float m = fmaxf(v.x, s.x), f = rebase(v.x, m), g = rebase(s.x, m);
-      v = make_float3(m, v.y * f + s.y * g, v.z * f + s.z * g);
+      const float listed = fmaxf(v.x, s.x), others = fmaxf(v.z, s.z);
+      v = make_float4(listed, v.y * rebase(v.x, listed) + s.y * rebase(s.x, listed), others, v.w * rebase(v.z, others) + s.w * rebase(s.z, others));
     }
     v = warp_join(v);
-    common = v.x;
-    total = v.y + v.z;
+    common = fmaxf(v.x, v.z);
+    const float listed = v.y * rebase(v.x, common), others = v.w * rebase(v.z, common);   // (may be nothing in 32 bits)
+    total = listed + others;
     inv_total = __frcp_rn(total);
-    outside = whole = mass;
-    rest = v.z * inv_total;
+    rest = others * inv_total;
+    log_rest = -INFINITY;
     rest_p = 0.f;
-    if (tail) {
-      rest_p = rest > 0.f ? fmaxf(1.f - mass, 0.f) : 0.f;
+    whole = mass;
+    from = common;
+    by = mass * inv_total;
+    if (tail && v.w != 0.f) {
+      log_rest = rest > 1e-30f ? logf(rest) : (v.z - common + (log2f(v.w) - log2f(total))) * 0.693147181f;
+      rest_p = fmaxf(1.f - mass, 0.f);
       if (rest_p > 0.f) {
-        outside = __fdividef(mass - v.y * inv_total, rest);
         whole = 1.f;
+        from = v.z;
+        by = __fdividef(mass - listed * inv_total, v.w);
       }
     }
   }
@@ -109,8 +119,8 @@ struct Student {
     }
     kl = warp_sum(kl);
     if (tail) {
-      const float d = logf(rest_p) - logf(rest);
-      kl += rest_p > 0.f ? rest_p * (d + expm1f(-d)) : rest > 0.f ? rest : mass - 1.f;
+      const float d = logf(rest_p) - log_rest;
+      kl += rest_p > 0.f ? rest_p * (d + expm1f(-d)) : log_rest > -INFINITY ? rest : mass - 1.f;
     }
     return kl;
   }
@@ -179,21 +189,23 @@ __device__ __forceinline__ bool arrived(uint32_t barrier, uint32_t parity, uint3
 // Sums of exponentials against a reference that the thread chooses as it goes.
 template <typename T>
 struct Sums {
-  float reference = -INFINITY, in_list = 0.f, others = 0.f;   // an exponent of two; what is summed is 2^(x c - reference)
+  float reference = -INFINITY, sum = 0.f;   // an exponent of two; what is summed is 2^(x c - reference)
 
   __device__ __forceinline__ void raise(float to) {
     if (!(to > reference)) return;
-    const float f = rebase(reference, to);
-    in_list *= f;
-    others *= f;
+    sum *= rebase(reference, to);
     reference = to;
+  }
+  __device__ __forceinline__ void add(float x, float c) {
+    raise(x * c);
+    sum += exp2_approx(fmaf(x, c, -no_less(reference)));
   }
   // N pieces. The reference is raised where a sum leaves the middle of the range; a maximum of every piece is not looked for.
   template <int N>
   __device__ __forceinline__ void add(const uint4 (&raw)[N], float c) {
     constexpr int PAIRS = RowPieces<T>::PER / 2;
     const uint64_t cc = two_of(c, c);
-    float sum;
+    float more;
     auto exponentials = [&]() {
       const float shift = -no_less(reference);
       const uint64_t ss = two_of(shift, shift);
@@ -209,15 +221,15 @@ struct Sums {
 #pragma unroll
       for (int i = 1; i < N; ++i) acc[0] = add_two(acc[0], acc[i]);
       const float2 v = halves(acc[0]);
-      sum = v.x + v.y;
+      more = v.x + v.y;
     };
     exponentials();
-    if (reference == -INFINITY || !(sum > 1e-18f && sum < 1e18f)) {
+    if (reference == -INFINITY || !(more > 1e-18f && more < 1e18f)) {
       const float before = reference;
       raise(most(raw) * c);
       if (reference != before) exponentials();
     }
-    others += sum;
+    sum += more;
   }
   template <int N>
   static __device__ __forceinline__ float most(const uint4 (&raw)[N]) {
@@ -387,7 +399,7 @@ distill_held_kernel(const DistillArgs a) {
         end = -1;
       }
       if (tid == 0) r2ptx::mbar_expect_tx(barrier, uint32_t(ranks * warps) * 16u);
-      Sums<T> sums;
+      Sums<T> listed, sums;
 #pragma unroll 1
       for (int j = tid; j < k; j += threads) {
         const int at = ids[b][j] - zero;
@@ -395,8 +407,7 @@ distill_held_kernel(const DistillArgs a) {
         const float v = take_out(tokens + at);
         if (v == -INFINITY) twice[b] = 1;
         taken[j] = v;   // (read again behind a barrier)
-        sums.raise(v * c);
-        sums.in_list += exp2_approx(fmaf(v, c, -no_less(sums.reference)));
+        listed.add(v, c);
       }
       meet();
       int at = tid;
@@ -416,17 +427,17 @@ distill_held_kernel(const DistillArgs a) {
         const uint4 raw[1] = {pieces[at]};
         sums.add(raw, c);
       }
-      if (lost) sums.others = NAN;   // (no sums of a share that is not there)
-      const float3 joined = warp_join(make_float3(sums.reference, sums.in_list, sums.others));
+      if (lost) sums.sum = NAN;   // (no sums of a share that is not there)
+      const float4 joined = warp_join(make_float4(listed.reference, listed.sum, sums.reference, sums.sum));
       if (lane < ranks)
-        send(cluster_address(&shares[b][rank * warps + warp], lane), cluster_address(&shared_in[b], lane), make_float4(joined.x, joined.y, joined.z, 0.f));
+        send(cluster_address(&shares[b][rank * warps + warp], lane), cluster_address(&shared_in[b], lane), joined);
       lost |= !arrived(barrier, phase);
       const float2 t = of_teacher[b];
       const Student q(shares[b], ranks * warps, lane, tail, t.y);
       if (tid == 0) students[b] = q;
-      const float scale = w * a.tau, by = scale * q.outside * q.inv_total;
+      const float scale = w * a.tau, by = scale * q.by;
       if (vectors) {
-        const uint64_t cc = two_of(c, c), ss = two_of(-q.common, -q.common), bb = two_of(by, by);
+        const uint64_t cc = two_of(c, c), ss = two_of(-q.from, -q.from), bb = two_of(by, by);
         auto gradient = [&](const uint4& raw) {
           uint64_t p[PER / 2];
           unpack_pairs(raw, p, static_cast<const T*>(nullptr));
@@ -447,9 +458,9 @@ distill_held_kernel(const DistillArgs a) {
         for (; at < high; at += threads) out[at] = gradient(pieces[at]);
       } else {
 #pragma unroll 1
-        for (at = low * PER + tid; at < high * PER; at += threads) grad[zero + at] = from_float<T>(exp2_approx(fmaf(to_float(tokens[at]), c, -q.common)) * by);
+        for (at = low * PER + tid; at < high * PER; at += threads) grad[zero + at] = from_float<T>(exp2_approx(fmaf(to_float(tokens[at]), c, -q.from)) * by);
       }
-      if (end >= 0) grad[zero + end] = from_float<T>(exp2_approx(fmaf(to_float(tokens[end]), c, -q.common)) * by);
+      if (end >= 0) grad[zero + end] = from_float<T>(exp2_approx(fmaf(to_float(tokens[end]), c, -q.from)) * by);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (the next copy comes by another path than what was written here)
       meet();   // the listed tokens' gradients lie over what stands there
       if (tid == 0 && w_next != 0.f && !lost) copy(row + step);
@@ -518,19 +529,6 @@ distill_streamed_kernel(const DistillArgs a) {
     if (mark_listed(bits_s, ids, k, x.first(g0), n * PER, tid, THREADS)) twice = 1;
   __syncthreads();
   Sums<T> own;
-  if (TAIL) {
-    for (int j = tid; j < k; j += THREADS) {
-      const int at = ids[j] - x.first(g0);
-      if (ids[j] < 0 || at < 0 || at >= n * PER) continue;
-      // (of a token that the list names more than once, one entry counts)
-      bool first = true;
-      if (twice)
-        for (int o = 0; o < j; ++o) first &= ids[o] != ids[j];
-      if (!first) continue;
-      own.raise(xk[j] * c);
-      own.in_list += exp2_approx(fmaf(xk[j], c, -no_less(own.reference)));
-    }
-  }
   // listed tokens and places that are not the row's are -inf in what is summed
   auto clear = [&](uint4& raw, int at) {
     if (TAIL) {
@@ -571,15 +569,27 @@ distill_streamed_kernel(const DistillArgs a) {
     clear(one[0], at);
     own.add(one, c);
   }
-  const float reference = own.reference, in_list = own.in_list, others = own.others;
-  const float3 sums = warp_join(make_float3(reference, in_list, others));
+  Sums<T> listed;   // (here, not before the row: its registers are the row's)
+  if (TAIL) {
+    for (int j = tid; j < k; j += THREADS) {
+      const int at = ids[j] - x.first(g0);
+      if (ids[j] < 0 || at < 0 || at >= n * PER) continue;
+      // (of a token that the list names more than once, one entry counts)
+      bool first = true;
+      if (twice)
+        for (int o = 0; o < j; ++o) first &= ids[o] != ids[j];
+      if (!first) continue;
+      listed.add(xk[j], c);
+    }
+  }
+  const float4 sums = warp_join(make_float4(listed.reference, listed.sum, own.reference, own.sum));
   if (ranks > 1) {
     cluster_wait();
-    if (lane < ranks) cluster_store(cluster_address(&shares[rank * (THREADS / 32) + (tid >> 5)], lane), make_float4(sums.x, sums.y, sums.z, 0.f));
+    if (lane < ranks) cluster_store(cluster_address(&shares[rank * (THREADS / 32) + (tid >> 5)], lane), sums);
     cluster_arrive();
     cluster_wait();
   } else {
-    if (lane == 0) shares[tid >> 5] = make_float4(sums.x, sums.y, sums.z, 0.f);
+    if (lane == 0) shares[tid >> 5] = sums;
     __syncthreads();
   }
   if (grad == nullptr && (rank > 0 || tid >= 32)) return;
@@ -590,7 +600,7 @@ distill_streamed_kernel(const DistillArgs a) {
     if (lane == 0) a.loss[row] = w * a.tau * a.tau * kl;
   }
   if (grad == nullptr) return;
-  const float scale = w * a.tau, by = scale * q.outside * q.inv_total;
+  const float scale = w * a.tau, by = scale * q.by;
   for (int c0 = tid; c0 < n; c0 += DEPTH * THREADS) {
     uint4 raw[DEPTH];
 #pragma unroll
@@ -602,7 +612,7 @@ distill_streamed_kernel(const DistillArgs a) {
       float v[PER];
       unpack(raw[i], v, static_cast<const T*>(nullptr));
 #pragma unroll
-      for (int e = 0; e < PER; ++e) v[e] = exp2_approx(fmaf(v[e], c, -q.common)) * by;
+      for (int e = 0; e < PER; ++e) v[e] = exp2_approx(fmaf(v[e], c, -q.from)) * by;
       store_piece<T, PER>(grad, x.first(g0 + c0 + i * THREADS), a.vocab, v, vectors);
     }
   }
