@@ -192,13 +192,13 @@ struct Sums {
   float reference = -INFINITY, sum = 0.f;   // an exponent of two; what is summed is 2^(x c - reference)
 
   __device__ __forceinline__ void raise(float to) {
-    if (!(to > reference)) return;
+    if (!(to > reference && to > -FAR_REFERENCE)) return;   // (what is lower leaves it as it is: nothing summed)
     sum *= rebase(reference, to);
     reference = to;
   }
   __device__ __forceinline__ void add(float x, float c) {
     raise(x * c);
-    sum += exp2_approx(fmaf(x, c, -no_less(reference)));
+    sum += exp2_approx(fmaf(x, c, shift_to(reference)));
   }
   // N pieces. The reference is raised where a sum leaves the middle of the range; a maximum of every piece is not looked for.
   template <int N>
@@ -207,7 +207,7 @@ struct Sums {
     const uint64_t cc = two_of(c, c);
     float more;
     auto exponentials = [&]() {
-      const float shift = -no_less(reference);
+      const float shift = shift_to(reference);
       const uint64_t ss = two_of(shift, shift);
       uint64_t acc[N];
 #pragma unroll

@@ -140,7 +140,13 @@ __device__ __forceinline__ float exp2_approx(float x) {  // 2^x within 2^-22; 0 
   return y;
 }
 
-// Sums of exponentials are kept against a reference, an exponent of two; -inf where nothing has been summed.
+// Sums of exponentials are kept against a reference, an exponent of two; -inf where nothing has been summed. A reference is a rounded product, and
+// 2^x is taken of exact products less it: off by up to 64 for references below 2^31, which the sums bear, and by ever more beyond. What is
+// summed against a reference beyond counts as nothing, a mask's low number as well as one above any logit; infinity against it is infinity.
+constexpr float FAR_REFERENCE = 2147483648.f, LARGEST_FLOAT = 3.40282347e38f;
+__device__ __forceinline__ float shift_to(float reference) {
+  return fabsf(reference) < FAR_REFERENCE ? -reference : reference > 0.f ? -LARGEST_FLOAT : 0.f;
+}
 __device__ __forceinline__ float no_less(float reference) { return reference == -INFINITY ? 0.f : reference; }
 // what sums against `reference` are in sums against `common`, the largest of several references
 __device__ __forceinline__ float rebase(float reference, float common) { return reference == -INFINITY ? 0.f : exp2_approx(reference - common); }

@@ -140,6 +140,10 @@ __device__ __forceinline__ unsigned long long composite(uint32_t key, int token)
   return (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - uint32_t(token));
 }
 
+// The logarithm of `total` against `common`; of a row that is nothing against it (FAR_REFERENCE), the largest term's, beside which the others' number
+// does not show.
+__device__ __forceinline__ float log_sum_of(float common, float total) { return (total != 0.f ? common + log2f(total) : common) * 0.693147181f; }
+
 __device__ __forceinline__ uint32_t floor_bits(float v) { return uint32_t(__bfloat16_as_ushort(__float2bfloat16_rd(v))); }
 // bfloat16 bits as 16-bit keys in the numbers' order, and back
 __device__ __forceinline__ uint32_t short_key(uint32_t bits) { return (bits & 0x8000u) ? ~bits & 0xffffu : bits | 0x8000u; }
@@ -421,7 +425,7 @@ __device__ __forceinline__ int read_shares(TopShared& shared, const ShareOf& sha
       sum *= rebase(reference, up);
       reference = up;
     }
-    const float minus = -no_less(reference);
+    const float minus = shift_to(reference);
     const uint64_t ss = two_of(minus, minus);
     auto sum_of = [&](const uint4& piece) {
       uint64_t p[PAIRS];
@@ -536,7 +540,7 @@ __device__ __forceinline__ void choose(const TopArgs& a, TopShared& shared, Shar
   const int k = min(a.k, end_token - first_token);   // of this share
   float common = 0.f, total = 0.f;   // (the second warp's)
   auto write_sum = [&]() {
-    if (lane == 0) a.log_sum[r] = (no_less(common) + log2f(total)) * 0.693147181f;
+    if (lane == 0) a.log_sum[r] = log_sum_of(common, total);
   };
   if (warp == 1) {
     const float2 part = lane < READING_WARPS ? place.sums[lane] : make_float2(-INFINITY, 0.f);
@@ -829,7 +833,7 @@ top_short_kernel(const TopArgs a) {
     most[i] = largest<T, 1>(one);
     row_most = fmaxf(row_most, most[i]);
   }
-  const float reference = warp_max(fminf(row_most * c, 3e38f)), minus = -no_less(reference);
+  const float reference = warp_max(fminf(row_most * c, 3e38f)), minus = shift_to(reference);
   const uint64_t cc = two_of(c, c), ss = two_of(minus, minus);
   uint64_t acc = 0ull;
 #pragma unroll
@@ -849,7 +853,7 @@ top_short_kernel(const TopArgs a) {
     common = warp_max(part.x);
     total = warp_sum(part.y * rebase(part.x, common));
   }
-  if (tid == 0) a.log_sum[r] = (no_less(common) + log2f(total)) * 0.693147181f;
+  if (tid == 0) a.log_sum[r] = log_sum_of(common, total);
 
   // what k pieces' maxima reach, or k numbers where there are not twice as many pieces: two values tried at a time (counts in 16 bits each)
   const bool fine = n < 2 * k;
