@@ -69,6 +69,13 @@ __device__ __forceinline__ float2 teacher_mass(const float* teacher, int k, int 
   return make_float2(against, warp_sum(mass));
 }
 
+// p log(p / q) - p + q of one outcome. Where q is larger by far, e^(log q - log p) is beyond 32 bits before p times it is, and nothing cancels.
+__device__ __forceinline__ float outcome(float p, float log_p, float log_q) {
+  const float d = log_p - log_q;
+  if (!(p > 0.f)) return expf(log_q);
+  return d < -1.f ? p * d + (expf(log_q) - p) : p * (d + expm1f(-d));
+}
+
 // The student's side of a row, joined over its warps.
 struct Student {
   float common, total, inv_total, whole;   // whole: the mass that its tokens' gradients share
@@ -113,15 +120,12 @@ struct Student {
     float kl = 0.f;
     for (int j = lane; j < k; j += 32) {
       if (ids[j] < 0) continue;
-      const float lq = (fmaf(xk[j], c, -common) - log2_total) * 0.693147181f, lp = teacher[j] - against, p = expf(lp), d = lp - lq;
-      if (tail) kl += p > 0.f ? p * (d + expm1f(-d)) : expf(lq);
-      else if (p > 0.f) kl += p * d;
+      const float lq = (fmaf(xk[j], c, -common) - log2_total) * 0.693147181f, lp = teacher[j] - against, p = expf(lp);
+      if (tail) kl += outcome(p, lp, lq);
+      else if (p > 0.f) kl += p * (lp - lq);
     }
     kl = warp_sum(kl);
-    if (tail) {
-      const float d = logf(rest_p) - log_rest;
-      kl += rest_p > 0.f ? rest_p * (d + expm1f(-d)) : log_rest > -INFINITY ? rest : mass - 1.f;
-    }
+    if (tail) kl += rest_p > 0.f ? outcome(rest_p, logf(rest_p), log_rest) : log_rest > -INFINITY ? rest : mass - 1.f;
     return kl;
   }
 };

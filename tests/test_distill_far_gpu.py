@@ -111,3 +111,16 @@ def test_distill_gradient_of_a_far_list_against_differences():
         got = float((gradient[r].double().cpu() * direction[r]).sum())
         # h^2 of a third derivative below 10; losses below 200 in 64 bits: 200 * 2^-52 / h; the gradient's numbers, below 1 in all, by 3e-5
         assert abs(got - slope) <= 1e-7 + 1e-9 + 3e-5 * float(direction[r].abs().max()) * 2, (got, slope)
+
+
+@pytest.mark.parametrize("faint", [-60.0, -86.0, -90.0, -95.0, -99.0, -103.0, -110.0])
+@pytest.mark.parametrize("tau", [1.0, 0.1])
+@pytest.mark.parametrize("vocab", [64, 50257])
+def test_distill_entries_of_hardly_any_mass(faint, tau, vocab):
+    """Listed tokens of which the teacher thinks next to nothing (below 32 bits' normal numbers, or nothing in 32 bits at all) and the student does not."""
+    case = Far(3, vocab, 6, 0, tau)
+    case.teacher[:, 3] = (case.log_sum.double() + faint).float() * tau
+    case.teacher[1, 5] = case.teacher[1, 3]
+    loss, gradient = case.run()
+    case.check(loss, gradient)
+    case.check(case.run(gradient=False)[0], None)
