@@ -125,6 +125,7 @@ struct Student {
       else if (p > 0.f) kl += p * (lp - lq);
     }
     kl = warp_sum(kl);
+    if (!(total > 0.f) && (tail || mass > 0.f)) return NAN;   // a row of nothing (without outcomes there is nothing to compare)
     if (tail) kl += rest_p > 0.f ? outcome(rest_p, logf(rest_p), log_rest) : log_rest > -INFINITY ? rest : mass - 1.f;
     return kl;
   }

@@ -124,3 +124,20 @@ def test_distill_entries_of_hardly_any_mass(faint, tau, vocab):
     loss, gradient = case.run()
     case.check(loss, gradient)
     case.check(case.run(gradient=False)[0], None)
+
+
+@pytest.mark.parametrize("vocab", [40, 50257])
+@pytest.mark.parametrize("tail", [True, False])
+def test_distill_rows_of_nothing_have_no_loss(vocab, tail):
+    """Logits that are all -inf, that hold infinity or NaN, or that no reference reaches: NaN, with entries and without."""
+    case = Far(9, vocab, 5, 0, 1.0)
+    x = case.x.clone()
+    x[0:2] = -math.inf
+    x[2:4] = torch.finfo(F32).min
+    x[4, 3], x[5, 3] = math.inf, math.nan
+    x[6, case.ids[6, 0].item()], x[7, case.ids[7, 0].item()] = math.inf, math.nan
+    case.ids[[1, 3, 5]] = -1
+    for gradient in (True, False):
+        loss, _ = ops().distill_loss(x, case.ids.to(DEV), case.teacher.to(DEV), log_sum=case.log_sum.to(DEV) if tail else None, gradient=gradient)
+        # (without the other outcome and without entries nothing is compared: 0)
+        assert torch.isnan(loss[:8] if tail else loss[[0, 2, 4, 6, 7]]).all() and torch.isfinite(loss[8])
