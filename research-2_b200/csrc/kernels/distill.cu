@@ -126,7 +126,7 @@ struct Student {
     }
     kl = warp_sum(kl);
     if (!(total > 0.f) && (tail || mass > 0.f)) return NAN;   // a row of nothing (without outcomes there is nothing to compare)
-    if (tail) kl += rest_p > 0.f ? outcome(rest_p, logf(rest_p), log_rest) : log_rest > -INFINITY ? rest : mass - 1.f;
+    if (tail) kl += rest_p > 0.f ? outcome(rest_p, logf(rest_p), log_rest) : (log_rest > -INFINITY ? rest : 0.f) + (mass - 1.f);
     return kl;
   }
 };

@@ -2154,8 +2154,8 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
     loss = weight * temperature^2 * KL(p || q). `log_sum` float32 [R] (top_logits' at the same temperature): p_k = exp(teacher / temperature -
     log_sum), and what is left of p stands against what is left of q as one more outcome (where the student leaves nothing, that outcome is
     left out). Without it p = softmax(teacher / temperature) over the listed tokens alone. `weight` float32 [R]: a row of weight 0 is not
-    read; its loss and gradient are 0. A row without entries and without `log_sum` has the loss 0, any other whose logits are all -inf (or as low as a type goes), or hold
-    +inf or NaN, a loss of NaN."""
+    read; its loss and gradient are 0. A row without entries and without `log_sum` has the loss 0, any other whose logits are all -inf (or as low
+    as a type goes), or hold +inf or NaN, a loss of NaN."""
     if logits.is_cuda:
         done = _logit_face("distill")(logits, ids, teacher, log_sum, temperature, weight, gradient, out, _error_address(logits))
         if done is not None:

@@ -141,3 +141,12 @@ def test_distill_rows_of_nothing_have_no_loss(vocab, tail):
         loss, _ = ops().distill_loss(x, case.ids.to(DEV), case.teacher.to(DEV), log_sum=case.log_sum.to(DEV) if tail else None, gradient=gradient)
         # (without the other outcome and without entries nothing is compared: 0)
         assert torch.isnan(loss[:8] if tail else loss[[0, 2, 4, 6, 7]]).all() and torch.isfinite(loss[8])
+
+
+@pytest.mark.parametrize("mass", [1.002, 1.3])
+@pytest.mark.parametrize("vocab", [40, 50257])
+def test_distill_lists_of_more_than_the_whole_mass(mass, vocab):
+    """A teacher's logits that were rounded after their sum was taken: more than 1 on the list, nothing left beside it."""
+    case = Far(3, vocab, 6, 0, 1.0, mass=mass)
+    case.check(*case.run())
+    case.check(case.run(gradient=False)[0], None)
