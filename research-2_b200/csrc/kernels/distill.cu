@@ -250,6 +250,17 @@ struct Sums {
   }
 };
 
+// What a CTA has in shared memory beside its pieces and the sums.
+struct __align__(16) HeldShared {
+  uint64_t landed, shared_in[2];     // barriers: a row's share is there; every warp of the cluster has sent its sums
+  int32_t ids[2][MOST_K];
+  float teacher[2][MOST_K], xk[2][MOST_K], taken[MOST_K];
+  float2 of_teacher[2];              // what the teacher's exponentials are taken against, and their sum
+  Student students[2];
+  int twice[2];
+};
+constexpr int sums_bytes(int ranks, int warps) { return 2 * ranks * warps * int(sizeof(float4)); }   // (reference, sum) twice of every warp
+
 // A block is twelve warps (fewer for short rows) that work on pieces and one more that brings: it has the next row's share copied, brings
 // its list and takes its mass, and finishes the loss of the row before, all beside the others, which meet it once a row. Rows that weigh
 // nothing are not brought; `slot` counts the others, two at a time.
@@ -262,14 +273,14 @@ template <typename T>
 __global__ void __launch_bounds__(32 * (MOST_WARPS + 1), 2)
 distill_held_kernel(const DistillArgs a) {
   constexpr int PER = RowPieces<T>::PER, AHEAD = 16 / PER;   // pieces that a thread takes at a time
-  extern __shared__ __align__(16) uint4 pieces[];            // of this CTA's share
-  __shared__ __align__(16) float4 shares[2][MOST_RANKS * MOST_WARPS];
-  __shared__ __align__(8) uint64_t landed, shared_in[2];     // barriers: a row's share is there; every warp of the cluster has sent its sums
-  __shared__ int32_t ids[2][MOST_K];
-  __shared__ float teacher[2][MOST_K], xk[2][MOST_K], taken[MOST_K];
-  __shared__ float2 of_teacher[2];   // what the teacher's exponentials are taken against, and their sum
-  __shared__ Student students[2];
-  __shared__ int twice[2];
+  extern __shared__ __align__(16) uint4 pieces[];            // of this CTA's share; behind them the sums of two rows
+  __shared__ HeldShared shared;
+  uint64_t &landed = shared.landed, (&shared_in)[2] = shared.shared_in;
+  int32_t (&ids)[2][MOST_K] = shared.ids;
+  float (&teacher)[2][MOST_K] = shared.teacher, (&xk)[2][MOST_K] = shared.xk, (&taken)[MOST_K] = shared.taken;
+  float2 (&of_teacher)[2] = shared.of_teacher;
+  Student (&students)[2] = shared.students;
+  int (&twice)[2] = shared.twice;
   pdl_launch_dependents();
   const int threads = int(blockDim.x) - 32, warps = threads >> 5;   // that work on pieces
   const int ranks = a.ranks, step = int(gridDim.x) / ranks, rank = int(blockIdx.x) % ranks, tid = int(threadIdx.x), lane = tid & 31, warp = tid >> 5;
@@ -433,12 +444,13 @@ distill_held_kernel(const DistillArgs a) {
         sums.add(raw, c);
       }
       if (lost) sums.sum = NAN;   // (no sums of a share that is not there)
+      float4* of_warps = reinterpret_cast<float4*>(pieces + a.per) + b * ranks * warps;
       const float4 joined = warp_join(make_float4(listed.reference, listed.sum, sums.reference, sums.sum));
       if (lane < ranks)
-        send(cluster_address(&shares[b][rank * warps + warp], lane), cluster_address(&shared_in[b], lane), joined);
+        send(cluster_address(of_warps + rank * warps + warp, lane), cluster_address(&shared_in[b], lane), joined);
       lost |= !arrived(barrier, phase);
       const float2 t = of_teacher[b];
-      const Student q(shares[b], ranks * warps, lane, tail, t.y);
+      const Student q(of_warps, ranks * warps, lane, tail, t.y);
       if (tid == 0) students[b] = q;
       const float scale = w * a.tau, by = scale * q.by;
       if (vectors) {
@@ -634,6 +646,10 @@ constexpr int MOST_STREAMED_BITS = 1 << 20;   // tokens of a CTA's share (128 KB
 // the other's copies (1,024 rows of 50,257: two CTAs of 100 KB a row 75 us, one of 200 KB with an SM to itself 77, shares for three or
 // four CTAs an SM 100 to 117); eight CTAs of a whole SM each hold the longest rows.
 constexpr int HELD_TWO = 6600, HELD_ONE = 13600;
+constexpr int SM_BYTES = 228 * 1024, CTA_BYTES = 227 * 1024, RESERVED = 1024;   // shared memory; RESERVED: the system's of every CTA's
+// (eight CTAs' sums are 0.3 KB too many: rows of eight shares of more than 6,584 pieces have the SMs to themselves)
+static_assert(2 * (HELD_TWO * 16 + sums_bytes(MOST_RANKS - 1, MOST_WARPS) + int(sizeof(HeldShared)) + RESERVED) <= SM_BYTES, "two CTAs an SM");
+static_assert(HELD_ONE * 16 + sums_bytes(MOST_RANKS, MOST_WARPS) + int(sizeof(HeldShared)) <= CTA_BYTES, "one CTA an SM");
 
 template <typename T>
 int launch_held(const DistillArgs& a, cudaStream_t stream) {
@@ -641,9 +657,9 @@ int launch_held(const DistillArgs& a, cudaStream_t stream) {
   // float32 numbers: twelve warps 62 us, three 30; 2,000 of 12,000: twelve 61, five 52; 100 of 4,000: twelve 6.0, three 6.2, one 8.0). By the row alone: its
   // sums are then added in the same order in every call.
   const int warps = max(1, min(min(MOST_WARPS, a.per / 64), max(3, a.per / 512)));
-  const size_t smem = size_t(a.per) * 16;
+  const size_t smem = size_t(a.per) * 16 + size_t(sums_bytes(a.ranks, warps));
   static std::atomic<bool> allowed[64];
-  const int status = allow_smem(distill_held_kernel<T>, size_t(HELD_ONE) * 16, allowed);
+  const int status = allow_smem(distill_held_kernel<T>, size_t(HELD_ONE) * 16 + sums_bytes(MOST_RANKS, MOST_WARPS), allowed);
   if (status != R2_OK) return status;
   // how many clusters run at a time, asked once for each device and shape (a table that forgets)
   struct Resident {
