@@ -729,38 +729,43 @@ int launch(DistillArgs a, cudaStream_t stream) {
   return launch_held<T>(a, stream);
 }
 
-// Rows times a factor each; a row whose factor is 1 is not touched.
+// Rows times a factor each. In place a row whose factor is 1 is not touched.
 template <typename T>
 __global__ void __launch_bounds__(256)
-scale_rows_kernel(T* x, long long ld, int vocab, int slices, const float* factors, int factor_step) {
+scale_rows_kernel(const T* x, long long ld, T* out, long long out_ld, int vocab, int slices, const float* factors, int factor_step) {
   pdl_launch_dependents();
   pdl_wait();
   const int row = int(blockIdx.x) / slices, slice = int(blockIdx.x) % slices;
   const float f = factors[(long long)row * factor_step];
-  if (f == 1.f) return;
-  T* at = x + (long long)row * ld;
+  const T* at = x + (long long)row * ld;
+  T* to = out + (long long)row * out_ld;
+  if (f == 1.f && at == to) return;
+  const bool vectors = ((reinterpret_cast<uintptr_t>(at) ^ reinterpret_cast<uintptr_t>(to)) & 15) == 0;
   const RowPieces<T> pieces(at, vocab);
   for (int g = slice * 2048 + int(threadIdx.x); g < min(pieces.count, (slice + 1) * 2048); g += 256) {
     float v[RowPieces<T>::PER];
     unpack(load_once(pieces, g), v, static_cast<const T*>(nullptr));
 #pragma unroll
     for (int e = 0; e < RowPieces<T>::PER; ++e) v[e] *= f;
-    store_piece<T, RowPieces<T>::PER>(at, pieces.first(g), vocab, v, true);
+    store_piece<T, RowPieces<T>::PER>(to, pieces.first(g), vocab, v, vectors);
   }
 }
 
 }  // namespace
 
-// x [rows, vocab] of dtype with row stride ld, in place, times factors[row * factor_step].
-extern "C" int r2_scale_rows(int dtype, void* x, long long ld, int rows, int vocab, const float* factors, int factor_step, cudaStream_t stream) {
+// x [rows, vocab] of dtype with row stride ld, times factors[row * factor_step] -> out of dtype with row stride out_ld (x itself, or apart from it).
+extern "C" int r2_scale_rows(int dtype, const void* x, long long ld, void* out, long long out_ld, int rows, int vocab, const float* factors,
+                             int factor_step, cudaStream_t stream) {
   if (dtype != R2_F32 && dtype != R2_BF16) return R2_BAD_DTYPE;
-  if (rows < 0 || vocab < 1 || vocab > (1 << 30) || ld < vocab || factor_step < 0 || factor_step > 1) return R2_BAD_SHAPE;
+  if (rows < 0 || vocab < 1 || vocab > (1 << 30) || ld < vocab || out_ld < vocab || factor_step < 0 || factor_step > 1) return R2_BAD_SHAPE;
   if (rows == 0) return R2_OK;
   const int per = dtype == R2_F32 ? 4 : 8, slices = ((vocab + 2 * per - 2) / per + 2047) / 2048;
   if ((long long)rows * slices > 0x7fffffffLL) return R2_BAD_SHAPE;
   const dim3 grid(unsigned(rows) * unsigned(slices));
-  if (dtype == R2_F32) r2_launch(scale_rows_kernel<float>, grid, dim3(256), size_t(0), stream, static_cast<float*>(x), ld, vocab, slices, factors, factor_step);
-  else r2_launch(scale_rows_kernel<bf16>, grid, dim3(256), size_t(0), stream, static_cast<bf16*>(x), ld, vocab, slices, factors, factor_step);
+  if (dtype == R2_F32)
+    r2_launch(scale_rows_kernel<float>, grid, dim3(256), size_t(0), stream, static_cast<const float*>(x), ld, static_cast<float*>(out), out_ld, vocab, slices, factors, factor_step);
+  else
+    r2_launch(scale_rows_kernel<bf16>, grid, dim3(256), size_t(0), stream, static_cast<const bf16*>(x), ld, static_cast<bf16*>(out), out_ld, vocab, slices, factors, factor_step);
   return launch_status();
 }
 

@@ -1935,7 +1935,7 @@ _LOGIT_SIGNATURES = {
     "top_logits": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float] + [C.c_void_p] * 5,
     "distill": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
                 C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p],
-    "scale_rows": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p],
+    "scale_rows": [C.c_int, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p],
 }
 _LOGIT_LIBRARIES = {"scale_rows": "distill"}   # where the library has another name than the entry
 _logit_entries: dict = {}
@@ -2184,12 +2184,14 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
     return loss, grad
 
 
-def scale_rows(x: torch.Tensor, factors: torch.Tensor) -> torch.Tensor:
-    """Rows x [R, V] (float32 or bfloat16) times a float32 factor each, in place; `factors` has one for every row, or one for all. A row whose
-    factor is 1 is not touched, so that a gradient which is wanted as it stands costs a look at its factors."""
+def scale_rows(x: torch.Tensor, factors: torch.Tensor, *, in_place: bool = True) -> torch.Tensor:
+    """Rows x [R, V] (float32 or bfloat16) times a float32 factor each; `factors` has one for every row, or one for all. In place a row whose
+    factor is 1 is not touched, so that a gradient which is wanted as it stands costs a look at its factors; else new rows are written."""
     code, rows, vocab, ld, device = _logit_rows(x, "scale_rows")
     one = factors.numel() == 1
     at = _per_row(factors.reshape(1) if one else factors, "factors", torch.float32, 1 if one else rows, device)
+    out, out_ld = (x, ld) if in_place else _like_logits(x, ld, None, "scale_rows")
     if rows:
-        _check(_logit_entry("scale_rows")(code, x.data_ptr(), ld, rows, vocab, at, 0 if one else 1, _current_stream(device)), "scale_rows")
-    return x
+        _check(_logit_entry("scale_rows")(code, x.data_ptr(), ld, out.data_ptr(), out_ld, rows, vocab, at, 0 if one else 1, _current_stream(device)),
+               "scale_rows")
+    return out

@@ -1,12 +1,17 @@
 """A student's loss against a teacher's top logits, for training with torch's gradients: the kernels behind `kernels.ops.distill_loss` compute loss
 and gradient in one pass over the logits, so the backward pass only scales the gradient by what comes down from above, and not even
-that where it is 1 (give a mean's 1 / n as `weight`, and sum)."""
+that where it is 1 (give a mean's 1 / n as `weight`, and sum). Where the graph is kept (`retain_graph`) the scaled gradient is written apart, and
+every backward pass over it starts from the same one."""
 
 from __future__ import annotations
 
 import torch
 
 from ..kernels import ops
+
+
+# Whether the backward pass that runs keeps its graph, in which what a node has saved is wanted again. (Where torch cannot say: it may.)
+_graph_is_kept = getattr(torch._C._autograd, "_get_current_graph_task_keep_graph", lambda: True)
 
 
 class _DistillLoss(torch.autograd.Function):
@@ -22,8 +27,7 @@ class _DistillLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, above):
         (gradient,) = ctx.saved_tensors
-        # (a copy only for a graph that is kept and run backwards once more would need one; torch forbids the second run by default)
-        return ops.scale_rows(gradient, above.to(torch.float32).contiguous()), None, None, None, None, None
+        return ops.scale_rows(gradient, above.to(torch.float32).contiguous(), in_place=not _graph_is_kept()), None, None, None, None, None
 
 
 def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, *, log_sum: torch.Tensor | None = None, temperature: float = 1.0,
