@@ -87,11 +87,15 @@ class StepControls:
         self._history: torch.Tensor | None = None
         self._done: torch.cuda.Event | None = None
 
-    def add(self, rid: int, controls: Controls, n_prompt: int) -> None:
+    def asked(self, controls: Controls, n_prompt: int) -> _Request:
+        """What a request will ask of its rows; its grammar is asked what may come first, so what is wrong with it shows here, before there is a request."""
         biases = sorted((controls.logit_bias or {}).items())
         request = _Request(controls, n_prompt, np.array([t for t, _ in biases], dtype=np.int32), np.array([v for _, v in biases], dtype=np.float32))
         if controls.grammar is not None:
             request.mask = allowed_words(controls.grammar, self.vocab_size)
+        return request
+
+    def add(self, rid: int, request: _Request) -> None:
         self.requests[rid] = request
 
     def forget(self, rid: int, keep: bool = False) -> None:

@@ -62,18 +62,22 @@ class Engine:
             controls = controls.checked(vocab_size)
         if seed is None:
             seed = (self.seed & 0xFFFFFFFF) | ((self._ordinal & 0xFFFFFFFF) << 32)
+        request = None
+        if controls:
+            config = self.scheduler.config
+            if self._controls is None:
+                from .controls import StepControls
+
+                self._controls = StepControls(self.step_fn, config.max_requests, config.max_seq_len, vocab_size)
+            if sum(self.scheduler.counts()) < config.max_requests:   # (else the scheduler refuses, and the grammar need not be asked)
+                request = self._controls.asked(controls, len(prompt))
         rid = self.scheduler.submit(prompt, max_new_tokens, temperature, top_k, seed, stop_token_ids)
         self._ordinal += 1
         self._pending[rid] = []
         if self._controls is not None:
             self._controls.forget(rid)   # (an id that is given again)
-        if controls:
-            if self._controls is None:
-                from .controls import StepControls
-
-                config = self.scheduler.config
-                self._controls = StepControls(self.step_fn, config.max_requests, config.max_seq_len, vocab_size)
-            self._controls.add(rid, controls, len(prompt))
+        if request is not None:
+            self._controls.add(rid, request)
         return rid
 
     def logprobs(self, rid: int):
