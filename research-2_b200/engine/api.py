@@ -5,6 +5,10 @@ rid = engine.submit(prompt, max_new_tokens=12); done = engine.wait(rid)`
 
 from __future__ import annotations
 
+import copy
+import dataclasses
+from collections import Counter
+
 from ..config.engine_options import EngineOptions
 from ..models.loading import load_model
 from .engine import Engine
@@ -26,7 +30,8 @@ def generate(  # noqa: PLR0913
 ) -> list[list[int]]:
     """Token ids in, token ids out: every prompt's continuation, in the order of `prompts`.
     Request i draws with key (seed, i), so its tokens do not depend on the batch it runs in.
-    `controls`: one `Controls` for all prompts, or one (or None) for each."""
+    `controls`: one `Controls` for all prompts, or one (or None) for each. A grammar that stands in the controls of several prompts is copied
+    for each of them, unless it says that it is `stateless`."""
     options.setdefault("max_requests", max(1, min(len(prompts), 256)))
     with run(model, device=device, dtype=dtype, seed=seed, **options) as engine:
         return generate_with(engine, prompts, max_new_tokens, temperature, top_k, seed, stop_token_ids, controls=controls)
@@ -42,9 +47,16 @@ def generate_with(engine: Engine, prompts, max_new_tokens, temperature=0.0, top_
     if isinstance(controls, (list, tuple)) and len(controls) != len(prompts):
         raise ValueError(f"{len(prompts)} prompts and controls for {len(controls)}")
 
+    each = list(controls) if isinstance(controls, (list, tuple)) else [controls] * len(prompts)
+    uses = Counter(id(c.grammar) for c in each if c is not None)
+
     def asked(i: int) -> dict:
-        own = controls[i] if isinstance(controls, (list, tuple)) else controls
-        return {} if own is None else {"controls": own}
+        own = each[i]
+        if own is None:
+            return {}
+        if own.grammar is not None and uses[id(own.grammar)] > 1 and not getattr(own.grammar, "stateless", False):
+            own = each[i] = dataclasses.replace(own, grammar=copy.deepcopy(own.grammar))   # (as it stands here: nobody tells this one anything)
+        return {"controls": own}
 
     out: list[list[int]] = [[] for _ in prompts]
     live: dict[int, int] = {}

@@ -89,6 +89,9 @@ class StepControls:
 
     def asked(self, controls: Controls, n_prompt: int) -> _Request:
         """What a request will ask of its rows; its grammar is asked what may come first, so what is wrong with it shows here, before there is a request."""
+        shared = controls.grammar is not None and any(r.controls.grammar is controls.grammar for r in self.requests.values())
+        if shared and not getattr(controls.grammar, "stateless", False):
+            raise ValueError("this grammar follows another request: give each request one of its own (or let it say that it is `stateless`)")
         biases = sorted((controls.logit_bias or {}).items())
         request = _Request(controls, n_prompt, np.array([t for t, _ in biases], dtype=np.int32), np.array([v for _, v in biases], dtype=np.float32))
         if controls.grammar is not None:

@@ -2,7 +2,9 @@
 tokens, a grammar, and the log-probabilities beside its tokens.
 
 A grammar is any object with two methods: `allowed()` returns which tokens may come next, as truth values [vocabulary] or as the words
-that `pack_mask` makes of them, and `advance(token)` tells it which one came. `AllowedTokens` is the simplest: the same tokens every time."""
+that `pack_mask` makes of them, and `advance(token)` tells it which one came. A grammar follows one request; one that answers the same whatever
+came says so by an attribute `stateless` that is true, and may serve any number of requests. `AllowedTokens` is the simplest: the same tokens
+every time."""
 
 from __future__ import annotations
 
@@ -26,6 +28,8 @@ def pack_mask(allowed: np.ndarray) -> np.ndarray:
 
 class AllowedTokens:
     """The grammar of a set of tokens: every next token is one of them."""
+
+    stateless = True
 
     def __init__(self, tokens, vocab_size: int):
         tokens = np.asarray(list(tokens), dtype=np.int64)

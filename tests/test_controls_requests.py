@@ -7,8 +7,9 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from research_2_b200.engine.api import generate_with
 from research_2_b200.engine.scheduler import Full
-from research_2_b200.sampling.controls import Controls
+from research_2_b200.sampling.controls import AllowedTokens, Controls
 from tests.test_controls import controlled_engine
 from tests.test_engine_protocol import VOCAB, continuation
 
@@ -64,3 +65,39 @@ def test_a_full_engine_does_not_ask_the_grammar():
         engine.wait(first)
         second = engine.submit([7], 2, controls=Controls(grammar=grammar))
         assert engine.wait(second).new_tokens == continuation([7], 2) and grammar.asked > 0
+
+
+@pytest.mark.parametrize("max_requests", [1, 2, 3])
+@pytest.mark.parametrize("as_list", [False, True])
+def test_a_grammar_for_several_prompts_follows_each_of_them(max_requests, as_list):
+    prompts = [[5, 6], [7], [8, 9, 10], [11]]
+    controls = Controls(grammar=Turns(1), top_logprobs=1)
+    with controlled_engine(max_requests=max_requests) as engine:
+        got = generate_with(engine, prompts, 6, controls=[controls, None, controls, controls] if as_list else controls)
+    assert controls.grammar.n == 1, "the one that was given is told nothing"
+    for i, tokens in enumerate(got):
+        if as_list and i == 1:
+            assert tokens == continuation(prompts[1], 6)
+        else:
+            assert [t % 3 for t in tokens] == [1, 2, 0, 1, 2, 0]
+
+
+def test_a_prompt_s_own_grammar_is_told_what_came():
+    own, other = Turns(), Turns(2)
+    with controlled_engine() as engine:
+        got = generate_with(engine, [[5], [6]], 4, controls=[Controls(grammar=own), Controls(grammar=other)])
+    assert (own.n, other.n) == (4, 6) and [t % 3 for t in got[1]] == [2, 0, 1, 2]
+
+
+def test_a_grammar_that_follows_a_request_is_refused_for_another():
+    shared = Turns()
+    allowed = AllowedTokens([3, 4, 5], VOCAB)
+    with controlled_engine(max_requests=4) as engine:
+        a = engine.submit([5], 3, controls=Controls(grammar=shared))
+        with pytest.raises(ValueError, match="another request"):
+            engine.submit([6], 3, controls=Controls(grammar=shared))
+        b, c = (engine.submit([6], 2, controls=Controls(grammar=allowed)) for _ in range(2))
+        assert len(engine.wait(a).new_tokens) == 3 and len(engine.wait(b).new_tokens) == len(engine.wait(c).new_tokens) == 2
+        again = engine.submit([6], 3, controls=Controls(grammar=shared))   # (its request has ended)
+        assert [t % 3 for t in engine.wait(again).new_tokens] == [0, 1, 2]
+        assert not engine.has_work()
