@@ -21,6 +21,14 @@ class _Request:
     bias_values: np.ndarray
     mask: np.ndarray | None = None      # words, what the grammar allows next
     logprobs: list[TokenLogprobs] = field(default_factory=list)
+    not_forbidden: np.ndarray | None = None   # words, what biases of -inf leave (None: there are none)
+
+    def nothing_left(self) -> bool:
+        """Whether no token may be drawn."""
+        if self.not_forbidden is None:
+            return self.mask is not None and not self.mask.any()
+        left = self.not_forbidden if self.mask is None else self.mask & self.not_forbidden
+        return not left.any()
 
 
 def allowed_words(grammar, vocab_size: int) -> np.ndarray:
@@ -94,6 +102,11 @@ class StepControls:
             raise ValueError("this grammar follows another request: give each request one of its own (or let it say that it is `stateless`)")
         biases = sorted((controls.logit_bias or {}).items())
         request = _Request(controls, n_prompt, np.array([t for t, _ in biases], dtype=np.int32), np.array([v for _, v in biases], dtype=np.float32))
+        forbidden = request.bias_ids[request.bias_values == -np.inf]
+        if len(forbidden):
+            left = np.ones(self.vocab_size, dtype=bool)
+            left[forbidden] = False
+            request.not_forbidden = pack_mask(left)
         if controls.grammar is not None:
             request.mask = allowed_words(controls.grammar, self.vocab_size)
         return request
@@ -114,11 +127,13 @@ class StepControls:
         return list(request.logprobs)
 
     def check(self, is_live) -> None:
-        """Raises NoTokenAllowed where a live request's grammar allows nothing (asked again each time: it may have been told more)."""
+        """Raises NoTokenAllowed where a live request's grammar allows nothing, or nothing that its biases do not forbid (the grammar is asked
+        again each time: it may have been told more)."""
         for rid, request in self.requests.items():
-            if request.mask is not None and not request.mask.any() and is_live(rid):
-                request.mask = allowed_words(request.controls.grammar, self.vocab_size)
-                if not request.mask.any():
+            if request.nothing_left() and is_live(rid):
+                if request.mask is not None:
+                    request.mask = allowed_words(request.controls.grammar, self.vocab_size)
+                if request.nothing_left():
                     raise NoTokenAllowed(rid)
 
     def concerns(self, plan) -> bool:

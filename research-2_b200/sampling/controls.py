@@ -96,10 +96,10 @@ class TokenLogprobs:
 
 
 class NoTokenAllowed(RuntimeError):
-    """A running request's grammar allows no token: cancel the request, or step on once its grammar does."""
+    """A running request's grammar allows no token, or none that its biases do not forbid: cancel the request, or step on once its grammar does."""
 
     def __init__(self, req_id: int):
-        super().__init__(f"request {req_id}: its grammar allows no token")
+        super().__init__(f"request {req_id}: its grammar and its biases allow no token")
         self.req_id = req_id
 
 

@@ -3,13 +3,14 @@ token. The engine stands above a step function that has no GPU."""
 
 from __future__ import annotations
 
+import math
 
 import numpy as np
 import pytest
 
 from research_2_b200.engine.api import generate_with
 from research_2_b200.engine.scheduler import Full
-from research_2_b200.sampling.controls import AllowedTokens, Controls
+from research_2_b200.sampling.controls import AllowedTokens, Controls, NoTokenAllowed
 from tests.test_controls import controlled_engine
 from tests.test_engine_protocol import VOCAB, continuation
 
@@ -101,3 +102,43 @@ def test_a_grammar_that_follows_a_request_is_refused_for_another():
         again = engine.submit([6], 3, controls=Controls(grammar=shared))   # (its request has ended)
         assert [t % 3 for t in engine.wait(again).new_tokens] == [0, 1, 2]
         assert not engine.has_work()
+
+
+@pytest.mark.parametrize("controls", [dict(grammar=AllowedTokens([7, 9], VOCAB), logit_bias={7: -math.inf, 9: -math.inf, 3: 1.0}),
+                                      dict(logit_bias=dict.fromkeys(range(VOCAB), -math.inf))])
+def test_biases_that_leave_no_token_are_said_before_the_next_plan(controls):
+    with controlled_engine() as engine:
+        rid = engine.submit([5, 6], 4, controls=Controls(**controls, top_logprobs=1))
+        other = engine.submit([9], 3)
+        for _ in range(2):
+            with pytest.raises(NoTokenAllowed) as raised:
+                engine.step()
+            assert raised.value.req_id == rid
+        engine.cancel(rid)
+        assert engine.wait(other).new_tokens == continuation([9], 3)
+
+
+def test_biases_that_leave_a_token_are_no_error():
+    some = {t: -math.inf for t in range(VOCAB) if t != 40}
+    with controlled_engine() as engine:
+        a = engine.submit([5, 6], 3, controls=Controls(logit_bias=some))
+        b = engine.submit([5, 6], 3, controls=Controls(grammar=AllowedTokens([40, 41], VOCAB), logit_bias={41: -math.inf, 40: -5.0}))
+        assert len(engine.wait(a).new_tokens) == len(engine.wait(b).new_tokens) == 3
+
+
+def test_a_grammar_that_comes_to_what_biases_forbid():
+    class Narrowing(Turns):
+        def allowed(self):
+            return np.arange(VOCAB) == 50 + self.n
+
+        def advance(self, token):
+            self.n += 1
+
+    with controlled_engine() as engine:
+        rid = engine.submit([5, 6], 9, controls=Controls(grammar=Narrowing(), logit_bias={52: -math.inf}))
+        engine.step()
+        engine.step()
+        with pytest.raises(NoTokenAllowed):
+            engine.step()
+        assert engine.poll(rid).new_tokens == [50, 51]
+        engine.cancel(rid)
