@@ -22,6 +22,7 @@ class _Request:
     mask: np.ndarray | None = None      # words, what the grammar allows next
     logprobs: list[TokenLogprobs] = field(default_factory=list)
     not_forbidden: np.ndarray | None = None   # words, what biases of -inf leave (None: there are none)
+    failure: Exception | None = None          # of its grammar, when it was told a token or asked after it
 
     def nothing_left(self) -> bool:
         """Whether no token may be drawn."""
@@ -128,8 +129,10 @@ class StepControls:
 
     def check(self, is_live) -> None:
         """Raises NoTokenAllowed where a live request's grammar allows nothing, or nothing that its biases do not forbid (the grammar is asked
-        again each time: it may have been told more)."""
+        again each time: it may have been told more), and what its grammar raised when it was told a token."""
         for rid, request in self.requests.items():
+            if request.failure is not None and is_live(rid):
+                raise request.failure
             if request.nothing_left() and is_live(rid):
                 if request.mask is not None:
                     request.mask = allowed_words(request.controls.grammar, self.vocab_size)
@@ -184,7 +187,9 @@ class StepControls:
         return out
 
     def committed(self, plan, tokens: np.ndarray) -> None:
-        """After the step's commit: grammars go on, log-probabilities are written down."""
+        """After the step's commit: grammars go on, log-probabilities are written down. What a grammar raises is raised when all requests have
+        been seen to (and again before each step, while its request lives: nobody knows what it allows)."""
+        failure = None
         for e, (rid, emits) in enumerate(zip(plan.req, plan.emits)):
             request = self.requests.get(int(rid)) if emits else None
             if request is None:
@@ -195,5 +200,11 @@ class StepControls:
                 top = tuple((int(i), float(v - log_sum)) for v, i in zip(values[:n_top], ids[:n_top]))
                 request.logprobs.append(TokenLogprobs(int(tokens[e]), float(chosen - log_sum), top))
             if request.controls.grammar is not None:
-                request.controls.grammar.advance(int(tokens[e]))
-                request.mask = allowed_words(request.controls.grammar, self.vocab_size)
+                try:
+                    request.controls.grammar.advance(int(tokens[e]))
+                    request.mask = allowed_words(request.controls.grammar, self.vocab_size)
+                except Exception as raised:  # noqa: BLE001
+                    request.failure = raised
+                    failure = failure or raised
+        if failure is not None:
+            raise failure

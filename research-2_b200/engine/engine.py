@@ -169,10 +169,10 @@ class Engine:
     def _controlled_step(self, batch, plan) -> StepEvent:
         tokens = self._controls.step(batch, plan)
         self.commit(tokens)
-        self._controls.committed(plan, tokens)   # (the plan's arrays hold until the next one)
         event = self.scheduler.event()
         if self.keep_events:
             self.events.append(event)
+        self._controls.committed(plan, tokens)   # (the plan's arrays hold until the next one)
         return event
 
     def finish(self, want_event: bool = True) -> StepEvent | None:

@@ -142,3 +142,48 @@ def test_a_grammar_that_comes_to_what_biases_forbid():
             engine.step()
         assert engine.poll(rid).new_tokens == [50, 51]
         engine.cancel(rid)
+
+
+@pytest.mark.parametrize("when", ["told", "asked"])
+def test_a_grammar_that_fails_fails_alone(when):
+    """What one request's grammar raises is raised by the step, and again until the request is cancelled; the others' grammars and records go on."""
+    class Failing(Turns):
+        def advance(self, token):
+            super().advance(token)
+            if when == "told" and self.n == 2:
+                raise OSError("lost")
+
+        def allowed(self):
+            if when == "asked" and self.n == 2:
+                raise OSError("lost")
+            return super().allowed()
+
+    other = Turns(1)
+    with controlled_engine() as engine:
+        engine.keep_events = True
+        bad = engine.submit([5, 6], 6, controls=Controls(grammar=Failing()))
+        good = engine.submit([7], 6, controls=Controls(grammar=other, top_logprobs=1))
+        engine.step()
+        for _ in range(3):
+            with pytest.raises(OSError, match="lost"):
+                engine.step()
+        assert other.n == 3 and len(engine.logprobs(good)) == 2 and len(engine.events) == 2
+        assert [t % 3 for t in engine.poll(bad).new_tokens] == [0, 1]
+        engine.cancel(bad)
+        assert [t % 3 for t in engine.wait(good).new_tokens] == [1, 2, 0, 1, 2, 0]
+        assert [r.token % 3 for r in engine.logprobs(good)] == [1, 2, 0, 1, 2, 0]
+
+
+def test_a_grammar_that_fails_at_its_last_token():
+    class Failing(Turns):
+        def advance(self, token):
+            super().advance(token)
+            if self.n == 2:
+                raise OSError("lost")
+
+    with controlled_engine() as engine:
+        bad, other = engine.submit([5, 6], 2, controls=Controls(grammar=Failing())), engine.submit([9], 4)
+        engine.step()
+        with pytest.raises(OSError):
+            engine.step()
+        assert engine.poll(bad).finished and engine.wait(other).new_tokens == continuation([9], 4)
