@@ -34,7 +34,12 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
                  weight: torch.Tensor | None = None) -> torch.Tensor:
     """weight * temperature^2 * KL(teacher || student) of every row, float32 [R], with a gradient for `logits` [R, V] (float32 or bfloat16). `ids`
     and `teacher` [R, K] are a teacher's top logits and `log_sum` [R] the logarithm of its sum of exponentials at this temperature, as
-    `ops.top_logits` and the `teach` command give them; without `log_sum` the teacher's probabilities are spread over its K tokens alone."""
+    `ops.top_logits` and the `teach` command give them; without `log_sum` the teacher's probabilities are spread over its K tokens alone. There is
+    no gradient for them nor for `weight`: one that asks for it is refused (`detach()` it)."""
+    if torch.is_grad_enabled():
+        for name, t in (("teacher", teacher), ("log_sum", log_sum), ("weight", weight)):
+            if t is not None and t.requires_grad:
+                raise ops.KernelError(f"distill_loss: {name} asks for a gradient and there is none: detach() it")
     return _DistillLoss.apply(logits, ids, teacher, log_sum, temperature, weight)
 
 

@@ -96,3 +96,12 @@ def test_scale_rows_into_new_rows(dtype, vocab, offset):
         assert got.data_ptr() != x.data_ptr() and got.dtype == dtype
         assert torch.equal(got, (x.float() * factors.reshape(-1, 1)).to(dtype)) and torch.equal(buf, before)
     assert ops.scale_rows(x[:0], torch.ones(1, device="cuda:0"), in_place=False).shape == (0, vocab)
+
+
+@pytest.mark.parametrize("name", ["teacher", "log_sum", "weight"])
+def test_what_has_no_gradient_is_refused_where_it_asks_for_one(name):
+    given = {"teacher": torch.randn(2, 3), "log_sum": torch.randn(2), "weight": torch.ones(2)}
+    given[name].requires_grad_()
+    x, ids = torch.randn(2, 9, requires_grad=True), torch.tensor([[0, 1, 2]] * 2, dtype=torch.int32)
+    with pytest.raises(ops.KernelError, match=f"{name} asks for a gradient"):
+        distill.distill_loss(x, ids, given.pop("teacher"), **given)
