@@ -10,10 +10,11 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import warnings
 
 import torch
 
-from ..csrc.build import faces_module, kernel_library
+from ..csrc.build import BuildError, faces_module, kernel_library
 
 F32, BF16 = 0, 1
 ACT_NONE, ACT_GELU_TANH, ACT_GELU_ERF = 0, 1, 2
@@ -151,7 +152,7 @@ def build_all(head_dims=()) -> None:
     for source in ("rowwise", "recurrent", "state_scan", "decay_chunks", "streams", "routing", "gemm_simt", "gemm_tc", "few_rows", "step_io", "attention_simt", "attention_prefill_tc", "latent_attention",
                    "sampling", "adjust_logits", "top_logits", "distill", "wait_selftest"):
         _lib(source)
-    faces_module()
+    _faces()
     kernel_library("sfu_probe")  # (profiling/sfu_probe.py: a measurement, no part of a step)
     kernel_library("distill", {"R2_SHARE_POLLS": 0})  # (waits that run out at once, for a test)
     for head_dim in head_dims:
@@ -1958,11 +1959,35 @@ _logit_faces: dict = {}
 _error_addresses: dict = {}
 
 
+class _NoFaces:
+    """Where the faces cannot be built (they need Python's and torch's headers): every call goes through the checks here."""
+
+    def bind(self, name: str, address: int) -> None:
+        pass
+
+    def __getattr__(self, name: str):
+        return lambda *arguments: None
+
+
+_faces_built = None
+
+
+def _faces():
+    global _faces_built
+    if _faces_built is None:
+        try:
+            _faces_built = faces_module()
+        except BuildError as err:
+            warnings.warn(f"operators on rows of logits are called through ctypes, some 8 us a call slower: {err}", stacklevel=2)
+            _faces_built = _NoFaces()
+    return _faces_built
+
+
 def _logit_face(name: str):
     """The operator called with tensors (`csrc/faces`): (status, tensors ...) for a plain call, None for one that the checks here have to look at."""
     face = _logit_faces.get(name)
     if face is None or face[0] is not _libs.get(name):
-        entry, module = _logit_entry(name), faces_module()
+        entry, module = _logit_entry(name), _faces()
         module.bind(name, C.cast(entry, C.c_void_p).value)
         face = _logit_faces[name] = (_libs[name], getattr(module, name))
     return face[1]
