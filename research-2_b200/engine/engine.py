@@ -117,7 +117,16 @@ class Engine:
     # ---- steps -----------------------------------------------------------------------------
     def plan(self) -> Plan | None:
         """The next step's entries, or None when there is nothing to run (the by-hand rung:
-        kelpie_engine/sdk/engine.py:585-601). Follow with `commit`."""
+        kelpie_engine/sdk/engine.py:585-601). Follow with `commit`. Controls are laid on logits by `step` alone: while a request
+        that has some is live, this refuses."""
+        if self._controls is not None and any(self._is_live(rid) for rid in self._controls.requests):
+            raise RuntimeError("a live request has controls, which only step() lays on its logits")
+        return self._next_plan()
+
+    def _is_live(self, rid: int) -> bool:
+        return not self.scheduler.request_info(rid)["state"].startswith("finished")
+
+    def _next_plan(self) -> Plan | None:
         self.finish(want_event=self.keep_events)   # (the record is only built where someone will read it)
         plan = self.scheduler.plan()
         if plan.n_entries == 0:
@@ -148,8 +157,8 @@ class Engine:
         what earlier steps produced); the return value is then None."""
         if self._controls is not None and self._controls.requests:
             self.finish(want_event=self.keep_events)
-            self._controls.check(lambda rid: not self.scheduler.request_info(rid)["state"].startswith("finished"))
-        plan = self.plan()
+            self._controls.check(self._is_live)
+        plan = self._next_plan()
         if plan is None:
             return None
         batch = self.build_batch(plan)

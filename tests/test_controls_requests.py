@@ -187,3 +187,17 @@ def test_a_grammar_that_fails_at_its_last_token():
         with pytest.raises(OSError):
             engine.step()
         assert engine.poll(bad).finished and engine.wait(other).new_tokens == continuation([9], 4)
+
+
+def test_plans_by_hand_refuse_requests_with_controls():
+    with controlled_engine() as engine:
+        rid = engine.submit([5, 6], 2, controls=Controls(grammar=Turns()))
+        with pytest.raises(RuntimeError, match="only step"):
+            engine.plan()
+        engine.step()
+        engine.step()
+        other = engine.submit([9], 2)
+        plan = engine.plan()   # (the one with controls has ended, polled or not)
+        assert plan.n_entries == 1 and engine.build_batch(plan).n_entries == 1
+        engine.commit([3])
+        assert engine.poll(rid).finished and engine.wait(other).new_tokens[0] == 3
