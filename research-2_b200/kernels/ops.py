@@ -9,6 +9,7 @@ are made here on the host: dtypes, contiguity, shapes, and that index tensors ar
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import os
 import warnings
 
@@ -2156,6 +2157,10 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0):
             _check(done[0], "top_logits")
             return done[1:]
     code, rows, vocab, ld, device = _logit_rows(logits, "top_logits")
+    try:
+        k = operator.index(k)
+    except TypeError:
+        raise KernelError(f"top_logits: k must be a whole number, got {k!r}") from None
     if not 1 <= k <= min(vocab, TOP_MOST):
         raise KernelError(f"top_logits: k must be in [1, {min(vocab, TOP_MOST)}], got {k}")
     temperature = _temperature(temperature, "top_logits")

@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -42,3 +43,17 @@ def test_operators_without_faces(no_faces):
     assert torch.all(loss.abs() < 1e-5) and torch.all(gradient.abs() < 1e-5)   # a student that is its teacher
     assert torch.equal(ops.adjust_logits(x, mask=torch.full((3, 33), -1, dtype=torch.int32, device="cuda:0")), x)
     assert len(no_faces) == 1
+
+
+@pytest.mark.gpu
+def test_numbers_that_are_not_python_s_own():
+    """The face takes Python's numbers; the checks behind it whatever is one."""
+    x = torch.randn(3, 1031, device="cuda:0")
+    want = ops.top_logits(x, 5, temperature=2.0)
+    for k, temperature in ((np.int64(5), 2.0), (np.uint8(5), np.float32(2.0)), (torch.tensor(5), torch.tensor(2.0)), (5, np.float64(2.0)), (5, 2)):
+        assert all(torch.equal(a, b) for a, b in zip(ops.top_logits(x, k, temperature=temperature), want))
+    before = ops.launch_count()
+    for k in (5.0, "5", None, np.float64(5)):
+        with pytest.raises(ops.KernelError):
+            ops.top_logits(x, k)
+    assert ops.launch_count() == before
