@@ -20,9 +20,10 @@
 // row (their places become -inf) before it is summed, so that what is left is summed without looking at the list. Losses alone, and rows that
 // no cluster holds, take a second kernel that streams.
 //
-// What bounds it. 1,024 float32 rows of 50,257 (64 listed): 75 us for 399 MB, 5.3 TB/s, 0.81 of a copy; nothing runs beside the first share's arrival
-// and the last one's gradient, 8 us. 4,096 bfloat16 rows (32 listed): 153 us, 5.1 TB/s: the special-function units are busy 58 % of the time,
-// with two exponentials a number. Losses of 2,047 float32 rows of 128,001: 156 us, 6.3 TB/s, 0.96 of a copy. 16 rows of 1,031: 4.9 us, a row's chain.
+// What bounds it. 1,024 float32 rows of 50,257 (64 listed): 75.7 us for 399 MB, 5.3 TB/s, 0.81 of a copy (with the list alone as outcomes the
+// same); nothing runs beside the first share's arrival and the last one's gradient, 8 us. 4,096 bfloat16 rows (32 listed): 155 us, 5.0 TB/s (165 with
+// "another token"): the special-function units are busy 57 % of the time, with two exponentials a number. Losses of 2,047 float32 rows of
+// 128,001: 155 us, 6.3 TB/s, 0.97 of a copy; of bfloat16 rows 98 us, 5.4 TB/s. 16 rows of 1,031: 5.0 us, a row's chain.
 #include "logit_rows.cuh"
 #include "sm100_ptx.cuh"
 
@@ -654,8 +655,8 @@ static_assert(HELD_ONE * 16 + sums_bytes(MOST_RANKS, MOST_WARPS) + int(sizeof(He
 template <typename T>
 int launch_held(const DistillArgs& a, cudaStream_t stream) {
   // Short rows get few warps, so that more of them are in hand: two pieces a thread at least, and beyond three warps sixteen (4,096 rows of 4,000
-  // float32 numbers: twelve warps 62 us, three 30; 2,000 of 12,000: twelve 61, five 52; 100 of 4,000: twelve 6.0, three 6.2, one 8.0). By the row alone: its
-  // sums are then added in the same order in every call.
+  // float32 numbers: twelve warps 62.6 us, three 30.0, one 38.5; 2,000 of 12,000: twelve 47.3, five 42.0, one 56.5; 100 of 4,000: twelve 6.0, three 6.3,
+  // one 8.1). By the row alone: its sums are then added in the same order in every call.
   const int warps = max(1, min(min(MOST_WARPS, a.per / 64), max(3, a.per / 512)));
   const size_t smem = size_t(a.per) * 16 + size_t(sums_bytes(a.ranks, warps));
   static std::atomic<bool> allowed[64];
@@ -714,8 +715,8 @@ int launch_streamed(DistillArgs a, int pieces, cudaStream_t stream) {
   a.per = (pieces + a.ranks - 1) / a.ranks;
   if (a.per * RowPieces<T>::PER > MOST_STREAMED_BITS) return R2_UNSUPPORTED;
   if ((long long)a.rows * a.ranks > 0x7fffffffLL) return R2_BAD_SHAPE;
-  // Half the threads where the rows are more than four CTAs an SM (2,047 rows of 128,001, 100 listed: 163 us with 256 threads, 156 with 128;
-  // 4,096 of 4,000: 45, 29; but 592 of 50,257: 19.9, 24.5).
+  // Half the threads where the rows are more than four CTAs an SM (2,047 rows of 128,001, 100 listed: 163 us with 256 threads, 155 with 128;
+  // 4,096 of 4,000, 64 listed: 54.1, 33.4; but 592 of 50,257: 21.8, 26.1).
   if ((long long)a.rows * a.ranks > 592) return launch_streamed<T, TAIL, 128>(a, stream);
   return launch_streamed<T, TAIL, 256>(a, stream);
 }
@@ -730,6 +731,8 @@ int launch(DistillArgs a, cudaStream_t stream) {
 }
 
 // Rows times a factor each. In place a row whose factor is 1 is not touched.
+// A CTA has 2,048 pieces, eight a thread, one under way each. 1,024 float32 rows of 50,257: 70 us into new rows (floor 63), 84 in place, 8 where
+// all factors are 1; bfloat16 38, 44 and 5.
 template <typename T>
 __global__ void __launch_bounds__(256)
 scale_rows_kernel(const T* x, long long ld, T* out, long long out_ld, int vocab, int slices, const float* factors, int factor_step) {

@@ -19,8 +19,9 @@
 //
 // What bounds it. Bytes: the readers alone take 2,048 float32 rows of 50,257 at 6.6 TB/s, as fast as a copy. With the teams beside them (k 64)
 // a pass is 75.7 us (5.45 TB/s): choosing a row is a chain of some 16,000 cycles for a team, as long as two rows take to pass, and the last
-// row's 8,000 have nothing beside them. 1,000 bfloat16 rows of 128,001 (k 128): 63.8 us (4.03 TB/s), of which the readers take 50, for twice the
-// exponentials a byte. A single row of 50,257 (k 5): 6.7 us, 2.6 of them until it is read, the rest the chain: a value by halving, groups, pieces, runs,
+// row's 8,000 have nothing beside them. 1,000 bfloat16 rows of 128,001 (k 128): 63.8 us (4.03 TB/s), of which the readers alone take 50 (a copy
+// 39): schedulers issue in 56 % of the cycles and the special-function units are busy in 52 %, so neither is full; a round's exponentials wait
+// for that round's maximum. A single row of 50,257 (k 5): 6.7 us, 2.6 of them until it is read, the rest the chain: a value by halving, groups, pieces, runs,
 // the cluster's hand-over.
 // Measured and not taken: readers' loads into their registers (85.2 and 67.1 us: what is on its way is bound by registers and by what shared
 // memory leaves of L1), two stages (83.0, 63.7), three teams of three warps (75.6, 64.3) or four (81.2, 62.3), 20 reading warps (79.0, 63.5).
@@ -931,9 +932,9 @@ top_short_kernel(const TopArgs a) {
 template <typename T>
 int launch(TopArgs a, int rows, cudaStream_t stream) {
   const int pieces = (a.vocab + 2 * RowPieces<T>::PER - 2) / RowPieces<T>::PER;   // of a row at any alignment, at most
-  // Rows that 128 threads hold in their registers (4,096 rows of 4,000 float32 numbers, k 64: 36 us, the other kernel 69; 16 rows 6.0, 6.1). One
-  // warp where that does, there is a row for every scheduler and k is not large (4,096 rows of 300, k 10: 8.4 us, 128 threads 19.5; but 300 rows
-  // of 1,000, k 100: 9.9, 7.9; 2,000 of them, k 256: 36.5, 31.6).
+  // Rows that 128 threads hold in their registers (4,096 rows of 4,000 float32 numbers, k 64: 37.3 us, the other kernel 69.7; 16 rows 6.0, 5.9). One
+  // warp where that does, there is a row for every scheduler and k is not large (4,096 rows of 300, k 10: 8.2 us, 128 threads 19.5; but 300 rows
+  // of 1,000, k 100: 9.8, 9.0; 2,000 of them, k 128: 25.8, 24.6, k 256: 37.5, 31.4).
   if (pieces <= SHORT_PIECES * SHORT_THREADS) {
     if (pieces <= SHORT_PIECES * 32 && rows >= 4 * 148 && a.k <= 128) r2_launch(top_short_kernel<T, 32>, dim3(unsigned(rows)), dim3(32), size_t(0), stream, a);
     else r2_launch(top_short_kernel<T, SHORT_THREADS>, dim3(unsigned(rows)), dim3(SHORT_THREADS), size_t(0), stream, a);

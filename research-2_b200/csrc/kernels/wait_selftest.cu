@@ -30,7 +30,7 @@ __global__ void wait_selftest_kernel(int* error_flag, uint32_t polls, int code) 
 
 }  // namespace
 
-// polls is capped at the kernels' own limit (a quarter of a second of polling at most).
+// polls is capped at the kernels' own limit (some 17 seconds: a poll that finds nothing takes 4 us).
 extern "C" int r2_wait_selftest(int* error_flag, unsigned polls, int code, cudaStream_t stream) {
   if (error_flag == nullptr || code < 1) return R2_BAD_SHAPE;
   if (polls > r2ptx::SPIN_LIMIT) polls = r2ptx::SPIN_LIMIT;

@@ -2182,8 +2182,8 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
     `logits` [R, V] are the student's (float32 or bfloat16), `ids` int32 [R, K] and `teacher` float32 [R, K] the teacher's top logits (K up to
     256; a token stands once in a row; an id outside the vocabulary, -1 say, is no entry). With q = softmax(logits / temperature),
     loss = weight * temperature^2 * KL(p || q). `log_sum` float32 [R] (top_logits' at the same temperature): p_k = exp(teacher / temperature -
-    log_sum), and what is left of p stands against what is left of q as one more outcome (where the student leaves nothing, that outcome is
-    left out). Without it p = softmax(teacher / temperature) over the listed tokens alone. `weight` float32 [R]: a row of weight 0 is not
+    log_sum), and what is left of p stands against what is left of q as one more outcome, however little that is (where the student leaves nothing
+    at all, logits of -inf or as low as a type goes, that outcome is left out). Without it p = softmax(teacher / temperature) over the listed tokens alone. `weight` float32 [R]: a row of weight 0 is not
     read; its loss and gradient are 0. A row without entries and without `log_sum` has the loss 0, any other whose logits are all -inf (or as low
     as a type goes), or hold +inf or NaN, a loss of NaN."""
     if logits.is_cuda:
