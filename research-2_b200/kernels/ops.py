@@ -151,7 +151,7 @@ def build_all(head_dims=()) -> None:
     """Compile every kernel library that does not depend on a model, and the attention kernels
     for the given head sizes (a model compiles its own head size at first use otherwise)."""
     for source in ("rowwise", "recurrent", "state_scan", "decay_chunks", "streams", "routing", "gemm_simt", "gemm_tc", "few_rows", "step_io", "attention_simt", "attention_prefill_tc", "latent_attention",
-                   "sampling", "adjust_logits", "top_logits", "distill", "wait_selftest"):
+                   "sampling", "adjust_logits", "top_logits", "distill", "token_loss", "token_rows", "wait_selftest"):
         _lib(source)
     _faces()
     kernel_library("sfu_probe")  # (profiling/sfu_probe.py: a measurement, no part of a step)
@@ -1938,8 +1938,19 @@ _LOGIT_SIGNATURES = {
     "distill": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
                 C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p],
     "scale_rows": [C.c_int, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p],
+    "token_loss": [C.c_int, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
+                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
+    "token_loss_gradient": [C.c_int, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                            C.c_float, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p],
+    "token_loss_space": [C.c_int] * 5,
+    "token_rows": [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float, C.c_void_p],
+    "token_rows_gradient": [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int,
+                            C.c_void_p, C.c_void_p],
+    "token_rows_space": [C.c_int] * 3,
 }
-_LOGIT_LIBRARIES = {"scale_rows": "distill"}   # where the library has another name than the entry
+# where the library has another name than the entry
+_LOGIT_LIBRARIES = {"scale_rows": "distill", "token_loss_gradient": "token_loss", "token_loss_space": "token_loss", "token_rows_gradient": "token_rows",
+                    "token_rows_space": "token_rows"}
 _logit_entries: dict = {}
 
 
@@ -1952,6 +1963,8 @@ def _logit_entry(name: str):
         lib = _lib(_LOGIT_LIBRARIES.get(name, name))
         fn = getattr(lib, "r2_" + name)
         fn.argtypes = _LOGIT_SIGNATURES[name]
+        if name.endswith("_space"):
+            fn.restype = C.c_longlong
         entry = _logit_entries[name] = (lib, fn)
     return entry[1]
 
@@ -2224,4 +2237,149 @@ def scale_rows(x: torch.Tensor, factors: torch.Tensor, *, in_place: bool = True)
     if rows:
         _check(_logit_entry("scale_rows")(code, x.data_ptr(), ld, out.data_ptr(), out_ld, rows, vocab, at, 0 if one else 1, _current_stream(device)),
                "scale_rows")
+    return out
+
+
+# ---- the two ends of a token table: the loss of tokens from hidden rows, rows by tokens, and their gradients ----
+
+def _matrix(t: torch.Tensor, name: str, what: str) -> tuple[int, int, int, int, int]:
+    """(type's code, rows, width, row stride, device) of a matrix of numbers whose rows are contiguous."""
+    if t.dim() != 2:
+        raise KernelError(f"{what}: {name} must have 2 dimensions, got shape {tuple(t.shape)}")
+    dtype, device = t.dtype, t.get_device()
+    if device < 0:
+        raise KernelError(f"{what}: {name} must be a CUDA tensor (there is no CPU path)")
+    if dtype is not torch.float32 and dtype is not torch.bfloat16:
+        raise KernelError(f"{what}: {name} must be float32 or bfloat16, got {dtype}")
+    rows, width = t.shape
+    ld, inner = t.stride()
+    if width > 1 and inner != 1:
+        raise KernelError(f"{what}: {name} must have contiguous rows, got shape {tuple(t.shape)} stride {t.stride()}")
+    if rows <= 1:
+        ld = max(ld, width)
+    return (F32 if dtype is torch.float32 else BF16), rows, width, ld, device
+
+
+def _space(device: torch.device, size: int) -> torch.Tensor:
+    """Scratch of one call, from torch's allocator: of the call's stream, and of the graph that captures it."""
+    return torch.empty_strided((size,), (1,), dtype=torch.uint8, device=device)
+
+
+def _loss_arguments(hidden, table, targets, weight, softcap, what):
+    code, rows, width, ld, device = _matrix(hidden, "hidden", what)
+    table_code, vocab, table_width, table_ld, table_device = _matrix(table, "table", what)
+    if table_code != code or table_width != width or table_device != device:
+        raise KernelError(f"{what}: a table {tuple(table.shape)} of {table.dtype} on {table.device} does not fit hidden rows {tuple(hidden.shape)} of "
+                          f"{hidden.dtype} on {hidden.device}")
+    if vocab < 1 or width < 1:
+        raise KernelError(f"{what}: a table of {vocab} tokens of {width} numbers")
+    targets_at = _per_row(targets, "targets", torch.int32, rows, device)
+    weight_at = _per_row(weight, "weight", torch.float32, rows, device)
+    softcap = float(softcap)
+    if not 0.0 <= softcap < float("inf"):
+        raise KernelError(f"{what}: softcap must be finite and not negative, got {softcap}")
+    return code, rows, width, ld, vocab, table_ld, device, targets_at, weight_at, softcap
+
+
+def token_loss(hidden: torch.Tensor, table: torch.Tensor, targets: torch.Tensor, *, weight: torch.Tensor | None = None, softcap: float = 0.0):
+    """How unlikely a model finds given tokens, from its hidden rows, without the logits in memory: (loss float32 [N], log_sum float32 [N]).
+
+    `hidden` [N, D] are the rows that the head multiplies with `table` [V, D] (both float32 or both bfloat16; rows contiguous, any row stride);
+    `targets` int32 [N] the tokens. With z = hidden @ table^T (`softcap` > 0: softcap * tanh(z / softcap)), log_sum is the logarithm of a row's
+    sum of exp(z), and loss = weight * (log_sum - z[target]), minus the token's log-probability at weight 1 (`weight` float32 [N]; None: 1). A target outside
+    [0, V) (-1 or -100, say) is none: its row has the loss 0, as has a row of weight 0. Logits that hold +inf or NaN, or nothing but -inf, make a
+    row's log_sum and loss NaN or infinite, and no other row's."""
+    code, rows, width, ld, vocab, table_ld, device, targets_at, weight_at, softcap = _loss_arguments(hidden, table, targets, weight, softcap, "token_loss")
+    where = hidden.device
+    loss = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=where)
+    log_sum = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=where)
+    if rows:
+        stream = _current_stream(device)
+        space = _space(where, _logit_entry("token_loss_space")(code, rows, width, vocab, 0))
+        _check(_logit_entry("token_loss")(code, hidden.data_ptr(), ld, table.data_ptr(), table_ld, rows, width, vocab, targets_at, weight_at, softcap,
+                                          loss.data_ptr(), log_sum.data_ptr(), space.data_ptr(), _workspace(where).error.data_ptr(), stream), "token_loss")
+    return loss, log_sum
+
+
+def token_loss_gradient(hidden: torch.Tensor, table: torch.Tensor, targets: torch.Tensor, log_sum: torch.Tensor, *, weight: torch.Tensor | None = None,
+                        softcap: float = 0.0, hidden_gradient: bool = True, table_gradient: bool = True):
+    """The gradients of the sum of `token_loss`'s losses: (of the hidden rows [N, D], of the table [V, D]), in their types; None for one that is not
+    asked for. `log_sum` is `token_loss`'s for the same hidden rows, table and softcap; the other arguments as there. A row without a target, or of weight 0,
+    has the gradient 0 and no part in the table's, whatever its hidden numbers are."""
+    code, rows, width, ld, vocab, table_ld, device, targets_at, weight_at, softcap = _loss_arguments(hidden, table, targets, weight, softcap,
+                                                                                                     "token_loss_gradient")
+    log_sum_at = _per_row(log_sum, "log_sum", torch.float32, rows, device)
+    if log_sum_at == 0 and rows:
+        raise KernelError("token_loss_gradient: log_sum is token_loss's, got None")
+    where = hidden.device
+    d_hidden = torch.empty_strided((rows, width), (width, 1), dtype=hidden.dtype, device=where) if hidden_gradient else None
+    if rows == 0:
+        return d_hidden, torch.zeros(vocab, width, dtype=table.dtype, device=where) if table_gradient else None
+    d_table = torch.empty_strided((vocab, width), (width, 1), dtype=table.dtype, device=where) if table_gradient else None
+    if hidden_gradient or table_gradient:
+        stream = _current_stream(device)
+        space = _space(where, _logit_entry("token_loss_space")(code, rows, width, vocab, 1))
+        _check(_logit_entry("token_loss_gradient")(
+            code, hidden.data_ptr(), ld, table.data_ptr(), table_ld, rows, width, vocab, targets_at, weight_at, log_sum_at, softcap,
+            d_hidden.data_ptr() if hidden_gradient else 0, width, d_table.data_ptr() if table_gradient else 0, width, space.data_ptr(),
+            _workspace(where).error.data_ptr(), stream), "token_loss_gradient")
+    return d_hidden, d_table
+
+
+def _scale(scale: float, what: str) -> float:
+    scale = float(scale)
+    if not abs(scale) < float("inf"):
+        raise KernelError(f"{what}: scale must be finite, got {scale}")
+    return scale
+
+
+def token_rows(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Rows of a table [V, D] (float32 or bfloat16; rows contiguous, any row stride) by tokens int32 [T], times `scale`: [T, D] in the table's
+    type or `out_dtype`, computed in float32 and rounded once. A token outside [0, V) gets a row of zeros. (`embed` is the engine's form: float32, with positions, ids checked before.)"""
+    code, vocab, width, ld, device = _matrix(table, "table", "token_rows")
+    tokens = ids.shape[0] if ids.dim() == 1 else -1
+    ids_at = _per_row(ids, "ids", torch.int32, tokens, device)
+    scale, out_dtype = _scale(scale, "token_rows"), out_dtype or table.dtype
+    out = torch.empty_strided((tokens, width), (width, 1), dtype=out_dtype, device=table.device)
+    out_code = dtype_code(out_dtype)
+    if tokens and width:
+        _check(_logit_entry("token_rows")(code, out_code, ids_at, table.data_ptr(), ld, out.data_ptr(), width, tokens, width, vocab, scale,
+                                          _current_stream(device)), "token_rows")
+    return out
+
+
+def token_rows_gradient(ids: torch.Tensor, above: torch.Tensor, vocab: int, *, scale: float = 1.0, out_dtype: torch.dtype | None = None,
+                        into: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of a table of `vocab` rows that `token_rows` read: [V, D], whose row v is `scale` times the sum of the rows of `above` [T, D] (float32
+    or bfloat16; rows contiguous, any row stride) at which `ids` (int32 [T]) is v, added in float32 in the order of the places and rounded once, so
+    that the same call gives the same bits. It is a new table in `above`'s type or `out_dtype`, zero where no token came; or the sums are added to `into` [V, D] (float32 or
+    bfloat16), whose rows without a token are left as they are: a tied table's gradient, begun by `token_loss_gradient`. Tokens outside [0, V) count for nothing."""
+    code, tokens, width, ld, device = _matrix(above, "above", "token_rows_gradient")
+    ids_at = _per_row(ids, "ids", torch.int32, tokens, device)
+    if ids.shape[0] != tokens:
+        raise KernelError(f"token_rows_gradient: {ids.shape[0]} tokens and {tokens} rows")
+    try:
+        vocab = operator.index(vocab)
+    except TypeError:
+        raise KernelError(f"token_rows_gradient: vocab must be a whole number, got {vocab!r}") from None
+    if not 1 <= vocab < 2**31:
+        raise KernelError(f"token_rows_gradient: vocab must be in [1, 2^31), got {vocab}")
+    scale = _scale(scale, "token_rows_gradient")
+    if into is None:
+        out_dtype = out_dtype or above.dtype
+        out_code, out_ld = dtype_code(out_dtype), width
+        if tokens == 0 or width == 0:
+            return torch.zeros(vocab, width, dtype=out_dtype, device=above.device)
+        out = torch.empty_strided((vocab, width), (width, 1), dtype=out_dtype, device=above.device)
+    else:
+        out = into
+        out_code, into_rows, into_width, out_ld, into_device = _matrix(into, "into", "token_rows_gradient")
+        if (into_rows, into_width) != (vocab, width) or into_device != device or (out_dtype or into.dtype) != into.dtype:
+            raise KernelError(f"token_rows_gradient: into {tuple(into.shape)} of {into.dtype} on {into.device} is not [{vocab}, {width}]")
+        if vocab > 1 and out_ld < width:
+            raise KernelError("token_rows_gradient: rows of into overlap")
+    if tokens and width:
+        space = _space(above.device, _logit_entry("token_rows_space")(tokens, width, vocab))
+        _check(_logit_entry("token_rows_gradient")(code, out_code, ids_at, above.data_ptr(), ld, out.data_ptr(), out_ld, tokens, width, vocab, scale,
+                                                   int(into is not None), space.data_ptr(), _current_stream(device)), "token_rows_gradient")
     return out

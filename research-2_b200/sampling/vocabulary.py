@@ -1,0 +1,69 @@
+"""The two ends of a token table, for training with torch's gradients: the rows that tokens look up, and the loss of tokens from hidden rows. The logits
+[N, V] are in memory at no time: the backward pass makes them again, a piece of the vocabulary at a time, with the factors that come down from above."""
+
+from __future__ import annotations
+
+import torch
+
+from ..kernels import ops
+
+
+def _tokens(t: torch.Tensor, vocab: int) -> torch.Tensor:
+    """int32; wider numbers that name no token stay such."""
+    return t if t.dtype is torch.int32 else t.clamp(-1, vocab).to(torch.int32)
+
+
+class _TokenLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, table, targets, weight, softcap):
+        loss, log_sum = ops.token_loss(hidden.detach(), table.detach(), targets, weight=weight, softcap=softcap)
+        ctx.save_for_backward(hidden, table, targets, weight, log_sum)
+        ctx.softcap = softcap
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, above):
+        hidden, table, targets, weight, log_sum = ctx.saved_tensors
+        factor = (above.to(torch.float32) if weight is None else above * weight).contiguous()
+        d_hidden, d_table = ops.token_loss_gradient(hidden, table, targets, log_sum, weight=factor, softcap=ctx.softcap,
+                                                    hidden_gradient=ctx.needs_input_grad[0], table_gradient=ctx.needs_input_grad[1])
+        return d_hidden, d_table, None, None, None
+
+
+def token_loss(hidden: torch.Tensor, table: torch.Tensor, targets: torch.Tensor, *, weight: torch.Tensor | None = None, softcap: float = 0.0) -> torch.Tensor:
+    """weight * (minus the log-probability of the target) of every row, float32 [N], with gradients for `hidden` [N, D] and `table` [V, D] (`ops.token_loss` says
+    what they are; `targets` may be int64). There is no gradient for `weight`: one that asks for it is refused (`detach()` it)."""
+    if weight is not None and torch.is_grad_enabled() and weight.requires_grad:
+        raise ops.KernelError("token_loss: weight asks for a gradient and there is none: detach() it")
+    if targets.dtype not in (torch.int32, torch.int64):
+        raise ops.KernelError(f"token_loss: targets must be int32 or int64, got {targets.dtype}")
+    return _TokenLoss.apply(hidden, table, _tokens(targets, table.shape[0]), weight, float(softcap))
+
+
+class _TokenRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, out_dtype):
+        ctx.save_for_backward(ids)
+        ctx.scale, ctx.vocab, ctx.dtype = scale, table.shape[0], table.dtype
+        return ops.token_rows(ids, table.detach(), scale=scale, out_dtype=out_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, above):
+        (ids,) = ctx.saved_tensors
+        if above.shape[1] > 1 and above.stride(1) != 1:
+            above = above.contiguous()
+        return None, ops.token_rows_gradient(ids, above, ctx.vocab, scale=ctx.scale, out_dtype=ctx.dtype), None, None
+
+
+def token_rows(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """scale * table[ids], of ids (int32 or int64) of any shape: [..., D], with a gradient for `table` [V, D], added in one order
+    (`ops.token_rows` and `ops.token_rows_gradient` say what they are). A token outside [0, V) gets zeros and gives nothing."""
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ops.KernelError(f"token_rows: ids must be int32 or int64, got {ids.dtype}")
+    rows = _TokenRows.apply(_tokens(ids, table.shape[0]).reshape(-1), table, float(scale), out_dtype)
+    return rows.view(*ids.shape, table.shape[1])
+
+
+__all__ = ["token_loss", "token_rows"]

@@ -1,0 +1,383 @@
+"""The loss of tokens from hidden rows and its gradients against 64 bits (`tests/plain/vocabulary_plain.py`, where the tolerances are derived): sizes
+around tiles, both types, strides and alignments, rows without a target, capped logits, infinities and NaN, streams, graphs, refusals."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests.plain.vocabulary_plain import Loss
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def ops():
+    from research_2_b200.kernels import ops as o
+
+    return o
+
+
+def gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def strided(values: torch.Tensor, dtype, offset: int = 0, pad: int = 0) -> torch.Tensor:
+    """The values as a view that starts `offset` places into rows of `offset + width + pad`; what lies around them is NaN."""
+    r, n = values.shape
+    buf = torch.full((r, offset + n + pad), float("nan"), dtype=dtype, device=DEV)
+    buf[:, offset: offset + n] = values.to(dtype)
+    return buf[:, offset: offset + n]
+
+
+class Case:
+    def __init__(self, rows, width, vocab, dtype, seed=0, offset=0, pad=0, table_offset=0, table_pad=0, softcap=0.0, weighted=True, size=2.0):
+        g = gen(seed)
+        table = torch.randn(vocab, width, generator=g, device=DEV) * (size / math.sqrt(width))
+        self.targets = torch.randint(0, vocab, (rows,), generator=g, device=DEV, dtype=torch.int32)
+        hidden = torch.randn(rows, width, generator=g, device=DEV) + 2 * torch.rand(rows, 1, generator=g, device=DEV) * table[self.targets.long()]
+        if rows > 2:
+            self.targets[0], self.targets[1], self.targets[2] = 0, vocab - 1, -100
+        if rows > 6:
+            self.targets[4], self.targets[5] = vocab, 2**31 - 1
+        self.weight = torch.randn(rows, generator=g, device=DEV) if weighted else None
+        if weighted and rows > 3:
+            self.weight[3] = 0
+        self.hidden, self.table = strided(hidden, dtype, offset, pad), strided(table, dtype, table_offset, table_pad)
+        self.softcap = softcap
+
+    def kwargs(self):
+        return dict(weight=self.weight, softcap=self.softcap)
+
+    def run(self, **wanted):
+        loss, log_sum = ops().token_loss(self.hidden, self.table, self.targets, **self.kwargs())
+        return loss, log_sum, *ops().token_loss_gradient(self.hidden, self.table, self.targets, log_sum, **self.kwargs(), **wanted)
+
+    def plain(self):
+        return Loss(self.hidden, self.table, self.targets, self.weight, self.softcap)
+
+    def check(self):
+        got, want = self.run(), self.plain()
+        ops().raise_on_device_error(DEV)
+        for name, t in zip(("loss", "log_sum", "d_hidden", "d_table"), got):
+            exact, off = getattr(want, name), getattr(want, name + "_off")
+            worst = ((t.double() - exact).abs() / off.clamp(min=1e-300)).nan_to_num(nan=math.inf).max().item()
+            assert torch.all((t.double() - exact).abs() <= off), (name, worst)
+        assert got[0].dtype == got[1].dtype == F32 and got[2].dtype == self.hidden.dtype and got[3].dtype == self.table.dtype
+        return got
+
+
+SIZES = [(1, 64, 300), (1, 768, 50257), (3, 100, 1031), (17, 33, 257), (5, 8, 1), (64, 1, 7), (128, 64, 256), (129, 72, 513), (256, 128, 512),
+         (257, 200, 1000), (300, 768, 2049), (1000, 48, 5000), (600, 320, 20011)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,width,vocab", SIZES)
+def test_against_64_bits(rows, width, vocab, dtype):
+    Case(rows, width, vocab, dtype, seed=rows + vocab).check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("offset,pad,table_offset,table_pad", [(1, 0, 0, 0), (0, 8, 8, 0), (0, 1, 0, 3), (4, 4, 4, 12), (8, 24, 16, 40)])
+def test_strides_and_alignments(dtype, offset, pad, table_offset, table_pad):
+    Case(140, 96, 700, dtype, 5, offset, pad, table_offset, table_pad).check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("softcap,size", [(30.0, 2.0), (5.0, 6.0), (0.3, 1.0), (1000.0, 2.0)])
+def test_capped(dtype, softcap, size):
+    Case(200, 128, 900, dtype, 6, softcap=softcap, size=size).check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_without_weights(dtype):
+    Case(70, 64, 500, dtype, 7, weighted=False).check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [1e-4, 40.0, 300.0])
+def test_flat_and_steep_rows(dtype, size):
+    Case(65, 128, 777, dtype, 8, size=size).check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_table_beyond_32_bits(dtype):
+    # rows 40,000 numbers apart: the last ones lie more than 2^31 numbers into the buffer
+    c = Case(20, 64, 100, dtype, 9)
+    vocab, ld = 60_000, 40_000
+    buffer = torch.empty(vocab, ld, dtype=dtype, device=DEV)
+    c.table = buffer[:, :64]
+    c.table.copy_(torch.randn(vocab, 64, generator=gen(10), device=DEV) / 4)
+    c.targets = torch.randint(0, vocab, (20,), generator=gen(11), device=DEV, dtype=torch.int32)
+    c.targets[0] = vocab - 1
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_broadcast_rows(dtype):
+    c = Case(9, 64, 300, dtype, 12)
+    c.hidden = c.hidden[:1].expand(9, 64)
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_one_gradient_alone(dtype):
+    c = Case(150, 64, 600, dtype, 13)
+    _, _, d_hidden, d_table = c.run()
+    _, _, only, none = c.run(table_gradient=False)
+    assert none is None and torch.equal(only, d_hidden)
+    _, _, none, only = c.run(hidden_gradient=False)
+    assert none is None and torch.equal(only, d_table)
+    assert c.run(hidden_gradient=False, table_gradient=False)[2:] == (None, None)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_same_bits_every_time(dtype):
+    c = Case(500, 320, 9001, dtype, 14)
+    first = c.run()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, c.run()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_without_a_target_may_hold_anything(dtype):
+    c = Case(300, 64, 700, dtype, 15)
+    c.targets[200:] = -1
+    c.targets[:200] = c.targets[:200].clamp(0, 699)
+    c.weight[:200] = 1.0
+    clean = c.run()
+    c.hidden[200:] = float("nan")
+    c.hidden[250] = float("inf")
+    loss, log_sum, d_hidden, d_table = c.run()
+    assert torch.equal(loss, clean[0]) and torch.equal(log_sum[:200], clean[1][:200])
+    assert torch.equal(d_hidden, clean[2]) and torch.equal(d_table, clean[3])
+    assert torch.all(loss[200:] == 0) and torch.all(d_hidden[200:] == 0)
+    c.targets[200:], c.weight[200:] = 5, 0.0
+    again = c.run()
+    assert torch.equal(again[0], loss) and torch.equal(again[2], d_hidden) and torch.equal(again[3], d_table)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_no_row_counts(dtype):
+    c = Case(40, 64, 700, dtype, 16)
+    c.targets[:] = -1
+    c.hidden[3] = float("nan")
+    loss, _, d_hidden, d_table = c.run()
+    assert not loss.any() and not d_hidden.any() and not d_table.any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_infinities_and_nan_stay_in_their_row(dtype):
+    c = Case(130, 64, 600, dtype, 17)
+    c.targets[:] = 7
+    clean = ops().token_loss(c.hidden, c.table, c.targets)
+    c.hidden[5], c.hidden[9, 3], c.hidden[128] = float("nan"), float("inf"), -float("inf")
+    got = ops().token_loss(c.hidden, c.table, c.targets)
+    bad = torch.zeros(130, dtype=torch.bool, device=DEV)
+    bad[[5, 9, 128]] = True
+    for a, b in zip(got, clean):
+        assert torch.equal(a[~bad], b[~bad]) and not torch.isfinite(a[bad]).any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_forbidden_tokens(dtype):
+    # a table with rows that make every logit -inf: such tokens have no share, and a row whose target is one has an infinite loss
+    c = Case(20, 64, 300, dtype, 18, weighted=False)
+    c.hidden[:, 0] = 1.0
+    c.table[10:290] = 0.0
+    c.table[10:290, 0] = -float("inf")
+    c.targets[:] = 3
+    c.targets[4] = 100
+    loss, log_sum = ops().token_loss(c.hidden, c.table, c.targets)
+    keep = [v for v in range(300) if not 10 <= v < 290]
+    want = Loss(c.hidden, c.table[keep], torch.full_like(c.targets, 3))
+    assert torch.all((log_sum.double() - want.log_sum).abs() <= want.log_sum_off)
+    assert loss[4].item() == math.inf and torch.isfinite(loss[torch.arange(20, device=DEV) != 4]).all()
+
+
+def test_no_rows():
+    for dtype in (F32, BF16):
+        c = Case(0, 64, 50, dtype)
+        c.weight = None
+        loss, log_sum, d_hidden, d_table = c.run()
+        assert loss.shape == log_sum.shape == (0,) and d_hidden.shape == (0, 64)
+        assert d_table.shape == (50, 64) and not d_table.any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradients_against_differences(dtype):
+    c = Case(12, 40, 90, dtype, 19, softcap=8.0)
+    _, _, d_hidden, d_table = c.run()
+    g = gen(20)
+    for which, grad in (("hidden", d_hidden), ("table", d_table)):
+        base = getattr(c, which).double()
+        step = torch.randn(base.shape, generator=g, device=DEV, dtype=torch.float64)
+        h = 1e-5
+
+        def total(sign):
+            moved = base + sign * h * step
+            x, w = (moved, c.table.double()) if which == "hidden" else (c.hidden.double(), moved)
+            return Loss(x, w, c.targets, c.weight, 8.0).loss.sum().item()
+
+        want = (total(1) - total(-1)) / (2 * h)
+        off = (c.plain().__dict__["d_" + which + "_off"] * step.abs()).sum().item() + 1e-7
+        assert abs((grad.double() * step).sum().item() - want) <= off
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_another_stream(dtype):
+    c = Case(200, 128, 3000, dtype, 21)
+    want = c.run()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    hidden = torch.zeros_like(c.hidden)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(2_000_000)
+        hidden.copy_(c.hidden)      # arrives late, on the stream of the call
+        c.hidden = hidden
+        got = c.run()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_captured_and_replayed(dtype):
+    cases = [Case(200, 128, 3000, dtype, 22), Case(77, 64, 1500, dtype, 23)]
+    wants = [c.run() for c in cases]
+    graphs = []
+    for c in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = c.run()
+        graphs.append((graph, out))
+    # two graphs in turn and side by side: neither has the other's scratch
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        for c in cases:
+            c.hidden.neg_()
+        torch.cuda.synchronize()
+        changed = [c.run() for c in cases]
+        torch.cuda.synchronize()
+        graphs[0][0].replay()
+        with torch.cuda.stream(side):
+            graphs[1][0].replay()
+        torch.cuda.synchronize()
+        for (_, out), want in zip(graphs, changed):
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+    for c in cases:
+        c.hidden.neg_()
+    graphs[0][0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(graphs[0][1], wants[0]))
+
+
+def test_nothing_around_the_results_is_written():
+    c = Case(130, 72, 515, BF16, 24, offset=8, pad=8, table_offset=8, table_pad=8)
+    before = [t.clone() for t in (c.hidden, c.table, c.targets, c.weight)]
+    c.run()
+    assert all(torch.equal(a, b) for a, b in zip(before, (c.hidden, c.table, c.targets, c.weight)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_with_torch_gradients(dtype, kind):
+    import research_2_b200 as r2
+
+    c = Case(90, 64, 400, dtype, 25, softcap=12.0)
+    hidden, table = c.hidden.clone().requires_grad_(), c.table.clone().requires_grad_()
+    above = torch.randn(90, generator=gen(26), device=DEV)
+    targets = c.targets.to(kind)
+    if kind is torch.int64:
+        targets[7] = 2**32 + 5    # no token, and none after a cut to 32 bits
+    loss = r2.token_loss(hidden, table, targets, weight=c.weight, softcap=12.0)
+    (loss * above).sum().backward(retain_graph=True)
+    held = torch.where((targets >= 0) & (targets < 400), targets, -1).to(torch.int32)
+    want = Loss(c.hidden, c.table, held, c.weight * above, 12.0)
+    for got, name in ((hidden.grad, "d_hidden"), (table.grad, "d_table")):
+        # (weight * above is rounded to float32: a unit more)
+        assert torch.all((got.double() - getattr(want, name)).abs() <= getattr(want, name + "_off") + 2.0**-24 * getattr(want, name).abs())
+    first = hidden.grad.clone(), table.grad.clone()
+    hidden.grad = table.grad = None
+    (loss * above).sum().backward()     # a kept graph, a second time
+    assert torch.equal(hidden.grad, first[0]) and torch.equal(table.grad, first[1])
+    frozen = r2.token_loss(hidden, table.detach(), targets, weight=c.weight, softcap=12.0)
+    assert torch.equal(torch.autograd.grad((frozen * above).sum(), hidden)[0], first[0])
+    with pytest.raises(ops().KernelError, match="detach"):
+        r2.token_loss(hidden, table, targets, weight=c.weight.clone().requires_grad_())
+
+
+def test_gradients_of_broadcast_rows():
+    import research_2_b200 as r2
+
+    c = Case(6, 64, 200, F32, 27, weighted=False)
+    c.targets[:] = torch.arange(6, device=DEV)
+    row = c.hidden[:1].clone().requires_grad_()
+    r2.token_loss(row.expand(6, 64), c.table, c.targets).sum().backward()
+    c.hidden = row.detach().expand(6, 64)
+    want = c.plain()
+    assert row.grad.shape == (1, 64)
+    assert torch.all((row.grad.double() - want.d_hidden.sum(0, keepdim=True)).abs() <= want.d_hidden_off.sum(0, keepdim=True) * 2)
+
+
+def test_a_tied_table_from_both_ends():
+    """Look up, a layer of torch's, the loss over the same table, both gradients, a step; then again."""
+    import research_2_b200 as r2
+
+    torch.manual_seed(0)
+    vocab, width = 1031, 64
+    table = (torch.randn(vocab, width, device=DEV) / 8).requires_grad_()
+    mix = (torch.randn(width, width, device=DEV) / 8).requires_grad_()
+    ids = torch.randint(0, vocab, (2, 33), device=DEV)
+    weight = torch.full((64,), 1.0 / 64, device=DEV)
+
+    def step(table, mix, rows, loss):
+        x = rows(ids[:, :-1], table)
+        h = torch.tanh(x.reshape(-1, width) @ mix)
+        return torch.autograd.grad(loss(h, table), (table, mix))
+
+    plain_rows = lambda i, t: t[i] * 8.0
+    plain_loss = lambda h, t: torch.nn.functional.cross_entropy(h @ t.t(), ids[:, 1:].reshape(-1))
+    for _ in range(2):
+        got = step(table, mix, lambda i, t: r2.token_rows(i, t, scale=8.0), lambda h, t: r2.token_loss(h, t, ids[:, 1:].reshape(-1), weight=weight).sum())
+        want = step(table.double().detach().requires_grad_(), mix.double().detach().requires_grad_(), plain_rows, plain_loss)
+        for a, b in zip(got, want):
+            # (torch's own products in float32 stand between: 64 terms, twice, and a tanh)
+            assert (a.double() - b).abs().max().item() <= 1e-4 * b.abs().max().item()
+        with torch.no_grad():
+            table -= 0.1 * got[0]
+            mix -= 0.1 * got[1]
+    # the same by the operators alone, one buffer for both ends
+    with torch.no_grad():
+        rows = ops().token_rows(ids[:, :-1].reshape(-1).to(torch.int32), table, scale=8.0)
+        h = torch.tanh(rows @ mix)
+        y = ids[:, 1:].reshape(-1).to(torch.int32)
+        loss, log_sum = ops().token_loss(h, table, y, weight=weight)
+        d_h, d_table = ops().token_loss_gradient(h, table, y, log_sum, weight=weight)
+        ops().token_rows_gradient(ids[:, :-1].reshape(-1).to(torch.int32), (d_h * (1 - h * h)) @ mix.t(), vocab, scale=8.0, into=d_table)
+    want = step(table.double().detach().requires_grad_(), mix.double().detach().requires_grad_(), plain_rows, plain_loss)[0]
+    assert (d_table.double() - want).abs().max().item() <= 1e-4 * want.abs().max().item()
+
+
+def test_refusals():
+    o = ops()
+    x, w = torch.zeros(4, 16, device=DEV), torch.zeros(10, 16, device=DEV)
+    y, s = torch.zeros(4, dtype=torch.int32, device=DEV), torch.zeros(4, device=DEV)
+    for bad in (dict(hidden=x.cpu()), dict(hidden=x[0]), dict(hidden=x.half()), dict(hidden=x.bfloat16()), dict(table=w[:, :8]), dict(table=w.t().contiguous().t()),
+                dict(hidden=x.t().contiguous().t()), dict(table=w[:0]), dict(targets=y.long()), dict(targets=y[:3]), dict(targets=y.cpu()),
+                dict(targets=torch.zeros(8, dtype=torch.int32, device=DEV)[::2]), dict(weight=s.double()), dict(weight=s[:2]), dict(softcap=-1.0),
+                dict(softcap=math.nan), dict(softcap=math.inf), dict(hidden=x[:, :0], table=w[:, :0])):
+        call = dict(hidden=x, table=w, targets=y, weight=None, softcap=0.0)
+        call.update(bad)
+        args = [call.pop(n) for n in ("hidden", "table", "targets")]
+        with pytest.raises(o.KernelError):
+            o.token_loss(*args, **call)
+        with pytest.raises(o.KernelError):
+            o.token_loss_gradient(*args, s, **call)
+    for log_sum in (None, s[:3], s.double(), s.cpu()):
+        with pytest.raises(o.KernelError):
+            o.token_loss_gradient(x, w, y, log_sum)
