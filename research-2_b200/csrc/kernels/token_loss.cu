@@ -4,241 +4,869 @@
 //   u = x W^T,  z = u  or  c tanh(u / c),  s_r = log(sum_v exp z_rv),  loss_r = a_r (s_r - z_r,y)
 //   dz = a_r (exp(z_rv - s_r) - [v = y_r]) (1 - (z_rv / c)^2),  dx = dz W,  dW = dz^T x
 //
-// Plain tiles on the CUDA cores: 64 x 64 results a CTA, 4 x 4 a thread.
+// All four products run on one kernel (`product_kernel`): CTA pairs (cta_group::2) with 256 x 256 tiles, operands by TMA, two accumulators in tensor memory, so
+// that eight warps work on one tile's results while the next one's products run. What differs is what those warps do with a tile:
+//
+//   LOGSUM   a tile of z, reduced to each row's largest number and the sum of exponentials against it, by halves of a tile; `finish_kernel` joins them
+//   FACTORS  a tile of z made again, turned into dz and rounded to bfloat16, a piece of the vocabulary at a time
+//   ROWS     dx: dz times the piece of the table, K split over the pairs where tiles are few; shares are float and added in one order (`join_kernel`)
+//   TABLE    dW: dz^T times the hidden rows, whole for each piece of the vocabulary and rounded once
+//
+// dz is rounded to bfloat16, the type of the gradients that it makes, so that both products run on the tensor cores at full rate.
+//
+// float32 operands are three bfloat16 planes each: x = x0 + x1 + x2 to the last bit (8 bits each), and a product is the six products x_i w_j
+// with i + j <= 2, smallest first; what is left out is below 2^-24 of it. dz is kept in three planes then, too.
+//
+// Rows without a token or of weight 0 have no part in the gradients: `gather_kernel` puts the others side by side, so that no product reads them
+// (whatever they hold) or spends time on them; the rest of the last 256 rows is zeros.
 #include <math.h>
 
 #include "common.cuh"
+#include "sm100_ptx.cuh"
+#include "tensor_maps.cuh"
 
 namespace {
 
-constexpr int TILE = 64, DEPTH = 16;
+using namespace r2ptx;
 
-enum Mode { LOGITS, DZ, STORE, ADD };
+constexpr int BM = 128;          // rows of a tile in one CTA
+constexpr int BN = 256;          // columns of a tile, half of their operand in each CTA
+constexpr int HALF = BN / 2;
+constexpr int BK = 64;           // one 128-byte swizzle span of bfloat16
+constexpr int UMMA_K = 16;
+constexpr int THREADS = 320;     // warp 0: TMA, warp 1: products + tensor memory, warps 2-9: results
+constexpr int WARPS = 8;
+constexpr int STAGES = 6;
+constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = HALF * BK * 2;
+constexpr size_t SMEM = 1024 + STAGES * size_t(A_BYTES + B_BYTES) + (2 * STAGES + 4) * 8 + 16;
 
-struct Operand {
-  const void* p;
-  long long outer, inner;   // strides of (row of the result or column of it, k)
-};
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+constexpr int ERR_FULL = 1, ERR_EMPTY = 2, ERR_ACC = 3;   // codes of waits that ran out, as of the other products
+
+enum Mode { LOGSUM, FACTORS, ROWS, TABLE };
 
 struct Work {
-  Operand a, b;
-  int m, n, k;
-  float softcap;
-  const int32_t* targets;
-  const float* weight;
+  int m, n, k;               // rows and columns of the result, and what is summed over
+  const int* count;          // FACTORS, ROWS: m, TABLE: k, on the device (the gathered rows)
+  int terms;                 // 1, or 6 for operands in three planes
+  int splits, per_split;     // ROWS: shares of k, in steps of BK
+  int add;                   // ROWS: to what earlier pieces left
+  float cap_in, cap_out;     // c > 0: z * log2 e = cap_out * tanh(u / c) with cap_in = 2 log2 e / c, cap_out = c log2 e; else 0
+  const int32_t* targets;    // FACTORS: of the gathered rows, with their factors and sums
+  const float* factor;
   const float* log_sum;
-  int first, vocab;          // of the tile's columns: tokens
-  float2* part;              // LOGITS: [column tile][row] the largest logit and the sum against it
-  float* at_target;          // LOGITS: [row]
-  void* out;                 // DZ: float [m, ld]; STORE, ADD: T or float [m, ld]
-  long long ld;
+  int first;                 // FACTORS: the piece's first token
+  float2* part;              // LOGSUM: [half tile][row]: the largest z log2 e and the sum of 2^(z log2 e - it)
+  bf16* dz;                  // FACTORS: [plane][row][ld]
+  long long dz_plane;
+  float* shares;             // ROWS: [split][row][ld]
+  long long share_plane;
+  void* out;                 // TABLE
+  long long ld;              // of dz, shares or out
+  int* error_flag;
 };
 
-template <typename TA, typename TB, typename TO, int MODE>
-__global__ void __launch_bounds__(256) tile_kernel(const Work w) {
-  __shared__ float as[DEPTH][TILE + 4], bs[DEPTH][TILE + 4];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int m0 = blockIdx.y * TILE, n0 = blockIdx.x * TILE;
-  const TA* a = static_cast<const TA*>(w.a.p);
-  const TB* b = static_cast<const TB*>(w.b.p);
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < w.k; k0 += DEPTH) {
-    for (int i = threadIdx.x; i < TILE * DEPTH; i += 256) {
-      const int r = w.a.inner == 1 ? i / DEPTH : i % TILE, k = w.a.inner == 1 ? i % DEPTH : i / TILE;
-      as[k][r] = (m0 + r < w.m && k0 + k < w.k) ? to_float(a[(m0 + r) * w.a.outer + (k0 + k) * w.a.inner]) : 0.f;
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int plane, uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(map), "r"(leader_bar), "r"(x), "r"(y), "r"(plane)
+      : "memory");
+}
+__device__ __forceinline__ void umma_pair(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t bar) {   // arrives on both CTAs' barrier at this offset
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(bar), "h"(uint16_t(3)) : "memory");
+}
+// Hands over tensor memory that this warp has read (ordered by tcgen05.wait::ld and the fence before it).
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The whole warp's wait: its lanes go on together, also when it ran out.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The planes of the k-th of the six products of float32 operands, smallest products first.
+__device__ __forceinline__ int plane_a(int terms, int t) { return terms == 1 ? 0 : (0x001102 >> (4 * t)) & 3; }   // 2 0 1 1 0 0
+__device__ __forceinline__ int plane_b(int terms, int t) { return terms == 1 ? 0 : (0x010120 >> (4 * t)) & 3; }   // 0 2 1 0 1 0
+
+// x = p[0] + p[1] + p[2] for a finite x; infinities become the largest bfloat16 numbers, NaN stays in p[0].
+__device__ __forceinline__ void split3(float x, bf16 (&p)[3]) {
+  const float most = 3.3895313892515355e38f;
+  if (fabsf(x) > most) x = copysignf(most, x);    // (false for NaN)
+  p[0] = __float2bfloat16_rn(x);
+  float rest = x - __bfloat162float(p[0]);
+  p[1] = __float2bfloat16_rn(rest);
+  rest -= __bfloat162float(p[1]);
+  p[2] = __float2bfloat16_rn(rest);
+}
+
+// z log2 e of an accumulator: for capped logits c log2 e (1 - 2 / (e^(2 u / c) + 1)), whose error is some units of c.
+template <bool CAPPED> __device__ __forceinline__ float log2_units(float u, const Work& w) {
+  if constexpr (!CAPPED) return u * LOG2E;
+  const float r = fast_rcp(fast_exp2(u * w.cap_in) + 1.f);
+  return fmaf(-2.f * w.cap_out, r, w.cap_out);
+}
+
+struct Unit {   // one tile, or one share of its k
+  int row, col, split, kb_begin, kb_end;
+};
+
+template <int MODE> __device__ __forceinline__ Unit unit_of(const Work& w, long long i, int row_tiles, int col_tiles, int n_kb) {
+  Unit u;
+  u.split = 0;
+  u.kb_begin = 0;
+  u.kb_end = n_kb;
+  if constexpr (MODE == LOGSUM || MODE == FACTORS) {   // all rows of a column tile follow one another: the table is read once
+    u.col = int(i / row_tiles);
+    u.row = int(i % row_tiles);
+  } else {
+    const long long tile = i % (static_cast<long long>(row_tiles) * col_tiles);
+    u.row = int(tile / col_tiles);
+    u.col = int(tile % col_tiles);
+    if constexpr (MODE == ROWS) {
+      u.split = int(i / (static_cast<long long>(row_tiles) * col_tiles));
+      u.kb_begin = u.split * w.per_split;
+      u.kb_end = min(n_kb, u.kb_begin + w.per_split);
     }
-    for (int i = threadIdx.x; i < TILE * DEPTH; i += 256) {
-      const int r = w.b.inner == 1 ? i / DEPTH : i % TILE, k = w.b.inner == 1 ? i % DEPTH : i / TILE;
-      bs[k][r] = (n0 + r < w.n && k0 + k < w.k) ? to_float(b[(n0 + r) * w.b.outer + (k0 + k) * w.b.inner]) : 0.f;
+  }
+  return u;
+}
+
+// 32 numbers of a row of results, from column c of [0, n) on.
+template <typename T> __device__ __forceinline__ void put32(T* row, int c, int n, const float (&v)[32], bool wide) {
+  if constexpr (sizeof(T) == 2) {
+    if (wide && c + 32 <= n) {
+      uint4* to = reinterpret_cast<uint4*>(row + c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        to[j] = make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]), pack_bf16(v[8 * j + 4], v[8 * j + 5]),
+                           pack_bf16(v[8 * j + 6], v[8 * j + 7]));
+      return;
     }
-    __syncthreads();
+  } else {
+    if (wide && c + 32 <= n) {
+      float4* to = reinterpret_cast<float4*>(row + c);
 #pragma unroll
-    for (int k = 0; k < DEPTH; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float f = as[k][ty * 4 + i];
-          // (a row without a target has no part in the table's gradient, whatever it holds)
-          if (MODE != STORE || f != 0.f) acc[i][j] = fmaf(f, bs[k][tx * 4 + j], acc[i][j]);
-        }
-    __syncthreads();
+      for (int j = 0; j < 8; ++j) to[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      return;
+    }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = m0 + ty * 4 + i;
-    if (r >= w.m) continue;   // (the sixteen threads of a row go together)
-    if constexpr (MODE == LOGITS) {
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (w.softcap > 0.f) acc[i][j] = w.softcap * tanhf(acc[i][j] / w.softcap);
-        const int v = n0 + tx * 4 + j;
-        if (v >= w.n) acc[i][j] = -INFINITY;
-        else if (w.targets[r] == w.first + v) w.at_target[r] = acc[i][j];
-        top = fmaxf(top, acc[i][j]);
-      }
-      const unsigned half = 0xffffu << (threadIdx.x & 16);
-      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(half, top, o));
-      const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum += expf(acc[i][j] - ref);
-      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(half, sum, o);
-      if (tx == 0) w.part[size_t(blockIdx.x) * w.m + r] = make_float2(top, sum);
-    } else {
-      TO* out = static_cast<TO*>(w.out) + r * w.ld;
-      const int y = MODE == DZ ? w.targets[r] : 0;
-      const float factor = MODE == DZ ? (y >= 0 && y < w.vocab ? (w.weight ? w.weight[r] : 1.f) : 0.f) : 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int v = n0 + tx * 4 + j;
-        if (v >= w.n) continue;
-        float g = acc[i][j];
-        if constexpr (MODE == DZ) {
-          float z = g, slope = 1.f;
-          if (w.softcap > 0.f) {
-            const float t = tanhf(z / w.softcap);
-            z = w.softcap * t;
-            slope = 1.f - t * t;
+  for (int j = 0; j < 32; ++j)
+    if (c + j < n) row[c + j] = from_float<T>(v[j]);
+}
+
+template <int MODE, bool CAPPED, typename T>
+__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Work w) {
+  constexpr bool A_MN = MODE == TABLE, B_MN = MODE == ROWS || MODE == TABLE;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t a_base = smem_u32(smem), b_base = a_base + STAGES * A_BYTES;
+  const uint32_t full = b_base + STAGES * B_BYTES, empty = full + STAGES * 8, acc_full = empty + STAGES * 8, acc_empty = acc_full + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + STAGES * size_t(A_BYTES + B_BYTES) + (2 * STAGES + 4) * 8);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;   // the cluster lies along x
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full + s * 8, 1);
+      mbar_init(empty + s * 8, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full + b * 8, 1);
+      mbar_init(acc_empty + b * 8, 2 * WARPS);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(uint32_t(2 * BN)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();   // both CTAs' barriers exist before either's loads, commits or arrivals signal them
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  uint32_t leader_full, leader_acc_empty;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(leader_full) : "r"(full), "r"(0u));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(leader_acc_empty) : "r"(acc_empty), "r"(0u));
+
+  const int m = (MODE == FACTORS || MODE == ROWS) ? *w.count : w.m;
+  const int k = MODE == TABLE ? *w.count : w.k;
+  const int n_kb = (k + BK - 1) / BK, row_tiles = (m + 2 * BM - 1) / (2 * BM), col_tiles = (w.n + BN - 1) / BN;
+  const long long n_units = static_cast<long long>(row_tiles) * col_tiles * (MODE == ROWS ? w.splits : 1);
+
+  if (warp == 0) {
+    // ---- operands: the warp runs the loop, one elected lane issues. A stage is waited for with the opposite of the ring's parity, which a
+    // fresh barrier passes at once.
+    int stage = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    for (long long i = pair; i < n_units && ok; i += n_pairs) {
+      const Unit u = unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
+      const int a0 = (u.row * 2 + int(rank)) * BM, b0 = u.col * BN + int(rank) * HALF;
+      for (int kb = u.kb_begin; kb < u.kb_end && ok; ++kb) {
+        for (int t = 0; t < w.terms; ++t) {
+          if (!warp_wait(empty + stage * 8, parity ^ 1u)) {
+            if (lane == 0) atomicMax(w.error_flag, ERR_EMPTY);
+            ok = false;
+            break;
           }
-          g = factor == 0.f ? 0.f : factor * (expf(z - w.log_sum[r]) - (w.first + v == y ? 1.f : 0.f)) * slope;
+          if (elect_one()) {
+            const uint32_t bar = leader_full + stage * 8;
+            const int k0 = kb * BK, pa = plane_a(w.terms, t), pb = plane_b(w.terms, t);
+            if (rank == 0) mbar_expect_tx(full + stage * 8, 2 * (A_BYTES + B_BYTES));
+            const uint32_t a = a_base + stage * A_BYTES, b = b_base + stage * B_BYTES;
+            if constexpr (A_MN) {
+              load_pair(a, &map_a, a0, k0, pa, bar);
+              load_pair(a + BK * 128, &map_a, a0 + 64, k0, pa, bar);
+            } else {
+              load_pair(a, &map_a, k0, a0, pa, bar);
+            }
+            if constexpr (B_MN) {
+              load_pair(b, &map_b, b0, k0, pb, bar);
+              load_pair(b + BK * 128, &map_b, b0 + 64, k0, pb, bar);
+            } else {
+              load_pair(b, &map_b, k0, b0, pb, bar);
+            }
+          }
+          __syncwarp();
+          if (++stage == STAGES) {
+            stage = 0;
+            parity ^= 1u;
+          }
         }
-        if constexpr (MODE == ADD) g += to_float(out[v]);
-        out[v] = from_float<TO>(g);
+      }
+    }
+  } else if (warp == 1 && rank == 0) {
+    // ---- products of the pair (256 rows over the two CTAs)
+    constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(BN >> 3) << 17) |
+                               (uint32_t((2 * BM) >> 4) << 24);
+    const uint64_t a_desc = A_MN ? smem_desc(0, BK * 128, 1024) : smem_desc(0, 16, 1024);
+    const uint64_t b_desc = B_MN ? smem_desc(0, BK * 128, 1024) : smem_desc(0, 16, 1024);
+    constexpr uint32_t a_step = (A_MN ? UMMA_K * 128 : 32) >> 4, b_step = (B_MN ? UMMA_K * 128 : 32) >> 4;
+    int stage = 0;
+    uint32_t parity = 0, local = 0;   // this pair's count of units: accumulator local & 1
+    bool ok = true;
+    for (long long i = pair; i < n_units && ok; i += n_pairs, ++local) {
+      const Unit u = unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
+      const uint32_t buf = local & 1u;
+      if (!warp_wait(acc_empty + buf * 8, ((local >> 1) & 1u) ^ 1u)) {
+        if (lane == 0) atomicMax(w.error_flag, ERR_ACC);
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t acc = tmem + buf * BN;
+      const int steps = (u.kb_end - u.kb_begin) * w.terms;
+      for (int it = 0; it < steps; ++it) {
+        if (!warp_wait(full + stage * 8, parity)) {
+          if (lane == 0) atomicMax(w.error_flag, ERR_FULL);
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (elect_one()) {
+          const uint32_t a = (a_base + stage * A_BYTES) >> 4, b = (b_base + stage * B_BYTES) >> 4;
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk)
+            umma_pair(acc, a_desc + (a & 0x3FFF) + kk * a_step, b_desc + (b & 0x3FFF) + kk * b_step, idesc, (it > 0 || kk > 0) ? 1u : 0u);
+          commit_pair(empty + stage * 8);
+        }
+        __syncwarp();
+        if (++stage == STAGES) {
+          stage = 0;
+          parity ^= 1u;
+        }
+      }
+      if (elect_one()) commit_pair(acc_full + buf * 8);   // also on the error path: the others go on and the flag tells
+      __syncwarp();
+    }
+  } else if (warp >= 2) {
+    // ---- results: each CTA its own 128 rows; a warp 32 of them (the lanes of tensor memory that it may read) and half of the columns
+    const int q = warp & 3, side = (warp - 2) >> 2;
+    uint32_t local = 0;
+    bool ok = true;
+    for (long long i = pair; i < n_units; i += n_pairs, ++local) {
+      const Unit u = unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
+      const uint32_t buf = local & 1u;
+      const int row = (u.row * 2 + int(rank)) * BM + q * 32 + lane;
+      const int col0 = u.col * BN;
+      int target = -1;
+      float factor = 0.f, sum2 = 0.f;
+      if constexpr (MODE == FACTORS) {
+        if (row < m) {
+          target = w.targets[row] - w.first - col0;   // (no overflow: both lie in [0, vocab))
+          factor = w.factor[row];
+          sum2 = w.log_sum[row] * LOG2E;
+        }
+      }
+      if (ok && !warp_wait(acc_full + buf * 8, (local >> 1) & 1u)) {
+        if (lane == 0) atomicMax(w.error_flag, ERR_ACC);
+        ok = false;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const bool none = u.kb_end <= u.kb_begin;   // nothing to sum over: zeros
+      float top = -3.4028234663852886e38f, sum = 0.f;
+#pragma unroll 1
+      for (int c = side * HALF; c < (side + 1) * HALF && ok; c += 32) {
+        if (col0 + c >= w.n && MODE != LOGSUM) break;
+        uint32_t r[32];
+        tmem_load32(tmem + buf * BN + uint32_t(c) + (uint32_t(q * 32) << 16), r);
+        tmem_load_wait(r);
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = none ? 0.f : __uint_as_float(r[j]);
+        if constexpr (MODE == LOGSUM) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = log2_units<CAPPED>(v[j], w);
+          if (col0 + c + 32 > w.n) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = col0 + c + j < w.n ? v[j] : -INFINITY;
+          }
+          float most = top;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) most = max3(most, v[j], v[j + 1]);
+          float s0 = sum * fast_exp2(top - most), s1 = 0.f;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            s0 += fast_exp2(v[j] - most);
+            s1 += fast_exp2(v[j + 1] - most);
+          }
+          sum = s0 + s1;
+          top = most;
+        } else if constexpr (MODE == FACTORS) {
+          float slope[CAPPED ? 32 : 1];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if constexpr (CAPPED) {
+              const float h = fast_rcp(fast_exp2(v[j] * w.cap_in) + 1.f);   // (1 - tanh) / 2
+              v[j] = fast_exp2(fmaf(-2.f * w.cap_out, h, w.cap_out) - sum2);
+              slope[j] = 4.f * h * (1.f - h);                               // 1 - tanh^2
+            } else {
+              v[j] = fast_exp2(fmaf(v[j], LOG2E, -sum2));
+            }
+          }
+          if (__any_sync(0xffffffffu, target >= c && target < c + 32)) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] -= target == c + j ? 1.f : 0.f;
+          }
+          const bool counts = factor != 0.f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if constexpr (CAPPED) v[j] *= slope[j];
+            v[j] = counts ? v[j] * factor : 0.f;
+          }
+          // (rows up to the end of the tile: zeros, which the table's gradient adds to the last of its sums)
+          bf16* to = w.dz + row * w.ld;
+          if (w.terms == 1) {
+            put32<bf16>(to, col0 + c, INT_MAX, v, true);
+          } else {
+            for (int plane = 0; plane < 3; ++plane) {
+              float high[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                high[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
+                v[j] -= high[j];
+              }
+              put32<bf16>(to + plane * w.dz_plane, col0 + c, INT_MAX, high, true);
+            }
+          }
+        } else if constexpr (MODE == ROWS) {
+          if (row < m) {
+            float* to = w.shares + u.split * w.share_plane + row * w.ld;
+            if (w.add) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (col0 + c + j < w.n) v[j] += to[col0 + c + j];
+            }
+            put32<float>(to, col0 + c, w.n, v, true);
+          }
+        } else {
+          if (row < m) put32<T>(static_cast<T*>(w.out) + row * w.ld, col0 + c, w.n, v, (w.ld * sizeof(T)) % 16 == 0);
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive_cluster(leader_acc_empty + buf * 8);
+      if constexpr (MODE == LOGSUM) {
+        if (row < m) w.part[(size_t(u.col) * 2 + side) * m + row] = ok ? make_float2(top, sum) : make_float2(NAN, NAN);
+      }
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();   // neither CTA frees tensor memory or leaves while the other may still use it
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(2 * BN)) : "memory");
+  }
+}
+
+// A block's rows: their parts joined, R rows by 256 / R slices of the parts, then the target's logit as a sum of float products by a warp.
+template <typename T, int R>
+__global__ void __launch_bounds__(256) finish_kernel(const float2* part, int parts, const T* hidden, long long ld_h, const T* table, long long ld_t, const int32_t* targets,
+                                                     const float* weight, int rows, int width, int vocab, float softcap, float* loss, float* log_sum) {
+  __shared__ float2 held[256];
+  __shared__ float sums[R];
+  const int r0 = blockIdx.x * R, mine = r0 + threadIdx.x % R;
+  float top = -3.4028234663852886e38f, sum = 0.f;
+  if (mine < rows) {
+#pragma unroll 4
+    for (int i = threadIdx.x / R; i < parts; i += 256 / R) {
+      const float2 p = part[size_t(i) * rows + mine];
+      const float most = fmaxf(top, p.x);
+      sum = sum * fast_exp2(top - most) + p.y * fast_exp2(p.x - most);
+      top = most;
+    }
+  }
+  held[threadIdx.x] = make_float2(top, sum);
+  __syncthreads();
+  if (threadIdx.x < R) {
+    for (int i = 1; i < 256 / R; ++i) {
+      const float2 p = held[i * R + threadIdx.x];
+      const float most = fmaxf(top, p.x);
+      sum = sum * fast_exp2(top - most) + p.y * fast_exp2(p.x - most);
+      top = most;
+    }
+    sums[threadIdx.x] = fmaf(top, LN2, logf(sum));
+  }
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = warp; i < R && r0 + i < rows; i += 8) {
+    const int r = r0 + i, y = targets[r];
+    const float factor = weight ? weight[r] : 1.f;
+    const bool counts = y >= 0 && y < vocab && factor != 0.f;
+    const T* x = hidden + size_t(r) * ld_h;
+    const T* t = table + size_t(counts ? y : 0) * ld_t;
+    float dot = 0.f;
+    bool fine = true;   // (float32's planes hold no infinities: a row with one, or with NaN, has no sum)
+    if (counts || sizeof(T) == 4) {
+      for (int d = lane; d < width; d += 32) {
+        const float a = to_float(x[d]);
+        if (sizeof(T) == 4) fine = fine && fabsf(a) < INFINITY;
+        if (counts) dot = fmaf(a, to_float(t[d]), dot);
+      }
+    }
+    dot = warp_sum(dot);
+    fine = __all_sync(0xffffffffu, fine);
+    if (lane == 0) {
+      const float s = fine ? sums[i] : NAN;
+      log_sum[r] = s;
+      const float z = softcap > 0.f ? softcap * tanhf(dot / softcap) : dot;
+      const float gap = s - z;   // (never negative but by rounding)
+      loss[r] = counts ? factor * (gap < 0.f ? 0.f : gap) : 0.f;
+    }
+  }
+}
+
+// The rows that count (a token of the vocabulary, a weight that is not 0) side by side, their numbers in one plane or three, zeros behind them up to a
+// multiple of 256 rows; `place[r]` is where row r went, -1 for none. A block looks at all rows' tokens and takes its own.
+template <typename T>
+__global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long ld, int rows, int width, int vocab, int own, const int32_t* targets, const float* weight,
+                                                     const float* log_sum, bf16* x, long long ld_x, long long plane, int32_t* y_out, float* f_out, float* s_out,
+                                                     int32_t* place, int* count) {
+  __shared__ int totals[2][8];
+  const int first = blockIdx.x * own, last = min(rows, first + own);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto counts = [&](int r) {
+    const int y = targets[r];
+    return y >= 0 && y < vocab && (weight == nullptr || weight[r] != 0.f);
+  };
+  int before = 0, all = 0;
+  for (int r = threadIdx.x; r < rows; r += 256) {
+    const int c = counts(r) ? 1 : 0;
+    all += c;
+    before += r < first ? c : 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if (lane == 0) {
+    totals[0][warp] = before;
+    totals[1][warp] = all;
+  }
+  __syncthreads();
+  before = all = 0;
+  for (int i = 0; i < 8; ++i) {
+    before += totals[0][i];
+    all += totals[1][i];
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *count = all;
+  auto copy = [&](int to, const T* from) {   // (null: zeros)
+    for (int d = lane; d < width; d += 32) {
+      if constexpr (sizeof(T) == 2) {
+        x[size_t(to) * ld_x + d] = from ? from[d] : from_float<bf16>(0.f);
+      } else {
+        bf16 p[3];
+        split3(from ? from[d] : 0.f, p);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) x[i * plane + size_t(to) * ld_x + d] = p[i];
+      }
+    }
+  };
+  // a block's rows, 32 at a time
+  for (int begin = first; begin < last; begin += 32) {
+    const bool c = begin + lane < last && counts(begin + lane);
+    const unsigned mask = __ballot_sync(0xffffffffu, c);
+    if (warp == 0 && begin + lane < last) {
+      const int r = begin + lane, at = before + __popc(mask & ((1u << lane) - 1u));
+      place[r] = c ? at : -1;
+      if (c) {
+        y_out[at] = targets[r];
+        f_out[at] = weight ? weight[r] : 1.f;
+        s_out[at] = log_sum[r];
+      }
+    }
+    for (int i = warp; i < 32; i += 8)
+      if (mask >> i & 1u) copy(before + __popc(mask & ((1u << i) - 1u)), hidden + size_t(begin + i) * ld);
+    before += __popc(mask);
+  }
+  const int end = (all + 255) / 256 * 256;
+  for (int at = all + blockIdx.x + warp * gridDim.x; at < end; at += 8 * gridDim.x) copy(at, static_cast<const T*>(nullptr));
+}
+
+// A matrix in planes of bfloat16 whose rows start at 16 bytes: float32 in three, bfloat16 that tensor copies cannot read in one.
+template <typename T>
+__global__ void __launch_bounds__(256) planes_kernel(const T* from, long long ld, int rows, int width, bf16* to, long long ld_to, long long plane) {
+  const int lane = threadIdx.x & 31;
+  for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8LL) {
+    const T* x = from + r * ld;
+    bf16* o = to + r * ld_to;
+    for (int d = lane; d < width; d += 32) {
+      if constexpr (sizeof(T) == 2) {
+        o[d] = x[d];
+      } else {
+        bf16 p[3];
+        split3(x[d], p);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) o[i * plane + d] = p[i];
       }
     }
   }
 }
 
-__global__ void finish_kernel(const float2* part, int tiles, const float* at_target, const int32_t* targets, const float* weight, int rows, int vocab,
-                              float* loss, float* log_sum) {
-  const int r = blockIdx.x * blockDim.x + threadIdx.x;
-  if (r >= rows) return;
-  float top = -INFINITY, sum = 0.f;
-  for (int t = 0; t < tiles; ++t) top = fmaxf(top, part[size_t(t) * rows + r].x);
-  const float ref = top == -INFINITY ? 0.f : top;
-  for (int t = 0; t < tiles; ++t) {
-    const float2 p = part[size_t(t) * rows + r];
-    sum += p.x == -INFINITY ? p.y : p.y * expf(p.x - ref);
+// The hidden rows' gradient: shares of a gathered row added in one order, zeros for the rows that were left out.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const float* shares, int splits, long long plane, long long ld, const int32_t* place, T* out, long long ld_o, int rows,
+                                                   int width) {
+  const int lane = threadIdx.x & 31;
+  for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8LL) {
+    const int at = place[r];
+    T* o = out + r * ld_o;
+    for (int d = lane; d < width; d += 32) {
+      float sum = 0.f;
+      if (at >= 0) {
+        const float* s = shares + at * ld + d;
+        for (int i = 0; i < splits; ++i) sum += s[i * plane];
+      }
+      o[d] = from_float<T>(sum);
+    }
   }
-  const float s = ref + logf(sum);
-  log_sum[r] = s;
-  const int y = targets[r];
-  const float factor = weight ? weight[r] : 1.f;
-  loss[r] = (y >= 0 && y < vocab && factor != 0.f) ? factor * (s - at_target[r]) : 0.f;
 }
 
-template <typename TA, typename TB, typename TO, int MODE>
-void tiles(const Work& w, cudaStream_t stream) {
-  tile_kernel<TA, TB, TO, MODE><<<dim3((w.n + TILE - 1) / TILE, (w.m + TILE - 1) / TILE), 256, 0, stream>>>(w);
+// ---- host side ------------------------------------------------------------------------------
+
+inline long long up(long long x, long long to) { return (x + to - 1) / to * to; }
+
+// A matrix [rows, width] as tensor copies read it.
+struct Operand {
+  const void* at;
+  long long ld, plane;
+  int planes;
+};
+
+bool make_map(CUtensorMap* map, const Operand& o, long long inner, long long outer, int box_outer) {
+  cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(outer), cuuint64_t(o.planes)};
+  cuuint64_t strides[2] = {cuuint64_t(o.ld) * 2, cuuint64_t(o.planes > 1 ? o.plane : o.ld) * 2};
+  cuuint32_t box[3] = {cuuint32_t(BK), cuuint32_t(box_outer), 1};
+  return r2::encode_bf16_map(map, o.at, 3, dims, strides, box);
 }
 
-constexpr int PIECE = 8192;   // tokens whose logits' gradients are in memory at a time
+// How many CTA pairs the current device holds at once.
+int resident_pairs() {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+  if (dev < 64 && cached[dev].load() > 0) return cached[dev].load();
+  auto kernel = product_kernel<LOGSUM, false, bf16>;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM));
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(2, 1, 1);
+  config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = SMEM;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = 64;
+  }
+  if (dev < 64) cached[dev].store(n);
+  return n;
+}
+
+template <int MODE, bool CAPPED, typename T>
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Work& w, long long units, cudaStream_t stream) {
+  auto kernel = product_kernel<MODE, CAPPED, T>;
+  static std::atomic<bool> done[64];
+  const int status = allow_smem(kernel, SMEM, done);
+  if (status != R2_OK) return status;
+  const int pairs = resident_pairs();
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(2 * unsigned(units < pairs ? units : pairs), 1, 1);
+  config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = SMEM;
+  config.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, ma, mb, w);
+  return e != cudaSuccess ? int(e) : launch_status();
+}
+
+template <int MODE, typename T>
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Work& w, long long units, bool capped, cudaStream_t stream) {
+  if constexpr (MODE == LOGSUM || MODE == FACTORS) {
+    if (capped) return launch<MODE, true, T>(ma, mb, w, units, stream);
+  }
+  return launch<MODE, false, T>(ma, mb, w, units, stream);
+}
+
+int row_blocks(long long rows) { return int(rows < 8 * 1184 ? (rows + 7) / 8 : 1184); }
+
+// What a call's scratch holds, in bytes from its start.
+constexpr long long FACTOR_BYTES = 256ll << 20;   // of dz at a time
+
+struct Layout {
+  int size, planes;                 // of a number; bfloat16 planes of an operand
+  long long rows_up, width_up;      // rows to a multiple of 256, numbers to one of 8
+  int pieces, splits, per_split;
+  long long piece;                  // tokens at a time, a multiple of 256
+  long long table, hidden, part, factors, shares, targets, factor, sums, place, count, total;
+};
+
+Layout layout(int dtype, long long rows, long long width, long long vocab, bool gradient) {
+  Layout l = {};
+  l.size = dtype == R2_F32 ? 4 : 2;
+  l.planes = dtype == R2_F32 ? 3 : 1;
+  l.rows_up = up(rows, 256);
+  l.width_up = up(width, 8);
+  long long at = 0;
+  auto take = [&](long long bytes) {
+    const long long begin = at;
+    at += up(bytes, 256);
+    return begin;
+  };
+  // (a bfloat16 table is read where it lies if tensor copies can; there is room for it in either case)
+  l.table = take(l.planes * vocab * l.width_up * 2);
+  l.hidden = take(l.planes * l.rows_up * l.width_up * 2);
+  if (!gradient) {
+    l.part = take(up(vocab, BN) / BN * 2 * rows * 8);
+  } else {
+    long long most = FACTOR_BYTES / (l.rows_up * 2 * l.planes) / BN * BN;
+    if (most < BN) most = BN;
+    l.pieces = int((vocab + most - 1) / most);
+    l.piece = up((vocab + l.pieces - 1) / l.pieces, BN);
+    const int n_kb = int((l.piece + BK - 1) / BK);
+    const long long tiles = l.rows_up / 256 * (up(width, BN) / BN);
+    const int pairs = resident_pairs();
+    // shares of k: so many that the last round of pairs is full, but no shorter than eight steps
+    long long best = -1;
+    for (int s = 1; s <= 64 && (s == 1 || n_kb / s >= 8); ++s) {
+      const long long cost = (tiles * s + pairs - 1) / pairs * (((n_kb + s - 1) / s) * l.planes * (l.planes + 1) / 2 + 8);
+      if (best < 0 || cost < best) {
+        best = cost;
+        l.per_split = (n_kb + s - 1) / s;
+        l.splits = (n_kb + l.per_split - 1) / l.per_split;
+      }
+    }
+    l.factors = take(l.planes * l.rows_up * l.piece * 2);
+    l.shares = take(l.splits * l.rows_up * l.width_up * 4);
+    l.targets = take(l.rows_up * 4);
+    l.factor = take(l.rows_up * 4);
+    l.sums = take(l.rows_up * 4);
+    l.place = take(rows * 4);
+    l.count = take(4);
+  }
+  l.total = at;
+  return l;
+}
+
+bool copies_read(const void* at, long long ld, long long rows, long long width) {
+  return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (rows <= 1 || (ld % 8 == 0 && ld >= width));
+}
+
+// The matrix itself where tensor copies can read it, else planes of it in `space`.
+template <typename T>
+Operand operand(const void* at, long long ld, long long rows, long long width, const Layout& l, char* space, cudaStream_t stream) {
+  if (sizeof(T) == 2 && copies_read(at, ld, rows, width)) return {at, rows <= 1 ? l.width_up : ld, 0, 1};
+  bf16* to = reinterpret_cast<bf16*>(space);
+  planes_kernel<T><<<row_blocks(rows), 256, 0, stream>>>(static_cast<const T*>(at), ld, int(rows), int(width), to, l.width_up, rows * l.width_up);
+  return {to, l.width_up, rows * l.width_up, l.planes};
+}
+
+void set_cap(Work& w, float softcap) {
+  if (softcap > 0.f) {
+    w.cap_in = 2.f * LOG2E / softcap;
+    w.cap_out = softcap * LOG2E;
+  }
+}
 
 template <typename T>
 int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_t, int rows, int width, int vocab, const int32_t* targets, const float* weight,
-            float softcap, float* loss, float* log_sum, char* space, cudaStream_t stream) {
+            float softcap, float* loss, float* log_sum, char* space, int* error, cudaStream_t stream) {
+  const Layout l = layout(sizeof(T) == 4 ? R2_F32 : R2_BF16, rows, width, vocab, false);
+  const Operand x = operand<T>(hidden, ld_h, rows, width, l, space + l.hidden, stream);
+  const Operand t = operand<T>(table, ld_t, vocab, width, l, space + l.table, stream);
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, x, width, rows, BM) || !make_map(&mb, t, width, vocab, HALF)) return R2_BAD_ALIGN;
   Work w = {};
-  w.a = {hidden, ld_h, 1};
-  w.b = {table, ld_t, 1};
   w.m = rows;
   w.n = vocab;
   w.k = width;
-  w.softcap = softcap;
-  w.targets = targets;
-  w.vocab = vocab;
-  w.at_target = reinterpret_cast<float*>(space);
-  w.part = reinterpret_cast<float2*>(space + (size_t(rows) * 4 + 15) / 16 * 16);
-  tiles<T, T, T, LOGITS>(w, stream);
-  finish_kernel<<<(rows + 127) / 128, 128, 0, stream>>>(w.part, (vocab + TILE - 1) / TILE, w.at_target, targets, weight, rows, vocab, loss, log_sum);
+  w.terms = l.planes * (l.planes + 1) / 2;
+  w.part = reinterpret_cast<float2*>(space + l.part);
+  w.error_flag = error;
+  set_cap(w, softcap);
+  const long long tiles = (l.rows_up / 256) * (up(vocab, BN) / BN);
+  const int status = launch<LOGSUM, bf16>(ma, mb, w, tiles, softcap > 0.f, stream);
+  if (status != R2_OK) return status;
+  const int parts = int(up(vocab, BN) / BN) * 2;
+  const T *h = static_cast<const T*>(hidden), *tab = static_cast<const T*>(table);
+  if (rows >= 4096) {
+    finish_kernel<T, 32><<<(rows + 31) / 32, 256, 0, stream>>>(w.part, parts, h, ld_h, tab, ld_t, targets, weight, rows, width, vocab, softcap, loss, log_sum);
+  } else {
+    finish_kernel<T, 8><<<(rows + 7) / 8, 256, 0, stream>>>(w.part, parts, h, ld_h, tab, ld_t, targets, weight, rows, width, vocab, softcap, loss, log_sum);
+  }
   return launch_status();
 }
 
 template <typename T>
 int gradient_of(const void* hidden, long long ld_h, const void* table, long long ld_t, int rows, int width, int vocab, const int32_t* targets, const float* weight,
-                const float* log_sum, float softcap, void* d_hidden, long long ld_dh, void* d_table, long long ld_dt, char* space, cudaStream_t stream) {
-  float* dz = reinterpret_cast<float*>(space);
-  const int piece = vocab < PIECE ? vocab : PIECE;
-  float* sums = dz + size_t(rows) * piece;
-  cudaMemsetAsync(sums, 0, size_t(rows) * width * 4, stream);
-  for (int first = 0; first < vocab; first += piece) {
-    const int n = vocab - first < piece ? vocab - first : piece;
-    const T* part = static_cast<const T*>(table) + size_t(first) * ld_t;
-    Work w = {};
-    w.a = {hidden, ld_h, 1};
-    w.b = {part, ld_t, 1};
-    w.m = rows;
+                const float* log_sum, float softcap, void* d_hidden, long long ld_dh, void* d_table, long long ld_dt, char* space, int* error, cudaStream_t stream) {
+  const Layout l = layout(sizeof(T) == 4 ? R2_F32 : R2_BF16, rows, width, vocab, true);
+  const Operand t = operand<T>(table, ld_t, vocab, width, l, space + l.table, stream);
+  bf16* gathered = reinterpret_cast<bf16*>(space + l.hidden);
+  const Operand x = {gathered, l.width_up, l.rows_up * l.width_up, l.planes};
+  int* count = reinterpret_cast<int*>(space + l.count);
+  int32_t* place = reinterpret_cast<int32_t*>(space + l.place);
+  int own = (rows + 591) / 592;
+  own = own > 32 ? 32 : own;
+  gather_kernel<T><<<(rows + own - 1) / own, 256, 0, stream>>>(
+      static_cast<const T*>(hidden), ld_h, rows, width, vocab, own, targets, weight, log_sum, gathered, x.ld, x.plane, reinterpret_cast<int32_t*>(space + l.targets),
+      reinterpret_cast<float*>(space + l.factor), reinterpret_cast<float*>(space + l.sums), place, count);
+  Work w = {};
+  w.m = rows;
+  w.count = count;
+  w.terms = l.planes * (l.planes + 1) / 2;
+  w.targets = reinterpret_cast<int32_t*>(space + l.targets);
+  w.factor = reinterpret_cast<float*>(space + l.factor);
+  w.log_sum = reinterpret_cast<float*>(space + l.sums);
+  w.dz = reinterpret_cast<bf16*>(space + l.factors);
+  w.dz_plane = l.rows_up * l.piece;
+  w.shares = reinterpret_cast<float*>(space + l.shares);
+  w.share_plane = l.rows_up * l.width_up;
+  w.error_flag = error;
+  set_cap(w, softcap);
+  const Operand dz = {w.dz, l.piece, w.dz_plane, l.planes};
+  CUtensorMap ma, mb;
+  int status = launch_status();
+  const long long row_tiles = l.rows_up / 256, width_tiles = up(width, BN) / BN;
+  for (long long first = 0; first < vocab && status == R2_OK; first += l.piece) {
+    const int n = int(vocab - first < l.piece ? vocab - first : l.piece);
+    const Operand part = {static_cast<const bf16*>(t.at) + first * t.ld, t.ld, t.plane, t.planes};
+    w.first = int(first);
     w.n = n;
     w.k = width;
-    w.softcap = softcap;
-    w.targets = targets;
-    w.weight = weight;
-    w.log_sum = log_sum;
-    w.first = first;
-    w.vocab = vocab;
-    w.out = dz;
-    w.ld = piece;
-    tiles<T, T, float, DZ>(w, stream);
-    if (d_hidden) {
-      Work d = {};
-      d.a = {dz, piece, 1};
-      d.b = {part, 1, ld_t};
-      d.m = rows;
+    w.ld = l.piece;
+    if (!make_map(&ma, x, width, l.rows_up, BM) || !make_map(&mb, part, width, n, HALF)) return R2_BAD_ALIGN;
+    status = launch<FACTORS, bf16>(ma, mb, w, row_tiles * (up(n, BN) / BN), softcap > 0.f, stream);
+    if (status == R2_OK && d_hidden) {
+      Work d = w;
       d.n = width;
       d.k = n;
-      d.out = sums;
-      d.ld = width;
-      tiles<float, T, float, ADD>(d, stream);
+      d.per_split = l.per_split;
+      d.splits = l.splits;
+      d.add = first > 0;
+      d.ld = l.width_up;
+      if (!make_map(&ma, dz, n, l.rows_up, BM) || !make_map(&mb, part, width, n, BK)) return R2_BAD_ALIGN;
+      status = launch<ROWS, bf16>(ma, mb, d, row_tiles * width_tiles * d.splits, false, stream);
     }
-    if (d_table) {
-      Work d = {};
-      d.a = {dz, 1, piece};
-      d.b = {hidden, 1, ld_h};
+    if (status == R2_OK && d_table) {
+      Work d = w;
       d.m = n;
       d.n = width;
-      d.k = rows;
-      d.out = static_cast<T*>(d_table) + size_t(first) * ld_dt;
+      d.out = static_cast<T*>(d_table) + first * ld_dt;
       d.ld = ld_dt;
-      tiles<float, T, T, STORE>(d, stream);
+      if (!make_map(&ma, dz, n, l.rows_up, BK) || !make_map(&mb, x, width, l.rows_up, BK)) return R2_BAD_ALIGN;
+      status = launch<TABLE, T>(ma, mb, d, up(n, 256) / 256 * width_tiles, false, stream);
     }
   }
-  return launch_status();
+  if (status == R2_OK && d_hidden) {
+    join_kernel<T><<<row_blocks(rows), 256, 0, stream>>>(w.shares, l.splits, w.share_plane, l.width_up, place, static_cast<T*>(d_hidden), ld_dh, rows, width);
+    status = launch_status();
+  }
+  return status;
 }
 
-template <typename T>
-__global__ void round_kernel(const float* from, T* to, long long ld, int rows, int width) {
-  for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < size_t(rows) * width; i += size_t(gridDim.x) * blockDim.x)
-    to[i / width * ld + i % width] = from_float<T>(from[i]);
-}
+constexpr int MOST = 1 << 30;   // rows, numbers of a row, tokens: indexes of tiles stay in 32 bits
 
 }  // namespace
 
+// Bytes of scratch for a call (of a loss, or of gradients).
 extern "C" long long r2_token_loss_space(int dtype, int rows, int width, int vocab, int gradient) {
-  if (!gradient) return (size_t(rows) * 4 + 15) / 16 * 16 + size_t((vocab + TILE - 1) / TILE) * rows * 8;
-  return (size_t(rows) * (vocab < PIECE ? vocab : PIECE) + size_t(rows) * width) * 4;
+  return layout(dtype, rows, width, vocab, gradient != 0).total;
 }
 
+// `space`: 256-byte aligned, r2_token_loss_space bytes.
 extern "C" int r2_token_loss(int dtype, const void* hidden, long long ld_h, const void* table, long long ld_t, int rows, int width, int vocab,
                              const int32_t* targets, const float* weight, float softcap, float* loss, float* log_sum, void* space, int* error, cudaStream_t stream) {
-  if (dtype == R2_F32) return loss_of<float>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, softcap, loss, log_sum, (char*)space, stream);
-  if (dtype == R2_BF16) return loss_of<bf16>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, softcap, loss, log_sum, (char*)space, stream);
+  if (rows < 1 || width < 1 || vocab < 1) return R2_BAD_SHAPE;
+  if (rows > MOST || width > MOST || vocab > MOST) return R2_UNSUPPORTED;
+  if (dtype == R2_F32) return loss_of<float>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, softcap, loss, log_sum, (char*)space, error, stream);
+  if (dtype == R2_BF16) return loss_of<bf16>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, softcap, loss, log_sum, (char*)space, error, stream);
   return R2_BAD_DTYPE;
 }
 
 extern "C" int r2_token_loss_gradient(int dtype, const void* hidden, long long ld_h, const void* table, long long ld_t, int rows, int width, int vocab,
                                       const int32_t* targets, const float* weight, const float* log_sum, float softcap, void* d_hidden, long long ld_dh,
                                       void* d_table, long long ld_dt, void* space, int* error, cudaStream_t stream) {
-  const float* sums = (const float*)space + size_t(rows) * (vocab < PIECE ? vocab : PIECE);
-  const int grid = int((size_t(rows) * width + 255) / 256 < 4096 ? (size_t(rows) * width + 255) / 256 : 4096);
-  int status;
-  if (dtype == R2_F32) {
-    status = gradient_of<float>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, log_sum, softcap, d_hidden, ld_dh, d_table, ld_dt, (char*)space, stream);
-    if (status == R2_OK && d_hidden) round_kernel<float><<<grid, 256, 0, stream>>>(sums, (float*)d_hidden, ld_dh, rows, width);
-  } else if (dtype == R2_BF16) {
-    status = gradient_of<bf16>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, log_sum, softcap, d_hidden, ld_dh, d_table, ld_dt, (char*)space, stream);
-    if (status == R2_OK && d_hidden) round_kernel<bf16><<<grid, 256, 0, stream>>>(sums, (bf16*)d_hidden, ld_dh, rows, width);
-  } else {
-    return R2_BAD_DTYPE;
-  }
-  return status == R2_OK ? launch_status() : status;
+  if (rows < 1 || width < 1 || vocab < 1) return R2_BAD_SHAPE;
+  if (rows > MOST || width > MOST || vocab > MOST) return R2_UNSUPPORTED;
+  if (dtype == R2_F32)
+    return gradient_of<float>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, log_sum, softcap, d_hidden, ld_dh, d_table, ld_dt, (char*)space, error, stream);
+  if (dtype == R2_BF16)
+    return gradient_of<bf16>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, log_sum, softcap, d_hidden, ld_dh, d_table, ld_dt, (char*)space, error, stream);
+  return R2_BAD_DTYPE;
 }
