@@ -2351,8 +2351,8 @@ def token_rows(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, ou
 def token_rows_gradient(ids: torch.Tensor, above: torch.Tensor, vocab: int, *, scale: float = 1.0, out_dtype: torch.dtype | None = None,
                         into: torch.Tensor | None = None) -> torch.Tensor:
     """The gradient of a table of `vocab` rows that `token_rows` read: [V, D], whose row v is `scale` times the sum of the rows of `above` [T, D] (float32
-    or bfloat16; rows contiguous, any row stride) at which `ids` (int32 [T]) is v, added in float32 in the order of the places and rounded once, so
-    that the same call gives the same bits. It is a new table in `above`'s type or `out_dtype`, zero where no token came; or the sums are added to `into` [V, D] (float32 or
+    or bfloat16; rows contiguous, any row stride) at which `ids` (int32 [T]) is v, added in float32 in an order that the call's sizes and ids decide (that of the
+    places, for 64 of them at most) and rounded once, so that the same call gives the same bits. It is a new table in `above`'s type or `out_dtype`, zero where no token came; or the sums are added to `into` [V, D] (float32 or
     bfloat16), whose rows without a token are left as they are: a tied table's gradient, begun by `token_loss_gradient`. Tokens outside [0, V) count for nothing."""
     code, tokens, width, ld, device = _matrix(above, "above", "token_rows_gradient")
     ids_at = _per_row(ids, "ids", torch.int32, tokens, device)
@@ -2378,6 +2378,10 @@ def token_rows_gradient(ids: torch.Tensor, above: torch.Tensor, vocab: int, *, s
             raise KernelError(f"token_rows_gradient: into {tuple(into.shape)} of {into.dtype} on {into.device} is not [{vocab}, {width}]")
         if vocab > 1 and out_ld < width:
             raise KernelError("token_rows_gradient: rows of into overlap")
+        for t in (above, ids):
+            begin, end = t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+            if t.numel() and begin < into.data_ptr() + ((vocab - 1) * out_ld + width) * into.element_size() and into.data_ptr() < end:
+                raise KernelError("token_rows_gradient: into overlaps what it is made from")
     if tokens and width:
         space = _space(above.device, _logit_entry("token_rows_space")(tokens, width, vocab))
         _check(_logit_entry("token_rows_gradient")(code, out_code, ids_at, above.data_ptr(), ld, out.data_ptr(), out_ld, tokens, width, vocab, scale,
