@@ -2,12 +2,15 @@
 //
 //   out_t = scale * W[i_t]  (zeros where i_t is no token),   dW_v = scale * sum over t with i_t = v of above_t, in one order
 //
-// The gradient is one launch and needs nothing between CTAs. The table's rows are dealt out by the remainder of their number (tokens that stand often
-// lie side by side in a vocabulary), its columns in slices, and a CTA owns a deal and a slice: it goes through all tokens, lists the places of its own in
-// their order, sorts the list by token (a count, a running sum, a stable placing), writes zeros to the rows without one and adds up the others. Its eight warps
-// share the sorted places evenly, eight rows from above on their way to each at any time, so that a token that stands everywhere and tokens that stand once take the
-// same time; a token whose places lie in several warps' shares is joined behind them, in their order. Going through the tokens costs each CTA 4 bytes
-// a token twice, read from L2; the rows from above, which are hundreds of times as much, are read once.
+// The gradient in two launches:
+//
+//   deal_kernel  sorts the places by token, stable, and writes zeros to the rows without one. The table's rows are dealt out to CTAs by the remainder of their
+//                number (tokens that stand often lie side by side in a vocabulary). A CTA goes through all tokens, counts its own and those of lower deals (so that
+//                it knows where in the sorted list its part begins, without a word between CTAs), lists its places in their order and places them by
+//                row; half of its warps write zeros meanwhile, which is most of what a small batch costs.
+//   sum_kernel   a CTA takes the sorted places of eight windows, a warp each, and up to 256 columns: a token that stands everywhere and tokens that stand once
+//                take the same time. A row whose places lie in several windows is joined in shared memory; one that goes on in other CTAs leaves float sums in
+//                memory, and the last of those CTAs adds them, in the order of the places whoever that is.
 //
 // Bound by the bytes of the rows from above and of the table.
 #include "common.cuh"
@@ -15,10 +18,11 @@
 namespace {
 
 constexpr int THREADS = 256, WARPS = 8;
-constexpr int SLICE = 256;          // columns of a CTA at most
-constexpr int LISTED = 6144;        // places that shared memory holds (beyond them: the scratch)
-constexpr int LISTED_BYTES = LISTED * 12;
-constexpr int MOST_ROWS = 8192;     // of a CTA (16 bits hold one)
+constexpr int SLICE = 256;             // columns of a warp at most
+constexpr int DEAL_THREADS = 1024, DEAL_WARPS = 32, SORTERS = 16;   // of a dealing CTA: those that sort; the others write zeros
+constexpr int LISTED = 256;            // places that shared memory holds of what a dealing warp lists (if one has more: the scratch)
+constexpr int MOST_ROWS = 16384;       // of a deal
+constexpr int LISTED_BYTES = DEAL_WARPS * LISTED * 8;
 
 struct Work {
   const int32_t* ids;
@@ -29,9 +33,15 @@ struct Work {
   int tokens, width, vocab;
   float scale;
   int add;
-  int deals, slice;                 // rows v with v mod deals = the CTA's; columns of a slice
+  int deals;                        // rows v with v mod deals = the CTA's
   unsigned long long inverse;       // v / deals = v * inverse >> 64
-  int32_t* spill;                   // [slice]: places [2][tokens], rows as 16 bits [2][tokens]
+  int32_t *row, *place;             // [tokens]: the sorted list: by deal, row and place
+  int32_t *list_row, *list_place;   // [tokens]: a deal's list before it is sorted, where shared memory does not hold it
+  int* held;                        // how many places hold a token
+  int slices, slice, window;        // of the columns, columns of one, sorted places of a warp
+  int* arrived;                     // [CTA of places][slice]: CTAs that have left their share of the row that goes on from this one
+  float* shares;                    // [CTA of places][2][width_up]: sums of a row that an earlier CTA began; of one that the next goes on with
+  int width_up, groups, wide;       // (groups: CTAs of places)
 };
 
 // A lane's columns of a slice: pieces of 16 bytes, or every 32nd number.
@@ -103,107 +113,120 @@ __device__ __forceinline__ void put_row(O* row, const Lane<T, WIDE>& sum, int wi
   }
 }
 
-template <typename T, typename O, bool WIDE>
-__global__ void __launch_bounds__(THREADS, 2) gradient_kernel(const Work w) {
+template <typename O>
+__global__ void __launch_bounds__(DEAL_THREADS, 1) deal_kernel(const Work w) {
   extern __shared__ int32_t shared[];
-  __shared__ int mine[WARPS], lower[WARPS], running[WARPS];
-  __shared__ int head_row[WARPS], tail_row[WARPS];   // whose sums are in `heads` and `tails`, -1: none
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int deal = blockIdx.x % w.deals, slice = blockIdx.x / w.deals;
-  const int rows = int((static_cast<long long>(w.vocab) - deal + w.deals - 1) / w.deals);   // that this CTA owns
-  int32_t* ends = shared;   // [rows]: counts, then where a row's places begin, then where they end
+  __shared__ int mine[DEAL_WARPS], lower[DEAL_WARPS], running[SORTERS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, deal = blockIdx.x;
+  const int rows = int((static_cast<long long>(w.vocab) - deal + w.deals - 1) / w.deals);
+  int32_t* ends = shared;                                              // [rows]: counts, then where a row's places begin in this deal's part, then where they end
+  uint32_t* empty = reinterpret_cast<uint32_t*>(shared + rows);        // a bit a row: no place (the counts change)
+  int32_t* list_row = reinterpret_cast<int32_t*>(empty + (rows + 31) / 32);   // [warp][LISTED]
+  int32_t* list_place = list_row + DEAL_WARPS * LISTED;
   const unsigned inverse_high = unsigned(w.inverse >> 32), inverse_low = unsigned(w.inverse);
   auto quotient = [&](int id) {
     const unsigned long long v = unsigned(id);
     return int((v * inverse_high + (v * inverse_low >> 32)) >> 32);
   };
-
-  for (int j = threadIdx.x; j < rows; j += THREADS) ends[j] = 0;
+  for (int j = threadIdx.x; j < rows; j += DEAL_THREADS) ends[j] = 0;
   __syncthreads();
+  pdl_launch_dependents();
+  pdl_wait();
+  for (long long i = deal * DEAL_THREADS + threadIdx.x; i < static_cast<long long>(w.groups) * w.slices; i += w.deals * DEAL_THREADS) w.arrived[i] = 0;
 
-  // ---- a warp's share of the places: how many are this CTA's, how many of a lower deal
-  const int share = ((w.tokens + WARPS - 1) / WARPS + 255) / 256 * 256;
-  const int first = int(min(static_cast<long long>(warp) * share, static_cast<long long>(w.tokens))), last = int(min(static_cast<long long>(first) + share, static_cast<long long>(w.tokens)));
-  int n_mine = 0, n_lower = 0;
-  for (int t0 = first; t0 < last; t0 += 256) {
-    int id[8];
+  // ---- a warp's share of the places: lists this CTA's (as far as there is room), counts those of lower deals
+  const int share = ((w.tokens + DEAL_WARPS - 1) / DEAL_WARPS + 255) / 256 * 256;
+  auto begin_of = [&](int i) { return int(min(static_cast<long long>(i) * share, static_cast<long long>(w.tokens))); };
+  auto walk = [&](int part, auto&& each) {   // each(row, place, own, owners before it in this part)
+    const int last = begin_of(part + 1);
+    int before = 0;
+    for (int t0 = begin_of(part); t0 < last; t0 += 256) {
+      int id[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) id[j] = t0 + 32 * j + lane < last ? __ldg(w.ids + t0 + 32 * j + lane) : -1;
+      for (int j = 0; j < 8; ++j) id[j] = t0 + 32 * j + lane < last ? w.ids[t0 + 32 * j + lane] : -1;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (id[j] < 0 || id[j] >= w.vocab) continue;
-      const int row = quotient(id[j]), at = id[j] - row * w.deals;
-      if (at == deal) {
-        atomicAdd(&ends[row], 1);
-        ++n_mine;
+      for (int j = 0; j < 8; ++j) {
+        const bool token = id[j] >= 0 && id[j] < w.vocab;
+        const int row = quotient(token ? id[j] : 0), at = id[j] - row * w.deals;
+        const unsigned mask = __ballot_sync(0xffffffffu, token && at == deal);
+        each(row, t0 + 32 * j + lane, token && at == deal, before + __popc(mask & ((1u << lane) - 1u)), token && at < deal);
+        before += __popc(mask);
       }
-      n_lower += at < deal ? 1 : 0;
     }
-  }
+    return before;
+  };
+  int n_lower = 0;
+  const int n_mine = walk(warp, [&](int row, int place, bool own, int at, bool below) {
+    if (own) {
+      atomicAdd(&ends[row], 1);
+      if (at < LISTED) {
+        list_row[warp * LISTED + at] = row;
+        list_place[warp * LISTED + at] = place;
+      }
+    }
+    n_lower += below ? 1 : 0;
+  });
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    n_mine += __shfl_xor_sync(0xffffffffu, n_mine, o);
-    n_lower += __shfl_xor_sync(0xffffffffu, n_lower, o);
-  }
+  for (int o = 16; o > 0; o >>= 1) n_lower += __shfl_xor_sync(0xffffffffu, n_lower, o);
   if (lane == 0) {
     mine[warp] = n_mine;
     lower[warp] = n_lower;
   }
   __syncthreads();
-  int total = 0, before = 0, offset = 0;
+  int total = mine[lane], offset = lower[lane], most = total;   // (a lane a warp)
 #pragma unroll
-  for (int i = 0; i < WARPS; ++i) {
-    before += i < warp ? mine[i] : 0;
-    total += mine[i];
-    offset += lower[i];
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    offset += __shfl_xor_sync(0xffffffffu, offset, o);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
   }
+  if (deal == w.deals - 1 && threadIdx.x == 0) *w.held = offset + total;
 
   // ---- rows without a place
-  const int col = slice * w.slice, width = min(w.slice, w.width - col);
-  const T* above = static_cast<const T*>(w.above) + col;
-  O* out = static_cast<O*>(w.out) + col;
-  Lane<T, WIDE> sum;
-  sum.clear();
-  if (!w.add) {
-    for (int j = warp; j < rows; j += WARPS)
-      if (ends[j] == 0) put_row<T, O, WIDE>(out + (static_cast<long long>(j) * w.deals + deal) * w.ld_o, sum, width, 1.f, false, lane);
+  for (int j0 = warp * 32; j0 < rows; j0 += DEAL_THREADS) {
+    const unsigned none = __ballot_sync(0xffffffffu, j0 + lane < rows && ends[j0 + lane] == 0);
+    if (lane == 0) empty[j0 / 32] = none;
   }
-  if (total == 0) return;
-  __syncthreads();   // (the counts become places)
-
-  // ---- the list (token and place) and the sorted one: in shared memory, or in this deal's part of the slice's scratch
-  int32_t* places = shared + rows;
-  long long apart = LISTED;
-  uint16_t* numbers = reinterpret_cast<uint16_t*>(places + 2 * LISTED);
-  if (total > LISTED) {
-    places = w.spill + static_cast<long long>(slice) * 3 * w.tokens + offset;
-    numbers = reinterpret_cast<uint16_t*>(w.spill + static_cast<long long>(slice) * 3 * w.tokens + 2 * static_cast<long long>(w.tokens)) + offset;
-    apart = w.tokens;
-  }
-  int32_t *list_place = places, *sorted_place = places + apart;
-  uint16_t *list_row = numbers, *sorted_row = numbers + apart;
-  if (n_mine > 0) {
-    for (int t0 = first; t0 < last; t0 += 256) {
-      int id[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) id[j] = t0 + 32 * j + lane < last ? __ldg(w.ids + t0 + 32 * j + lane) : -1;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int row = quotient(id[j] < 0 ? 0 : id[j]);
-        const bool own = id[j] >= 0 && id[j] < w.vocab && id[j] - row * w.deals == deal;
-        const unsigned mask = __ballot_sync(0xffffffffu, own);
-        if (own) {
-          const int at = before + __popc(mask & ((1u << lane) - 1u));
-          list_row[at] = uint16_t(row);
-          list_place[at] = t0 + 32 * j + lane;
+  __syncthreads();
+  if (warp >= SORTERS || total == 0) {
+    if (!w.add) {
+      const int n = total == 0 ? DEAL_WARPS : DEAL_WARPS - SORTERS, first = total == 0 ? warp : warp - SORTERS;
+      for (int j = first; j < rows; j += n) {
+        if (!(empty[j >> 5] >> (j & 31) & 1u)) continue;
+        O* to = static_cast<O*>(w.out) + (static_cast<long long>(j) * w.deals + deal) * w.ld_o;
+        if (w.wide) {
+          for (int c = lane * int(16 / sizeof(O)); c < w.width; c += 32 * int(16 / sizeof(O))) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
+        } else {
+          for (int c = lane; c < w.width; c += 32) to[c] = from_float<O>(0.f);
         }
-        before += __popc(mask);
       }
+    }
+    return;
+  }
+  auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(SORTERS * 32) : "memory"); };
+
+  // ---- a list that shared memory does not hold: listed again, as one
+  int apart = LISTED;
+  if (most > LISTED) {
+    list_row = w.list_row + offset;
+    list_place = w.list_place + offset;
+    apart = 0;
+    for (int part = warp; part < DEAL_WARPS; part += SORTERS) {
+      int before = lane < part ? mine[lane] : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+      walk(part, [&](int row, int place, bool own, int at, bool) {
+        if (own) {
+          list_row[before + at] = row;
+          list_place[before + at] = place;
+        }
+      });
     }
   }
   // where each row's places begin: a thread's share of the rows, then the threads'
   {
-    const int per = (rows + THREADS - 1) / THREADS, from = min(rows, int(threadIdx.x) * per), to = min(rows, from + per);
+    constexpr int N = SORTERS * 32;
+    const int per = (rows + N - 1) / N, from = min(rows, int(threadIdx.x) * per), to = min(rows, from + per);
     int own = 0;
     for (int j = from; j < to; ++j) own += ends[j];
     int up = own;
@@ -213,97 +236,121 @@ __global__ void __launch_bounds__(THREADS, 2) gradient_kernel(const Work w) {
       up += lane >= o ? x : 0;
     }
     if (lane == 31) running[warp] = up;
-    __syncthreads();
-    int begin = up - own;
+    sync();
+    int begin = (lane < warp ? running[lane] : 0);
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) begin += i < warp ? running[i] : 0;
+    for (int o = 16; o > 0; o >>= 1) begin += __shfl_xor_sync(0xffffffffu, begin, o);
+    begin += up - own;
     for (int j = from; j < to; ++j) {
       const int n = ends[j];
       ends[j] = begin;
       begin += n;
     }
-    __syncthreads();
+    sync();
   }
-  // a stable placing: a warp takes the rows of its number mod 8 from the list, in the list's order
-  int next_row = lane < total ? list_row[lane] : -1, next_place = lane < total ? list_place[lane] : 0;
-  for (int i0 = 0; i0 < total; i0 += 32) {
-    const int row = next_row, place = next_place;
-    if (i0 + 32 < total) {   // (asked for ahead: the list may lie in memory)
-      next_row = i0 + 32 + lane < total ? list_row[i0 + 32 + lane] : -1;
-      next_place = i0 + 32 + lane < total ? list_place[i0 + 32 + lane] : 0;
+  // a stable placing: a warp takes the rows of its number mod 16 from the list, in the list's order
+  auto place_all = [&](const int32_t* from_row, const int32_t* from_place, int n) {
+    int next_row = lane < n ? from_row[lane] : -1, next_place = lane < n ? from_place[lane] : 0;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int row = next_row, place = next_place;
+      if (i0 + 32 < n) {   // (asked for ahead: the list may lie in memory)
+        next_row = i0 + 32 + lane < n ? from_row[i0 + 32 + lane] : -1;
+        next_place = i0 + 32 + lane < n ? from_place[i0 + 32 + lane] : 0;
+      }
+      const bool own = row >= 0 && (row & (SORTERS - 1)) == warp;
+      const unsigned owners = __ballot_sync(0xffffffffu, own);
+      if (owners == 0) continue;
+      const int one = __shfl_sync(0xffffffffu, row, __ffs(int(owners)) - 1);
+      const bool alike = __all_sync(0xffffffffu, !own || row == one);   // (a token that stands everywhere)
+      int at = 0;
+      unsigned peers = owners;
+      if (own) {
+        if (!alike) peers = __match_any_sync(owners, row);
+        at = ends[row] + __popc(peers & ((1u << lane) - 1u));
+        w.row[offset + at] = row * w.deals + deal;
+        w.place[offset + at] = place;
+      }
+      __syncwarp();
+      if (own && (peers >> lane) == 1u) ends[row] = at + 1;   // (the last of them)
+      __syncwarp();
     }
-    const bool own = row >= 0 && (row & (WARPS - 1)) == warp;
-    const unsigned owners = __ballot_sync(0xffffffffu, own);
-    if (owners == 0) continue;
-    int at = 0;
-    unsigned peers = 0;
-    if (own) {
-      peers = __match_any_sync(owners, row);
-      at = ends[row] + __popc(peers & ((1u << lane) - 1u));
-      sorted_row[at] = uint16_t(row);
-      sorted_place[at] = place;
-    }
-    __syncwarp();
-    if (own && (peers >> lane) == 1u) ends[row] = at + 1;   // (the last of them)
-    __syncwarp();
+  };
+  if (apart == 0) {
+    place_all(list_row, list_place, total);
+  } else {
+    for (int part = 0; part < DEAL_WARPS; ++part) place_all(list_row + part * LISTED, list_place + part * LISTED, mine[part]);
   }
-  __syncthreads();
+}
 
-  // ---- sums: an even share of the sorted places a warp, in order. A lane holds one of 32 places and rows, of this window and of the next.
-  constexpr int AHEAD = WIDE && sizeof(T) == 2 ? 16 : 8;   // rows from above on their way to a warp (what registers hold)
-  float (*heads)[SLICE] = reinterpret_cast<float (*)[SLICE]>(shared);   // (the counts and the list, which are done with)
-  float (*tails)[SLICE] = heads + WARPS;
-  const int part = max(((total + WARPS - 1) / WARPS + 7) / 8 * 8, 8);
-  const int from = min(total, warp * part), to = min(total, from + part);
-  const int before_row = from > 0 && from < to ? sorted_row[from - 1] : -1, after_row = to < total && from < to ? sorted_row[to] : -1;
+template <typename T, typename O, bool WIDE>
+__global__ void __launch_bounds__(THREADS) sum_kernel(const Work w) {
+  __shared__ float heads[WARPS][SLICE], tails[WARPS][SLICE];   // of a window: the sum of the row that an earlier one began; of the row that the next goes on with
+  __shared__ int head_row[WARPS], tail_row[WARPS];             // -1: none
+  __shared__ int last_of_chain;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, held = *w.held;
+  const int group = blockIdx.x / w.slices, slice = blockIdx.x % w.slices, span = WARPS * w.window;
+  const int col = slice * w.slice, width = min(w.slice, w.width - col);
+  const int group_from = group * span;
+  if (group_from >= held) return;
+  const T* above = static_cast<const T*>(w.above) + col;
+  O* out = static_cast<O*>(w.out) + col;
+
+  // ---- a warp's window
+  const int from = group_from + warp * w.window, n = min(w.window, held - from);
   int head = -1, tail = -1;
-  auto at_place = [&](int i) { return i < to ? sorted_place[i] : -1; };
-  auto at_row = [&](int i) { return i < to ? int(sorted_row[i]) : after_row; };
-  int place[2] = {at_place(from + lane), at_place(from + 32 + lane)}, number[2] = {at_row(from + lane), at_row(from + 32 + lane)};
-  __syncthreads();   // (behind it the sums of warps take the place of the counts and of the list; the sorted places stay)
-  if (from < to) {
-    Raw<T, WIDE> raw[AHEAD];
+  if (n > 0) {
+    const int place = lane < n ? w.place[from + lane] : 0, number = lane < n ? w.row[from + lane] : -1;
+    const int before = from > 0 ? w.row[from - 1] : -1, after = from + n < held ? w.row[from + n] : -1;
+    constexpr int BATCH = WIDE && sizeof(T) == 2 ? 8 : 4;   // rows asked for together; two batches are on their way
+    Raw<T, WIDE> raw[2][BATCH];
+    auto load = [&](Raw<T, WIDE> (&r)[BATCH], int i0) {
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const int t = __shfl_sync(0xffffffffu, place[0], j);
-      if (t >= 0) raw[j].load(above + t * w.ld, width, lane);
-    }
-    int row = __shfl_sync(0xffffffffu, number[0], 0);
-    bool began_here = before_row != row;
-    for (int i0 = from; i0 < to; i0 += 32) {
-      const int place2 = at_place(i0 + 64 + lane), number2 = at_row(i0 + 64 + lane);
-#pragma unroll 1
-      for (int g = 0; g < 32; g += AHEAD) {
+      for (int j = 0; j < BATCH; ++j) {
+        const int t = __shfl_sync(0xffffffffu, place, (i0 + j) & 31);
+        if (i0 + j < n) r[j].load(above + t * w.ld, width, lane);
+      }
+    };
+    Lane<T, WIDE> sum;
+    sum.clear();
+    int row = __shfl_sync(0xffffffffu, number, 0);
+    bool began_here = before != row;
+    auto keep = [&](float* to) {
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-          const int i = g + j;   // of the window
-          if (i0 + i >= to) break;
-          raw[j].add_to(sum);
-          const int t = __shfl_sync(0xffffffffu, i + AHEAD < 32 ? place[0] : place[1], (i + AHEAD) & 31);
-          if (t >= 0) raw[j].load(above + t * w.ld, width, lane);
-          const int next = __shfl_sync(0xffffffffu, i + 1 < 32 ? number[0] : number[1], (i + 1) & 31);
+      for (int k = 0; k < SLICE / 32; ++k) to[Lane<T, WIDE>::column(k / Lane<T, WIDE>::PIECE, lane) + k % Lane<T, WIDE>::PIECE] = sum.v[k];
+    };
+    auto take = [&](const Raw<T, WIDE> (&r)[BATCH], int i0) {
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const int i = i0 + j;
+        if (i < n) {
+          r[j].add_to(sum);
+          const int other = __shfl_sync(0xffffffffu, number, (i + 1) & 31), next = i + 1 < n ? other : after;
           if (next != row) {
             if (began_here) {
-              put_row<T, O, WIDE>(out + (static_cast<long long>(row) * w.deals + deal) * w.ld_o, sum, width, w.scale, w.add != 0, lane);
+              put_row<T, O, WIDE>(out + row * w.ld_o, sum, width, w.scale, w.add != 0, lane);
             } else {
               head = row;
-#pragma unroll
-              for (int k = 0; k < SLICE / 32; ++k) heads[warp][k * 32 + lane] = sum.v[k];
+              keep(heads[warp]);
             }
             began_here = true;
             sum.clear();
             row = next;
-          } else if (i0 + i + 1 == to) {   // the next share goes on with it (it may have gone through this one whole)
+          } else if (i + 1 == n) {   // the next window goes on with it (it may have gone through this one whole)
             tail = row;
-#pragma unroll
-            for (int k = 0; k < SLICE / 32; ++k) tails[warp][k * 32 + lane] = sum.v[k];
+            keep(tails[warp]);
           }
         }
       }
-      place[0] = place[1];
-      number[0] = number[1];
-      place[1] = place2;
-      number[1] = number2;
+    };
+    load(raw[0], 0);
+#pragma unroll 1
+    for (int i = 0; i < n; i += 2 * BATCH) {
+      load(raw[1], i + BATCH);
+      take(raw[0], i);
+      load(raw[0], i + 2 * BATCH);
+      take(raw[1], i + BATCH);
     }
   }
   if (lane == 0) {
@@ -311,20 +358,77 @@ __global__ void __launch_bounds__(THREADS, 2) gradient_kernel(const Work w) {
     tail_row[warp] = tail;
   }
   __syncthreads();
-  if (warp == 0) {
-    sum.clear();
-    for (int i = 0; i < WARPS; ++i) {
-      if (head_row[i] >= 0) {   // the end of the row that is open
-#pragma unroll
-        for (int k = 0; k < SLICE / 32; ++k) sum.v[k] += heads[i][k * 32 + lane];
-        put_row<T, O, WIDE>(out + (static_cast<long long>(head_row[i]) * w.deals + deal) * w.ld_o, sum, width, w.scale, w.add != 0, lane);
-        sum.clear();
+
+  // ---- rows of several windows, a thread a column
+  const int c = threadIdx.x;
+  bool began_before = group_from > 0 && w.row[group_from - 1] == w.row[group_from];   // (the first row; it ends in a head, or goes on as a tail)
+  float* shares = w.shares + static_cast<long long>(group) * 2 * w.width_up + col;
+  auto put = [&](int row, float sum) {
+    O* to = out + row * w.ld_o + c;
+    *to = from_float<O>(sum * w.scale + (w.add ? to_float(*to) : 0.f));
+  };
+  int ended = -1, open = -1;   // rows of other CTAs, too: the one that ends here, the one that goes on
+  float sum = 0.f;
+  for (int i = 0; i < WARPS; ++i) {
+    if (head_row[i] >= 0) {
+      if (c < width) {
+        sum += heads[i][c];
+        if (began_before) shares[c] = sum;
+        else put(head_row[i], sum);
       }
-      if (tail_row[i] >= 0) {
-#pragma unroll
-        for (int k = 0; k < SLICE / 32; ++k) sum.v[k] += tails[i][k * 32 + lane];
-      }
+      if (began_before) ended = head_row[i];
+      began_before = false;
+      sum = 0.f;
     }
+    open = tail_row[i];
+    if (open >= 0 && c < width) sum += tails[i][c];
+  }
+  if (open >= 0 && c < width) shares[w.width_up + c] = sum;
+
+  // ---- rows of several CTAs: whoever comes last adds their shares
+  auto chain = [&](int row, int first, int last) {   // CTAs first .. last of places hold it
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      last_of_chain = atomicAdd(w.arrived + static_cast<long long>(first) * w.slices + slice, 1) == last - first;
+      __threadfence();
+    }
+    __syncthreads();
+    if (last_of_chain && c < width) {
+      const float* from_here = w.shares + static_cast<long long>(first) * 2 * w.width_up + col + c;
+      float all = 0.f;
+#pragma unroll 8
+      for (int i = 0; i < last - first; ++i) all += __ldcg(from_here + (2ll * i + 1) * w.width_up);
+      all += __ldcg(from_here + 2ll * (last - first) * w.width_up);
+      put(row, all);
+    }
+    __syncthreads();
+  };
+  auto first_of = [&](int row) {   // of the CTAs of a row that began before this one, 32 at a look
+    int g = group - 1;
+    while (true) {
+      const int at = g - lane;
+      const bool through = at > 0 && w.row[at > 0 ? at * span : 0] == row && w.row[at > 0 ? at * span - 1 : 0] == row;
+      const unsigned stops = ~__ballot_sync(0xffffffffu, through);
+      if (stops != 0) return g - (__ffs(int(stops)) - 1);
+      g -= 32;
+    }
+  };
+  const bool open_before = began_before;   // (nothing has ended since the CTA's first place)
+  if (ended >= 0) chain(ended, first_of(ended), group);
+  if (open >= 0) {
+    const int first = open_before ? first_of(open) : group;
+    int g = group + 1;
+    while (true) {
+      const long long next = (g + 1ll + lane) * span;
+      const unsigned stops = ~__ballot_sync(0xffffffffu, next < held && w.row[next < held ? next : 0] == open);
+      if (stops != 0) {
+        g += __ffs(int(stops)) - 1;
+        break;
+      }
+      g += 32;
+    }
+    chain(open, first, g);
   }
 }
 
@@ -363,36 +467,40 @@ int n_sms() {
   return n;
 }
 
-struct Deal {
-  int slices, slice, deals;
-  unsigned long long inverse;
-};
-
-// Slices of the columns, and as many deals of the rows as give every SM two CTAs; no CTA more rows than its shared memory counts. The quotient
-// v / deals is v * inverse >> 64 with the inverse of 2^64 rounded up (two deals at least, so that it is below 2^64): exact, since the excess
-// of v * inverse is below v * deals < 2^64 parts of 1 / deals.
-Deal deal_of(int width, int vocab) {
-  Deal d;
-  d.slices = (width + SLICE - 1) / SLICE;
-  d.slice = ((width + d.slices - 1) / d.slices + 7) / 8 * 8;
-  d.slices = (width + d.slice - 1) / d.slice;
-  int deals = 2 * n_sms() / d.slices;
+// As many deals as SMs, of no more rows than a CTA counts. The quotient v / deals is v * inverse >> 64 with the inverse of 2^64 rounded up (two deals at least, so
+// that it is below 2^64): exact, since the excess of v * inverse is below v * deals < 2^64 parts of 1 / deals.
+int deals_of(int vocab) {
+  int deals = n_sms();
   if (deals > vocab) deals = vocab;
   if (deals < (vocab - 1) / MOST_ROWS + 1) deals = (vocab - 1) / MOST_ROWS + 1;
-  d.deals = deals < 2 ? 2 : deals;
-  d.inverse = ~0ull / unsigned(d.deals) + 1;
-  return d;
+  return deals < 2 ? 2 : deals;
+}
+
+template <typename O> int launch_deal(const Work& w, cudaStream_t stream) {
+  auto kernel = deal_kernel<O>;
+  static std::atomic<bool> done[64];
+  const int status = allow_smem(kernel, MOST_ROWS * 4 + MOST_ROWS / 8 + 8 + LISTED_BYTES, done);
+  if (status != R2_OK) return status;
+  const size_t rows = size_t((w.vocab - 1) / w.deals + 1);
+  r2_launch(kernel, dim3(w.deals), dim3(DEAL_THREADS), rows * 4 + (rows + 31) / 32 * 4 + LISTED_BYTES, stream, w);
+  return launch_status();
 }
 
 template <typename T, typename O, bool WIDE>
-int launch_gradient(const Work& w, const Deal& d, cudaStream_t stream) {
-  auto kernel = gradient_kernel<T, O, WIDE>;
-  static std::atomic<bool> done[64];
-  const int status = allow_smem(kernel, MOST_ROWS * 4 + LISTED_BYTES, done);
-  if (status != R2_OK) return status;
-  const int rows = (w.vocab - 1) / d.deals + 1;
-  kernel<<<unsigned(d.slices) * d.deals, THREADS, size_t(rows) * 4 + LISTED_BYTES, stream>>>(w);
+int launch_sums(const Work& w, cudaStream_t stream) {
+  r2_launch(sum_kernel<T, O, WIDE>, dim3(unsigned(w.groups) * unsigned(w.slices)), dim3(THREADS), size_t(0), stream, w);
   return launch_status();
+}
+
+// Slices of the columns; windows of 32 places, or of fewer where that would leave SMs without a CTA.
+void share_out(Work& w) {
+  w.slices = (w.width + SLICE - 1) / SLICE;
+  w.slice = ((w.width + w.slices - 1) / w.slices + 7) / 8 * 8;
+  w.slices = (w.width + w.slice - 1) / w.slice;
+  w.window = 32;
+  while (w.window > 8 && static_cast<long long>(w.tokens) * w.slices < 2ll * n_sms() * WARPS * w.window) w.window /= 2;
+  w.groups = (w.tokens + WARPS * w.window - 1) / (WARPS * w.window);
+  w.width_up = (w.width + 7) / 8 * 8;
 }
 
 bool at_16(const void* p, long long ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
@@ -419,22 +527,41 @@ extern "C" int r2_token_rows(int dtype, int out_dtype, const int32_t* ids, const
   return launch_status();
 }
 
-// Bytes of scratch for a gradient.
-extern "C" long long r2_token_rows_space(int tokens, int width, int vocab) { return static_cast<long long>(deal_of(width, vocab).slices) * 3 * tokens * 4; }
+// Bytes of scratch for a gradient: four lists of the places, their number, what CTAs of places leave of rows that lie in several.
+extern "C" long long r2_token_rows_space(int tokens, int width, int vocab) {
+  Work w = {};
+  w.tokens = tokens;
+  w.width = width;
+  share_out(w);
+  return 16ll * tokens + 16 + static_cast<long long>(w.groups) * (2ll * w.width_up + w.slices) * 4;
+}
 
 extern "C" int r2_token_rows_gradient(int dtype, int out_dtype, const int32_t* ids, const void* above, long long ld, void* out, long long ld_o, int tokens, int width,
                                       int vocab, float scale, int add, void* space, cudaStream_t stream) {
   if (tokens < 1 || width < 1 || vocab < 1) return R2_BAD_SHAPE;
   if (tokens > MOST || width > MOST) return R2_UNSUPPORTED;
   const int size = dtype == R2_F32 ? 4 : 2, out_size = out_dtype == R2_F32 ? 4 : 2;
-  const Deal d = deal_of(width, vocab);
-  const Work w = {ids, above, ld, out, ld_o, tokens, width, vocab, scale, add, d.deals, d.slice, d.inverse, static_cast<int32_t*>(space)};
-  const bool wide = at_16(above, ld, size) && at_16(out, ld_o, out_size) && width * size % 16 == 0;
-#define R2_CASE(T, O) (wide ? launch_gradient<T, O, true>(w, d, stream) : launch_gradient<T, O, false>(w, d, stream))
+  const bool wide = at_16(above, ld, size) && at_16(out, ld_o, out_size) && width * size % 16 == 0 && width * out_size % 16 == 0;
+  Work w = {ids, above, ld, out, ld_o, tokens, width, vocab, scale, add};
+  w.deals = deals_of(vocab);
+  w.inverse = ~0ull / unsigned(w.deals) + 1;
+  share_out(w);
+  if (static_cast<long long>(w.groups) * w.slices >= 1ll << 31) return R2_UNSUPPORTED;
+  w.row = static_cast<int32_t*>(space);
+  w.place = w.row + tokens;
+  w.list_row = w.place + tokens;
+  w.list_place = w.list_row + tokens;
+  w.held = w.list_place + tokens;
+  w.shares = reinterpret_cast<float*>(w.held + 4);
+  w.arrived = reinterpret_cast<int*>(w.shares + static_cast<long long>(w.groups) * 2 * w.width_up);
+  w.wide = wide;
+  int status = out_dtype == R2_F32 ? launch_deal<float>(w, stream) : out_dtype == R2_BF16 ? launch_deal<bf16>(w, stream) : R2_BAD_DTYPE;
+  if (status != R2_OK) return status;
+#define R2_CASE(T, O) (wide ? launch_sums<T, O, true>(w, stream) : launch_sums<T, O, false>(w, stream))
   if (dtype == R2_F32 && out_dtype == R2_F32) return R2_CASE(float, float);
-  if (dtype == R2_F32 && out_dtype == R2_BF16) return R2_CASE(float, bf16);
+  if (dtype == R2_F32) return R2_CASE(float, bf16);
   if (dtype == R2_BF16 && out_dtype == R2_F32) return R2_CASE(bf16, float);
-  if (dtype == R2_BF16 && out_dtype == R2_BF16) return R2_CASE(bf16, bf16);
+  if (dtype == R2_BF16) return R2_CASE(bf16, bf16);
 #undef R2_CASE
   return R2_BAD_DTYPE;
 }
