@@ -4,10 +4,11 @@
 //
 // The gradient in two launches:
 //
-//   deal_kernel  sorts the places by token, stable, and writes zeros to the rows without one. The table's rows are dealt out to CTAs by the remainder of their
-//                number (tokens that stand often lie side by side in a vocabulary). A CTA goes through all tokens, counts its own and those of lower deals (so that
-//                it knows where in the sorted list its part begins, without a word between CTAs), lists its places in their order and places them by
-//                row; half of its warps write zeros meanwhile, which is most of what a small batch costs.
+//   deal_kernel  sorts the places by token, stable. The table's rows are dealt out to CTAs by the remainder of their number (tokens that stand often lie side
+//                by side in a vocabulary). A CTA goes through all tokens, a share a warp, and lists its own with their rank among the share's of their row, beside a
+//                count of those of lower deals, so that it knows where in the sorted list its part begins without a word between CTAs. Running sums of the shares' and rows'
+//                counts then say where each place goes. Meanwhile zeros go to the whole table in bulk copies from shared memory, without a look at which rows
+//                need them: that is most of what a small batch costs, and hides the sorting; the rows that are written twice are fewer than the places.
 //   sum_kernel   a CTA takes the sorted places of eight windows, a warp each, and up to 256 columns: a token that stands everywhere and tokens that stand once
 //                take the same time. A row whose places lie in several windows is joined in shared memory; one that goes on in other CTAs leaves float sums in
 //                memory, and the last of those CTAs adds them, in the order of the places whoever that is.
@@ -19,10 +20,11 @@ namespace {
 
 constexpr int THREADS = 256, WARPS = 8;
 constexpr int SLICE = 256;             // columns of a warp at most
-constexpr int DEAL_THREADS = 1024, DEAL_WARPS = 32, SORTERS = 16;   // of a dealing CTA: those that sort; the others write zeros
-constexpr int LISTED = 256;            // places that shared memory holds of what a dealing warp lists (if one has more: the scratch)
-constexpr int MOST_ROWS = 16384;       // of a deal
+constexpr int DEAL_THREADS = 1024, DEAL_WARPS = 32;
+constexpr int LISTED = 128;            // places that shared memory holds of what a dealing warp lists (where one has more, all go through the tokens again)
+constexpr int MOST_ROWS = 1200;        // of a deal
 constexpr int LISTED_BYTES = DEAL_WARPS * LISTED * 8;
+constexpr int ZEROS = 16384;           // bytes of a bulk copy
 
 struct Work {
   const int32_t* ids;
@@ -36,12 +38,12 @@ struct Work {
   int deals;                        // rows v with v mod deals = the CTA's
   unsigned long long inverse;       // v / deals = v * inverse >> 64
   int32_t *row, *place;             // [tokens]: the sorted list: by deal, row and place
-  int32_t *list_row, *list_place;   // [tokens]: a deal's list before it is sorted, where shared memory does not hold it
   int* held;                        // how many places hold a token
+  long long bytes;                  // of the table
   int slices, slice, window;        // of the columns, columns of one, sorted places of a warp
   int* arrived;                     // [CTA of places][slice]: CTAs that have left their share of the row that goes on from this one
   float* shares;                    // [CTA of places][2][width_up]: sums of a row that an earlier CTA began; of one that the next goes on with
-  int width_up, groups, wide;       // (groups: CTAs of places)
+  int width_up, groups;             // (groups: CTAs of places)
 };
 
 // A lane's columns of a slice: pieces of 16 bytes, or every 32nd number.
@@ -95,9 +97,16 @@ __device__ __forceinline__ void put_row(O* row, const Lane<T, WIDE>& sum, int wi
   for (int p = 0; p < L::PIECES; ++p) {
     const int c = L::column(p, lane);
     if (c >= width) continue;
+    float old[L::PIECE];
+#pragma unroll
+    for (int j = 0; j < L::PIECE; ++j) old[j] = 0.f;
+    if (add) {
+#pragma unroll
+      for (int j = 0; j < L::PIECE; ++j) old[j] = to_float(row[c + j]);
+    }
     alignas(16) O out[L::PIECE];
 #pragma unroll
-    for (int j = 0; j < L::PIECE; ++j) out[j] = from_float<O>(sum.v[p * L::PIECE + j] * scale + (add ? to_float(row[c + j]) : 0.f));
+    for (int j = 0; j < L::PIECE; ++j) out[j] = from_float<O>(fmaf(sum.v[p * L::PIECE + j], scale, old[j]));
     if constexpr (WIDE) {
       if constexpr (sizeof(out) == 32) {
         reinterpret_cast<uint4*>(row + c)[0] = reinterpret_cast<const uint4*>(out)[0];
@@ -113,58 +122,79 @@ __device__ __forceinline__ void put_row(O* row, const Lane<T, WIDE>& sum, int wi
   }
 }
 
-template <typename O>
+__device__ __forceinline__ int quotient_of(unsigned long long v, unsigned long long inverse) {
+  return int((v * unsigned(inverse >> 32) + (v * unsigned(inverse) >> 32)) >> 32);
+}
+
 __global__ void __launch_bounds__(DEAL_THREADS, 1) deal_kernel(const Work w) {
   extern __shared__ int32_t shared[];
-  __shared__ int mine[DEAL_WARPS], lower[DEAL_WARPS], running[SORTERS];
+  __shared__ int mine[DEAL_WARPS], lower[DEAL_WARPS], running[DEAL_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, deal = blockIdx.x;
   const int rows = int((static_cast<long long>(w.vocab) - deal + w.deals - 1) / w.deals);
-  int32_t* ends = shared;                                              // [rows]: counts, then where a row's places begin in this deal's part, then where they end
-  uint32_t* empty = reinterpret_cast<uint32_t*>(shared + rows);        // a bit a row: no place (the counts change)
-  int32_t* list_row = reinterpret_cast<int32_t*>(empty + (rows + 31) / 32);   // [warp][LISTED]
-  int32_t* list_place = list_row + DEAL_WARPS * LISTED;
-  const unsigned inverse_high = unsigned(w.inverse >> 32), inverse_low = unsigned(w.inverse);
-  auto quotient = [&](int id) {
-    const unsigned long long v = unsigned(id);
-    return int((v * inverse_high + (v * inverse_low >> 32)) >> 32);
-  };
-  for (int j = threadIdx.x; j < rows; j += DEAL_THREADS) ends[j] = 0;
+  int32_t* counts = shared;                          // [warp][rows]: a row's places in the warp's share, then where the first of them goes
+  int32_t* list_place = counts + DEAL_WARPS * rows;  // [warp][LISTED]
+  uint32_t* list_row = reinterpret_cast<uint32_t*>(list_place + DEAL_WARPS * LISTED);   // row * LISTED + rank
+  __shared__ alignas(16) uint4 zeros[ZEROS / 16];
+  for (int j = threadIdx.x; j < DEAL_WARPS * rows; j += DEAL_THREADS) counts[j] = 0;
+  if (!w.add) {
+    for (int j = threadIdx.x; j < ZEROS / 16; j += DEAL_THREADS) zeros[j] = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
   __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
   for (long long i = deal * DEAL_THREADS + threadIdx.x; i < static_cast<long long>(w.groups) * w.slices; i += w.deals * DEAL_THREADS) w.arrived[i] = 0;
 
-  // ---- a warp's share of the places: lists this CTA's (as far as there is room), counts those of lower deals
-  const int share = ((w.tokens + DEAL_WARPS - 1) / DEAL_WARPS + 255) / 256 * 256;
-  auto begin_of = [&](int i) { return int(min(static_cast<long long>(i) * share, static_cast<long long>(w.tokens))); };
-  auto walk = [&](int part, auto&& each) {   // each(row, place, own, owners before it in this part)
-    const int last = begin_of(part + 1);
-    int before = 0;
-    for (int t0 = begin_of(part); t0 < last; t0 += 256) {
-      int id[8];
+  // ---- zeros: the CTAs' pieces side by side, so that all of them write in one part of the table; a lane of the last warp a piece
+  const bool zeroing = !w.add && warp == DEAL_WARPS - 1;
+  if (zeroing) {
+    char* out = static_cast<char*>(w.out);
+    const long long whole = w.bytes / 16 * 16;
+    for (long long at = (deal + static_cast<long long>(lane) * w.deals) * ZEROS; at < whole; at += 32ll * w.deals * ZEROS) {
+      const unsigned n = unsigned(whole - at < ZEROS ? whole - at : ZEROS);
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(out + at), "r"(uint32_t(__cvta_generic_to_shared(zeros))), "r"(n) : "memory");
+    }
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    if (deal == 0 && whole + lane < w.bytes) out[whole + lane] = 0;
+  }
+
+  // ---- a warp's share of the places, in order: each(row, place, rank behind what counts says at the start, how many of the share came before)
+  constexpr int LOADS = 16;
+  const int share = ((w.tokens + DEAL_WARPS - 1) / DEAL_WARPS + 31) / 32 * 32;
+  const int first = int(min(static_cast<long long>(warp) * share, static_cast<long long>(w.tokens))), last = int(min(static_cast<long long>(first) + share, static_cast<long long>(w.tokens)));
+  int32_t* own_counts = counts + warp * rows;
+  int n_mine = 0, n_lower = 0;
+  auto walk = [&](auto&& each) {
+    n_mine = n_lower = 0;
+    for (int t0 = first; t0 < last; t0 += 32 * LOADS) {
+      int id[LOADS];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) id[j] = t0 + 32 * j + lane < last ? w.ids[t0 + 32 * j + lane] : -1;
+      for (int j = 0; j < LOADS; ++j) id[j] = t0 + 32 * j + lane < last ? w.ids[t0 + 32 * j + lane] : -1;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < LOADS; ++j) {
         const bool token = id[j] >= 0 && id[j] < w.vocab;
-        const int row = quotient(token ? id[j] : 0), at = id[j] - row * w.deals;
-        const unsigned mask = __ballot_sync(0xffffffffu, token && at == deal);
-        each(row, t0 + 32 * j + lane, token && at == deal, before + __popc(mask & ((1u << lane) - 1u)), token && at < deal);
-        before += __popc(mask);
+        const int row = quotient_of(unsigned(token ? id[j] : 0), w.inverse), at = id[j] - row * w.deals;
+        n_lower += token && at < deal ? 1 : 0;
+        const bool own = token && at == deal;
+        const unsigned owners = __ballot_sync(0xffffffffu, own);
+        if (owners == 0) continue;
+        if (own) {
+          const unsigned peers = __match_any_sync(owners, row), before = (1u << lane) - 1u;
+          const int count = own_counts[row];
+          __syncwarp(owners);
+          if ((peers >> lane) == 1u) own_counts[row] = count + __popc(peers);   // (the last of them)
+          each(row, t0 + 32 * j + lane, count + __popc(peers & before), n_mine + __popc(owners & before));
+        }
+        __syncwarp();
+        n_mine += __popc(owners);
       }
     }
-    return before;
   };
-  int n_lower = 0;
-  const int n_mine = walk(warp, [&](int row, int place, bool own, int at, bool below) {
-    if (own) {
-      atomicAdd(&ends[row], 1);
-      if (at < LISTED) {
-        list_row[warp * LISTED + at] = row;
-        list_place[warp * LISTED + at] = place;
-      }
+  walk([&](int row, int place, int rank, int at) {
+    if (at < LISTED) {
+      list_row[warp * LISTED + at] = unsigned(row) * LISTED + unsigned(rank);
+      list_place[warp * LISTED + at] = place;
     }
-    n_lower += below ? 1 : 0;
   });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n_lower += __shfl_xor_sync(0xffffffffu, n_lower, o);
@@ -182,114 +212,68 @@ __global__ void __launch_bounds__(DEAL_THREADS, 1) deal_kernel(const Work w) {
   }
   if (deal == w.deals - 1 && threadIdx.x == 0) *w.held = offset + total;
 
-  // ---- rows without a place
-  for (int j0 = warp * 32; j0 < rows; j0 += DEAL_THREADS) {
-    const unsigned none = __ballot_sync(0xffffffffu, j0 + lane < rows && ends[j0 + lane] == 0);
-    if (lane == 0) empty[j0 / 32] = none;
+  // ---- running sums: of a row over the shares, of the rows (up to two a thread, side by side) over the threads
+  constexpr int PER = (MOST_ROWS + DEAL_THREADS - 1) / DEAL_THREADS;
+  int of_row[PER], own = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int j = int(threadIdx.x) * PER + i;
+    of_row[i] = 0;
+    if (j < rows) {
+      for (int part = 0; part < DEAL_WARPS; ++part) of_row[i] += counts[part * rows + j];
+    }
+    own += of_row[i];
   }
+  int up = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, up, o);
+    up += lane >= o ? x : 0;
+  }
+  if (lane == 31) running[warp] = up;
   __syncthreads();
-  if (warp >= SORTERS || total == 0) {
-    if (!w.add) {
-      const int n = total == 0 ? DEAL_WARPS : DEAL_WARPS - SORTERS, first = total == 0 ? warp : warp - SORTERS;
-      for (int j = first; j < rows; j += n) {
-        if (!(empty[j >> 5] >> (j & 31) & 1u)) continue;
-        O* to = static_cast<O*>(w.out) + (static_cast<long long>(j) * w.deals + deal) * w.ld_o;
-        if (w.wide) {
-          for (int c = lane * int(16 / sizeof(O)); c < w.width; c += 32 * int(16 / sizeof(O))) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
-        } else {
-          for (int c = lane; c < w.width; c += 32) to[c] = from_float<O>(0.f);
-        }
-      }
-    }
-    return;
-  }
-  auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(SORTERS * 32) : "memory"); };
-
-  // ---- a list that shared memory does not hold: listed again, as one
-  int apart = LISTED;
-  if (most > LISTED) {
-    list_row = w.list_row + offset;
-    list_place = w.list_place + offset;
-    apart = 0;
-    for (int part = warp; part < DEAL_WARPS; part += SORTERS) {
-      int before = lane < part ? mine[lane] : 0;
+  int begin = lane < warp ? running[lane] : 0;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-      walk(part, [&](int row, int place, bool own, int at, bool) {
-        if (own) {
-          list_row[before + at] = row;
-          list_place[before + at] = place;
-        }
-      });
-    }
-  }
-  // where each row's places begin: a thread's share of the rows, then the threads'
-  {
-    constexpr int N = SORTERS * 32;
-    const int per = (rows + N - 1) / N, from = min(rows, int(threadIdx.x) * per), to = min(rows, from + per);
-    int own = 0;
-    for (int j = from; j < to; ++j) own += ends[j];
-    int up = own;
+  for (int o = 16; o > 0; o >>= 1) begin += __shfl_xor_sync(0xffffffffu, begin, o);
+  begin += offset + up - own;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, up, o);
-      up += lane >= o ? x : 0;
-    }
-    if (lane == 31) running[warp] = up;
-    sync();
-    int begin = (lane < warp ? running[lane] : 0);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) begin += __shfl_xor_sync(0xffffffffu, begin, o);
-    begin += up - own;
-    for (int j = from; j < to; ++j) {
-      const int n = ends[j];
-      ends[j] = begin;
+  for (int i = 0; i < PER; ++i) {
+    const int j = int(threadIdx.x) * PER + i;
+    if (j >= rows) continue;
+    for (int part = 0; part < DEAL_WARPS; ++part) {
+      const int n = counts[part * rows + j];
+      counts[part * rows + j] = begin;
       begin += n;
     }
-    sync();
   }
-  // a stable placing: a warp takes the rows of its number mod 16 from the list, in the list's order
-  auto place_all = [&](const int32_t* from_row, const int32_t* from_place, int n) {
-    int next_row = lane < n ? from_row[lane] : -1, next_place = lane < n ? from_place[lane] : 0;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const int row = next_row, place = next_place;
-      if (i0 + 32 < n) {   // (asked for ahead: the list may lie in memory)
-        next_row = i0 + 32 + lane < n ? from_row[i0 + 32 + lane] : -1;
-        next_place = i0 + 32 + lane < n ? from_place[i0 + 32 + lane] : 0;
-      }
-      const bool own = row >= 0 && (row & (SORTERS - 1)) == warp;
-      const unsigned owners = __ballot_sync(0xffffffffu, own);
-      if (owners == 0) continue;
-      const int one = __shfl_sync(0xffffffffu, row, __ffs(int(owners)) - 1);
-      const bool alike = __all_sync(0xffffffffu, !own || row == one);   // (a token that stands everywhere)
-      int at = 0;
-      unsigned peers = owners;
-      if (own) {
-        if (!alike) peers = __match_any_sync(owners, row);
-        at = ends[row] + __popc(peers & ((1u << lane) - 1u));
-        w.row[offset + at] = row * w.deals + deal;
-        w.place[offset + at] = place;
-      }
-      __syncwarp();
-      if (own && (peers >> lane) == 1u) ends[row] = at + 1;   // (the last of them)
-      __syncwarp();
+  __syncthreads();
+
+  // ---- where each place goes
+  if (most <= LISTED) {
+    for (int i = lane; i < n_mine; i += 32) {
+      const unsigned entry = list_row[warp * LISTED + i];
+      const int row = int(entry / LISTED), at = own_counts[row] + int(entry % LISTED);
+      w.row[at] = row * w.deals + deal;
+      w.place[at] = list_place[warp * LISTED + i];
     }
-  };
-  if (apart == 0) {
-    place_all(list_row, list_place, total);
   } else {
-    for (int part = 0; part < DEAL_WARPS; ++part) place_all(list_row + part * LISTED, list_place + part * LISTED, mine[part]);
+    walk([&](int row, int place, int at, int) {
+      w.row[at] = row * w.deals + deal;
+      w.place[at] = place;
+    });
   }
+  if (zeroing) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 template <typename T, typename O, bool WIDE>
-__global__ void __launch_bounds__(THREADS) sum_kernel(const Work w) {
+__global__ void __launch_bounds__(THREADS, 2) sum_kernel(const Work w) {
   __shared__ float heads[WARPS][SLICE], tails[WARPS][SLICE];   // of a window: the sum of the row that an earlier one began; of the row that the next goes on with
   __shared__ int head_row[WARPS], tail_row[WARPS];             // -1: none
   __shared__ int last_of_chain;
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, held = *w.held;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int held = *w.held;
   const int group = blockIdx.x / w.slices, slice = blockIdx.x % w.slices, span = WARPS * w.window;
   const int col = slice * w.slice, width = min(w.slice, w.width - col);
   const int group_from = group * span;
@@ -303,7 +287,7 @@ __global__ void __launch_bounds__(THREADS) sum_kernel(const Work w) {
   if (n > 0) {
     const int place = lane < n ? w.place[from + lane] : 0, number = lane < n ? w.row[from + lane] : -1;
     const int before = from > 0 ? w.row[from - 1] : -1, after = from + n < held ? w.row[from + n] : -1;
-    constexpr int BATCH = WIDE && sizeof(T) == 2 ? 8 : 4;   // rows asked for together; two batches are on their way
+    constexpr int BATCH = WIDE && sizeof(T) == 2 ? 8 : 4;   // rows asked for together; two batches are on their way (what the registers hold)
     Raw<T, WIDE> raw[2][BATCH];
     auto load = [&](Raw<T, WIDE> (&r)[BATCH], int i0) {
 #pragma unroll
@@ -476,13 +460,11 @@ int deals_of(int vocab) {
   return deals < 2 ? 2 : deals;
 }
 
-template <typename O> int launch_deal(const Work& w, cudaStream_t stream) {
-  auto kernel = deal_kernel<O>;
+int launch_deal(const Work& w, cudaStream_t stream) {
   static std::atomic<bool> done[64];
-  const int status = allow_smem(kernel, MOST_ROWS * 4 + MOST_ROWS / 8 + 8 + LISTED_BYTES, done);
+  const int status = allow_smem(deal_kernel, DEAL_WARPS * MOST_ROWS * 4 + LISTED_BYTES, done);
   if (status != R2_OK) return status;
-  const size_t rows = size_t((w.vocab - 1) / w.deals + 1);
-  r2_launch(kernel, dim3(w.deals), dim3(DEAL_THREADS), rows * 4 + (rows + 31) / 32 * 4 + LISTED_BYTES, stream, w);
+  r2_launch(deal_kernel, dim3(w.deals), dim3(DEAL_THREADS), ((w.vocab - 1) / w.deals + 1) * size_t(DEAL_WARPS * 4) + LISTED_BYTES, stream, w);
   return launch_status();
 }
 
@@ -495,12 +477,14 @@ int launch_sums(const Work& w, cudaStream_t stream) {
 // Slices of the columns; windows of 32 places, or of fewer where that would leave SMs without a CTA.
 void share_out(Work& w) {
   w.slices = (w.width + SLICE - 1) / SLICE;
-  w.slice = ((w.width + w.slices - 1) / w.slices + 7) / 8 * 8;
+  w.slice = ((w.width + w.slices - 1) / w.slices + 63) / 64 * 64;   // (whole lines of 128 bytes)
   w.slices = (w.width + w.slice - 1) / w.slice;
   w.window = 32;
   while (w.window > 8 && static_cast<long long>(w.tokens) * w.slices < 2ll * n_sms() * WARPS * w.window) w.window /= 2;
   w.groups = (w.tokens + WARPS * w.window - 1) / (WARPS * w.window);
   w.width_up = (w.width + 7) / 8 * 8;
+  w.deals = deals_of(w.vocab);
+  w.inverse = ~0ull / unsigned(w.deals) + 1;
 }
 
 bool at_16(const void* p, long long ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
@@ -527,41 +511,39 @@ extern "C" int r2_token_rows(int dtype, int out_dtype, const int32_t* ids, const
   return launch_status();
 }
 
-// Bytes of scratch for a gradient: four lists of the places, their number, what CTAs of places leave of rows that lie in several.
+// Bytes of scratch for a gradient: two lists of the places, their number, what CTAs of places leave of rows that lie in several.
 extern "C" long long r2_token_rows_space(int tokens, int width, int vocab) {
   Work w = {};
   w.tokens = tokens;
   w.width = width;
+  w.vocab = vocab;
   share_out(w);
-  return 16ll * tokens + 16 + static_cast<long long>(w.groups) * (2ll * w.width_up + w.slices) * 4;
+  return 8ll * tokens + 16 + static_cast<long long>(w.groups) * (2ll * w.width_up + w.slices) * 4;
 }
 
 extern "C" int r2_token_rows_gradient(int dtype, int out_dtype, const int32_t* ids, const void* above, long long ld, void* out, long long ld_o, int tokens, int width,
                                       int vocab, float scale, int add, void* space, cudaStream_t stream) {
   if (tokens < 1 || width < 1 || vocab < 1) return R2_BAD_SHAPE;
   if (tokens > MOST || width > MOST) return R2_UNSUPPORTED;
+  if (!add && (ld_o != width || reinterpret_cast<uintptr_t>(out) % 16 != 0)) return R2_BAD_ALIGN;   // (a new table is one piece)
   const int size = dtype == R2_F32 ? 4 : 2, out_size = out_dtype == R2_F32 ? 4 : 2;
   const bool wide = at_16(above, ld, size) && at_16(out, ld_o, out_size) && width * size % 16 == 0 && width * out_size % 16 == 0;
   Work w = {ids, above, ld, out, ld_o, tokens, width, vocab, scale, add};
-  w.deals = deals_of(vocab);
-  w.inverse = ~0ull / unsigned(w.deals) + 1;
   share_out(w);
   if (static_cast<long long>(w.groups) * w.slices >= 1ll << 31) return R2_UNSUPPORTED;
   w.row = static_cast<int32_t*>(space);
   w.place = w.row + tokens;
-  w.list_row = w.place + tokens;
-  w.list_place = w.list_row + tokens;
-  w.held = w.list_place + tokens;
+  w.held = w.place + tokens;
   w.shares = reinterpret_cast<float*>(w.held + 4);
   w.arrived = reinterpret_cast<int*>(w.shares + static_cast<long long>(w.groups) * 2 * w.width_up);
-  w.wide = wide;
-  int status = out_dtype == R2_F32 ? launch_deal<float>(w, stream) : out_dtype == R2_BF16 ? launch_deal<bf16>(w, stream) : R2_BAD_DTYPE;
+  w.bytes = static_cast<long long>(vocab) * width * out_size;
+  if (dtype < R2_F32 || dtype > R2_BF16 || out_dtype < R2_F32 || out_dtype > R2_BF16) return R2_BAD_DTYPE;
+  const int status = launch_deal(w, stream);
   if (status != R2_OK) return status;
 #define R2_CASE(T, O) (wide ? launch_sums<T, O, true>(w, stream) : launch_sums<T, O, false>(w, stream))
   if (dtype == R2_F32 && out_dtype == R2_F32) return R2_CASE(float, float);
   if (dtype == R2_F32) return R2_CASE(float, bf16);
   if (dtype == R2_BF16 && out_dtype == R2_F32) return R2_CASE(bf16, float);
-  if (dtype == R2_BF16) return R2_CASE(bf16, bf16);
+  return R2_CASE(bf16, bf16);
 #undef R2_CASE
-  return R2_BAD_DTYPE;
 }
