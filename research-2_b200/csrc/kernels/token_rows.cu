@@ -20,7 +20,7 @@ namespace {
 
 constexpr int THREADS = 256, WARPS = 8;
 constexpr int SLICE = 256;             // columns of a warp at most
-constexpr int DEAL_THREADS = 1024, DEAL_WARPS = 32;
+constexpr int DEAL_WARPS = 31, DEAL_THREADS = DEAL_WARPS * 32;   // of a dealing CTA, beside a warp that writes zeros
 constexpr int LISTED = 128;            // places that shared memory holds of what a dealing warp lists (where one has more, all go through the tokens again)
 constexpr int MOST_ROWS = 1200;        // of a deal
 constexpr int LISTED_BYTES = DEAL_WARPS * LISTED * 8;
@@ -90,8 +90,8 @@ template <typename T, bool WIDE> struct Raw {
   }
 };
 
-template <typename T, typename O, bool WIDE>
-__device__ __forceinline__ void put_row(O* row, const Lane<T, WIDE>& sum, int width, float scale, bool add, int lane) {
+template <bool ADD, typename T, typename O, bool WIDE>
+__device__ __forceinline__ void put_row(O* row, const Lane<T, WIDE>& sum, int width, float scale, int lane) {
   using L = Lane<T, WIDE>;
 #pragma unroll
   for (int p = 0; p < L::PIECES; ++p) {
@@ -100,7 +100,7 @@ __device__ __forceinline__ void put_row(O* row, const Lane<T, WIDE>& sum, int wi
     float old[L::PIECE];
 #pragma unroll
     for (int j = 0; j < L::PIECE; ++j) old[j] = 0.f;
-    if (add) {
+    if (ADD) {
 #pragma unroll
       for (int j = 0; j < L::PIECE; ++j) old[j] = to_float(row[c + j]);
     }
@@ -126,7 +126,7 @@ __device__ __forceinline__ int quotient_of(unsigned long long v, unsigned long l
   return int((v * unsigned(inverse >> 32) + (v * unsigned(inverse) >> 32)) >> 32);
 }
 
-__global__ void __launch_bounds__(DEAL_THREADS, 1) deal_kernel(const Work w) {
+__global__ void __launch_bounds__(DEAL_THREADS + 32, 1) deal_kernel(const Work w) {
   extern __shared__ int32_t shared[];
   __shared__ int mine[DEAL_WARPS], lower[DEAL_WARPS], running[DEAL_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, deal = blockIdx.x;
@@ -135,19 +135,15 @@ __global__ void __launch_bounds__(DEAL_THREADS, 1) deal_kernel(const Work w) {
   int32_t* list_place = counts + DEAL_WARPS * rows;  // [warp][LISTED]
   uint32_t* list_row = reinterpret_cast<uint32_t*>(list_place + DEAL_WARPS * LISTED);   // row * LISTED + rank
   __shared__ alignas(16) uint4 zeros[ZEROS / 16];
-  for (int j = threadIdx.x; j < DEAL_WARPS * rows; j += DEAL_THREADS) counts[j] = 0;
-  if (!w.add) {
-    for (int j = threadIdx.x; j < ZEROS / 16; j += DEAL_THREADS) zeros[j] = make_uint4(0, 0, 0, 0);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
-  __syncthreads();
+  auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(DEAL_THREADS) : "memory"); };
   pdl_launch_dependents();
-  pdl_wait();
-  for (long long i = deal * DEAL_THREADS + threadIdx.x; i < static_cast<long long>(w.groups) * w.slices; i += w.deals * DEAL_THREADS) w.arrived[i] = 0;
-
-  // ---- zeros: the CTAs' pieces side by side, so that all of them write in one part of the table; a lane of the last warp a piece
-  const bool zeroing = !w.add && warp == DEAL_WARPS - 1;
-  if (zeroing) {
+  if (warp == DEAL_WARPS) {
+    // ---- zeros: the CTAs' pieces side by side, so that all of them write in one part of the table; a lane a piece
+    if (w.add) return;
+    for (int j = lane; j < ZEROS / 16; j += 32) zeros[j] = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    pdl_wait();
     char* out = static_cast<char*>(w.out);
     const long long whole = w.bytes / 16 * 16;
     for (long long at = (deal + static_cast<long long>(lane) * w.deals) * ZEROS; at < whole; at += 32ll * w.deals * ZEROS) {
@@ -156,7 +152,13 @@ __global__ void __launch_bounds__(DEAL_THREADS, 1) deal_kernel(const Work w) {
     }
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     if (deal == 0 && whole + lane < w.bytes) out[whole + lane] = 0;
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    return;
   }
+  for (int j = threadIdx.x; j < DEAL_WARPS * rows; j += DEAL_THREADS) counts[j] = 0;
+  sync();
+  pdl_wait();
+  for (long long i = deal * DEAL_THREADS + threadIdx.x; i < static_cast<long long>(w.groups) * w.slices; i += w.deals * DEAL_THREADS) w.arrived[i] = 0;
 
   // ---- a warp's share of the places, in order: each(row, place, rank behind what counts says at the start, how many of the share came before)
   constexpr int LOADS = 16;
@@ -202,8 +204,8 @@ __global__ void __launch_bounds__(DEAL_THREADS, 1) deal_kernel(const Work w) {
     mine[warp] = n_mine;
     lower[warp] = n_lower;
   }
-  __syncthreads();
-  int total = mine[lane], offset = lower[lane], most = total;   // (a lane a warp)
+  sync();
+  int total = lane < DEAL_WARPS ? mine[lane] : 0, offset = lane < DEAL_WARPS ? lower[lane] : 0, most = total;   // (a lane a warp)
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(DEAL_THREADS, 1) deal_kernel(const Work w) {
     up += lane >= o ? x : 0;
   }
   if (lane == 31) running[warp] = up;
-  __syncthreads();
+  sync();
   int begin = lane < warp ? running[lane] : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) begin += __shfl_xor_sync(0xffffffffu, begin, o);
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(DEAL_THREADS, 1) deal_kernel(const Work w) {
       begin += n;
     }
   }
-  __syncthreads();
+  sync();
 
   // ---- where each place goes
   if (most <= LISTED) {
@@ -262,10 +264,9 @@ __global__ void __launch_bounds__(DEAL_THREADS, 1) deal_kernel(const Work w) {
       w.place[at] = place;
     });
   }
-  if (zeroing) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
-template <typename T, typename O, bool WIDE>
+template <typename T, typename O, bool WIDE, bool ADD>
 __global__ void __launch_bounds__(THREADS, 2) sum_kernel(const Work w) {
   __shared__ float heads[WARPS][SLICE], tails[WARPS][SLICE];   // of a window: the sum of the row that an earlier one began; of the row that the next goes on with
   __shared__ int head_row[WARPS], tail_row[WARPS];             // -1: none
@@ -287,13 +288,14 @@ __global__ void __launch_bounds__(THREADS, 2) sum_kernel(const Work w) {
   if (n > 0) {
     const int place = lane < n ? w.place[from + lane] : 0, number = lane < n ? w.row[from + lane] : -1;
     const int before = from > 0 ? w.row[from - 1] : -1, after = from + n < held ? w.row[from + n] : -1;
+    const long long from_place = place * w.ld, to_number = number * w.ld_o;   // (a lane's, once; the warp asks the lane)
     constexpr int BATCH = WIDE && sizeof(T) == 2 ? 8 : 4;   // rows asked for together; two batches are on their way (what the registers hold)
     Raw<T, WIDE> raw[2][BATCH];
     auto load = [&](Raw<T, WIDE> (&r)[BATCH], int i0) {
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) {
-        const int t = __shfl_sync(0xffffffffu, place, (i0 + j) & 31);
-        if (i0 + j < n) r[j].load(above + t * w.ld, width, lane);
+        const long long t = __shfl_sync(0xffffffffu, from_place, (i0 + j) & 31);
+        if (i0 + j < n) r[j].load(above + t, width, lane);
       }
     };
     Lane<T, WIDE> sum;
@@ -312,8 +314,9 @@ __global__ void __launch_bounds__(THREADS, 2) sum_kernel(const Work w) {
           r[j].add_to(sum);
           const int other = __shfl_sync(0xffffffffu, number, (i + 1) & 31), next = i + 1 < n ? other : after;
           if (next != row) {
+            const long long to_row = __shfl_sync(0xffffffffu, to_number, i);
             if (began_here) {
-              put_row<T, O, WIDE>(out + row * w.ld_o, sum, width, w.scale, w.add != 0, lane);
+              put_row<ADD>(out + to_row, sum, width, w.scale, lane);
             } else {
               head = row;
               keep(heads[warp]);
@@ -349,7 +352,7 @@ __global__ void __launch_bounds__(THREADS, 2) sum_kernel(const Work w) {
   float* shares = w.shares + static_cast<long long>(group) * 2 * w.width_up + col;
   auto put = [&](int row, float sum) {
     O* to = out + row * w.ld_o + c;
-    *to = from_float<O>(sum * w.scale + (w.add ? to_float(*to) : 0.f));
+    *to = from_float<O>(fmaf(sum, w.scale, ADD ? to_float(*to) : 0.f));
   };
   int ended = -1, open = -1;   // rows of other CTAs, too: the one that ends here, the one that goes on
   float sum = 0.f;
@@ -433,7 +436,7 @@ __global__ void __launch_bounds__(THREADS) token_rows_kernel(const int32_t* ids,
         raw.load(table + id * ld + c, width - c, lane);
         raw.add_to(row);
       }
-      put_row<T, O, WIDE>(out + t * ld_o + c, row, width - c, held ? scale : 0.f, false, lane);
+      put_row<false>(out + t * ld_o + c, row, width - c, held ? scale : 0.f, lane);
     }
   }
 }
@@ -464,13 +467,13 @@ int launch_deal(const Work& w, cudaStream_t stream) {
   static std::atomic<bool> done[64];
   const int status = allow_smem(deal_kernel, DEAL_WARPS * MOST_ROWS * 4 + LISTED_BYTES, done);
   if (status != R2_OK) return status;
-  r2_launch(deal_kernel, dim3(w.deals), dim3(DEAL_THREADS), ((w.vocab - 1) / w.deals + 1) * size_t(DEAL_WARPS * 4) + LISTED_BYTES, stream, w);
+  r2_launch(deal_kernel, dim3(w.deals), dim3(DEAL_THREADS + 32), ((w.vocab - 1) / w.deals + 1) * size_t(DEAL_WARPS * 4) + LISTED_BYTES, stream, w);
   return launch_status();
 }
 
 template <typename T, typename O, bool WIDE>
 int launch_sums(const Work& w, cudaStream_t stream) {
-  r2_launch(sum_kernel<T, O, WIDE>, dim3(unsigned(w.groups) * unsigned(w.slices)), dim3(THREADS), size_t(0), stream, w);
+  r2_launch(w.add ? sum_kernel<T, O, WIDE, true> : sum_kernel<T, O, WIDE, false>, dim3(unsigned(w.groups) * unsigned(w.slices)), dim3(THREADS), size_t(0), stream, w);
   return launch_status();
 }
 
@@ -480,7 +483,7 @@ void share_out(Work& w) {
   w.slice = ((w.width + w.slices - 1) / w.slices + 63) / 64 * 64;   // (whole lines of 128 bytes)
   w.slices = (w.width + w.slice - 1) / w.slice;
   w.window = 32;
-  while (w.window > 8 && static_cast<long long>(w.tokens) * w.slices < 2ll * n_sms() * WARPS * w.window) w.window /= 2;
+  while (w.window > 4 && static_cast<long long>(w.tokens) * w.slices < 2ll * n_sms() * WARPS * w.window) w.window /= 2;
   w.groups = (w.tokens + WARPS * w.window - 1) / (WARPS * w.window);
   w.width_up = (w.width + 7) / 8 * 8;
   w.deals = deals_of(w.vocab);
