@@ -36,9 +36,10 @@ constexpr int BK = 64;           // one 128-byte swizzle span of bfloat16
 constexpr int UMMA_K = 16;
 constexpr int THREADS = 320;     // warp 0: TMA, warp 1: products + tensor memory, warps 2-9: results
 constexpr int WARPS = 8;
-constexpr int STAGES = 6;
+constexpr int STAGES = 5;
 constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = HALF * BK * 2;
-constexpr size_t SMEM = 1024 + STAGES * size_t(A_BYTES + B_BYTES) + (2 * STAGES + 4) * 8 + 16;
+constexpr uint32_t SLAB = 32 * 128;   // 32 rows of 128 bytes on their way out; a warp has two
+constexpr size_t SMEM = 1024 + STAGES * size_t(A_BYTES + B_BYTES) + 2 * WARPS * SLAB + (2 * STAGES + 4) * 8 + 16;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -58,12 +59,8 @@ struct Work {
   const float* log_sum;
   int first;                 // FACTORS: the piece's first token
   float2* part;              // LOGSUM: [half tile][row]: the largest z log2 e and the sum of 2^(z log2 e - it)
-  bf16* dz;                  // FACTORS: [plane][row][ld]
-  long long dz_plane;
-  float* shares;             // ROWS: [split][row][ld]
-  long long share_plane;
-  void* out;                 // TABLE
-  long long ld;              // of dz, shares or out
+  void* out;                 // TABLE, where tensor copies cannot write it
+  long long ld;
   int* error_flag;
 };
 
@@ -95,6 +92,17 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
 }
 // The whole warp's wait: its lanes go on together, also when it ran out.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+// 32 rows of 128 bytes from shared memory into a box of the map (what lies outside is left out), or added to float numbers there.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, int plane, uint32_t from) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(from), "r"(x), "r"(y), "r"(plane) : "memory");
+}
+__device__ __forceinline__ void add_box(const CUtensorMap* map, int x, int y, int plane, uint32_t from) {
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(map), "r"(from), "r"(x), "r"(y), "r"(plane) : "memory");
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 __device__ __forceinline__ float fast_rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -148,38 +156,52 @@ template <int MODE> __device__ __forceinline__ Unit unit_of(const Work& w, long 
   return u;
 }
 
-// 32 numbers of a row of results, from column c of [0, n) on.
-template <typename T> __device__ __forceinline__ void put32(T* row, int c, int n, const float (&v)[32], bool wide) {
-  if constexpr (sizeof(T) == 2) {
-    if (wide && c + 32 <= n) {
-      uint4* to = reinterpret_cast<uint4*>(row + c);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        to[j] = make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]), pack_bf16(v[8 * j + 4], v[8 * j + 5]),
-                           pack_bf16(v[8 * j + 6], v[8 * j + 7]));
-      return;
-    }
-  } else {
-    if (wide && c + 32 <= n) {
-      float4* to = reinterpret_cast<float4*>(row + c);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) to[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-      return;
+// A warp's way out: rows of 128 bytes (the lane's row), two slabs in turn, each stored once it is whole.
+struct Slabs {
+  uint32_t base;   // of the warp's two
+  int lane, turn;
+  __device__ __forceinline__ uint32_t begin() {   // a slab that the copies have read
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    __syncwarp();
+    return base + (turn++ & 1) * SLAB;
+  }
+  __device__ __forceinline__ void put16(uint32_t slab, int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {   // swizzled, as the map has it
+    st_shared16(slab + lane * 128 + ((piece ^ (lane & 7)) << 4), a, b, c, d);
+  }
+  __device__ __forceinline__ void end(const CUtensorMap* map, int x, int y, int plane, uint32_t slab, bool add) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      if (add) add_box(map, x, y, plane, slab);
+      else store_box(map, x, y, plane, slab);
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
   }
+};
+
+// 64 columns of the thread's tensor-memory lane.
+__device__ __forceinline__ void tmem_row64(uint32_t taddr, float (&v)[64]) {
+  uint32_t a[32], b[32];
+  tmem_load32(taddr, a);
+  tmem_load32(taddr + 32, b);
+  tmem_load_wait(a);
+  tmem_tie(b);
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (c + j < n) row[c + j] = from_float<T>(v[j]);
+  for (int j = 0; j < 32; ++j) {
+    v[j] = __uint_as_float(a[j]);
+    v[32 + j] = __uint_as_float(b[j]);
+  }
 }
 
 template <int MODE, bool CAPPED, typename T>
-__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Work w) {
+__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                              const __grid_constant__ CUtensorMap map_out, const Work w) {
   constexpr bool A_MN = MODE == TABLE, B_MN = MODE == ROWS || MODE == TABLE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t a_base = smem_u32(smem), b_base = a_base + STAGES * A_BYTES;
-  const uint32_t full = b_base + STAGES * B_BYTES, empty = full + STAGES * 8, acc_full = empty + STAGES * 8, acc_empty = acc_full + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + STAGES * size_t(A_BYTES + B_BYTES) + (2 * STAGES + 4) * 8);
+  const uint32_t slabs = b_base + STAGES * B_BYTES, full = slabs + 2 * WARPS * SLAB, empty = full + STAGES * 8, acc_full = empty + STAGES * 8, acc_empty = acc_full + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + STAGES * size_t(A_BYTES + B_BYTES) + 2 * WARPS * SLAB + (2 * STAGES + 4) * 8);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank;
@@ -305,6 +327,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
   } else if (warp >= 2) {
     // ---- results: each CTA its own 128 rows; a warp 32 of them (the lanes of tensor memory that it may read) and half of the columns
     const int q = warp & 3, side = (warp - 2) >> 2;
+    Slabs out = {slabs + (warp - 2) * 2 * SLAB, lane, 0};
     uint32_t local = 0;
     bool ok = true;
     for (long long i = pair; i < n_units; i += n_pairs, ++local) {
@@ -327,83 +350,92 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const bool none = u.kb_end <= u.kb_begin;   // nothing to sum over: zeros
+      const int row0 = (u.row * 2 + int(rank)) * BM + q * 32;
       float top = -3.4028234663852886e38f, sum = 0.f;
 #pragma unroll 1
-      for (int c = side * HALF; c < (side + 1) * HALF && ok; c += 32) {
-        if (col0 + c >= w.n && MODE != LOGSUM) break;
-        uint32_t r[32];
-        tmem_load32(tmem + buf * BN + uint32_t(c) + (uint32_t(q * 32) << 16), r);
-        tmem_load_wait(r);
-        float v[32];
+      for (int c = side * HALF; c < (side + 1) * HALF && ok; c += 64) {
+        if (col0 + c >= w.n || (MODE != LOGSUM && MODE != FACTORS && row0 >= m)) break;
+        float v[64];
+        tmem_row64(tmem + buf * BN + uint32_t(c) + (uint32_t(q * 32) << 16), v);
+        if constexpr (MODE == ROWS || MODE == TABLE) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = none ? 0.f : __uint_as_float(r[j]);
+          for (int j = 0; j < 64; ++j) v[j] = none ? 0.f : v[j];
+        }
         if constexpr (MODE == LOGSUM) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = log2_units<CAPPED>(v[j], w);
-          if (col0 + c + 32 > w.n) {
+          for (int j = 0; j < 64; ++j) v[j] = log2_units<CAPPED>(v[j], w);
+          if (col0 + c + 64 > w.n) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = col0 + c + j < w.n ? v[j] : -INFINITY;
+            for (int j = 0; j < 64; ++j) v[j] = col0 + c + j < w.n ? v[j] : -INFINITY;
           }
           float most = top;
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) most = max3(most, v[j], v[j + 1]);
+          for (int j = 0; j < 64; j += 2) most = max3(most, v[j], v[j + 1]);
           float s0 = sum * fast_exp2(top - most), s1 = 0.f;
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
+          for (int j = 0; j < 64; j += 2) {
             s0 += fast_exp2(v[j] - most);
             s1 += fast_exp2(v[j + 1] - most);
           }
           sum = s0 + s1;
           top = most;
         } else if constexpr (MODE == FACTORS) {
-          float slope[CAPPED ? 32 : 1];
+          const bool counts = factor != 0.f;   // (rows behind the last one are zeros, which the table's gradient adds to the last of its sums)
+          const bool learns = __any_sync(0xffffffffu, target >= c && target < c + 64);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
+          for (int j = 0; j < 64; ++j) {
+            float slope = 1.f;
             if constexpr (CAPPED) {
               const float h = fast_rcp(fast_exp2(v[j] * w.cap_in) + 1.f);   // (1 - tanh) / 2
               v[j] = fast_exp2(fmaf(-2.f * w.cap_out, h, w.cap_out) - sum2);
-              slope[j] = 4.f * h * (1.f - h);                               // 1 - tanh^2
+              slope = 4.f * h * (1.f - h);                                  // 1 - tanh^2
             } else {
               v[j] = fast_exp2(fmaf(v[j], LOG2E, -sum2));
             }
-          }
-          if (__any_sync(0xffffffffu, target >= c && target < c + 32)) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] -= target == c + j ? 1.f : 0.f;
-          }
-          const bool counts = factor != 0.f;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if constexpr (CAPPED) v[j] *= slope[j];
+            if (learns) v[j] -= target == c + j ? 1.f : 0.f;
+            if constexpr (CAPPED) v[j] *= slope;
             v[j] = counts ? v[j] * factor : 0.f;
           }
-          // (rows up to the end of the tile: zeros, which the table's gradient adds to the last of its sums)
-          bf16* to = w.dz + row * w.ld;
-          if (w.terms == 1) {
-            put32<bf16>(to, col0 + c, INT_MAX, v, true);
-          } else {
-            for (int plane = 0; plane < 3; ++plane) {
-              float high[32];
+          for (int plane = 0; plane < (w.terms == 1 ? 1 : 3); ++plane) {
+            const uint32_t slab = out.begin();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                high[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
-                v[j] -= high[j];
+            for (int p = 0; p < 8; ++p) {
+              uint32_t r[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) r[j] = pack_bf16(v[8 * p + 2 * j], v[8 * p + 2 * j + 1]);
+              out.put16(slab, p, r[0], r[1], r[2], r[3]);
+              if (w.terms > 1) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  v[8 * p + 2 * j] -= __uint_as_float(r[j] << 16);
+                  v[8 * p + 2 * j + 1] -= __uint_as_float(r[j] & 0xffff0000u);
+                }
               }
-              put32<bf16>(to + plane * w.dz_plane, col0 + c, INT_MAX, high, true);
             }
+            out.end(&map_out, col0 + c, row0, plane, slab, false);
           }
-        } else if constexpr (MODE == ROWS) {
-          if (row < m) {
-            float* to = w.shares + u.split * w.share_plane + row * w.ld;
-            if (w.add) {
+        } else if (MODE == TABLE && w.out != nullptr) {
+          T* to = static_cast<T*>(w.out) + row * w.ld + col0 + c;
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (col0 + c + j < w.n) v[j] += to[col0 + c + j];
-            }
-            put32<float>(to, col0 + c, w.n, v, true);
-          }
+          for (int j = 0; j < 64; ++j)
+            if (row < m && col0 + c + j < w.n) to[j] = from_float<T>(v[j]);
+        } else if constexpr (sizeof(T) == 2 && MODE == TABLE) {
+          const uint32_t slab = out.begin();
+#pragma unroll
+          for (int p = 0; p < 8; ++p)
+            out.put16(slab, p, pack_bf16(v[8 * p], v[8 * p + 1]), pack_bf16(v[8 * p + 2], v[8 * p + 3]), pack_bf16(v[8 * p + 4], v[8 * p + 5]),
+                      pack_bf16(v[8 * p + 6], v[8 * p + 7]));
+          out.end(&map_out, col0 + c, row0, 0, slab, false);
         } else {
-          if (row < m) put32<T>(static_cast<T*>(w.out) + row * w.ld, col0 + c, w.n, v, (w.ld * sizeof(T)) % 16 == 0);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t slab = out.begin();
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+              out.put16(slab, p, __float_as_uint(v[32 * half + 4 * p]), __float_as_uint(v[32 * half + 4 * p + 1]), __float_as_uint(v[32 * half + 4 * p + 2]),
+                        __float_as_uint(v[32 * half + 4 * p + 3]));
+            out.end(&map_out, col0 + c + 32 * half, row0, u.split, slab, MODE == ROWS && w.add);
+          }
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -413,6 +445,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         if (row < m) w.part[(size_t(u.col) * 2 + side) * m + row] = ok ? make_float2(top, sum) : make_float2(NAN, NAN);
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -599,11 +632,25 @@ struct Operand {
   int planes;
 };
 
+bool encode(CUtensorMap* map, CUtensorMapDataType type, int size, const void* at, long long inner, long long outer, long long planes, long long ld, long long plane, int box_inner,
+            int box_outer) {
+  const r2::EncodeTiledFn fn = r2::encode_fn();
+  cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(outer), cuuint64_t(planes)};
+  cuuint64_t strides[2] = {cuuint64_t(ld) * size, cuuint64_t(planes > 1 ? plane : ld) * size};
+  cuuint32_t box[3] = {cuuint32_t(box_inner), cuuint32_t(box_outer), 1}, steps[3] = {1, 1, 1};
+  return fn != nullptr && fn(map, type, 3, const_cast<void*>(at), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Boxes of 64 numbers and box_outer rows, as the products load them.
 bool make_map(CUtensorMap* map, const Operand& o, long long inner, long long outer, int box_outer) {
-  cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(outer), cuuint64_t(o.planes)};
-  cuuint64_t strides[2] = {cuuint64_t(o.ld) * 2, cuuint64_t(o.planes > 1 ? o.plane : o.ld) * 2};
-  cuuint32_t box[3] = {cuuint32_t(BK), cuuint32_t(box_outer), 1};
-  return r2::encode_bf16_map(map, o.at, 3, dims, strides, box);
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, o.at, inner, outer, o.planes, o.ld, o.plane, BK, box_outer);
+}
+
+// Boxes of 128 bytes and 32 rows, as results are stored.
+template <typename T> bool make_out_map(CUtensorMap* map, const void* at, long long inner, long long outer, long long planes, long long ld, long long plane) {
+  return encode(map, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, int(sizeof(T)), at, inner, outer, planes, ld, plane,
+                128 / int(sizeof(T)), 32);
 }
 
 // How many CTA pairs the current device holds at once.
@@ -634,7 +681,7 @@ int resident_pairs() {
 }
 
 template <int MODE, bool CAPPED, typename T>
-int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Work& w, long long units, cudaStream_t stream) {
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Work& w, long long units, cudaStream_t stream) {
   auto kernel = product_kernel<MODE, CAPPED, T>;
   static std::atomic<bool> done[64];
   const int status = allow_smem(kernel, SMEM, done);
@@ -651,16 +698,16 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Work& w, long lon
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
   config.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, ma, mb, w);
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, ma, mb, mo, w);
   return e != cudaSuccess ? int(e) : launch_status();
 }
 
 template <int MODE, typename T>
-int launch(const CUtensorMap& ma, const CUtensorMap& mb, const Work& w, long long units, bool capped, cudaStream_t stream) {
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Work& w, long long units, bool capped, cudaStream_t stream) {
   if constexpr (MODE == LOGSUM || MODE == FACTORS) {
-    if (capped) return launch<MODE, true, T>(ma, mb, w, units, stream);
+    if (capped) return launch<MODE, true, T>(ma, mb, mo, w, units, stream);
   }
-  return launch<MODE, false, T>(ma, mb, w, units, stream);
+  return launch<MODE, false, T>(ma, mb, mo, w, units, stream);
 }
 
 int row_blocks(long long rows) { return int(rows < 8 * 1184 ? (rows + 7) / 8 : 1184); }
@@ -760,7 +807,7 @@ int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_
   w.error_flag = error;
   set_cap(w, softcap);
   const long long tiles = (l.rows_up / 256) * (up(vocab, BN) / BN);
-  const int status = launch<LOGSUM, bf16>(ma, mb, w, tiles, softcap > 0.f, stream);
+  const int status = launch<LOGSUM, bf16>(ma, mb, ma, w, tiles, softcap > 0.f, stream);
   if (status != R2_OK) return status;
   const int parts = int(up(vocab, BN) / BN) * 2;
   const T *h = static_cast<const T*>(hidden), *tab = static_cast<const T*>(table);
@@ -793,14 +840,12 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
   w.targets = reinterpret_cast<int32_t*>(space + l.targets);
   w.factor = reinterpret_cast<float*>(space + l.factor);
   w.log_sum = reinterpret_cast<float*>(space + l.sums);
-  w.dz = reinterpret_cast<bf16*>(space + l.factors);
-  w.dz_plane = l.rows_up * l.piece;
-  w.shares = reinterpret_cast<float*>(space + l.shares);
-  w.share_plane = l.rows_up * l.width_up;
   w.error_flag = error;
   set_cap(w, softcap);
-  const Operand dz = {w.dz, l.piece, w.dz_plane, l.planes};
-  CUtensorMap ma, mb;
+  const Operand dz = {space + l.factors, l.piece, l.rows_up * l.piece, l.planes};
+  float* shares = reinterpret_cast<float*>(space + l.shares);
+  const long long share_plane = l.rows_up * l.width_up;
+  CUtensorMap ma, mb, mo;
   int status = launch_status();
   const long long row_tiles = l.rows_up / 256, width_tiles = up(width, BN) / BN;
   for (long long first = 0; first < vocab && status == R2_OK; first += l.piece) {
@@ -809,9 +854,10 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
     w.first = int(first);
     w.n = n;
     w.k = width;
-    w.ld = l.piece;
-    if (!make_map(&ma, x, width, l.rows_up, BM) || !make_map(&mb, part, width, n, HALF)) return R2_BAD_ALIGN;
-    status = launch<FACTORS, bf16>(ma, mb, w, row_tiles * (up(n, BN) / BN), softcap > 0.f, stream);
+    if (!make_map(&ma, x, width, l.rows_up, BM) || !make_map(&mb, part, width, n, HALF) ||
+        !make_out_map<bf16>(&mo, dz.at, l.piece, l.rows_up, l.planes, l.piece, dz.plane))
+      return R2_BAD_ALIGN;
+    status = launch<FACTORS, bf16>(ma, mb, mo, w, row_tiles * (up(n, BN) / BN), softcap > 0.f, stream);
     if (status == R2_OK && d_hidden) {
       Work d = w;
       d.n = width;
@@ -819,22 +865,29 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
       d.per_split = l.per_split;
       d.splits = l.splits;
       d.add = first > 0;
-      d.ld = l.width_up;
-      if (!make_map(&ma, dz, n, l.rows_up, BM) || !make_map(&mb, part, width, n, BK)) return R2_BAD_ALIGN;
-      status = launch<ROWS, bf16>(ma, mb, d, row_tiles * width_tiles * d.splits, false, stream);
+      if (!make_map(&ma, dz, n, l.rows_up, BM) || !make_map(&mb, part, width, n, BK) ||
+          !make_out_map<float>(&mo, shares, width, l.rows_up, l.splits, l.width_up, share_plane))
+        return R2_BAD_ALIGN;
+      status = launch<ROWS, float>(ma, mb, mo, d, row_tiles * width_tiles * d.splits, false, stream);
     }
     if (status == R2_OK && d_table) {
       Work d = w;
       d.m = n;
       d.n = width;
-      d.out = static_cast<T*>(d_table) + first * ld_dt;
-      d.ld = ld_dt;
+      T* out = static_cast<T*>(d_table) + first * ld_dt;
       if (!make_map(&ma, dz, n, l.rows_up, BK) || !make_map(&mb, x, width, l.rows_up, BK)) return R2_BAD_ALIGN;
-      status = launch<TABLE, T>(ma, mb, d, up(n, 256) / 256 * width_tiles, false, stream);
+      if (reinterpret_cast<uintptr_t>(out) % 16 == 0 && ld_dt * sizeof(T) % 16 == 0) {
+        if (!make_out_map<T>(&mo, out, width, n, 1, ld_dt, 0)) return R2_BAD_ALIGN;
+      } else {
+        mo = ma;
+        d.out = out;
+        d.ld = ld_dt;
+      }
+      status = launch<TABLE, T>(ma, mb, mo, d, up(n, 256) / 256 * width_tiles, false, stream);
     }
   }
   if (status == R2_OK && d_hidden) {
-    join_kernel<T><<<row_blocks(rows), 256, 0, stream>>>(w.shares, l.splits, w.share_plane, l.width_up, place, static_cast<T*>(d_hidden), ld_dh, rows, width);
+    join_kernel<T><<<row_blocks(rows), 256, 0, stream>>>(shares, l.splits, share_plane, l.width_up, place, static_cast<T*>(d_hidden), ld_dh, rows, width);
     status = launch_status();
   }
   return status;
