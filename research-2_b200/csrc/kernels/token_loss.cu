@@ -457,60 +457,103 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
   }
 }
 
-// A block's rows: their parts joined, R rows by 256 / R slices of the parts, then the target's logit as a sum of float products by a warp.
-template <typename T, int R>
+// Eight numbers of a row from column c on (zeros behind the last); `wide`: rows start at 16 bytes and hold whole eights.
+template <typename T> __device__ __forceinline__ void load8(const T* row, int c, int width, bool wide, float (&v)[8]) {
+  if (wide) {
+    if constexpr (sizeof(T) == 2) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + c));
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    } else {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(row + c)), y = __ldg(reinterpret_cast<const float4*>(row + c + 4));
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = c + j < width ? to_float(row[c + j]) : 0.f;
+}
+
+// The same numbers in one plane or in three, at places of 16 bytes.
+template <typename T> __device__ __forceinline__ void put_planes8(bf16* to, long long plane, const float (&v)[8]) {
+  uint4 out[sizeof(T) == 2 ? 1 : 3];
+  bf16(*p)[8] = reinterpret_cast<bf16(*)[8]>(out);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if constexpr (sizeof(T) == 2) {
+      p[0][j] = __float2bfloat16_rn(v[j]);
+    } else {
+      bf16 s[3];
+      split3(v[j], s);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) p[i][j] = s[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < int(sizeof(T) == 2 ? 1 : 3); ++i) *reinterpret_cast<uint4*>(to + i * plane) = out[i];
+}
+
+template <typename T> __device__ __forceinline__ bool rows_wide(const T* at, long long ld, int width) {
+  return reinterpret_cast<uintptr_t>(at) % 16 == 0 && ld * sizeof(T) % 16 == 0 && width % 8 == 0;
+}
+
+// A warp a row: its parts joined, and the target's logit as a sum of float products.
+template <typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const float2* part, int parts, const T* hidden, long long ld_h, const T* table, long long ld_t, const int32_t* targets,
                                                      const float* weight, int rows, int width, int vocab, float softcap, float* loss, float* log_sum) {
-  __shared__ float2 held[256];
-  __shared__ float sums[R];
-  const int r0 = blockIdx.x * R, mine = r0 + threadIdx.x % R;
-  float top = -3.4028234663852886e38f, sum = 0.f;
-  if (mine < rows) {
-#pragma unroll 4
-    for (int i = threadIdx.x / R; i < parts; i += 256 / R) {
-      const float2 p = part[size_t(i) * rows + mine];
-      const float most = fmaxf(top, p.x);
-      sum = sum * fast_exp2(top - most) + p.y * fast_exp2(p.x - most);
-      top = most;
-    }
-  }
-  held[threadIdx.x] = make_float2(top, sum);
-  __syncthreads();
-  if (threadIdx.x < R) {
-    for (int i = 1; i < 256 / R; ++i) {
-      const float2 p = held[i * R + threadIdx.x];
-      const float most = fmaxf(top, p.x);
-      sum = sum * fast_exp2(top - most) + p.y * fast_exp2(p.x - most);
-      top = most;
-    }
-    sums[threadIdx.x] = fmaf(top, LN2, logf(sum));
-  }
-  __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = warp; i < R && r0 + i < rows; i += 8) {
-    const int r = r0 + i, y = targets[r];
-    const float factor = weight ? weight[r] : 1.f;
-    const bool counts = y >= 0 && y < vocab && factor != 0.f;
-    const T* x = hidden + size_t(r) * ld_h;
-    const T* t = table + size_t(counts ? y : 0) * ld_t;
-    float dot = 0.f;
-    bool fine = true;   // (float32's planes hold no infinities: a row with one, or with NaN, has no sum)
-    if (counts || sizeof(T) == 4) {
-      for (int d = lane; d < width; d += 32) {
-        const float a = to_float(x[d]);
-        if (sizeof(T) == 4) fine = fine && fabsf(a) < INFINITY;
-        if (counts) dot = fmaf(a, to_float(t[d]), dot);
+  const int lane = threadIdx.x & 31, r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const int y = targets[r];
+  const float factor = weight ? weight[r] : 1.f;
+  const bool counts = y >= 0 && y < vocab && factor != 0.f;
+  const T* x = hidden + size_t(r) * ld_h;
+  const T* t = table + size_t(counts ? y : 0) * ld_t;
+  const bool wide = rows_wide(hidden, ld_h, width) && rows_wide(table, ld_t, width);
+  float dot = 0.f;
+  bool fine = true;   // (float32's planes hold no infinities: a row with one, or with NaN, has no sum)
+  if (counts || sizeof(T) == 4) {
+#pragma unroll 2
+    for (int c = lane * 8; c < width; c += 256) {
+      float a[8], b[8];
+      load8(x, c, width, wide, a);
+      load8(t, c, width, wide, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (sizeof(T) == 4) fine = fine && fabsf(a[j]) < INFINITY;
+        dot = fmaf(a[j], b[j], dot);
       }
     }
-    dot = warp_sum(dot);
-    fine = __all_sync(0xffffffffu, fine);
-    if (lane == 0) {
-      const float s = fine ? sums[i] : NAN;
-      log_sum[r] = s;
-      const float z = softcap > 0.f ? softcap * tanhf(dot / softcap) : dot;
-      const float gap = s - z;   // (never negative but by rounding)
-      loss[r] = counts ? factor * (gap < 0.f ? 0.f : gap) : 0.f;
+  }
+  float top = -3.4028234663852886e38f, sum = 0.f;
+  for (int i0 = lane; i0 < parts; i0 += 32 * 8) {
+    float2 p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = i0 + 32 * j < parts ? part[size_t(i0 + 32 * j) * rows + r] : make_float2(-3.4028234663852886e38f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float most = fmaxf(top, p[j].x);
+      sum = sum * fast_exp2(top - most) + p[j].y * fast_exp2(p[j].x - most);
+      top = most;
     }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float other = __shfl_xor_sync(0xffffffffu, top, o), more = __shfl_xor_sync(0xffffffffu, sum, o), most = fmaxf(top, other);
+    sum = sum * fast_exp2(top - most) + more * fast_exp2(other - most);
+    top = most;
+  }
+  dot = warp_sum(dot);
+  fine = __all_sync(0xffffffffu, fine);
+  if (lane == 0) {
+    const float s = fine ? fmaf(top, LN2, logf(sum)) : NAN;
+    log_sum[r] = s;
+    const float z = softcap > 0.f ? softcap * tanhf(dot / softcap) : dot;
+    const float gap = s - z;   // (never negative but by rounding)
+    loss[r] = counts ? factor * (gap < 0.f ? 0.f : gap) : 0.f;
   }
 }
 
@@ -549,16 +592,12 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
     all += totals[1][i];
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) *count = all;
+  const bool wide = rows_wide(hidden, ld, width);
   auto copy = [&](int to, const T* from) {   // (null: zeros)
-    for (int d = lane; d < width; d += 32) {
-      if constexpr (sizeof(T) == 2) {
-        x[size_t(to) * ld_x + d] = from ? from[d] : from_float<bf16>(0.f);
-      } else {
-        bf16 p[3];
-        split3(from ? from[d] : 0.f, p);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) x[i * plane + size_t(to) * ld_x + d] = p[i];
-      }
+    for (int c = lane * 8; c < width; c += 256) {
+      float v[8] = {};
+      if (from) load8(from, c, width, wide, v);
+      put_planes8<T>(x + size_t(to) * ld_x + c, plane, v);
     }
   };
   // a block's rows, 32 at a time
@@ -586,18 +625,13 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
 template <typename T>
 __global__ void __launch_bounds__(256) planes_kernel(const T* from, long long ld, int rows, int width, bf16* to, long long ld_to, long long plane) {
   const int lane = threadIdx.x & 31;
+  const bool wide = rows_wide(from, ld, width);
   for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8LL) {
-    const T* x = from + r * ld;
-    bf16* o = to + r * ld_to;
-    for (int d = lane; d < width; d += 32) {
-      if constexpr (sizeof(T) == 2) {
-        o[d] = x[d];
-      } else {
-        bf16 p[3];
-        split3(x[d], p);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) o[i * plane + d] = p[i];
-      }
+#pragma unroll 2
+    for (int c = lane * 8; c < width; c += 256) {
+      float v[8];
+      load8(from + r * ld, c, width, wide, v);
+      put_planes8<T>(to + r * ld_to + c, plane, v);
     }
   }
 }
@@ -607,16 +641,29 @@ template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const float* shares, int splits, long long plane, long long ld, const int32_t* place, T* out, long long ld_o, int rows,
                                                    int width) {
   const int lane = threadIdx.x & 31;
+  const bool wide = rows_wide(out, ld_o, width);
   for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8LL) {
     const int at = place[r];
     T* o = out + r * ld_o;
-    for (int d = lane; d < width; d += 32) {
-      float sum = 0.f;
+    for (int c = lane * 4; c < width; c += 128) {
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
       if (at >= 0) {
-        const float* s = shares + at * ld + d;
-        for (int i = 0; i < splits; ++i) sum += s[i * plane];
+        const float* s = shares + at * ld + c;   // (rows of whole eights)
+#pragma unroll 4
+        for (int i = 0; i < splits; ++i) {
+          const float4 v = __ldg(reinterpret_cast<const float4*>(s + i * plane));
+          sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
       }
-      o[d] = from_float<T>(sum);
+      if (wide) {
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(o + c) = make_uint2(pack_bf16(sum.x, sum.y), pack_bf16(sum.z, sum.w));
+        else *reinterpret_cast<float4*>(o + c) = sum;
+      } else {
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < width) o[c + j] = from_float<T>(v[j]);
+      }
     }
   }
 }
@@ -710,7 +757,7 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, 
   return launch<MODE, false, T>(ma, mb, mo, w, units, stream);
 }
 
-int row_blocks(long long rows) { return int(rows < 8 * 1184 ? (rows + 7) / 8 : 1184); }
+int row_blocks(long long rows) { return int(rows < 8 * 4736 ? (rows + 7) / 8 : 4736); }
 
 // What a call's scratch holds, in bytes from its start.
 constexpr long long FACTOR_BYTES = 256ll << 20;   // of dz at a time
@@ -748,14 +795,17 @@ Layout layout(int dtype, long long rows, long long width, long long vocab, bool 
     const int n_kb = int((l.piece + BK - 1) / BK);
     const long long tiles = l.rows_up / 256 * (up(width, BN) / BN);
     const int pairs = resident_pairs();
-    // shares of k: so many that the last round of pairs is full, but no shorter than eight steps
-    long long best = -1;
+    // shares of k, of no fewer than eight steps: more of them fill the last round of pairs, and each is written for every piece and read once more (a tile's
+    // 256 KB take a seventh of a step's time, a step of 64 being 0.29 us on a pair)
+    double best = -1;
     for (int s = 1; s <= 64 && (s == 1 || n_kb / s >= 8); ++s) {
-      const long long cost = (tiles * s + pairs - 1) / pairs * (((n_kb + s - 1) / s) * l.planes * (l.planes + 1) / 2 + 8);
+      const int per = (n_kb + s - 1) / s;
+      const double rounds = double((tiles * s + pairs - 1) / pairs), steps = per * l.planes * (l.planes + 1) / 2 + 8;
+      const double cost = l.pieces * rounds * steps + double(s) * tiles * 0.14 * (l.pieces + 1);
       if (best < 0 || cost < best) {
         best = cost;
-        l.per_split = (n_kb + s - 1) / s;
-        l.splits = (n_kb + l.per_split - 1) / l.per_split;
+        l.per_split = per;
+        l.splits = (n_kb + per - 1) / per;
       }
     }
     l.factors = take(l.planes * l.rows_up * l.piece * 2);
@@ -811,11 +861,7 @@ int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_
   if (status != R2_OK) return status;
   const int parts = int(up(vocab, BN) / BN) * 2;
   const T *h = static_cast<const T*>(hidden), *tab = static_cast<const T*>(table);
-  if (rows >= 4096) {
-    finish_kernel<T, 32><<<(rows + 31) / 32, 256, 0, stream>>>(w.part, parts, h, ld_h, tab, ld_t, targets, weight, rows, width, vocab, softcap, loss, log_sum);
-  } else {
-    finish_kernel<T, 8><<<(rows + 7) / 8, 256, 0, stream>>>(w.part, parts, h, ld_h, tab, ld_t, targets, weight, rows, width, vocab, softcap, loss, log_sum);
-  }
+  finish_kernel<T><<<(rows + 7) / 8, 256, 0, stream>>>(w.part, parts, h, ld_h, tab, ld_t, targets, weight, rows, width, vocab, softcap, loss, log_sum);
   return launch_status();
 }
 
