@@ -230,6 +230,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
   cluster_sync();   // both CTAs' barriers exist before either's loads, commits or arrivals signal them
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
+  pdl_wait();
   uint32_t leader_full, leader_acc_empty;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(leader_full) : "r"(full), "r"(0u));
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(leader_acc_empty) : "r"(acc_empty), "r"(0u));
@@ -336,12 +337,12 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
       const int row = (u.row * 2 + int(rank)) * BM + q * 32 + lane;
       const int col0 = u.col * BN;
       int target = -1;
-      float factor = 0.f, sum2 = 0.f;
+      float factor = 0.f, less2 = 0.f;   // |factor| exp(z - log_sum) is 2^(z log2 e - less2)
       if constexpr (MODE == FACTORS) {
         if (row < m) {
           target = w.targets[row] - w.first - col0;   // (no overflow: both lie in [0, vocab))
           factor = w.factor[row];
-          sum2 = w.log_sum[row] * LOG2E;
+          less2 = w.log_sum[row] * LOG2E - log2f(fabsf(factor));
         }
       }
       if (ok && !warp_wait(acc_full + buf * 8, (local >> 1) & 1u)) {
@@ -380,21 +381,25 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
           sum = s0 + s1;
           top = most;
         } else if constexpr (MODE == FACTORS) {
-          const bool counts = factor != 0.f;   // (rows behind the last one are zeros, which the table's gradient adds to the last of its sums)
+          const float size = fabsf(factor);
+          // of a pair, once it is rounded: the factor's sign; zeros in rows behind the last one, which the table's gradient adds to its sums
+          const uint32_t sign = factor < 0.f ? 0x80008000u : 0u, held = row < m ? 0xffffffffu : 0u;
           const bool learns = __any_sync(0xffffffffu, target >= c && target < c + 64);
+          if constexpr (CAPPED) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) {
-            float slope = 1.f;
-            if constexpr (CAPPED) {
-              const float h = fast_rcp(fast_exp2(v[j] * w.cap_in) + 1.f);   // (1 - tanh) / 2
-              v[j] = fast_exp2(fmaf(-2.f * w.cap_out, h, w.cap_out) - sum2);
-              slope = 4.f * h * (1.f - h);                                  // 1 - tanh^2
-            } else {
-              v[j] = fast_exp2(fmaf(v[j], LOG2E, -sum2));
+            for (int j = 0; j < 64; ++j) {
+              const float h = fast_rcp(fast_exp2(v[j] * w.cap_in) + 1.f);   // (1 - tanh) / 2; the slope 1 - tanh^2 is 4 h (1 - h)
+              v[j] = fast_exp2(fmaf(-2.f * w.cap_out, h, w.cap_out) - less2);
+              if (learns) v[j] -= target == c + j ? size : 0.f;
+              v[j] *= 4.f * h * (1.f - h);
             }
-            if (learns) v[j] -= target == c + j ? 1.f : 0.f;
-            if constexpr (CAPPED) v[j] *= slope;
-            v[j] = counts ? v[j] * factor : 0.f;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] = fast_exp2(fmaf(v[j], LOG2E, -less2));
+            if (learns) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j) v[j] -= target == c + j ? size : 0.f;
+            }
           }
           for (int plane = 0; plane < (w.terms == 1 ? 1 : 3); ++plane) {
             const uint32_t slab = out.begin();
@@ -403,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
               uint32_t r[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j) r[j] = pack_bf16(v[8 * p + 2 * j], v[8 * p + 2 * j + 1]);
-              out.put16(slab, p, r[0], r[1], r[2], r[3]);
+              out.put16(slab, p, (r[0] & held) ^ sign, (r[1] & held) ^ sign, (r[2] & held) ^ sign, (r[3] & held) ^ sign);
               if (w.terms > 1) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -448,6 +453,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
+  // (The next kernel's CTAs start here, not earlier: ones that wait beside a product of 100 us made it 12 us longer.)
+  pdl_launch_dependents();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   cluster_sync();   // neither CTA frees tensor memory or leaves while the other may still use it
@@ -505,6 +512,8 @@ template <typename T> __device__ __forceinline__ bool rows_wide(const T* at, lon
 template <typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const float2* part, int parts, const T* hidden, long long ld_h, const T* table, long long ld_t, const int32_t* targets,
                                                      const float* weight, int rows, int width, int vocab, float softcap, float* loss, float* log_sum) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31, r = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (r >= rows) return;
   const int y = targets[r];
@@ -564,6 +573,8 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
                                                      const float* log_sum, bf16* x, long long ld_x, long long plane, int32_t* y_out, float* f_out, float* s_out,
                                                      int32_t* place, int* count) {
   __shared__ int totals[2][8];
+  pdl_launch_dependents();
+  pdl_wait();
   const int first = blockIdx.x * own, last = min(rows, first + own);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto counts = [&](int r) {
@@ -624,6 +635,8 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
 // A matrix in planes of bfloat16 whose rows start at 16 bytes: float32 in three, bfloat16 that tensor copies cannot read in one.
 template <typename T>
 __global__ void __launch_bounds__(256) planes_kernel(const T* from, long long ld, int rows, int width, bf16* to, long long ld_to, long long plane) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const bool wide = rows_wide(from, ld, width);
   for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8LL) {
@@ -640,6 +653,8 @@ __global__ void __launch_bounds__(256) planes_kernel(const T* from, long long ld
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const float* shares, int splits, long long plane, long long ld, const int32_t* place, T* out, long long ld_o, int rows,
                                                    int width) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const bool wide = rows_wide(out, ld_o, width);
   for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8LL) {
@@ -739,12 +754,14 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, 
   config.blockDim = dim3(THREADS);
   config.dynamicSmemBytes = SMEM;
   config.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attr;
-  config.numAttrs = 1;
+  config.numAttrs = g_r2_pdl ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, ma, mb, mo, w);
   return e != cudaSuccess ? int(e) : launch_status();
 }
@@ -829,7 +846,7 @@ template <typename T>
 Operand operand(const void* at, long long ld, long long rows, long long width, const Layout& l, char* space, cudaStream_t stream) {
   if (sizeof(T) == 2 && copies_read(at, ld, rows, width)) return {at, rows <= 1 ? l.width_up : ld, 0, 1};
   bf16* to = reinterpret_cast<bf16*>(space);
-  planes_kernel<T><<<row_blocks(rows), 256, 0, stream>>>(static_cast<const T*>(at), ld, int(rows), int(width), to, l.width_up, rows * l.width_up);
+  r2_launch(planes_kernel<T>, dim3(row_blocks(rows)), dim3(256), size_t(0), stream, static_cast<const T*>(at), ld, int(rows), int(width), to, l.width_up, rows * l.width_up);
   return {to, l.width_up, rows * l.width_up, l.planes};
 }
 
@@ -861,7 +878,7 @@ int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_
   if (status != R2_OK) return status;
   const int parts = int(up(vocab, BN) / BN) * 2;
   const T *h = static_cast<const T*>(hidden), *tab = static_cast<const T*>(table);
-  finish_kernel<T><<<(rows + 7) / 8, 256, 0, stream>>>(w.part, parts, h, ld_h, tab, ld_t, targets, weight, rows, width, vocab, softcap, loss, log_sum);
+  r2_launch(finish_kernel<T>, dim3((rows + 7) / 8), dim3(256), size_t(0), stream, static_cast<const float2*>(w.part), parts, h, ld_h, tab, ld_t, targets, weight, rows, width, vocab, softcap, loss, log_sum);
   return launch_status();
 }
 
@@ -876,7 +893,7 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
   int32_t* place = reinterpret_cast<int32_t*>(space + l.place);
   int own = (rows + 591) / 592;
   own = own > 32 ? 32 : own;
-  gather_kernel<T><<<(rows + own - 1) / own, 256, 0, stream>>>(
+  r2_launch(gather_kernel<T>, dim3((rows + own - 1) / own), dim3(256), size_t(0), stream,
       static_cast<const T*>(hidden), ld_h, rows, width, vocab, own, targets, weight, log_sum, gathered, x.ld, x.plane, reinterpret_cast<int32_t*>(space + l.targets),
       reinterpret_cast<float*>(space + l.factor), reinterpret_cast<float*>(space + l.sums), place, count);
   Work w = {};
@@ -933,7 +950,8 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
     }
   }
   if (status == R2_OK && d_hidden) {
-    join_kernel<T><<<row_blocks(rows), 256, 0, stream>>>(shares, l.splits, share_plane, l.width_up, place, static_cast<T*>(d_hidden), ld_dh, rows, width);
+    r2_launch(join_kernel<T>, dim3(row_blocks(rows)), dim3(256), size_t(0), stream, static_cast<const float*>(shares), l.splits, share_plane, l.width_up,
+              static_cast<const int32_t*>(place), static_cast<T*>(d_hidden), ld_dh, rows, width);
     status = launch_status();
   }
   return status;

@@ -381,3 +381,19 @@ def test_refusals():
     for log_sum in (None, s[:3], s.double(), s.cpu()):
         with pytest.raises(o.KernelError):
             o.token_loss_gradient(x, w, y, log_sum)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_without_a_target_beside_a_table_with_infinities(dtype):
+    # products of a left-out row's place and an infinity are nothing
+    c = Case(300, 64, 700, dtype, 28)
+    c.targets[:] = 3
+    c.targets[70:] = -1
+    c.weight[:] = 1.0
+    c.hidden[:, 0], c.table[:, 0], c.table[500:] = 1.0, 0.0, 0.0
+    c.table[500:, 0] = -float("inf")
+    loss, log_sum, d_hidden, d_table = c.run()
+    keep = Loss(c.hidden, c.table[:500], c.targets, c.weight)
+    assert torch.all((loss.double() - keep.loss).abs() <= keep.loss_off)
+    assert torch.isfinite(d_table).all() and not d_table[500:].any() and not d_hidden[70:].any()
+    assert torch.all((d_table[:500].double() - keep.d_table).abs() <= keep.d_table_off)
