@@ -15,7 +15,9 @@
 // dz is rounded to bfloat16, the type of the gradients that it makes, so that both products run on the tensor cores at full rate.
 //
 // float32 operands are three bfloat16 planes each: x = x0 + x1 + x2 to the last bit (8 bits each), and a product is the six products x_i w_j
-// with i + j <= 2, smallest first; what is left out is below 2^-24 of it. dz is kept in three planes then, too.
+// with i + j <= 2; what is left out is below 2^-24 of it. dz is kept in three planes then, too. The tensor cores add to an accumulator without rounding to nearest: each
+// addition of 16 products takes up to a unit of 2^-24 off, always towards zero. So the small products are added first, over all of k, while the accumulator is small
+// (one after the other for each k they took 4e-6 off a sum of 768 products; so it is 7e-7), and k is cut into shorter shares.
 //
 // Rows without a token or of weight 0 have no part in the gradients: `gather_kernel` puts the others side by side, so that no product reads them
 // (whatever they hold) or spends time on them; the rest of the last 256 rows is zeros.
@@ -102,6 +104,11 @@ __device__ __forceinline__ void add_box(const CUtensorMap* map, int x, int y, in
 }
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// Behind a wait that ran out: the copies that this warp has asked for land (or that wait runs out, too) before its CTA ends. Stages below `stage` were filled
+// in this round of the ring, the others in the one before.
+__device__ __forceinline__ void settle(uint32_t full, int stages, int stage, uint32_t parity) {
+  for (int s = 0; s < stages; ++s) warp_wait(full + s * 8, s < stage ? parity : parity ^ 1u);
 }
 __device__ __forceinline__ float fast_rcp(float x) {
   float y;
@@ -249,8 +256,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     for (long long i = pair; i < n_units && ok; i += n_pairs) {
       const Unit u = unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
       const int a0 = (u.row * 2 + int(rank)) * BM, b0 = u.col * BN + int(rank) * HALF;
-      for (int kb = u.kb_begin; kb < u.kb_end && ok; ++kb) {
-        for (int t = 0; t < w.terms; ++t) {
+      for (int t = 0; t < w.terms && ok; ++t) {   // (all of k for the smallest products first: see below)
+        for (int kb = u.kb_begin; kb < u.kb_end; ++kb) {
           if (!warp_wait(empty + stage * 8, parity ^ 1u)) {
             if (lane == 0) atomicMax(w.error_flag, ERR_EMPTY);
             ok = false;
@@ -282,6 +289,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         }
       }
     }
+    if (!ok && rank == 0) settle(full, STAGES, stage, parity);
   } else if (warp == 1 && rank == 0) {
     // ---- products of the pair (256 rows over the two CTAs)
     constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(A_MN) << 15) | (uint32_t(B_MN) << 16) | (uint32_t(BN >> 3) << 17) |
@@ -461,6 +469,380 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(2 * BN)) : "memory");
+  }
+}
+
+// ---- few rows: LOGSUM and FACTORS of up to 128 ----------------------------------------------
+//
+// The pass over the table is what such a call costs, so the operands change sides: a tile is 128 tokens of the vocabulary by all rows (up to 128 columns of the
+// accumulator), one CTA to an SM, and float32 tables are read as they are: four warps turn each 128 x 32 numbers into the three planes in shared memory, where
+// the others' planes would have been written to memory and read again (six bytes a number, twice). A tile's results go through shared memory, 32
+// rows of the batch at a time, so that a thread has 32 tokens of one row: sums over them need no exchange, and dz leaves in pieces of 64 bytes.
+//
+// LOGSUM keeps a row's largest logit and sum for each of a CTA's four parts of 32 tokens over all its tiles.
+
+constexpr int FEW = 128;            // rows at most
+constexpr int FEW_STAGES = 8;       // of operands, at most
+constexpr int TURNED = 132;         // floats of a row of the turned tile (128 tokens and four of padding)
+
+struct FewWork {
+  int rows, columns;                // of the batch; a multiple of 16: columns of the accumulator
+  int n, k;                         // tokens (of the table, or of a piece); width
+  int stages, loads;                // of operands; float32: of operands in planes, of the table's numbers
+  Work w;                           // count, cap_in, cap_out, targets, factor, log_sum, first, part, error_flag as above
+  bf16* dz;
+  long long dz_plane, ld;
+};
+
+__device__ __forceinline__ uint64_t smem_desc_64(uint32_t addr) {   // K-major rows of 64 bytes, 64-byte swizzle
+  uint64_t d = 0;
+  d |= uint64_t((addr >> 4) & 0x3FFF);
+  d |= uint64_t(1) << 16;
+  d |= uint64_t(512 >> 4) << 32;
+  d |= uint64_t(1) << 46;
+  d |= uint64_t(4) << 61;
+  return d;
+}
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, int plane, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(plane) : "memory");
+}
+
+// Shared memory from its 1,024-byte aligned start. bfloat16: stages of 16 KB of the table and columns * 128 bytes of rows. float32: `loads` of 16 KB of the
+// table's numbers, stages of three planes of 8 KB and columns * 64 bytes each. Then the turned tile and the barriers.
+template <bool F32> __host__ __device__ inline uint32_t few_stage_bytes(int columns) {
+  return F32 ? 3u * (8192u + uint32_t(columns) * 64u) : 16384u + uint32_t(columns) * 128u;
+}
+template <bool F32> __host__ __device__ inline uint32_t few_smem(int columns, int stages, int loads) {
+  return 1024u + uint32_t(stages) * few_stage_bytes<F32>(columns) + (F32 ? uint32_t(loads) * 16384u : 0u) + 32 * TURNED * 4 + (4 * FEW_STAGES + 4) * 8 + 16;
+}
+
+template <int MODE, bool CAPPED, bool F32>
+__global__ void __launch_bounds__(F32 ? 320 : 192, 1) few_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_x, const FewWork f) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t stage_bytes = few_stage_bytes<F32>(f.columns);
+  const uint32_t loads_at = smem_u32(smem), stages_at = loads_at + (F32 ? uint32_t(f.loads) * 16384u : 0u);
+  float* turned = reinterpret_cast<float*>(smem + (stages_at - loads_at) + size_t(f.stages) * stage_bytes);
+  const uint32_t full = smem_u32(turned) + 32 * TURNED * 4, empty = full + FEW_STAGES * 8, loaded = empty + FEW_STAGES * 8, taken = loaded + FEW_STAGES * 8,
+                 acc_full = taken + FEW_STAGES * 8, acc_empty = acc_full + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turned + 32 * TURNED + (4 * FEW_STAGES + 4) * 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Two accumulators, in float32 two parts each: of the products of the first planes, and of the small ones, which would be cut off against it.
+  const uint32_t apart = uint32_t(f.columns + 31) / 32 * 32, both = F32 ? 2 * apart : apart;
+  uint32_t tmem_cols = 32;
+  while (tmem_cols < 2u * both) tmem_cols <<= 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < FEW_STAGES; ++s) {
+      mbar_init(full + s * 8, F32 ? 5 : 1);   // the copies, and four warps' planes
+      mbar_init(empty + s * 8, 1);
+      mbar_init(loaded + s * 8, 1);
+      mbar_init(taken + s * 8, 4);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full + b * 8, 1);
+      mbar_init(acc_empty + b * 8, 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_t) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  const int tiles = (f.n + 127) / 128;
+  constexpr int STEP = F32 ? 32 : 64;   // of k
+  const int n_kb = (f.k + STEP - 1) / STEP;
+  const uint32_t x_bytes = uint32_t(f.columns) * STEP * 2;
+
+  if (warp == 0) {
+    // ---- copies
+    int stage = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      for (int kb = 0; kb < n_kb; ++kb) {
+        // (float32: the table's numbers; the rows' planes come with the table's, below)
+        const uint32_t slot = F32 ? taken : empty;
+        if (!warp_wait(slot + stage * 8, parity ^ 1u)) {
+          if (lane == 0) atomicMax(f.w.error_flag, ERR_EMPTY);
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
+          if constexpr (F32) {
+            mbar_expect_tx(loaded + stage * 8, 16384);
+            load_box(loads_at + stage * 16384, &map_t, kb * STEP, tile * 128, 0, loaded + stage * 8);
+          } else {
+            const uint32_t at = stages_at + stage * stage_bytes, bar = full + stage * 8;
+            mbar_expect_tx(bar, 16384 + x_bytes);
+            load_box(at, &map_t, kb * STEP, tile * 128, 0, bar);
+            load_box(at + 16384, &map_x, kb * STEP, 0, 0, bar);
+          }
+        }
+        __syncwarp();
+        if (++stage == (F32 ? f.loads : f.stages)) {
+          stage = 0;
+          parity ^= 1u;
+        }
+      }
+    }
+    if (!ok) settle(F32 ? loaded : full, F32 ? f.loads : f.stages, stage, parity);
+  } else if (warp == 1) {
+    // ---- products
+    const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(f.columns >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+    int stage = 0;
+    uint32_t parity = 0, local = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++local) {
+      const uint32_t buf = local & 1u;
+      if (!warp_wait(acc_empty + buf * 8, ((local >> 1) & 1u) ^ 1u)) {
+        if (lane == 0) atomicMax(f.w.error_flag, ERR_ACC);
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t acc = tmem + buf * both;
+      for (int kb = 0; kb < n_kb; ++kb) {
+        if (!warp_wait(full + stage * 8, parity)) {
+          if (lane == 0) atomicMax(f.w.error_flag, ERR_FULL);
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (elect_one()) {
+          const uint32_t at = stages_at + stage * stage_bytes;
+          if constexpr (F32) {
+#pragma unroll
+            for (int t = 0; t < 6; ++t) {
+              const uint64_t a = smem_desc_64(at + plane_a(6, t) * 8192), b = smem_desc_64(at + 3 * 8192 + plane_b(6, t) * x_bytes);
+#pragma unroll
+              for (int kk = 0; kk < 2; ++kk)
+                umma_bf16(t < 5 ? acc + apart : acc, a + kk * 2, b + kk * 2, idesc, (kb > 0 || (t > 0 && t < 5) || kk > 0) ? 1u : 0u);
+            }
+          } else {
+            const uint64_t a = smem_desc(at, 16, 1024), b = smem_desc(at + 16384, 16, 1024);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) umma_bf16(acc, a + kk * 2, b + kk * 2, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(empty + stage * 8);
+        }
+        __syncwarp();
+        if (++stage == f.stages) {
+          stage = 0;
+          parity ^= 1u;
+        }
+      }
+      if (elect_one()) umma_commit(acc_full + buf * 8);   // also on the error path: the others go on and the flag tells
+      __syncwarp();
+    }
+  } else if (warp < 6) {
+    // ---- results
+    const int q = warp & 3, part = warp - 2;   // tensor-memory lanes q * 32 ..; behind the turn: 32 tokens (part) of row `lane` of 32
+    const int m = MODE == FACTORS ? *f.w.count : f.rows;
+    const int groups = MODE == FACTORS ? (f.rows + 63) / 64 * 2 : (f.rows + 31) / 32;   // of 32 rows; dz has zeros up to a multiple of 64 rows
+    float top[FEW / 32], sum[FEW / 32];
+#pragma unroll
+    for (int g = 0; g < FEW / 32; ++g) {
+      top[g] = -3.4028234663852886e38f;
+      sum[g] = 0.f;
+    }
+    uint32_t local = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++local) {
+      const uint32_t buf = local & 1u;
+      if (ok && !warp_wait(acc_full + buf * 8, (local >> 1) & 1u)) {
+        if (lane == 0) atomicMax(f.w.error_flag, ERR_ACC);
+        ok = false;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int left = f.n - tile * 128 - part * 32;   // tokens of the thread's 32 that there are
+#pragma unroll
+      for (int g = 0; g < FEW / 32; ++g) {
+        if (g >= groups) break;
+        if (uint32_t(g * 32) < apart) {
+          uint32_t r[32];
+          tmem_load32(tmem + buf * both + uint32_t(g * 32) + (uint32_t(q * 32) << 16), r);
+          if constexpr (F32) {
+            uint32_t small[32];
+            tmem_load32(tmem + buf * both + apart + uint32_t(g * 32) + (uint32_t(q * 32) << 16), small);
+            tmem_load_wait(r);
+            tmem_tie(small);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(small[j]));
+          } else {
+            tmem_load_wait(r);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) turned[j * TURNED + q * 32 + lane] = __uint_as_float(r[j]);
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const int row = g * 32 + lane;
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 x = *reinterpret_cast<const float4*>(turned + lane * TURNED + part * 32 + 4 * i);
+          v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+        }
+        if constexpr (MODE == LOGSUM) {
+          float most = top[g];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = log2_units<CAPPED>(v[j], f.w);
+          if (left < 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = j < left ? v[j] : -INFINITY;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) most = max3(most, v[j], v[j + 1]);
+          float s0 = sum[g] * fast_exp2(top[g] - most), s1 = 0.f;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            s0 += fast_exp2(v[j] - most);
+            s1 += fast_exp2(v[j + 1] - most);
+          }
+          sum[g] = s0 + s1;
+          top[g] = most;
+        } else {
+          int target = -1;
+          float factor = 0.f, size = 0.f, less2 = 0.f;
+          const int token0 = tile * 128 + part * 32;
+          if (row < m) {
+            target = f.w.targets[row] - f.w.first - token0;
+            factor = f.w.factor[row];
+            size = fabsf(factor);
+            less2 = f.w.log_sum[row] * LOG2E - log2f(size);
+          }
+          const bool learns = target >= 0 && target < 32;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if constexpr (CAPPED) {
+              const float h = fast_rcp(fast_exp2(v[j] * f.w.cap_in) + 1.f);
+              v[j] = fast_exp2(fmaf(-2.f * f.w.cap_out, h, f.w.cap_out) - less2);
+              if (learns) v[j] -= target == j ? size : 0.f;
+              v[j] *= 4.f * h * (1.f - h);
+            } else {
+              v[j] = fast_exp2(fmaf(v[j], LOG2E, -less2));
+              if (learns) v[j] -= target == j ? size : 0.f;
+            }
+          }
+          const uint32_t sign = factor < 0.f ? 0x80008000u : 0u, held = row < m ? 0xffffffffu : 0u;
+          if (left > 0 && ok) {
+            bf16* to = f.dz + row * f.ld + token0;
+            for (int plane = 0; plane < (F32 ? 3 : 1); ++plane) {
+#pragma unroll
+              for (int p = 0; p < 4; ++p) {
+                uint32_t r[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[j] = pack_bf16(v[8 * p + 2 * j], v[8 * p + 2 * j + 1]);
+                *reinterpret_cast<uint4*>(to + plane * f.dz_plane + 8 * p) =
+                    make_uint4((r[0] & held) ^ sign, (r[1] & held) ^ sign, (r[2] & held) ^ sign, (r[3] & held) ^ sign);
+                if constexpr (F32) {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    v[8 * p + 2 * j] -= __uint_as_float(r[j] << 16);
+                    v[8 * p + 2 * j + 1] -= __uint_as_float(r[j] & 0xffff0000u);
+                  }
+                }
+              }
+            }
+          }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");   // (the turned tile is read)
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty + buf * 8);
+    }
+    if constexpr (MODE == LOGSUM) {
+#pragma unroll
+      for (int g = 0; g < FEW / 32; ++g) {
+        const int row = g * 32 + lane;
+        if (row < m) f.w.part[(size_t(blockIdx.x) * 4 + part) * m + row] = ok ? make_float2(top[g], sum[g]) : make_float2(NAN, NAN);
+      }
+    }
+  } else if constexpr (F32) {
+    // ---- planes: a thread a token's 32 numbers
+    const int row = (warp - 6) * 32 + lane;
+    int stage = 0, load = 0;
+    uint32_t parity = 0, load_parity = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      for (int kb = 0; kb < n_kb; ++kb) {
+        if (!warp_wait(loaded + load * 8, load_parity)) {
+          if (lane == 0) atomicMax(f.w.error_flag, ERR_FULL);
+          ok = false;
+          break;
+        }
+        const uint8_t* from = smem + load * 16384 + row * 128;
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 x = *reinterpret_cast<const float4*>(from + ((j ^ (row & 7)) << 4));
+          v[4 * j] = x.x, v[4 * j + 1] = x.y, v[4 * j + 2] = x.z, v[4 * j + 3] = x.w;
+        }
+        if (!warp_wait(empty + stage * 8, parity ^ 1u)) {
+          if (lane == 0) atomicMax(f.w.error_flag, ERR_EMPTY);
+          ok = false;
+          break;
+        }
+        if (warp == 6 && elect_one()) {
+          mbar_expect_tx(full + stage * 8, 3 * x_bytes);
+          for (int p = 0; p < 3; ++p) load_box(stages_at + stage * stage_bytes + 3 * 8192 + p * x_bytes, &map_x, kb * STEP, 0, p, full + stage * 8);
+        }
+        __syncwarp();
+        const uint32_t to = stages_at + stage * stage_bytes + row * 64;
+        const float most = 3.3895313892515355e38f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (fabsf(v[j]) > most) v[j] = copysignf(most, v[j]);   // (as split3)
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              r[j] = pack_bf16(v[8 * c + 2 * j], v[8 * c + 2 * j + 1]);
+              if (p < 2) {
+                v[8 * c + 2 * j] -= __uint_as_float(r[j] << 16);
+                v[8 * c + 2 * j + 1] -= __uint_as_float(r[j] & 0xffff0000u);
+              }
+            }
+            st_shared16(to + p * 8192 + ((c ^ ((row >> 1) & 3)) << 4), r[0], r[1], r[2], r[3]);
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(full + stage * 8);
+          mbar_arrive(taken + load * 8);   // (here, where the numbers have been used: handed back right behind the loads, the next copy has overtaken them)
+        }
+        if (++load == f.loads) {
+          load = 0;
+          load_parity ^= 1u;
+        }
+        if (++stage == f.stages) {
+          stage = 0;
+          parity ^= 1u;
+        }
+      }
+    }
+    if (!ok && warp == 6) settle(full, f.stages, stage, parity);
+  }
+
+  pdl_launch_dependents();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
   }
 }
 
@@ -695,12 +1077,12 @@ struct Operand {
 };
 
 bool encode(CUtensorMap* map, CUtensorMapDataType type, int size, const void* at, long long inner, long long outer, long long planes, long long ld, long long plane, int box_inner,
-            int box_outer) {
+            int box_outer, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   const r2::EncodeTiledFn fn = r2::encode_fn();
   cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(outer), cuuint64_t(planes)};
   cuuint64_t strides[2] = {cuuint64_t(ld) * size, cuuint64_t(planes > 1 ? plane : ld) * size};
   cuuint32_t box[3] = {cuuint32_t(box_inner), cuuint32_t(box_outer), 1}, steps[3] = {1, 1, 1};
-  return fn != nullptr && fn(map, type, 3, const_cast<void*>(at), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  return fn != nullptr && fn(map, type, 3, const_cast<void*>(at), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -774,6 +1156,52 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, 
   return launch<MODE, false, T>(ma, mb, mo, w, units, stream);
 }
 
+int n_sms() {
+  static std::atomic<int> cached[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64 && (n = cached[dev].load()) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = 148;
+  }
+  if (dev < 64) cached[dev].store(n);
+  return n;
+}
+
+int few_ctas(long long vocab) {
+  const long long tiles = (vocab + 127) / 128;
+  return int(tiles < n_sms() ? tiles : n_sms());
+}
+
+template <int MODE, bool CAPPED, bool F32>
+int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, FewWork f, cudaStream_t stream) {
+  constexpr uint32_t most = 227 * 1024;
+  auto kernel = few_kernel<MODE, CAPPED, F32>;
+  static std::atomic<bool> done[64];
+  const int status = allow_smem(kernel, most, done);
+  if (status != R2_OK) return status;
+  f.stages = F32 ? 3 : FEW_STAGES;   // (float32: two stages fill while one is read; the rest of the memory keeps the table coming)
+  f.loads = F32 ? FEW_STAGES : 0;
+  while (f.loads > 2 && few_smem<F32>(f.columns, f.stages, f.loads) > most) --f.loads;
+  while (f.stages > 2 && few_smem<F32>(f.columns, f.stages, f.loads) > most) --f.stages;
+  r2_launch(kernel, dim3(few_ctas(f.n)), dim3(F32 ? 320 : 192), size_t(few_smem<F32>(f.columns, f.stages, f.loads)), stream, mt, mx, f);
+  return launch_status();
+}
+
+template <int MODE, bool F32> int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, const FewWork& f, bool capped, cudaStream_t stream) {
+  return capped ? launch_few<MODE, true, F32>(mt, mx, f, stream) : launch_few<MODE, false, F32>(mt, mx, f, stream);
+}
+
+// Both operands' maps for few rows: the table [vocab, width] as it lies, the rows in planes.
+template <typename T> bool make_few_maps(CUtensorMap* mt, CUtensorMap* mx, const void* table, long long ld_t, long long vocab, const Operand& x, long long width, long long rows,
+                                         int columns) {
+  constexpr bool F32 = sizeof(T) == 4;
+  return encode(mt, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, int(sizeof(T)), table, width, vocab, 1, ld_t, 0, 128 / int(sizeof(T)), 128) &&
+         encode(mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x.at, width, rows, x.planes, x.ld, x.plane, F32 ? 32 : 64, columns,
+                F32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 int row_blocks(long long rows) { return int(rows < 8 * 4736 ? (rows + 7) / 8 : 4736); }
 
 // What a call's scratch holds, in bytes from its start.
@@ -784,6 +1212,7 @@ struct Layout {
   long long rows_up, width_up;      // rows to a multiple of 256, numbers to one of 8
   int pieces, splits, per_split;
   long long piece;                  // tokens at a time, a multiple of 256
+  long long parts;
   long long table, hidden, part, factors, shares, targets, factor, sums, place, count, total;
 };
 
@@ -803,7 +1232,9 @@ Layout layout(int dtype, long long rows, long long width, long long vocab, bool 
   l.table = take(l.planes * vocab * l.width_up * 2);
   l.hidden = take(l.planes * l.rows_up * l.width_up * 2);
   if (!gradient) {
-    l.part = take(up(vocab, BN) / BN * 2 * rows * 8);
+    l.parts = rows <= FEW ? few_ctas(vocab) * 4 : up(vocab, BN) / BN * 2;
+    if (l.parts < up(vocab, BN) / BN * 2) l.parts = up(vocab, BN) / BN * 2;   // (whichever kernel it is)
+    l.part = take(l.parts * rows * 8);
   } else {
     long long most = FACTOR_BYTES / (l.rows_up * 2 * l.planes) / BN * BN;
     if (most < BN) most = BN;
@@ -817,6 +1248,7 @@ Layout layout(int dtype, long long rows, long long width, long long vocab, bool 
     double best = -1;
     for (int s = 1; s <= 64 && (s == 1 || n_kb / s >= 8); ++s) {
       const int per = (n_kb + s - 1) / s;
+      if (l.planes > 1 && per > 64 && n_kb / (s + 1) >= 8 && s < 64) continue;   // (float32: no more than 256 additions to an accumulator)
       const double rounds = double((tiles * s + pairs - 1) / pairs), steps = per * l.planes * (l.planes + 1) / 2 + 8;
       const double cost = l.pieces * rounds * steps + double(s) * tiles * 0.14 * (l.pieces + 1);
       if (best < 0 || cost < best) {
@@ -837,8 +1269,8 @@ Layout layout(int dtype, long long rows, long long width, long long vocab, bool 
   return l;
 }
 
-bool copies_read(const void* at, long long ld, long long rows, long long width) {
-  return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (rows <= 1 || (ld % 8 == 0 && ld >= width));
+bool copies_read(const void* at, long long ld, long long rows, long long width, int size = 2) {
+  return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (rows <= 1 || (ld * size % 16 == 0 && ld >= width));
 }
 
 // The matrix itself where tensor copies can read it, else planes of it in `space`.
@@ -862,21 +1294,40 @@ int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_
             float softcap, float* loss, float* log_sum, char* space, int* error, cudaStream_t stream) {
   const Layout l = layout(sizeof(T) == 4 ? R2_F32 : R2_BF16, rows, width, vocab, false);
   const Operand x = operand<T>(hidden, ld_h, rows, width, l, space + l.hidden, stream);
-  const Operand t = operand<T>(table, ld_t, vocab, width, l, space + l.table, stream);
-  CUtensorMap ma, mb;
-  if (!make_map(&ma, x, width, rows, BM) || !make_map(&mb, t, width, vocab, HALF)) return R2_BAD_ALIGN;
   Work w = {};
-  w.m = rows;
-  w.n = vocab;
-  w.k = width;
-  w.terms = l.planes * (l.planes + 1) / 2;
   w.part = reinterpret_cast<float2*>(space + l.part);
   w.error_flag = error;
   set_cap(w, softcap);
-  const long long tiles = (l.rows_up / 256) * (up(vocab, BN) / BN);
-  const int status = launch<LOGSUM, bf16>(ma, mb, ma, w, tiles, softcap > 0.f, stream);
+  CUtensorMap ma, mb;
+  int status, parts;
+  if (rows <= FEW && (sizeof(T) == 2 || copies_read(table, ld_t, vocab, width, 4))) {
+    const void* at = table;
+    long long ld = vocab > 1 ? ld_t : l.width_up;
+    if (sizeof(T) == 2) {
+      const Operand t = operand<T>(table, ld_t, vocab, width, l, space + l.table, stream);
+      at = t.at;
+      ld = t.ld;
+    }
+    FewWork f = {};
+    f.rows = rows;
+    f.columns = (rows + 15) / 16 * 16;
+    f.n = vocab;
+    f.k = width;
+    f.w = w;
+    if (!make_few_maps<T>(&mb, &ma, at, ld, vocab, x, width, rows, f.columns)) return R2_BAD_ALIGN;
+    status = launch_few<LOGSUM, sizeof(T) == 4>(mb, ma, f, softcap > 0.f, stream);
+    parts = few_ctas(vocab) * 4;
+  } else {
+    const Operand t = operand<T>(table, ld_t, vocab, width, l, space + l.table, stream);
+    if (!make_map(&ma, x, width, rows, BM) || !make_map(&mb, t, width, vocab, HALF)) return R2_BAD_ALIGN;
+    w.m = rows;
+    w.n = vocab;
+    w.k = width;
+    w.terms = l.planes * (l.planes + 1) / 2;
+    status = launch<LOGSUM, bf16>(ma, mb, ma, w, (l.rows_up / 256) * (up(vocab, BN) / BN), softcap > 0.f, stream);
+    parts = int(up(vocab, BN) / BN) * 2;
+  }
   if (status != R2_OK) return status;
-  const int parts = int(up(vocab, BN) / BN) * 2;
   const T *h = static_cast<const T*>(hidden), *tab = static_cast<const T*>(table);
   r2_launch(finish_kernel<T>, dim3((rows + 7) / 8), dim3(256), size_t(0), stream, static_cast<const float2*>(w.part), parts, h, ld_h, tab, ld_t, targets, weight, rows, width, vocab, softcap, loss, log_sum);
   return launch_status();
@@ -886,7 +1337,9 @@ template <typename T>
 int gradient_of(const void* hidden, long long ld_h, const void* table, long long ld_t, int rows, int width, int vocab, const int32_t* targets, const float* weight,
                 const float* log_sum, float softcap, void* d_hidden, long long ld_dh, void* d_table, long long ld_dt, char* space, int* error, cudaStream_t stream) {
   const Layout l = layout(sizeof(T) == 4 ? R2_F32 : R2_BF16, rows, width, vocab, true);
-  const Operand t = operand<T>(table, ld_t, vocab, width, l, space + l.table, stream);
+  const bool few = rows <= FEW && (sizeof(T) == 2 || copies_read(table, ld_t, vocab, width, 4));
+  Operand t = {};   // (few float32 rows read the table as it is for their factors)
+  if (!few || sizeof(T) == 2 || d_hidden) t = operand<T>(table, ld_t, vocab, width, l, space + l.table, stream);
   bf16* gathered = reinterpret_cast<bf16*>(space + l.hidden);
   const Operand x = {gathered, l.width_up, l.rows_up * l.width_up, l.planes};
   int* count = reinterpret_cast<int*>(space + l.count);
@@ -917,10 +1370,26 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
     w.first = int(first);
     w.n = n;
     w.k = width;
-    if (!make_map(&ma, x, width, l.rows_up, BM) || !make_map(&mb, part, width, n, HALF) ||
-        !make_out_map<bf16>(&mo, dz.at, l.piece, l.rows_up, l.planes, l.piece, dz.plane))
-      return R2_BAD_ALIGN;
-    status = launch<FACTORS, bf16>(ma, mb, mo, w, row_tiles * (up(n, BN) / BN), softcap > 0.f, stream);
+    if (few) {
+      FewWork f = {};
+      f.rows = rows;
+      f.columns = (rows + 15) / 16 * 16;
+      f.n = n;
+      f.k = width;
+      f.w = w;
+      f.dz = reinterpret_cast<bf16*>(space + l.factors);
+      f.dz_plane = dz.plane;
+      f.ld = l.piece;
+      const void* at = sizeof(T) == 2 ? part.at : static_cast<const T*>(table) + first * ld_t;
+      const long long ld = sizeof(T) == 2 ? part.ld : n > 1 ? ld_t : l.width_up;
+      if (!make_few_maps<T>(&mb, &ma, at, ld, n, x, width, l.rows_up, f.columns)) return R2_BAD_ALIGN;
+      status = launch_few<FACTORS, sizeof(T) == 4>(mb, ma, f, softcap > 0.f, stream);
+    } else {
+      if (!make_map(&ma, x, width, l.rows_up, BM) || !make_map(&mb, part, width, n, HALF) ||
+          !make_out_map<bf16>(&mo, dz.at, l.piece, l.rows_up, l.planes, l.piece, dz.plane))
+        return R2_BAD_ALIGN;
+      status = launch<FACTORS, bf16>(ma, mb, mo, w, row_tiles * (up(n, BN) / BN), softcap > 0.f, stream);
+    }
     if (status == R2_OK && d_hidden) {
       Work d = w;
       d.n = width;
