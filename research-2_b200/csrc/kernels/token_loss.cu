@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
 // ---- few rows: LOGSUM and FACTORS of up to 128 ----------------------------------------------
 //
 // The pass over the table is what such a call costs, so the operands change sides: a tile is 128 tokens of the vocabulary by all rows (up to 128 columns of the
-// accumulator), one CTA to an SM, and float32 tables are read as they are: four warps turn each 128 x 32 numbers into the three planes in shared memory, where
+// accumulator), one CTA to an SM, and float32 tables are read as they are: eight warps turn each 128 x 32 numbers into the three planes in shared memory, where
 // the others' planes would have been written to memory and read again (six bytes a number, twice). A tile's results go through shared memory, 32
 // rows of the batch at a time, so that a thread has 32 tokens of one row: sums over them need no exchange, and dz leaves in pieces of 64 bytes.
 //
@@ -518,7 +518,7 @@ template <bool F32> __host__ __device__ inline uint32_t few_smem(int columns, in
 }
 
 template <int MODE, bool CAPPED, bool F32>
-__global__ void __launch_bounds__(F32 ? 320 : 192, 1) few_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_x, const FewWork f) {
+__global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_x, const FewWork f) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t stage_bytes = few_stage_bytes<F32>(f.columns);
@@ -768,73 +768,69 @@ __global__ void __launch_bounds__(F32 ? 320 : 192, 1) few_kernel(const __grid_co
       }
     }
   } else if constexpr (F32) {
-    // ---- planes: a thread a token's 32 numbers
-    const int row = (warp - 6) * 32 + lane;
-    int stage = 0, load = 0;
+    // ---- planes: a thread a token's 32 numbers; two groups of four warps take the steps in turn (what a step takes is a chain: half as long, each, it was no faster)
+    const int group = (warp - 6) / 4, row = (warp - 6) % 4 * 32 + lane;
+    const int steps = (tiles - int(blockIdx.x) + int(gridDim.x) - 1) / int(gridDim.x) * n_kb;   // of all this CTA's tiles
+    int stage = 0, load = 0, kb = 0;
     uint32_t parity = 0, load_parity = 0;
+    auto forward = [&](int n) {
+      kb = (kb + n) % n_kb;
+      for (stage += n; stage >= f.stages; stage -= f.stages) parity ^= 1u;
+      for (load += n; load >= f.loads; load -= f.loads) load_parity ^= 1u;
+    };
+    forward(group);
     bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-      for (int kb = 0; kb < n_kb; ++kb) {
-        if (!warp_wait(loaded + load * 8, load_parity)) {
-          if (lane == 0) atomicMax(f.w.error_flag, ERR_FULL);
-          ok = false;
-          break;
-        }
-        const uint8_t* from = smem + load * 16384 + row * 128;
-        float v[32];
+    for (int i = group; i < steps; i += 2, forward(2)) {
+      if (!warp_wait(loaded + load * 8, load_parity)) {
+        if (lane == 0) atomicMax(f.w.error_flag, ERR_FULL);
+        ok = false;
+        break;
+      }
+      const uint8_t* from = smem + load * 16384 + row * 128;
+      float v[32];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float4 x = *reinterpret_cast<const float4*>(from + ((j ^ (row & 7)) << 4));
-          v[4 * j] = x.x, v[4 * j + 1] = x.y, v[4 * j + 2] = x.z, v[4 * j + 3] = x.w;
-        }
-        if (!warp_wait(empty + stage * 8, parity ^ 1u)) {
-          if (lane == 0) atomicMax(f.w.error_flag, ERR_EMPTY);
-          ok = false;
-          break;
-        }
-        if (warp == 6 && elect_one()) {
-          mbar_expect_tx(full + stage * 8, 3 * x_bytes);
-          for (int p = 0; p < 3; ++p) load_box(stages_at + stage * stage_bytes + 3 * 8192 + p * x_bytes, &map_x, kb * STEP, 0, p, full + stage * 8);
-        }
-        __syncwarp();
-        const uint32_t to = stages_at + stage * stage_bytes + row * 64;
-        const float most = 3.3895313892515355e38f;
+      for (int j = 0; j < 8; ++j) {
+        const float4 x = *reinterpret_cast<const float4*>(from + ((j ^ (row & 7)) << 4));
+        v[4 * j] = x.x, v[4 * j + 1] = x.y, v[4 * j + 2] = x.z, v[4 * j + 3] = x.w;
+      }
+      if (!warp_wait(empty + stage * 8, parity ^ 1u)) {
+        if (lane == 0) atomicMax(f.w.error_flag, ERR_EMPTY);
+        ok = false;
+        break;
+      }
+      if (warp == 6 + 4 * group && elect_one()) {
+        mbar_expect_tx(full + stage * 8, 3 * x_bytes);
+        for (int p = 0; p < 3; ++p) load_box(stages_at + stage * stage_bytes + 3 * 8192 + p * x_bytes, &map_x, kb * STEP, 0, p, full + stage * 8);
+      }
+      __syncwarp();
+      const uint32_t to = stages_at + stage * stage_bytes + row * 64;
+      const float most = 3.3895313892515355e38f;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (fabsf(v[j]) > most) v[j] = copysignf(most, v[j]);   // (as split3)
+      for (int j = 0; j < 32; ++j) asm("min.NaN.f32 %0, %0, %1;\n\tmax.NaN.f32 %0, %0, %2;" : "+f"(v[j]) : "f"(most), "f"(-most));   // (as split3)
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
+      for (int p = 0; p < 3; ++p) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t r[4];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t r[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              r[j] = pack_bf16(v[8 * c + 2 * j], v[8 * c + 2 * j + 1]);
-              if (p < 2) {
-                v[8 * c + 2 * j] -= __uint_as_float(r[j] << 16);
-                v[8 * c + 2 * j + 1] -= __uint_as_float(r[j] & 0xffff0000u);
-              }
+          for (int j = 0; j < 4; ++j) {
+            r[j] = pack_bf16(v[8 * c + 2 * j], v[8 * c + 2 * j + 1]);
+            if (p < 2) {
+              v[8 * c + 2 * j] -= __uint_as_float(r[j] << 16);
+              v[8 * c + 2 * j + 1] -= __uint_as_float(r[j] & 0xffff0000u);
             }
-            st_shared16(to + p * 8192 + ((c ^ ((row >> 1) & 3)) << 4), r[0], r[1], r[2], r[3]);
           }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(full + stage * 8);
-          mbar_arrive(taken + load * 8);   // (here, where the numbers have been used: handed back right behind the loads, the next copy has overtaken them)
-        }
-        if (++load == f.loads) {
-          load = 0;
-          load_parity ^= 1u;
-        }
-        if (++stage == f.stages) {
-          stage = 0;
-          parity ^= 1u;
+          st_shared16(to + p * 8192 + ((c ^ ((row >> 1) & 3)) << 4), r[0], r[1], r[2], r[3]);
         }
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(full + stage * 8);
+        mbar_arrive(taken + load * 8);   // (here, where the numbers have been used: handed back right behind the loads, the next copy has overtaken them)
+      }
     }
-    if (!ok && warp == 6) settle(full, f.stages, stage, parity);
+    if (!ok && warp == 6 + 4 * group) settle(full, f.stages, stage, parity);
   }
 
   pdl_launch_dependents();
@@ -1185,7 +1181,7 @@ int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, FewWork f, cudaStre
   f.loads = F32 ? FEW_STAGES : 0;
   while (f.loads > 2 && few_smem<F32>(f.columns, f.stages, f.loads) > most) --f.loads;
   while (f.stages > 2 && few_smem<F32>(f.columns, f.stages, f.loads) > most) --f.stages;
-  r2_launch(kernel, dim3(few_ctas(f.n)), dim3(F32 ? 320 : 192), size_t(few_smem<F32>(f.columns, f.stages, f.loads)), stream, mt, mx, f);
+  r2_launch(kernel, dim3(few_ctas(f.n)), dim3(F32 ? 448 : 192), size_t(few_smem<F32>(f.columns, f.stages, f.loads)), stream, mt, mx, f);
   return launch_status();
 }
 
@@ -1243,13 +1239,14 @@ Layout layout(int dtype, long long rows, long long width, long long vocab, bool 
     const int n_kb = int((l.piece + BK - 1) / BK);
     const long long tiles = l.rows_up / 256 * (up(width, BN) / BN);
     const int pairs = resident_pairs();
+    const int terms = l.planes * (l.planes + 1) / 2;
     // shares of k, of no fewer than eight steps: more of them fill the last round of pairs, and each is written for every piece and read once more (a tile's
     // 256 KB take a seventh of a step's time, a step of 64 being 0.29 us on a pair)
     double best = -1;
-    for (int s = 1; s <= 64 && (s == 1 || n_kb / s >= 8); ++s) {
+    for (int s = 1; s <= 64 && (s == 1 || n_kb * terms / s >= 8); ++s) {
       const int per = (n_kb + s - 1) / s;
-      if (l.planes > 1 && per > 64 && n_kb / (s + 1) >= 8 && s < 64) continue;   // (float32: no more than 256 additions to an accumulator)
-      const double rounds = double((tiles * s + pairs - 1) / pairs), steps = per * l.planes * (l.planes + 1) / 2 + 8;
+      if (terms > 1 && per > 64 && s < 64) continue;   // (float32: no more than 256 additions to an accumulator)
+      const double rounds = double((tiles * s + pairs - 1) / pairs), steps = per * terms + 8;
       const double cost = l.pieces * rounds * steps + double(s) * tiles * 0.14 * (l.pieces + 1);
       if (best < 0 || cost < best) {
         best = cost;
