@@ -1206,7 +1206,7 @@ constexpr long long FACTOR_BYTES = 256ll << 20;   // of dz at a time
 struct Layout {
   int size, planes;                 // of a number; bfloat16 planes of an operand
   long long rows_up, width_up;      // rows to a multiple of 256, numbers to one of 8
-  int pieces, splits, per_split;
+  int pieces, splits;
   long long piece;                  // tokens at a time, a multiple of 256
   long long parts;
   long long table, hidden, part, factors, shares, targets, factor, sums, place, count, total;
@@ -1232,25 +1232,35 @@ Layout layout(int dtype, long long rows, long long width, long long vocab, bool 
     if (l.parts < up(vocab, BN) / BN * 2) l.parts = up(vocab, BN) / BN * 2;   // (whichever kernel it is)
     l.part = take(l.parts * rows * 8);
   } else {
-    long long most = FACTOR_BYTES / (l.rows_up * 2 * l.planes) / BN * BN;
-    if (most < BN) most = BN;
-    l.pieces = int((vocab + most - 1) / most);
-    l.piece = up((vocab + l.pieces - 1) / l.pieces, BN);
+    const int pairs = resident_pairs(), terms = l.planes * (l.planes + 1) / 2;
+    const long long row_tiles = l.rows_up / 256, width_tiles = up(width, BN) / BN, tiles = row_tiles * width_tiles, all = up(vocab, BN) / BN;
+    // tokens at a time: as few rounds of the pairs as can be in all pieces' FACTORS and TABLE (a piece of as many tiles as there are pairs leaves none of them idle)
+    long long most = FACTOR_BYTES / (l.rows_up * 2 * l.planes) / BN, piece = 1;
+    most = most < 1 ? 1 : most > all ? all : most;
+    auto rounds = [&](long long n) {   // of a piece of n tiles, in steps of k; and its launches
+      return double((n * row_tiles + pairs - 1) / pairs) * (up(width, BK) / BK * terms + 2) + double((n * width_tiles + pairs - 1) / pairs) * (l.rows_up / BK * terms + 2) + 40;
+    };
+    double least = -1;
+    for (long long p = most; p >= 1 && p >= most / 2; --p) {
+      const double cost = double(all / p) * rounds(p) + (all % p ? rounds(all % p) : 0);
+      if (least < 0 || cost < least) {
+        least = cost;
+        piece = p;
+      }
+    }
+    l.piece = piece * BN;
+    l.pieces = int((all + piece - 1) / piece);
     const int n_kb = int((l.piece + BK - 1) / BK);
-    const long long tiles = l.rows_up / 256 * (up(width, BN) / BN);
-    const int pairs = resident_pairs();
-    const int terms = l.planes * (l.planes + 1) / 2;
     // shares of k, of no fewer than eight steps: more of them fill the last round of pairs, and each is written for every piece and read once more (a tile's
     // 256 KB take a seventh of a step's time, a step of 64 being 0.29 us on a pair)
     double best = -1;
     for (int s = 1; s <= 64 && (s == 1 || n_kb * terms / s >= 8); ++s) {
       const int per = (n_kb + s - 1) / s;
       if (terms > 1 && per > 64 && s < 64) continue;   // (float32: no more than 256 additions to an accumulator)
-      const double rounds = double((tiles * s + pairs - 1) / pairs), steps = per * terms + 8;
-      const double cost = l.pieces * rounds * steps + double(s) * tiles * 0.14 * (l.pieces + 1);
+      const double steps = per * terms + 8;
+      const double cost = l.pieces * double((tiles * s + pairs - 1) / pairs) * steps + double(s) * tiles * 0.14 * (l.pieces + 1);
       if (best < 0 || cost < best) {
         best = cost;
-        l.per_split = per;
         l.splits = (n_kb + per - 1) / per;
       }
     }
@@ -1391,7 +1401,7 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
       Work d = w;
       d.n = width;
       d.k = n;
-      d.per_split = l.per_split;
+      d.per_split = ((n + BK - 1) / BK + l.splits - 1) / l.splits;   // (the last piece is shorter)
       d.splits = l.splits;
       d.add = first > 0;
       if (!make_map(&ma, dz, n, l.rows_up, BM) || !make_map(&mb, part, width, n, BK) ||
