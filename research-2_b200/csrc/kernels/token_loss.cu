@@ -55,7 +55,7 @@ struct Work {
   int terms;                 // 1, or 6 for operands in three planes
   int splits, per_split;     // ROWS: shares of k, in steps of BK
   int add;                   // ROWS: to what earlier pieces left
-  float cap_in, cap_out;     // c > 0: z * log2 e = cap_out * tanh(u / c) with cap_in = 2 log2 e / c, cap_out = c log2 e; else 0
+  float cap, cap_out;        // c > 0: 1 / c and c log2 e, so that z log2 e = cap_out tanh(cap u); else 0
   const int32_t* targets;    // FACTORS: of the gathered rows, with their factors and sums
   const float* factor;
   const float* log_sum;
@@ -131,11 +131,21 @@ __device__ __forceinline__ void split3(float x, bf16 (&p)[3]) {
   p[2] = __float2bfloat16_rn(rest);
 }
 
-// z log2 e of an accumulator: for capped logits c log2 e (1 - 2 / (e^(2 u / c) + 1)), whose error is some units of c.
+// tanh(x) and 1 - tanh(x)^2: 1 - 2 h with h = 1 / (e^(2 x) + 1), and 4 h (1 - h); near 0, where the difference would cancel, the odd series up to
+// x^7 (its next term is below 6e-8 of it). Either is off by less than 1e-6 of itself, so that a cap far above the logits leaves them as they are.
+__device__ __forceinline__ float cap_tanh(float x, float& slope) {
+  const float h = fast_rcp(fast_exp2(x * (2.f * LOG2E)) + 1.f), q = x * x;
+  const float series = fmaf(x * q, fmaf(q, fmaf(q, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), x);
+  const bool near = q < 0.04f;
+  slope = near ? fmaf(-series, series, 1.f) : 4.f * h * (1.f - h);
+  return near ? series : fmaf(-2.f, h, 1.f);
+}
+
+// z log2 e of an accumulator.
 template <bool CAPPED> __device__ __forceinline__ float log2_units(float u, const Work& w) {
   if constexpr (!CAPPED) return u * LOG2E;
-  const float r = fast_rcp(fast_exp2(u * w.cap_in) + 1.f);
-  return fmaf(-2.f * w.cap_out, r, w.cap_out);
+  float slope;
+  return w.cap_out * cap_tanh(u * w.cap, slope);
 }
 
 struct Unit {   // one tile, or one share of its k
@@ -396,10 +406,10 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
           if constexpr (CAPPED) {
 #pragma unroll
             for (int j = 0; j < 64; ++j) {
-              const float h = fast_rcp(fast_exp2(v[j] * w.cap_in) + 1.f);   // (1 - tanh) / 2; the slope 1 - tanh^2 is 4 h (1 - h)
-              v[j] = fast_exp2(fmaf(-2.f * w.cap_out, h, w.cap_out) - less2);
+              float slope;
+              v[j] = fast_exp2(fmaf(w.cap_out, cap_tanh(v[j] * w.cap, slope), -less2));
               if (learns) v[j] -= target == c + j ? size : 0.f;
-              v[j] *= 4.f * h * (1.f - h);
+              v[j] *= slope;
             }
           } else {
 #pragma unroll
@@ -489,7 +499,7 @@ struct FewWork {
   int rows, columns;                // of the batch; a multiple of 16: columns of the accumulator
   int n, k;                         // tokens (of the table, or of a piece); width
   int stages, loads;                // of operands; float32: of operands in planes, of the table's numbers
-  Work w;                           // count, cap_in, cap_out, targets, factor, log_sum, first, part, error_flag as above
+  Work w;                           // count, cap, cap_out, targets, factor, log_sum, first, part, error_flag as above
   bf16* dz;
   long long dz_plane, ld;
 };
@@ -723,10 +733,10 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             if constexpr (CAPPED) {
-              const float h = fast_rcp(fast_exp2(v[j] * f.w.cap_in) + 1.f);
-              v[j] = fast_exp2(fmaf(-2.f * f.w.cap_out, h, f.w.cap_out) - less2);
+              float slope;
+              v[j] = fast_exp2(fmaf(f.w.cap_out, cap_tanh(v[j] * f.w.cap, slope), -less2));
               if (learns) v[j] -= target == j ? size : 0.f;
-              v[j] *= 4.f * h * (1.f - h);
+              v[j] *= slope;
             } else {
               v[j] = fast_exp2(fmaf(v[j], LOG2E, -less2));
               if (learns) v[j] -= target == j ? size : 0.f;
@@ -1291,7 +1301,7 @@ Operand operand(const void* at, long long ld, long long rows, long long width, c
 
 void set_cap(Work& w, float softcap) {
   if (softcap > 0.f) {
-    w.cap_in = 2.f * LOG2E / softcap;
+    w.cap = 1.f / softcap;
     w.cap_out = softcap * LOG2E;
   }
 }

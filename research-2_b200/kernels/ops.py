@@ -2276,8 +2276,8 @@ def _loss_arguments(hidden, table, targets, weight, softcap, what):
     targets_at = _per_row(targets, "targets", torch.int32, rows, device)
     weight_at = _per_row(weight, "weight", torch.float32, rows, device)
     softcap = float(softcap)
-    if not 0.0 <= softcap < float("inf"):
-        raise KernelError(f"{what}: softcap must be finite and not negative, got {softcap}")
+    if softcap != 0.0 and not 1e-6 <= softcap <= 1e30:
+        raise KernelError(f"{what}: softcap must be 0 or in [1e-6, 1e30], got {softcap}")
     return code, rows, width, ld, vocab, table_ld, device, targets_at, weight_at, softcap
 
 

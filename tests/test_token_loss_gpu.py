@@ -370,7 +370,7 @@ def test_refusals():
     for bad in (dict(hidden=x.cpu()), dict(hidden=x[0]), dict(hidden=x.half()), dict(hidden=x.bfloat16()), dict(table=w[:, :8]), dict(table=w.t().contiguous().t()),
                 dict(hidden=x.t().contiguous().t()), dict(table=w[:0]), dict(targets=y.long()), dict(targets=y[:3]), dict(targets=y.cpu()),
                 dict(targets=torch.zeros(8, dtype=torch.int32, device=DEV)[::2]), dict(weight=s.double()), dict(weight=s[:2]), dict(softcap=-1.0),
-                dict(softcap=math.nan), dict(softcap=math.inf), dict(hidden=x[:, :0], table=w[:, :0])):
+                dict(softcap=math.nan), dict(softcap=math.inf), dict(softcap=1e-7), dict(softcap=1e31), dict(hidden=x[:, :0], table=w[:, :0])):
         call = dict(hidden=x, table=w, targets=y, weight=None, softcap=0.0)
         call.update(bad)
         args = [call.pop(n) for n in ("hidden", "table", "targets")]
@@ -397,3 +397,68 @@ def test_rows_without_a_target_beside_a_table_with_infinities(dtype):
     assert torch.all((loss.double() - keep.loss).abs() <= keep.loss_off)
     assert torch.isfinite(d_table).all() and not d_table[500:].any() and not d_hidden[70:].any()
     assert torch.all((d_table[:500].double() - keep.d_table).abs() <= keep.d_table_off)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [20, 200])
+@pytest.mark.parametrize("softcap", [1e4, 1e8, 1e30])
+def test_a_cap_far_above_the_logits_changes_nothing(dtype, rows, softcap):
+    # |logits| below 40: their cube over 3 cap^2 is below 3e-4; the tanh is off by 2e-6 of itself at most, as much again in the slope
+    c = Case(rows, 96, 700, dtype, 29, softcap=softcap)
+    got, want = c.run(), Loss(c.hidden, c.table, c.targets, c.weight)
+    assert want.z.abs().max().item() < 40
+    moved = 40**3 / (3 * softcap**2) + 2e-6 * 40
+    a = torch.where((c.targets >= 0) & (c.targets < 700), c.weight, 0.0).double().abs()
+    assert torch.all((got[1].double() - want.log_sum).abs() <= want.log_sum_off + moved)
+    assert torch.all((got[0].double() - want.loss).abs() <= want.loss_off + 2 * a * moved)
+    # a factor moves by its exponent's error and its slope's; the rounding counts again on what moved
+    p = torch.exp(want.z - want.log_sum[:, None])
+    dz = (2.1 * (2 * moved + 40**2 / softcap**2 + 4e-6)) * a[:, None] * p.scatter_add(1, c.targets.clamp(0, 699).long()[:, None], torch.ones(rows, 1, dtype=p.dtype, device=DEV))
+    assert torch.all((got[2].double() - want.d_hidden).abs() <= want.d_hidden_off + dz @ c.table.double().abs())
+    assert torch.all((got[3].double() - want.d_table).abs() <= want.d_table_off + dz.t() @ torch.where(a[:, None] != 0, c.hidden.double(), 0.0).abs())
+
+
+def test_rows_of_any_shape_with_torch_gradients():
+    import research_2_b200 as r2
+
+    c = Case(60, 64, 400, F32, 30)
+    hidden, table = c.hidden.clone().requires_grad_(), c.table.clone().requires_grad_()
+    flat = r2.token_loss(hidden, table, c.targets, weight=c.weight)
+    want = torch.autograd.grad(flat.sum(), (hidden, table))
+    shaped = r2.token_loss(hidden.view(3, 20, 64), table, c.targets.view(3, 20), weight=c.weight.view(3, 20))
+    assert shaped.shape == (3, 20) and torch.equal(shaped.reshape(-1), flat)
+    got = torch.autograd.grad(shaped.sum(), (hidden, table))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    turned = hidden.detach().t().contiguous().t().requires_grad_()
+    wide = table.detach().t().contiguous().t().requires_grad_()
+    got = torch.autograd.grad(r2.token_loss(turned, wide, c.targets, weight=c.weight).sum(), (turned, wide))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for bad in (dict(targets=c.targets[:5]), dict(weight=c.weight[:5]), dict(targets=c.targets.float()), dict(table=table[0])):
+        call = dict(table=table, targets=c.targets, weight=None)
+        call.update(bad)
+        with pytest.raises(ops().KernelError):
+            r2.token_loss(hidden, **call)
+
+
+def test_gradients_captured_into_a_graph():
+    import research_2_b200 as r2
+
+    c = Case(150, 64, 900, BF16, 31)
+    hidden, table = c.hidden.clone().requires_grad_(), c.table.clone().requires_grad_()
+
+    def step():
+        return torch.autograd.grad(r2.token_loss(hidden, table, c.targets, weight=c.weight).sum(), (hidden, table))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        hidden.neg_()
+    graph.replay()
+    torch.cuda.synchronize()
+    want = step()
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
