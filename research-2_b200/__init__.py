@@ -2,7 +2,8 @@
 
 Import name: `research_2_b200`. Public entry points: `run`, `generate`, `Engine`
 (engine/), `load_model` (models/), `write_model_folder` (weights/), `Controls` (penalties, biases, grammars
-and log-probabilities of a request), `distill_loss`, `token_loss` and `token_rows` (sampling/), `teach` (engine/).
+and log-probabilities of a request), `distill_loss`, `token_loss` and `token_rows`
+(sampling/), `teach` and `score` (engine/).
 """
 
 __version__ = "0.1.0"
@@ -17,6 +18,7 @@ _LAZY = {
     "AllowedTokens": ("sampling.controls", "AllowedTokens"),
     "distill_loss": ("sampling.distill", "distill_loss"),
     "teach": ("engine.teach", "teach"),
+    "score": ("engine.score", "score"),
     "token_loss": ("sampling.vocabulary", "token_loss"),
     "token_rows": ("sampling.vocabulary", "token_rows"),
     "write_model_folder": ("weights.model_folder", "write_model_folder"),

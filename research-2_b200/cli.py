@@ -1,4 +1,4 @@
-"""Command line: generate tokens, write a random model folder, replay a trace, write a teacher's top logits.
+"""Command line: generate tokens, write a random model folder, replay a trace, write a teacher's top logits, score given tokens.
 
 Option names follow the reference's `kelpie serve` where it has them (`--model`, `--device`,
 `--max-requests`, `--num-slabs`, `--capture/--no-capture`: kelpie-http/kelpie_http/sdk/serve.py:
@@ -9,6 +9,7 @@ only", kelpie/docs/core-api.md:18).
 
     python -m research_2_b200 generate --model DIR --prompt-tokens 5,17,3 --max-new-tokens 16
     python -m research_2_b200 teach --model DIR --tokens 5,17,3 --top 64 --out lesson.npz
+    python -m research_2_b200 score --model DIR --tokens 5,17,3
     python -m research_2_b200 random --config config.json --seed 0 --out DIR
     python -m research_2_b200 replay --model DIR --dtype float32 --out DIR --max-tokens 256 < steps.jsonl
 """
@@ -101,6 +102,18 @@ def cmd_teach(args) -> int:
     return 0
 
 
+def cmd_score(args) -> int:
+    from .engine.score import score
+
+    sequences = [_ints(t) for t in args.tokens]
+    if not sequences:
+        print("score: give --tokens (repeatable)", file=sys.stderr)
+        return 2
+    for tokens, log_probs in zip(sequences, score(args.model, sequences, dtype=args.dtype, device=args.device, portion=args.portion)):
+        print(json.dumps({"tokens": tokens, "log_probs": [float(p) for p in log_probs]}))
+    return 0
+
+
 def cmd_random(args) -> int:
     from .config.registry import architecture_of
     from . import models  # noqa: F401  (registers the architectures)
@@ -157,6 +170,13 @@ def main(argv=None) -> int:
     e.add_argument("--dtype", default="bfloat16", choices=("bfloat16", "float32"))
     e.add_argument("--device", default="cuda:0")
     e.set_defaults(fn=cmd_teach)
+    s = sub.add_parser("score", help="print the log-probability of each given token behind those before it")
+    s.add_argument("--model", required=True, help="a folder with config.json and model.safetensors")
+    s.add_argument("--tokens", action="append", default=[], metavar="1,2,3", help="one sequence; repeat for more")
+    s.add_argument("--portion", type=int, default=2048, help="tokens of a step")
+    s.add_argument("--dtype", default="bfloat16", choices=("bfloat16", "float32"))
+    s.add_argument("--device", default="cuda:0")
+    s.set_defaults(fn=cmd_score)
     t = sub.add_parser("replay", help="feed given tokens step by step and write logits (bin/trace_run)")
     t.add_argument("--model", required=True)
     t.add_argument("--dtype", required=True, choices=("bfloat16", "float32"))

@@ -69,7 +69,11 @@ class Replay:
         exponentials at the temperature (`ops.top_logits`), instead of all logits: what a student learns from."""
         return self._step(record, lambda logits: tuple(t.cpu().numpy() for t in ops.top_logits(logits, k, temperature=temperature)))
 
-    def _step(self, record: dict, take):
+    def step_losses(self, record: dict, targets) -> np.ndarray | None:
+        """Run one step; returns minus the log-probabilities of `targets`, one for each wanted row in their order (`ops.token_loss`), instead of logits."""
+        return self._step(record, lambda losses: losses.cpu().numpy(), np.asarray(targets, dtype=np.int32))
+
+    def _step(self, record: dict, take, targets: np.ndarray | None = None):
         entries = record.get("entries", [])
         reqs, starts, token_lists, wants = [], [], [], []
         self.pages_of_last_step = {}
@@ -98,11 +102,11 @@ class Replay:
             self.cache.fill(batch)
             rows = [int(batch.q_start[e]) + w for e, want in enumerate(wants) for w in want]
             batch.set_logit_rows(rows)
-            logits = self.step_fn(batch)
+            out = self.step_fn(batch) if targets is None else self.step_fn.losses(batch, targets)
             for entry, tokens in zip(entries, token_lists):
                 self.fed[str(entry["id"])] += len(tokens)
             if n_want:
-                result = take(logits)
+                result = take(out)
             else:
                 torch.cuda.synchronize(self.step_fn.device)
             ops.raise_on_device_error(self.step_fn.device)  # a kernel that gave up a bounded wait: the step is void

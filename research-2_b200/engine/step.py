@@ -43,6 +43,8 @@ class StepContext:
         # the one in front: whoever puts a plain operation (the copy of the batch, the kernel that fetches it) directly in front of the pass sets it. A
         # context that was uploaded some time ago may follow another pass whose kernels still run.
         self.cache_settled = False
+        # int32 on the device, a token for each logit row: the pass ends in their losses instead of in logits (`StepFunction.losses`)
+        self.targets = None
         # (stream tensor, its rows in the compute dtype): a block whose last kernel wrote both leaves the pair here for the next one
         self.stream_rounded = None
         # shape facts that choose kernels: inside a graph every row is an entry of its own and
@@ -307,14 +309,17 @@ class StepFunction:
         self.h2d_bytes += batch.buf.nbytes
         return StepContext(batch, dev)
 
-    def _launch_by_launch(self, batch: StepBatch, sampled: bool) -> tuple[torch.Tensor, StepContext]:
-        """The pass of a batch that is no graph: logits, or with `sampled` the tokens, and the context that it read."""
+    def _launch_by_launch(self, batch: StepBatch, sampled: bool, targets: np.ndarray | None = None) -> tuple[torch.Tensor, StepContext]:
+        """The pass of a batch that is no graph: logits, or with `sampled` the tokens, or the losses of `targets`, and the context that it read."""
         # in a caller's own graph nothing can wait for what lies outside it: the caller orders its replays
         ordered = not torch.cuda.is_current_stream_capturing()
         if ordered:
             self.order.begin()
+        if targets is not None:
+            targets = torch.from_numpy(np.ascontiguousarray(targets, dtype=np.int32)).to(self.device)
         ctx = self.upload(batch)
         ctx.cache_settled = True   # (the copy lies directly in front of the pass)
+        ctx.targets = targets
         out = self.forward(ctx)
         if sampled:
             out = self.sample(out, ctx)
@@ -368,6 +373,18 @@ class StepFunction:
                 self.h2d_bytes += batch.buf.nbytes
                 return graph.logits[: batch.n_logit_rows], graph.ctx
             return self._launch_by_launch(batch, sampled=False)
+
+    @torch.no_grad()
+    def losses(self, batch: StepBatch, targets: np.ndarray) -> torch.Tensor:
+        """Minus the log-probabilities of `targets`, a token for each logit row of a batch that has rows: float32 [n_logit_rows] on the device, without
+        logits in memory."""
+        self.validate(batch)
+        if targets.shape != (batch.n_logit_rows,):
+            raise ValueError(f"{batch.n_logit_rows} logit rows and targets {targets.shape}")
+        if self._graph_of(batch) is not None:
+            raise ValueError("a batch that runs as a graph has logits and no losses")
+        with torch.cuda.device(self.device):
+            return self._launch_by_launch(batch, sampled=False, targets=targets)[0]
 
     def launch_graph(self, batch: StepBatch) -> StepGraph | None:
         """Launches the step as its CUDA graph, if the batch is one that the scheduler filled and

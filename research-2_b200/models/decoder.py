@@ -122,7 +122,8 @@ class DecoderModel:
         return [cache[i] for i in range(len(cache))], [state[i] for i in range(len(state))]
 
     def forward(self, ctx, cache_members, state_tensors) -> torch.Tensor:
-        """The residual stream through the schedule, then logits at ctx.logit_rows: [W, V] float32."""
+        """The residual stream through the schedule, then logits at ctx.logit_rows: [W, V] float32 (or, where ctx.targets names a token for each
+        of these rows, the tokens' losses: [W])."""
         table = self.positions.additive_table() if self.positions is not None else None
         x = self.embedding.forward(ctx, table)
         if ctx.decode_only and ctx.n_tokens <= ops_resident_rows():
@@ -130,7 +131,7 @@ class DecoderModel:
                 self._resident_tried = True
                 self._resident = ResidentLayers.build(self.blocks, self.schedule, self.rt)
             if self._resident is not None and self._resident.forward(x, ctx, cache_members) is not None:
-                return self.head.forward(x, ctx.logit_rows)
+                return self._answer(x, ctx)
         for i, entry in enumerate(self.schedule):
             cache = cache_members[entry.cache] if entry.cache is not None else None
             state = state_tensors[entry.state] if entry.state is not None else None
@@ -138,7 +139,11 @@ class DecoderModel:
             if getattr(block, "looks_ahead", False):   # its last launch also prepares what the next block reads
                 ahead["upcoming"] = self.blocks[self.schedule[i + 1].layer] if i + 1 < len(self.schedule) else None
             x = block.forward(x, ctx, cache, state, entry.writes_cache, **ahead)
-        return self.head.forward(x, ctx.logit_rows)
+        return self._answer(x, ctx)
+
+    def _answer(self, x, ctx) -> torch.Tensor:
+        targets = getattr(ctx, "targets", None)
+        return self.head.forward(x, ctx.logit_rows) if targets is None else self.head.losses(x, ctx.logit_rows, targets)
 
     def weight_bytes_per_step(self) -> int:
         """Bytes of weights that one step reads (each used tensor once)."""

@@ -37,3 +37,7 @@ class Head:
         last = self.norm.forward(x, self.compute_dtype, rows=rows, lazy=True) if lazy else self.norm.forward(x, self.compute_dtype, rows=rows)
         logits = ops.linear(last, self.table, None, w_is_nk=True, out_dtype=torch.float32)
         return ops.soft_cap(logits, self.softcap) if self.softcap > 0.0 else logits
+
+    def losses(self, x, rows, targets):
+        """Minus the log-probability of targets[i] (int32) behind row rows[i], float32 [W]: the logits' loss without the logits in memory."""
+        return ops.token_loss(self.norm.forward(x, self.compute_dtype, rows=rows), self.table, targets, softcap=self.softcap)[0]
