@@ -1043,30 +1043,30 @@ __global__ void __launch_bounds__(256) join_kernel(const float* shares, int spli
                                                    int width) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, pieces = (width + 127) / 128;   // a warp a row's 128 numbers: the shares of a few rows are one chain of loads otherwise
   const bool wide = rows_wide(out, ld_o, width);
-  for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8LL) {
-    const int at = place[r];
+  for (long long i = blockIdx.x * 8LL + (threadIdx.x >> 5); i < static_cast<long long>(rows) * pieces; i += gridDim.x * 8LL) {
+    const long long r = i / pieces;
+    const int c = int(i % pieces) * 128 + lane * 4, at = place[r];
+    if (c >= width) continue;
     T* o = out + r * ld_o;
-    for (int c = lane * 4; c < width; c += 128) {
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (at >= 0) {
-        const float* s = shares + at * ld + c;   // (rows of whole eights)
-#pragma unroll 4
-        for (int i = 0; i < splits; ++i) {
-          const float4 v = __ldg(reinterpret_cast<const float4*>(s + i * plane));
-          sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-        }
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (at >= 0) {
+      const float* s = shares + at * ld + c;   // (rows of whole eights)
+#pragma unroll 8
+      for (int j = 0; j < splits; ++j) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(s + j * plane));
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
       }
-      if (wide) {
-        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(o + c) = make_uint2(pack_bf16(sum.x, sum.y), pack_bf16(sum.z, sum.w));
-        else *reinterpret_cast<float4*>(o + c) = sum;
-      } else {
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+    }
+    if (wide) {
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(o + c) = make_uint2(pack_bf16(sum.x, sum.y), pack_bf16(sum.z, sum.w));
+      else *reinterpret_cast<float4*>(o + c) = sum;
+    } else {
+      const float v[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + j < width) o[c + j] = from_float<T>(v[j]);
-      }
+      for (int j = 0; j < 4; ++j)
+        if (c + j < width) o[c + j] = from_float<T>(v[j]);
     }
   }
 }
@@ -1436,7 +1436,7 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
     }
   }
   if (status == R2_OK && d_hidden) {
-    r2_launch(join_kernel<T>, dim3(row_blocks(rows)), dim3(256), size_t(0), stream, static_cast<const float*>(shares), l.splits, share_plane, l.width_up,
+    r2_launch(join_kernel<T>, dim3(row_blocks(static_cast<long long>(rows) * ((width + 127) / 128))), dim3(256), size_t(0), stream, static_cast<const float*>(shares), l.splits, share_plane, l.width_up,
               static_cast<const int32_t*>(place), static_cast<T*>(d_hidden), ld_dh, rows, width);
     status = launch_status();
   }

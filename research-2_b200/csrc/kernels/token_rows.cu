@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(DEAL_THREADS + 32, 1) deal_kernel(const Work w
 }
 
 template <typename T, typename O, bool WIDE, bool ADD>
-__global__ void __launch_bounds__(THREADS, 2) sum_kernel(const Work w) {
+__global__ void __launch_bounds__(THREADS, 3) sum_kernel(const Work w) {
   __shared__ float heads[WARPS][SLICE], tails[WARPS][SLICE];   // of a window: the sum of the row that an earlier one began; of the row that the next goes on with
   __shared__ int head_row[WARPS], tail_row[WARPS];             // -1: none
   __shared__ int last_of_chain;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(THREADS, 2) sum_kernel(const Work w) {
     const int place = lane < n ? w.place[from + lane] : 0, number = lane < n ? w.row[from + lane] : -1;
     const int before = from > 0 ? w.row[from - 1] : -1, after = from + n < held ? w.row[from + n] : -1;
     const long long from_place = place * w.ld, to_number = number * w.ld_o;   // (a lane's, once; the warp asks the lane)
-    constexpr int BATCH = WIDE && sizeof(T) == 2 ? 8 : 4;   // rows asked for together; two batches are on their way (what the registers hold)
+    constexpr int BATCH = WIDE && sizeof(T) == 2 ? 4 : 2;   // rows asked for together; two batches are on their way (what the registers of three CTAs an SM hold)
     Raw<T, WIDE> raw[2][BATCH];
     auto load = [&](Raw<T, WIDE> (&r)[BATCH], int i0) {
 #pragma unroll
