@@ -16,8 +16,9 @@
 //
 // float32 operands are three bfloat16 planes each: x = x0 + x1 + x2 to the last bit (8 bits each), and a product is the six products x_i w_j
 // with i + j <= 2; what is left out is below 2^-24 of it. dz is kept in three planes then, too. The tensor cores add to an accumulator without rounding to nearest: each
-// addition of 16 products takes up to a unit of 2^-24 off, always towards zero. So the small products are added first, over all of k, while the accumulator is small
-// (one after the other for each k they took 4e-6 off a sum of 768 products; so it is 7e-7), and k is cut into shorter shares.
+// addition of 16 products takes up to a unit of 2^-24 off, always towards zero (4e-6 off a sum of 768 products, when all six went into it for each k). So
+// only 256 of k (or 128) are added there, the small products first, while the accumulator is small; the sums of these pieces are added in registers, rounded to nearest,
+// while the next piece's products run.
 //
 // Rows without a token or of weight 0 have no part in the gradients: `gather_kernel` puts the others side by side, so that no product reads them
 // (whatever they hold) or spends time on them; the rest of the last 256 rows is zeros.
@@ -41,6 +42,7 @@ constexpr int WARPS = 8;
 constexpr int STAGES = 5;
 constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = HALF * BK * 2;
 constexpr uint32_t SLAB = 32 * 128;   // 32 rows of 128 bytes on their way out; a warp has two
+constexpr int CHUNK = 4;              // float32: steps of k that are added in tensor memory before their sum goes into registers
 constexpr size_t SMEM = 1024 + STAGES * size_t(A_BYTES + B_BYTES) + 2 * WARPS * SLAB + (2 * STAGES + 4) * 8 + 16;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -52,7 +54,6 @@ enum Mode { LOGSUM, FACTORS, ROWS, TABLE };
 struct Work {
   int m, n, k;               // rows and columns of the result, and what is summed over
   const int* count;          // FACTORS, ROWS: m, TABLE: k, on the device (the gathered rows)
-  int terms;                 // 1, or 6 for operands in three planes
   int splits, per_split;     // ROWS: shares of k, in steps of BK
   int add;                   // ROWS: to what earlier pieces left
   float cap, cap_out;        // c > 0: 1 / c and c log2 e, so that z log2 e = cap_out tanh(cap u); else 0
@@ -173,6 +174,11 @@ template <int MODE> __device__ __forceinline__ Unit unit_of(const Work& w, long 
   return u;
 }
 
+// How many times a unit's products go through an accumulator.
+template <bool PLANES> __device__ __forceinline__ int sums_of(const Unit& u) {
+  return PLANES ? max(0, (u.kb_end - u.kb_begin + CHUNK - 1) / CHUNK) : 1;
+}
+
 // A warp's way out: rows of 128 bytes (the lane's row), two slabs in turn, each stored once it is whole.
 struct Slabs {
   uint32_t base;   // of the warp's two
@@ -210,7 +216,7 @@ __device__ __forceinline__ void tmem_row64(uint32_t taddr, float (&v)[64]) {
   }
 }
 
-template <int MODE, bool CAPPED, typename T>
+template <int MODE, bool CAPPED, typename T, bool PLANES>
 __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                               const __grid_constant__ CUtensorMap map_out, const Work w) {
   constexpr bool A_MN = MODE == TABLE, B_MN = MODE == ROWS || MODE == TABLE;
@@ -254,6 +260,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
 
   const int m = (MODE == FACTORS || MODE == ROWS) ? *w.count : w.m;
   const int k = MODE == TABLE ? *w.count : w.k;
+  constexpr int TERMS = PLANES ? 6 : 1;
   const int n_kb = (k + BK - 1) / BK, row_tiles = (m + 2 * BM - 1) / (2 * BM), col_tiles = (w.n + BN - 1) / BN;
   const long long n_units = static_cast<long long>(row_tiles) * col_tiles * (MODE == ROWS ? w.splits : 1);
 
@@ -266,35 +273,38 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     for (long long i = pair; i < n_units && ok; i += n_pairs) {
       const Unit u = unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
       const int a0 = (u.row * 2 + int(rank)) * BM, b0 = u.col * BN + int(rank) * HALF;
-      for (int t = 0; t < w.terms && ok; ++t) {   // (all of k for the smallest products first: see below)
-        for (int kb = u.kb_begin; kb < u.kb_end; ++kb) {
-          if (!warp_wait(empty + stage * 8, parity ^ 1u)) {
-            if (lane == 0) atomicMax(w.error_flag, ERR_EMPTY);
-            ok = false;
-            break;
-          }
-          if (elect_one()) {
-            const uint32_t bar = leader_full + stage * 8;
-            const int k0 = kb * BK, pa = plane_a(w.terms, t), pb = plane_b(w.terms, t);
-            if (rank == 0) mbar_expect_tx(full + stage * 8, 2 * (A_BYTES + B_BYTES));
-            const uint32_t a = a_base + stage * A_BYTES, b = b_base + stage * B_BYTES;
-            if constexpr (A_MN) {
-              load_pair(a, &map_a, a0, k0, pa, bar);
-              load_pair(a + BK * 128, &map_a, a0 + 64, k0, pa, bar);
-            } else {
-              load_pair(a, &map_a, k0, a0, pa, bar);
+      for (int lo = u.kb_begin; lo < u.kb_end && ok; lo += PLANES ? CHUNK : u.kb_end - u.kb_begin) {
+        const int hi = PLANES ? min(lo + CHUNK, u.kb_end) : u.kb_end;
+        for (int t = 0; t < TERMS && ok; ++t) {   // (the smallest products first)
+          for (int kb = lo; kb < hi; ++kb) {
+            if (!warp_wait(empty + stage * 8, parity ^ 1u)) {
+              if (lane == 0) atomicMax(w.error_flag, ERR_EMPTY);
+              ok = false;
+              break;
             }
-            if constexpr (B_MN) {
-              load_pair(b, &map_b, b0, k0, pb, bar);
-              load_pair(b + BK * 128, &map_b, b0 + 64, k0, pb, bar);
-            } else {
-              load_pair(b, &map_b, k0, b0, pb, bar);
+            if (elect_one()) {
+              const uint32_t bar = leader_full + stage * 8;
+              const int k0 = kb * BK, pa = plane_a(TERMS, t), pb = plane_b(TERMS, t);
+              if (rank == 0) mbar_expect_tx(full + stage * 8, 2 * (A_BYTES + B_BYTES));
+              const uint32_t a = a_base + stage * A_BYTES, b = b_base + stage * B_BYTES;
+              if constexpr (A_MN) {
+                load_pair(a, &map_a, a0, k0, pa, bar);
+                load_pair(a + BK * 128, &map_a, a0 + 64, k0, pa, bar);
+              } else {
+                load_pair(a, &map_a, k0, a0, pa, bar);
+              }
+              if constexpr (B_MN) {
+                load_pair(b, &map_b, b0, k0, pb, bar);
+                load_pair(b + BK * 128, &map_b, b0 + 64, k0, pb, bar);
+              } else {
+                load_pair(b, &map_b, k0, b0, pb, bar);
+              }
             }
-          }
-          __syncwarp();
-          if (++stage == STAGES) {
-            stage = 0;
-            parity ^= 1u;
+            __syncwarp();
+            if (++stage == STAGES) {
+              stage = 0;
+              parity ^= 1u;
+            }
           }
         }
       }
@@ -308,40 +318,44 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     const uint64_t b_desc = B_MN ? smem_desc(0, BK * 128, 1024) : smem_desc(0, 16, 1024);
     constexpr uint32_t a_step = (A_MN ? UMMA_K * 128 : 32) >> 4, b_step = (B_MN ? UMMA_K * 128 : 32) >> 4;
     int stage = 0;
-    uint32_t parity = 0, local = 0;   // this pair's count of units: accumulator local & 1
+    uint32_t parity = 0, local = 0;   // this pair's count of sums: accumulator local & 1
     bool ok = true;
-    for (long long i = pair; i < n_units && ok; i += n_pairs, ++local) {
+    for (long long i = pair; i < n_units && ok; i += n_pairs) {
       const Unit u = unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
-      const uint32_t buf = local & 1u;
-      if (!warp_wait(acc_empty + buf * 8, ((local >> 1) & 1u) ^ 1u)) {
-        if (lane == 0) atomicMax(w.error_flag, ERR_ACC);
-        break;
-      }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t acc = tmem + buf * BN;
-      const int steps = (u.kb_end - u.kb_begin) * w.terms;
-      for (int it = 0; it < steps; ++it) {
-        if (!warp_wait(full + stage * 8, parity)) {
-          if (lane == 0) atomicMax(w.error_flag, ERR_FULL);
+      const int sums = sums_of<PLANES>(u);
+      for (int s = 0; s < sums && ok; ++s, ++local) {
+        const uint32_t buf = local & 1u;
+        if (!warp_wait(acc_empty + buf * 8, ((local >> 1) & 1u) ^ 1u)) {
+          if (lane == 0) atomicMax(w.error_flag, ERR_ACC);
           ok = false;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (elect_one()) {
-          const uint32_t a = (a_base + stage * A_BYTES) >> 4, b = (b_base + stage * B_BYTES) >> 4;
+        const uint32_t acc = tmem + buf * BN;
+        const int steps = PLANES ? min(CHUNK, u.kb_end - u.kb_begin - s * CHUNK) * TERMS : u.kb_end - u.kb_begin;
+        for (int it = 0; it < steps; ++it) {
+          if (!warp_wait(full + stage * 8, parity)) {
+            if (lane == 0) atomicMax(w.error_flag, ERR_FULL);
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (elect_one()) {
+            const uint32_t a = (a_base + stage * A_BYTES) >> 4, b = (b_base + stage * B_BYTES) >> 4;
 #pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk)
-            umma_pair(acc, a_desc + (a & 0x3FFF) + kk * a_step, b_desc + (b & 0x3FFF) + kk * b_step, idesc, (it > 0 || kk > 0) ? 1u : 0u);
-          commit_pair(empty + stage * 8);
+            for (int kk = 0; kk < BK / UMMA_K; ++kk)
+              umma_pair(acc, a_desc + (a & 0x3FFF) + kk * a_step, b_desc + (b & 0x3FFF) + kk * b_step, idesc, (it > 0 || kk > 0) ? 1u : 0u);
+            commit_pair(empty + stage * 8);
+          }
+          __syncwarp();
+          if (++stage == STAGES) {
+            stage = 0;
+            parity ^= 1u;
+          }
         }
+        if (elect_one()) commit_pair(acc_full + buf * 8);   // also on the error path: the others go on and the flag tells
         __syncwarp();
-        if (++stage == STAGES) {
-          stage = 0;
-          parity ^= 1u;
-        }
       }
-      if (elect_one()) commit_pair(acc_full + buf * 8);   // also on the error path: the others go on and the flag tells
-      __syncwarp();
     }
   } else if (warp >= 2) {
     // ---- results: each CTA its own 128 rows; a warp 32 of them (the lanes of tensor memory that it may read) and half of the columns
@@ -349,9 +363,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     Slabs out = {slabs + (warp - 2) * 2 * SLAB, lane, 0};
     uint32_t local = 0;
     bool ok = true;
-    for (long long i = pair; i < n_units; i += n_pairs, ++local) {
+    for (long long i = pair; i < n_units; i += n_pairs) {
       const Unit u = unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
-      const uint32_t buf = local & 1u;
       const int row = (u.row * 2 + int(rank)) * BM + q * 32 + lane;
       const int col0 = u.col * BN;
       int target = -1;
@@ -363,23 +376,10 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
           less2 = w.log_sum[row] * LOG2E - log2f(fabsf(factor));
         }
       }
-      if (ok && !warp_wait(acc_full + buf * 8, (local >> 1) & 1u)) {
-        if (lane == 0) atomicMax(w.error_flag, ERR_ACC);
-        ok = false;
-      }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const bool none = u.kb_end <= u.kb_begin;   // nothing to sum over: zeros
       const int row0 = (u.row * 2 + int(rank)) * BM + q * 32;
       float top = -3.4028234663852886e38f, sum = 0.f;
-#pragma unroll 1
-      for (int c = side * HALF; c < (side + 1) * HALF && ok; c += 64) {
-        if (col0 + c >= w.n || (MODE != LOGSUM && MODE != FACTORS && row0 >= m)) break;
-        float v[64];
-        tmem_row64(tmem + buf * BN + uint32_t(c) + (uint32_t(q * 32) << 16), v);
-        if constexpr (MODE == ROWS || MODE == TABLE) {
-#pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] = none ? 0.f : v[j];
-        }
+      // 64 finished numbers of a row, from column c of the tile on
+      auto finish = [&](int c, float (&v)[64]) {
         if constexpr (MODE == LOGSUM) {
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] = log2_units<CAPPED>(v[j], w);
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
               for (int j = 0; j < 64; ++j) v[j] -= target == c + j ? size : 0.f;
             }
           }
-          for (int plane = 0; plane < (w.terms == 1 ? 1 : 3); ++plane) {
+          for (int plane = 0; plane < (PLANES ? 3 : 1); ++plane) {
             const uint32_t slab = out.begin();
 #pragma unroll
             for (int p = 0; p < 8; ++p) {
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
 #pragma unroll
               for (int j = 0; j < 4; ++j) r[j] = pack_bf16(v[8 * p + 2 * j], v[8 * p + 2 * j + 1]);
               out.put16(slab, p, (r[0] & held) ^ sign, (r[1] & held) ^ sign, (r[2] & held) ^ sign, (r[3] & held) ^ sign);
-              if (w.terms > 1) {
+              if constexpr (PLANES) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                   v[8 * p + 2 * j] -= __uint_as_float(r[j] << 16);
@@ -460,10 +460,61 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
             out.end(&map_out, col0 + c + 32 * half, row0, u.split, slab, MODE == ROWS && w.add);
           }
         }
+      };
+      auto left = [&](int c) { return col0 + c < w.n && (MODE == LOGSUM || MODE == FACTORS || row0 < m); };
+      const uint32_t lanes = uint32_t(q * 32) << 16;
+      auto wait_sum = [&](uint32_t buf) {
+        if (ok && !warp_wait(acc_full + buf * 8, (local >> 1) & 1u)) {
+          if (lane == 0) atomicMax(w.error_flag, ERR_ACC);
+          ok = false;   // this and the later tiles are not written; the flag tells
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      };
+      auto hand_back = [&](uint32_t buf) {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive_cluster(leader_acc_empty + buf * 8);
+        ++local;
+      };
+      if constexpr (PLANES) {
+        float lo[64], hi[64];
+#pragma unroll
+        for (int j = 0; j < 64; ++j) lo[j] = hi[j] = 0.f;
+        const int sums = sums_of<PLANES>(u);   // (none: zeros)
+#pragma unroll 1
+        for (int s = 0; s < sums; ++s) {
+          const uint32_t buf = local & 1u;
+          wait_sum(buf);
+          if (ok && left(side * HALF)) {
+            uint32_t r[32];
+#pragma unroll
+            for (int part = 0; part < 4; ++part) {
+              tmem_load32(tmem + buf * BN + uint32_t(side * HALF + part * 32) + lanes, r);
+              tmem_load_wait(r);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) (part < 2 ? lo : hi)[part % 2 * 32 + j] += __uint_as_float(r[j]);
+            }
+          }
+          hand_back(buf);
+        }
+        if (ok && left(side * HALF)) finish(side * HALF, lo);
+        if (ok && left(side * HALF + 64)) finish(side * HALF + 64, hi);
+      } else {
+        const uint32_t buf = local & 1u;
+        wait_sum(buf);
+        const bool none = u.kb_end <= u.kb_begin;   // nothing to sum over: zeros
+#pragma unroll 1
+        for (int c = side * HALF; c < (side + 1) * HALF && ok && left(c); c += 64) {
+          float v[64];
+          tmem_row64(tmem + buf * BN + uint32_t(c) + lanes, v);
+          if constexpr (MODE == ROWS || MODE == TABLE) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] = none ? 0.f : v[j];
+          }
+          finish(c, v);
+        }
+        hand_back(buf);
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) arrive_cluster(leader_acc_empty + buf * 8);
       if constexpr (MODE == LOGSUM) {
         if (row < m) w.part[(size_t(u.col) * 2 + side) * m + row] = ok ? make_float2(top, sum) : make_float2(NAN, NAN);
       }
@@ -494,6 +545,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
 constexpr int FEW = 128;            // rows at most
 constexpr int FEW_STAGES = 8;       // of operands, at most
 constexpr int TURNED = 132;         // floats of a row of the turned tile (128 tokens and four of padding)
+constexpr int FEW_CHUNK = 4;        // float32: steps of k (of 32) that are added in tensor memory before their sum goes to the turned tile
 
 struct FewWork {
   int rows, columns;                // of the batch; a multiple of 16: columns of the accumulator
@@ -523,8 +575,9 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
 template <bool F32> __host__ __device__ inline uint32_t few_stage_bytes(int columns) {
   return F32 ? 3u * (8192u + uint32_t(columns) * 64u) : 16384u + uint32_t(columns) * 128u;
 }
+template <bool F32> __host__ __device__ inline uint32_t turned_bytes(int columns) { return uint32_t(F32 ? (columns + 31) / 32 * 32 : 32) * TURNED * 4; }
 template <bool F32> __host__ __device__ inline uint32_t few_smem(int columns, int stages, int loads) {
-  return 1024u + uint32_t(stages) * few_stage_bytes<F32>(columns) + (F32 ? uint32_t(loads) * 16384u : 0u) + 32 * TURNED * 4 + (4 * FEW_STAGES + 4) * 8 + 16;
+  return 1024u + uint32_t(stages) * few_stage_bytes<F32>(columns) + (F32 ? uint32_t(loads) * 16384u : 0u) + turned_bytes<F32>(columns) + (4 * FEW_STAGES + 4) * 8 + 16;
 }
 
 template <int MODE, bool CAPPED, bool F32>
@@ -534,9 +587,9 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
   const uint32_t stage_bytes = few_stage_bytes<F32>(f.columns);
   const uint32_t loads_at = smem_u32(smem), stages_at = loads_at + (F32 ? uint32_t(f.loads) * 16384u : 0u);
   float* turned = reinterpret_cast<float*>(smem + (stages_at - loads_at) + size_t(f.stages) * stage_bytes);
-  const uint32_t full = smem_u32(turned) + 32 * TURNED * 4, empty = full + FEW_STAGES * 8, loaded = empty + FEW_STAGES * 8, taken = loaded + FEW_STAGES * 8,
+  const uint32_t full = smem_u32(turned) + turned_bytes<F32>(f.columns), empty = full + FEW_STAGES * 8, loaded = empty + FEW_STAGES * 8, taken = loaded + FEW_STAGES * 8,
                  acc_full = taken + FEW_STAGES * 8, acc_empty = acc_full + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turned + 32 * TURNED + (4 * FEW_STAGES + 4) * 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(turned) + turned_bytes<F32>(f.columns) + (4 * FEW_STAGES + 4) * 8);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // Two accumulators, in float32 two parts each: of the products of the first planes, and of the small ones, which would be cut off against it.
   const uint32_t apart = uint32_t(f.columns + 31) / 32 * 32, both = F32 ? 2 * apart : apart;
@@ -571,6 +624,7 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
   const int tiles = (f.n + 127) / 128;
   constexpr int STEP = F32 ? 32 : 64;   // of k
   const int n_kb = (f.k + STEP - 1) / STEP;
+  const int per_sum = F32 ? FEW_CHUNK : n_kb;
   const uint32_t x_bytes = uint32_t(f.columns) * STEP * 2;
 
   if (warp == 0) {
@@ -612,46 +666,49 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
     int stage = 0;
     uint32_t parity = 0, local = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++local) {
-      const uint32_t buf = local & 1u;
-      if (!warp_wait(acc_empty + buf * 8, ((local >> 1) & 1u) ^ 1u)) {
-        if (lane == 0) atomicMax(f.w.error_flag, ERR_ACC);
-        break;
-      }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t acc = tmem + buf * both;
-      for (int kb = 0; kb < n_kb; ++kb) {
-        if (!warp_wait(full + stage * 8, parity)) {
-          if (lane == 0) atomicMax(f.w.error_flag, ERR_FULL);
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      for (int lo = 0; lo < n_kb && ok; lo += per_sum, ++local) {
+        const uint32_t buf = local & 1u;
+        if (!warp_wait(acc_empty + buf * 8, ((local >> 1) & 1u) ^ 1u)) {
+          if (lane == 0) atomicMax(f.w.error_flag, ERR_ACC);
           ok = false;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (elect_one()) {
-          const uint32_t at = stages_at + stage * stage_bytes;
-          if constexpr (F32) {
-#pragma unroll
-            for (int t = 0; t < 6; ++t) {
-              const uint64_t a = smem_desc_64(at + plane_a(6, t) * 8192), b = smem_desc_64(at + 3 * 8192 + plane_b(6, t) * x_bytes);
-#pragma unroll
-              for (int kk = 0; kk < 2; ++kk)
-                umma_bf16(t < 5 ? acc + apart : acc, a + kk * 2, b + kk * 2, idesc, (kb > 0 || (t > 0 && t < 5) || kk > 0) ? 1u : 0u);
-            }
-          } else {
-            const uint64_t a = smem_desc(at, 16, 1024), b = smem_desc(at + 16384, 16, 1024);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) umma_bf16(acc, a + kk * 2, b + kk * 2, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+        const uint32_t acc = tmem + buf * both;
+        for (int kb = lo; kb < min(n_kb, lo + per_sum); ++kb) {
+          if (!warp_wait(full + stage * 8, parity)) {
+            if (lane == 0) atomicMax(f.w.error_flag, ERR_FULL);
+            ok = false;
+            break;
           }
-          umma_commit(empty + stage * 8);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (elect_one()) {
+            const uint32_t at = stages_at + stage * stage_bytes;
+            if constexpr (F32) {
+#pragma unroll
+              for (int t = 0; t < 6; ++t) {
+                const uint64_t a = smem_desc_64(at + plane_a(6, t) * 8192), b = smem_desc_64(at + 3 * 8192 + plane_b(6, t) * x_bytes);
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk)
+                  umma_bf16(t < 5 ? acc + apart : acc, a + kk * 2, b + kk * 2, idesc, (kb > lo || (t > 0 && t < 5) || kk > 0) ? 1u : 0u);
+              }
+            } else {
+              const uint64_t a = smem_desc(at, 16, 1024), b = smem_desc(at + 16384, 16, 1024);
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) umma_bf16(acc, a + kk * 2, b + kk * 2, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            }
+            umma_commit(empty + stage * 8);
+          }
+          __syncwarp();
+          if (++stage == f.stages) {
+            stage = 0;
+            parity ^= 1u;
+          }
         }
+        if (elect_one()) umma_commit(acc_full + buf * 8);   // also on the error path: the others go on and the flag tells
         __syncwarp();
-        if (++stage == f.stages) {
-          stage = 0;
-          parity ^= 1u;
-        }
       }
-      if (elect_one()) umma_commit(acc_full + buf * 8);   // also on the error path: the others go on and the flag tells
-      __syncwarp();
     }
   } else if (warp < 6) {
     // ---- results
@@ -666,39 +723,57 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
     }
     uint32_t local = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++local) {
-      const uint32_t buf = local & 1u;
-      if (ok && !warp_wait(acc_full + buf * 8, (local >> 1) & 1u)) {
-        if (lane == 0) atomicMax(f.w.error_flag, ERR_ACC);
-        ok = false;
-      }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
       const int left = f.n - tile * 128 - part * 32;   // tokens of the thread's 32 that there are
+      // float32: the sums of the pieces of k, in the turned tile of all rows (a lane its token's column)
+      uint32_t buf = 0;
+      for (int lo = 0; lo < n_kb; lo += per_sum) {
+        buf = local & 1u;
+        if (ok && !warp_wait(acc_full + buf * 8, (local >> 1) & 1u)) {
+          if (lane == 0) atomicMax(f.w.error_flag, ERR_ACC);
+          ok = false;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if constexpr (F32) {
+#pragma unroll 1
+          for (int c = 0; c < int(apart); c += 32) {
+            uint32_t r[32], small[32];
+            tmem_load32(tmem + buf * both + uint32_t(c) + (uint32_t(q * 32) << 16), r);
+            tmem_load32(tmem + buf * both + apart + uint32_t(c) + (uint32_t(q * 32) << 16), small);
+            tmem_load_wait(r);
+            tmem_tie(small);
+            float* to = turned + c * TURNED + q * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float piece = __uint_as_float(r[j]) + __uint_as_float(small[j]);
+              to[j * TURNED] = lo == 0 ? piece : to[j * TURNED] + piece;
+            }
+          }
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty + buf * 8);
+          ++local;
+        }
+      }
+      if constexpr (F32) asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
       for (int g = 0; g < FEW / 32; ++g) {
         if (g >= groups) break;
-        if (uint32_t(g * 32) < apart) {
-          uint32_t r[32];
-          tmem_load32(tmem + buf * both + uint32_t(g * 32) + (uint32_t(q * 32) << 16), r);
-          if constexpr (F32) {
-            uint32_t small[32];
-            tmem_load32(tmem + buf * both + apart + uint32_t(g * 32) + (uint32_t(q * 32) << 16), small);
+        if constexpr (!F32) {
+          if (uint32_t(g * 32) < apart) {
+            uint32_t r[32];
+            tmem_load32(tmem + buf * both + uint32_t(g * 32) + (uint32_t(q * 32) << 16), r);
             tmem_load_wait(r);
-            tmem_tie(small);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(small[j]));
-          } else {
-            tmem_load_wait(r);
+            for (int j = 0; j < 32; ++j) turned[j * TURNED + q * 32 + lane] = __uint_as_float(r[j]);
           }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) turned[j * TURNED + q * 32 + lane] = __uint_as_float(r[j]);
+          asm volatile("bar.sync 1, 128;" ::: "memory");
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
         const int row = g * 32 + lane;
         float v[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 x = *reinterpret_cast<const float4*>(turned + lane * TURNED + part * 32 + 4 * i);
+          const float4 x = *reinterpret_cast<const float4*>(turned + ((F32 && uint32_t(g * 32) < apart ? g * 32 : 0) + lane) * TURNED + part * 32 + 4 * i);
           v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
         }
         if constexpr (MODE == LOGSUM) {
@@ -764,11 +839,16 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
             }
           }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");   // (the turned tile is read)
+        if constexpr (!F32) asm volatile("bar.sync 1, 128;" ::: "memory");   // (the turned tile is read)
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty + buf * 8);
+      if constexpr (F32) {
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      } else {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty + buf * 8);
+        ++local;
+      }
     }
     if constexpr (MODE == LOGSUM) {
 #pragma unroll
@@ -1109,7 +1189,7 @@ int resident_pairs() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 1;
   if (dev < 64 && cached[dev].load() > 0) return cached[dev].load();
-  auto kernel = product_kernel<LOGSUM, false, bf16>;
+  auto kernel = product_kernel<LOGSUM, false, bf16, false>;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM));
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(2, 1, 1);
@@ -1130,9 +1210,9 @@ int resident_pairs() {
   return n;
 }
 
-template <int MODE, bool CAPPED, typename T>
+template <int MODE, bool CAPPED, typename T, bool PLANES>
 int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Work& w, long long units, cudaStream_t stream) {
-  auto kernel = product_kernel<MODE, CAPPED, T>;
+  auto kernel = product_kernel<MODE, CAPPED, T, PLANES>;
   static std::atomic<bool> done[64];
   const int status = allow_smem(kernel, SMEM, done);
   if (status != R2_OK) return status;
@@ -1154,12 +1234,12 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, 
   return e != cudaSuccess ? int(e) : launch_status();
 }
 
-template <int MODE, typename T>
+template <int MODE, typename T, bool PLANES>
 int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Work& w, long long units, bool capped, cudaStream_t stream) {
   if constexpr (MODE == LOGSUM || MODE == FACTORS) {
-    if (capped) return launch<MODE, true, T>(ma, mb, mo, w, units, stream);
+    if (capped) return launch<MODE, true, T, PLANES>(ma, mb, mo, w, units, stream);
   }
-  return launch<MODE, false, T>(ma, mb, mo, w, units, stream);
+  return launch<MODE, false, T, PLANES>(ma, mb, mo, w, units, stream);
 }
 
 int n_sms() {
@@ -1191,6 +1271,7 @@ int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, FewWork f, cudaStre
   f.loads = F32 ? FEW_STAGES : 0;
   while (f.loads > 2 && few_smem<F32>(f.columns, f.stages, f.loads) > most) --f.loads;
   while (f.stages > 2 && few_smem<F32>(f.columns, f.stages, f.loads) > most) --f.stages;
+  while (F32 && f.loads < FEW_STAGES && few_smem<F32>(f.columns, f.stages, f.loads + 1) <= most) ++f.loads;
   r2_launch(kernel, dim3(few_ctas(f.n)), dim3(F32 ? 448 : 192), size_t(few_smem<F32>(f.columns, f.stages, f.loads)), stream, mt, mx, f);
   return launch_status();
 }
@@ -1266,7 +1347,6 @@ Layout layout(int dtype, long long rows, long long width, long long vocab, bool 
     double best = -1;
     for (int s = 1; s <= 64 && (s == 1 || n_kb * terms / s >= 8); ++s) {
       const int per = (n_kb + s - 1) / s;
-      if (terms > 1 && per > 64 && s < 64) continue;   // (float32: no more than 256 additions to an accumulator)
       const double steps = per * terms + 8;
       const double cost = l.pieces * double((tiles * s + pairs - 1) / pairs) * steps + double(s) * tiles * 0.14 * (l.pieces + 1);
       if (best < 0 || cost < best) {
@@ -1340,8 +1420,7 @@ int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_
     w.m = rows;
     w.n = vocab;
     w.k = width;
-    w.terms = l.planes * (l.planes + 1) / 2;
-    status = launch<LOGSUM, bf16>(ma, mb, ma, w, (l.rows_up / 256) * (up(vocab, BN) / BN), softcap > 0.f, stream);
+    status = launch<LOGSUM, bf16, sizeof(T) == 4>(ma, mb, ma, w, (l.rows_up / 256) * (up(vocab, BN) / BN), softcap > 0.f, stream);
     parts = int(up(vocab, BN) / BN) * 2;
   }
   if (status != R2_OK) return status;
@@ -1369,7 +1448,6 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
   Work w = {};
   w.m = rows;
   w.count = count;
-  w.terms = l.planes * (l.planes + 1) / 2;
   w.targets = reinterpret_cast<int32_t*>(space + l.targets);
   w.factor = reinterpret_cast<float*>(space + l.factor);
   w.log_sum = reinterpret_cast<float*>(space + l.sums);
@@ -1405,7 +1483,7 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
       if (!make_map(&ma, x, width, l.rows_up, BM) || !make_map(&mb, part, width, n, HALF) ||
           !make_out_map<bf16>(&mo, dz.at, l.piece, l.rows_up, l.planes, l.piece, dz.plane))
         return R2_BAD_ALIGN;
-      status = launch<FACTORS, bf16>(ma, mb, mo, w, row_tiles * (up(n, BN) / BN), softcap > 0.f, stream);
+      status = launch<FACTORS, bf16, sizeof(T) == 4>(ma, mb, mo, w, row_tiles * (up(n, BN) / BN), softcap > 0.f, stream);
     }
     if (status == R2_OK && d_hidden) {
       Work d = w;
@@ -1417,7 +1495,7 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
       if (!make_map(&ma, dz, n, l.rows_up, BM) || !make_map(&mb, part, width, n, BK) ||
           !make_out_map<float>(&mo, shares, width, l.rows_up, l.splits, l.width_up, share_plane))
         return R2_BAD_ALIGN;
-      status = launch<ROWS, float>(ma, mb, mo, d, row_tiles * width_tiles * d.splits, false, stream);
+      status = launch<ROWS, float, sizeof(T) == 4>(ma, mb, mo, d, row_tiles * width_tiles * d.splits, false, stream);
     }
     if (status == R2_OK && d_table) {
       Work d = w;
@@ -1432,7 +1510,7 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
         d.out = out;
         d.ld = ld_dt;
       }
-      status = launch<TABLE, T>(ma, mb, mo, d, up(n, 256) / 256 * width_tiles, false, stream);
+      status = launch<TABLE, T, sizeof(T) == 4>(ma, mb, mo, d, up(n, 256) / 256 * width_tiles, false, stream);
     }
   }
   if (status == R2_OK && d_hidden) {
