@@ -42,7 +42,6 @@ constexpr int WARPS = 8;
 constexpr int STAGES = 5;
 constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = HALF * BK * 2;
 constexpr uint32_t SLAB = 32 * 128;   // 32 rows of 128 bytes on their way out; a warp has two
-constexpr int CHUNK = 4;              // float32: steps of k that are added in tensor memory before their sum goes into registers
 constexpr size_t SMEM = 1024 + STAGES * size_t(A_BYTES + B_BYTES) + 2 * WARPS * SLAB + (2 * STAGES + 4) * 8 + 16;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -174,9 +173,14 @@ template <int MODE> __device__ __forceinline__ Unit unit_of(const Work& w, long 
   return u;
 }
 
+// Steps of k that are added in tensor memory before their sum goes into registers (0: all): 256 of k with the products of planes; 512 where float results are
+// made of more than 1,024 bfloat16 products (1,600 of them: off by 2.4e-7 of the loss in place of 7.7e-7, and 5 % slower).
+constexpr int PLANES_CHUNK = 4, LONG_CHUNK = 8, LONG_STEPS = 16;
+
 // How many times a unit's products go through an accumulator.
-template <bool PLANES> __device__ __forceinline__ int sums_of(const Unit& u) {
-  return PLANES ? max(0, (u.kb_end - u.kb_begin + CHUNK - 1) / CHUNK) : 1;
+template <int CHUNKED> __device__ __forceinline__ int sums_of(const Unit& u) {
+  if constexpr (CHUNKED > 0) return max(0, (u.kb_end - u.kb_begin + CHUNKED - 1) / CHUNKED);
+  return 1;
 }
 
 // A warp's way out: rows of 128 bytes (the lane's row), two slabs in turn, each stored once it is whole.
@@ -216,7 +220,7 @@ __device__ __forceinline__ void tmem_row64(uint32_t taddr, float (&v)[64]) {
   }
 }
 
-template <int MODE, bool CAPPED, typename T, bool PLANES>
+template <int MODE, bool CAPPED, typename T, bool PLANES, int CHUNKED>
 __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                               const __grid_constant__ CUtensorMap map_out, const Work w) {
   constexpr bool A_MN = MODE == TABLE, B_MN = MODE == ROWS || MODE == TABLE;
@@ -273,8 +277,8 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     for (long long i = pair; i < n_units && ok; i += n_pairs) {
       const Unit u = unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
       const int a0 = (u.row * 2 + int(rank)) * BM, b0 = u.col * BN + int(rank) * HALF;
-      for (int lo = u.kb_begin; lo < u.kb_end && ok; lo += PLANES ? CHUNK : u.kb_end - u.kb_begin) {
-        const int hi = PLANES ? min(lo + CHUNK, u.kb_end) : u.kb_end;
+      for (int lo = u.kb_begin; lo < u.kb_end && ok; lo += CHUNKED > 0 ? CHUNKED : u.kb_end - u.kb_begin) {
+        const int hi = CHUNKED > 0 ? min(lo + CHUNKED, u.kb_end) : u.kb_end;
         for (int t = 0; t < TERMS && ok; ++t) {   // (the smallest products first)
           for (int kb = lo; kb < hi; ++kb) {
             if (!warp_wait(empty + stage * 8, parity ^ 1u)) {
@@ -322,7 +326,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     bool ok = true;
     for (long long i = pair; i < n_units && ok; i += n_pairs) {
       const Unit u = unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
-      const int sums = sums_of<PLANES>(u);
+      const int sums = sums_of<CHUNKED>(u);
       for (int s = 0; s < sums && ok; ++s, ++local) {
         const uint32_t buf = local & 1u;
         if (!warp_wait(acc_empty + buf * 8, ((local >> 1) & 1u) ^ 1u)) {
@@ -332,7 +336,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t acc = tmem + buf * BN;
-        const int steps = PLANES ? min(CHUNK, u.kb_end - u.kb_begin - s * CHUNK) * TERMS : u.kb_end - u.kb_begin;
+        const int steps = CHUNKED > 0 ? min(CHUNKED, u.kb_end - u.kb_begin - s * CHUNKED) * TERMS : u.kb_end - u.kb_begin;
         for (int it = 0; it < steps; ++it) {
           if (!warp_wait(full + stage * 8, parity)) {
             if (lane == 0) atomicMax(w.error_flag, ERR_FULL);
@@ -476,11 +480,11 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
         if (lane == 0) arrive_cluster(leader_acc_empty + buf * 8);
         ++local;
       };
-      if constexpr (PLANES) {
+      if constexpr (CHUNKED > 0) {
         float lo[64], hi[64];
 #pragma unroll
         for (int j = 0; j < 64; ++j) lo[j] = hi[j] = 0.f;
-        const int sums = sums_of<PLANES>(u);   // (none: zeros)
+        const int sums = sums_of<CHUNKED>(u);   // (none: zeros)
 #pragma unroll 1
         for (int s = 0; s < sums; ++s) {
           const uint32_t buf = local & 1u;
@@ -545,7 +549,7 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
 constexpr int FEW = 128;            // rows at most
 constexpr int FEW_STAGES = 8;       // of operands, at most
 constexpr int TURNED = 132;         // floats of a row of the turned tile (128 tokens and four of padding)
-constexpr int FEW_CHUNK = 4;        // float32: steps of k (of 32) that are added in tensor memory before their sum goes to the turned tile
+constexpr int FEW_CHUNK = 8;        // steps of k that are added in tensor memory before their sum goes to the turned tile: 256 of k in float32; 512 of more than 1,024 in bfloat16
 
 struct FewWork {
   int rows, columns;                // of the batch; a multiple of 16: columns of the accumulator
@@ -575,21 +579,21 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
 template <bool F32> __host__ __device__ inline uint32_t few_stage_bytes(int columns) {
   return F32 ? 3u * (8192u + uint32_t(columns) * 64u) : 16384u + uint32_t(columns) * 128u;
 }
-template <bool F32> __host__ __device__ inline uint32_t turned_bytes(int columns) { return uint32_t(F32 ? (columns + 31) / 32 * 32 : 32) * TURNED * 4; }
-template <bool F32> __host__ __device__ inline uint32_t few_smem(int columns, int stages, int loads) {
-  return 1024u + uint32_t(stages) * few_stage_bytes<F32>(columns) + (F32 ? uint32_t(loads) * 16384u : 0u) + turned_bytes<F32>(columns) + (4 * FEW_STAGES + 4) * 8 + 16;
+template <bool SUMS> __host__ __device__ inline uint32_t turned_bytes(int columns) { return uint32_t(SUMS ? (columns + 31) / 32 * 32 : 32) * TURNED * 4; }
+template <bool F32, bool SUMS> __host__ __device__ inline uint32_t few_smem(int columns, int stages, int loads) {
+  return 1024u + uint32_t(stages) * few_stage_bytes<F32>(columns) + (F32 ? uint32_t(loads) * 16384u : 0u) + turned_bytes<SUMS>(columns) + (4 * FEW_STAGES + 4) * 8 + 16;
 }
 
-template <int MODE, bool CAPPED, bool F32>
+template <int MODE, bool CAPPED, bool F32, bool SUMS>
 __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_x, const FewWork f) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t stage_bytes = few_stage_bytes<F32>(f.columns);
   const uint32_t loads_at = smem_u32(smem), stages_at = loads_at + (F32 ? uint32_t(f.loads) * 16384u : 0u);
   float* turned = reinterpret_cast<float*>(smem + (stages_at - loads_at) + size_t(f.stages) * stage_bytes);
-  const uint32_t full = smem_u32(turned) + turned_bytes<F32>(f.columns), empty = full + FEW_STAGES * 8, loaded = empty + FEW_STAGES * 8, taken = loaded + FEW_STAGES * 8,
+  const uint32_t full = smem_u32(turned) + turned_bytes<SUMS>(f.columns), empty = full + FEW_STAGES * 8, loaded = empty + FEW_STAGES * 8, taken = loaded + FEW_STAGES * 8,
                  acc_full = taken + FEW_STAGES * 8, acc_empty = acc_full + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(turned) + turned_bytes<F32>(f.columns) + (4 * FEW_STAGES + 4) * 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(turned) + turned_bytes<SUMS>(f.columns) + (4 * FEW_STAGES + 4) * 8);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // Two accumulators, in float32 two parts each: of the products of the first planes, and of the small ones, which would be cut off against it.
   const uint32_t apart = uint32_t(f.columns + 31) / 32 * 32, both = F32 ? 2 * apart : apart;
@@ -624,7 +628,7 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
   const int tiles = (f.n + 127) / 128;
   constexpr int STEP = F32 ? 32 : 64;   // of k
   const int n_kb = (f.k + STEP - 1) / STEP;
-  const int per_sum = F32 ? FEW_CHUNK : n_kb;
+  const int per_sum = SUMS ? FEW_CHUNK : n_kb;
   const uint32_t x_bytes = uint32_t(f.columns) * STEP * 2;
 
   if (warp == 0) {
@@ -696,7 +700,7 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
             } else {
               const uint64_t a = smem_desc(at, 16, 1024), b = smem_desc(at + 16384, 16, 1024);
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk) umma_bf16(acc, a + kk * 2, b + kk * 2, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+              for (int kk = 0; kk < 4; ++kk) umma_bf16(acc, a + kk * 2, b + kk * 2, idesc, (kb > lo || kk > 0) ? 1u : 0u);
             }
             umma_commit(empty + stage * 8);
           }
@@ -725,7 +729,7 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
     bool ok = true;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
       const int left = f.n - tile * 128 - part * 32;   // tokens of the thread's 32 that there are
-      // float32: the sums of the pieces of k, in the turned tile of all rows (a lane its token's column)
+      // the sums of the pieces of k, in the turned tile of all rows (a lane its token's column)
       uint32_t buf = 0;
       for (int lo = 0; lo < n_kb; lo += per_sum) {
         buf = local & 1u;
@@ -734,18 +738,18 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
           ok = false;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if constexpr (F32) {
+        if constexpr (SUMS) {
 #pragma unroll 1
           for (int c = 0; c < int(apart); c += 32) {
             uint32_t r[32], small[32];
             tmem_load32(tmem + buf * both + uint32_t(c) + (uint32_t(q * 32) << 16), r);
-            tmem_load32(tmem + buf * both + apart + uint32_t(c) + (uint32_t(q * 32) << 16), small);
+            if constexpr (F32) tmem_load32(tmem + buf * both + apart + uint32_t(c) + (uint32_t(q * 32) << 16), small);
             tmem_load_wait(r);
-            tmem_tie(small);
+            if constexpr (F32) tmem_tie(small);
             float* to = turned + c * TURNED + q * 32 + lane;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-              const float piece = __uint_as_float(r[j]) + __uint_as_float(small[j]);
+              const float piece = F32 ? __uint_as_float(r[j]) + __uint_as_float(small[j]) : __uint_as_float(r[j]);
               to[j * TURNED] = lo == 0 ? piece : to[j * TURNED] + piece;
             }
           }
@@ -755,11 +759,11 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
           ++local;
         }
       }
-      if constexpr (F32) asm volatile("bar.sync 1, 128;" ::: "memory");
+      if constexpr (SUMS) asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
       for (int g = 0; g < FEW / 32; ++g) {
         if (g >= groups) break;
-        if constexpr (!F32) {
+        if constexpr (!SUMS) {
           if (uint32_t(g * 32) < apart) {
             uint32_t r[32];
             tmem_load32(tmem + buf * both + uint32_t(g * 32) + (uint32_t(q * 32) << 16), r);
@@ -773,7 +777,7 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
         float v[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 x = *reinterpret_cast<const float4*>(turned + ((F32 && uint32_t(g * 32) < apart ? g * 32 : 0) + lane) * TURNED + part * 32 + 4 * i);
+          const float4 x = *reinterpret_cast<const float4*>(turned + ((SUMS && uint32_t(g * 32) < apart ? g * 32 : 0) + lane) * TURNED + part * 32 + 4 * i);
           v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
         }
         if constexpr (MODE == LOGSUM) {
@@ -839,9 +843,9 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
             }
           }
         }
-        if constexpr (!F32) asm volatile("bar.sync 1, 128;" ::: "memory");   // (the turned tile is read)
+        if constexpr (!SUMS) asm volatile("bar.sync 1, 128;" ::: "memory");   // (the turned tile is read)
       }
-      if constexpr (F32) {
+      if constexpr (SUMS) {
         asm volatile("bar.sync 1, 128;" ::: "memory");
       } else {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1189,7 +1193,7 @@ int resident_pairs() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 1;
   if (dev < 64 && cached[dev].load() > 0) return cached[dev].load();
-  auto kernel = product_kernel<LOGSUM, false, bf16, false>;
+  auto kernel = product_kernel<LOGSUM, false, bf16, false, 0>;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM));
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(2, 1, 1);
@@ -1210,9 +1214,9 @@ int resident_pairs() {
   return n;
 }
 
-template <int MODE, bool CAPPED, typename T, bool PLANES>
+template <int MODE, bool CAPPED, typename T, bool PLANES, int CHUNKED>
 int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Work& w, long long units, cudaStream_t stream) {
-  auto kernel = product_kernel<MODE, CAPPED, T, PLANES>;
+  auto kernel = product_kernel<MODE, CAPPED, T, PLANES, CHUNKED>;
   static std::atomic<bool> done[64];
   const int status = allow_smem(kernel, SMEM, done);
   if (status != R2_OK) return status;
@@ -1234,12 +1238,12 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, 
   return e != cudaSuccess ? int(e) : launch_status();
 }
 
-template <int MODE, typename T, bool PLANES>
+template <int MODE, typename T, bool PLANES, int CHUNKED = PLANES ? PLANES_CHUNK : 0>
 int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Work& w, long long units, bool capped, cudaStream_t stream) {
   if constexpr (MODE == LOGSUM || MODE == FACTORS) {
-    if (capped) return launch<MODE, true, T, PLANES>(ma, mb, mo, w, units, stream);
+    if (capped) return launch<MODE, true, T, PLANES, CHUNKED>(ma, mb, mo, w, units, stream);
   }
-  return launch<MODE, false, T, PLANES>(ma, mb, mo, w, units, stream);
+  return launch<MODE, false, T, PLANES, CHUNKED>(ma, mb, mo, w, units, stream);
 }
 
 int n_sms() {
@@ -1260,24 +1264,27 @@ int few_ctas(long long vocab) {
   return int(tiles < n_sms() ? tiles : n_sms());
 }
 
-template <int MODE, bool CAPPED, bool F32>
+template <int MODE, bool CAPPED, bool F32, bool SUMS>
 int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, FewWork f, cudaStream_t stream) {
   constexpr uint32_t most = 227 * 1024;
-  auto kernel = few_kernel<MODE, CAPPED, F32>;
+  auto kernel = few_kernel<MODE, CAPPED, F32, SUMS>;
   static std::atomic<bool> done[64];
   const int status = allow_smem(kernel, most, done);
   if (status != R2_OK) return status;
   f.stages = F32 ? 3 : FEW_STAGES;   // (float32: two stages fill while one is read; the rest of the memory keeps the table coming)
   f.loads = F32 ? FEW_STAGES : 0;
-  while (f.loads > 2 && few_smem<F32>(f.columns, f.stages, f.loads) > most) --f.loads;
-  while (f.stages > 2 && few_smem<F32>(f.columns, f.stages, f.loads) > most) --f.stages;
-  while (F32 && f.loads < FEW_STAGES && few_smem<F32>(f.columns, f.stages, f.loads + 1) <= most) ++f.loads;
-  r2_launch(kernel, dim3(few_ctas(f.n)), dim3(F32 ? 448 : 192), size_t(few_smem<F32>(f.columns, f.stages, f.loads)), stream, mt, mx, f);
+  while (f.loads > 2 && few_smem<F32, SUMS>(f.columns, f.stages, f.loads) > most) --f.loads;
+  while (f.stages > 2 && few_smem<F32, SUMS>(f.columns, f.stages, f.loads) > most) --f.stages;
+  while (F32 && f.loads < FEW_STAGES && few_smem<F32, SUMS>(f.columns, f.stages, f.loads + 1) <= most) ++f.loads;
+  r2_launch(kernel, dim3(few_ctas(f.n)), dim3(F32 ? 448 : 192), size_t(few_smem<F32, SUMS>(f.columns, f.stages, f.loads)), stream, mt, mx, f);
   return launch_status();
 }
 
 template <int MODE, bool F32> int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, const FewWork& f, bool capped, cudaStream_t stream) {
-  return capped ? launch_few<MODE, true, F32>(mt, mx, f, stream) : launch_few<MODE, false, F32>(mt, mx, f, stream);
+  if constexpr (MODE == LOGSUM && !F32) {
+    if (f.k > LONG_STEPS * BK) return capped ? launch_few<MODE, true, F32, true>(mt, mx, f, stream) : launch_few<MODE, false, F32, true>(mt, mx, f, stream);
+  }
+  return capped ? launch_few<MODE, true, F32, F32>(mt, mx, f, stream) : launch_few<MODE, false, F32, F32>(mt, mx, f, stream);
 }
 
 // Both operands' maps for few rows: the table [vocab, width] as it lies, the rows in planes.
@@ -1420,7 +1427,9 @@ int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_
     w.m = rows;
     w.n = vocab;
     w.k = width;
-    status = launch<LOGSUM, bf16, sizeof(T) == 4>(ma, mb, ma, w, (l.rows_up / 256) * (up(vocab, BN) / BN), softcap > 0.f, stream);
+    const long long tiles = (l.rows_up / 256) * (up(vocab, BN) / BN);
+    if (sizeof(T) == 2 && width > LONG_STEPS * BK) status = launch<LOGSUM, bf16, false, LONG_CHUNK>(ma, mb, ma, w, tiles, softcap > 0.f, stream);
+    else status = launch<LOGSUM, bf16, sizeof(T) == 4>(ma, mb, ma, w, tiles, softcap > 0.f, stream);
     parts = int(up(vocab, BN) / BN) * 2;
   }
   if (status != R2_OK) return status;

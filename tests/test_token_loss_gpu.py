@@ -462,3 +462,22 @@ def test_gradients_captured_into_a_graph():
     torch.cuda.synchronize()
     want = step()
     assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,width,vocab,softcap", [(1, 1600, 1000, 0.0), (20, 1032, 900, 25.0), (128, 2500, 700, 0.0), (300, 1600, 1500, 0.0), (260, 4100, 400, 30.0)])
+def test_long_rows(rows, width, vocab, softcap, dtype):
+    Case(rows, width, vocab, dtype, 32, softcap=softcap).check()
+
+
+@pytest.mark.parametrize("rows", [100, 300])
+def test_float32_is_no_further_off_than_float32_sums(rows):
+    """What rounds towards zero 96 times and more shows as a bias: the logits of one token, 1,536 products each, against 64 bits, beside torch's own
+    (whose error is what rounding to nearest leaves)."""
+    g = gen(33)
+    x, w = torch.randn(rows, 1536, generator=g, device=DEV), torch.randn(1, 1536, generator=g, device=DEV)
+    exact = (x.double() @ w.double().t())[:, 0]
+    _, log_sum = ops().token_loss(x, w, torch.zeros(rows, dtype=torch.int32, device=DEV))
+    size = exact.pow(2).mean().sqrt()
+    # six pieces of 256 products: 16 additions of up to a unit each to a part of it, which grows; half of the units' mean, rounding to nearest above
+    assert (log_sum.double() - exact).pow(2).mean().sqrt() <= 16 * 2.0**-24 * size
