@@ -1301,7 +1301,8 @@ int row_blocks(long long rows) { return int(rows < 8 * 4736 ? (rows + 7) / 8 : 4
 constexpr long long FACTOR_BYTES = 256ll << 20;   // of dz at a time
 
 struct Layout {
-  int size, planes;                 // of a number; bfloat16 planes of an operand
+  int planes;                       // bfloat16 planes of an operand
+  bool copied;                      // the table's planes are in the scratch; else it is read where it lies
   long long rows_up, width_up;      // rows to a multiple of 256, numbers to one of 8
   int pieces, splits;
   long long piece;                  // tokens at a time, a multiple of 256
@@ -1309,9 +1310,17 @@ struct Layout {
   long long table, hidden, part, factors, shares, targets, factor, sums, place, count, total;
 };
 
-Layout layout(int dtype, long long rows, long long width, long long vocab, bool gradient) {
+bool copies_read(const void* at, long long ld, long long rows, long long width, int size = 2) {
+  return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (rows <= 1 || (ld * size % 16 == 0 && ld >= width));
+}
+
+// Up to FEW rows read a table as it lies, in either type, where tensor copies can. (The hidden rows' gradient reads float32's planes all the same.)
+bool few_rows(int dtype, const void* table, long long ld_t, long long rows, long long width, long long vocab) {
+  return rows <= FEW && (dtype == R2_BF16 || copies_read(table, ld_t, vocab, width, 4));
+}
+
+Layout layout(int dtype, const void* table, long long ld_t, long long rows, long long width, long long vocab, bool gradient, bool d_hidden) {
   Layout l = {};
-  l.size = dtype == R2_F32 ? 4 : 2;
   l.planes = dtype == R2_F32 ? 3 : 1;
   l.rows_up = up(rows, 256);
   l.width_up = up(width, 8);
@@ -1321,12 +1330,12 @@ Layout layout(int dtype, long long rows, long long width, long long vocab, bool 
     at += up(bytes, 256);
     return begin;
   };
-  // (a bfloat16 table is read where it lies if tensor copies can; there is room for it in either case)
-  l.table = take(l.planes * vocab * l.width_up * 2);
+  const bool few = few_rows(dtype, table, ld_t, rows, width, vocab);
+  l.copied = dtype == R2_BF16 ? !copies_read(table, ld_t, vocab, width) : !few || d_hidden;
+  l.table = take(l.copied ? l.planes * vocab * l.width_up * 2 : 0);
   l.hidden = take(l.planes * l.rows_up * l.width_up * 2);
   if (!gradient) {
-    l.parts = rows <= FEW ? few_ctas(vocab) * 4 : up(vocab, BN) / BN * 2;
-    if (l.parts < up(vocab, BN) / BN * 2) l.parts = up(vocab, BN) / BN * 2;   // (whichever kernel it is)
+    l.parts = few ? few_ctas(vocab) * 4 : up(vocab, BN) / BN * 2;
     l.part = take(l.parts * rows * 8);
   } else {
     const int pairs = resident_pairs(), terms = l.planes * (l.planes + 1) / 2;
@@ -1361,7 +1370,7 @@ Layout layout(int dtype, long long rows, long long width, long long vocab, bool 
       }
     }
     l.factors = take(l.planes * l.rows_up * l.piece * 2);
-    l.shares = take(l.splits * l.rows_up * l.width_up * 4);
+    l.shares = take(d_hidden ? l.splits * l.rows_up * l.width_up * 4 : 0);
     l.targets = take(l.rows_up * 4);
     l.factor = take(l.rows_up * 4);
     l.sums = take(l.rows_up * 4);
@@ -1370,10 +1379,6 @@ Layout layout(int dtype, long long rows, long long width, long long vocab, bool 
   }
   l.total = at;
   return l;
-}
-
-bool copies_read(const void* at, long long ld, long long rows, long long width, int size = 2) {
-  return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (rows <= 1 || (ld * size % 16 == 0 && ld >= width));
 }
 
 // The matrix itself where tensor copies can read it, else planes of it in `space`.
@@ -1395,15 +1400,16 @@ void set_cap(Work& w, float softcap) {
 template <typename T>
 int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_t, int rows, int width, int vocab, const int32_t* targets, const float* weight,
             float softcap, float* loss, float* log_sum, char* space, int* error, cudaStream_t stream) {
-  const Layout l = layout(sizeof(T) == 4 ? R2_F32 : R2_BF16, rows, width, vocab, false);
+  constexpr int dtype = sizeof(T) == 4 ? R2_F32 : R2_BF16;
+  const Layout l = layout(dtype, table, ld_t, rows, width, vocab, false, false);
   const Operand x = operand<T>(hidden, ld_h, rows, width, l, space + l.hidden, stream);
   Work w = {};
   w.part = reinterpret_cast<float2*>(space + l.part);
   w.error_flag = error;
   set_cap(w, softcap);
   CUtensorMap ma, mb;
-  int status, parts;
-  if (rows <= FEW && (sizeof(T) == 2 || copies_read(table, ld_t, vocab, width, 4))) {
+  int status;
+  if (few_rows(dtype, table, ld_t, rows, width, vocab)) {
     const void* at = table;
     long long ld = vocab > 1 ? ld_t : l.width_up;
     if (sizeof(T) == 2) {
@@ -1419,7 +1425,6 @@ int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_
     f.w = w;
     if (!make_few_maps<T>(&mb, &ma, at, ld, vocab, x, width, rows, f.columns)) return R2_BAD_ALIGN;
     status = launch_few<LOGSUM, sizeof(T) == 4>(mb, ma, f, softcap > 0.f, stream);
-    parts = few_ctas(vocab) * 4;
   } else {
     const Operand t = operand<T>(table, ld_t, vocab, width, l, space + l.table, stream);
     if (!make_map(&ma, x, width, rows, BM) || !make_map(&mb, t, width, vocab, HALF)) return R2_BAD_ALIGN;
@@ -1429,21 +1434,21 @@ int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_
     const long long tiles = (l.rows_up / 256) * (up(vocab, BN) / BN);
     if (sizeof(T) == 2 && width > LONG_STEPS * BK) status = launch<LOGSUM, bf16, false, LONG_CHUNK>(ma, mb, ma, w, tiles, softcap > 0.f, stream);
     else status = launch<LOGSUM, bf16, sizeof(T) == 4>(ma, mb, ma, w, tiles, softcap > 0.f, stream);
-    parts = int(up(vocab, BN) / BN) * 2;
   }
   if (status != R2_OK) return status;
   const T *h = static_cast<const T*>(hidden), *tab = static_cast<const T*>(table);
-  r2_launch(finish_kernel<T>, dim3((rows + 7) / 8), dim3(256), size_t(0), stream, static_cast<const float2*>(w.part), parts, h, ld_h, tab, ld_t, targets, weight, rows, width, vocab, softcap, loss, log_sum);
+  r2_launch(finish_kernel<T>, dim3((rows + 7) / 8), dim3(256), size_t(0), stream, static_cast<const float2*>(w.part), int(l.parts), h, ld_h, tab, ld_t, targets, weight, rows, width, vocab, softcap, loss, log_sum);
   return launch_status();
 }
 
 template <typename T>
 int gradient_of(const void* hidden, long long ld_h, const void* table, long long ld_t, int rows, int width, int vocab, const int32_t* targets, const float* weight,
                 const float* log_sum, float softcap, void* d_hidden, long long ld_dh, void* d_table, long long ld_dt, char* space, int* error, cudaStream_t stream) {
-  const Layout l = layout(sizeof(T) == 4 ? R2_F32 : R2_BF16, rows, width, vocab, true);
-  const bool few = rows <= FEW && (sizeof(T) == 2 || copies_read(table, ld_t, vocab, width, 4));
+  constexpr int dtype = sizeof(T) == 4 ? R2_F32 : R2_BF16;
+  const Layout l = layout(dtype, table, ld_t, rows, width, vocab, true, d_hidden != nullptr);
+  const bool few = few_rows(dtype, table, ld_t, rows, width, vocab);
   Operand t = {};   // (few float32 rows read the table as it is for their factors)
-  if (!few || sizeof(T) == 2 || d_hidden) t = operand<T>(table, ld_t, vocab, width, l, space + l.table, stream);
+  if (sizeof(T) == 2 || l.copied) t = operand<T>(table, ld_t, vocab, width, l, space + l.table, stream);
   bf16* gathered = reinterpret_cast<bf16*>(space + l.hidden);
   const Operand x = {gathered, l.width_up, l.rows_up * l.width_up, l.planes};
   int* count = reinterpret_cast<int*>(space + l.count);
@@ -1533,9 +1538,9 @@ constexpr int MOST = 1 << 30;   // rows, numbers of a row, tokens: indexes of ti
 
 }  // namespace
 
-// Bytes of scratch for a call (of a loss, or of gradients).
-extern "C" long long r2_token_loss_space(int dtype, int rows, int width, int vocab, int gradient) {
-  return layout(dtype, rows, width, vocab, gradient != 0).total;
+// Bytes of scratch for a call: of a loss, or (`gradient`) of gradients, of the hidden rows' (`d_hidden`) or of the table's alone.
+extern "C" long long r2_token_loss_space(int dtype, const void* table, long long ld_t, int rows, int width, int vocab, int gradient, int d_hidden) {
+  return layout(dtype, table, ld_t, rows, width, vocab, gradient != 0, d_hidden != 0).total;
 }
 
 // `space`: 256-byte aligned, r2_token_loss_space bytes.

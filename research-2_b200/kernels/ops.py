@@ -1942,7 +1942,7 @@ _LOGIT_SIGNATURES = {
                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
     "token_loss_gradient": [C.c_int, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
                             C.c_float, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p],
-    "token_loss_space": [C.c_int] * 5,
+    "token_loss_space": [C.c_int, C.c_void_p, C.c_longlong] + [C.c_int] * 5,
     "token_rows": [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float, C.c_void_p],
     "token_rows_gradient": [C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int,
                             C.c_void_p, C.c_void_p],
@@ -2246,6 +2246,8 @@ def _matrix(t: torch.Tensor, name: str, what: str) -> tuple[int, int, int, int, 
     """(type's code, rows, width, row stride, device) of a matrix of numbers whose rows are contiguous."""
     if t.dim() != 2:
         raise KernelError(f"{what}: {name} must have 2 dimensions, got shape {tuple(t.shape)}")
+    if t.shape[0] > 2**30 or t.shape[1] > 2**30:
+        raise KernelError(f"{what}: {name} may have 2^30 rows and columns at most, got shape {tuple(t.shape)}")
     dtype, device = t.dtype, t.get_device()
     if device < 0:
         raise KernelError(f"{what}: {name} must be a CUDA tensor (there is no CPU path)")
@@ -2288,14 +2290,15 @@ def token_loss(hidden: torch.Tensor, table: torch.Tensor, targets: torch.Tensor,
     `targets` int32 [N] the tokens. With z = hidden @ table^T (`softcap` > 0: softcap * tanh(z / softcap)), log_sum is the logarithm of a row's
     sum of exp(z), and loss = weight * (log_sum - z[target]), minus the token's log-probability at weight 1 (`weight` float32 [N]; None: 1). A target outside
     [0, V) (-1 or -100, say) is none: its row has the loss 0, as has a row of weight 0. Logits that hold +inf or NaN, or nothing but -inf, make a
-    row's log_sum and loss NaN or infinite, and no other row's."""
+    row's log_sum and loss NaN or infinite, and no other row's. (float32 products are made of bfloat16 planes, which hold no infinities: an infinite number of a float32 table
+    counts as 3.39e38, and a float32 hidden row with one has the log_sum NaN.)"""
     code, rows, width, ld, vocab, table_ld, device, targets_at, weight_at, softcap = _loss_arguments(hidden, table, targets, weight, softcap, "token_loss")
     where = hidden.device
     loss = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=where)
     log_sum = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=where)
     if rows:
         stream = _current_stream(device)
-        space = _space(where, _logit_entry("token_loss_space")(code, rows, width, vocab, 0))
+        space = _space(where, _logit_entry("token_loss_space")(code, table.data_ptr(), table_ld, rows, width, vocab, 0, 0))
         _check(_logit_entry("token_loss")(code, hidden.data_ptr(), ld, table.data_ptr(), table_ld, rows, width, vocab, targets_at, weight_at, softcap,
                                           loss.data_ptr(), log_sum.data_ptr(), space.data_ptr(), _workspace(where).error.data_ptr(), stream), "token_loss")
     return loss, log_sum
@@ -2318,7 +2321,7 @@ def token_loss_gradient(hidden: torch.Tensor, table: torch.Tensor, targets: torc
     d_table = torch.empty_strided((vocab, width), (width, 1), dtype=table.dtype, device=where) if table_gradient else None
     if hidden_gradient or table_gradient:
         stream = _current_stream(device)
-        space = _space(where, _logit_entry("token_loss_space")(code, rows, width, vocab, 1))
+        space = _space(where, _logit_entry("token_loss_space")(code, table.data_ptr(), table_ld, rows, width, vocab, 1, int(hidden_gradient)))
         _check(_logit_entry("token_loss_gradient")(
             code, hidden.data_ptr(), ld, table.data_ptr(), table_ld, rows, width, vocab, targets_at, weight_at, log_sum_at, softcap,
             d_hidden.data_ptr() if hidden_gradient else 0, width, d_table.data_ptr() if table_gradient else 0, width, space.data_ptr(),
@@ -2339,6 +2342,8 @@ def token_rows(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, ou
     code, vocab, width, ld, device = _matrix(table, "table", "token_rows")
     tokens = ids.shape[0] if ids.dim() == 1 else -1
     ids_at = _per_row(ids, "ids", torch.int32, tokens, device)
+    if tokens > 2**30:
+        raise KernelError(f"token_rows: {tokens} tokens, 2^30 at most")
     scale, out_dtype = _scale(scale, "token_rows"), out_dtype or table.dtype
     out = torch.empty_strided((tokens, width), (width, 1), dtype=out_dtype, device=table.device)
     out_code = dtype_code(out_dtype)
@@ -2362,8 +2367,8 @@ def token_rows_gradient(ids: torch.Tensor, above: torch.Tensor, vocab: int, *, s
         vocab = operator.index(vocab)
     except TypeError:
         raise KernelError(f"token_rows_gradient: vocab must be a whole number, got {vocab!r}") from None
-    if not 1 <= vocab < 2**31:
-        raise KernelError(f"token_rows_gradient: vocab must be in [1, 2^31), got {vocab}")
+    if not 1 <= vocab <= 2**30:
+        raise KernelError(f"token_rows_gradient: vocab must be in [1, 2^30], got {vocab}")
     scale = _scale(scale, "token_rows_gradient")
     if into is None:
         out_dtype = out_dtype or above.dtype

@@ -481,3 +481,25 @@ def test_float32_is_no_further_off_than_float32_sums(rows):
     size = exact.pow(2).mean().sqrt()
     # six pieces of 256 products: 16 additions of up to a unit each to a part of it, which grows; half of the units' mean, rounding to nearest above
     assert (log_sum.double() - exact).pow(2).mean().sqrt() <= 16 * 2.0**-24 * size
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_table_that_is_read_where_it_lies_is_not_copied(dtype):
+    rows, width, vocab = 64, 256, 20000
+    c = Case(rows, width, vocab, dtype, 23)
+    c.run()
+
+    def extra(call):
+        before = torch.cuda.memory_allocated(DEV)
+        torch.cuda.reset_peak_memory_stats(DEV)
+        out = call()
+        peak = torch.cuda.max_memory_allocated(DEV) - before
+        return out, peak - sum(t.numel() * t.element_size() for t in out if t is not None)
+
+    table, planes = vocab * width * c.table.element_size(), 1 if dtype is BF16 else 3
+    (loss, log_sum), most = extra(lambda: ops().token_loss(c.hidden, c.table, c.targets))
+    assert most < table / 4
+    # the gradient's factors are bfloat16 [256, vocab] in as many planes, the rows as many of [256, width]
+    factors = 256 * (vocab + 256 + width) * 2 * planes
+    _, most = extra(lambda: ops().token_loss_gradient(c.hidden, c.table, c.targets, log_sum, hidden_gradient=False))
+    assert most < factors + table / 4
