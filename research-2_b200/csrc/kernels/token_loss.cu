@@ -548,7 +548,12 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
 constexpr int FEW = 128;            // rows at most
 constexpr int FEW_STAGES = 8;       // of operands, at most
 constexpr int TURNED = 132;         // floats of a row of the turned tile (128 tokens and four of padding)
-constexpr int FEW_CHUNK = 8;        // steps of k that are added in tensor memory before their sum goes to the turned tile: 256 of k in float32; 512 of more than 1,024 in bfloat16
+constexpr int FEW_CHUNK = 8;        // steps of k that are added in tensor memory before their sum is rounded: 256 of k in float32; 512 of more than 1,024 in bfloat16
+
+// Groups of four warps that split float32 numbers, and stages of planes. At GPT-2's table, a call with cold caches: 96 rows with two groups 66.6 us, three 68.6; 16 rows with three,
+// four and five stages 56 to 58. (Without five of the six products 52 and 58, without the splitting 54 and 63: no part of a step bounds it alone.)
+constexpr int GROUPS = 2, F32_STAGES = 3;
+constexpr int few_threads(bool f32) { return 192 + (f32 ? GROUPS * 128 : 0); }
 
 struct FewWork {
   int rows, columns;                // of the batch; a multiple of 16: columns of the accumulator
@@ -578,26 +583,28 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
 template <bool F32> __host__ __device__ inline uint32_t few_stage_bytes(int columns) {
   return F32 ? 3u * (8192u + uint32_t(columns) * 64u) : 16384u + uint32_t(columns) * 128u;
 }
-template <bool SUMS> __host__ __device__ inline uint32_t turned_bytes(int columns) { return uint32_t(SUMS ? (columns + 31) / 32 * 32 : 32) * TURNED * 4; }
-template <bool F32, bool SUMS> __host__ __device__ inline uint32_t few_smem(int columns, int stages, int loads) {
-  return 1024u + uint32_t(stages) * few_stage_bytes<F32>(columns) + (F32 ? uint32_t(loads) * 16384u : 0u) + turned_bytes<SUMS>(columns) + (4 * FEW_STAGES + 4) * 8 + 16;
+constexpr uint32_t TURNED_BYTES = 32 * TURNED * 4;
+template <bool F32> __host__ __device__ inline uint32_t few_smem(int columns, int stages, int loads) {
+  return 1024u + uint32_t(stages) * few_stage_bytes<F32>(columns) + (F32 ? uint32_t(loads) * 16384u : 0u) + TURNED_BYTES + (4 * FEW_STAGES + 4) * 8 + 16;
 }
 
 template <int MODE, bool CAPPED, bool F32, bool SUMS>
-__global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_x, const FewWork f) {
+__global__ void __launch_bounds__(few_threads(F32), 1) few_kernel(const __grid_constant__ CUtensorMap map_t, const __grid_constant__ CUtensorMap map_x, const FewWork f) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t stage_bytes = few_stage_bytes<F32>(f.columns);
   const uint32_t loads_at = smem_u32(smem), stages_at = loads_at + (F32 ? uint32_t(f.loads) * 16384u : 0u);
   float* turned = reinterpret_cast<float*>(smem + (stages_at - loads_at) + size_t(f.stages) * stage_bytes);
-  const uint32_t full = smem_u32(turned) + turned_bytes<SUMS>(f.columns), empty = full + FEW_STAGES * 8, loaded = empty + FEW_STAGES * 8, taken = loaded + FEW_STAGES * 8,
+  const uint32_t full = smem_u32(turned) + TURNED_BYTES, empty = full + FEW_STAGES * 8, loaded = empty + FEW_STAGES * 8, taken = loaded + FEW_STAGES * 8,
                  acc_full = taken + FEW_STAGES * 8, acc_empty = acc_full + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(turned) + turned_bytes<SUMS>(f.columns) + (4 * FEW_STAGES + 4) * 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(turned) + TURNED_BYTES + (4 * FEW_STAGES + 4) * 8);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // Two accumulators, in float32 two parts each: of the products of the first planes, and of the small ones, which would be cut off against it.
+  // Two accumulators, in float32 of two parts each: the products of the first planes, and the small ones, which would be cut off against them; behind them the
+  // sums of a tile's pieces. (More than 96 float32 rows have one: tensor memory has no columns for another.)
   const uint32_t apart = uint32_t(f.columns + 31) / 32 * 32, both = F32 ? 2 * apart : apart;
+  const uint32_t bufs = 2 * both + (SUMS ? apart : 0) <= 512 ? 2 : 1, sums_at = bufs * both;
   uint32_t tmem_cols = 32;
-  while (tmem_cols < 2u * both) tmem_cols <<= 1;
+  while (tmem_cols < sums_at + (SUMS ? apart : 0)) tmem_cols <<= 1;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < FEW_STAGES; ++s) {
@@ -671,8 +678,8 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
     bool ok = true;
     for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
       for (int lo = 0; lo < n_kb && ok; lo += per_sum, ++local) {
-        const uint32_t buf = local & 1u;
-        if (!warp_wait(acc_empty + buf * 8, ((local >> 1) & 1u) ^ 1u)) {
+        const uint32_t buf = local & (bufs - 1);
+        if (!warp_wait(acc_empty + buf * 8, ((local >> (bufs - 1)) & 1u) ^ 1u)) {
           if (lane == 0) atomicMax(f.w.error_flag, ERR_ACC);
           ok = false;
           break;
@@ -728,55 +735,60 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
     bool ok = true;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
       const int left = f.n - tile * 128 - part * 32;   // tokens of the thread's 32 that there are
-      // the sums of the pieces of k, in the turned tile of all rows (a lane its token's column)
       uint32_t buf = 0;
       for (int lo = 0; lo < n_kb; lo += per_sum) {
-        buf = local & 1u;
-        if (ok && !warp_wait(acc_full + buf * 8, (local >> 1) & 1u)) {
+        buf = local & (bufs - 1);
+        if (ok && !warp_wait(acc_full + buf * 8, (local >> (bufs - 1)) & 1u)) {
           if (lane == 0) atomicMax(f.w.error_flag, ERR_ACC);
           ok = false;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if constexpr (SUMS) {
+        if constexpr (SUMS) {   // the sum of the pieces of k so far
 #pragma unroll 1
-          for (int c = 0; c < int(apart); c += 32) {
-            uint32_t r[32], small[32];
-            tmem_load32(tmem + buf * both + uint32_t(c) + (uint32_t(q * 32) << 16), r);
-            if constexpr (F32) tmem_load32(tmem + buf * both + apart + uint32_t(c) + (uint32_t(q * 32) << 16), small);
-            tmem_load_wait(r);
-            if constexpr (F32) tmem_tie(small);
-            float* to = turned + c * TURNED + q * 32 + lane;
+          for (uint32_t c = uint32_t(q * 32) << 16; (c & 0xffffu) < apart; c += 32) {
+            uint32_t r[32], more[32];
+            tmem_load32(tmem + buf * both + c, r);
+            if constexpr (F32) {
+              tmem_load32(tmem + buf * both + apart + c, more);
+              tmem_load_wait(r);
+              tmem_tie(more);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float piece = F32 ? __uint_as_float(r[j]) + __uint_as_float(small[j]) : __uint_as_float(r[j]);
-              to[j * TURNED] = lo == 0 ? piece : to[j * TURNED] + piece;
+              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(more[j]));
             }
+            if (lo > 0) {
+              tmem_load32(tmem + sums_at + c, more);
+              tmem_load_wait(r);
+              tmem_tie(more);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(more[j]));
+            } else {
+              tmem_load_wait(r);
+            }
+            tmem_store32(tmem + sums_at + c, r);
           }
+          tmem_store_wait();
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
           if (lane == 0) mbar_arrive(acc_empty + buf * 8);
           ++local;
         }
       }
-      if constexpr (SUMS) asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
       for (int g = 0; g < FEW / 32; ++g) {
         if (g >= groups) break;
-        if constexpr (!SUMS) {
-          if (uint32_t(g * 32) < apart) {
-            uint32_t r[32];
-            tmem_load32(tmem + buf * both + uint32_t(g * 32) + (uint32_t(q * 32) << 16), r);
-            tmem_load_wait(r);
+        if (uint32_t(g * 32) < apart) {
+          uint32_t r[32];
+          tmem_load32(tmem + (SUMS ? sums_at : buf * both) + uint32_t(g * 32) + (uint32_t(q * 32) << 16), r);
+          tmem_load_wait(r);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) turned[j * TURNED + q * 32 + lane] = __uint_as_float(r[j]);
-          }
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+          for (int j = 0; j < 32; ++j) turned[j * TURNED + q * 32 + lane] = __uint_as_float(r[j]);
         }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
         const int row = g * 32 + lane;
         float v[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 x = *reinterpret_cast<const float4*>(turned + ((SUMS && uint32_t(g * 32) < apart ? g * 32 : 0) + lane) * TURNED + part * 32 + 4 * i);
+          const float4 x = *reinterpret_cast<const float4*>(turned + lane * TURNED + part * 32 + 4 * i);
           v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
         }
         if constexpr (MODE == LOGSUM) {
@@ -842,11 +854,9 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
             }
           }
         }
-        if constexpr (!SUMS) asm volatile("bar.sync 1, 128;" ::: "memory");   // (the turned tile is read)
+        asm volatile("bar.sync 1, 128;" ::: "memory");   // (the turned tile is read)
       }
-      if constexpr (SUMS) {
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-      } else {
+      if constexpr (!SUMS) {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(acc_empty + buf * 8);
@@ -861,7 +871,7 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
       }
     }
   } else if constexpr (F32) {
-    // ---- planes: a thread a token's 32 numbers; two groups of four warps take the steps in turn (what a step takes is a chain: half as long, each, it was no faster)
+    // ---- planes: a thread a token's 32 numbers; groups of four warps take the steps in turn
     const int group = (warp - 6) / 4, row = (warp - 6) % 4 * 32 + lane;
     const int steps = (tiles - int(blockIdx.x) + int(gridDim.x) - 1) / int(gridDim.x) * n_kb;   // of all this CTA's tiles
     int stage = 0, load = 0, kb = 0;
@@ -873,7 +883,7 @@ __global__ void __launch_bounds__(F32 ? 448 : 192, 1) few_kernel(const __grid_co
     };
     forward(group);
     bool ok = true;
-    for (int i = group; i < steps; i += 2, forward(2)) {
+    for (int i = group; i < steps; i += GROUPS, forward(GROUPS)) {
       if (!warp_wait(loaded + load * 8, load_parity)) {
         if (lane == 0) atomicMax(f.w.error_flag, ERR_FULL);
         ok = false;
@@ -1270,12 +1280,13 @@ int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, FewWork f, cudaStre
   static std::atomic<bool> done[64];
   const int status = allow_smem(kernel, most, done);
   if (status != R2_OK) return status;
-  f.stages = F32 ? 3 : FEW_STAGES;   // (float32: two stages fill while one is read; the rest of the memory keeps the table coming)
-  f.loads = F32 ? FEW_STAGES : 0;
-  while (f.loads > 2 && few_smem<F32, SUMS>(f.columns, f.stages, f.loads) > most) --f.loads;
-  while (f.stages > 2 && few_smem<F32, SUMS>(f.columns, f.stages, f.loads) > most) --f.stages;
-  while (F32 && f.loads < FEW_STAGES && few_smem<F32, SUMS>(f.columns, f.stages, f.loads + 1) <= most) ++f.loads;
-  r2_launch(kernel, dim3(few_ctas(f.n)), dim3(F32 ? 448 : 192), size_t(few_smem<F32, SUMS>(f.columns, f.stages, f.loads)), stream, mt, mx, f);
+  // float32: as many stages of planes as there are groups at least, and loads that go evenly into the groups, so that a group comes back to the barriers it has waited
+  // for (one that others have waited for could be two phases behind, which a wait by parity takes for done).
+  f.stages = F32 ? F32_STAGES : FEW_STAGES;
+  f.loads = F32 ? GROUPS : 0;
+  while (f.stages > (F32 ? GROUPS : 2) && few_smem<F32>(f.columns, f.stages, f.loads) > most) --f.stages;
+  while (F32 && f.loads + GROUPS <= FEW_STAGES && few_smem<F32>(f.columns, f.stages, f.loads + GROUPS) <= most) f.loads += GROUPS;
+  r2_launch(kernel, dim3(few_ctas(f.n)), dim3(few_threads(F32)), size_t(few_smem<F32>(f.columns, f.stages, f.loads)), stream, mt, mx, f);
   return launch_status();
 }
 
