@@ -1,4 +1,4 @@
-// The operators on rows of logits, called with tensors: what Python does for a call (checks, new tensors, the stream) in one step. A call
+// The operators on rows of logits and at the two ends of a token table, called with tensors: what Python does for a call (checks, new tensors, the stream) in one step. A call
 // through Python's checks and ctypes takes 12 to 15 us of host time, four fifths of it beside the launch; a step between a model and its next
 // token calls these on a few rows, whose kernels take 3 to 9 us.
 //
@@ -10,6 +10,7 @@
 #include <ATen/ops/empty_strided.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -24,11 +25,24 @@ using AdjustEntry = int (*)(int, const void*, long long, void*, long long, int, 
 using TopEntry = int (*)(int, const void*, long long, int, int, int, float, float*, int32_t*, float*, int*, cudaStream_t);
 using DistillEntry = int (*)(int, const void*, long long, int, int, const int32_t*, const float*, int, const float*, const float*, float, float*, void*,
                              long long, int*, cudaStream_t);
+using LossEntry = int (*)(int, const void*, long long, const void*, long long, int, int, int, const int32_t*, const float*, float, float*, float*, void*, int*, cudaStream_t);
+using LossGradientEntry = int (*)(int, const void*, long long, const void*, long long, int, int, int, const int32_t*, const float*, const float*, float, void*, long long, void*,
+                                  long long, void*, int*, cudaStream_t);
+using LossSpace = long long (*)(int, const void*, long long, int, int, int, int, int);
+using RowsEntry = int (*)(int, int, const int32_t*, const void*, long long, void*, long long, int, int, int, float, cudaStream_t);
+using RowsGradientEntry = int (*)(int, int, const int32_t*, const void*, long long, void*, long long, int, int, int, float, int, void*, cudaStream_t);
+using RowsSpace = long long (*)(int, int, int);
 AdjustEntry adjust_entry = nullptr;
 TopEntry top_entry = nullptr;
 DistillEntry distill_entry = nullptr;
+LossEntry loss_entry = nullptr;
+LossGradientEntry loss_gradient_entry = nullptr;
+LossSpace loss_space = nullptr;
+RowsEntry rows_entry = nullptr;
+RowsGradientEntry rows_gradient_entry = nullptr;
+RowsSpace rows_space = nullptr;
 
-constexpr int64_t MOST = 0x7fffffff, TOP_MOST = 256;
+constexpr int64_t MOST = 0x7fffffff, TOP_MOST = 256, TABLE_MOST = 1 << 30;
 
 // An argument as a tensor: nullptr for None. False: not plain.
 bool tensor_of(PyObject* o, const at::Tensor*& t) {
@@ -236,6 +250,133 @@ PyObject* distill(PyObject*, PyObject* const* arg, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// A factor or a limit.
+bool number_of(PyObject* o, double& v) {
+  if (!PyFloat_Check(o) && !PyLong_Check(o)) return false;
+  v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return std::isfinite(v) && std::isfinite(float(v));
+}
+
+// Hidden rows, their table, tokens, weights and the limit of the logits.
+struct Loss {
+  Rows x, w;
+  const int32_t* targets;
+  const float* weight;
+  double softcap;
+
+  bool of(PyObject* hidden, PyObject* table, PyObject* tokens, PyObject* weights, PyObject* cap) {
+    return x.of(hidden) && w.of(table) && w.code == x.code && w.vocab == x.vocab && w.device == x.device && x.rows <= TABLE_MOST && x.vocab <= TABLE_MOST &&
+           w.rows <= TABLE_MOST && tokens != Py_None && numbers(tokens, x, x.rows, targets) && numbers(weights, x, x.rows, weight) && number_of(cap, softcap) &&
+           (softcap == 0.0 || (softcap >= 1e-6 && softcap <= 1e30));
+  }
+  at::Tensor space(bool gradient, bool d_hidden) const {
+    return at::empty_strided({loss_space(x.code, w.t->data_ptr(), w.ld, int(x.rows), int(x.vocab), int(w.rows), gradient, d_hidden)}, {1}, x.like(at::kByte));
+  }
+};
+
+// (hidden, table, targets, weight, softcap, error word's address)
+PyObject* token_loss(PyObject*, PyObject* const* arg, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Loss l;
+  if (n_args != 6 || loss_entry == nullptr || loss_space == nullptr || !l.of(arg[0], arg[1], arg[2], arg[3], arg[4])) Py_RETURN_NONE;
+  int* error = static_cast<int*>(PyLong_AsVoidPtr(arg[5]));
+  at::Tensor loss = at::empty_strided({l.x.rows}, {1}, l.x.like(at::kFloat)), log_sum = at::empty_strided({l.x.rows}, {1}, l.x.like(at::kFloat)), space = l.space(false, false);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(l.x.device).stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = loss_entry(l.x.code, l.x.t->data_ptr(), l.x.ld, l.w.t->data_ptr(), l.w.ld, int(l.x.rows), int(l.x.vocab), int(l.w.rows), l.targets, l.weight, float(l.softcap),
+                      static_cast<float*>(loss.data_ptr()), static_cast<float*>(log_sum.data_ptr()), space.data_ptr(), error, stream);
+  Py_END_ALLOW_THREADS
+  return answer(status, loss, log_sum);
+  END_HANDLE_TH_ERRORS
+}
+
+// (hidden, table, targets, log_sum, weight, softcap, hidden_gradient, table_gradient, error word's address)
+PyObject* token_loss_gradient(PyObject*, PyObject* const* arg, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Loss l;
+  const float* log_sum;
+  if (n_args != 9 || loss_gradient_entry == nullptr || loss_space == nullptr || !l.of(arg[0], arg[1], arg[2], arg[4], arg[5]) || arg[3] == Py_None ||
+      !numbers(arg[3], l.x, l.x.rows, log_sum) || !PyBool_Check(arg[6]) || !PyBool_Check(arg[7]) || (arg[6] == Py_False && arg[7] == Py_False))
+    Py_RETURN_NONE;
+  int* error = static_cast<int*>(PyLong_AsVoidPtr(arg[8]));
+  const int64_t width = l.x.vocab;
+  const at::TensorOptions options = l.x.like(l.x.t->scalar_type());
+  at::Tensor d_hidden, d_table, space = l.space(true, arg[6] == Py_True);
+  if (arg[6] == Py_True) d_hidden = at::empty_strided({l.x.rows, width}, {width, 1}, options);
+  if (arg[7] == Py_True) d_table = at::empty_strided({l.w.rows, width}, {width, 1}, options);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(l.x.device).stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = loss_gradient_entry(l.x.code, l.x.t->data_ptr(), l.x.ld, l.w.t->data_ptr(), l.w.ld, int(l.x.rows), int(width), int(l.w.rows), l.targets, l.weight, log_sum,
+                               float(l.softcap), d_hidden.defined() ? d_hidden.data_ptr() : nullptr, width, d_table.defined() ? d_table.data_ptr() : nullptr, width,
+                               space.data_ptr(), error, stream);
+  Py_END_ALLOW_THREADS
+  return answer(status, d_hidden, d_table);
+  END_HANDLE_TH_ERRORS
+}
+
+// The type of new rows: None is the other rows'.
+bool type_of(PyObject* o, const Rows& x, at::ScalarType& type, int& code) {
+  if (o == Py_None) type = x.t->scalar_type();
+  else if (THPDtype_Check(o)) type = reinterpret_cast<THPDtype*>(o)->scalar_type;
+  else return false;
+  code = type == at::kFloat ? 0 : 1;
+  return type == at::kFloat || type == at::kBFloat16;
+}
+
+// (ids, table, scale, out_dtype)
+PyObject* token_rows(PyObject*, PyObject* const* arg, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Rows w;
+  const int32_t* ids;
+  double scale;
+  at::ScalarType type;
+  int code;
+  if (n_args != 4 || rows_entry == nullptr || !w.of(arg[1]) || w.rows > TABLE_MOST || w.vocab > TABLE_MOST || arg[0] == Py_None || !numbers(arg[0], w, 1, ids) ||
+      !number_of(arg[2], scale) || !type_of(arg[3], w, type, code))
+    Py_RETURN_NONE;
+  const int64_t tokens = THPVariable_Unpack(arg[0]).numel();
+  if (tokens > TABLE_MOST) Py_RETURN_NONE;
+  at::Tensor out = at::empty_strided({tokens, w.vocab}, {w.vocab, 1}, w.like(type));
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(w.device).stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = rows_entry(w.code, code, ids, w.t->data_ptr(), w.ld, out.data_ptr(), w.vocab, int(tokens), int(w.vocab), int(w.rows), float(scale), stream);
+  Py_END_ALLOW_THREADS
+  return answer(status, out);
+  END_HANDLE_TH_ERRORS
+}
+
+// (ids, above, vocab, scale, out_dtype): into a new table
+PyObject* token_rows_gradient(PyObject*, PyObject* const* arg, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Rows x;
+  const int32_t* ids;
+  double scale;
+  at::ScalarType type;
+  int code, over = 0;
+  if (n_args != 5 || rows_gradient_entry == nullptr || rows_space == nullptr || !x.of(arg[1]) || x.rows > TABLE_MOST || x.vocab > TABLE_MOST || arg[0] == Py_None ||
+      !numbers(arg[0], x, x.rows, ids) || THPVariable_Unpack(arg[0]).numel() != x.rows || !PyLong_CheckExact(arg[2]) || !number_of(arg[3], scale) ||
+      !type_of(arg[4], x, type, code))
+    Py_RETURN_NONE;
+  const long long vocab = PyLong_AsLongLongAndOverflow(arg[2], &over);
+  if (over != 0 || vocab < 1 || vocab > TABLE_MOST) Py_RETURN_NONE;
+  at::Tensor out = at::empty_strided({vocab, x.vocab}, {x.vocab, 1}, x.like(type)),
+             space = at::empty_strided({rows_space(int(x.rows), int(x.vocab), int(vocab))}, {1}, x.like(at::kByte));
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x.device).stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = rows_gradient_entry(x.code, code, ids, x.t->data_ptr(), x.ld, out.data_ptr(), x.vocab, int(x.rows), int(x.vocab), int(vocab), float(scale), 0, space.data_ptr(), stream);
+  Py_END_ALLOW_THREADS
+  return answer(status, out);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(name, address): the kernel library's entry that a face calls
 PyObject* bind(PyObject*, PyObject* const* arg, Py_ssize_t n_args) {
   if (n_args != 2 || !PyUnicode_Check(arg[0])) {
@@ -247,6 +388,12 @@ PyObject* bind(PyObject*, PyObject* const* arg, Py_ssize_t n_args) {
   if (PyUnicode_CompareWithASCIIString(arg[0], "adjust_logits") == 0) adjust_entry = reinterpret_cast<AdjustEntry>(address);
   else if (PyUnicode_CompareWithASCIIString(arg[0], "top_logits") == 0) top_entry = reinterpret_cast<TopEntry>(address);
   else if (PyUnicode_CompareWithASCIIString(arg[0], "distill") == 0) distill_entry = reinterpret_cast<DistillEntry>(address);
+  else if (PyUnicode_CompareWithASCIIString(arg[0], "token_loss") == 0) loss_entry = reinterpret_cast<LossEntry>(address);
+  else if (PyUnicode_CompareWithASCIIString(arg[0], "token_loss_gradient") == 0) loss_gradient_entry = reinterpret_cast<LossGradientEntry>(address);
+  else if (PyUnicode_CompareWithASCIIString(arg[0], "token_loss_space") == 0) loss_space = reinterpret_cast<LossSpace>(address);
+  else if (PyUnicode_CompareWithASCIIString(arg[0], "token_rows") == 0) rows_entry = reinterpret_cast<RowsEntry>(address);
+  else if (PyUnicode_CompareWithASCIIString(arg[0], "token_rows_gradient") == 0) rows_gradient_entry = reinterpret_cast<RowsGradientEntry>(address);
+  else if (PyUnicode_CompareWithASCIIString(arg[0], "token_rows_space") == 0) rows_space = reinterpret_cast<RowsSpace>(address);
   else {
     PyErr_SetString(PyExc_ValueError, "no such face");
     return nullptr;
@@ -259,7 +406,8 @@ constexpr PyMethodDef face(const char* name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
 }
 
-PyMethodDef methods[] = {face<adjust>("adjust_logits"), face<top>("top_logits"), face<distill>("distill"), face<bind>("bind"), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {face<adjust>("adjust_logits"), face<top>("top_logits"), face<distill>("distill"), face<token_loss>("token_loss"),
+                         face<token_loss_gradient>("token_loss_gradient"), face<token_rows>("token_rows"), face<token_rows_gradient>("token_rows_gradient"), face<bind>("bind"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "r2faces", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

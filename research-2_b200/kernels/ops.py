@@ -1951,6 +1951,8 @@ _LOGIT_SIGNATURES = {
 # where the library has another name than the entry
 _LOGIT_LIBRARIES = {"scale_rows": "distill", "token_loss_gradient": "token_loss", "token_loss_space": "token_loss", "token_rows_gradient": "token_rows",
                     "token_rows_space": "token_rows"}
+# whose bytes of scratch come from another entry
+_LOGIT_SPACES = {"token_loss": "token_loss_space", "token_loss_gradient": "token_loss_space", "token_rows_gradient": "token_rows_space"}
 _logit_entries: dict = {}
 
 
@@ -1999,11 +2001,12 @@ def _faces():
 
 def _logit_face(name: str):
     """The operator called with tensors (`csrc/faces`): (status, tensors ...) for a plain call, None for one that the checks here have to look at."""
-    face = _logit_faces.get(name)
-    if face is None or face[0] is not _libs.get(name):
-        entry, module = _logit_entry(name), _faces()
-        module.bind(name, C.cast(entry, C.c_void_p).value)
-        face = _logit_faces[name] = (_libs[name], getattr(module, name))
+    face, library = _logit_faces.get(name), _LOGIT_LIBRARIES.get(name, name)
+    if face is None or face[0] is not _libs.get(library):
+        module = _faces()
+        for entry in (name, _LOGIT_SPACES[name]) if name in _LOGIT_SPACES else (name,):
+            module.bind(entry, C.cast(_logit_entry(entry), C.c_void_p).value)
+        face = _logit_faces[name] = (_libs[library], getattr(module, name))
     return face[1]
 
 
@@ -2292,6 +2295,11 @@ def token_loss(hidden: torch.Tensor, table: torch.Tensor, targets: torch.Tensor,
     [0, V) (-1 or -100, say) is none: its row has the loss 0, as has a row of weight 0. Logits that hold +inf or NaN, or nothing but -inf, make a
     row's log_sum and loss NaN or infinite, and no other row's. (float32 products are made of bfloat16 planes, which hold no infinities: an infinite number of a float32 table
     counts as 3.39e38, and a float32 hidden row with one has the log_sum NaN.)"""
+    if hidden.is_cuda:
+        done = _logit_face("token_loss")(hidden, table, targets, weight, softcap, _error_address(hidden))
+        if done is not None:
+            _check(done[0], "token_loss")
+            return done[1:]
     code, rows, width, ld, vocab, table_ld, device, targets_at, weight_at, softcap = _loss_arguments(hidden, table, targets, weight, softcap, "token_loss")
     where = hidden.device
     loss = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=where)
@@ -2309,6 +2317,11 @@ def token_loss_gradient(hidden: torch.Tensor, table: torch.Tensor, targets: torc
     """The gradients of the sum of `token_loss`'s losses: (of the hidden rows [N, D], of the table [V, D]), in their types; None for one that is not
     asked for. `log_sum` is `token_loss`'s for the same hidden rows, table and softcap; the other arguments as there. A row without a target, or of weight 0,
     has the gradient 0 and no part in the table's, whatever its hidden numbers are."""
+    if hidden.is_cuda:
+        done = _logit_face("token_loss_gradient")(hidden, table, targets, log_sum, weight, softcap, hidden_gradient, table_gradient, _error_address(hidden))
+        if done is not None:
+            _check(done[0], "token_loss_gradient")
+            return done[1:]
     code, rows, width, ld, vocab, table_ld, device, targets_at, weight_at, softcap = _loss_arguments(hidden, table, targets, weight, softcap,
                                                                                                      "token_loss_gradient")
     log_sum_at = _per_row(log_sum, "log_sum", torch.float32, rows, device)
@@ -2339,6 +2352,11 @@ def _scale(scale: float, what: str) -> float:
 def token_rows(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """Rows of a table [V, D] (float32 or bfloat16; rows contiguous, any row stride) by tokens int32 [T], times `scale`: [T, D] in the table's
     type or `out_dtype`, computed in float32 and rounded once. A token outside [0, V) gets a row of zeros. (`embed` is the engine's form: float32, with positions, ids checked before.)"""
+    if table.is_cuda:
+        done = _logit_face("token_rows")(ids, table, scale, out_dtype)
+        if done is not None:
+            _check(done[0], "token_rows")
+            return done[1]
     code, vocab, width, ld, device = _matrix(table, "table", "token_rows")
     tokens = ids.shape[0] if ids.dim() == 1 else -1
     ids_at = _per_row(ids, "ids", torch.int32, tokens, device)
@@ -2359,6 +2377,11 @@ def token_rows_gradient(ids: torch.Tensor, above: torch.Tensor, vocab: int, *, s
     or bfloat16; rows contiguous, any row stride) at which `ids` (int32 [T]) is v, added in float32 in an order that the call's sizes and ids decide (that of the
     places, for 64 of them at most) and rounded once, so that the same call gives the same bits. It is a new table in `above`'s type or `out_dtype`, zero where no token came; or the sums are added to `into` [V, D] (float32 or
     bfloat16), whose rows without a token are left as they are: a tied table's gradient, begun by `token_loss_gradient`. Tokens outside [0, V) count for nothing."""
+    if above.is_cuda and into is None:
+        done = _logit_face("token_rows_gradient")(ids, above, vocab, scale, out_dtype)
+        if done is not None:
+            _check(done[0], "token_rows_gradient")
+            return done[1]
     code, tokens, width, ld, device = _matrix(above, "above", "token_rows_gradient")
     ids_at = _per_row(ids, "ids", torch.int32, tokens, device)
     if ids.shape[0] != tokens:
