@@ -220,9 +220,9 @@ __device__ __forceinline__ void tmem_row64(uint32_t taddr, float (&v)[64]) {
   }
 }
 
+// The work of pair `pair` of `n_pairs`.
 template <int MODE, bool CAPPED, typename T, bool PLANES, int CHUNKED>
-__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                              const __grid_constant__ CUtensorMap map_out, const Work w) {
+__device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_out, const Work& w, const int pair, const int n_pairs) {
   constexpr bool A_MN = MODE == TABLE, B_MN = MODE == ROWS || MODE == TABLE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -233,7 +233,6 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;   // the cluster lies along x
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -534,6 +533,25 @@ __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_consta
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(2 * BN)) : "memory");
   }
+}
+
+template <int MODE, bool CAPPED, typename T, bool PLANES, int CHUNKED>
+__global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                              const __grid_constant__ CUtensorMap map_out, const Work w) {
+  product<MODE, CAPPED, T, PLANES, CHUNKED>(map_a, map_b, map_out, w, int(blockIdx.x >> 1), int(gridDim.x >> 1));   // the cluster lies along x
+}
+
+// Both products with dz side by side, where their tiles do not fill the GPU together: a launch less, and neither waits for the other (16 float32 rows of 100, 1,031 tokens: loss and gradients 55 to 47 us with the copies of rows and table in one launch).
+struct Both {
+  CUtensorMap rows_a, rows_b, rows_out, table_a, table_b, table_out;
+  Work rows, table;
+  int rows_pairs;
+};
+
+template <typename T, bool PLANES, int CHUNKED> __global__ void __launch_bounds__(THREADS, 1) both_kernel(const __grid_constant__ Both b) {
+  const int pair = int(blockIdx.x >> 1), n_pairs = int(gridDim.x >> 1);
+  if (pair < b.rows_pairs) product<ROWS, false, float, PLANES, CHUNKED>(b.rows_a, b.rows_b, b.rows_out, b.rows, pair, b.rows_pairs);
+  else product<TABLE, false, T, PLANES, CHUNKED>(b.table_a, b.table_b, b.table_out, b.table, pair - b.rows_pairs, n_pairs - b.rows_pairs);
 }
 
 // ---- few rows: LOGSUM and FACTORS of up to 128 ----------------------------------------------
@@ -1047,15 +1065,48 @@ __global__ void __launch_bounds__(256) finish_kernel(const float2* part, int par
   }
 }
 
+// A matrix in planes of bfloat16 whose rows start at 16 bytes: float32 in three, bfloat16 that tensor copies cannot read in one.
+template <typename T> struct Planes {
+  const T* from;
+  long long ld;
+  int rows, width, blocks;
+  bf16* to;
+  long long ld_to, plane;
+};
+
+template <typename T> __device__ __forceinline__ void split_rows(const Planes<T>& p, int block) {
+  const int lane = threadIdx.x & 31;
+  const bool wide = rows_wide(p.from, p.ld, p.width);
+  for (long long r = block * 8LL + (threadIdx.x >> 5); r < p.rows; r += p.blocks * 8LL) {
+#pragma unroll 2
+    for (int c = lane * 8; c < p.width; c += 256) {
+      float v[8];
+      load8(p.from + r * p.ld, c, p.width, wide, v);
+      put_planes8<T>(p.to + r * p.ld_to + c, p.plane, v);
+    }
+  }
+}
+
+template <typename T> __global__ void __launch_bounds__(256) planes_kernel(const Planes<T> p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  split_rows(p, int(blockIdx.x));
+}
+
 // The rows that count (a token of the vocabulary, a weight that is not 0) side by side, their numbers in one plane or three, zeros behind them up to a
-// multiple of 256 rows; `place[r]` is where row r went, -1 for none. A block looks at all rows' tokens and takes its own.
+// multiple of 256 rows; `place[r]` is where row r went, -1 for none. A block looks at all rows' tokens and takes its own. Behind these blocks: the table's planes.
 template <typename T>
 __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long ld, int rows, int width, int vocab, int own, const int32_t* targets, const float* weight,
                                                      const float* log_sum, bf16* x, long long ld_x, long long plane, int32_t* y_out, float* f_out, float* s_out,
-                                                     int32_t* place, int* count) {
+                                                     int32_t* place, int* count, const Planes<T> table) {
   __shared__ int totals[2][8];
   pdl_launch_dependents();
   pdl_wait();
+  const int blocks = int(gridDim.x) - table.blocks;
+  if (int(blockIdx.x) >= blocks) {
+    split_rows(table, int(blockIdx.x) - blocks);
+    return;
+  }
   const int first = blockIdx.x * own, last = min(rows, first + own);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto counts = [&](int r) {
@@ -1110,24 +1161,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
     before += __popc(mask);
   }
   const int end = (all + 255) / 256 * 256;
-  for (int at = all + blockIdx.x + warp * gridDim.x; at < end; at += 8 * gridDim.x) copy(at, static_cast<const T*>(nullptr));
-}
-
-// A matrix in planes of bfloat16 whose rows start at 16 bytes: float32 in three, bfloat16 that tensor copies cannot read in one.
-template <typename T>
-__global__ void __launch_bounds__(256) planes_kernel(const T* from, long long ld, int rows, int width, bf16* to, long long ld_to, long long plane) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const bool wide = rows_wide(from, ld, width);
-  for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8LL) {
-#pragma unroll 2
-    for (int c = lane * 8; c < width; c += 256) {
-      float v[8];
-      load8(from + r * ld, c, width, wide, v);
-      put_planes8<T>(to + r * ld_to + c, plane, v);
-    }
-  }
+  for (int at = all + blockIdx.x + warp * blocks; at < end; at += 8 * blocks) copy(at, static_cast<const T*>(nullptr));
 }
 
 // The hidden rows' gradient: shares of a gathered row added in one order, zeros for the rows that were left out.
@@ -1223,15 +1257,11 @@ int resident_pairs() {
   return n;
 }
 
-template <int MODE, bool CAPPED, typename T, bool PLANES, int CHUNKED>
-int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Work& w, long long units, cudaStream_t stream) {
-  auto kernel = product_kernel<MODE, CAPPED, T, PLANES, CHUNKED>;
-  static std::atomic<bool> done[64];
+template <typename... P, typename... Args> int launch_pairs(void (*kernel)(P...), std::atomic<bool> (&done)[64], long long pairs, cudaStream_t stream, const Args&... args) {
   const int status = allow_smem(kernel, SMEM, done);
   if (status != R2_OK) return status;
-  const int pairs = resident_pairs();
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(2 * unsigned(units < pairs ? units : pairs), 1, 1);
+  config.gridDim = dim3(2 * unsigned(pairs), 1, 1);
   config.blockDim = dim3(THREADS);
   config.dynamicSmemBytes = SMEM;
   config.stream = stream;
@@ -1243,8 +1273,15 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attr;
   config.numAttrs = g_r2_pdl ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, ma, mb, mo, w);
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
   return e != cudaSuccess ? int(e) : launch_status();
+}
+
+template <int MODE, bool CAPPED, typename T, bool PLANES, int CHUNKED>
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Work& w, long long units, cudaStream_t stream) {
+  static std::atomic<bool> done[64];
+  const int pairs = resident_pairs();
+  return launch_pairs(product_kernel<MODE, CAPPED, T, PLANES, CHUNKED>, done, units < pairs ? units : pairs, stream, ma, mb, mo, w);
 }
 
 template <int MODE, typename T, bool PLANES, int CHUNKED = PLANES ? PLANES_CHUNK : 0>
@@ -1392,13 +1429,17 @@ Layout layout(int dtype, const void* table, long long ld_t, long long rows, long
   return l;
 }
 
-// The matrix itself where tensor copies can read it, else planes of it in `space`.
-template <typename T>
-Operand operand(const void* at, long long ld, long long rows, long long width, const Layout& l, char* space, cudaStream_t stream) {
+// The matrix itself where tensor copies can read it, else where its planes will be: `p` says how they are made.
+template <typename T> Operand operand(const void* at, long long ld, long long rows, long long width, const Layout& l, char* space, Planes<T>& p) {
   if (sizeof(T) == 2 && copies_read(at, ld, rows, width)) return {at, rows <= 1 ? l.width_up : ld, 0, 1};
-  bf16* to = reinterpret_cast<bf16*>(space);
-  r2_launch(planes_kernel<T>, dim3(row_blocks(rows)), dim3(256), size_t(0), stream, static_cast<const T*>(at), ld, int(rows), int(width), to, l.width_up, rows * l.width_up);
-  return {to, l.width_up, rows * l.width_up, l.planes};
+  p = {static_cast<const T*>(at), ld, int(rows), int(width), row_blocks(rows), reinterpret_cast<bf16*>(space), l.width_up, rows * l.width_up};
+  return {space, l.width_up, rows * l.width_up, l.planes};
+}
+template <typename T> Operand operand(const void* at, long long ld, long long rows, long long width, const Layout& l, char* space, cudaStream_t stream) {
+  Planes<T> p = {};
+  const Operand o = operand<T>(at, ld, rows, width, l, space, p);
+  if (p.blocks > 0) r2_launch(planes_kernel<T>, dim3(p.blocks), dim3(256), size_t(0), stream, p);
+  return o;
 }
 
 void set_cap(Work& w, float softcap) {
@@ -1459,16 +1500,17 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
   const Layout l = layout(dtype, table, ld_t, rows, width, vocab, true, d_hidden != nullptr);
   const bool few = few_rows(dtype, table, ld_t, rows, width, vocab);
   Operand t = {};   // (few float32 rows read the table as it is for their factors)
-  if (sizeof(T) == 2 || l.copied) t = operand<T>(table, ld_t, vocab, width, l, space + l.table, stream);
+  Planes<T> planes = {};
+  if (sizeof(T) == 2 || l.copied) t = operand<T>(table, ld_t, vocab, width, l, space + l.table, planes);
   bf16* gathered = reinterpret_cast<bf16*>(space + l.hidden);
   const Operand x = {gathered, l.width_up, l.rows_up * l.width_up, l.planes};
   int* count = reinterpret_cast<int*>(space + l.count);
   int32_t* place = reinterpret_cast<int32_t*>(space + l.place);
   int own = (rows + 591) / 592;
   own = own > 32 ? 32 : own;
-  r2_launch(gather_kernel<T>, dim3((rows + own - 1) / own), dim3(256), size_t(0), stream,
+  r2_launch(gather_kernel<T>, dim3((rows + own - 1) / own + planes.blocks), dim3(256), size_t(0), stream,
       static_cast<const T*>(hidden), ld_h, rows, width, vocab, own, targets, weight, log_sum, gathered, x.ld, x.plane, reinterpret_cast<int32_t*>(space + l.targets),
-      reinterpret_cast<float*>(space + l.factor), reinterpret_cast<float*>(space + l.sums), place, count);
+      reinterpret_cast<float*>(space + l.factor), reinterpret_cast<float*>(space + l.sums), place, count, planes);
   Work w = {};
   w.m = rows;
   w.count = count;
@@ -1480,7 +1522,7 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
   const Operand dz = {space + l.factors, l.piece, l.rows_up * l.piece, l.planes};
   float* shares = reinterpret_cast<float*>(space + l.shares);
   const long long share_plane = l.rows_up * l.width_up;
-  CUtensorMap ma, mb, mo;
+  CUtensorMap ma, mb, mo;   // of the factors
   int status = launch_status();
   const long long row_tiles = l.rows_up / 256, width_tiles = up(width, BN) / BN;
   for (long long first = 0; first < vocab && status == R2_OK; first += l.piece) {
@@ -1509,33 +1551,45 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
         return R2_BAD_ALIGN;
       status = launch<FACTORS, bf16, sizeof(T) == 4>(ma, mb, mo, w, row_tiles * (up(n, BN) / BN), softcap > 0.f, stream);
     }
-    if (status == R2_OK && d_hidden) {
-      Work d = w;
+    if (status != R2_OK) break;
+    Both b = {};
+    long long rows_units = 0, table_units = 0;
+    if (d_hidden) {
+      Work& d = b.rows = w;
       d.n = width;
       d.k = n;
       d.per_split = ((n + BK - 1) / BK + l.splits - 1) / l.splits;   // (the last piece is shorter)
       d.splits = l.splits;
       d.add = first > 0;
-      if (!make_map(&ma, dz, n, l.rows_up, BM) || !make_map(&mb, part, width, n, BK) ||
-          !make_out_map<float>(&mo, shares, width, l.rows_up, l.splits, l.width_up, share_plane))
+      if (!make_map(&b.rows_a, dz, n, l.rows_up, BM) || !make_map(&b.rows_b, part, width, n, BK) ||
+          !make_out_map<float>(&b.rows_out, shares, width, l.rows_up, l.splits, l.width_up, share_plane))
         return R2_BAD_ALIGN;
-      status = launch<ROWS, float, sizeof(T) == 4>(ma, mb, mo, d, row_tiles * width_tiles * d.splits, false, stream);
+      rows_units = row_tiles * width_tiles * d.splits;
     }
-    if (status == R2_OK && d_table) {
-      Work d = w;
+    if (d_table) {
+      Work& d = b.table = w;
       d.m = n;
       d.n = width;
       T* out = static_cast<T*>(d_table) + first * ld_dt;
-      if (!make_map(&ma, dz, n, l.rows_up, BK) || !make_map(&mb, x, width, l.rows_up, BK)) return R2_BAD_ALIGN;
+      if (!make_map(&b.table_a, dz, n, l.rows_up, BK) || !make_map(&b.table_b, x, width, l.rows_up, BK)) return R2_BAD_ALIGN;
       if (reinterpret_cast<uintptr_t>(out) % 16 == 0 && ld_dt * sizeof(T) % 16 == 0) {
-        if (!make_out_map<T>(&mo, out, width, n, 1, ld_dt, 0)) return R2_BAD_ALIGN;
+        if (!make_out_map<T>(&b.table_out, out, width, n, 1, ld_dt, 0)) return R2_BAD_ALIGN;
       } else {
-        mo = ma;
+        b.table_out = b.table_a;
         d.out = out;
         d.ld = ld_dt;
       }
-      status = launch<TABLE, T, sizeof(T) == 4>(ma, mb, mo, d, up(n, 256) / 256 * width_tiles, false, stream);
+      table_units = up(n, 256) / 256 * width_tiles;
     }
+    constexpr bool F32 = sizeof(T) == 4;
+    if (rows_units > 0 && table_units > 0 && rows_units + table_units <= resident_pairs()) {
+      static std::atomic<bool> done[64];
+      b.rows_pairs = int(rows_units);
+      status = launch_pairs(both_kernel<T, F32, F32 ? PLANES_CHUNK : 0>, done, rows_units + table_units, stream, b);
+      continue;
+    }
+    if (rows_units > 0) status = launch<ROWS, float, F32>(b.rows_a, b.rows_b, b.rows_out, b.rows, rows_units, false, stream);
+    if (status == R2_OK && table_units > 0) status = launch<TABLE, T, F32>(b.table_a, b.table_b, b.table_out, b.table, table_units, false, stream);
   }
   if (status == R2_OK && d_hidden) {
     r2_launch(join_kernel<T>, dim3(row_blocks(static_cast<long long>(rows) * ((width + 127) / 128))), dim3(256), size_t(0), stream, static_cast<const float*>(shares), l.splits, share_plane, l.width_up,
