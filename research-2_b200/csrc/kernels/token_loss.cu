@@ -12,7 +12,9 @@
 //   ROWS     dx: dz times the piece of the table, K split over the pairs where tiles are few; shares are float and added in one order (`join_kernel`)
 //   TABLE    dW: dz^T times the hidden rows, whole for each piece of the vocabulary and rounded once
 //
-// dz is rounded to bfloat16, the type of the gradients that it makes, so that both products run on the tensor cores at full rate.
+// dz is rounded to bfloat16, the type of the gradients that it makes, so that both products run on the tensor cores at full rate. Its largest number by far is often the token's
+// own, a_r (p - 1): what the rounding leaves of that one (`rest`) is kept in float and goes into dx where its shares are joined, and into dW where rows are few. (Without it either
+// gradient's error was that of two roundings, 1.44 times that of its own; of many rows dW's still is.)
 //
 // float32 operands are three bfloat16 planes each: x = x0 + x1 + x2 to the last bit (8 bits each), and a product is the six products x_i w_j
 // with i + j <= 2; what is left out is below 2^-24 of it. dz is kept in three planes then, too. The tensor cores add to an accumulator without rounding to nearest: each
@@ -44,6 +46,8 @@ constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = HALF * BK * 2;
 constexpr uint32_t SLAB = 32 * 128;   // 32 rows of 128 bytes on their way out; a warp has two
 constexpr size_t SMEM = 1024 + STAGES * size_t(A_BYTES + B_BYTES) + 2 * WARPS * SLAB + (2 * STAGES + 4) * 8 + 16;
 
+constexpr int FEW = 128;         // rows that go through the other kernel below, at most
+
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 constexpr int ERR_FULL = 1, ERR_EMPTY = 2, ERR_ACC = 3;   // codes of waits that ran out, as of the other products
@@ -59,7 +63,10 @@ struct Work {
   const int32_t* targets;    // FACTORS: of the gathered rows, with their factors and sums
   const float* factor;
   const float* log_sum;
-  int first;                 // FACTORS: the piece's first token
+  int first;                 // FACTORS, TABLE: the piece's first token
+  float* rest;               // bfloat16: what rounding left of dz at each row's token; FACTORS writes it, TABLE adds it where it is given
+  const bf16* x;             // TABLE with it: the gathered rows
+  long long ld_x;
   float2* part;              // LOGSUM: [half tile][row]: the largest z log2 e and the sum of 2^(z log2 e - it)
   void* out;                 // TABLE, where tensor copies cannot write it
   long long ld;
@@ -174,8 +181,8 @@ template <int MODE> __device__ __forceinline__ Unit unit_of(const Work& w, long 
 }
 
 // Steps of k that are added in tensor memory before their sum goes into registers (0: all): 256 of k with the products of planes; 512 where float results are
-// made of more than 1,024 bfloat16 products (1,600 of them: off by 2.4e-7 of the loss in place of 7.7e-7, and 5 % slower).
-constexpr int PLANES_CHUNK = 4, LONG_CHUNK = 8, LONG_STEPS = 16;
+// made of more than 768 bfloat16 products (1,024 of them: off by up to 1.2e-6 of the loss otherwise; 1,600: by 2.4e-7 in place of 7.7e-7, and 5 % slower).
+constexpr int PLANES_CHUNK = 4, LONG_CHUNK = 8, LONG_STEPS = 12;
 
 // How many times a unit's products go through an accumulator.
 template <int CHUNKED> __device__ __forceinline__ int sums_of(const Unit& u) {
@@ -381,6 +388,40 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
       }
       const int row0 = (u.row * 2 + int(rank)) * BM + q * 32;
       float top = -3.4028234663852886e38f, sum = 0.f;
+      // TABLE: what rounding left of dz at the tokens of the warp's 32 rows, in the order of the gathered rows (FEW of them at most; their tokens are asked for
+      // before the accumulator is waited for)
+      int token[FEW / 32];
+      if constexpr (MODE == TABLE && sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < FEW / 32; ++i) token[i] = w.rest != nullptr && 32 * i + lane < k ? w.targets[32 * i + lane] - w.first - row0 : -1;
+      }
+      auto add_rest = [&](int c, float (&v)[64]) {
+        if constexpr (MODE == TABLE && sizeof(T) == 2) {
+#pragma unroll
+          for (int i = 0; i < FEW / 32; ++i) {
+#pragma unroll 1
+            for (unsigned mask = __ballot_sync(0xffffffffu, token[i] >= 0 && token[i] < 32); mask != 0; mask &= mask - 1u) {
+              const int from = __ffs(int(mask)) - 1, to = __shfl_sync(0xffffffffu, token[i], from);
+              if (lane == to) {
+                const float rest = w.rest[32 * i + from];
+                const bf16* x = w.x + (32 * i + from) * w.ld_x + col0 + c;
+#pragma unroll
+                for (int p = 0; p < 8; ++p) {
+                  if (col0 + c + 8 * p < w.n) {   // (rows of whole eights)
+                    const uint4 q8 = *reinterpret_cast<const uint4*>(x + 8 * p);
+                    const uint32_t q2[4] = {q8.x, q8.y, q8.z, q8.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                      v[8 * p + 2 * j] = fmaf(rest, __uint_as_float(q2[j] << 16), v[8 * p + 2 * j]);
+                      v[8 * p + 2 * j + 1] = fmaf(rest, __uint_as_float(q2[j] & 0xffff0000u), v[8 * p + 2 * j + 1]);
+                    }
+                  }
+                }
+              }
+            }
+          }
+        }
+      };
       // 64 finished numbers of a row, from column c of the tile on
       auto finish = [&](int c, float (&v)[64]) {
         if constexpr (MODE == LOGSUM) {
@@ -422,6 +463,14 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
               for (int j = 0; j < 64; ++j) v[j] -= target == c + j ? size : 0.f;
             }
           }
+          if constexpr (!PLANES) {
+            if (learns && target >= c && target < c + 64) {
+              float rest = 0.f;
+#pragma unroll
+              for (int j = 0; j < 64; ++j) rest = target == c + j ? v[j] - __bfloat162float(__float2bfloat16_rn(v[j])) : rest;
+              w.rest[row] = factor < 0.f ? -rest : rest;
+            }
+          }
           for (int plane = 0; plane < (PLANES ? 3 : 1); ++plane) {
             const uint32_t slab = out.begin();
 #pragma unroll
@@ -441,11 +490,13 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
             out.end(&map_out, col0 + c, row0, plane, slab, false);
           }
         } else if (MODE == TABLE && w.out != nullptr) {
+          add_rest(c, v);
           T* to = static_cast<T*>(w.out) + row * w.ld + col0 + c;
 #pragma unroll
           for (int j = 0; j < 64; ++j)
             if (row < m && col0 + c + j < w.n) to[j] = from_float<T>(v[j]);
         } else if constexpr (sizeof(T) == 2 && MODE == TABLE) {
+          add_rest(c, v);
           const uint32_t slab = out.begin();
 #pragma unroll
           for (int p = 0; p < 8; ++p)
@@ -563,10 +614,9 @@ template <typename T, bool PLANES, int CHUNKED> __global__ void __launch_bounds_
 //
 // LOGSUM keeps a row's largest logit and sum for each of a CTA's four parts of 32 tokens over all its tiles.
 
-constexpr int FEW = 128;            // rows at most
 constexpr int FEW_STAGES = 8;       // of operands, at most
 constexpr int TURNED = 132;         // floats of a row of the turned tile (128 tokens and four of padding)
-constexpr int FEW_CHUNK = 8;        // steps of k that are added in tensor memory before their sum is rounded: 256 of k in float32; 512 of more than 1,024 in bfloat16
+constexpr int FEW_CHUNK = 256;      // of k are added in tensor memory before their sum is rounded (three bfloat16 rows of 768: loss off by 1.4e-6 without, 8e-7 with; same time)
 
 // Groups of four warps that split float32 numbers, and stages of planes. At GPT-2's table, a call with cold caches: 96 rows with two groups 66.6 us, three 68.6; 16 rows with three,
 // four and five stages 56 to 58. (Without five of the six products 52 and 58, without the splitting 54 and 63: no part of a step bounds it alone.)
@@ -652,7 +702,7 @@ __global__ void __launch_bounds__(few_threads(F32), 1) few_kernel(const __grid_c
   const int tiles = (f.n + 127) / 128;
   constexpr int STEP = F32 ? 32 : 64;   // of k
   const int n_kb = (f.k + STEP - 1) / STEP;
-  const int per_sum = SUMS ? FEW_CHUNK : n_kb;
+  const int per_sum = SUMS ? FEW_CHUNK / STEP : n_kb;
   const uint32_t x_bytes = uint32_t(f.columns) * STEP * 2;
 
   if (warp == 0) {
@@ -848,6 +898,14 @@ __global__ void __launch_bounds__(few_threads(F32), 1) few_kernel(const __grid_c
             } else {
               v[j] = fast_exp2(fmaf(v[j], LOG2E, -less2));
               if (learns) v[j] -= target == j ? size : 0.f;
+            }
+          }
+          if constexpr (!F32) {
+            if (learns) {
+              float rest = 0.f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) rest = target == j ? v[j] - __bfloat162float(__float2bfloat16_rn(v[j])) : rest;
+              f.w.rest[row] = factor < 0.f ? -rest : rest;
             }
           }
           const uint32_t sign = factor < 0.f ? 0x80008000u : 0u, held = row < m ? 0xffffffffu : 0u;
@@ -1164,10 +1222,11 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
   for (int at = all + blockIdx.x + warp * blocks; at < end; at += 8 * blocks) copy(at, static_cast<const T*>(nullptr));
 }
 
-// The hidden rows' gradient: shares of a gathered row added in one order, zeros for the rows that were left out.
+// The hidden rows' gradient: shares of a gathered row added in one order, and what rounding left of dz at its token (`rest`, null in float32) times the token's row of the
+// table; zeros for the rows that were left out.
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const float* shares, int splits, long long plane, long long ld, const int32_t* place, T* out, long long ld_o, int rows,
-                                                   int width) {
+__global__ void __launch_bounds__(256) join_kernel(const float* shares, int splits, long long plane, long long ld, const int32_t* place, const float* rest, const int32_t* targets,
+                                                   const T* table, long long ld_t, T* out, long long ld_o, int rows, int width) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, pieces = (width + 127) / 128;   // a warp a row's 128 numbers: the shares of a few rows are one chain of loads otherwise
@@ -1184,6 +1243,14 @@ __global__ void __launch_bounds__(256) join_kernel(const float* shares, int spli
       for (int j = 0; j < splits; ++j) {
         const float4 v = __ldg(reinterpret_cast<const float4*>(s + j * plane));
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+      }
+      if (sizeof(T) == 2) {
+        const T* t = table + targets[at] * ld_t + c;
+        const float left = rest[at];
+        sum.x = fmaf(left, to_float(t[0]), sum.x);
+        if (c + 1 < width) sum.y = fmaf(left, to_float(t[1]), sum.y);
+        if (c + 2 < width) sum.z = fmaf(left, to_float(t[2]), sum.z);
+        if (c + 3 < width) sum.w = fmaf(left, to_float(t[3]), sum.w);
       }
     }
     if (wide) {
@@ -1329,7 +1396,7 @@ int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, FewWork f, cudaStre
 
 template <int MODE, bool F32> int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, const FewWork& f, bool capped, cudaStream_t stream) {
   if constexpr (MODE == LOGSUM && !F32) {
-    if (f.k > LONG_STEPS * BK) return capped ? launch_few<MODE, true, F32, true>(mt, mx, f, stream) : launch_few<MODE, false, F32, true>(mt, mx, f, stream);
+    if (f.k > FEW_CHUNK) return capped ? launch_few<MODE, true, F32, true>(mt, mx, f, stream) : launch_few<MODE, false, F32, true>(mt, mx, f, stream);
   }
   return capped ? launch_few<MODE, true, F32, F32>(mt, mx, f, stream) : launch_few<MODE, false, F32, F32>(mt, mx, f, stream);
 }
@@ -1355,7 +1422,7 @@ struct Layout {
   int pieces, splits;
   long long piece;                  // tokens at a time, a multiple of 256
   long long parts;
-  long long table, hidden, part, factors, shares, targets, factor, sums, place, count, total;
+  long long table, hidden, part, factors, shares, targets, factor, sums, rest, place, count, total;
 };
 
 bool copies_read(const void* at, long long ld, long long rows, long long width, int size = 2) {
@@ -1422,6 +1489,7 @@ Layout layout(int dtype, const void* table, long long ld_t, long long rows, long
     l.targets = take(l.rows_up * 4);
     l.factor = take(l.rows_up * 4);
     l.sums = take(l.rows_up * 4);
+    l.rest = take(l.rows_up * 4);
     l.place = take(rows * 4);
     l.count = take(4);
   }
@@ -1517,6 +1585,7 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
   w.targets = reinterpret_cast<int32_t*>(space + l.targets);
   w.factor = reinterpret_cast<float*>(space + l.factor);
   w.log_sum = reinterpret_cast<float*>(space + l.sums);
+  w.rest = reinterpret_cast<float*>(space + l.rest);
   w.error_flag = error;
   set_cap(w, softcap);
   const Operand dz = {space + l.factors, l.piece, l.rows_up * l.piece, l.planes};
@@ -1568,6 +1637,9 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
     }
     if (d_table) {
       Work& d = b.table = w;
+      d.rest = few && sizeof(T) == 2 ? w.rest : nullptr;
+      d.x = gathered;
+      d.ld_x = x.ld;
       d.m = n;
       d.n = width;
       T* out = static_cast<T*>(d_table) + first * ld_dt;
@@ -1593,7 +1665,7 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
   }
   if (status == R2_OK && d_hidden) {
     r2_launch(join_kernel<T>, dim3(row_blocks(static_cast<long long>(rows) * ((width + 127) / 128))), dim3(256), size_t(0), stream, static_cast<const float*>(shares), l.splits, share_plane, l.width_up,
-              static_cast<const int32_t*>(place), static_cast<T*>(d_hidden), ld_dh, rows, width);
+              static_cast<const int32_t*>(place), static_cast<const float*>(w.rest), w.targets, static_cast<const T*>(table), ld_t, static_cast<T*>(d_hidden), ld_dh, rows, width);
     status = launch_status();
   }
   return status;

@@ -503,3 +503,30 @@ def test_a_table_that_is_read_where_it_lies_is_not_copied(dtype):
     factors = 256 * (vocab + 256 + width) * 2 * planes
     _, most = extra(lambda: ops().token_loss_gradient(c.hidden, c.table, c.targets, log_sum, hidden_gradient=False))
     assert most < factors + table / 4
+
+
+@pytest.mark.parametrize("rows,width,vocab", [(3, 768, 2000), (40, 64, 1500), (128, 200, 3000), (300, 96, 2500)])
+def test_what_rounding_leaves_of_a_tokens_own_factor_is_added(rows, width, vocab):
+    """bfloat16, tokens that the model finds unlikely: a row's factor is nearly all at its own token, a (p - 1). Its rounding, half a step of |a (p - 1)| times the row of the
+    other operand, is not in the hidden rows' gradient, and of up to 128 rows not in the table's: the tolerance is the oracle's without it (4 units of 2^-24 in its place)."""
+    c = Case(rows, width, vocab, BF16, rows, size=0.05)
+    got, want = c.run(), c.plain()
+    a = torch.where((c.targets >= 0) & (c.targets < vocab), c.weight.double(), 0.0)
+    y = c.targets.clamp(0, vocab - 1).long()
+    own = a * torch.expm1(want.z.gather(1, y[:, None])[:, 0] - want.log_sum)
+    less = (2.0**-8 - 4 * 2.0**-24) * own.abs()[:, None]
+    x, w = torch.where(a[:, None] != 0, c.hidden.double(), 0.0), c.table.double()
+    off = want.d_hidden_off - less * w[y].abs()
+    assert torch.all((got[2].double() - want.d_hidden).abs() <= off)
+    if rows <= 128:
+        off = want.d_table_off.index_add(0, y, -less * x.abs())
+        assert torch.all((got[3].double() - want.d_table).abs() <= off)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [100, 300])
+def test_one_token_for_all_rows(dtype, rows):
+    for token in (0, 40, 599):
+        c = Case(rows, 96, 600, dtype, 31)
+        c.targets[7:] = token
+        c.check()
