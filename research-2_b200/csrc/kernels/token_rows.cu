@@ -7,11 +7,11 @@
 //   deal_kernel  sorts the places by token, stable. The table's rows are dealt out to CTAs by the remainder of their number (tokens that stand often lie side
 //                by side in a vocabulary). A CTA goes through all tokens, a share a warp, and lists its own with their rank among the share's of their row, beside a
 //                count of those of lower deals, so that it knows where in the sorted list its part begins without a word between CTAs. Running sums of the shares' and rows'
-//                counts then say where each place goes. Meanwhile zeros go to the whole table in bulk copies from shared memory, without a look at which rows
-//                need them: that is most of what a small batch costs, and hides the sorting; the rows that are written twice are fewer than the places.
+//                counts then say where each place goes. Meanwhile zeros go to the table's first part in bulk copies from shared memory, without a look at which rows
+//                need them: they are most of what a small batch costs, and hide the sorting; the rows that are written twice are fewer than the places.
 //   sum_kernel   a CTA takes the sorted places of eight windows, a warp each, and up to 256 columns: a token that stands everywhere and tokens that stand once
 //                take the same time. A row whose places lie in several windows is joined in shared memory; one that goes on in other CTAs leaves float sums in
-//                memory, and the last of those CTAs adds them, in the order of the places whoever that is.
+//                memory, and the last of those CTAs adds them, in the order of the places whoever that is. Beside them, the other rows' zeros.
 //
 // Bound by the bytes of the rows from above and of the table.
 #include "common.cuh"
@@ -26,6 +26,11 @@ constexpr int MOST_ROWS = 1200;        // of a deal
 constexpr int LISTED_BYTES = DEAL_WARPS * LISTED * 8;
 constexpr int ZEROS = 16384;           // bytes of a bulk copy
 
+// Zeros that are written beside the sorting, as many as it takes time for (1,024 tokens, 154 MB: with 24, 32, 44 and 56 MB 28.2, 27.2, 26.7 and 27.1 us, with all 34.2; 4,096 tokens, 77
+// MB: 19.5, 20.4, 21.3, 22.5 and 22.0). The others go beside the sums, to rows that no token came for, if rows are long enough to be runs of bulk copies.
+constexpr long long EARLY_BYTES = 32 << 20, EARLY_BYTES_A_TOKEN = 4608, LONG_ROW = 512;
+constexpr int UNIT = 8;   // rows of a warp's step, a CTA an SM: what an SM can write bounds it, so all of them have to have the same
+
 struct Work {
   const int32_t* ids;
   const void* above;
@@ -39,11 +44,14 @@ struct Work {
   unsigned long long inverse;       // v / deals = v * inverse >> 64
   int32_t *row, *place;             // [tokens]: the sorted list: by deal, row and place
   int* held;                        // how many places hold a token
-  long long bytes;                  // of the table
+  int zero_ctas;                    // of the sums' launch, its first ones
+  int zero_from;                    // rows from this one on get zeros beside the sums, and only where no token came; those before it beside the sorting
+  uint32_t* has;                    // [deal][62]: bits of a deal's rows that a token came for, 32 even ones, 32 odd ones in turn
   int slices, slice, window;        // of the columns, columns of one, sorted places of a warp
   int* arrived;                     // [CTA of places][slice]: CTAs that have left their share of the row that goes on from this one
   float* shares;                    // [CTA of places][2][width_up]: sums of a row that an earlier CTA began; of one that the next goes on with
   int width_up, groups;             // (groups: CTAs of places)
+  int out_size;                     // bytes of a number of the table
 };
 
 // A lane's columns of a slice: pieces of 16 bytes, or every 32nd number.
@@ -126,6 +134,36 @@ __device__ __forceinline__ int quotient_of(unsigned long long v, unsigned long l
   return int((v * unsigned(inverse >> 32) + (v * unsigned(inverse) >> 32)) >> 32);
 }
 
+__device__ __forceinline__ long long row_bytes(const Work& w) { return static_cast<long long>(w.width) * w.out_size; }
+
+// Zeros for the rows from zero_from on that no token came for: runs of empty ones at once, in bulk copies between what is left of 16 bytes at a run's ends.
+__device__ __forceinline__ void write_zeros(const Work& w, uint4* zeros, int block, int blocks) {
+  const int lane = threadIdx.x & 31;
+  for (int j = threadIdx.x; j < ZEROS / 16; j += THREADS) zeros[j] = make_uint4(0, 0, 0, 0);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  const long long size = row_bytes(w);
+  for (long long first = w.zero_from + (block + (threadIdx.x >> 5) * blocks) * static_cast<long long>(UNIT); first < w.vocab; first += blocks * WARPS * static_cast<long long>(UNIT)) {
+    const bool there = lane < UNIT && first + lane < w.vocab;
+    const unsigned v = unsigned(there ? first + lane : first), row = unsigned(quotient_of(v, w.inverse)), deal = v - row * w.deals;
+    unsigned empty = __ballot_sync(0xffffffffu, there && (w.has[(deal * DEAL_WARPS + row / 64) * 2 + row % 2] >> (row / 2 % 32) & 1u) == 0);
+    while (empty != 0) {
+      const int begin = __ffs(int(empty)) - 1, rows = __ffs(int(~(empty >> begin) | (begin > 0 ? 1u << (32 - begin) : 0u))) - 1, n = rows < 0 ? 32 : rows;
+      empty &= n == 32 ? 0u : ~(((1u << n) - 1u) << begin);
+      char* at = static_cast<char*>(w.out) + (first + begin) * size;
+      const long long bytes = n * size, short_of_16 = -reinterpret_cast<intptr_t>(at) & 15, head = short_of_16 < bytes ? short_of_16 : bytes, whole = (bytes - head) / 16 * 16;
+      if (lane < head) at[lane] = 0;
+      for (long long o = lane * ZEROS; o < whole; o += 32 * ZEROS) {
+        const unsigned piece = unsigned(whole - o < ZEROS ? whole - o : ZEROS);
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(at + head + o), "r"(uint32_t(__cvta_generic_to_shared(zeros))), "r"(piece) : "memory");
+      }
+      if (head + whole + lane < bytes) at[head + whole + lane] = 0;
+    }
+  }
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
 __global__ void __launch_bounds__(DEAL_THREADS + 32, 1) deal_kernel(const Work w) {
   extern __shared__ int32_t shared[];
   __shared__ int mine[DEAL_WARPS], lower[DEAL_WARPS], running[DEAL_WARPS];
@@ -136,7 +174,7 @@ __global__ void __launch_bounds__(DEAL_THREADS + 32, 1) deal_kernel(const Work w
   uint32_t* list_row = reinterpret_cast<uint32_t*>(list_place + DEAL_WARPS * LISTED);   // row * LISTED + rank
   __shared__ alignas(16) uint4 zeros[ZEROS / 16];
   auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(DEAL_THREADS) : "memory"); };
-  pdl_launch_dependents();
+  if (w.zero_ctas == 0) pdl_launch_dependents();   // (CTAs that write zeros have to lie evenly on the SMs: started in what shared memory the sorting leaves, they took twice the time)
   if (warp == DEAL_WARPS) {
     // ---- zeros: the CTAs' pieces side by side, so that all of them write in one part of the table; a lane a piece
     if (w.add) return;
@@ -145,13 +183,13 @@ __global__ void __launch_bounds__(DEAL_THREADS + 32, 1) deal_kernel(const Work w
     __syncwarp();
     pdl_wait();
     char* out = static_cast<char*>(w.out);
-    const long long whole = w.bytes / 16 * 16;
+    const long long bytes = w.zero_from * row_bytes(w), whole = bytes / 16 * 16;
     for (long long at = (deal + static_cast<long long>(lane) * w.deals) * ZEROS; at < whole; at += 32ll * w.deals * ZEROS) {
       const unsigned n = unsigned(whole - at < ZEROS ? whole - at : ZEROS);
       asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(out + at), "r"(uint32_t(__cvta_generic_to_shared(zeros))), "r"(n) : "memory");
     }
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-    if (deal == 0 && whole + lane < w.bytes) out[whole + lane] = 0;
+    if (deal == 0 && whole + lane < bytes) out[whole + lane] = 0;
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     return;
   }
@@ -224,6 +262,9 @@ __global__ void __launch_bounds__(DEAL_THREADS + 32, 1) deal_kernel(const Work w
     if (j < rows) {
       for (int part = 0; part < DEAL_WARPS; ++part) of_row[i] += counts[part * rows + j];
     }
+    static_assert(PER == 2);
+    const unsigned bits = __ballot_sync(0xffffffffu, of_row[i] > 0);
+    if (lane == 0 && warp * 64 < rows && w.zero_from < w.vocab) w.has[(deal * DEAL_WARPS + warp) * 2 + i] = bits;
     own += of_row[i];
   }
   int up = own;
@@ -268,14 +309,22 @@ __global__ void __launch_bounds__(DEAL_THREADS + 32, 1) deal_kernel(const Work w
 
 template <typename T, typename O, bool WIDE, bool ADD>
 __global__ void __launch_bounds__(THREADS, 3) sum_kernel(const Work w) {
-  __shared__ float heads[WARPS][SLICE], tails[WARPS][SLICE];   // of a window: the sum of the row that an earlier one began; of the row that the next goes on with
+  __shared__ alignas(16) float ends[2][WARPS][SLICE];
+  auto &heads = ends[0], &tails = ends[1];                     // of a window: the sum of the row that an earlier one began; of the row that the next goes on with
   __shared__ int head_row[WARPS], tail_row[WARPS];             // -1: none
   __shared__ int last_of_chain;
   pdl_launch_dependents();
   pdl_wait();
+  if constexpr (!ADD) {
+    if (int(blockIdx.x) < w.zero_ctas) {
+      static_assert(sizeof(ends) == ZEROS);
+      write_zeros(w, reinterpret_cast<uint4*>(ends), int(blockIdx.x), w.zero_ctas);
+      return;
+    }
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int held = *w.held;
-  const int group = blockIdx.x / w.slices, slice = blockIdx.x % w.slices, span = WARPS * w.window;
+  const int block = int(blockIdx.x) - w.zero_ctas, group = block / w.slices, slice = block % w.slices, span = WARPS * w.window;
   const int col = slice * w.slice, width = min(w.slice, w.width - col);
   const int group_from = group * span;
   if (group_from >= held) return;
@@ -473,7 +522,7 @@ int launch_deal(const Work& w, cudaStream_t stream) {
 
 template <typename T, typename O, bool WIDE>
 int launch_sums(const Work& w, cudaStream_t stream) {
-  r2_launch(w.add ? sum_kernel<T, O, WIDE, true> : sum_kernel<T, O, WIDE, false>, dim3(unsigned(w.groups) * unsigned(w.slices)), dim3(THREADS), size_t(0), stream, w);
+  r2_launch(w.add ? sum_kernel<T, O, WIDE, true> : sum_kernel<T, O, WIDE, false>, dim3(unsigned(w.groups) * unsigned(w.slices) + unsigned(w.zero_ctas)), dim3(THREADS), size_t(0), stream, w);
   return launch_status();
 }
 
@@ -521,7 +570,7 @@ extern "C" long long r2_token_rows_space(int tokens, int width, int vocab) {
   w.width = width;
   w.vocab = vocab;
   share_out(w);
-  return 8ll * tokens + 16 + static_cast<long long>(w.groups) * (2ll * w.width_up + w.slices) * 4;
+  return 8ll * tokens + 16 + static_cast<long long>(w.groups) * (2ll * w.width_up + w.slices) * 4 + w.deals * (DEAL_WARPS * 8ll);
 }
 
 extern "C" int r2_token_rows_gradient(int dtype, int out_dtype, const int32_t* ids, const void* above, long long ld, void* out, long long ld_o, int tokens, int width,
@@ -539,7 +588,12 @@ extern "C" int r2_token_rows_gradient(int dtype, int out_dtype, const int32_t* i
   w.held = w.place + tokens;
   w.shares = reinterpret_cast<float*>(w.held + 4);
   w.arrived = reinterpret_cast<int*>(w.shares + static_cast<long long>(w.groups) * 2 * w.width_up);
-  w.bytes = static_cast<long long>(vocab) * width * out_size;
+  w.has = reinterpret_cast<uint32_t*>(w.arrived + static_cast<long long>(w.groups) * w.slices);
+  w.out_size = out_size;
+  const long long row = static_cast<long long>(width) * out_size, early = (EARLY_BYTES + EARLY_BYTES_A_TOKEN * tokens) / row;
+  w.zero_from = add || row < LONG_ROW || early > vocab ? vocab : int(early);
+  const int rest = (vocab - w.zero_from + UNIT - 1) / UNIT;
+  w.zero_ctas = rest < n_sms() ? rest : n_sms();
   if (dtype < R2_F32 || dtype > R2_BF16 || out_dtype < R2_F32 || out_dtype > R2_BF16) return R2_BAD_DTYPE;
   const int status = launch_deal(w, stream);
   if (status != R2_OK) return status;

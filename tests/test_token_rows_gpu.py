@@ -200,3 +200,27 @@ def test_refusals():
         args = [call.pop(n) for n in ("ids", "table")]
         with pytest.raises(o.KernelError):
             o.token_rows(*args, **call)
+
+
+# tables beyond what gets its zeros beside the sorting (32 MB and some for each token), with rows at and off 16 bytes
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,width,vocab", [(1, 768, 50257), (60, 513, 60001), (1000, 301, 130003), (9, 128, 260000), (33, 127, 400000)])
+@pytest.mark.parametrize("tokens", ["any", "ends", "runs", "none"])
+def test_tables_whose_zeros_are_written_beside_the_sums(n, width, vocab, dtype, tokens):
+    g = torch.Generator(device=DEV).manual_seed(n + width)
+    ids = torch.randint(0, vocab, (n,), generator=g, device=DEV, dtype=torch.int32)
+    if tokens == "ends":
+        ids[: n // 2], ids[n // 2:] = vocab - 1, vocab - 2
+        ids[: n // 3] = 0
+    elif tokens == "runs":
+        ids = vocab - 1 - torch.arange(n, device=DEV, dtype=torch.int32) // 2
+    elif tokens == "none":
+        ids.fill_(-1)
+    above = torch.randn(n, width, generator=g, device=DEV).to(dtype)
+    junk = torch.full((vocab * width + 64,), 3.0, dtype=dtype, device=DEV)   # (what the allocator hands out next is not zero)
+    del junk
+    got = ops().token_rows_gradient(ids, above, vocab)
+    want, off = rows_gradient(ids, above, vocab)
+    off = off + want.abs() * (torch.finfo(dtype).eps / 2)
+    assert torch.all((got.double() - want).abs() <= off)
+    assert torch.equal(got, ops().token_rows_gradient(ids, above, vocab))
