@@ -530,3 +530,12 @@ def test_one_token_for_all_rows(dtype, rows):
         c = Case(rows, 96, 600, dtype, 31)
         c.targets[7:] = token
         c.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(20, 700001), (100, 530000), (300, 400003)])
+def test_several_pieces_of_the_vocabulary(rows, vocab, dtype):
+    """More tokens than a piece of the factors holds: targets in every piece."""
+    c = Case(rows, 24, vocab, dtype, 41)
+    c.targets[8], c.targets[9], c.targets[10] = vocab - 2, vocab // 2, 524288 if vocab > 524288 else 262144
+    c.check()
