@@ -6,7 +6,8 @@
 //
 //   deal_kernel  sorts the places by token, stable. The table's rows are dealt out to CTAs by the remainder of their number (tokens that stand often lie side
 //                by side in a vocabulary). A CTA goes through all tokens, a share a warp, and lists its own with their rank among the share's of their row, beside a
-//                count of those of lower deals, so that it knows where in the sorted list its part begins without a word between CTAs. Running sums of the shares' and rows'
+//                count of those of lower deals, so that it knows where in the sorted list its part begins without a word between CTAs. (Places wait until there are 32 of
+//                them to look at: the CTA of a token that stands everywhere is the last to be done. 32,768 tokens, one in ten the same: 26.5 to 16.0 us.) Running sums of the shares' and rows'
 //                counts then say where each place goes. Meanwhile zeros go to the table's first part in bulk copies from shared memory, without a look at which rows
 //                need them: they are most of what a small batch costs, and hide the sorting; the rows that are written twice are fewer than the places.
 //   sum_kernel   a CTA takes the sorted places of eight windows, a warp each, and up to 256 columns: a token that stands everywhere and tokens that stand once
@@ -14,7 +15,7 @@
 //                memory, and the last of those CTAs adds them, in the order of the places whoever that is. Beside them, the other rows' zeros.
 //
 // Bound by the bytes of the rows from above and of the table where these are many: 1,024 float32 rows of 768 into 50,257 take 27.2 us (157 MB, 0.87 of a copy's rate). 32,768 bfloat16 rows of
-// 1,600 take 71 us (266 MB, 0.57): sorting 29 beside the zeros, sums 45 with the issue slots half full.
+// 1,600 take 66.7 us (266 MB, 0.61): sorting 16 beside two thirds of the zeros, then the sums (45 alone, issue slots half full) beside the rest.
 #include "common.cuh"
 
 namespace {
@@ -22,14 +23,13 @@ namespace {
 constexpr int THREADS = 256, WARPS = 8;
 constexpr int SLICE = 256;             // columns of a warp at most
 constexpr int DEAL_WARPS = 31, DEAL_THREADS = DEAL_WARPS * 32;   // of a dealing CTA, beside a warp that writes zeros
-constexpr int LISTED = 128;            // places that shared memory holds of what a dealing warp lists (where one has more, all go through the tokens again)
 constexpr int MOST_ROWS = 1200;        // of a deal
-constexpr int LISTED_BYTES = DEAL_WARPS * LISTED * 8;
+constexpr int DEAL_BYTES = 200 * 1024; // of shared memory: rows' counts, and the rest for what dealing warps list (where one has more places, all go through the tokens again)
 constexpr int ZEROS = 16384;           // bytes of a bulk copy
 
-// Zeros that are written beside the sorting, as many as it takes time for (1,024 tokens, 154 MB: with 24, 32, 44 and 56 MB 28.2, 27.2, 26.7 and 27.1 us, with all 34.2; 4,096 tokens, 77
-// MB: 19.5, 20.4, 21.3, 22.5 and 22.0). The others go beside the sums, to rows that no token came for, if rows are long enough to be runs of bulk copies.
-constexpr long long EARLY_BYTES = 32 << 20, EARLY_BYTES_A_TOKEN = 4608, LONG_ROW = 512;
+// Zeros that are written beside the sorting, as many as it takes time for (1,024 tokens, 154 MB: with 24, 32 and 44 MB 28.2, 27.2 and 26.7 us, with all 34.2; 32,768 tokens, 161 MB: with 1,024,
+// 2,304 and 3,200 bytes a token 71.5, 66.7 and 67.5, with all 69.6). The others go beside the sums, to rows that no token came for, if rows are long enough to be runs of bulk copies.
+constexpr long long EARLY_BYTES = 32 << 20, EARLY_BYTES_A_TOKEN = 2304, LONG_ROW = 512;
 constexpr int UNIT = 8;   // rows of a warp's step, a CTA an SM: what an SM can write bounds it, so all of them have to have the same
 
 struct Work {
@@ -42,7 +42,8 @@ struct Work {
   float scale;
   int add;
   int deals;                        // rows v with v mod deals = the CTA's
-  unsigned long long inverse;       // v / deals = v * inverse >> 64
+  int listed;                       // logarithm of the places that a dealing warp lists
+  unsigned inverse, shift;          // v / deals = v * inverse >> 32 + shift
   int32_t *row, *place;             // [tokens]: the sorted list: by deal, row and place
   int* held;                        // how many places hold a token
   int zero_ctas;                    // of the sums' launch, its first ones
@@ -131,9 +132,7 @@ __device__ __forceinline__ void put_row(O* row, const Lane<T, WIDE>& sum, int wi
   }
 }
 
-__device__ __forceinline__ int quotient_of(unsigned long long v, unsigned long long inverse) {
-  return int((v * unsigned(inverse >> 32) + (v * unsigned(inverse) >> 32)) >> 32);
-}
+__device__ __forceinline__ unsigned quotient_of(unsigned v, const Work& w) { return __umulhi(v, w.inverse) >> w.shift; }
 
 __device__ __forceinline__ long long row_bytes(const Work& w) { return static_cast<long long>(w.width) * w.out_size; }
 
@@ -146,7 +145,7 @@ __device__ __forceinline__ void write_zeros(const Work& w, uint4* zeros, int blo
   const long long size = row_bytes(w);
   for (long long first = w.zero_from + (block + (threadIdx.x >> 5) * blocks) * static_cast<long long>(UNIT); first < w.vocab; first += blocks * WARPS * static_cast<long long>(UNIT)) {
     const bool there = lane < UNIT && first + lane < w.vocab;
-    const unsigned v = unsigned(there ? first + lane : first), row = unsigned(quotient_of(v, w.inverse)), deal = v - row * w.deals;
+    const unsigned v = unsigned(there ? first + lane : first), row = quotient_of(v, w), deal = v - row * w.deals;
     unsigned empty = __ballot_sync(0xffffffffu, there && (w.has[(deal * DEAL_WARPS + row / 64) * 2 + row % 2] >> (row / 2 % 32) & 1u) == 0);
     while (empty != 0) {
       const int begin = __ffs(int(empty)) - 1, rows = __ffs(int(~(empty >> begin) | (begin > 0 ? 1u << (32 - begin) : 0u))) - 1, n = rows < 0 ? 32 : rows;
@@ -171,8 +170,8 @@ __global__ void __launch_bounds__(DEAL_THREADS + 32, 1) deal_kernel(const Work w
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, deal = blockIdx.x;
   const int rows = int((static_cast<long long>(w.vocab) - deal + w.deals - 1) / w.deals);
   int32_t* counts = shared;                          // [warp][rows]: a row's places in the warp's share, then where the first of them goes
-  int32_t* list_place = counts + DEAL_WARPS * rows;  // [warp][LISTED]
-  uint32_t* list_row = reinterpret_cast<uint32_t*>(list_place + DEAL_WARPS * LISTED);   // row * LISTED + rank
+  int32_t* list_place = counts + DEAL_WARPS * rows;  // [warp][listed]
+  uint32_t* list_row = reinterpret_cast<uint32_t*>(list_place + (DEAL_WARPS << w.listed));   // row << listed, rank
   __shared__ alignas(16) uint4 zeros[ZEROS / 16];
   auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(DEAL_THREADS) : "memory"); };
   if (w.zero_ctas == 0) pdl_launch_dependents();   // (CTAs that write zeros have to lie evenly on the SMs: started in what shared memory the sorting leaves, they took twice the time)
@@ -205,36 +204,57 @@ __global__ void __launch_bounds__(DEAL_THREADS + 32, 1) deal_kernel(const Work w
   const int first = int(min(static_cast<long long>(warp) * share, static_cast<long long>(w.tokens))), last = int(min(static_cast<long long>(first) + share, static_cast<long long>(w.tokens)));
   int32_t* own_counts = counts + warp * rows;
   int n_mine = 0, n_lower = 0;
+  __shared__ int waiting[DEAL_WARPS][64];   // places that a warp has come across, a ring: they are looked at 32 at a time
+  const unsigned before = (1u << lane) - 1u;
   auto walk = [&](auto&& each) {
     n_mine = n_lower = 0;
+    int pending = 0;
+    auto look = [&](int n) {
+      if (lane < n) {
+        const unsigned all = n == 32 ? 0xffffffffu : (1u << n) - 1u;
+        const int place = waiting[warp][(n_mine + lane) & 63], row = int(quotient_of(unsigned(w.ids[place]), w));
+        const unsigned peers = __match_any_sync(all, row);
+        const int count = own_counts[row];
+        __syncwarp(all);
+        if ((peers >> lane) == 1u) own_counts[row] = count + __popc(peers);   // (the last of them)
+        each(row, place, count + __popc(peers & before), n_mine + lane);
+      }
+      __syncwarp();
+      n_mine += n;
+      pending -= n;
+    };
     for (int t0 = first; t0 < last; t0 += 32 * LOADS) {
-      int id[LOADS];
+      unsigned id[LOADS];
 #pragma unroll
-      for (int j = 0; j < LOADS; ++j) id[j] = t0 + 32 * j + lane < last ? w.ids[t0 + 32 * j + lane] : -1;
+      for (int j = 0; j < LOADS; ++j) id[j] = t0 + 32 * j + lane < last ? unsigned(w.ids[t0 + 32 * j + lane]) : 0xffffffffu;
+      // few of 32 tokens are the CTA's: which of the pieces hold one, first
+      unsigned pieces = 0;
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
-        const bool token = id[j] >= 0 && id[j] < w.vocab;
-        const int row = quotient_of(unsigned(token ? id[j] : 0), w.inverse), at = id[j] - row * w.deals;
-        n_lower += token && at < deal ? 1 : 0;
-        const bool own = token && at == deal;
+        const unsigned at = id[j] < unsigned(w.vocab) ? id[j] - quotient_of(id[j], w) * unsigned(w.deals) : 0xffffffffu;
+        n_lower += at < unsigned(deal) ? 1 : 0;
+        pieces |= at == unsigned(deal) ? 1u << j : 0u;
+      }
+      const unsigned own_pieces = pieces;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) pieces |= __shfl_xor_sync(0xffffffffu, pieces, o);
+#pragma unroll 1
+      for (; pieces != 0; pieces &= pieces - 1u) {
+        const int j = __ffs(int(pieces)) - 1;
+        const bool own = own_pieces >> j & 1u;
         const unsigned owners = __ballot_sync(0xffffffffu, own);
-        if (owners == 0) continue;
-        if (own) {
-          const unsigned peers = __match_any_sync(owners, row), before = (1u << lane) - 1u;
-          const int count = own_counts[row];
-          __syncwarp(owners);
-          if ((peers >> lane) == 1u) own_counts[row] = count + __popc(peers);   // (the last of them)
-          each(row, t0 + 32 * j + lane, count + __popc(peers & before), n_mine + __popc(owners & before));
-        }
+        if (own) waiting[warp][(n_mine + pending + __popc(owners & before)) & 63] = t0 + 32 * j + lane;
         __syncwarp();
-        n_mine += __popc(owners);
+        pending += __popc(owners);
+        if (pending >= 32) look(32);
       }
     }
+    if (pending > 0) look(pending);
   };
   walk([&](int row, int place, int rank, int at) {
-    if (at < LISTED) {
-      list_row[warp * LISTED + at] = unsigned(row) * LISTED + unsigned(rank);
-      list_place[warp * LISTED + at] = place;
+    if (at < 1 << w.listed) {
+      list_row[(warp << w.listed) + at] = (unsigned(row) << w.listed) + unsigned(rank);
+      list_place[(warp << w.listed) + at] = place;
     }
   });
 #pragma unroll
@@ -293,12 +313,12 @@ __global__ void __launch_bounds__(DEAL_THREADS + 32, 1) deal_kernel(const Work w
   sync();
 
   // ---- where each place goes
-  if (most <= LISTED) {
+  if (most <= 1 << w.listed) {
     for (int i = lane; i < n_mine; i += 32) {
-      const unsigned entry = list_row[warp * LISTED + i];
-      const int row = int(entry / LISTED), at = own_counts[row] + int(entry % LISTED);
+      const unsigned entry = list_row[(warp << w.listed) + i];
+      const int row = int(entry >> w.listed), at = own_counts[row] + int(entry & ((1u << w.listed) - 1u));
       w.row[at] = row * w.deals + deal;
-      w.place[at] = list_place[warp * LISTED + i];
+      w.place[at] = list_place[(warp << w.listed) + i];
     }
   } else {
     walk([&](int row, int place, int at, int) {
@@ -504,8 +524,7 @@ int n_sms() {
   return n;
 }
 
-// As many deals as SMs, of no more rows than a CTA counts. The quotient v / deals is v * inverse >> 64 with the inverse of 2^64 rounded up (two deals at least, so
-// that it is below 2^64): exact, since the excess of v * inverse is below v * deals < 2^64 parts of 1 / deals.
+// As many deals as SMs, of no more rows than a CTA counts.
 int deals_of(int vocab) {
   int deals = n_sms();
   if (deals > vocab) deals = vocab;
@@ -515,9 +534,9 @@ int deals_of(int vocab) {
 
 int launch_deal(const Work& w, cudaStream_t stream) {
   static std::atomic<bool> done[64];
-  const int status = allow_smem(deal_kernel, DEAL_WARPS * MOST_ROWS * 4 + LISTED_BYTES, done);
+  const int status = allow_smem(deal_kernel, DEAL_BYTES, done);
   if (status != R2_OK) return status;
-  r2_launch(deal_kernel, dim3(w.deals), dim3(DEAL_THREADS + 32), ((w.vocab - 1) / w.deals + 1) * size_t(DEAL_WARPS * 4) + LISTED_BYTES, stream, w);
+  r2_launch(deal_kernel, dim3(w.deals), dim3(DEAL_THREADS + 32), size_t(DEAL_WARPS) * (((w.vocab - 1) / w.deals + 1) * 4 + (8 << w.listed)), stream, w);
   return launch_status();
 }
 
@@ -537,7 +556,14 @@ void share_out(Work& w) {
   w.groups = (w.tokens + WARPS * w.window - 1) / (WARPS * w.window);
   w.width_up = (w.width + 7) / 8 * 8;
   w.deals = deals_of(w.vocab);
-  w.inverse = ~0ull / unsigned(w.deals) + 1;
+  // v / deals for v < 2^30: with 2^(s - 1) < deals <= 2^s the inverse of 2^(31 + s), rounded up, is below 2^32, and v times its excess below 2^30 deals < 2^(31 + s)
+  int s = 1;
+  while (1ll << s < w.deals) ++s;
+  w.inverse = unsigned(((1ull << (31 + s)) + unsigned(w.deals) - 1) / unsigned(w.deals));
+  w.shift = unsigned(s - 1);
+  const int rows = (w.vocab - 1) / w.deals + 1;
+  w.listed = 7;   // (MOST_ROWS leave room for 128)
+  while (w.listed < 10 && DEAL_WARPS * (rows * 4 + (16 << w.listed)) <= DEAL_BYTES) ++w.listed;
 }
 
 bool at_16(const void* p, long long ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
@@ -577,7 +603,7 @@ extern "C" long long r2_token_rows_space(int tokens, int width, int vocab) {
 extern "C" int r2_token_rows_gradient(int dtype, int out_dtype, const int32_t* ids, const void* above, long long ld, void* out, long long ld_o, int tokens, int width,
                                       int vocab, float scale, int add, void* space, cudaStream_t stream) {
   if (tokens < 1 || width < 1 || vocab < 1) return R2_BAD_SHAPE;
-  if (tokens > MOST || width > MOST) return R2_UNSUPPORTED;
+  if (tokens > MOST || width > MOST || vocab > MOST) return R2_UNSUPPORTED;
   if (!add && (ld_o != width || reinterpret_cast<uintptr_t>(out) % 16 != 0)) return R2_BAD_ALIGN;   // (a new table is one piece)
   const int size = dtype == R2_F32 ? 4 : 2, out_size = out_dtype == R2_F32 ? 4 : 2;
   const bool wide = at_16(above, ld, size) && at_16(out, ld_o, out_size) && width * size % 16 == 0 && width * out_size % 16 == 0;

@@ -224,3 +224,13 @@ def test_tables_whose_zeros_are_written_beside_the_sums(n, width, vocab, dtype, 
     off = off + want.abs() * (torch.finfo(dtype).eps / 2)
     assert torch.all((got.double() - want).abs() <= off)
     assert torch.equal(got, ops().token_rows_gradient(ids, above, vocab))
+
+
+@pytest.mark.parametrize("n,vocab,which", [(40000, 300, (7,)), (100000, 300, (7, 7 + 148, 299)), (66000, 50257, (13,)), (3000, 2000003, (5, 1999999))])
+def test_tokens_that_a_sorting_warp_cannot_list(n, vocab, which):
+    """A few tokens at most places: more of a CTA's own than shared memory lists; and more rows than the SMs' CTAs count."""
+    g = gen(n)
+    ids = torch.randint(0, vocab, (n,), generator=g, device=DEV, dtype=torch.int32)
+    often = torch.tensor(which, dtype=torch.int32, device=DEV)[torch.randint(0, len(which), (n,), generator=g, device=DEV)]
+    ids = torch.where(torch.rand(n, generator=g, device=DEV) < 0.95, often, ids)
+    check(ids, torch.randn(n, 8, generator=g, device=DEV), vocab)
