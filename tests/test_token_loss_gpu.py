@@ -539,3 +539,14 @@ def test_several_pieces_of_the_vocabulary(rows, vocab, dtype):
     c = Case(rows, 24, vocab, dtype, 41)
     c.targets[8], c.targets[9], c.targets[10] = vocab - 2, vocab // 2, 524288 if vocab > 524288 else 262144
     c.check()
+
+
+@pytest.mark.parametrize("rows,width,vocab", [(1, 768, 20011), (16, 300, 30000), (17, 257, 40001), (33, 1031, 25000), (64, 96, 70000), (40, 24, 530001)])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_few_float32_rows_at_large_tables(rows, width, vocab, softcap):
+    """Tables of more tiles than the GPU holds at once: the loss reads them as they are, the hidden rows' gradient their planes."""
+    pad = -width % 4
+    c = Case(rows, width, vocab, F32, rows, table_pad=pad, softcap=softcap)
+    c.check()
+    again = c.run()
+    assert all(torch.equal(a, b) for a, b in zip(again, c.run()))
