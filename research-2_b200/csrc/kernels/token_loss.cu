@@ -1078,7 +1078,6 @@ template <typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const float2* part, int parts, const T* hidden, long long ld_h, const T* table, long long ld_t, const int32_t* targets,
                                                      const float* weight, int rows, int width, int vocab, float softcap, float* loss, float* log_sum) {
   pdl_launch_dependents();
-  pdl_wait();
   const int lane = threadIdx.x & 31, r = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (r >= rows) return;
   const int y = targets[r];
@@ -1087,18 +1086,6 @@ __global__ void __launch_bounds__(256) finish_kernel(const float2* part, int par
   const T* x = hidden + size_t(r) * ld_h;
   const T* t = table + size_t(counts ? y : 0) * ld_t;
   const bool wide = rows_wide(hidden, ld_h, width) && rows_wide(table, ld_t, width);
-  float top = -3.4028234663852886e38f, sum = 0.f;
-  for (int i0 = lane; i0 < parts; i0 += 32 * 16) {
-    float2 p[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) p[j] = i0 + 32 * j < parts ? part[size_t(r) * parts + i0 + 32 * j] : make_float2(-3.4028234663852886e38f, 0.f);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float most = fmaxf(top, p[j].x);
-      sum = sum * fast_exp2(top - most) + p[j].y * fast_exp2(p[j].x - most);
-      top = most;
-    }
-  }
   float dot = 0.f;
   bool fine = true;   // (float32's planes hold no infinities: a row with one, or with NaN, has no sum)
   if (counts || sizeof(T) == 4) {
@@ -1120,6 +1107,19 @@ __global__ void __launch_bounds__(256) finish_kernel(const float2* part, int par
           dot = fmaf(a[i][j], b[i][j], dot);
         }
       }
+    }
+  }
+  pdl_wait();   // (the sums' kernel lets this one in behind its own wait: what was there before that call is there)
+  float top = -3.4028234663852886e38f, sum = 0.f;
+  for (int i0 = lane; i0 < parts; i0 += 32 * 16) {
+    float2 p[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) p[j] = i0 + 32 * j < parts ? part[size_t(r) * parts + i0 + 32 * j] : make_float2(-3.4028234663852886e38f, 0.f);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float most = fmaxf(top, p[j].x);
+      sum = sum * fast_exp2(top - most) + p[j].y * fast_exp2(p[j].x - most);
+      top = most;
     }
   }
 #pragma unroll
