@@ -26,7 +26,7 @@
 // (whatever they hold) or spends time on them; the rest of the last 256 rows is zeros.
 //
 // Bound by the tensor cores from some 200 rows on, by the pass over the table below. At a table of 50,257 x 768, bfloat16, 1,965 MHz: LOGSUM of 4,096 rows 191 us (1.66 PFLOP/s, tensor cores
-// active 96 % of an SM's time), FACTORS of 3,840 that count 213 us (1.39; its results' instructions share the SM with the warps that feed the tensor cores), ROWS 220 (1.35) and TABLE
+// active 96 % of an SM's time), FACTORS of 3,840 that count 213 us (1.39; 190 without the stores of dz, which the operands' loads share the L2 with), ROWS 220 (1.35) and TABLE
 // 199 (1.49; operands whose rows lie along K are read at 0.9 of the rate). Tiles of 256 x 256 on pairs read 64 KB for each 64 of k and pair where 128 x 128 read twice that for the work,
 // which shared memory does not keep up with.
 #include <math.h>
@@ -1429,7 +1429,9 @@ template <typename T> bool make_few_maps(CUtensorMap* mt, CUtensorMap* mx, const
 int row_blocks(long long rows) { return int(rows < 8 * 4736 ? (rows + 7) / 8 : 4736); }
 
 // What a call's scratch holds, in bytes from its start.
-constexpr long long FACTOR_BYTES = 256ll << 20;   // of dz at a time
+// Of dz at a time. (4,096 rows at GPT-2's table with 128, 256, 512 MB and 1 GB: 931, 855, 833 and 833 us; 2,047 at a table of 128,001 x 1,600 2,487, 2,441, 2,418 and 2,418. Pieces that L2
+// would hold make for more launches and rounds that are not full.)
+constexpr long long FACTOR_BYTES = 512ll << 20;
 
 struct Layout {
   int planes;                       // bfloat16 planes of an operand

@@ -550,3 +550,11 @@ def test_few_float32_rows_at_large_tables(rows, width, vocab, softcap):
     c.check()
     again = c.run()
     assert all(torch.equal(a, b) for a, b in zip(again, c.run()))
+
+
+@pytest.mark.parametrize("rows,vocab", [(20, 1100003), (100, 1048833), (300, 600001)])
+def test_several_pieces_of_a_bfloat16_vocabulary(rows, vocab):
+    """Targets at both sides of where pieces end, first and last tokens; few rows with what rounding leaves in every piece."""
+    c = Case(rows, 16, vocab, BF16, 43)
+    c.targets[7:14] = torch.tensor([524287, 524288, vocab - 2, vocab // 2, 262143, 524032, vocab - 257], dtype=torch.int32, device=DEV)
+    c.check()
