@@ -102,3 +102,33 @@ def test_scratch_of_a_call_is_of_its_stream():
     torch.cuda.synchronize(DEV)
     for a, b in zip(got, want):
         the_same(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 100, 200])
+def test_a_chain_of_calls_waits_for_what_it_reads(rows, dtype):
+    """Each kernel starts beside the one in front of it: a chain in which every call reads what the last one wrote has the bits of one with waits in between."""
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    vocab, width = 20000, 256
+    for _ in range(10):
+        ids = torch.randint(0, vocab, (3000,), device=DEV, dtype=torch.int32, generator=g)
+        above, hidden = torch.randn(3000, width, device=DEV, generator=g).to(dtype), torch.randn(rows, width, device=DEV, generator=g).to(dtype)
+        targets, weight = torch.randint(0, vocab, (rows,), device=DEV, dtype=torch.int32, generator=g), torch.rand(rows, device=DEV, generator=g)
+
+        def chain(wait):
+            def step(t):
+                if wait:
+                    torch.cuda.synchronize(DEV)
+                return t
+
+            step(None)
+            table = step(ops.token_rows_gradient(ids, above, vocab))
+            scaled = step(ops.scale_rows(hidden, weight + 0.5, in_place=False))
+            loss, log_sum = step(ops.token_loss(scaled, table, targets, weight=weight))
+            d_hidden, d_table = step(ops.token_loss_gradient(scaled, table, targets, log_sum, weight=weight))
+            rows_back = step(ops.token_rows_gradient(targets, d_hidden, vocab))
+            return (table, loss, log_sum, d_hidden, d_table, rows_back, *step(ops.token_loss(scaled, d_table, targets)))
+
+        first = chain(False)
+        the_same(first, chain(True))
