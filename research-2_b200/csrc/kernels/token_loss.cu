@@ -13,8 +13,8 @@
 //   TABLE    dW: dz^T times the hidden rows, whole for each piece of the vocabulary and rounded once
 //
 // dz is rounded to bfloat16, the type of the gradients that it makes, so that both products run on the tensor cores at full rate. Its largest number by far is often the token's
-// own, a_r (p - 1): what the rounding leaves of that one (`rest`) is kept in float and goes into dx where its shares are joined, and into dW where rows are few. (Without it either
-// gradient's error was that of two roundings, 1.44 times that of its own; of many rows dW's still is.)
+// own, a_r (p - 1): what the rounding leaves of that one (`rest`) is kept in float and goes into dx where its shares are joined, and into dW with a tile's results. (Without it either
+// gradient's error was that of two roundings, 1.44 times that of its own.)
 //
 // float32 operands are three bfloat16 planes each: x = x0 + x1 + x2 to the last bit (8 bits each), and a product is the six products x_i w_j
 // with i + j <= 2; what is left out is below 2^-24 of it. dz is kept in three planes then, too. The tensor cores add to an accumulator without rounding to nearest: each
@@ -55,11 +55,15 @@ constexpr size_t SMEM = 1024 + STAGES * size_t(A_BYTES + B_BYTES) + 2 * WARPS * 
 // tiles of 256 rows 161 and 282, 153 and 284, 153 and 302), bfloat16 25 and 69, 27 and 71, 29 and 81 (31 and 72, 29 and 73, 29 and 77 without `rest`).
 constexpr int FEW = 128;
 
+constexpr int WINDOW = 64;   // sorted rows whose sums by token a warp makes
+
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 constexpr int ERR_FULL = 1, ERR_EMPTY = 2, ERR_ACC = 3;   // codes of waits that ran out, as of the other products
 
-enum Mode { LOGSUM, FACTORS, ROWS, TABLE };
+enum Mode { LOGSUM, FACTORS, ROWS, TABLE, TABLE_FEW };   // (TABLE_FEW: bfloat16 rows that a tile's warps find by themselves)
+
+constexpr bool is_table(int mode) { return mode == TABLE || mode == TABLE_FEW; }
 
 struct Work {
   int m, n, k;               // rows and columns of the result, and what is summed over
@@ -71,9 +75,13 @@ struct Work {
   const float* factor;
   const float* log_sum;
   int first;                 // FACTORS, TABLE: the piece's first token
-  float* rest;               // bfloat16: what rounding left of dz at each row's token; FACTORS writes it, TABLE adds it where it is given
-  const bf16* x;             // TABLE with it: the gathered rows
+  float* rest;               // bfloat16: what rounding left of dz at each row's token; FACTORS writes it, TABLE_FEW adds it
+  const bf16* x;             // TABLE_FEW: the gathered rows
   long long ld_x;
+  const int2* runs;          // bfloat16 TABLE: of each of the piece's tokens, in each segment of the sorted rows, its first row and the one behind its last
+  const float* sums;         // and what rounding left at its own rows, summed by WINDOW of them (rests_kernel)
+  long long ld_sums;
+  int segments, run_tokens;
   float2* part;              // LOGSUM: [row][parts]: of a half tile the largest z log2 e and the sum of 2^(z log2 e - it)
   int parts;
   void* out;                 // TABLE, where tensor copies cannot write it
@@ -238,7 +246,7 @@ __device__ __forceinline__ void tmem_row64(uint32_t taddr, float (&v)[64]) {
 // The work of pair `pair` of `n_pairs`.
 template <int MODE, bool CAPPED, typename T, bool PLANES, int CHUNKED>
 __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensorMap& map_b, const CUtensorMap& map_out, const Work& w, const int pair, const int n_pairs) {
-  constexpr bool A_MN = MODE == TABLE, B_MN = MODE == ROWS || MODE == TABLE;
+  constexpr bool A_MN = is_table(MODE), B_MN = MODE == ROWS || is_table(MODE);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t a_base = smem_u32(smem), b_base = a_base + STAGES * A_BYTES;
@@ -277,7 +285,7 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(leader_acc_empty) : "r"(acc_empty), "r"(0u));
 
   const int m = (MODE == FACTORS || MODE == ROWS) ? *w.count : w.m;
-  const int k = MODE == TABLE ? *w.count : w.k;
+  const int k = is_table(MODE) ? *w.count : w.k;
   constexpr int TERMS = PLANES ? 6 : 1;
   const int n_kb = (k + BK - 1) / BK, row_tiles = (m + 2 * BM - 1) / (2 * BM), col_tiles = (w.n + BN - 1) / BN;
   const long long n_units = static_cast<long long>(row_tiles) * col_tiles * (MODE == ROWS ? w.splits : 1);
@@ -381,8 +389,16 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
     Slabs out = {slabs + (warp - 2) * 2 * SLAB, lane, 0};
     uint32_t local = 0;
     bool ok = true;
+    constexpr bool RESTS = MODE == TABLE && sizeof(T) == 2;
+    auto run_of = [&](long long i, const Unit& u) {   // of the lane's token of a unit
+      const int row = (u.row * 2 + int(rank)) * BM + q * 32 + lane;
+      return i < n_units && row < m && w.segments > 0 ? __ldg(w.runs + row) : make_int2(0, 0);
+    };
+    Unit u_ahead = unit_of<MODE>(w, pair, row_tiles, col_tiles, n_kb);
+    int2 run_ahead = make_int2(0, 0);
+    if constexpr (RESTS) run_ahead = run_of(pair, u_ahead);
     for (long long i = pair; i < n_units; i += n_pairs) {
-      const Unit u = unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
+      const Unit u = RESTS ? u_ahead : unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
       const int row = (u.row * 2 + int(rank)) * BM + q * 32 + lane;
       const int col0 = u.col * BN;
       int target = -1;
@@ -396,15 +412,15 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
       }
       const int row0 = (u.row * 2 + int(rank)) * BM + q * 32;
       float top = -3.4028234663852886e38f, sum = 0.f;
-      // TABLE: what rounding left of dz at the tokens of the warp's 32 rows, in the order of the gathered rows (FEW of them at most; their tokens are asked for
+      // TABLE_FEW: what rounding left of dz at the tokens of the warp's 32 rows, in the order of the gathered rows (FEW of them at most; their tokens are asked for
       // before the accumulator is waited for)
       int token[FEW / 32];
-      if constexpr (MODE == TABLE && sizeof(T) == 2) {
+      if constexpr (MODE == TABLE_FEW) {
 #pragma unroll
-        for (int i = 0; i < FEW / 32; ++i) token[i] = w.rest != nullptr && 32 * i + lane < k ? w.targets[32 * i + lane] - w.first - row0 : -1;
+        for (int i = 0; i < FEW / 32; ++i) token[i] = 32 * i + lane < k ? w.targets[32 * i + lane] - w.first - row0 : -1;
       }
       auto add_rest = [&](int c, float (&v)[64]) {
-        if constexpr (MODE == TABLE && sizeof(T) == 2) {
+        if constexpr (MODE == TABLE_FEW) {
 #pragma unroll
           for (int i = 0; i < FEW / 32; ++i) {
 #pragma unroll 1
@@ -430,8 +446,33 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
           }
         }
       };
+      // bfloat16 TABLE: their sums by rests_kernel, of a few of the warp's 32 tokens (asked for a tile ahead)
+      const int2 run = run_ahead;
+      if constexpr (RESTS) {
+        u_ahead = unit_of<MODE>(w, i + n_pairs, row_tiles, col_tiles, n_kb);
+        run_ahead = run_of(i + n_pairs, u_ahead);
+      }
+      auto add_rests = [&](int c, float (&v)[64]) {
+        if constexpr (RESTS) {
+          for (int segment = 0; segment < w.segments; ++segment) {
+            const int2 of = segment == 0 ? run : row < m ? __ldg(w.runs + static_cast<long long>(segment) * w.run_tokens + row) : make_int2(0, 0);
+#pragma unroll 1
+            for (int at = of.x; at < of.y; at = (at / WINDOW + 1) * WINDOW) {
+              const float4* sum = reinterpret_cast<const float4*>(w.sums + at * w.ld_sums + col0 + c);
+              const int last = (w.n - col0 - c - 1) / 4;   // (what is added behind it is not stored)
+              float4 q[16];
+#pragma unroll
+              for (int p = 0; p < 16; ++p) q[p] = __ldg(sum + min(p, last));
+#pragma unroll
+              for (int p = 0; p < 16; ++p) v[4 * p] += q[p].x, v[4 * p + 1] += q[p].y, v[4 * p + 2] += q[p].z, v[4 * p + 3] += q[p].w;
+            }
+          }
+        }
+      };
       // 64 finished numbers of a row, from column c of the tile on
       auto finish = [&](int c, float (&v)[64]) {
+        if constexpr (MODE == TABLE_FEW) add_rest(c, v);
+        if constexpr (RESTS) add_rests(c, v);
         if constexpr (MODE == LOGSUM) {
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] = log2_units<CAPPED>(v[j], w);
@@ -497,14 +538,12 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
             }
             out.end(&map_out, col0 + c, row0, plane, slab, false);
           }
-        } else if (MODE == TABLE && w.out != nullptr) {
-          add_rest(c, v);
+        } else if (is_table(MODE) && w.out != nullptr) {
           T* to = static_cast<T*>(w.out) + row * w.ld + col0 + c;
 #pragma unroll
           for (int j = 0; j < 64; ++j)
             if (row < m && col0 + c + j < w.n) to[j] = from_float<T>(v[j]);
-        } else if constexpr (sizeof(T) == 2 && MODE == TABLE) {
-          add_rest(c, v);
+        } else if constexpr (is_table(MODE) && sizeof(T) == 2) {
           const uint32_t slab = out.begin();
 #pragma unroll
           for (int p = 0; p < 8; ++p)
@@ -569,7 +608,7 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
         for (int c = side * HALF; c < (side + 1) * HALF && ok && left(c); c += 64) {
           float v[64];
           tmem_row64(tmem + buf * BN + uint32_t(c) + lanes, v);
-          if constexpr (MODE == ROWS || MODE == TABLE) {
+          if constexpr (MODE == ROWS || is_table(MODE)) {
 #pragma unroll
             for (int j = 0; j < 64; ++j) v[j] = none ? 0.f : v[j];
           }
@@ -607,10 +646,10 @@ struct Both {
   int rows_pairs;
 };
 
-template <typename T, bool PLANES, int CHUNKED> __global__ void __launch_bounds__(THREADS, 1) both_kernel(const __grid_constant__ Both b) {
+template <int TABLE_MODE, typename T, bool PLANES, int CHUNKED> __global__ void __launch_bounds__(THREADS, 1) both_kernel(const __grid_constant__ Both b) {
   const int pair = int(blockIdx.x >> 1), n_pairs = int(gridDim.x >> 1);
   if (pair < b.rows_pairs) product<ROWS, false, float, PLANES, CHUNKED>(b.rows_a, b.rows_b, b.rows_out, b.rows, pair, b.rows_pairs);
-  else product<TABLE, false, T, PLANES, CHUNKED>(b.table_a, b.table_b, b.table_out, b.table, pair - b.rows_pairs, n_pairs - b.rows_pairs);
+  else product<TABLE_MODE, false, T, PLANES, CHUNKED>(b.table_a, b.table_b, b.table_out, b.table, pair - b.rows_pairs, n_pairs - b.rows_pairs);
 }
 
 // ---- few rows: LOGSUM and FACTORS of up to 128 ----------------------------------------------
@@ -1168,12 +1207,18 @@ template <typename T> __global__ void __launch_bounds__(256) planes_kernel(const
 }
 
 // The rows that count (a token of the vocabulary, a weight that is not 0) side by side, their numbers in one plane or three, zeros behind them up to a
-// multiple of 256 rows; `place[r]` is where row r went, -1 for none. A block looks at all rows' tokens and takes its own. Behind these blocks: the table's planes.
-template <typename T>
+// multiple of 256 rows; `place[r]` is where row r went, -1 for none. SORTED (bfloat16, more than FEW): by their tokens (rows of one token in their order), SEGMENT of the call's rows at a time, `starts` says
+// where a segment's begin: what the table's gradient adds in float for a token then stands side by side. A block looks at all rows' tokens and takes its own; a row's place is the number
+// of those that go before it (a segment's square of comparisons, 5 us for 4,096 rows; segments keep it below the products' time however many rows there are). Behind these blocks: the table's planes.
+constexpr int SEGMENT = 65536;
+constexpr int OWN = 32;   // rows of a block at most; a segment's are whole blocks
+
+template <typename T, bool SORTED>
 __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long ld, int rows, int width, int vocab, int own, const int32_t* targets, const float* weight,
                                                      const float* log_sum, bf16* x, long long ld_x, long long plane, int32_t* y_out, float* f_out, float* s_out,
-                                                     int32_t* place, int* count, const Planes<T> table) {
-  __shared__ int totals[2][8];
+                                                     int32_t* place, int* count, int* starts, const Planes<T> table) {
+  constexpr int NONE = 0x7ffffffe, PASS = 8, AHEAD = 8;   // rows whose places are found in one look at the segment
+  __shared__ int totals[2][8], before_of[OWN], key_of[OWN], ranks[PASS][8];
   pdl_launch_dependents();
   pdl_wait();
   const int blocks = int(gridDim.x) - table.blocks;
@@ -1182,22 +1227,44 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
     return;
   }
   const int first = blockIdx.x * own, last = min(rows, first + own);
+  const int begin = SORTED ? first / SEGMENT * SEGMENT : first, end = min(rows, begin + SEGMENT);   // of the block's segment
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto counts = [&](int r) {
+  auto key = [&](int r) {
     const int y = targets[r];
-    return y >= 0 && y < vocab && (weight == nullptr || weight[r] != 0.f);
+    return y >= 0 && y < vocab && (weight == nullptr || weight[r] != 0.f) ? y : NONE;
   };
+  if (threadIdx.x < OWN) key_of[threadIdx.x] = first + int(threadIdx.x) < last ? key(first + threadIdx.x) : NONE;
+  __syncthreads();
   int before = 0, all = 0;
-  for (int r = threadIdx.x; r < rows; r += 256) {
-    const int c = counts(r) ? 1 : 0;
-    all += c;
-    before += r < first ? c : 0;
-  }
+  // how many rows of from .. to count, in all and in front of the block's (segment); how many of the segment's go before each of PASS rows of the block, by their tokens and places
+  auto scan = [&](long long from, long long to, int p, int (&n)[PASS]) {
+    int mine[PASS];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
+    for (int j = 0; j < PASS; ++j) {
+      mine[j] = SORTED ? key_of[p + j] : 0;
+      n[j] = 0;
+    }
+    for (long long r0 = from + threadIdx.x; r0 < to; r0 += 256 * AHEAD) {
+      int k[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) k[i] = r0 + 256 * i < to ? key(int(r0) + 256 * i) : NONE;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const long long r = r0 + 256 * i;
+        all += k[i] != NONE ? 1 : 0;
+        before += k[i] != NONE && r < begin ? 1 : 0;
+        if constexpr (SORTED) {
+          const int with = r < begin || r >= end ? NONE + 1 : k[i] + (r >= first ? 1 : 0);   // (of the block's own, equal ones are counted below)
+#pragma unroll
+          for (int j = 0; j < PASS; ++j) n[j] += with <= mine[j] ? 1 : 0;
+        }
+      }
+    }
+  };
+  int n[PASS];
+  scan(0, rows, 0, n);
+  before = __reduce_add_sync(0xffffffffu, before);
+  all = __reduce_add_sync(0xffffffffu, all);
   if (lane == 0) {
     totals[0][warp] = before;
     totals[1][warp] = all;
@@ -1209,6 +1276,32 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
     all += totals[1][i];
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) *count = all;
+  if constexpr (SORTED) {
+    if (first == begin && threadIdx.x == 0) starts[first / SEGMENT] = before;
+    const int in_front = before, counted = all;
+    for (int p = 0; p < last - first; p += PASS) {
+      if (p > 0) scan(begin, end, p, n);
+#pragma unroll
+      for (int j = 0; j < PASS; ++j) {
+        n[j] = __reduce_add_sync(0xffffffffu, n[j]);
+        if (lane == 0) ranks[j][warp] = n[j];
+      }
+      __syncthreads();
+      if (threadIdx.x < PASS) {
+        const int j = p + threadIdx.x;
+        int rank = in_front;
+        for (int i = 0; i < 8; ++i) rank += ranks[threadIdx.x][i];
+        for (int i = 0; i < j; ++i) rank += key_of[i] == key_of[j] ? 1 : 0;
+        before_of[j] = rank;
+      }
+      __syncthreads();
+    }
+    all = counted;
+  } else {
+    const unsigned held = __ballot_sync(0xffffffffu, key_of[lane] != NONE);
+    if (warp == 0) before_of[lane] = before + __popc(held & ((1u << lane) - 1u));
+    __syncthreads();
+  }
   const bool wide = rows_wide(hidden, ld, width);
   auto copy = [&](int to, const T* from) {   // (null: zeros)
     for (int c = lane * 8; c < width; c += 256) {
@@ -1217,25 +1310,103 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
       put_planes8<T>(x + size_t(to) * ld_x + c, plane, v);
     }
   };
-  // a block's rows, 32 at a time
-  for (int begin = first; begin < last; begin += 32) {
-    const bool c = begin + lane < last && counts(begin + lane);
-    const unsigned mask = __ballot_sync(0xffffffffu, c);
-    if (warp == 0 && begin + lane < last) {
-      const int r = begin + lane, at = before + __popc(mask & ((1u << lane) - 1u));
-      place[r] = c ? at : -1;
-      if (c) {
-        y_out[at] = targets[r];
-        f_out[at] = weight ? weight[r] : 1.f;
-        s_out[at] = log_sum[r];
-      }
+  if (int(threadIdx.x) < last - first) {
+    const int r = first + threadIdx.x, at = before_of[threadIdx.x];
+    const bool c = key_of[threadIdx.x] != NONE;
+    place[r] = c ? at : -1;
+    if (c) {
+      y_out[at] = targets[r];
+      f_out[at] = weight ? weight[r] : 1.f;
+      s_out[at] = log_sum[r];
     }
-    for (int i = warp; i < 32; i += 8)
-      if (mask >> i & 1u) copy(before + __popc(mask & ((1u << i) - 1u)), hidden + size_t(begin + i) * ld);
-    before += __popc(mask);
   }
-  const int end = (all + 255) / 256 * 256;
-  for (int at = all + blockIdx.x + warp * blocks; at < end; at += 8 * blocks) copy(at, static_cast<const T*>(nullptr));
+  for (int i = warp; i < last - first; i += 8)
+    if (key_of[i] != NONE) copy(before_of[i], hidden + size_t(first + i) * ld);
+  const int filled = (all + 255) / 256 * 256;
+  for (int at = all + blockIdx.x + warp * blocks; at < filled; at += 8 * blocks) copy(at, static_cast<const T*>(nullptr));
+}
+
+// bfloat16, more than FEW rows: what rounding left of dz at the tokens' own rows, times the hidden rows, summed in float by token, for the piece's tokens. A warp takes WINDOW of the sorted rows and 128
+// columns, and leaves a token's sum at the place of the first of its rows there: a token that stands everywhere is many warps' work, and its sums are added by TABLE, in order. Other warps look up where
+// each token's rows begin and end, a lane a token. (4,096 rows, a tenth of them one token: 10 us; TABLE adding the rows themselves took 100 us longer, a CTA for 128 tokens 40. With WINDOW 32 this takes 8 us
+// and TABLE 213 in place of 200, where a lane adds a token's sums.)
+struct Rests {
+  const bf16* x;
+  long long ld_x;
+  const int32_t* targets;
+  const float* rest;
+  const int *count, *starts;
+  int first, n, width, slices, segments;   // of the piece: its first token, tokens; of the columns
+  long long warps;                         // of sums; those of the look-up stand behind them
+  float* sums;
+  long long ld_sums;
+  int2* runs;
+  int run_tokens;
+};
+
+__global__ void __launch_bounds__(128) rests_kernel(const Rests w) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, k = *w.count;
+  const long long job = blockIdx.x * 4LL + (threadIdx.x >> 5);
+  auto start_of = [&](int segment) { return segment < w.segments ? __ldg(w.starts + segment) : k; };
+  if (job >= w.warps) {
+    const long long groups = w.run_tokens / 32, at = job - w.warps;
+    const int segment = int(at / groups), own = int(at % groups) * 32 + lane;
+    if (segment >= w.segments) return;
+    auto bound = [&](int token) {
+      int a = start_of(segment), b = start_of(segment + 1);
+      while (a < b) {
+        const int middle = a + (b - a) / 2;
+        if (__ldg(w.targets + middle) < token) a = middle + 1;
+        else b = middle;
+      }
+      return a;
+    };
+    const int begin = bound(w.first + own);
+    int end = __shfl_down_sync(0xffffffffu, begin, 1);
+    if (lane == 31) end = bound(w.first + own + 1);
+    w.runs[static_cast<long long>(segment) * w.run_tokens + own] = make_int2(begin, end);
+    return;
+  }
+  const int from = int(job / w.slices) * WINDOW, to = min(k, from + WINDOW), col = int(job % w.slices) * 128 + lane * 4;
+  const bool wide = col < w.width;   // (rows of whole eights)
+  float sum[4] = {};
+  int at = -1;   // the place of what is summed
+  auto keep = [&] {
+    if (wide && at >= 0) *reinterpret_cast<float4*>(w.sums + at * w.ld_sums + col) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+  };
+#pragma unroll 1
+  for (int i = from; i < to; i += 32) {
+    const bool there = i + lane < to;
+    const int token = there ? __ldg(w.targets + i + lane) : -1, before = there && i + lane > from ? __ldg(w.targets + i + lane - 1) : -1;
+    if (!__any_sync(0xffffffffu, there && token >= w.first && token - w.first < w.n)) {   // (of other pieces: nobody reads their sums)
+      keep();
+      at = -1;
+      continue;
+    }
+    const float rest = there ? __ldg(w.rest + i + lane) : 0.f;
+    uint2 x[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = wide && i + j < to ? __ldg(reinterpret_cast<const uint2*>(w.x + (i + j) * w.ld_x + col)) : make_uint2(0, 0);
+    bool first = there && token != before;
+    for (int s = 1; s < w.segments; ++s) first = first || (there && i + lane == start_of(s));
+    const unsigned begins = __ballot_sync(0xffffffffu, first);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const float by = __shfl_sync(0xffffffffu, rest, j);
+      if (begins >> j & 1u) {
+        keep();
+        at = i + j;
+      }
+      sum[0] = fmaf(by, __uint_as_float(x[j].x << 16), sum[0]);
+      sum[1] = fmaf(by, __uint_as_float(x[j].x & 0xffff0000u), sum[1]);
+      sum[2] = fmaf(by, __uint_as_float(x[j].y << 16), sum[2]);
+      sum[3] = fmaf(by, __uint_as_float(x[j].y & 0xffff0000u), sum[3]);
+    }
+  }
+  keep();
 }
 
 // The hidden rows' gradient: shares of a gathered row added in one order, and what rounding left of dz at its token (`rest`, null in float32) times the token's row of the
@@ -1440,7 +1611,7 @@ struct Layout {
   int pieces, splits;
   long long piece;                  // tokens at a time, a multiple of 256
   long long parts;
-  long long table, hidden, part, factors, shares, targets, factor, sums, rest, place, count, total;
+  long long table, hidden, part, factors, shares, targets, factor, sums, rest, rests, runs, place, starts, count, total;
 };
 
 bool copies_read(const void* at, long long ld, long long rows, long long width, int size = 2) {
@@ -1508,7 +1679,11 @@ Layout layout(int dtype, const void* table, long long ld_t, long long rows, long
     l.factor = take(l.rows_up * 4);
     l.sums = take(l.rows_up * 4);
     l.rest = take(l.rows_up * 4);
+    const long long segments = up(rows, SEGMENT) / SEGMENT;
+    l.rests = take(dtype == R2_BF16 && !few ? l.rows_up * l.width_up * 4 : 0);
+    l.runs = take(dtype == R2_BF16 && !few ? segments * l.piece * 8 : 0);
     l.place = take(rows * 4);
+    l.starts = take(dtype == R2_BF16 && !few ? segments * 4 : 0);
     l.count = take(4);
   }
   l.total = at;
@@ -1593,11 +1768,13 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
   const Operand x = {gathered, l.width_up, l.rows_up * l.width_up, l.planes};
   int* count = reinterpret_cast<int*>(space + l.count);
   int32_t* place = reinterpret_cast<int32_t*>(space + l.place);
+  int* starts = reinterpret_cast<int*>(space + l.starts);
   int own = (rows + 591) / 592;
-  own = own > 32 ? 32 : own;
-  r2_launch(gather_kernel<T>, dim3((rows + own - 1) / own + planes.blocks), dim3(256), size_t(0), stream,
+  own = own > OWN || rows > SEGMENT ? OWN : own;
+  constexpr bool BF16 = sizeof(T) == 2;
+  r2_launch(BF16 && !few ? gather_kernel<T, BF16> : gather_kernel<T, false>, dim3((rows + own - 1) / own + planes.blocks), dim3(256), size_t(0), stream,
       static_cast<const T*>(hidden), ld_h, rows, width, vocab, own, targets, weight, log_sum, gathered, x.ld, x.plane, reinterpret_cast<int32_t*>(space + l.targets),
-      reinterpret_cast<float*>(space + l.factor), reinterpret_cast<float*>(space + l.sums), place, count, planes);
+      reinterpret_cast<float*>(space + l.factor), reinterpret_cast<float*>(space + l.sums), place, count, starts, planes);
   Work w = {};
   w.m = rows;
   w.count = count;
@@ -1656,9 +1833,22 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
     }
     if (d_table) {
       Work& d = b.table = w;
-      d.rest = few && sizeof(T) == 2 ? w.rest : nullptr;
       d.x = gathered;
       d.ld_x = x.ld;
+      if (BF16 && !few) {
+        const int segments = int(up(rows, SEGMENT) / SEGMENT);
+        const long long slices = up(width, 128) / 128, warps = up(rows, WINDOW) / WINDOW * slices;
+        const Rests rests = {gathered, x.ld, w.targets, w.rest, count, starts, int(first), n, width, int(slices), segments, warps, reinterpret_cast<float*>(space + l.rests), l.width_up,
+                             reinterpret_cast<int2*>(space + l.runs), int(up(n, 32))};
+        const long long blocks = (warps + segments * (rests.run_tokens / 32) + 3) / 4;
+        if (blocks >= 1ll << 31) return R2_UNSUPPORTED;
+        r2_launch(rests_kernel, dim3(unsigned(blocks)), dim3(128), size_t(0), stream, rests);
+        d.runs = rests.runs;
+        d.sums = rests.sums;
+        d.ld_sums = rests.ld_sums;
+        d.segments = segments;
+        d.run_tokens = rests.run_tokens;
+      }
       d.m = n;
       d.n = width;
       T* out = static_cast<T*>(d_table) + first * ld_dt;
@@ -1674,13 +1864,18 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
     }
     constexpr bool F32 = sizeof(T) == 4;
     if (rows_units > 0 && table_units > 0 && rows_units + table_units <= resident_pairs()) {
-      static std::atomic<bool> done[64];
+      static std::atomic<bool> done[64], done_few[64];
+      constexpr int CHUNKED = F32 ? PLANES_CHUNK : 0;
       b.rows_pairs = int(rows_units);
-      status = launch_pairs(both_kernel<T, F32, F32 ? PLANES_CHUNK : 0>, done, rows_units + table_units, stream, b);
+      status = few && !F32 ? launch_pairs(both_kernel<F32 ? TABLE : TABLE_FEW, T, F32, CHUNKED>, done_few, rows_units + table_units, stream, b)
+                           : launch_pairs(both_kernel<TABLE, T, F32, CHUNKED>, done, rows_units + table_units, stream, b);
       continue;
     }
     if (rows_units > 0) status = launch<ROWS, float, F32>(b.rows_a, b.rows_b, b.rows_out, b.rows, rows_units, false, stream);
-    if (status == R2_OK && table_units > 0) status = launch<TABLE, T, F32>(b.table_a, b.table_b, b.table_out, b.table, table_units, false, stream);
+    if (status == R2_OK && table_units > 0) {
+      if (few && !F32) status = launch<F32 ? TABLE : TABLE_FEW, T, F32>(b.table_a, b.table_b, b.table_out, b.table, table_units, false, stream);
+      else status = launch<TABLE, T, F32>(b.table_a, b.table_b, b.table_out, b.table, table_units, false, stream);
+    }
   }
   if (status == R2_OK && d_hidden) {
     r2_launch(join_kernel<T>, dim3(row_blocks(static_cast<long long>(rows) * ((width + 127) / 128))), dim3(256), size_t(0), stream, static_cast<const float*>(shares), l.splits, share_plane, l.width_up,

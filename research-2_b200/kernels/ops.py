@@ -2317,7 +2317,7 @@ def token_loss_gradient(hidden: torch.Tensor, table: torch.Tensor, targets: torc
     """The gradients of the sum of `token_loss`'s losses: (of the hidden rows [N, D], of the table [V, D]), in their types; None for one that is not
     asked for. `log_sum` is `token_loss`'s for the same hidden rows, table and softcap; the other arguments as there. A row without a target, or of weight 0,
     has the gradient 0 and no part in the table's, whatever its hidden numbers are. (A factor of a logit below 2^-126 counts as 0. bfloat16 gradients: factors
-    but a row's own token's are rounded to bfloat16 before the products, the table's of more than 128 rows all of them.)"""
+    but a row's own token's are rounded to bfloat16 before the products.)"""
     if hidden.is_cuda:
         done = _logit_face("token_loss_gradient")(hidden, table, targets, log_sum, weight, softcap, hidden_gradient, table_gradient, _error_address(hidden))
         if done is not None:

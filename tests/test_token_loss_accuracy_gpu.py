@@ -1,0 +1,44 @@
+"""How exact losses of tokens and their gradients are where many rows, long rows or large batches could cost it: against 64 bits, with tolerances derived beside them
+(`tests/plain/vocabulary_plain.py` has the operators' own)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_token_loss_gpu import BF16, DEV, F32, Case, gen
+
+pytestmark = pytest.mark.gpu
+
+
+def common(c: Case, token: int, share: float) -> Case:
+    """One token for a share of the rows, scattered; its neighbours for a few more."""
+    hot = torch.rand(len(c.targets), generator=gen(1), device=DEV) < share
+    hot[:8] = False
+    c.targets[hot] = token
+    c.targets[7], c.targets[8], c.targets[9] = token - 1, token + 1, token + 32
+    return c
+
+
+@pytest.mark.parametrize("rows,width,vocab,token,share", [
+    (129, 64, 1500, 40, 0.0), (300, 96, 2500, 31, 0.1), (700, 257, 300, 255, 0.5), (1000, 72, 5000, 4000, 0.3), (513, 40, 64, 20, 0.95), (2000, 130, 900, 640, 0.04),
+    (70001, 40, 300, 77, 0.2)])
+def test_what_rounding_leaves_of_a_tokens_own_factor_is_in_the_tables_gradient(rows, width, vocab, token, share):
+    """bfloat16, tokens that the model finds unlikely: a row's factor is nearly all at its own token, a (p - 1). Its rounding, half a step of |a (p - 1)| times the hidden row, is not
+    in the table's gradient however many rows there are: the tolerance is the oracle's without it (4 units of 2^-24 in its place)."""
+    c = common(Case(rows, width, vocab, BF16, rows, size=0.05), token, share)
+    got, want = c.run(), c.plain()
+    a = torch.where((c.targets >= 0) & (c.targets < vocab), c.weight.double(), 0.0)
+    y = c.targets.clamp(0, vocab - 1).long()
+    own = a * torch.expm1(want.z.gather(1, y[:, None])[:, 0] - want.log_sum)
+    less = (2.0**-8 - 4 * 2.0**-24) * own.abs()[:, None]
+    x = torch.where(a[:, None] != 0, c.hidden.double(), 0.0)
+    off = want.d_table_off.index_add(0, y, -less * x.abs())
+    assert torch.all((got[3].double() - want.d_table).abs() <= off)
+    assert all(torch.equal(one, other) for one, other in zip(got, c.run()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,width,vocab", [(4096, 768, 50257), (2047, 1600, 10007)])
+def test_steps_of_training(rows, width, vocab, dtype):
+    common(Case(rows, width, vocab, dtype, rows), 13, 0.1).check()
