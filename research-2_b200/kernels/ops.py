@@ -2270,7 +2270,13 @@ def _space(device: torch.device, size: int) -> torch.Tensor:
     return torch.empty_strided((size,), (1,), dtype=torch.uint8, device=device)
 
 
+def _tokens_given(t, name: str, what: str) -> None:
+    if t is None:   # (`_per_row` takes None for a number that may be left out)
+        raise KernelError(f"{what}: {name} must be a tensor of int32, got None")
+
+
 def _loss_arguments(hidden, table, targets, weight, softcap, what):
+    _tokens_given(targets, "targets", what)
     code, rows, width, ld, device = _matrix(hidden, "hidden", what)
     table_code, vocab, table_width, table_ld, table_device = _matrix(table, "table", what)
     if table_code != code or table_width != width or table_device != device:
@@ -2358,6 +2364,7 @@ def token_rows(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, ou
         if done is not None:
             _check(done[0], "token_rows")
             return done[1]
+    _tokens_given(ids, "ids", "token_rows")
     code, vocab, width, ld, device = _matrix(table, "table", "token_rows")
     tokens = ids.shape[0] if ids.dim() == 1 else -1
     ids_at = _per_row(ids, "ids", torch.int32, tokens, device)
@@ -2383,6 +2390,7 @@ def token_rows_gradient(ids: torch.Tensor, above: torch.Tensor, vocab: int, *, s
         if done is not None:
             _check(done[0], "token_rows_gradient")
             return done[1]
+    _tokens_given(ids, "ids", "token_rows_gradient")
     code, tokens, width, ld, device = _matrix(above, "above", "token_rows_gradient")
     ids_at = _per_row(ids, "ids", torch.int32, tokens, device)
     if ids.shape[0] != tokens:
