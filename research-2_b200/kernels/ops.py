@@ -2351,8 +2351,8 @@ def token_loss_gradient(hidden: torch.Tensor, table: torch.Tensor, targets: torc
 
 def _scale(scale: float, what: str) -> float:
     scale = float(scale)
-    if not abs(scale) < float("inf"):
-        raise KernelError(f"{what}: scale must be finite, got {scale}")
+    if not abs(C.c_float(scale).value) < float("inf"):   # (as the kernel has it)
+        raise KernelError(f"{what}: scale must be finite in float32, got {scale}")
     return scale
 
 
@@ -2365,12 +2365,13 @@ def token_rows(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, ou
             _check(done[0], "token_rows")
             return done[1]
     _tokens_given(ids, "ids", "token_rows")
+    scale = _scale(scale, "token_rows")
     code, vocab, width, ld, device = _matrix(table, "table", "token_rows")
     tokens = ids.shape[0] if ids.dim() == 1 else -1
     ids_at = _per_row(ids, "ids", torch.int32, tokens, device)
     if tokens > 2**30:
         raise KernelError(f"token_rows: {tokens} tokens, 2^30 at most")
-    scale, out_dtype = _scale(scale, "token_rows"), out_dtype or table.dtype
+    out_dtype = out_dtype or table.dtype
     out = torch.empty_strided((tokens, width), (width, 1), dtype=out_dtype, device=table.device)
     out_code = dtype_code(out_dtype)
     if tokens and width:
@@ -2391,6 +2392,7 @@ def token_rows_gradient(ids: torch.Tensor, above: torch.Tensor, vocab: int, *, s
             _check(done[0], "token_rows_gradient")
             return done[1]
     _tokens_given(ids, "ids", "token_rows_gradient")
+    scale = _scale(scale, "token_rows_gradient")
     code, tokens, width, ld, device = _matrix(above, "above", "token_rows_gradient")
     ids_at = _per_row(ids, "ids", torch.int32, tokens, device)
     if ids.shape[0] != tokens:
@@ -2401,7 +2403,6 @@ def token_rows_gradient(ids: torch.Tensor, above: torch.Tensor, vocab: int, *, s
         raise KernelError(f"token_rows_gradient: vocab must be a whole number, got {vocab!r}") from None
     if not 1 <= vocab <= 2**30:
         raise KernelError(f"token_rows_gradient: vocab must be in [1, 2^30], got {vocab}")
-    scale = _scale(scale, "token_rows_gradient")
     if into is None:
         out_dtype = out_dtype or above.dtype
         out_code, out_ld = dtype_code(out_dtype), width

@@ -15,3 +15,11 @@ def test_tokens_that_are_not_there(call, name):
     """None is no address: a kernel would read its tokens from 0."""
     with pytest.raises(ops.KernelError, match=name):
         call()
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 3.4028236e38, float("inf"), float("nan")])
+def test_a_scale_that_the_kernel_would_have_as_infinity(scale):
+    for call in (lambda: ops.token_rows(Y, W, scale=scale), lambda: ops.token_rows_gradient(Y, X, 10, scale=scale), lambda: ops.token_rows_gradient(Y, X, 10, scale=scale, into=W)):
+        with pytest.raises(ops.KernelError, match="scale must be finite"):
+            call()
+    assert ops._scale(3.4028234663852886e38, "token_rows") == 3.4028234663852886e38
