@@ -23,6 +23,19 @@ from ..models.loading import load_model
 from .step import StepFunction
 
 
+def token_sequences(sequences) -> list[np.ndarray]:
+    """Sequences of token ids as int32; ValueError for one that has none, or numbers that are no token ids."""
+    out = []
+    for n, s in enumerate(sequences):
+        tokens = np.asarray(s).reshape(-1)
+        if len(tokens) == 0:
+            raise ValueError(f"sequence {n}: a sequence has no tokens")
+        if tokens.dtype.kind not in "iub" or tokens.min() < -(2**31) or tokens.max() >= 2**31:   # (a cast would make other tokens of them)
+            raise ValueError(f"sequence {n}: token ids must be whole numbers of 32 bits, got {tokens.dtype}")
+        out.append(tokens.astype(np.int32))
+    return out
+
+
 class Replay:
     """`max_tokens` is the most tokens that live requests hold at any time, each request's count
     rounded up to a multiple of `round_to`; the pool gets the pages for that many (a request whose

@@ -5,15 +5,13 @@ from __future__ import annotations
 
 import numpy as np
 
-from .replay import Replay
+from .replay import Replay, token_sequences
 
 
 def score(model_dir, sequences, *, dtype: str = "bfloat16", device: str = "cuda:0", portion: int = 2048, block_size: int = 16) -> list[np.ndarray]:
     """For each sequence of T token ids the log-probabilities of its tokens from the second on, float32 [T - 1]: entry t is that of tokens[t + 1] behind
     tokens[: t + 1]. `portion`: rows of a step."""
-    sequences = [np.asarray(s, dtype=np.int32).reshape(-1) for s in sequences]
-    if any(len(s) == 0 for s in sequences):
-        raise ValueError("a sequence has no tokens")
+    sequences = token_sequences(sequences)
     if portion < 1:
         raise ValueError(f"portion must be >= 1, got {portion}")
     longest = max((len(s) for s in sequences), default=0)

@@ -8,7 +8,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from .replay import Replay
+from .replay import Replay, token_sequences
 
 
 @dataclass(frozen=True)
@@ -26,9 +26,7 @@ class Lesson:
 def teach(model_dir, sequences, k: int = 64, temperature: float = 1.0, *, dtype: str = "bfloat16", device: str = "cuda:0", portion: int = 1024,
           block_size: int = 16) -> list[Lesson]:
     """A lesson for each sequence of token ids. `portion`: rows of a step (their logits are on the device at a time)."""
-    sequences = [np.asarray(s, dtype=np.int32).reshape(-1) for s in sequences]
-    if any(len(s) == 0 for s in sequences):
-        raise ValueError("a sequence has no tokens")
+    sequences = token_sequences(sequences)
     if portion < 1:
         raise ValueError(f"portion must be >= 1, got {portion}")
     if not sequences:
