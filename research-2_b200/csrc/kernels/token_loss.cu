@@ -154,14 +154,15 @@ __device__ __forceinline__ void split3(float x, bf16 (&p)[3]) {
   p[2] = __float2bfloat16_rn(rest);
 }
 
-// tanh(x) and 1 - tanh(x)^2: 1 - 2 h with h = 1 / (e^(2 x) + 1), and 4 h (1 - h); near 0, where the difference would cancel, the odd series up to
-// x^7 (its next term is below 6e-8 of it). Either is off by less than 1e-6 of itself, so that a cap far above the logits leaves them as they are.
+// tanh(x) and 1 - tanh(x)^2: with h = 1 / (e^(2 |x|) + 1), which is half at most, 1 - 2 h with x's sign, and 4 h (1 - h); near 0, where the difference would cancel, the odd
+// series up to x^7 (its next term is below 6e-8 of it). The tanh is off by less than 1e-6 of itself, so that a cap far above the logits leaves them as they are; the slope, on either side of 0, by
+// half a millionth and what rounding the exponent makes of it, 1.2e-7 |x|.
 __device__ __forceinline__ float cap_tanh(float x, float& slope) {
-  const float h = fast_rcp(fast_exp2(x * (2.f * LOG2E)) + 1.f), q = x * x;
+  const float h = fast_rcp(fast_exp2(fabsf(x) * (2.f * LOG2E)) + 1.f), q = x * x;
   const float series = fmaf(x * q, fmaf(q, fmaf(q, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), x);
   const bool near = q < 0.04f;
   slope = near ? fmaf(-series, series, 1.f) : 4.f * h * (1.f - h);
-  return near ? series : fmaf(-2.f, h, 1.f);
+  return near ? series : copysignf(fmaf(-2.f, h, 1.f), x);
 }
 
 // z log2 e of an accumulator.

@@ -42,3 +42,31 @@ def test_what_rounding_leaves_of_a_tokens_own_factor_is_in_the_tables_gradient(r
 @pytest.mark.parametrize("rows,width,vocab", [(4096, 768, 50257), (2047, 1600, 10007)])
 def test_steps_of_training(rows, width, vocab, dtype):
     common(Case(rows, width, vocab, dtype, rows), 13, 0.1).check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [40, 200])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_targets_far_beyond_the_cap(rows, dtype, sign):
+    """Row i learns token i, whose raw logit u is 3 to 12 caps below (above) 0: a factor is (p - 1 at a row's own token, p elsewhere) times the slope 1 - tanh(u / cap)^2, which has to be right relative to
+    itself however small it is. u is one exact product; u / cap and the exponent 2 |u / cap| log2 e are rounded five times, so that exp(2 |u / cap|) is off by 2 |u / cap| times five units of 2^-24, and a few
+    units come from the functions and the slope's products: (12 |u / cap| + 64) units of a factor. The rest as the oracle has it, each times the slope: what the logarithm of the sum leaves of a p, the 1's
+    rounding, the factors' (bfloat16), the sums' and the result's. (Above 0 a token's p of all rows nearly cancel its 1, so that these are most of it.)"""
+    cap, vocab, width = 6.0, 600, 8
+    table = torch.randn(vocab, width, generator=gen(2), device=DEV)
+    far = sign * cap * (3 + 9 * torch.rand(rows, generator=gen(3), device=DEV))
+    table[:rows, 0] = far
+    hidden = torch.zeros(rows, width, device=DEV)
+    hidden[:, 0] = 1.0
+    c = Case(1, width, vocab, dtype)
+    c.hidden, c.table, c.softcap, c.weight = hidden.to(dtype), table.to(dtype), cap, None
+    c.targets = torch.arange(rows, dtype=torch.int32, device=DEV)
+    _, _, _, d_table = c.run()
+    want = c.plain()
+    x = c.table[:rows, 0].double().abs() / cap
+    z = want.z[:, :rows]   # [row, token]
+    p, slope, own = torch.exp(z - want.log_sum[:, None]), 1 / torch.cosh(c.table[:rows, 0].double() / cap) ** 2, torch.eye(rows, device=DEV, dtype=torch.float64)
+    dz = (p - own).abs() * slope
+    dz_off = p * slope * torch.expm1(2 * want.log_sum_off)[:, None] + own * slope * 4 * 2.0**-24 + dz * ((12 * x + 64) * 2.0**-24 + (2.0**-8 if dtype is BF16 else 0.0))
+    off = dz_off.sum(0) + (4 * rows / 8 + 64) * 2.0**-24 * dz.sum(0) + (2.0**-8 if dtype is BF16 else 2.0**-24) * want.d_table[:rows, 0].abs()
+    assert torch.all((d_table[:rows, 0].double() - ((p - own) * slope).sum(0)).abs() <= off)
