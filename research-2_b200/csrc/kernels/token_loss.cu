@@ -197,9 +197,10 @@ template <int MODE> __device__ __forceinline__ Unit unit_of(const Work& w, long 
   return u;
 }
 
-// Steps of k that are added in tensor memory before their sum goes into registers (0: all): 256 of k with the products of planes; 512 where float results are
-// made of more than 768 bfloat16 products (1,024 of them: off by up to 1.2e-6 of the loss otherwise; 1,600: by 2.4e-7 in place of 7.7e-7, and 5 % slower).
-constexpr int PLANES_CHUNK = 4, LONG_CHUNK = 8, LONG_STEPS = 12;
+// Steps of k that are added in tensor memory before their sum goes into registers (0: all): 256 of k with the products of planes; 512 where logits are
+// made of more than 768 bfloat16 products (1,024 of them: off by up to 1.2e-6 of the loss otherwise; 1,600: by 2.4e-7 in place of 7.7e-7, and 5 % slower), in the loss and in its
+// gradients alike; 32,768 in gradients, whose sums are then off by 2^-13 at most, a 32th of half a step of bfloat16.
+constexpr int PLANES_CHUNK = 4, LONG_CHUNK = 8, LONG_STEPS = 12, GRADIENT_CHUNK = 512;
 
 // How many times a unit's products go through an accumulator.
 template <int CHUNKED> __device__ __forceinline__ int sums_of(const Unit& u) {
@@ -1583,7 +1584,7 @@ int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, FewWork f, cudaStre
 }
 
 template <int MODE, bool F32> int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, const FewWork& f, bool capped, cudaStream_t stream) {
-  if constexpr (MODE == LOGSUM && !F32) {
+  if constexpr (!F32) {
     if (f.k > FEW_CHUNK) return capped ? launch_few<MODE, true, F32, true>(mt, mx, f, stream) : launch_few<MODE, false, F32, true>(mt, mx, f, stream);
   }
   return capped ? launch_few<MODE, true, F32, F32>(mt, mx, f, stream) : launch_few<MODE, false, F32, F32>(mt, mx, f, stream);
@@ -1815,7 +1816,9 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
       if (!make_map(&ma, x, width, l.rows_up, BM) || !make_map(&mb, part, width, n, HALF) ||
           !make_out_map<bf16>(&mo, dz.at, l.piece, l.rows_up, l.planes, l.piece, dz.plane))
         return R2_BAD_ALIGN;
-      status = launch<FACTORS, bf16, sizeof(T) == 4>(ma, mb, mo, w, row_tiles * (up(n, BN) / BN), softcap > 0.f, stream);
+      const long long tiles = row_tiles * (up(n, BN) / BN);
+      if (BF16 && width > LONG_STEPS * BK) status = launch<FACTORS, bf16, false, LONG_CHUNK>(ma, mb, mo, w, tiles, softcap > 0.f, stream);
+      else status = launch<FACTORS, bf16, sizeof(T) == 4>(ma, mb, mo, w, tiles, softcap > 0.f, stream);
     }
     if (status != R2_OK) break;
     Both b = {};
@@ -1872,10 +1875,17 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
                            : launch_pairs(both_kernel<TABLE, T, F32, CHUNKED>, done, rows_units + table_units, stream, b);
       continue;
     }
-    if (rows_units > 0) status = launch<ROWS, float, F32>(b.rows_a, b.rows_b, b.rows_out, b.rows, rows_units, false, stream);
-    if (status == R2_OK && table_units > 0) {
-      if (few && !F32) status = launch<F32 ? TABLE : TABLE_FEW, T, F32>(b.table_a, b.table_b, b.table_out, b.table, table_units, false, stream);
-      else status = launch<TABLE, T, F32>(b.table_a, b.table_b, b.table_out, b.table, table_units, false, stream);
+    if constexpr (F32) {
+      if (rows_units > 0) status = launch<ROWS, float, true>(b.rows_a, b.rows_b, b.rows_out, b.rows, rows_units, false, stream);
+      if (status == R2_OK && table_units > 0) status = launch<TABLE, T, true>(b.table_a, b.table_b, b.table_out, b.table, table_units, false, stream);
+    } else {
+      if (rows_units > 0)
+        status = b.rows.per_split > GRADIENT_CHUNK ? launch<ROWS, float, false, GRADIENT_CHUNK>(b.rows_a, b.rows_b, b.rows_out, b.rows, rows_units, false, stream)
+                                                   : launch<ROWS, float, false>(b.rows_a, b.rows_b, b.rows_out, b.rows, rows_units, false, stream);
+      if (status == R2_OK && table_units > 0)
+        status = few                         ? launch<TABLE_FEW, T, false>(b.table_a, b.table_b, b.table_out, b.table, table_units, false, stream)
+                 : rows > GRADIENT_CHUNK * BK ? launch<TABLE, T, false, GRADIENT_CHUNK>(b.table_a, b.table_b, b.table_out, b.table, table_units, false, stream)
+                                             : launch<TABLE, T, false>(b.table_a, b.table_b, b.table_out, b.table, table_units, false, stream);
     }
   }
   if (status == R2_OK && d_hidden) {

@@ -6,7 +6,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_token_loss_gpu import BF16, DEV, F32, Case, gen
+from tests.plain.vocabulary_plain import Loss
+from tests.test_token_loss_gpu import BF16, DEV, F32, Case, gen, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +71,40 @@ def test_targets_far_beyond_the_cap(rows, dtype, sign):
     dz_off = p * slope * torch.expm1(2 * want.log_sum_off)[:, None] + own * slope * 4 * 2.0**-24 + dz * ((12 * x + 64) * 2.0**-24 + (2.0**-8 if dtype is BF16 else 0.0))
     off = dz_off.sum(0) + (4 * rows / 8 + 64) * 2.0**-24 * dz.sum(0) + (2.0**-8 if dtype is BF16 else 2.0**-24) * want.d_table[:rows, 0].abs()
     assert torch.all((d_table[:rows, 0].double() - ((p - own) * slope).sum(0)).abs() <= off)
+
+
+def test_sums_over_very_many_rows():
+    """Tensor cores cut every addition of 16 products by up to a unit of 2^-24 of the sum, towards zero, so that sums of one sign are off by as many units as they have additions: 524,288 rows have
+    32,768 of them. Sums of 32,768 rows at most are made there (2,048 units at most), and joined rounded to nearest. The mean over a table's gradient of 31 x 1,024 numbers of the error relative to each: of
+    the cuts 2^-13; of the results' and factors' rounding, 2^-8 / sqrt(3) each for one number, 6 deviations of the mean; of the probabilities 1e-5, as the oracle has it."""
+    rows, width, vocab = 524288, 1024, 32
+    hidden = torch.empty(rows, width, dtype=BF16, device=DEV)
+    for i in range(0, rows, 65536):   # positive; columns all over a binade, so that their roundings differ
+        hidden[i: i + 65536] = (0.5 + torch.rand(65536, width, generator=gen(i), device=DEV)) * 2 ** torch.linspace(0, 1, width, device=DEV)
+    table = (torch.randn(vocab, width, generator=gen(5), device=DEV) / 32).to(BF16)
+    targets = torch.zeros(rows, dtype=torch.int32, device=DEV)
+    _, log_sum = ops().token_loss(hidden, table, targets)
+    _, d_table = ops().token_loss_gradient(hidden, table, targets, log_sum, hidden_gradient=False)
+    ops().raise_on_device_error(DEV)
+    want = torch.zeros(vocab, width, dtype=torch.float64, device=DEV)
+    for i in range(0, rows, 65536):
+        x = hidden[i: i + 65536].double()
+        want += torch.softmax(x @ table.double().t(), 1).t() @ x
+    error = ((d_table.double() - want) / want)[1:]   # (token 0's: p - 1)
+    assert abs(error.mean().item()) <= 2.0**-13 + 6 * 2 * 2.0**-8 / 3**0.5 / error.numel() ** 0.5 + 1e-5
+
+
+@pytest.mark.parametrize("rows", [64, 256])
+def test_the_gradients_logits_are_the_losses(rows):
+    """Rows of 16,384 positive numbers, logits near 40: products added in one sum on the tensor cores would leave them 1,024 cuts of up to 2^-24 of 40 too low (2.4e-3), pieces of 512 (256) 32 (16) of them.
+    A factor exp(z - log_sum) takes its z from the loss's pieces: the mean over all factors, relative, differs by what cuts differ by (none) and what the sum's logarithm (near 48, rounded three times:
+    1.2e-5), exponent and function (5e-6) are rounded to; the factors' own rounding, 6 deviations of the mean; the cuts of 256 rows' sums (16 units of 2^-24)."""
+    width, vocab = 16384, 2000
+    hidden = (1 + torch.rand(rows, width, generator=gen(6), device=DEV)).to(BF16)
+    table = ((0.5 + torch.rand(vocab, width, generator=gen(7), device=DEV)) * (40 / 1.5 / width)).to(BF16)
+    targets = torch.zeros(rows, dtype=torch.int32, device=DEV)
+    loss, log_sum = ops().token_loss(hidden, table, targets)
+    _, d_table = ops().token_loss_gradient(hidden, table, targets, log_sum, hidden_gradient=False)
+    want = Loss(hidden, table, targets)
+    error = ((d_table.double() - want.d_table) / want.d_table)[1:]
+    assert abs(error.mean().item()) <= 1.7e-5 + 6 * 2.0**-8 / 3**0.5 / ((vocab - 1) * rows) ** 0.5 + 6 * 2.0**-8 / 3**0.5 / error.numel() ** 0.5 + 16 * 2.0**-24
