@@ -61,6 +61,12 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 constexpr int ERR_FULL = 1, ERR_EMPTY = 2, ERR_ACC = 3;   // codes of waits that ran out, as of the other products
 
+// A wait that ran out leaves NaN: a sum that is not whole is not handed over, so that the wait for it runs out, too; warps that have given up a wait hand nothing back, which others would take for
+// a word of those that still read, and make NaN of their tile and the later ones, in dz as in the results. (A test builds this file with warps that give up: of results, 1, or of products, 2.)
+#ifndef R2_LOSS_GIVES_UP
+#define R2_LOSS_GIVES_UP 0
+#endif
+
 enum Mode { LOGSUM, FACTORS, ROWS, TABLE, TABLE_FEW };   // (TABLE_FEW: bfloat16 rows that a tile's warps find by themselves)
 
 constexpr bool is_table(int mode) { return mode == TABLE || mode == TABLE_FEW; }
@@ -115,8 +121,14 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {   // arrives on both
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// The whole warp's wait: its lanes go on together, also when it ran out.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+// The whole warp's wait: its lanes go on together, also when it ran out (after some 17 seconds; 65 ms where a test has warps give up).
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+  bool done = false;
+  if constexpr (R2_LOSS_GIVES_UP == 0) done = mbar_wait(bar, parity);
+  else
+    for (int i = 0; i < 1 << 14 && !done; ++i) done = mbar_try_wait(bar, parity) != 0;
+  return __all_sync(0xffffffffu, done);
+}
 // 32 rows of 128 bytes from shared memory into a box of the map (what lies outside is left out), or added to float numbers there.
 __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, int plane, uint32_t from) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(from), "r"(x), "r"(y), "r"(plane) : "memory");
@@ -381,7 +393,11 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
             parity ^= 1u;
           }
         }
-        if (elect_one()) commit_pair(acc_full + buf * 8);   // also on the error path: the others go on and the flag tells
+        if (R2_LOSS_GIVES_UP == 2) {
+          if (lane == 0) atomicMax(w.error_flag, ERR_FULL);
+          ok = false;
+        }
+        if (ok && elect_one()) commit_pair(acc_full + buf * 8);
         __syncwarp();
       }
     }
@@ -565,15 +581,42 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
         }
       };
       auto left = [&](int c) { return col0 + c < w.n && (MODE == LOGSUM || MODE == FACTORS || row0 < m); };
+      auto give_up = [&] {   // NaN in place of the warp's part of the tile (for LOGSUM below)
+        if constexpr (MODE != LOGSUM) {
+          constexpr bool NARROW = MODE == FACTORS || sizeof(T) == 2;   // two numbers to four bytes
+          constexpr int COLUMNS = NARROW ? 64 : 32;
+          const uint32_t nan = MODE == FACTORS && row >= m ? 0u : NARROW ? 0x7fff7fffu : 0x7fffffffu;
+          if constexpr (MODE == FACTORS && !PLANES) {
+            if (target >= side * HALF && target < (side + 1) * HALF) w.rest[row] = NAN;
+          }
+#pragma unroll 1
+          for (int c = side * HALF; c < (side + 1) * HALF && left(c); c += COLUMNS) {
+            if (is_table(MODE) && w.out != nullptr) {
+#pragma unroll 1
+              for (int j = 0; j < COLUMNS; ++j)
+                if (row < m && col0 + c + j < w.n) static_cast<T*>(w.out)[row * w.ld + col0 + c + j] = from_float<T>(NAN);
+              continue;
+            }
+#pragma unroll 1
+            for (int plane = 0; plane < (PLANES && MODE == FACTORS ? 3 : 1); ++plane) {
+              const uint32_t slab = out.begin();
+#pragma unroll 1
+              for (int p = 0; p < 8; ++p) out.put16(slab, p, nan, nan, nan, nan);
+              out.end(&map_out, col0 + c, row0, MODE == ROWS ? u.split : plane, slab, MODE == ROWS && w.add);
+            }
+          }
+        }
+      };
       const uint32_t lanes = uint32_t(q * 32) << 16;
       auto wait_sum = [&](uint32_t buf) {
-        if (ok && !warp_wait(acc_full + buf * 8, (local >> 1) & 1u)) {
+        if (ok && (!warp_wait(acc_full + buf * 8, (local >> 1) & 1u) || R2_LOSS_GIVES_UP == 1)) {
           if (lane == 0) atomicMax(w.error_flag, ERR_ACC);
-          ok = false;   // this and the later tiles are not written; the flag tells
+          ok = false;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       };
       auto hand_back = [&](uint32_t buf) {
+        if (!ok) return;
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) arrive_cluster(leader_acc_empty + buf * 8);
@@ -600,6 +643,7 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
           }
           hand_back(buf);
         }
+        if (!ok) give_up();
         if (ok && left(side * HALF)) finish(side * HALF, lo);
         if (ok && left(side * HALF + 64)) finish(side * HALF + 64, hi);
       } else {
@@ -616,6 +660,7 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
           }
           finish(c, v);
         }
+        if (!ok) give_up();
         hand_back(buf);
       }
       if constexpr (MODE == LOGSUM) {
@@ -693,6 +738,13 @@ __device__ __forceinline__ uint64_t smem_desc_64(uint32_t addr) {   // K-major r
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, int plane, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(plane) : "memory");
+}
+
+// Whether any of the 128 threads of barrier 1 says so, which meet there.
+__device__ __forceinline__ bool any_of_128(bool mine) {
+  uint32_t any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"(uint32_t(mine)) : "memory");
+  return any != 0;
 }
 
 // Shared memory from its 1,024-byte aligned start. bfloat16: stages of 16 KB of the table and columns * 128 bytes of rows. float32: `loads` of 16 KB of the
@@ -833,7 +885,11 @@ __global__ void __launch_bounds__(few_threads(F32), 1) few_kernel(const __grid_c
             parity ^= 1u;
           }
         }
-        if (elect_one()) umma_commit(acc_full + buf * 8);   // also on the error path: the others go on and the flag tells
+        if (R2_LOSS_GIVES_UP == 2) {
+          if (lane == 0) atomicMax(f.w.error_flag, ERR_FULL);
+          ok = false;
+        }
+        if (ok && elect_one()) umma_commit(acc_full + buf * 8);
         __syncwarp();
       }
     }
@@ -855,7 +911,7 @@ __global__ void __launch_bounds__(few_threads(F32), 1) few_kernel(const __grid_c
       uint32_t buf = 0;
       for (int lo = 0; lo < n_kb; lo += per_sum) {
         buf = local & (bufs - 1);
-        if (ok && !warp_wait(acc_full + buf * 8, (local >> (bufs - 1)) & 1u)) {
+        if (ok && (!warp_wait(acc_full + buf * 8, (local >> (bufs - 1)) & 1u) || R2_LOSS_GIVES_UP == 1)) {
           if (lane == 0) atomicMax(f.w.error_flag, ERR_ACC);
           ok = false;
         }
@@ -886,7 +942,7 @@ __global__ void __launch_bounds__(few_threads(F32), 1) few_kernel(const __grid_c
           tmem_store_wait();
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty + buf * 8);
+          if (lane == 0 && ok) mbar_arrive(acc_empty + buf * 8);
           ++local;
         }
       }
@@ -900,12 +956,16 @@ __global__ void __launch_bounds__(few_threads(F32), 1) few_kernel(const __grid_c
 #pragma unroll
           for (int j = 0; j < 32; ++j) turned[j * TURNED + q * 32 + lane] = __uint_as_float(r[j]);
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        ok = !any_of_128(!ok);   // (what a warp turns is of all four warps' lanes)
+        if (!ok) {
+#pragma unroll 1
+          for (int j = 0; j < 32; ++j) turned[lane * TURNED + part * 32 + j] = NAN;   // (what this thread reads)
+        }
         const int row = g * 32 + lane;
         float v[32];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 x = *reinterpret_cast<const float4*>(turned + lane * TURNED + part * 32 + 4 * i);
+          const float4 x = *reinterpret_cast<const float4*>(turned + lane * TURNED + part * 32 + 4 * i);   // (given up: NaN, below)
           v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
         }
         if constexpr (MODE == LOGSUM) {
@@ -958,7 +1018,7 @@ __global__ void __launch_bounds__(few_threads(F32), 1) few_kernel(const __grid_c
             }
           }
           const uint32_t sign = factor < 0.f ? 0x80008000u : 0u, held = row < m ? 0xffffffffu : 0u;
-          if (left > 0 && ok) {
+          if (left > 0) {
             bf16* to = f.dz + row * f.ld + token0;
             for (int plane = 0; plane < (F32 ? 3 : 1); ++plane) {
 #pragma unroll
@@ -984,7 +1044,7 @@ __global__ void __launch_bounds__(few_threads(F32), 1) few_kernel(const __grid_c
       if constexpr (!SUMS) {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty + buf * 8);
+        if (lane == 0 && ok) mbar_arrive(acc_empty + buf * 8);
         ++local;
       }
     }
