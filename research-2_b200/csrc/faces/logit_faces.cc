@@ -25,7 +25,7 @@ using AdjustEntry = int (*)(int, const void*, long long, void*, long long, int, 
 using TopEntry = int (*)(int, const void*, long long, int, int, int, float, float*, int32_t*, float*, int*, cudaStream_t);
 using DistillEntry = int (*)(int, const void*, long long, int, int, const int32_t*, const float*, int, const float*, const float*, float, float*, void*,
                              long long, int*, cudaStream_t);
-using LossEntry = int (*)(int, const void*, long long, const void*, long long, int, int, int, const int32_t*, const float*, float, float*, float*, void*, int*, cudaStream_t);
+using LossEntry = int (*)(int, const void*, long long, const void*, long long, int, int, int, const int32_t*, const float*, float, int, float*, float*, void*, int*, cudaStream_t);
 using LossGradientEntry = int (*)(int, const void*, long long, const void*, long long, int, int, int, const int32_t*, const float*, const float*, float, void*, long long, void*,
                                   long long, void*, int*, cudaStream_t);
 using LossSpace = long long (*)(int, const void*, long long, int, int, int, int, int);
@@ -288,7 +288,7 @@ PyObject* token_loss(PyObject*, PyObject* const* arg, Py_ssize_t n_args) {
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(l.x.device).stream();
   int status;
   Py_BEGIN_ALLOW_THREADS
-  status = loss_entry(l.x.code, l.x.t->data_ptr(), l.x.ld, l.w.t->data_ptr(), l.w.ld, int(l.x.rows), int(l.x.vocab), int(l.w.rows), l.targets, l.weight, float(l.softcap),
+  status = loss_entry(l.x.code, l.x.t->data_ptr(), l.x.ld, l.w.t->data_ptr(), l.w.ld, int(l.x.rows), int(l.x.vocab), int(l.w.rows), l.targets, l.weight, float(l.softcap), 0,
                       static_cast<float*>(loss.data_ptr()), static_cast<float*>(log_sum.data_ptr()), space.data_ptr(), error, stream);
   Py_END_ALLOW_THREADS
   return answer(status, loss, log_sum);

@@ -1685,7 +1685,7 @@ bool few_rows(int dtype, const void* table, long long ld_t, long long rows, long
   return rows <= FEW && (dtype == R2_BF16 || copies_read(table, ld_t, vocab, width, 4));
 }
 
-Layout layout(int dtype, const void* table, long long ld_t, long long rows, long long width, long long vocab, bool gradient, bool d_hidden) {
+Layout layout(int dtype, const void* table, long long ld_t, long long rows, long long width, long long vocab, bool few, bool gradient, bool d_hidden) {
   Layout l = {};
   l.planes = dtype == R2_F32 ? 3 : 1;
   l.rows_up = up(rows, 256);
@@ -1696,7 +1696,6 @@ Layout layout(int dtype, const void* table, long long ld_t, long long rows, long
     at += up(bytes, 256);
     return begin;
   };
-  const bool few = few_rows(dtype, table, ld_t, rows, width, vocab);
   l.copied = dtype == R2_BF16 ? !copies_read(table, ld_t, vocab, width) : !few || d_hidden;
   l.table = take(l.copied ? l.planes * vocab * l.width_up * 2 : 0);
   l.hidden = take(l.planes * l.rows_up * l.width_up * 2);
@@ -1774,9 +1773,10 @@ void set_cap(Work& w, float softcap) {
 
 template <typename T>
 int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_t, int rows, int width, int vocab, const int32_t* targets, const float* weight,
-            float softcap, float* loss, float* log_sum, char* space, int* error, cudaStream_t stream) {
+            float softcap, bool alike, float* loss, float* log_sum, char* space, int* error, cudaStream_t stream) {
   constexpr int dtype = sizeof(T) == 4 ? R2_F32 : R2_BF16;
-  const Layout l = layout(dtype, table, ld_t, rows, width, vocab, false, false);
+  const bool few = !alike && few_rows(dtype, table, ld_t, rows, width, vocab);
+  const Layout l = layout(dtype, table, ld_t, rows, width, vocab, few, false, false);
   const Operand x = operand<T>(hidden, ld_h, rows, width, l, space + l.hidden, stream);
   Work w = {};
   w.part = reinterpret_cast<float2*>(space + l.part);
@@ -1785,7 +1785,7 @@ int loss_of(const void* hidden, long long ld_h, const void* table, long long ld_
   set_cap(w, softcap);
   CUtensorMap ma, mb;
   int status;
-  if (few_rows(dtype, table, ld_t, rows, width, vocab)) {
+  if (few) {
     const void* at = table;
     long long ld = vocab > 1 ? ld_t : l.width_up;
     if (sizeof(T) == 2) {
@@ -1821,8 +1821,8 @@ template <typename T>
 int gradient_of(const void* hidden, long long ld_h, const void* table, long long ld_t, int rows, int width, int vocab, const int32_t* targets, const float* weight,
                 const float* log_sum, float softcap, void* d_hidden, long long ld_dh, void* d_table, long long ld_dt, char* space, int* error, cudaStream_t stream) {
   constexpr int dtype = sizeof(T) == 4 ? R2_F32 : R2_BF16;
-  const Layout l = layout(dtype, table, ld_t, rows, width, vocab, true, d_hidden != nullptr);
   const bool few = few_rows(dtype, table, ld_t, rows, width, vocab);
+  const Layout l = layout(dtype, table, ld_t, rows, width, vocab, few, true, d_hidden != nullptr);
   Operand t = {};   // (few float32 rows read the table as it is for their factors)
   Planes<T> planes = {};
   if (sizeof(T) == 2 || l.copied) t = operand<T>(table, ld_t, vocab, width, l, space + l.table, planes);
@@ -1960,18 +1960,19 @@ constexpr int MOST = 1 << 30;   // rows, numbers of a row, tokens: indexes of ti
 
 }  // namespace
 
-// Bytes of scratch for a call: of a loss, or (`gradient`) of gradients, of the hidden rows' (`d_hidden`) or of the table's alone.
-extern "C" long long r2_token_loss_space(int dtype, const void* table, long long ld_t, int rows, int width, int vocab, int gradient, int d_hidden) {
-  return layout(dtype, table, ld_t, rows, width, vocab, gradient != 0, d_hidden != 0).total;
+// Bytes of scratch for a call: of a loss (`choice`: `alike`), or (`gradient`) of gradients, of the hidden rows' too (`choice`) or of the table's alone.
+extern "C" long long r2_token_loss_space(int dtype, const void* table, long long ld_t, int rows, int width, int vocab, int gradient, int choice) {
+  const bool few = (gradient || !choice) && few_rows(dtype, table, ld_t, rows, width, vocab);
+  return layout(dtype, table, ld_t, rows, width, vocab, few, gradient != 0, gradient && choice).total;
 }
 
-// `space`: 256-byte aligned, r2_token_loss_space bytes.
+// `space`: 256-byte aligned, r2_token_loss_space bytes. `alike`: a row's results do not depend on how many rows there are (few ones go through the many's kernel).
 extern "C" int r2_token_loss(int dtype, const void* hidden, long long ld_h, const void* table, long long ld_t, int rows, int width, int vocab,
-                             const int32_t* targets, const float* weight, float softcap, float* loss, float* log_sum, void* space, int* error, cudaStream_t stream) {
+                             const int32_t* targets, const float* weight, float softcap, int alike, float* loss, float* log_sum, void* space, int* error, cudaStream_t stream) {
   if (rows < 1 || width < 1 || vocab < 1) return R2_BAD_SHAPE;
   if (rows > MOST || width > MOST || vocab > MOST) return R2_UNSUPPORTED;
-  if (dtype == R2_F32) return loss_of<float>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, softcap, loss, log_sum, (char*)space, error, stream);
-  if (dtype == R2_BF16) return loss_of<bf16>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, softcap, loss, log_sum, (char*)space, error, stream);
+  if (dtype == R2_F32) return loss_of<float>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, softcap, alike != 0, loss, log_sum, (char*)space, error, stream);
+  if (dtype == R2_BF16) return loss_of<bf16>(hidden, ld_h, table, ld_t, rows, width, vocab, targets, weight, softcap, alike != 0, loss, log_sum, (char*)space, error, stream);
   return R2_BAD_DTYPE;
 }
 

@@ -10,7 +10,7 @@ from .replay import Replay, token_sequences
 
 def score(model_dir, sequences, *, dtype: str = "bfloat16", device: str = "cuda:0", portion: int = 2048, block_size: int = 16) -> list[np.ndarray]:
     """For each sequence of T token ids the log-probabilities of its tokens from the second on, float32 [T - 1]: entry t is that of tokens[t + 1] behind
-    tokens[: t + 1]. `portion`: rows of a step."""
+    tokens[: t + 1]. `portion`: rows of a step; float32 scores are the same bits whatever it is."""
     sequences = token_sequences(sequences)
     if portion < 1:
         raise ValueError(f"portion must be >= 1, got {portion}")

@@ -1938,7 +1938,7 @@ _LOGIT_SIGNATURES = {
     "distill": [C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
                 C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p],
     "scale_rows": [C.c_int, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p],
-    "token_loss": [C.c_int, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
+    "token_loss": [C.c_int, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_int, C.c_void_p,
                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
     "token_loss_gradient": [C.c_int, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
                             C.c_float, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p],
@@ -2292,7 +2292,7 @@ def _loss_arguments(hidden, table, targets, weight, softcap, what):
     return code, rows, width, ld, vocab, table_ld, device, targets_at, weight_at, softcap
 
 
-def token_loss(hidden: torch.Tensor, table: torch.Tensor, targets: torch.Tensor, *, weight: torch.Tensor | None = None, softcap: float = 0.0):
+def token_loss(hidden: torch.Tensor, table: torch.Tensor, targets: torch.Tensor, *, weight: torch.Tensor | None = None, softcap: float = 0.0, alike: bool = False):
     """How unlikely a model finds given tokens, from its hidden rows, without the logits in memory: (loss float32 [N], log_sum float32 [N]).
 
     `hidden` [N, D] are the rows that the head multiplies with `table` [V, D] (both float32 or both bfloat16; rows contiguous, any row stride);
@@ -2300,8 +2300,9 @@ def token_loss(hidden: torch.Tensor, table: torch.Tensor, targets: torch.Tensor,
     sum of exp(z), and loss = weight * (log_sum - z[target]), minus the token's log-probability at weight 1 (`weight` float32 [N]; None: 1). A target outside
     [0, V) (-1 or -100, say) is none: its row has the loss 0, as has a row of weight 0. Logits that hold +inf or NaN, or nothing but -inf, make a
     row's log_sum and loss NaN or infinite, and no other row's. (float32 products are made of bfloat16 planes, which hold no infinities: an infinite number of a float32 table
-    counts as 3.39e38, and a float32 hidden row with one has the log_sum NaN.)"""
-    if hidden.is_cuda:
+    counts as 3.39e38, and a float32 hidden row with one has the log_sum NaN.) `alike`: a row's results are the same bits however many rows are beside it; without, up to 128 rows go through
+    a kernel of their own, which is faster and adds in another order."""
+    if hidden.is_cuda and not alike:
         done = _logit_face("token_loss")(hidden, table, targets, weight, softcap, _error_address(hidden))
         if done is not None:
             _check(done[0], "token_loss")
@@ -2312,8 +2313,8 @@ def token_loss(hidden: torch.Tensor, table: torch.Tensor, targets: torch.Tensor,
     log_sum = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=where)
     if rows:
         stream = _current_stream(device)
-        space = _space(where, _logit_entry("token_loss_space")(code, table.data_ptr(), table_ld, rows, width, vocab, 0, 0))
-        _check(_logit_entry("token_loss")(code, hidden.data_ptr(), ld, table.data_ptr(), table_ld, rows, width, vocab, targets_at, weight_at, softcap,
+        space = _space(where, _logit_entry("token_loss_space")(code, table.data_ptr(), table_ld, rows, width, vocab, 0, int(alike)))
+        _check(_logit_entry("token_loss")(code, hidden.data_ptr(), ld, table.data_ptr(), table_ld, rows, width, vocab, targets_at, weight_at, softcap, int(alike),
                                           loss.data_ptr(), log_sum.data_ptr(), space.data_ptr(), _workspace(where).error.data_ptr(), stream), "token_loss")
     return loss, log_sum
 

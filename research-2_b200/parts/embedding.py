@@ -39,5 +39,5 @@ class Head:
         return ops.soft_cap(logits, self.softcap) if self.softcap > 0.0 else logits
 
     def losses(self, x, rows, targets):
-        """Minus the log-probability of targets[i] (int32) behind row rows[i], float32 [W]: the logits' loss without the logits in memory."""
-        return ops.token_loss(self.norm.forward(x, self.compute_dtype, rows=rows), self.table, targets, softcap=self.softcap)[0]
+        """Minus the log-probability of targets[i] (int32) behind row rows[i], float32 [W]: the logits' loss without the logits in memory. In float32 it does not depend on how many rows there are, as logits do not."""
+        return ops.token_loss(self.norm.forward(x, self.compute_dtype, rows=rows), self.table, targets, softcap=self.softcap, alike=self.compute_dtype is torch.float32)[0]

@@ -35,7 +35,7 @@ def test_a_wait_that_runs_out_is_marked(rows, width, vocab, dtype, gives_up, mon
     space = torch.empty(size, dtype=torch.uint8, device=DEV)
     loss, log_sum, d_hidden, d_table = (torch.full_like(t, -1.0) for t in want)
     error, stream = o._error_address(hidden), o._current_stream(0)
-    assert entry("token_loss")(code, hidden.data_ptr(), width, table.data_ptr(), width, rows, width, vocab, c.targets.data_ptr(), c.weight.data_ptr(), 0.0, loss.data_ptr(),
+    assert entry("token_loss")(code, hidden.data_ptr(), width, table.data_ptr(), width, rows, width, vocab, c.targets.data_ptr(), c.weight.data_ptr(), 0.0, 0, loss.data_ptr(),
                                log_sum.data_ptr(), space.data_ptr(), error, stream) == 0
     with pytest.raises(o.KernelTimeout):
         o.raise_on_device_error(DEV)
