@@ -749,11 +749,11 @@ __device__ __forceinline__ bool any_of_128(bool mine) {
 
 // Shared memory from its 1,024-byte aligned start. bfloat16: stages of 16 KB of the table and columns * 128 bytes of rows. float32: `loads` of 16 KB of the
 // table's numbers, stages of three planes of 8 KB and columns * 64 bytes each. Then the turned tile and the barriers.
-template <bool F32> __host__ __device__ inline uint32_t few_stage_bytes(int columns) {
+template <bool F32> __host__ __device__ constexpr uint32_t few_stage_bytes(int columns) {
   return F32 ? 3u * (8192u + uint32_t(columns) * 64u) : 16384u + uint32_t(columns) * 128u;
 }
 constexpr uint32_t TURNED_BYTES = 32 * TURNED * 4;
-template <bool F32> __host__ __device__ inline uint32_t few_smem(int columns, int stages, int loads) {
+template <bool F32> __host__ __device__ constexpr uint32_t few_smem(int columns, int stages, int loads) {
   return 1024u + uint32_t(stages) * few_stage_bytes<F32>(columns) + (F32 ? uint32_t(loads) * 16384u : 0u) + TURNED_BYTES + (4 * FEW_STAGES + 4) * 8 + 16;
 }
 
@@ -1635,9 +1635,11 @@ int launch_few(const CUtensorMap& mt, const CUtensorMap& mx, FewWork f, cudaStre
   if (status != R2_OK) return status;
   // float32: as many stages of planes as there are groups at least, and loads that go evenly into the groups, so that a group comes back to the barriers it has waited
   // for (one that others have waited for could be two phases behind, which a wait by parity takes for done).
+  constexpr int LEAST = F32 ? GROUPS : 2;
+  static_assert(F32_STAGES >= GROUPS && F32_STAGES <= FEW_STAGES && few_smem<F32>(FEW, LEAST, F32 ? GROUPS : 0) <= most);   // (the loops below leave so many, whatever the rows)
   f.stages = F32 ? F32_STAGES : FEW_STAGES;
   f.loads = F32 ? GROUPS : 0;
-  while (f.stages > (F32 ? GROUPS : 2) && few_smem<F32>(f.columns, f.stages, f.loads) > most) --f.stages;
+  while (f.stages > LEAST && few_smem<F32>(f.columns, f.stages, f.loads) > most) --f.stages;
   while (F32 && f.loads + GROUPS <= FEW_STAGES && few_smem<F32>(f.columns, f.stages, f.loads + GROUPS) <= most) f.loads += GROUPS;
   r2_launch(kernel, dim3(few_ctas(f.n)), dim3(few_threads(F32)), size_t(few_smem<F32>(f.columns, f.stages, f.loads)), stream, mt, mx, f);
   return launch_status();
