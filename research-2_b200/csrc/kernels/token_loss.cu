@@ -1919,7 +1919,7 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
       d.n = width;
       T* out = static_cast<T*>(d_table) + first * ld_dt;
       if (!make_map(&b.table_a, dz, n, l.rows_up, BK) || !make_map(&b.table_b, x, width, l.rows_up, BK)) return R2_BAD_ALIGN;
-      if (reinterpret_cast<uintptr_t>(out) % 16 == 0 && ld_dt * sizeof(T) % 16 == 0) {
+      if (reinterpret_cast<uintptr_t>(out) % 16 == 0 && ld_dt * sizeof(T) % 16 == 0 && width * sizeof(T) % 16 == 0) {   // (a copy writes whole 16 bytes, beyond a row's end, too)
         if (!make_out_map<T>(&b.table_out, out, width, n, 1, ld_dt, 0)) return R2_BAD_ALIGN;
       } else {
         b.table_out = b.table_a;
