@@ -31,6 +31,8 @@
 // which shared memory does not keep up with.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "sm100_ptx.cuh"
 #include "tensor_maps.cuh"
@@ -55,7 +57,7 @@ constexpr size_t SMEM = 1024 + STAGES * size_t(A_BYTES + B_BYTES) + 2 * WARPS * 
 // tiles of 256 rows 161 and 282, 153 and 284, 153 and 302), bfloat16 25 and 69, 27 and 71, 29 and 81 (31 and 72, 29 and 73, 29 and 77 without `rest`).
 constexpr int FEW = 128;
 
-constexpr int WINDOW = 64;   // sorted rows whose sums by token a warp makes
+constexpr int WINDOW = 512;   // sorted rows whose sums by token are made together
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -1270,17 +1272,17 @@ template <typename T> __global__ void __launch_bounds__(256) planes_kernel(const
 
 // The rows that count (a token of the vocabulary, a weight that is not 0) side by side, their numbers in one plane or three, zeros behind them up to a
 // multiple of 256 rows; `place[r]` is where row r went, -1 for none. SORTED (bfloat16, more than FEW): by their tokens (rows of one token in their order), SEGMENT of the call's rows at a time, `starts` says
-// where a segment's begin: what the table's gradient adds in float for a token then stands side by side. A block looks at all rows' tokens and takes its own; a row's place is the number
-// of those that go before it (a segment's square of comparisons, 5 us for 4,096 rows; segments keep it below the products' time however many rows there are). Behind these blocks: the table's planes.
-constexpr int SEGMENT = 65536;
-constexpr int OWN = 32;   // rows of a block at most; a segment's are whole blocks
+// where a segment's begin: what the table's gradient adds in float for a token then stands side by side. A block looks at all rows' tokens and takes its own; a sorted row's place is the number
+// of those of its segment that go before it, a comparison each (4,096 rows 1 us; segments keep it below the products' time however many rows there are). Behind these blocks: the table's planes.
+constexpr int SEGMENT = 8192;
+constexpr int OWN = 128;   // rows of a block at most; a segment's are whole blocks
 
 template <typename T, bool SORTED>
 __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long ld, int rows, int width, int vocab, int own, const int32_t* targets, const float* weight,
                                                      const float* log_sum, bf16* x, long long ld_x, long long plane, int32_t* y_out, float* f_out, float* s_out,
                                                      int32_t* place, int* count, int* starts, const Planes<T> table) {
-  constexpr int NONE = 0x7ffffffe, PASS = 8, AHEAD = 8;   // rows whose places are found in one look at the segment
-  __shared__ int totals[2][8], before_of[OWN], key_of[OWN], ranks[PASS][8];
+  constexpr int NONE = 0x7ffffffe, PASS = 8, AHEAD = 8;   // (PASS: rows whose places are found in one look at the segment)
+  __shared__ int totals[2][8], before_of[OWN], key_of[OWN], ranks[PASS][8], keys[SORTED ? SEGMENT : 1];
   pdl_launch_dependents();
   pdl_wait();
   const int blocks = int(gridDim.x) - table.blocks;
@@ -1289,42 +1291,34 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
     return;
   }
   const int first = blockIdx.x * own, last = min(rows, first + own);
-  const int begin = SORTED ? first / SEGMENT * SEGMENT : first, end = min(rows, begin + SEGMENT);   // of the block's segment
+  const int begin = SORTED ? first / SEGMENT * SEGMENT : first, end = SORTED ? min(rows, begin + SEGMENT) : first;   // of the block's segment
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto key = [&](int r) {
-    const int y = targets[r];
-    return y >= 0 && y < vocab && (weight == nullptr || weight[r] != 0.f) ? y : NONE;
+    const int y = __ldg(targets + r);
+    const float a = weight ? __ldg(weight + r) : 1.f;   // (not asked for behind the token: both are on their way together)
+    return (unsigned(y) < unsigned(vocab)) & (a != 0.f) ? y : NONE;
   };
-  if (threadIdx.x < OWN) key_of[threadIdx.x] = first + int(threadIdx.x) < last ? key(first + threadIdx.x) : NONE;
-  __syncthreads();
-  int before = 0, all = 0;
-  // how many rows of from .. to count, in all and in front of the block's (segment); how many of the segment's go before each of PASS rows of the block, by their tokens and places
-  auto scan = [&](long long from, long long to, int p, int (&n)[PASS]) {
-    int mine[PASS];
-#pragma unroll
-    for (int j = 0; j < PASS; ++j) {
-      mine[j] = SORTED ? key_of[p + j] : 0;
-      n[j] = 0;
-    }
+  auto scan = [&](long long from, long long to, auto&& keep) {   // how many rows count
+    int counted = 0;
     for (long long r0 = from + threadIdx.x; r0 < to; r0 += 256 * AHEAD) {
       int k[AHEAD];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) k[i] = r0 + 256 * i < to ? key(int(r0) + 256 * i) : NONE;
+      for (int i = 0; i < AHEAD; ++i) k[i] = key(int(min(r0 + 256 * i, to - 1)));
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        const long long r = r0 + 256 * i;
-        all += k[i] != NONE ? 1 : 0;
-        before += k[i] != NONE && r < begin ? 1 : 0;
-        if constexpr (SORTED) {
-          const int with = r < begin || r >= end ? NONE + 1 : k[i] + (r >= first ? 1 : 0);   // (of the block's own, equal ones are counted below)
-#pragma unroll
-          for (int j = 0; j < PASS; ++j) n[j] += with <= mine[j] ? 1 : 0;
+        if (r0 + 256 * i < to) {
+          counted += k[i] != NONE ? 1 : 0;
+          keep(int(r0 + 256 * i), k[i]);
         }
       }
     }
+    return counted;
   };
-  int n[PASS];
-  scan(0, rows, 0, n);
+  auto forget = [](int, int) {};
+  if (threadIdx.x < OWN) key_of[threadIdx.x] = first + int(threadIdx.x) < last ? key(first + threadIdx.x) : NONE;
+  int before = scan(0, begin, forget);
+  int all = before + scan(end, rows, forget);
+  if constexpr (SORTED) all += scan(begin, end, [&](int r, int k) { keys[r - begin] = k; });
   before = __reduce_add_sync(0xffffffffu, before);
   all = __reduce_add_sync(0xffffffffu, all);
   if (lane == 0) {
@@ -1340,28 +1334,43 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
   if (blockIdx.x == 0 && threadIdx.x == 0) *count = all;
   if constexpr (SORTED) {
     if (first == begin && threadIdx.x == 0) starts[first / SEGMENT] = before;
-    const int in_front = before, counted = all;
+    if (int(threadIdx.x) < last - first) {   // equal ones of the block
+      int equal = 0;
+      for (int i = 0; i < int(threadIdx.x); ++i) equal += key_of[i] == key_of[threadIdx.x] ? 1 : 0;
+      before_of[threadIdx.x] = before + equal;
+    }
     for (int p = 0; p < last - first; p += PASS) {
-      if (p > 0) scan(begin, end, p, n);
+      int mine[PASS], n[PASS];
+#pragma unroll
+      for (int j = 0; j < PASS; ++j) {
+        mine[j] = key_of[p + j];
+        n[j] = 0;
+      }
+#pragma unroll 4
+      for (int r = threadIdx.x; r < end - begin; r += 256) {
+        const int with = keys[r] + (begin + r >= first ? 1 : 0);   // (of the block's own, equal ones are counted above)
+#pragma unroll
+        for (int j = 0; j < PASS; ++j) n[j] += with <= mine[j] ? 1 : 0;
+      }
 #pragma unroll
       for (int j = 0; j < PASS; ++j) {
         n[j] = __reduce_add_sync(0xffffffffu, n[j]);
         if (lane == 0) ranks[j][warp] = n[j];
       }
       __syncthreads();
-      if (threadIdx.x < PASS) {
-        const int j = p + threadIdx.x;
-        int rank = in_front;
+      if (int(threadIdx.x) < min(PASS, last - first - p)) {
+        int rank = 0;
         for (int i = 0; i < 8; ++i) rank += ranks[threadIdx.x][i];
-        for (int i = 0; i < j; ++i) rank += key_of[i] == key_of[j] ? 1 : 0;
-        before_of[j] = rank;
+        before_of[p + threadIdx.x] += rank;
       }
       __syncthreads();
     }
-    all = counted;
   } else {
-    const unsigned held = __ballot_sync(0xffffffffu, key_of[lane] != NONE);
-    if (warp == 0) before_of[lane] = before + __popc(held & ((1u << lane) - 1u));
+    if (int(threadIdx.x) < last - first) {
+      int counted = before;
+      for (int i = 0; i < int(threadIdx.x); ++i) counted += key_of[i] != NONE ? 1 : 0;
+      before_of[threadIdx.x] = counted;
+    }
     __syncthreads();
   }
   const bool wide = rows_wide(hidden, ld, width);
@@ -1388,10 +1397,10 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
   for (int at = all + blockIdx.x + warp * blocks; at < filled; at += 8 * blocks) copy(at, static_cast<const T*>(nullptr));
 }
 
-// bfloat16, more than FEW rows: what rounding left of dz at the tokens' own rows, times the hidden rows, summed in float by token, for the piece's tokens. A warp takes WINDOW of the sorted rows and 128
-// columns, and leaves a token's sum at the place of the first of its rows there: a token that stands everywhere is many warps' work, and its sums are added by TABLE, in order. Other warps look up where
-// each token's rows begin and end, a lane a token. (4,096 rows, a tenth of them one token: 10 us; TABLE adding the rows themselves took 100 us longer, a CTA for 128 tokens 40. With WINDOW 32 this takes 8 us
-// and TABLE 213 in place of 200, where a lane adds a token's sums.)
+// bfloat16, more than FEW rows: what rounding left of dz at the tokens' own rows, times the hidden rows, summed in float by token, for the piece's tokens. A CTA takes WINDOW of the sorted rows and 128
+// columns, a warp 64 of the rows, and leaves a token's sum at the place of the first of its rows in the window; one that lies in several warps' is joined in shared memory. A token that stands
+// everywhere is many CTAs' work, and TABLE adds its sums, in order. Other CTAs look up where each token's rows begin and end, a lane a token. (4,096 rows, a tenth of them one token: 14 us; TABLE
+// adding the rows themselves took 100 us longer, a CTA for 128 tokens 40. Sums of 64 rows: TABLE, where a lane adds a token's, 470 in place of 344 for 65,536 rows of 64.)
 struct Rests {
   const bf16* x;
   long long ld_x;
@@ -1399,22 +1408,24 @@ struct Rests {
   const float* rest;
   const int *count, *starts;
   int first, n, width, slices, segments;   // of the piece: its first token, tokens; of the columns
-  long long warps;                         // of sums; those of the look-up stand behind them
+  long long blocks;                        // of sums; those of the look-up stand behind them
   float* sums;
   long long ld_sums;
   int2* runs;
   int run_tokens;
 };
 
-__global__ void __launch_bounds__(128) rests_kernel(const Rests w) {
+__global__ void __launch_bounds__(256) rests_kernel(const Rests w) {
+  constexpr int SLICE = 128, OF_WARP = WINDOW / 8;
+  __shared__ int head[8], tail[8], tail_at[8];   // a sum that an earlier warp began ends here; one goes on from here; its place, -1: an earlier warp's
+  __shared__ alignas(16) float heads[8][SLICE], tails[8][SLICE];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, k = *w.count;
-  const long long job = blockIdx.x * 4LL + (threadIdx.x >> 5);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k = *w.count;
   auto start_of = [&](int segment) { return segment < w.segments ? __ldg(w.starts + segment) : k; };
-  if (job >= w.warps) {
-    const long long groups = w.run_tokens / 32, at = job - w.warps;
-    const int segment = int(at / groups), own = int(at % groups) * 32 + lane;
+  if (blockIdx.x >= w.blocks) {
+    const long long groups = w.run_tokens / 32, job = (blockIdx.x - w.blocks) * 8 + warp;
+    const int segment = int(job / groups), own = int(job % groups) * 32 + lane;
     if (segment >= w.segments) return;
     auto bound = [&](int token) {
       int a = start_of(segment), b = start_of(segment + 1);
@@ -1431,44 +1442,80 @@ __global__ void __launch_bounds__(128) rests_kernel(const Rests w) {
     w.runs[static_cast<long long>(segment) * w.run_tokens + own] = make_int2(begin, end);
     return;
   }
-  const int from = int(job / w.slices) * WINDOW, to = min(k, from + WINDOW), col = int(job % w.slices) * 128 + lane * 4;
+  const int window = int(blockIdx.x / w.slices) * WINDOW, slice = int(blockIdx.x % w.slices) * SLICE, col = slice + lane * 4;
+  const int from = window + warp * OF_WARP, to = min(k, from + OF_WARP), window_end = min(k, window + WINDOW);
+  bool ours = false;
+  for (int i = window + int(threadIdx.x); i < window_end; i += 256) {
+    const int token = __ldg(w.targets + i) - w.first;
+    ours = ours || (token >= 0 && token < w.n);
+  }
+  if (!__syncthreads_or(ours)) return;   // (tokens of other pieces: nobody reads their sums now)
+  // bits of the 32 rows from i on (of this window) whose sum begins there: the window's first, another token than the one before, a segment's first
+  auto begins_of = [&](int i) {
+    const int at = i + lane, token = at < window_end ? __ldg(w.targets + at) : -1, before = at < window_end && at > window ? __ldg(w.targets + at - 1) : -1;
+    unsigned begins = __ballot_sync(0xffffffffu, at < window_end && token != before);
+    for (int s = 0; s < w.segments; s += 32) {
+      const int start = s + lane < w.segments ? __ldg(w.starts + s + lane) : -1;
+      begins |= __reduce_or_sync(0xffffffffu, start >= i && start < i + 32 && start < window_end ? 1u << (start - i) : 0u);
+    }
+    return begins;
+  };
   const bool wide = col < w.width;   // (rows of whole eights)
   float sum[4] = {};
-  int at = -1;   // the place of what is summed
+  int at = -1;          // the place of what is summed, -1: an earlier warp's
+  bool ended = false;   // that one ends in this warp
   auto keep = [&] {
-    if (wide && at >= 0) *reinterpret_cast<float4*>(w.sums + at * w.ld_sums + col) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    if (at < 0) {
+      ended = true;
+      *reinterpret_cast<float4*>(&heads[warp][lane * 4]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    } else if (wide) {
+      *reinterpret_cast<float4*>(w.sums + at * w.ld_sums + col) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    }
     sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
   };
+  bool goes_on = false;
+  if (from < to) {
 #pragma unroll 1
-  for (int i = from; i < to; i += 32) {
-    const bool there = i + lane < to;
-    const int token = there ? __ldg(w.targets + i + lane) : -1, before = there && i + lane > from ? __ldg(w.targets + i + lane - 1) : -1;
-    if (!__any_sync(0xffffffffu, there && token >= w.first && token - w.first < w.n)) {   // (of other pieces: nobody reads their sums)
-      keep();
-      at = -1;
-      continue;
-    }
-    const float rest = there ? __ldg(w.rest + i + lane) : 0.f;
-    uint2 x[32];
+    for (int i = from; i < to; i += 32) {
+      const float rest = i + lane < to ? __ldg(w.rest + i + lane) : 0.f;
+      uint2 x[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) x[j] = wide && i + j < to ? __ldg(reinterpret_cast<const uint2*>(w.x + (i + j) * w.ld_x + col)) : make_uint2(0, 0);
-    bool first = there && token != before;
-    for (int s = 1; s < w.segments; ++s) first = first || (there && i + lane == start_of(s));
-    const unsigned begins = __ballot_sync(0xffffffffu, first);
+      for (int j = 0; j < 32; ++j) x[j] = wide && i + j < to ? __ldg(reinterpret_cast<const uint2*>(w.x + (i + j) * w.ld_x + col)) : make_uint2(0, 0);
+      const unsigned begins = begins_of(i);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const float by = __shfl_sync(0xffffffffu, rest, j);
-      if (begins >> j & 1u) {
-        keep();
-        at = i + j;
+      for (int j = 0; j < 32; ++j) {
+        const float by = __shfl_sync(0xffffffffu, rest, j);
+        if (begins >> j & 1u) {
+          if (i + j > from) keep();
+          at = i + j;
+        }
+        sum[0] = fmaf(by, __uint_as_float(x[j].x << 16), sum[0]);
+        sum[1] = fmaf(by, __uint_as_float(x[j].x & 0xffff0000u), sum[1]);
+        sum[2] = fmaf(by, __uint_as_float(x[j].y << 16), sum[2]);
+        sum[3] = fmaf(by, __uint_as_float(x[j].y & 0xffff0000u), sum[3]);
       }
-      sum[0] = fmaf(by, __uint_as_float(x[j].x << 16), sum[0]);
-      sum[1] = fmaf(by, __uint_as_float(x[j].x & 0xffff0000u), sum[1]);
-      sum[2] = fmaf(by, __uint_as_float(x[j].y << 16), sum[2]);
-      sum[3] = fmaf(by, __uint_as_float(x[j].y & 0xffff0000u), sum[3]);
+    }
+    goes_on = to < window_end && (begins_of(to) & 1u) == 0;
+    if (goes_on) *reinterpret_cast<float4*>(&tails[warp][lane * 4]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    else keep();
+  }
+  if (lane == 0) {
+    head[warp] = ended;
+    tail[warp] = goes_on;
+    tail_at[warp] = at;
+  }
+  __syncthreads();
+  const int c = threadIdx.x;   // a thread a column
+  if (c >= SLICE || slice + c >= w.width) return;
+  float all = 0.f;
+  int place = -1;
+  for (int i = 0; i < 8; ++i) {
+    if (head[i]) w.sums[place * w.ld_sums + slice + c] = all + heads[i][c];
+    if (tail[i]) {
+      all = tail_at[i] >= 0 ? tails[i][c] : all + tails[i][c];
+      place = tail_at[i] >= 0 ? tail_at[i] : place;
     }
   }
-  keep();
 }
 
 // The hidden rows' gradient: shares of a gathered row added in one order, and what rounding left of dz at its token (`rest`, null in float32) times the token's row of the
@@ -1834,7 +1881,12 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
   int32_t* place = reinterpret_cast<int32_t*>(space + l.place);
   int* starts = reinterpret_cast<int*>(space + l.starts);
   int own = (rows + 591) / 592;
-  own = own > OWN || rows > SEGMENT ? OWN : own;
+  if (sizeof(T) == 4 || few || rows <= SEGMENT) {
+    own = own > 32 ? 32 : own;
+  } else {
+    own = own > OWN ? OWN : own;
+    while (SEGMENT % own != 0) ++own;
+  }
   constexpr bool BF16 = sizeof(T) == 2;
   r2_launch(BF16 && !few ? gather_kernel<T, BF16> : gather_kernel<T, false>, dim3((rows + own - 1) / own + planes.blocks), dim3(256), size_t(0), stream,
       static_cast<const T*>(hidden), ld_h, rows, width, vocab, own, targets, weight, log_sum, gathered, x.ld, x.plane, reinterpret_cast<int32_t*>(space + l.targets),
@@ -1903,12 +1955,12 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
       d.ld_x = x.ld;
       if (BF16 && !few) {
         const int segments = int(up(rows, SEGMENT) / SEGMENT);
-        const long long slices = up(width, 128) / 128, warps = up(rows, WINDOW) / WINDOW * slices;
-        const Rests rests = {gathered, x.ld, w.targets, w.rest, count, starts, int(first), n, width, int(slices), segments, warps, reinterpret_cast<float*>(space + l.rests), l.width_up,
+        const long long slices = up(width, 128) / 128, sums = up(rows, WINDOW) / WINDOW * slices;
+        const Rests rests = {gathered, x.ld, w.targets, w.rest, count, starts, int(first), n, width, int(slices), segments, sums, reinterpret_cast<float*>(space + l.rests), l.width_up,
                              reinterpret_cast<int2*>(space + l.runs), int(up(n, 32))};
-        const long long blocks = (warps + segments * (rests.run_tokens / 32) + 3) / 4;
+        const long long blocks = sums + (segments * (rests.run_tokens / 32ll) + 7) / 8;
         if (blocks >= 1ll << 31) return R2_UNSUPPORTED;
-        r2_launch(rests_kernel, dim3(unsigned(blocks)), dim3(128), size_t(0), stream, rests);
+        r2_launch(rests_kernel, dim3(unsigned(blocks)), dim3(256), size_t(0), stream, rests);
         d.runs = rests.runs;
         d.sums = rests.sums;
         d.ld_sums = rests.ld_sums;
