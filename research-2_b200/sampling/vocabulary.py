@@ -50,6 +50,8 @@ def token_loss(hidden: torch.Tensor, table: torch.Tensor, targets: torch.Tensor,
                               (f" and weights {tuple(weight.shape)}" if weight is not None else "") + " do not fit")
     if table.dim() != 2:
         raise ops.KernelError(f"token_loss: table must have 2 dimensions, got shape {tuple(table.shape)}")
+    if hidden.shape[-1] < 1:
+        raise ops.KernelError(f"token_loss: hidden rows {tuple(hidden.shape)} have no numbers")
     rows = hidden.reshape(-1, hidden.shape[-1])
     loss = _TokenLoss.apply(_contiguous_rows(rows), _contiguous_rows(table), _tokens(targets, table.shape[0]).reshape(-1).contiguous(),
                             None if weight is None else weight.reshape(-1).contiguous(), float(softcap))
@@ -67,6 +69,8 @@ class _TokenRows(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, above):
         (ids,) = ctx.saved_tensors
+        if ctx.vocab == 0:   # (all rows were zeros)
+            return None, above.new_zeros((0, above.shape[1]), dtype=ctx.dtype), None, None
         return None, ops.token_rows_gradient(ids, _contiguous_rows(above), ctx.vocab, scale=ctx.scale, out_dtype=ctx.dtype), None, None
 
 
