@@ -1,4 +1,4 @@
-// The loss of given tokens from hidden rows and a token table, and its gradients, without the logits in memory. With hidden rows x [N, D], table
+// The loss of given tokens from hidden rows and a token table, and its gradients, without keeping logits. With hidden rows x [N, D], table
 // W [V, D], tokens y [N] and weights a [N]:
 //
 //   u = x W^T,  z = u  or  c tanh(u / c),  s_r = log(sum_v exp z_rv),  loss_r = a_r (s_r - z_r,y)
@@ -1711,7 +1711,7 @@ template <typename T> bool make_few_maps(CUtensorMap* mt, CUtensorMap* mx, const
 int row_blocks(long long rows) { return int(rows < 8 * 4736 ? (rows + 7) / 8 : 4736); }
 
 // What a call's scratch holds, in bytes from its start.
-// Of dz at a time. (4,096 rows at GPT-2's table with 128, 256, 512 MB and 1 GB: 931, 855, 833 and 833 us; 2,047 at a table of 128,001 x 1,600 2,487, 2,441, 2,418 and 2,418. Pieces that L2
+// Of dz at a time: pieces bound what a call takes, and a call whose dz is smaller has one. (4,096 rows at GPT-2's table with 128, 256, 512 MB and 1 GB: 931, 855, 833 and 833 us; 2,047 at a table of 128,001 x 1,600 2,487, 2,441, 2,418 and 2,418. Pieces that L2
 // would hold make for more launches and rounds that are not full.)
 constexpr long long FACTOR_BYTES = 512ll << 20;
 

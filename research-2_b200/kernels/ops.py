@@ -2293,7 +2293,7 @@ def _loss_arguments(hidden, table, targets, weight, softcap, what):
 
 
 def token_loss(hidden: torch.Tensor, table: torch.Tensor, targets: torch.Tensor, *, weight: torch.Tensor | None = None, softcap: float = 0.0, alike: bool = False):
-    """How unlikely a model finds given tokens, from its hidden rows, without the logits in memory: (loss float32 [N], log_sum float32 [N]).
+    """How unlikely a model finds given tokens, from its hidden rows, without the logits in memory (scratch: 8 bytes for each row and 128 tokens): (loss float32 [N], log_sum float32 [N]).
 
     `hidden` [N, D] are the rows that the head multiplies with `table` [V, D] (both float32 or both bfloat16; rows contiguous, any row stride);
     `targets` int32 [N] the tokens. With z = hidden @ table^T (`softcap` > 0: softcap * tanh(z / softcap)), log_sum is the logarithm of a row's
@@ -2323,7 +2323,8 @@ def token_loss_gradient(hidden: torch.Tensor, table: torch.Tensor, targets: torc
                         softcap: float = 0.0, hidden_gradient: bool = True, table_gradient: bool = True):
     """The gradients of the sum of `token_loss`'s losses: (of the hidden rows [N, D], of the table [V, D]), in their types; None for one that is not
     asked for. `log_sum` is `token_loss`'s for the same hidden rows, table and softcap; the other arguments as there. A row without a target, or of weight 0,
-    has the gradient 0 and no part in the table's, whatever its hidden numbers are. (A factor of a logit below 2^-126 counts as 0. bfloat16 gradients: factors
+    has the gradient 0 and no part in the table's, whatever its hidden numbers are. (Scratch: the factors, bfloat16 or three times that, of a piece of the vocabulary, 512 MB at most, or of 256 tokens; and the rows' own, once gathered and once in float.
+    A factor of a logit below 2^-126 counts as 0. bfloat16 gradients: factors
     but a row's own token's are rounded to bfloat16 before the products.)"""
     if hidden.is_cuda:
         done = _logit_face("token_loss_gradient")(hidden, table, targets, log_sum, weight, softcap, hidden_gradient, table_gradient, _error_address(hidden))

@@ -1,5 +1,5 @@
-"""The two ends of a token table, for training with torch's gradients: the rows that tokens look up, and the loss of tokens from hidden rows. The logits
-[N, V] are in memory at no time: the backward pass makes them again, a piece of the vocabulary at a time, with the factors that come down from above.
+"""The two ends of a token table, for training with torch's gradients: the rows that tokens look up, and the loss of tokens from hidden rows. The loss keeps no
+logits [N, V]: the backward pass makes them again, as factors of up to 512 MB at a time (a piece of the vocabulary, or all of it where it fits), with the factors that come down from above.
 (A step that is to be captured into a graph asks for its gradients with `torch.autograd.grad`, or calls the operators themselves: while an eager graph over the same
 parameters lives, torch itself cannot capture a `backward()` that adds to their `.grad`.)"""
 
