@@ -212,9 +212,9 @@ template <int MODE> __device__ __forceinline__ Unit unit_of(const Work& w, long 
 }
 
 // Steps of k that are added in tensor memory before their sum goes into registers (0: all): 256 of k with the products of planes; 512 where logits are
-// made of more than 768 bfloat16 products (1,024 of them: off by up to 1.2e-6 of the loss otherwise; 1,600: by 2.4e-7 in place of 7.7e-7, and 5 % slower), in the loss and in its
-// gradients alike; 32,768 in gradients, whose sums are then off by 2^-13 at most, a 32th of half a step of bfloat16.
-constexpr int PLANES_CHUNK = 4, LONG_CHUNK = 8, LONG_STEPS = 12, GRADIENT_CHUNK = 512;
+// made of more than 768 bfloat16 products (1,024 of them: off by up to 1.2e-6 of the loss otherwise; 1,600: by 2.4e-7 in place of 7.7e-7, and 5 % slower); 1,024 for the
+// factors' logits, whose tiles take longer to finish than two accumulators of 512 hold products for (2,047 rows of 1,600: 728 us, of 1,024 612, all in one 572); 32,768 in gradients, whose sums are then off by 2^-13 at most, a 32th of half a step of bfloat16.
+constexpr int PLANES_CHUNK = 4, LONG_CHUNK = 8, LONG_STEPS = 12, FACTORS_CHUNK = 16, GRADIENT_CHUNK = 512;
 
 // How many times a unit's products go through an accumulator.
 template <int CHUNKED> __device__ __forceinline__ int sums_of(const Unit& u) {
@@ -1931,7 +1931,7 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
           !make_out_map<bf16>(&mo, dz.at, l.piece, l.rows_up, l.planes, l.piece, dz.plane))
         return R2_BAD_ALIGN;
       const long long tiles = row_tiles * (up(n, BN) / BN);
-      if (BF16 && width > LONG_STEPS * BK) status = launch<FACTORS, bf16, false, LONG_CHUNK>(ma, mb, mo, w, tiles, softcap > 0.f, stream);
+      if (BF16 && width > FACTORS_CHUNK * BK) status = launch<FACTORS, bf16, false, FACTORS_CHUNK>(ma, mb, mo, w, tiles, softcap > 0.f, stream);
       else status = launch<FACTORS, bf16, sizeof(T) == 4>(ma, mb, mo, w, tiles, softcap > 0.f, stream);
     }
     if (status != R2_OK) break;
