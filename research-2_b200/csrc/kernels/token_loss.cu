@@ -1398,8 +1398,8 @@ __global__ void __launch_bounds__(256) gather_kernel(const T* hidden, long long 
 }
 
 // bfloat16, more than FEW rows: what rounding left of dz at the tokens' own rows, times the hidden rows, summed in float by token, for the piece's tokens. A CTA takes WINDOW of the sorted rows and 128
-// columns, a warp 64 of the rows, and leaves a token's sum at the place of the first of its rows in the window; one that lies in several warps' is joined in shared memory. A token that stands
-// everywhere is many CTAs' work, and TABLE adds its sums, in order. Other CTAs look up where each token's rows begin and end, a lane a token. (4,096 rows, a tenth of them one token: 14 us; TABLE
+// columns, a warp 32 of the rows, and leaves a token's sum at the place of the first of its rows in the window; one that lies in several warps' is joined in shared memory. A token that stands
+// everywhere is many CTAs' work, and TABLE adds its sums, in order. Other CTAs look up where each token's rows begin and end, a warp 32 tokens. (4,096 rows, a tenth of them one token: 11 us; TABLE
 // adding the rows themselves took 100 us longer, a CTA for 128 tokens 40. Sums of 64 rows: TABLE, where a lane adds a token's, 470 in place of 344 for 65,536 rows of 64.)
 struct Rests {
   const bf16* x;
@@ -1408,58 +1408,67 @@ struct Rests {
   const float* rest;
   const int *count, *starts;
   int first, n, width, slices, segments;   // of the piece: its first token, tokens; of the columns
-  long long blocks;                        // of sums; those of the look-up stand behind them
+  long long blocks;                        // of sums; those that look up stand behind them
   float* sums;
   long long ld_sums;
   int2* runs;
   int run_tokens;
 };
 
-__global__ void __launch_bounds__(256) rests_kernel(const Rests w) {
-  constexpr int SLICE = 128, OF_WARP = WINDOW / 8;
-  __shared__ int head[8], tail[8], tail_at[8];   // a sum that an earlier warp began ends here; one goes on from here; its place, -1: an earlier warp's
-  __shared__ alignas(16) float heads[8][SLICE], tails[8][SLICE];
+constexpr int REST_WARPS = WINDOW / 32;
+
+__global__ void __launch_bounds__(REST_WARPS * 32) rests_kernel(const Rests w) {
+  constexpr int SLICE = 128;
+  __shared__ int head[REST_WARPS], tail[REST_WARPS], tail_at[REST_WARPS];   // a sum that an earlier warp began ends here; one goes on from here; its place, -1: an earlier warp's
+  __shared__ alignas(16) float heads[REST_WARPS][SLICE], tails[REST_WARPS][SLICE];
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k = *w.count;
-  auto start_of = [&](int segment) { return segment < w.segments ? __ldg(w.starts + segment) : k; };
   if (blockIdx.x >= w.blocks) {
-    const long long groups = w.run_tokens / 32, job = (blockIdx.x - w.blocks) * 8 + warp;
-    const int segment = int(job / groups), own = int(job % groups) * 32 + lane;
+    // ---- where the rows of 32 tokens begin: the warp looks for the first and the last, and counts between them
+    const long long groups = w.run_tokens / 32, job = (blockIdx.x - w.blocks) * REST_WARPS + warp;
+    const int segment = int(job / groups), first = w.first + int(job % groups) * 32;
     if (segment >= w.segments) return;
-    auto bound = [&](int token) {
-      int a = start_of(segment), b = start_of(segment + 1);
-      while (a < b) {
-        const int middle = a + (b - a) / 2;
-        if (__ldg(w.targets + middle) < token) a = middle + 1;
-        else b = middle;
-      }
-      return a;
+    int from = __ldg(w.starts + segment), end = segment + 1 < w.segments ? __ldg(w.starts + segment + 1) : k, to = from, to_end = end;
+    auto narrow = [&](int& a, int& b, int token) {   // a .. b holds the first place whose token is `token` or a later one
+      const int step = (b - a + 31) / 32, at = a + lane * step;
+      const int n = __popc(__ballot_sync(0xffffffffu, at < b && __ldg(w.targets + at) < token));
+      b = n == 0 ? a : min(b, a + n * step);
+      a += n == 0 ? 0 : (n - 1) * step + 1;
     };
-    const int begin = bound(w.first + own);
-    int end = __shfl_down_sync(0xffffffffu, begin, 1);
-    if (lane == 31) end = bound(w.first + own + 1);
-    w.runs[static_cast<long long>(segment) * w.run_tokens + own] = make_int2(begin, end);
+    while (from < end || to < to_end) {
+      narrow(from, end, first);
+      narrow(to, to_end, first + 32);
+    }
+    int begin = from;   // of the lane's token
+    if (to - from <= 32) {
+      const int token = from + lane < to ? __ldg(w.targets + from + lane) - first : 32;
+      for (int j = 0; j < to - from; ++j) begin += __shfl_sync(0xffffffffu, token, j) < lane ? 1 : 0;
+    } else {
+      for (int last = to; begin < last;) {
+        const int middle = begin + (last - begin) / 2;
+        if (__ldg(w.targets + middle) < first + lane) begin = middle + 1;
+        else last = middle;
+      }
+    }
+    int next = __shfl_down_sync(0xffffffffu, begin, 1);
+    if (lane == 31) next = to;
+    w.runs[static_cast<long long>(segment) * w.run_tokens + (first - w.first) + lane] = make_int2(begin, next);
     return;
   }
   const int window = int(blockIdx.x / w.slices) * WINDOW, slice = int(blockIdx.x % w.slices) * SLICE, col = slice + lane * 4;
-  const int from = window + warp * OF_WARP, to = min(k, from + OF_WARP), window_end = min(k, window + WINDOW);
-  bool ours = false;
-  for (int i = window + int(threadIdx.x); i < window_end; i += 256) {
-    const int token = __ldg(w.targets + i) - w.first;
-    ours = ours || (token >= 0 && token < w.n);
+  const int from = window + warp * 32, to = min(k, from + 32), window_end = min(k, window + WINDOW);
+  const bool there = from + lane < to;
+  const int token = there ? __ldg(w.targets + from + lane) : -1;
+  const int in_front = from < to && warp > 0 ? __ldg(w.targets + from - 1) : -1, behind = to < window_end ? __ldg(w.targets + to) : -1;
+  unsigned begins = 0;       // bits of the rows that a segment begins with, then of those that a sum begins with
+  bool behind_begins = false;
+  for (int s = 0; s < w.segments; s += 32) {
+    const int start = s + lane < w.segments ? __ldg(w.starts + s + lane) : -1;
+    begins |= __reduce_or_sync(0xffffffffu, start >= from && start < to ? 1u << (start - from) : 0u);
+    behind_begins |= __any_sync(0xffffffffu, start == to) != 0;
   }
-  if (!__syncthreads_or(ours)) return;   // (tokens of other pieces: nobody reads their sums now)
-  // bits of the 32 rows from i on (of this window) whose sum begins there: the window's first, another token than the one before, a segment's first
-  auto begins_of = [&](int i) {
-    const int at = i + lane, token = at < window_end ? __ldg(w.targets + at) : -1, before = at < window_end && at > window ? __ldg(w.targets + at - 1) : -1;
-    unsigned begins = __ballot_sync(0xffffffffu, at < window_end && token != before);
-    for (int s = 0; s < w.segments; s += 32) {
-      const int start = s + lane < w.segments ? __ldg(w.starts + s + lane) : -1;
-      begins |= __reduce_or_sync(0xffffffffu, start >= i && start < i + 32 && start < window_end ? 1u << (start - i) : 0u);
-    }
-    return begins;
-  };
+  if (!__syncthreads_or(there && token >= w.first && token - w.first < w.n)) return;   // (tokens of other pieces: nobody reads their sums now)
   const bool wide = col < w.width;   // (rows of whole eights)
   float sum[4] = {};
   int at = -1;          // the place of what is summed, -1: an earlier warp's
@@ -1475,27 +1484,25 @@ __global__ void __launch_bounds__(256) rests_kernel(const Rests w) {
   };
   bool goes_on = false;
   if (from < to) {
-#pragma unroll 1
-    for (int i = from; i < to; i += 32) {
-      const float rest = i + lane < to ? __ldg(w.rest + i + lane) : 0.f;
-      uint2 x[32];
+    const float rest = there ? __ldg(w.rest + from + lane) : 0.f;
+    uint2 x[32];
 #pragma unroll
-      for (int j = 0; j < 32; ++j) x[j] = wide && i + j < to ? __ldg(reinterpret_cast<const uint2*>(w.x + (i + j) * w.ld_x + col)) : make_uint2(0, 0);
-      const unsigned begins = begins_of(i);
+    for (int j = 0; j < 32; ++j) x[j] = wide && from + j < to ? __ldg(reinterpret_cast<const uint2*>(w.x + (from + j) * w.ld_x + col)) : make_uint2(0, 0);
+    const int shifted = __shfl_up_sync(0xffffffffu, token, 1), last = __shfl_sync(0xffffffffu, token, 31);
+    begins |= __ballot_sync(0xffffffffu, there && token != (lane == 0 ? in_front : shifted));
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const float by = __shfl_sync(0xffffffffu, rest, j);
-        if (begins >> j & 1u) {
-          if (i + j > from) keep();
-          at = i + j;
-        }
-        sum[0] = fmaf(by, __uint_as_float(x[j].x << 16), sum[0]);
-        sum[1] = fmaf(by, __uint_as_float(x[j].x & 0xffff0000u), sum[1]);
-        sum[2] = fmaf(by, __uint_as_float(x[j].y << 16), sum[2]);
-        sum[3] = fmaf(by, __uint_as_float(x[j].y & 0xffff0000u), sum[3]);
+    for (int j = 0; j < 32; ++j) {
+      const float by = __shfl_sync(0xffffffffu, rest, j);
+      if (begins >> j & 1u) {
+        if (j > 0) keep();
+        at = from + j;
       }
+      sum[0] = fmaf(by, __uint_as_float(x[j].x << 16), sum[0]);
+      sum[1] = fmaf(by, __uint_as_float(x[j].x & 0xffff0000u), sum[1]);
+      sum[2] = fmaf(by, __uint_as_float(x[j].y << 16), sum[2]);
+      sum[3] = fmaf(by, __uint_as_float(x[j].y & 0xffff0000u), sum[3]);
     }
-    goes_on = to < window_end && (begins_of(to) & 1u) == 0;
+    goes_on = to < window_end && !behind_begins && behind == last;
     if (goes_on) *reinterpret_cast<float4*>(&tails[warp][lane * 4]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
     else keep();
   }
@@ -1509,7 +1516,7 @@ __global__ void __launch_bounds__(256) rests_kernel(const Rests w) {
   if (c >= SLICE || slice + c >= w.width) return;
   float all = 0.f;
   int place = -1;
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < REST_WARPS; ++i) {
     if (head[i]) w.sums[place * w.ld_sums + slice + c] = all + heads[i][c];
     if (tail[i]) {
       all = tail_at[i] >= 0 ? tails[i][c] : all + tails[i][c];
@@ -1958,9 +1965,9 @@ int gradient_of(const void* hidden, long long ld_h, const void* table, long long
         const long long slices = up(width, 128) / 128, sums = up(rows, WINDOW) / WINDOW * slices;
         const Rests rests = {gathered, x.ld, w.targets, w.rest, count, starts, int(first), n, width, int(slices), segments, sums, reinterpret_cast<float*>(space + l.rests), l.width_up,
                              reinterpret_cast<int2*>(space + l.runs), int(up(n, 32))};
-        const long long blocks = sums + (segments * (rests.run_tokens / 32ll) + 7) / 8;
+        const long long blocks = sums + (segments * (rests.run_tokens / 32ll) + REST_WARPS - 1) / REST_WARPS;
         if (blocks >= 1ll << 31) return R2_UNSUPPORTED;
-        r2_launch(rests_kernel, dim3(unsigned(blocks)), dim3(256), size_t(0), stream, rests);
+        r2_launch(rests_kernel, dim3(unsigned(blocks)), dim3(REST_WARPS * 32), size_t(0), stream, rests);
         d.runs = rests.runs;
         d.sums = rests.sums;
         d.ld_sums = rests.ld_sums;
