@@ -25,9 +25,9 @@
 // Rows without a token or of weight 0 have no part in the gradients: `gather_kernel` puts the others side by side, so that no product reads them
 // (whatever they hold) or spends time on them; the rest of the last 256 rows is zeros.
 //
-// Bound by the tensor cores from some 200 rows on, by the pass over the table below. At a table of 50,257 x 768, bfloat16, 1,965 MHz: LOGSUM of 4,096 rows 191 us (1.66 PFLOP/s, tensor cores
-// active 96 % of an SM's time), FACTORS of 3,840 that count 213 us (1.39; 190 without the stores of dz, which the operands' loads share the L2 with), ROWS 220 (1.35) and TABLE
-// 199 (1.49; operands whose rows lie along K are read at 0.9 of the rate). Tiles of 256 x 256 on pairs read 64 KB for each 64 of k and pair where 128 x 128 read twice that for the work,
+// Bound by the tensor cores from some 200 rows on, by the pass over the table below. At a table of 50,257 x 768, bfloat16, 1,965 MHz: LOGSUM of 4,096 rows 189 us (1.68 PFLOP/s, tensor cores
+// active 96 % of an SM's time), FACTORS of 3,840 that count 206 us (1.44; 190 without the stores of dz, which the operands' loads share the L2 with), ROWS 196 (1.51) and TABLE
+// 184 to 200 (1.61; operands whose rows lie along K are read at 0.9 of the rate). Tiles of 256 x 256 on pairs read 64 KB for each 64 of k and pair where 128 x 128 read twice that for the work,
 // which shared memory does not keep up with.
 #include <math.h>
 
@@ -53,8 +53,8 @@ constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = HALF * BK * 2;
 constexpr uint32_t SLAB = 32 * 128;   // 32 rows of 128 bytes on their way out; a warp has two
 constexpr size_t SMEM = 1024 + STAGES * size_t(A_BYTES + B_BYTES) + 2 * WARPS * SLAB + (2 * STAGES + 4) * 8 + 16;
 
-// Rows that go through the other kernel below, at most. At GPT-2's table with cold caches, loss and gradients of 16, 64 and 128 rows: float32 54 and 247, 59 and 251, 73 and 290 us (by the
-// tiles of 256 rows 161 and 282, 153 and 284, 153 and 302), bfloat16 25 and 69, 27 and 71, 29 and 81 (31 and 72, 29 and 73, 29 and 77 without `rest`).
+// Rows that go through the other kernel below, at most. At GPT-2's table with cold caches, loss and gradients of 16, 64 and 128 rows: float32 53 and 245, 57 and 249, 70 and 288 us (by the
+// tiles of 256 rows 161 and 282, 153 and 284, 153 and 302), bfloat16 25 and 69, 27 and 73, 29 and 87 (106 where a tenth of the rows has one token, whose rests a lane adds; by rests_kernel 80, 84, 99 and 98).
 constexpr int FEW = 128;
 
 constexpr int WINDOW = 512;   // sorted rows whose sums by token are made together
@@ -213,7 +213,7 @@ template <int MODE> __device__ __forceinline__ Unit unit_of(const Work& w, long 
 
 // Steps of k that are added in tensor memory before their sum goes into registers (0: all): 256 of k with the products of planes; 512 where logits are
 // made of more than 768 bfloat16 products (1,024 of them: off by up to 1.2e-6 of the loss otherwise; 1,600: by 2.4e-7 in place of 7.7e-7, and 5 % slower); 1,024 for the
-// factors' logits, whose tiles take longer to finish than two accumulators of 512 hold products for (2,047 rows of 1,600: 728 us, of 1,024 612, all in one 572); 32,768 in gradients, whose sums are then off by 2^-13 at most, a 32th of half a step of bfloat16.
+// factors' logits, whose tiles take longer to finish than two accumulators of 512 hold products for (2,047 rows of 1,600: 728 us, of 1,024 615, all in one 572); 32,768 in gradients, whose sums are then off by 2^-13 at most, a 32th of half a step of bfloat16.
 constexpr int PLANES_CHUNK = 4, LONG_CHUNK = 8, LONG_STEPS = 12, FACTORS_CHUNK = 16, GRADIENT_CHUNK = 512;
 
 // How many times a unit's products go through an accumulator.
