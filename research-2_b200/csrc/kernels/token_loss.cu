@@ -414,9 +414,12 @@ __device__ __forceinline__ void product(const CUtensorMap& map_a, const CUtensor
       const int row = (u.row * 2 + int(rank)) * BM + q * 32 + lane;
       return i < n_units && row < m && w.segments > 0 ? __ldg(w.runs + row) : make_int2(0, 0);
     };
-    Unit u_ahead = unit_of<MODE>(w, pair, row_tiles, col_tiles, n_kb);
-    int2 run_ahead = make_int2(0, 0);
-    if constexpr (RESTS) run_ahead = run_of(pair, u_ahead);
+    [[maybe_unused]] Unit u_ahead = {};
+    [[maybe_unused]] int2 run_ahead = make_int2(0, 0);
+    if constexpr (RESTS) {
+      u_ahead = unit_of<MODE>(w, pair, row_tiles, col_tiles, n_kb);
+      run_ahead = run_of(pair, u_ahead);
+    }
     for (long long i = pair; i < n_units; i += n_pairs) {
       const Unit u = RESTS ? u_ahead : unit_of<MODE>(w, i, row_tiles, col_tiles, n_kb);
       const int row = (u.row * 2 + int(rank)) * BM + q * 32 + lane;

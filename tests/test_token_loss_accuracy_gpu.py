@@ -110,3 +110,15 @@ def test_the_gradients_logits_are_the_losses(rows):
     error = ((d_table.double() - want.d_table) / want.d_table)[1:]
     cuts = 32 * 2.0**-24 * 48 if rows > 128 else 0.0
     assert abs(error.mean().item()) <= cuts + 1.7e-5 + 6 * 2.0**-8 / 3**0.5 / ((vocab - 1) * rows) ** 0.5 + 6 * 2.0**-8 / 3**0.5 / error.numel() ** 0.5 + 16 * 2.0**-24
+
+
+@pytest.mark.parametrize("rows,width,vocab", [(300, 16, 1200003), (9000, 40, 50001), (20000, 72, 3000)])
+def test_one_gradient_alone_of_sorted_rows(rows, width, vocab):
+    """bfloat16, several pieces of the vocabulary or several segments of rows: what a gradient is made from lies where the piece before left its own; alone it is what it is beside the other."""
+    c = common(Case(rows, width, vocab, BF16, rows), vocab // 2, 0.1)
+    c.targets[10:16] = torch.tensor([0, vocab - 1, vocab // 3, 524287 % vocab, 524288 % vocab, 1048575 % vocab], dtype=torch.int32, device=DEV)
+    both = c.run()
+    for _ in range(3):
+        assert torch.equal(c.run(hidden_gradient=False)[3], both[3]) and torch.equal(c.run(table_gradient=False)[2], both[2])
+    if rows * vocab < 4e8:
+        c.check()
